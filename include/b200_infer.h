@@ -55,6 +55,11 @@ extern "C" {
 #define B200_PREC_FFMA 0 /* exact F32 FFMA (reference tolerance 1e-5) */
 #define B200_PREC_TF32 1 /* tcgen05 tensor cores, TF32 inputs, F32 accumulate */
 
+/* Element type of the batched operators' tensors. */
+#define B200_DTYPE_F32 0
+#define B200_DTYPE_F16 1
+#define B200_DTYPE_BF16 2
+
 const char *b200_status_string(int status);
 /* 1 if the library was built for and runs on an sm_100 device, else 0. */
 int b200_device_supported(int device);
@@ -218,6 +223,93 @@ size_t b200_argmax_workspace_bytes(int64_t n);
 #define B200_ARGMAX_NOALLOC_MAX_N 2147483647LL
 int b200_argmax_noalloc(const float *logits, int64_t n, int32_t *out_id, int32_t *dev_status,
                         void *stream);
+
+/* ------------------------------------------------------------------------
+ * Batched serving: many sequences in one call. Lengths are device arrays, so the
+ * calls take no host copy of them and can be captured into a CUDA graph once per
+ * shape bound. Tensors are F32, F16 or BF16 (`dtype`, one for all tensors of a call;
+ * sums, softmax statistics and accumulators are F32). Strides count elements; the
+ * head_dim axis is contiguous; every row must start on a 16-byte boundary
+ * (B200_ERR_NOT_SUPPORTED otherwise). A device-side length, offset or block index out
+ * of range is never followed: what it names is skipped and B200_DEV_BAD_POSITION is
+ * recorded in dev_status (nullable). No counterpart in the reference, which serves
+ * one sequence (include/kvcache/kvutil.hpp:43-44 declares the paged cache only).
+ * ------------------------------------------------------------------------ */
+
+/* A pool of cache blocks: element (block b, token t of it, KV head h, dim d) of K at
+ * k[b * block_stride + t * tok_stride + h * head_stride + d], of V likewise from v. */
+typedef struct b200_kv_pool {
+    void *k, *v;
+    int64_t n_blocks, block_tokens;
+    int64_t block_stride, tok_stride, head_stride;
+    int64_t n_head_kv, head_dim;
+    int32_t dtype;
+} b200_kv_pool;
+
+/* Causal GQA attention of packed sequences. Sequence s has the query rows
+ * [cu_q[s], cu_q[s + 1]) of q [total_q][Hq][D] and the keys [cu_k[s], cu_k[s + 1]) of
+ * k, v [total_k][Hkv][D]; cu_* are device int32 [n_seqs + 1], ascending from 0. Query
+ * row i of a sequence with nq queries and nk keys sees its keys 0 .. nk - nq + i (the
+ * last query sees the last key); a row that sees none (nk < nq) is zero. Rows outside
+ * every sequence are left untouched. scale <= 0 selects 1/sqrt(D). D 64 or 128, any
+ * Hq that is a multiple of Hkv. `workspace` (16-byte aligned, contents ignored) of
+ * b200_flash_attn_packed_workspace_bytes(...) bytes; may be NULL where that is 0. */
+int b200_flash_attn_packed(const void *q, int64_t q_tok_stride, int64_t q_head_stride, const void *k,
+                           int64_t k_tok_stride, int64_t k_head_stride, const void *v, int64_t v_tok_stride,
+                           int64_t v_head_stride, void *out, int64_t out_tok_stride, int64_t out_head_stride,
+                           const int32_t *cu_q, const int32_t *cu_k, int64_t n_seqs, int64_t total_q,
+                           int64_t total_k, int64_t D, int64_t Hq, int64_t Hkv, float scale, int32_t dtype,
+                           void *workspace, size_t workspace_bytes, int32_t *dev_status, void *stream);
+size_t b200_flash_attn_packed_workspace_bytes(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t D,
+                                              int64_t Hq, int64_t Hkv, int32_t dtype);
+
+/* The K / V rows of new tokens (packed: sequence s owns rows [cu_new[s], cu_new[s + 1])
+ * of k, v [n_tokens][Hkv][D]) into the pool. seq_lens[s] counts the sequence's tokens
+ * with the new ones, so its rows go to its last positions; position p lies in block
+ * block_table[s * table_stride + p / block_tokens] (device int32, max_blocks valid
+ * entries a row). */
+int b200_paged_kv_append(const void *k, int64_t k_tok_stride, int64_t k_head_stride, const void *v,
+                         int64_t v_tok_stride, int64_t v_head_stride, const int32_t *cu_new,
+                         const int32_t *seq_lens, int64_t n_seqs, int64_t n_tokens, const b200_kv_pool *pool,
+                         const int32_t *block_table, int64_t table_stride, int64_t max_blocks,
+                         int32_t *dev_status, void *stream);
+
+/* GQA attention of one new token per sequence: q, out [n_seqs][Hq][D]; sequence s
+ * attends to positions [0, seq_lens[s]) of the pool through its row of block_table (as
+ * above; its own K / V already appended). A sequence of length 0 gives zeros; one
+ * longer than max_blocks * block_tokens is cut there. The keys of all sequences are
+ * spread evenly over the SMs; the parts of a split sequence are joined in a fixed
+ * order, so results do not depend on timing. Keys in a block whose index is out of
+ * range are left out. D 64 or 128. `workspace` as above
+ * (b200_flash_attn_paged_batch_workspace_bytes). */
+int b200_flash_attn_paged_batch(const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
+                                int64_t out_seq_stride, int64_t out_head_stride, const b200_kv_pool *pool,
+                                const int32_t *block_table, int64_t table_stride, int64_t max_blocks,
+                                const int32_t *seq_lens, int64_t n_seqs, int64_t Hq, float scale,
+                                void *workspace, size_t workspace_bytes, int32_t *dev_status, void *stream);
+size_t b200_flash_attn_paged_batch_workspace_bytes(int64_t n_seqs, int64_t D, int64_t Hq, int64_t Hkv,
+                                                   int32_t dtype);
+
+/* Samples one token per row of logits [n_rows][n_vocab] (row stride `row_stride`
+ * elements, any alignment) from given uniform numbers u[n_rows] in [0, 1). Per row,
+ * with device arrays temperature (required) and top_k, top_p, min_p (each nullable:
+ * filter off):
+ *   weight of token i: floor(2^40 * exp((x_i - max x) * (1 / temperature))), a whole
+ *   number, so every sum below is exact and the result does not depend on how the row
+ *   is split over the GPU;
+ *   order: by logit, largest first, equal logits by index;
+ *   top_k > 0 keeps the first top_k tokens of that order;
+ *   top_p < 1 keeps the shortest head of what top_k kept whose weights reach
+ *   floor(top_p * their sum), at least one token;
+ *   min_p drops the tokens below min_p (cut to at most 1) of the likeliest token;
+ *   the draw is the first kept token, by index, at which the running sum of kept
+ *   weights passes floor(u * the sum) (u outside [0, 1) is cut to it).
+ * temperature <= 0: the first index of the maximum. Logits of -inf have weight 0. A row
+ * with NaN or +inf, or with -inf alone, or with a NaN parameter, gives -1 and records
+ * B200_DEV_BAD_LOGITS (sampler.cpp:42-65). n_vocab <= 2^21; no workspace. */
+int b200_sample(const void *logits, int64_t row_stride, int64_t n_rows, int64_t n_vocab, int32_t dtype,
+                const float *u, const float *temperature, const int32_t *top_k, const float *top_p,
+                const float *min_p, int32_t *out_ids, int32_t *dev_status, void *stream);
 
 /* ------------------------------------------------------------------------
  * Qwen3 engine: device-resident weights, KV cache and activation arenas, the

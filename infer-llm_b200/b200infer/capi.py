@@ -90,6 +90,15 @@ _SIGS = {
     "b200_flash_attn_paged": ([_vp, _vp, _vp, C.c_int64, C.c_int64, _vp, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
                                C.c_int64, C.c_int64, C.c_float, _vp, _sz, _vp, _vp], C.c_int),
     "b200_flash_attn_paged_workspace_bytes": ([C.c_int64] * 5, _sz),
+    "b200_flash_attn_packed": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64,
+                                _i64, _i64, _i64, _i64, _i64, _f32, _i32, _vp, _sz, _vp, _vp], C.c_int),
+    "b200_flash_attn_packed_workspace_bytes": ([_i64] * 6 + [_i32], _sz),
+    "b200_paged_kv_append": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp],
+                             C.c_int),
+    "b200_flash_attn_paged_batch": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _f32,
+                                     _vp, _sz, _vp, _vp], C.c_int),
+    "b200_flash_attn_paged_batch_workspace_bytes": ([_i64] * 4 + [_i32], _sz),
+    "b200_sample": ([_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp], C.c_int),
     "b200_engine_inject_withhold": ([_vp, C.c_int32, C.c_int32], C.c_int),
     "b200_engine_set_decode_launch_counter": ([_vp, C.c_uint64], C.c_int),
     "b200_tp_unique_id": ([_vp], C.c_int),
@@ -298,4 +307,186 @@ class PagedKV:
         _chk("b200_flash_attn_paged", lib().b200_flash_attn_paged(
             _p(q), _p(self.ktab), _p(self.vtab), self.n_blocks, self.bt, _p(out), D, Hq, self.Hkv, Tq, Tkv, n_past,
             scale, _p(workspace), workspace.numel(), _p(status), _stream()))
+        return out
+
+
+# ---------------------------------------------------------------------------
+# Batched serving: packed prompts, paged caches of many sequences, sampling. Tensors
+# are float32, float16 or bfloat16, on one device, with a contiguous last axis; calls
+# go to the current torch stream of that device.
+
+class _KVPool(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("n_blocks", _i64), ("block_tokens", _i64), ("block_stride", _i64),
+                ("tok_stride", _i64), ("head_stride", _i64), ("n_head_kv", _i64), ("head_dim", _i64),
+                ("dtype", C.c_int32)]
+
+
+_DTYPES = {}
+
+
+def _dtype(t):
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise TypeError(f"expected float32, float16 or bfloat16, got {t.dtype}")
+    return d
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _rows(t, name, like):
+    """A [rows][heads][D] tensor of like's type and device, last axis contiguous."""
+    _need(t.dim() == 3 and t.dtype == like.dtype and t.device == like.device and
+          (t.stride(2) == 1 or t.shape[2] == 1), f"{name}: expected (rows, heads, D) of {like.dtype} on {like.device}, "
+                                                 "last axis contiguous")
+
+
+def _ints(t, name, n, dev):
+    import torch
+    _need(t.dim() == 1 and t.numel() == n and t.dtype == torch.int32 and t.device == dev and t.is_contiguous(),
+          f"{name}: expected {n} int32 on {dev}")
+
+
+def _raw_stream(dev):
+    import torch
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _on(t):
+    import torch
+    _need(t.is_cuda, "expected CUDA tensors")
+    return torch.cuda.device(t.device)
+
+
+def _status_word(status, dev):
+    if status is not None:
+        import torch
+        _need(status.dtype == torch.int32 and status.device == dev and status.numel() >= 1, "status: expected int32")
+    return _ptr(status)
+
+
+def _scratch(workspace, nbytes, dev):
+    import torch
+    if workspace is None:
+        return torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+    _need(workspace.is_contiguous() and workspace.device == dev and
+          workspace.numel() * workspace.element_size() >= nbytes, f"workspace: expected {nbytes} bytes on {dev}")
+    return workspace
+
+
+def flash_attn_packed(q, k, v, cu_q, cu_k=None, scale=0.0, out=None, workspace=None, status=None):
+    """Causal attention of packed sequences: q (Tq, Hq, D); k, v (Tk, Hkv, D); cu_q, cu_k int32
+    (n + 1,) offsets of the n sequences (cu_k None: as cu_q). Row i of a sequence with nq
+    queries and nk keys sees its keys 0 .. nk - nq + i. Returns (Tq, Hq, D)."""
+    import torch
+    with _on(q):
+        dev = q.device
+        _rows(q, "q", q), _rows(k, "k", q), _rows(v, "v", q)
+        Tq, Hq, D = q.shape
+        Tk, Hkv, _ = k.shape
+        _need(v.shape == k.shape and k.shape[2] == D and Hkv > 0 and Hq % Hkv == 0, "k, v: shapes do not go with q")
+        cu_k = cu_q if cu_k is None else cu_k
+        n = cu_q.numel() - 1
+        _ints(cu_q, "cu_q", n + 1, dev), _ints(cu_k, "cu_k", n + 1, dev)
+        if out is None:
+            out = torch.empty((Tq, Hq, D), device=dev, dtype=q.dtype)
+        else:
+            _rows(out, "out", q)
+            _need(out.shape == q.shape, "out: expected q's shape")
+        dt = _dtype(q)
+        nbytes = lib().b200_flash_attn_packed_workspace_bytes(n, Tq, Tk, D, Hq, Hkv, dt)
+        ws = _scratch(workspace, nbytes, dev)
+        _chk("b200_flash_attn_packed", lib().b200_flash_attn_packed(
+            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+            v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, D,
+            Hq, Hkv, scale, dt, _ptr(ws), nbytes, _status_word(status, dev), _raw_stream(dev)))
+        return out
+
+
+def _pool(k_pool, v_pool):
+    _need(k_pool.dim() == 4 and k_pool.shape == v_pool.shape and k_pool.stride() == v_pool.stride() and
+          k_pool.dtype == v_pool.dtype and k_pool.device == v_pool.device and k_pool.stride(3) == 1,
+          "k_pool, v_pool: expected two (blocks, block_tokens, Hkv, D) tensors alike, last axis contiguous")
+    n, bt, Hkv, D = k_pool.shape
+    s = k_pool.stride()
+    return _KVPool(k_pool.data_ptr(), v_pool.data_ptr(), n, bt, s[0], s[1], s[2], Hkv, D, _dtype(k_pool))
+
+
+def _table(block_table, n, dev):
+    import torch
+    _need(block_table.dim() == 2 and block_table.shape[0] == n and block_table.dtype == torch.int32 and
+          block_table.device == dev and (block_table.stride(1) == 1 or block_table.shape[1] == 1),
+          f"block_table: expected int32 ({n}, blocks) on {dev}")
+
+
+def paged_kv_append(k, v, cu_new, seq_lens, k_pool, v_pool, block_table, status=None):
+    """The rows k, v (T, Hkv, D) of new tokens into the pools (blocks, block_tokens, Hkv, D):
+    sequence s owns rows [cu_new[s], cu_new[s + 1]), which become its last positions;
+    seq_lens (n,) counts them in, block_table (n, max blocks) names its blocks; all int32."""
+    with _on(k):
+        dev = k.device
+        pool = _pool(k_pool, v_pool)
+        _rows(k, "k", k_pool), _rows(v, "v", k_pool)
+        _need(k.shape == v.shape and tuple(k.shape[1:]) == tuple(k_pool.shape[2:]), "k, v: expected (T, Hkv, D)")
+        n = seq_lens.numel()
+        _ints(cu_new, "cu_new", n + 1, dev), _ints(seq_lens, "seq_lens", n, dev), _table(block_table, n, dev)
+        _chk("b200_paged_kv_append", lib().b200_paged_kv_append(
+            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), cu_new.data_ptr(),
+            seq_lens.data_ptr(), n, k.shape[0], C.byref(pool), block_table.data_ptr(), block_table.stride(0),
+            block_table.shape[1], _status_word(status, dev), _raw_stream(dev)))
+
+
+def flash_attn_paged_batch(q, k_pool, v_pool, block_table, seq_lens, scale=0.0, out=None, workspace=None, status=None):
+    """One new token of each sequence, q (n, Hq, D), against its seq_lens[s] cached positions
+    in the pools (arguments as for paged_kv_append). Returns (n, Hq, D)."""
+    import torch
+    with _on(q):
+        dev = q.device
+        pool = _pool(k_pool, v_pool)
+        _rows(q, "q", k_pool)
+        n, Hq, D = q.shape
+        Hkv = k_pool.shape[2]
+        _need(D == k_pool.shape[3] and Hkv > 0 and Hq % Hkv == 0, "q: shape does not go with the pools")
+        _ints(seq_lens, "seq_lens", n, dev), _table(block_table, n, dev)
+        if out is None:
+            out = torch.empty((n, Hq, D), device=dev, dtype=q.dtype)
+        else:
+            _rows(out, "out", q)
+            _need(out.shape == q.shape, "out: expected q's shape")
+        nbytes = lib().b200_flash_attn_paged_batch_workspace_bytes(n, D, Hq, Hkv, pool.dtype)
+        ws = _scratch(workspace, nbytes, dev)
+        _chk("b200_flash_attn_paged_batch", lib().b200_flash_attn_paged_batch(
+            q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), C.byref(pool),
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), n, Hq, scale,
+            _ptr(ws), nbytes, _status_word(status, dev), _raw_stream(dev)))
+        return out
+
+
+def sample(logits, u, temperature, top_k=None, top_p=None, min_p=None, out=None, status=None):
+    """One token id per row of logits (n, vocab), drawn with u (n,) uniform in [0, 1);
+    temperature, top_p, min_p float32 (n,), top_k int32 (n,) (None: that filter is off).
+    Returns int32 (n,); -1 for a row that cannot be sampled."""
+    import torch
+    with _on(logits):
+        dev = logits.device
+        _need(logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1), "logits: expected (n, vocab)")
+        n, vocab = logits.shape
+        for t, name, kind in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
+                              (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                              (min_p, "min_p", torch.float32), (out, "out", torch.int32)):
+            _need(t is None or (t.dtype == kind and t.device == dev and t.numel() == n and t.is_contiguous()),
+                  f"{name}: expected {n} {kind} on {dev}")
+        out = torch.empty(n, device=dev, dtype=torch.int32) if out is None else out
+        _chk("b200_sample", lib().b200_sample(
+            logits.data_ptr(), logits.stride(0), n, vocab, _dtype(logits), u.data_ptr(), temperature.data_ptr(),
+            _ptr(top_k), _ptr(top_p), _ptr(min_p), out.data_ptr(), _status_word(status, dev), _raw_stream(dev)))
         return out
