@@ -26,8 +26,8 @@ __global__ void __launch_bounds__(kPkThreads, 2) packed_ffma_kernel(const Packed
     float *kt = qt + D * kPkPad;       // [D][key]; then P [key][row]
     float *vs = kt + D * kPkPad;       // [key][D]
     const int kvh = blockIdx.x % a.Hkv;
-    const PackedTile p = find_packed_tile<kPkRows>(a.cu_q, a.cu_k, a.n_seqs, a.total_q, a.total_k, a.G,
-                                                   blockIdx.x / a.Hkv, a.status);
+    const PackedTile p = find_packed_tile(a.cu_q, a.cu_k, a.n_seqs, a.total_q, a.total_k, a.G, kPkRows,
+                                          blockIdx.x / a.Hkv, a.status);
     if (p.seq < 0) return;
     const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
     const int rows = min(kPkRows, p.nq * a.G - p.tile * kPkRows);
@@ -214,6 +214,8 @@ int b200_flash_attn_packed(const void *q, int64_t q_tok_stride, int64_t q_head_s
     a.ws = workspace;
     a.status = dev_status;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const cudaError_t tc = packed_tc_launch(a, st);
+    if (tc != cudaErrorNotSupported) return status_of(tc);
     switch (dtype) {
         case B200_DTYPE_F16: return status_of(packed_by_dim<__half>(a, st));
         case B200_DTYPE_BF16: return status_of(packed_by_dim<__nv_bfloat16>(a, st));

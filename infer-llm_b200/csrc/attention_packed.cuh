@@ -18,4 +18,7 @@ struct PackedArgs {
     int32_t *status = nullptr;
 };
 
+// The tensor-core kernel; cudaErrorNotSupported (nothing launched) where it does not apply.
+cudaError_t packed_tc_launch(const PackedArgs &a, cudaStream_t stream);
+
 }  // namespace b200

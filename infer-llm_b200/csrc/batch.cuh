@@ -78,9 +78,8 @@ B200_DEVICE bool packed_range(const int32_t *cu, int s, int64_t total, int64_t &
 
 // Tile `at` of the line of all tiles (a sequence's last tiles, which see the most keys,
 // first), found by a whole warp; each lane takes every 32nd sequence.
-template <int M>
 B200_DEVICE PackedTile find_packed_tile(const int32_t *cu_q, const int32_t *cu_k, int n_seqs, int64_t total_q,
-                                        int64_t total_k, int G, int64_t at, int32_t *status) {
+                                        int64_t total_k, int G, int M, int64_t at, int32_t *status) {
     const int lane = threadIdx.x & 31;
     PackedTile p;
     int64_t before = 0;

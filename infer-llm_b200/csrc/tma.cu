@@ -27,6 +27,11 @@ EncodeTiledFn encode_fn() {
 
 bool tma_encode_f32(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
                     const uint32_t *box, CUtensorMapSwizzle swizzle) {
+    return tma_encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, rank, dims, strides_bytes, box, swizzle);
+}
+
+bool tma_encode(CUtensorMap *map, CUtensorMapDataType type, const void *base, int rank, const uint64_t *dims,
+                const uint64_t *strides_bytes, const uint32_t *box, CUtensorMapSwizzle swizzle) {
     EncodeTiledFn fn = encode_fn();
     if (!fn || rank < 1 || rank > 5) return false;
     cuuint64_t d[5], st[4];
@@ -37,7 +42,7 @@ bool tma_encode_f32(CUtensorMap *map, const void *base, int rank, const uint64_t
         es[i] = 1;
         if (i + 1 < rank) st[i] = strides_bytes[i];
     }
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, static_cast<cuuint32_t>(rank), const_cast<void *>(base), d, st, bx,
+    return fn(map, type, static_cast<cuuint32_t>(rank), const_cast<void *>(base), d, st, bx,
               es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

@@ -15,6 +15,10 @@ namespace b200 {
 bool tma_encode_f32(CUtensorMap *map, const void *base, int rank, const uint64_t *dims, const uint64_t *strides_bytes,
                     const uint32_t *box, CUtensorMapSwizzle swizzle);
 
+// The same for elements of another type.
+bool tma_encode(CUtensorMap *map, CUtensorMapDataType type, const void *base, int rank, const uint64_t *dims,
+                const uint64_t *strides_bytes, const uint32_t *box, CUtensorMapSwizzle swizzle);
+
 B200_DEVICE void tma_load_3d(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z, uint32_t bar,
                              uint64_t policy) {
     asm volatile(
