@@ -321,172 +321,201 @@ class _KVPool(C.Structure):
                 ("dtype", C.c_int32)]
 
 
-_DTYPES = {}
+class _Host:
+    """What the batched calls take from torch, looked up once: a decode step makes several of
+    these calls per layer, and each is only microseconds on the device."""
+
+    def __init__(self):
+        import torch
+        self.torch = torch
+        self.empty, self.i32, self.f32, self.u8 = torch.empty, torch.int32, torch.float32, torch.uint8
+        self.dtypes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        self.current = torch._C._cuda_getDevice
+        self.stream = torch._C._cuda_getCurrentRawStream
+        L = lib()
+        self.packed, self.packed_bytes = L.b200_flash_attn_packed, L.b200_flash_attn_packed_workspace_bytes
+        self.batch, self.batch_bytes = L.b200_flash_attn_paged_batch, L.b200_flash_attn_paged_batch_workspace_bytes
+        self.append, self.sample = L.b200_paged_kv_append, L.b200_sample
+
+
+_host = None
+
+
+def _start(t):
+    """(host, device index) for a call whose first tensor is t."""
+    global _host
+    if not t.is_cuda:
+        raise ValueError("expected CUDA tensors")
+    if _host is None:
+        _host = _Host()
+    return _host, t.get_device()
+
+
+def _elsewhere(fn, dev, *args, **kw):
+    """The call with its tensors' device made current."""
+    with _host.torch.cuda.device(dev):
+        return fn(*args, **kw)
 
 
 def _dtype(t):
-    if not _DTYPES:
-        import torch
-        _DTYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
-    d = _DTYPES.get(t.dtype)
+    d = _host.dtypes.get(t.dtype)
     if d is None:
         raise TypeError(f"expected float32, float16 or bfloat16, got {t.dtype}")
     return d
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+def _rows(t, name, dtype, dev):
+    """Checks a (rows, heads, D) tensor with a contiguous last axis; its shape and strides."""
+    st = t.stride()
+    if len(st) != 3 or t.dtype != dtype or t.get_device() != dev or (st[2] != 1 and t.shape[2] != 1):
+        raise ValueError(f"{name}: expected (rows, heads, D) of {dtype} on cuda:{dev}, last axis contiguous")
+    return st
 
 
-def _rows(t, name, like):
-    """A [rows][heads][D] tensor of like's type and device, last axis contiguous."""
-    _need(t.dim() == 3 and t.dtype == like.dtype and t.device == like.device and
-          (t.stride(2) == 1 or t.shape[2] == 1), f"{name}: expected (rows, heads, D) of {like.dtype} on {like.device}, "
-                                                 "last axis contiguous")
-
-
-def _ints(t, name, n, dev):
-    import torch
-    _need(t.dim() == 1 and t.numel() == n and t.dtype == torch.int32 and t.device == dev and t.is_contiguous(),
-          f"{name}: expected {n} int32 on {dev}")
-
-
-def _raw_stream(dev):
-    import torch
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _on(t):
-    import torch
-    _need(t.is_cuda, "expected CUDA tensors")
-    return torch.cuda.device(t.device)
+def _vector(t, name, n, dtype, dev):
+    if t.dtype != dtype or t.get_device() != dev or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name}: expected {n} contiguous {dtype} on cuda:{dev}")
+    return t.data_ptr()
 
 
 def _status_word(status, dev):
-    if status is not None:
-        import torch
-        _need(status.dtype == torch.int32 and status.device == dev and status.numel() >= 1, "status: expected int32")
-    return _ptr(status)
+    if status is None:
+        return None
+    if status.dtype != _host.i32 or status.get_device() != dev or status.numel() < 1:
+        raise ValueError(f"status: expected int32 on cuda:{dev}")
+    return status.data_ptr()
 
 
-def _scratch(workspace, nbytes, dev):
-    import torch
+def _scratch(workspace, nbytes, like, dev):
     if workspace is None:
-        return torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
-    _need(workspace.is_contiguous() and workspace.device == dev and
-          workspace.numel() * workspace.element_size() >= nbytes, f"workspace: expected {nbytes} bytes on {dev}")
+        return _host.empty(nbytes, device=like.device, dtype=_host.u8) if nbytes else None
+    if not workspace.is_contiguous() or workspace.get_device() != dev or workspace.nbytes < nbytes:
+        raise ValueError(f"workspace: expected {nbytes} bytes on cuda:{dev}")
     return workspace
+
+
+def _out_rows(out, q, dev):
+    if out is None:
+        return _host.empty(q.shape, device=q.device, dtype=q.dtype)
+    if out.shape != q.shape:
+        raise ValueError("out: expected q's shape")
+    _rows(out, "out", q.dtype, dev)
+    return out
 
 
 def flash_attn_packed(q, k, v, cu_q, cu_k=None, scale=0.0, out=None, workspace=None, status=None):
     """Causal attention of packed sequences: q (Tq, Hq, D); k, v (Tk, Hkv, D); cu_q, cu_k int32
     (n + 1,) offsets of the n sequences (cu_k None: as cu_q). Row i of a sequence with nq
     queries and nk keys sees its keys 0 .. nk - nq + i. Returns (Tq, Hq, D)."""
-    import torch
-    with _on(q):
-        dev = q.device
-        _rows(q, "q", q), _rows(k, "k", q), _rows(v, "v", q)
-        Tq, Hq, D = q.shape
-        Tk, Hkv, _ = k.shape
-        _need(v.shape == k.shape and k.shape[2] == D and Hkv > 0 and Hq % Hkv == 0, "k, v: shapes do not go with q")
-        cu_k = cu_q if cu_k is None else cu_k
-        n = cu_q.numel() - 1
-        _ints(cu_q, "cu_q", n + 1, dev), _ints(cu_k, "cu_k", n + 1, dev)
-        if out is None:
-            out = torch.empty((Tq, Hq, D), device=dev, dtype=q.dtype)
-        else:
-            _rows(out, "out", q)
-            _need(out.shape == q.shape, "out: expected q's shape")
-        dt = _dtype(q)
-        nbytes = lib().b200_flash_attn_packed_workspace_bytes(n, Tq, Tk, D, Hq, Hkv, dt)
-        ws = _scratch(workspace, nbytes, dev)
-        _chk("b200_flash_attn_packed", lib().b200_flash_attn_packed(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-            v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), cu_q.data_ptr(), cu_k.data_ptr(), n, Tq, Tk, D,
-            Hq, Hkv, scale, dt, _ptr(ws), nbytes, _status_word(status, dev), _raw_stream(dev)))
-        return out
+    h, dev = _start(q)
+    if h.current() != dev:
+        return _elsewhere(flash_attn_packed, dev, q, k, v, cu_q, cu_k, scale, out, workspace, status)
+    kind, dt = q.dtype, _dtype(q)
+    qs, ks, vs = _rows(q, "q", kind, dev), _rows(k, "k", kind, dev), _rows(v, "v", kind, dev)
+    Tq, Hq, D = q.shape
+    Tk, Hkv, Dk = k.shape
+    if v.shape != k.shape or Dk != D or Hkv <= 0 or Hq % Hkv:
+        raise ValueError("k, v: shapes do not go with q")
+    n = cu_q.shape[0] - 1
+    pq = _vector(cu_q, "cu_q", n + 1, h.i32, dev)
+    pk = pq if cu_k is None else _vector(cu_k, "cu_k", n + 1, h.i32, dev)
+    out = _out_rows(out, q, dev)
+    os = out.stride()
+    nbytes = h.packed_bytes(n, Tq, Tk, D, Hq, Hkv, dt)
+    ws = _scratch(workspace, nbytes, q, dev)
+    _chk("b200_flash_attn_packed", h.packed(
+        q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], out.data_ptr(), os[0], os[1],
+        pq, pk, n, Tq, Tk, D, Hq, Hkv, scale, dt, None if ws is None else ws.data_ptr(), nbytes, _status_word(status, dev),
+        h.stream(dev)))
+    return out
 
 
 def _pool(k_pool, v_pool):
-    _need(k_pool.dim() == 4 and k_pool.shape == v_pool.shape and k_pool.stride() == v_pool.stride() and
-          k_pool.dtype == v_pool.dtype and k_pool.device == v_pool.device and k_pool.stride(3) == 1,
-          "k_pool, v_pool: expected two (blocks, block_tokens, Hkv, D) tensors alike, last axis contiguous")
-    n, bt, Hkv, D = k_pool.shape
     s = k_pool.stride()
-    return _KVPool(k_pool.data_ptr(), v_pool.data_ptr(), n, bt, s[0], s[1], s[2], Hkv, D, _dtype(k_pool))
+    if len(s) != 4 or k_pool.shape != v_pool.shape or s != v_pool.stride() or k_pool.dtype != v_pool.dtype or \
+            k_pool.get_device() != v_pool.get_device() or s[3] != 1:
+        raise ValueError("k_pool, v_pool: expected two (blocks, block_tokens, Hkv, D) tensors alike, last axis contiguous")
+    n, bt, Hkv, D = k_pool.shape
+    return _KVPool(k_pool.data_ptr(), v_pool.data_ptr(), n, bt, s[0], s[1], s[2], Hkv, D, _dtype(k_pool)), Hkv, D
 
 
-def _table(block_table, n, dev):
-    import torch
-    _need(block_table.dim() == 2 and block_table.shape[0] == n and block_table.dtype == torch.int32 and
-          block_table.device == dev and (block_table.stride(1) == 1 or block_table.shape[1] == 1),
-          f"block_table: expected int32 ({n}, blocks) on {dev}")
+def _table(t, n, dev):
+    if t.dim() != 2 or t.shape[0] != n or t.dtype != _host.i32 or t.get_device() != dev or \
+            (t.stride(1) != 1 and t.shape[1] != 1):
+        raise ValueError(f"block_table: expected int32 ({n}, blocks) on cuda:{dev}")
+    # a table of one row may report any stride; the rows must not overlap
+    return t.data_ptr(), t.stride(0) if n > 1 else t.shape[1], t.shape[1]
 
 
 def paged_kv_append(k, v, cu_new, seq_lens, k_pool, v_pool, block_table, status=None):
     """The rows k, v (T, Hkv, D) of new tokens into the pools (blocks, block_tokens, Hkv, D):
     sequence s owns rows [cu_new[s], cu_new[s + 1]), which become its last positions;
     seq_lens (n,) counts them in, block_table (n, max blocks) names its blocks; all int32."""
-    with _on(k):
-        dev = k.device
-        pool = _pool(k_pool, v_pool)
-        _rows(k, "k", k_pool), _rows(v, "v", k_pool)
-        _need(k.shape == v.shape and tuple(k.shape[1:]) == tuple(k_pool.shape[2:]), "k, v: expected (T, Hkv, D)")
-        n = seq_lens.numel()
-        _ints(cu_new, "cu_new", n + 1, dev), _ints(seq_lens, "seq_lens", n, dev), _table(block_table, n, dev)
-        _chk("b200_paged_kv_append", lib().b200_paged_kv_append(
-            k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), cu_new.data_ptr(),
-            seq_lens.data_ptr(), n, k.shape[0], C.byref(pool), block_table.data_ptr(), block_table.stride(0),
-            block_table.shape[1], _status_word(status, dev), _raw_stream(dev)))
+    h, dev = _start(k)
+    if h.current() != dev:
+        return _elsewhere(paged_kv_append, dev, k, v, cu_new, seq_lens, k_pool, v_pool, block_table, status)
+    kind = k.dtype
+    if k_pool.get_device() != dev or k_pool.dtype != kind:
+        raise ValueError(f"k_pool: expected {kind} on cuda:{dev}")
+    pool, Hkv, D = _pool(k_pool, v_pool)
+    ks, vs = _rows(k, "k", kind, dev), _rows(v, "v", kind, dev)
+    T = k.shape[0]
+    if k.shape != v.shape or k.shape[1] != Hkv or k.shape[2] != D:
+        raise ValueError("k, v: expected (T, Hkv, D)")
+    n = seq_lens.shape[0]
+    table, stride, blocks = _table(block_table, n, dev)
+    _chk("b200_paged_kv_append", h.append(
+        k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _vector(cu_new, "cu_new", n + 1, h.i32, dev),
+        _vector(seq_lens, "seq_lens", n, h.i32, dev), n, T, C.byref(pool), table, stride, blocks, _status_word(status, dev),
+        h.stream(dev)))
 
 
 def flash_attn_paged_batch(q, k_pool, v_pool, block_table, seq_lens, scale=0.0, out=None, workspace=None, status=None):
     """One new token of each sequence, q (n, Hq, D), against its seq_lens[s] cached positions
     in the pools (arguments as for paged_kv_append). Returns (n, Hq, D)."""
-    import torch
-    with _on(q):
-        dev = q.device
-        pool = _pool(k_pool, v_pool)
-        _rows(q, "q", k_pool)
-        n, Hq, D = q.shape
-        Hkv = k_pool.shape[2]
-        _need(D == k_pool.shape[3] and Hkv > 0 and Hq % Hkv == 0, "q: shape does not go with the pools")
-        _ints(seq_lens, "seq_lens", n, dev), _table(block_table, n, dev)
-        if out is None:
-            out = torch.empty((n, Hq, D), device=dev, dtype=q.dtype)
-        else:
-            _rows(out, "out", q)
-            _need(out.shape == q.shape, "out: expected q's shape")
-        nbytes = lib().b200_flash_attn_paged_batch_workspace_bytes(n, D, Hq, Hkv, pool.dtype)
-        ws = _scratch(workspace, nbytes, dev)
-        _chk("b200_flash_attn_paged_batch", lib().b200_flash_attn_paged_batch(
-            q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), C.byref(pool),
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), n, Hq, scale,
-            _ptr(ws), nbytes, _status_word(status, dev), _raw_stream(dev)))
-        return out
+    h, dev = _start(q)
+    if h.current() != dev:
+        return _elsewhere(flash_attn_paged_batch, dev, q, k_pool, v_pool, block_table, seq_lens, scale, out, workspace,
+                          status)
+    kind, dt = q.dtype, _dtype(q)
+    if k_pool.get_device() != dev or k_pool.dtype != kind:
+        raise ValueError(f"k_pool: expected {kind} on cuda:{dev}")
+    pool, Hkv, Dk = _pool(k_pool, v_pool)
+    qs = _rows(q, "q", kind, dev)
+    n, Hq, D = q.shape
+    if D != Dk or Hkv <= 0 or Hq % Hkv:
+        raise ValueError("q: shape does not go with the pools")
+    table, stride, blocks = _table(block_table, n, dev)
+    out = _out_rows(out, q, dev)
+    os = out.stride()
+    nbytes = h.batch_bytes(n, D, Hq, Hkv, dt)
+    ws = _scratch(workspace, nbytes, q, dev)
+    _chk("b200_flash_attn_paged_batch", h.batch(
+        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], C.byref(pool), table, stride, blocks,
+        _vector(seq_lens, "seq_lens", n, h.i32, dev), n, Hq, scale, None if ws is None else ws.data_ptr(), nbytes,
+        _status_word(status, dev), h.stream(dev)))
+    return out
 
 
 def sample(logits, u, temperature, top_k=None, top_p=None, min_p=None, out=None, status=None):
     """One token id per row of logits (n, vocab), drawn with u (n,) uniform in [0, 1);
     temperature, top_p, min_p float32 (n,), top_k int32 (n,) (None: that filter is off).
     Returns int32 (n,); -1 for a row that cannot be sampled."""
-    import torch
-    with _on(logits):
-        dev = logits.device
-        _need(logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1), "logits: expected (n, vocab)")
-        n, vocab = logits.shape
-        for t, name, kind in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
-                              (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
-                              (min_p, "min_p", torch.float32), (out, "out", torch.int32)):
-            _need(t is None or (t.dtype == kind and t.device == dev and t.numel() == n and t.is_contiguous()),
-                  f"{name}: expected {n} {kind} on {dev}")
-        out = torch.empty(n, device=dev, dtype=torch.int32) if out is None else out
-        _chk("b200_sample", lib().b200_sample(
-            logits.data_ptr(), logits.stride(0), n, vocab, _dtype(logits), u.data_ptr(), temperature.data_ptr(),
-            _ptr(top_k), _ptr(top_p), _ptr(min_p), out.data_ptr(), _status_word(status, dev), _raw_stream(dev)))
-        return out
+    h, dev = _start(logits)
+    if h.current() != dev:
+        return _elsewhere(sample, dev, logits, u, temperature, top_k, top_p, min_p, out, status)
+    st = logits.stride()
+    dt = _dtype(logits)
+    if len(st) != 2 or (st[1] != 1 and logits.shape[1] != 1):
+        raise ValueError("logits: expected (n, vocab), last axis contiguous")
+    n, vocab = logits.shape
+    if out is None:
+        out = h.empty(n, device=logits.device, dtype=h.i32)
+    _chk("b200_sample", h.sample(
+        logits.data_ptr(), st[0], n, vocab, dt, _vector(u, "u", n, h.f32, dev),
+        _vector(temperature, "temperature", n, h.f32, dev),
+        None if top_k is None else _vector(top_k, "top_k", n, h.i32, dev),
+        None if top_p is None else _vector(top_p, "top_p", n, h.f32, dev),
+        None if min_p is None else _vector(min_p, "min_p", n, h.f32, dev), _vector(out, "out", n, h.i32, dev),
+        _status_word(status, dev), h.stream(dev)))
+    return out
