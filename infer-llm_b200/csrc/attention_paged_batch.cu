@@ -34,6 +34,8 @@ namespace {
 
 constexpr int kPbWarps = 4;
 constexpr int kPbThreads = 32 * kPbWarps;
+constexpr int kPbMostCtas = 320;
+constexpr int kJoinThreads = 256;
 
 struct PbArgs {
     const void *q = nullptr;
@@ -553,8 +555,9 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const PbArgs
 // Joins the parts of each pair that more than one CTA took, and clears the rows of empty
 // sequences. One CTA a pair.
 template <typename T, int D, int HB>
-__global__ void __launch_bounds__(128) paged_batch_join_kernel(const PbArgs a, const int64_t grid) {
+__global__ void __launch_bounds__(kJoinThreads) paged_batch_join_kernel(const PbArgs a, const int64_t grid) {
     using Ge = Geometry<T, D, HB>;
+    __shared__ float factor[HB * kPbMostCtas], scale[HB];
     const int b = static_cast<int>(blockIdx.x / a.VH), vh = static_cast<int>(blockIdx.x % a.VH);
     const int64_t before = tiles_before<Ge::kTile>(a, b);
     const int64_t total = tiles_before<Ge::kTile>(a, a.n_seqs) * a.VH;
@@ -567,35 +570,53 @@ __global__ void __launch_bounds__(128) paged_batch_join_kernel(const PbArgs a, c
         const int64_t n = __ldg(a.lens + b);
         if (n < 0 || n > a.max_keys) set_status(a.status, B200_DEV_BAD_POSITION);
     }
-    int64_t ua = 0, c0 = 0, c1 = -1;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int64_t c0 = 0;
+    int parts = 0, slot0 = 0;  // CTAs c0 .. c0 + parts - 1 hold parts; only the first's may be a second part
     if (tiles > 0) {
-        ua = before * a.VH + static_cast<int64_t>(vh) * tiles;
+        const int64_t ua = before * a.VH + static_cast<int64_t>(vh) * tiles;
         c0 = share_owner(total, ua, ctas);
-        c1 = share_owner(total, ua + tiles - 1, ctas);
+        parts = static_cast<int>(share_owner(total, ua + tiles - 1, ctas) - c0) + 1;
+        slot0 = share_begin(total, c0, ctas) >= ua ? 0 : 1;
     }
     grid_wait();
-    if (c0 == c1) return;  // whole: written by its CTA
-    for (int i = threadIdx.x; i < heads * D; i += blockDim.x) {
-        const int g = i / D;
-        float M = -INFINITY, ls = 0.f, os = 0.f;
-        for (int64_t c = c0; c <= c1; ++c) {
-            const int slot = share_begin(total, c, ctas) >= ua ? 0 : 1;
-            const float *rec = a.ws + (c * 2 + slot) * Ge::kRec;
-            M = fmaxf(M, __ldcg(rec + HB * D + g));
+    if (parts == 1) return;  // whole: written by its CTA
+    if (parts == 0) {
+        for (int i = tid; i < heads * D; i += kJoinThreads) out[(i / D) * a.o_head + i % D] = from_f32<T>(0.f);
+        return;
+    }
+    const float *first = a.ws + (c0 * 2 + slot0) * Ge::kRec, *rest = a.ws + c0 * 2 * Ge::kRec;
+    const auto part = [&](int i) { return i == 0 ? first : rest + static_cast<int64_t>(i) * 2 * Ge::kRec; };
+    // each part's factor 2^(m - M) / sum, a warp per head and a lane per part
+    for (int g = warp; g < heads; g += kJoinThreads / 32) {
+        float M = -INFINITY;
+        for (int i = lane; i < parts; i += 32) {
+            const float m = __ldcg(part(i) + HB * D + g);
+            factor[g * kPbMostCtas + i] = m;
+            M = fmaxf(M, m);
         }
+        M = warp_max(M);
         const float ms = M == -INFINITY ? 0.f : M;
-        for (int64_t c = c0; c <= c1; ++c) {
-            const int slot = share_begin(total, c, ctas) >= ua ? 0 : 1;
-            const float *rec = a.ws + (c * 2 + slot) * Ge::kRec;
-            const float f = exp2_approx(__ldcg(rec + HB * D + g) - ms);
-            ls = fmaf(f, __ldcg(rec + HB * D + HB + g), ls);
-            os = fmaf(f, __ldcg(rec + i), os);
+        float sum = 0.f;
+        for (int i = lane; i < parts; i += 32) {
+            const float f = exp2_approx(factor[g * kPbMostCtas + i] - ms);
+            factor[g * kPbMostCtas + i] = f;
+            sum = fmaf(f, __ldcg(part(i) + HB * D + HB + g), sum);
         }
-        out[g * a.o_head + (i - g * D)] = from_f32<T>(ls > 0.f || ls != ls ? os / ls : 0.f);
+        sum = warp_sum(sum);
+        if (lane == 0) scale[g] = sum != 0.f ? 1.0f / sum : 0.f;
+    }
+    __syncthreads();
+    for (int j = tid; j < heads * D; j += kJoinThreads) {
+        const int g = j / D;
+        float acc = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < parts; ++i) acc = fmaf(factor[g * kPbMostCtas + i], __ldcg(part(i) + j), acc);
+        out[g * a.o_head + (j - g * D)] = from_f32<T>(acc * scale[g]);
     }
 }
 
-int pb_max_ctas() { return 2 * device_sm_count(); }
+int pb_max_ctas() { return device_sm_count() * 2 < kPbMostCtas ? device_sm_count() * 2 : kPbMostCtas; }
 
 // heads a block handles: the next instantiated size
 int pb_heads(int64_t G, bool f32) {
@@ -619,7 +640,8 @@ cudaError_t pb_launch(PbArgs a, int64_t Hkv, cudaStream_t st) {
     const int64_t ctas = min64(pb_max_ctas(), most > pb_max_ctas() ? pb_max_ctas() : pairs * most);
     e = b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPbThreads), Ge::kSmem, st, false, a);
     if (e != cudaSuccess) return e;
-    return b200_launch(paged_batch_join_kernel<T, D, HB>, dim3(static_cast<unsigned>(pairs)), dim3(128), 0, st, true, a,
+    return b200_launch(paged_batch_join_kernel<T, D, HB>, dim3(static_cast<unsigned>(pairs)), dim3(kJoinThreads), 0, st, true,
+                       a,
                        ctas);
 }
 
