@@ -1,4 +1,4 @@
-// Packed causal attention on the 5th-generation tensor cores for F16 and BF16.
+// Packed causal attention on the 5th-generation tensor cores, for F16, BF16 and F32.
 //
 // A CTA owns two slots, each a 128-row accumulator: scores S (128 x 128 keys) and output O
 // (128 x D) in tensor memory, and one softmax warpgroup with a thread per row. A step i
@@ -12,7 +12,8 @@
 //           end (half as long a chain for calls with few query tiles).
 // A query tile's rows are tokens times the G heads of a KV head (row = token * G + head), as
 // many whole tokens as fit 128 rows, so the heads that share keys share every tile.
-// Warp roles: warp 0 TMA, warp 1 tensor cores, warps 2-3 V check, warps 4-11 softmax.
+// Warp roles: warp 0 TMA, warp 1 tensor cores, warps 2-3 V check, warps 4-11 softmax, and for
+// F32 warps 12-15 the output's sum.
 //   * The running maximum moves only when it grows by more than 2^8, so rescaling O is rare
 //     (the result is unchanged: every p is bounded by 2^8). Statistics are F32; P is
 //     rounded to the element type, the sum is taken before that.
@@ -20,6 +21,16 @@
 //     have P = 0, but 0 times a V that is no number is not 0. The V check looks for such
 //     rows in the tiles that hide keys, clears them in shared memory, and notes them; rows that do
 //     see one of them add its term in the epilogue.
+//   * F32 (NT = 1) runs as three F16 products. With a tile's values scaled by a power of two to a
+//     largest magnitude in [2^14, 2^15), x = hi + lo of two F16 numbers holds 22 bits
+//     of x (and an absolute 2^-39 of the tile's largest), and x y = hi hi + hi lo + lo hi
+//     up to 2^-22. packed_split_kernel writes K and V so, as hi and lo planes with one
+//     exponent per 128-key tile and KV head; Q rows are split by the softmax threads
+//     (an exponent per row), P by construction (p <= 1, times 2^14). The tensor cores
+//     round their sums toward zero: over a long row that bias reached 1e-5 at 8192 keys. So each
+//     step's O starts from zero (lo products first), and a fourth warpgroup adds the steps
+//     up in F32 registers, each with its own row maximum and V exponent. An FFMA kernel has no
+//     such rounding but a 20th of the rate; TF32 products would keep 11 bits.
 // Every mbarrier wait is bounded; one that runs out records B200_DEV_TIMEOUT, and the CTA
 // waits (bounded) for its copies and products and frees its tensor memory.
 #include "attention_packed.cuh"
@@ -31,22 +42,26 @@ namespace b200 {
 namespace {
 
 constexpr int kPtRows = 128, kPtKeys = 128;
-constexpr int kPtThreads = 384;
+template <typename T>
+constexpr int kPtThreads = __is_same(T, float) ? 512 : 384;
 constexpr int kMaskedTiles = 4;  // key tiles in which some row of a CTA hides keys (at most 256 tokens)
 constexpr float kPtRescale = 8.0f;
 
-template <int D, int NT>
+// PL: planes of an operand tile (2: hi and lo of F32)
+template <int D, int NT, int PL>
 struct PtGeometry {
+    static_assert(PL == 1 || NT == 1, "F32 tiles leave room for one query tile");
     static constexpr uint32_t kBox = kPtKeys * 128;           // 64 elements of 128 rows
-    static constexpr uint32_t kTile = (D / 64) * kBox;        // a 128-row tile of Q, K or V
-    static constexpr int kStages = D == 128 ? (NT == 2 ? 5 : 6) : 8;
-    static constexpr uint32_t kOffRing = NT * kTile;
+    static constexpr uint32_t kTile = (D / 64) * kBox;        // a plane of a 128-row tile of Q, K or V
+    static constexpr int kStages = D == 128 ? (PL == 2 ? 4 : NT == 2 ? 5 : 6) : 8;
+    static constexpr uint32_t kOffRing = NT * PL * kTile;
     static constexpr uint32_t kOffBar = kOffRing + kStages * kTile;
-    static constexpr uint32_t kOffBad = kOffBar + 320;        // [kMaskedTiles][4] words, then "any"
+    static constexpr uint32_t kOffStat = kOffBar + 384;       // F32: (m, l) of a slot's last two steps
+    static constexpr uint32_t kOffBad = kOffStat + (PL == 2 ? 4 * kPtRows * 8 : 0);        // [kMaskedTiles][4] words, then "any"
     static constexpr size_t kSmem = 1024 + kOffBad + 128;
 };
 
-// The planes (K or V tiles) of a key-tile sequence in the order of their first use.
+// K and V tiles of a key-tile sequence, numbered in the order of their first use.
 template <int NT>
 B200_DEVICE int plane_k(int t) { return NT == 2 ? 2 * t : (t == 0 ? 0 : 2 * t - 1); }
 template <int NT>
@@ -63,12 +78,98 @@ B200_DEVICE uint32_t pack_pair(float x, float y) {
     }
 }
 
+// F32 operands split for the tensor cores: planes of F16 rows [2][total_k][Hkv][D], and per
+// (key tile, KV head) the exponents of K and of V.
+struct SplitView {
+    const int32_t *exps = nullptr;
+    int64_t total_k = 0;
+};
+constexpr int kTop = 14;  // largest magnitudes in [2^14, 2^15); P <= 1 times 2^14
+
+// A tile's place in `exps`: increasing along the packed keys for any lengths, since
+// floor(x) + ceil(y) <= floor(x + y) + 1.
+B200_DEVICE int64_t split_index(int64_t k0, int seq, int t) { return k0 / kPtKeys + seq + t; }
+
+B200_DEVICE float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(max(-126, min(127, e)) + 127) << 23); }
+
+// floor(log2 x) of the largest finite magnitude (as its bits), at least -100
+B200_DEVICE int top_exponent(uint32_t bits) { return max(-100, static_cast<int>(bits >> 23) - 127); }
+B200_DEVICE uint32_t finite_magnitude(float x) {
+    const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
+    return u < 0x7F800000u ? u : 0u;
+}
+// hi + lo = x (22 bits); a value that is no number stays one, in hi
+B200_DEVICE void split_f16(float x, __half &hi, __half &lo) {
+    hi = __float2half_rn(x);
+    lo = finite_magnitude(x) || x == 0.f ? __float2half_rn(x - __half2float(hi)) : __half(0.f);
+}
+B200_DEVICE void split_f16x2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&r);
+}
+
+constexpr int kSplitThreads = 256;
+
+// One CTA: the K or V rows of one key tile and KV head, as hi and lo planes with the tile's
+// exponent. A pass over the bytes: HBM bounds it.
+template <int D>
+__global__ void __launch_bounds__(kSplitThreads) packed_split_kernel(const PackedArgs a, __half *planes, int32_t *exps) {
+    constexpr int V4 = D / 4, PER = kPtKeys * V4 / kSplitThreads;  // float4 a row, a thread
+    __shared__ uint32_t warp_top[kSplitThreads / 32];
+    grid_launch_dependents();
+    const int kvh = (blockIdx.x >> 1) % a.Hkv, is_v = blockIdx.x & 1;
+    const PackedTile p = find_packed_tile(a.cu_k, a.cu_k, a.n_seqs, a.total_k, a.total_k, 1, kPtKeys,
+                                          (blockIdx.x >> 1) / a.Hkv, nullptr);
+    if (p.seq < 0) return;
+    const float *src = static_cast<const float *>(is_v ? a.v : a.k) + kvh * (is_v ? a.v_head : a.k_head);
+    const int64_t tok = is_v ? a.v_tok : a.k_tok;
+    const int rows = min(kPtKeys, p.nk - p.tile * kPtKeys);
+    const int64_t first = p.k0 + static_cast<int64_t>(p.tile) * kPtKeys;
+    float4 x[PER];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int e = threadIdx.x + i * kSplitThreads, r = e / V4, c = e % V4;
+        x[i] = r < rows ? __ldg(reinterpret_cast<const float4 *>(src + (first + r) * tok) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        top = max(max(top, max(finite_magnitude(x[i].x), finite_magnitude(x[i].y))),
+                  max(finite_magnitude(x[i].z), finite_magnitude(x[i].w)));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSplitThreads / 32; ++w) top = max(top, warp_top[w]);
+    const int e = top_exponent(top);
+    const float s = pow2(kTop - e);
+    if (threadIdx.x == 0) exps[(split_index(p.k0, p.seq, p.tile) * a.Hkv + kvh) * 2 + is_v] = e - kTop;
+    const int64_t plane = a.total_k * a.Hkv * D;
+    __half *dst = planes + (is_v ? 2 * plane : 0) + kvh * D;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int el = threadIdx.x + i * kSplitThreads, r = el / V4, c = el % V4;
+        if (r >= rows) continue;
+        __half h[4], l[4];
+        split_f16(x[i].x * s, h[0], l[0]);
+        split_f16(x[i].y * s, h[1], l[1]);
+        split_f16(x[i].z * s, h[2], l[2]);
+        split_f16(x[i].w * s, h[3], l[3]);
+        __half *d = dst + (first + r) * a.Hkv * D + 4 * c;
+        *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<const uint2 *>(h);
+        *reinterpret_cast<uint2 *>(d + plane) = *reinterpret_cast<const uint2 *>(l);
+    }
+}
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kPtThreads, 1)
+__global__ void __launch_bounds__(kPtThreads<T>, 1)
     packed_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                     const __grid_constant__ CUtensorMap tv, const PackedArgs a) {
-    using Ge = PtGeometry<D, NT>;
-    constexpr bool kBf16 = !__is_same(T, __half);
+                     const __grid_constant__ CUtensorMap tv, const PackedArgs a, const SplitView sp) {
+    constexpr bool SPLIT = __is_same(T, float);
+    constexpr int PL = SPLIT ? 2 : 1;
+    using Ge = PtGeometry<D, NT, PL>;
+    constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
     constexpr uint32_t kIdS = idesc_f16(kPtRows, kPtKeys, kBf16, false, false);
     constexpr uint32_t kIdO = idesc_f16(kPtRows, D, kBf16, false, true);
     constexpr int S = Ge::kStages;
@@ -77,15 +178,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const uint32_t sbase = (raw + 1023u) & ~1023u;
     unsigned char *base = pt_raw + (sbase - raw);
     uint64_t *bars = reinterpret_cast<uint64_t *>(base + Ge::kOffBar);
-    uint64_t *full = bars;            // [S] plane landed
+    uint64_t *full = bars;            // [S] a plane of a K or V tile landed
     uint64_t *empty = bars + S;       // [S] plane read by its last product
     uint64_t *q_full = bars + 2 * S;
     uint64_t *s_full = q_full + 1;    // [2] scores of the slot's step complete (and all earlier products)
     uint64_t *p_full = s_full + 2;    // [2] P written, O rescaled
-    uint64_t *o_final = p_full + 2;   // [2] the slot's last product complete
+    uint64_t *o_final = p_full + 2;   // [2] the slot's last product complete (F32: each step's)
     uint64_t *v_ok = o_final + 2;     // [kMaskedTiles] the masked tile's V checked
     uint64_t *v_ask = v_ok + kMaskedTiles;  // [kMaskedTiles] its V landed: to be checked
-    uint64_t *idle = v_ask + kMaskedTiles;
+    uint64_t *o_empty = v_ask + kMaskedTiles;  // [2] F32: the step's O has been added up
+    uint64_t *st_full = o_empty + 2;           // [2] F32: the step's (m, l) written
+    uint64_t *idle = st_full + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(idle + 1);
     uint32_t *bad = reinterpret_cast<uint32_t *>(base + Ge::kOffBad);
 
@@ -107,11 +210,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        mbar_init(q_full, 1);
+        mbar_init(q_full, SPLIT ? 256 : 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&s_full[s], 1);
             mbar_init(&p_full[s], 128);
             mbar_init(&o_final[s], 1);
+            mbar_init(&o_empty[s], 128);
+            mbar_init(&st_full[s], 128);
         }
         for (int s = 0; s < kMaskedTiles; ++s) {
             mbar_init(&v_ok[s], 64);
@@ -130,6 +235,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    if (SPLIT) grid_wait();  // the split planes
     const auto col_s = [&](int slot) { return tmem + static_cast<uint32_t>(slot * kPtKeys); };
     const auto col_o = [&](int slot) { return tmem + 256u + static_cast<uint32_t>(slot * 128); };
     const auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -138,72 +244,130 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         return false;
     };
 
+            // softmax and output threads: a row of the slot's query tile, a lane of tensor memory
+    const int slot = (warp - 4) >> 2, qq = warp & 3;
+            const int r = 32 * qq + lane;
+            const uint32_t lanes = static_cast<uint32_t>(32 * qq) << 16;
+            const int tok = t0 + (NT == 2 ? slot * BQ : 0) + r / G;
+            const bool live = r < BQ * G && tok < p.nq;
+            const int last = live ? tok + shift : -1;  // last key the row sees
+            const T *q_row = static_cast<const T *>(a.q) + (p.q0 + tok) * a.q_tok + (kvh * G + r % G) * a.q_head;
+            T *dst = static_cast<T *>(a.out) + (p.q0 + tok) * a.o_tok + (kvh * G + r % G) * a.o_head;
+            // x (columns [c, c + 32) of the row's output) plus the terms of the cleared V rows it sees
+            const auto add_cleared = [&](float (&x)[32], int c, float m_row, float inv) {
+                for (int w = 0; w < 4 * kMaskedTiles; ++w) {
+                    for (uint32_t mask = bad[w]; mask; mask &= mask - 1) {
+                        const int key = first_masked * kPtKeys + 32 * w + __ffs(static_cast<int>(mask)) - 1;
+                        if (key > last) continue;
+                        const T *kr = static_cast<const T *>(a.k) + (p.k0 + key) * a.k_tok + kvh * a.k_head;
+                        const T *vr = static_cast<const T *>(a.v) + (p.k0 + key) * a.v_tok + kvh * a.v_head;
+                        float s = 0.f;
+                        for (int d = 0; d < D; ++d) s = fmaf(to_f32<T>(q_row[d]), to_f32<T>(kr[d]), s);
+                        const float pr = exp2_approx(fmaf(s, a.sl2, -m_row)) * inv;
+    #pragma unroll
+                        for (int j = 0; j < 32; ++j) x[j] = fmaf(pr, to_f32<T>(vr[c + j]), x[j]);
+                    }
+                }
+            };
+
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if constexpr (SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 0 && lane == 0 && nt > 0) {
             // ---- TMA
             const uint64_t pol = policy_evict_last();  // K / V are read again by the other query tiles
-            mbar_arrive_expect_tx(q_full, NT * (D / 64) * static_cast<uint32_t>(BQ * G) * 128u);
-            for (int x = 0; x < NT; ++x)
-                for (int b = 0; b < D / 64; ++b)
-                    tma_load_3d(sbase + x * Ge::kTile + b * Ge::kBox, &tq, 64 * b, kvh * G,
-                                static_cast<int32_t>(p.q0) + t0 + x * BQ, smem_addr(q_full), pol);
+            if (!SPLIT) {
+                mbar_arrive_expect_tx(q_full, NT * (D / 64) * static_cast<uint32_t>(BQ * G) * 128u);
+                for (int x = 0; x < NT; ++x)
+                    for (int b = 0; b < D / 64; ++b)
+                        tma_load_3d(sbase + x * Ge::kTile + b * Ge::kBox, &tq, 64 * b, kvh * G,
+                                    static_cast<int32_t>(p.q0) + t0 + x * BQ, smem_addr(q_full), pol);
+            }
             int issued = 0;
-            const auto plane = [&](const CUtensorMap *map, int t) {
-                const int st = issued % S;
-                if (issued >= S && !wait(&empty[st], ((issued / S) - 1) & 1)) return false;
-                mbar_arrive_expect_tx(&full[st], Ge::kTile);
+            const auto tile = [&](const CUtensorMap *map, int t) {
+                for (int h = PL - 1; h >= 0; --h) {  // lo, then hi
+                    const int st = issued % S;
+                    if (issued >= S && !wait(&empty[st], ((issued / S) - 1) & 1)) return false;
+                    mbar_arrive_expect_tx(&full[st], Ge::kTile);
 #pragma unroll
-                for (int b = 0; b < D / 64; ++b)
-                    tma_load_3d(sbase + Ge::kOffRing + st * Ge::kTile + b * Ge::kBox, map, 64 * b, kvh,
-                                static_cast<int32_t>(p.k0) + t * kPtKeys, smem_addr(&full[st]), pol);
-                ++issued;
+                    for (int b = 0; b < D / 64; ++b)
+                        tma_load_3d(sbase + Ge::kOffRing + st * Ge::kTile + b * Ge::kBox, map, 64 * b, kvh,
+                                    static_cast<int32_t>(p.k0 + h * sp.total_k) + t * kPtKeys, smem_addr(&full[st]), pol);
+                    ++issued;
+                }
                 return true;
             };
             bool ok = true;
             if (NT == 1) {
-                ok = plane(&tk, 0) && (nt < 2 || plane(&tk, 1));
-                for (int t = 0; t < nt && ok; ++t) ok = plane(&tv, t) && (t + 2 >= nt || plane(&tk, t + 2));
+                ok = tile(&tk, 0) && (nt < 2 || tile(&tk, 1));
+                for (int t = 0; t < nt && ok; ++t) ok = tile(&tv, t) && (t + 2 >= nt || tile(&tk, t + 2));
             } else {
-                for (int t = 0; t < nt && ok; ++t) ok = plane(&tk, t) && plane(&tv, t);
+                for (int t = 0; t < nt && ok; ++t) ok = tile(&tk, t) && tile(&tv, t);
             }
             // copies still landing in this CTA's shared memory
-            wait_poll(q_full, 0, nullptr);
+            if (!SPLIT) wait_poll(q_full, 0, nullptr);
             for (int i = max(0, issued - S); i < issued; ++i) wait_poll(&full[i % S], (i / S) & 1, nullptr);
         } else if (warp == 1 && lane == 0 && nt > 0) {
             // ---- tensor cores
             const auto at = [&](int pl) { return sbase + Ge::kOffRing + (pl % S) * Ge::kTile; };
-            const auto issue_s = [&](int i) {
-                const int slot = i & 1, t = NT == 2 ? i >> 1 : i, pl = plane_k<NT>(t);
-                if (!wait(&full[pl % S], (pl / S) & 1)) return false;
-                tc_fence_after();
-                const uint32_t q = sbase + (NT == 2 ? slot : 0) * Ge::kTile, k = at(pl);
+            const auto landed = [&](int pl) { return wait(&full[pl % S], (pl / S) & 1); };
+            // S (+)= a plane of Q . a plane of K
+            const auto scores = [&](int slot, uint32_t q, int pl, bool add) {
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk)
                     tc_mma_f16(col_s(slot), desc_k_sw128(q + (kk >> 2) * Ge::kBox) + 2 * (kk & 3),
-                               desc_k_sw128(k + (kk >> 2) * Ge::kBox) + 2 * (kk & 3), kIdS, kk > 0 ? 1u : 0u);
+                               desc_k_sw128(at(pl) + (kk >> 2) * Ge::kBox) + 2 * (kk & 3), kIdS, add || kk > 0 ? 1u : 0u);
+            };
+            // O (+)= P . a plane of V. P lies over the scores: 16 keys in 8 columns; F32: each 32
+            // columns hold hi, then lo of their 32 keys
+            const auto values = [&](int slot, bool lo, int pl, bool add) {
+#pragma unroll
+                for (int kk = 0; kk < kPtKeys / 16; ++kk) {
+                    const uint32_t c = SPLIT ? 32 * (kk >> 1) + 8 * (kk & 1) + (lo ? 16 : 0) : 8 * kk;
+                    tc_mma_f16_ts(col_o(slot), col_s(slot) + c, desc_mn_sw128(at(pl) + kk * 2048, Ge::kBox), kIdO,
+                                  add || kk > 0 ? 1u : 0u);
+                }
+            };
+            const auto issue_s = [&](int i) {
+                const int slot = i & 1, pl = PL * plane_k<NT>(NT == 2 ? i >> 1 : i);
+                const uint32_t q = sbase + (NT == 2 ? slot : 0) * Ge::kTile;
+                if (!landed(pl)) return false;
+                tc_fence_after();
+                scores(slot, q, pl, false);
+                if (SPLIT) {  // the small products first: the sum loses least
+                    tc_commit(smem_addr(&empty[pl % S]));
+                    if (!landed(pl + 1)) return false;
+                    tc_fence_after();
+                    scores(slot, q + Ge::kTile, pl + 1, true);
+                    scores(slot, q, pl + 1, true);
+                }
                 tc_commit(smem_addr(&s_full[slot]));
-                if (NT == 1 || slot == 1) tc_commit(smem_addr(&empty[pl % S]));
+                if (NT == 1 || slot == 1) tc_commit(smem_addr(&empty[(pl + PL - 1) % S]));
                 return true;
             };
             bool ok = wait(q_full, 0);
             for (int i = 0; i < min(2, steps) && ok; ++i) ok = issue_s(i);
             for (int i = 0; i < steps && ok; ++i) {
-                const int slot = i & 1, t = NT == 2 ? i >> 1 : i, pl = plane_v<NT>(t, nt);
+                const int slot = i & 1, t = NT == 2 ? i >> 1 : i, pl = PL * plane_v<NT>(t, nt);
                 const bool check = t >= first_masked && (NT == 1 || slot == 0);
-                ok = wait(&full[pl % S], (pl / S) & 1);
+                ok = landed(pl) && (!SPLIT || !check || landed(pl + 1));
                 if (!ok) break;
                 if (check) mbar_arrive(&v_ask[t - first_masked]);  // done while the softmax runs
-                ok = wait(&p_full[slot], (i >> 1) & 1) && (!check || wait(&v_ok[t - first_masked], 0));
+                ok = wait(&p_full[slot], (i >> 1) & 1) && (!check || wait(&v_ok[t - first_masked], 0)) &&
+                     (!SPLIT || i < 2 || wait(&o_empty[slot], ((i >> 1) - 1) & 1));
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t v = at(pl);
-#pragma unroll
-                for (int kk = 0; kk < kPtKeys / 16; ++kk)
-                    tc_mma_f16_ts(col_o(slot), col_s(slot) + 8 * kk, desc_mn_sw128(v + kk * 2048, Ge::kBox), kIdO,
-                                  (i >= 2 || kk > 0) ? 1u : 0u);
-                if (NT == 1 || slot == 1) tc_commit(smem_addr(&empty[pl % S]));
-                if (i + 2 >= steps) tc_commit(smem_addr(&o_final[slot]));
+                values(slot, false, pl, !SPLIT && i >= 2);
+                if (SPLIT) {
+                    tc_commit(smem_addr(&empty[pl % S]));
+                    ok = landed(pl + 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    values(slot, true, pl + 1, true);
+                    values(slot, false, pl + 1, true);
+                }
+                if (NT == 1 || slot == 1) tc_commit(smem_addr(&empty[(pl + PL - 1) % S]));
+                if (SPLIT || i + 2 >= steps) tc_commit(smem_addr(&o_final[slot]));
                 if (i + 2 < steps) ok = issue_s(i + 2);
             }
             // no product may still use tensor memory or the ring when the CTA exits
@@ -213,19 +377,22 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             // ---- V check: rows of the masked tiles that hold Inf or NaN, cleared and noted
             constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
             for (int t = first_masked; t < nt; ++t) {
-                const int pl = plane_v<NT>(t, nt);
+                const int pl = PL * plane_v<NT>(t, nt);
                 // the tensor-core warp has seen this phase of `full` and holds it until the
                 // check is done, so its parity is not ambiguous here
-                if (!__all_sync(0xffffffffu, wait(&v_ask[t - first_masked], 0) && wait(&full[pl % S], (pl / S) & 1))) break;
+                if (!__all_sync(0xffffffffu, wait(&v_ask[t - first_masked], 0) && wait(&full[pl % S], (pl / S) & 1) &&
+                                                 (!SPLIT || wait(&full[(pl + 1) % S], ((pl + 1) / S) & 1))))
+                    break;
                 unsigned char *v = base + Ge::kOffRing + (pl % S) * Ge::kTile;
+                unsigned char *v2 = base + Ge::kOffRing + ((pl + PL - 1) % S) * Ge::kTile;  // F32: both planes
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int row = 64 * half + (warp - 2) * 32 + lane;
                     bool odd = false;
-#pragma unroll
-                    for (int c = 0; c < D / 8; ++c) {
-                        const uint4 u = *reinterpret_cast<const uint4 *>(v + (c >> 3) * Ge::kBox + row * 128 +
-                                                                         (((c & 7) ^ (row & 7)) << 4));
+#pragma unroll 4
+                    for (int c = 0; c < PL * D / 8; ++c) {
+                        const uint4 u = *reinterpret_cast<const uint4 *>(
+                            (c < D / 8 ? v : v2) + ((c % (D / 8)) >> 3) * Ge::kBox + row * 128 + (((c & 7) ^ (row & 7)) << 4));
                         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
@@ -234,9 +401,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     const uint32_t mask = __ballot_sync(0xffffffffu, odd);
                     if (mask) {
                         if (odd)
-                            for (int c = 0; c < D / 8; ++c)
-                                *reinterpret_cast<uint4 *>(v + (c >> 3) * Ge::kBox + row * 128 + (c & 7) * 16) =
-                                    make_uint4(0, 0, 0, 0);
+                            for (int c = 0; c < D / 8; ++c) {
+                                const uint32_t off = (c >> 3) * Ge::kBox + row * 128 + (c & 7) * 16;
+                                *reinterpret_cast<uint4 *>(v + off) = make_uint4(0, 0, 0, 0);
+                                *reinterpret_cast<uint4 *>(v2 + off) = make_uint4(0, 0, 0, 0);
+                            }
                         if (lane == 0) {
                             bad[(t - first_masked) * 4 + row / 32] = mask;
                             bad[4 * kMaskedTiles] = 1;
@@ -247,168 +416,300 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                 mbar_arrive(&v_ok[t - first_masked]);
             }
         }
+    } else if (SPLIT && warp >= 12) {
+        // ---- F32: the output's sum
+        if constexpr (SPLIT) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+            float2 *stat = reinterpret_cast<float2 *>(base + Ge::kOffStat);  // [step / 2 % 2][slot][row]
+            const int32_t *exps = sp.exps + (split_index(p.k0, p.seq, 0) * a.Hkv + kvh) * 2;
+            const int64_t ex_step = static_cast<int64_t>(a.Hkv) * 2;
+                            // the steps' O added up. Step i holds sum p v = O 2^(m + ev); l counts in 2^m
+                            float acc[D], L = 0.f, M = -INFINITY, R = -INFINITY;
+            #pragma unroll
+                            for (int d = 0; d < D; ++d) acc[d] = 0.f;
+                            int ev = steps > 0 ? __ldg(exps + 1) : 0;
+                            bool ok = true;
+            #pragma unroll 1
+                            for (int i = 0; i < steps; ++i) {
+                                const int sl = i & 1;
+                                ok = __all_sync(0xffffffffu, wait(&st_full[sl], (i >> 1) & 1) && wait(&o_final[sl], (i >> 1) & 1));
+                                if (!ok) break;
+                                tc_fence_after();
+                                const float2 st = stat[(((i >> 1) & 1) * 2 + sl) * kPtRows + r];
+                                const float e = st.x + static_cast<float>(ev);
+                                if (i + 1 < steps) ev = __ldg(exps + (i + 1) * ex_step + 1);
+                                if (st.x > M) {
+                                    L *= exp2_approx(M - st.x);
+                                    M = st.x;
+                                }
+                                const float f_l = st.x == -INFINITY ? 0.f : exp2_approx(st.x - M);
+                                L = fmaf(f_l, st.y, L);
+                                const float Rn = fmaxf(R, e);
+                                const float f_old = R == -INFINITY ? 0.f : exp2_approx(R - Rn);
+                                const float f_new = e == -INFINITY ? 0.f : exp2_approx(e - Rn);
+                                if (__any_sync(0xffffffffu, Rn > R)) {
+            #pragma unroll
+                                    for (int d = 0; d < D; ++d) acc[d] *= f_old;
+                                }
+                                R = Rn;
+            #pragma unroll
+                                for (int c = 0; c < D / 32; ++c) {
+                                    uint32_t o[32];
+                                    tc_ld32_nowait(col_o(sl) + lanes + 32 * c, o);
+                                    tc_wait_ld();
+                                    tc_reg_fence(o);
+            #pragma unroll
+                                    for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(o[j]), f_new, acc[32 * c + j]);
+                                }
+                                tc_fence_before();
+                                mbar_arrive(&o_empty[sl]);
+                            }
+                            const float inv = L != 0.f ? 1.0f / L : 0.f;  // a row that sees no key: zeros
+                            // P and l both carry 2^kTop; two factors, neither of which overflows
+                            const float half = R == -INFINITY ? 0.f : 0.5f * (R - M);
+                            const float undo = exp2_approx(half);
+                            if (ok && live) {
+                                const bool any_bad = bad[4 * kMaskedTiles] != 0;
+            #pragma unroll
+                                for (int c = 0; c < D / 32; ++c) {
+                                    float x[32];
+            #pragma unroll
+                                    for (int j = 0; j < 32; ++j) x[j] = acc[32 * c + j] * inv * undo * undo;
+                                    if (any_bad) add_cleared(x, 32 * c, M, inv * pow2(kTop));
+            #pragma unroll
+                                    for (int j = 0; j < 32; j += 4)
+                                        *reinterpret_cast<float4 *>(dst + 32 * c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                                }
+                            }
+        }
+    } else if constexpr (SPLIT) {
+        // ---- F32 softmax
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+        float2 *stat = reinterpret_cast<float2 *>(base + Ge::kOffStat);  // [step / 2 % 2][slot][row]
+        const int32_t *exps = sp.exps + (split_index(p.k0, p.seq, 0) * a.Hkv + kvh) * 2;
+        const int64_t ex_step = static_cast<int64_t>(a.Hkv) * 2;
+                        // the row of Q as hi and lo planes: this warpgroup writes half of its columns
+                        const float4 *q4 = reinterpret_cast<const float4 *>(q_row);
+                        uint32_t top = 0;
+#pragma unroll 8
+                        for (int c = 0; c < D / 4; ++c) {
+                            const float4 x = live ? __ldg(q4 + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            top = max(max(top, max(finite_magnitude(x.x), finite_magnitude(x.y))),
+                                      max(finite_magnitude(x.z), finite_magnitude(x.w)));
+                        }
+                        const int eq = top_exponent(top) - kTop;
+                        const float s = pow2(-eq);
+#pragma unroll 2
+                        for (int c = 0; c < D / 16; ++c) {  // 16-byte chunks of eight halves
+                            const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+                            const float4 x = live ? __ldg(q4 + slot * (D / 8) + 2 * c) : zero;
+                            const float4 y = live ? __ldg(q4 + slot * (D / 8) + 2 * c + 1) : zero;
+                            const float e[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                            __align__(16) __half h[8], lo[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) split_f16(e[j] * s, h[j], lo[j]);
+                            const int chunk = slot * (D / 16) + c;
+                            unsigned char *at = base + (chunk >> 3) * Ge::kBox + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+                            *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(h);
+                            *reinterpret_cast<uint4 *>(at + Ge::kTile) = *reinterpret_cast<const uint4 *>(lo);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        mbar_arrive(q_full);
+                        const uint32_t ts = col_s(slot) + lanes;
+                        int ek = slot < steps ? __ldg(exps + slot * ex_step) : 0;
+        #pragma unroll 1
+                        for (int i = slot; i < steps; i += 2) {
+                            const float sl2 = a.sl2 * pow2(ek + eq);
+                            if (i + 2 < steps) ek = __ldg(exps + (i + 2) * ex_step);
+                            if (!__all_sync(0xffffffffu, wait(&s_full[slot], (i >> 1) & 1))) break;
+                            tc_fence_after();
+                            const int vis = last + 1 - i * kPtKeys;  // keys of the tile the row sees
+                            const bool whole = __all_sync(0xffffffffu, vis >= kPtKeys);
+                            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        #pragma unroll
+                            for (int c = 0; c < 4; c += 2) {
+                                uint32_t sv[2][32];
+                                tc_ld32_nowait(ts + 32 * c, sv[0]);
+                                tc_ld32_nowait(ts + 32 * c + 32, sv[1]);
+                                tc_wait_ld();
+        #pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    tc_reg_fence(sv[h]);
+        #pragma unroll
+                                    for (int j = 0; j < 32; ++j)
+                                        if (whole || 32 * (c + h) + j < vis) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(sv[h][j]));
+                                }
+                            }
+                            const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+                            const float shift_p = static_cast<float>(kTop) - (m == -INFINITY ? 0.f : m);
+                            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        #pragma unroll 1
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t sv[32], pv[32];
+                                tc_ld32_nowait(ts + 32 * c, sv);
+                                tc_wait_ld();
+                                tc_reg_fence(sv);
+        #pragma unroll
+                                for (int j = 0; j < 16; ++j) {
+                                    float x = exp2_approx(fmaf(__uint_as_float(sv[2 * j]), sl2, shift_p));
+                                    float y = exp2_approx(fmaf(__uint_as_float(sv[2 * j + 1]), sl2, shift_p));
+                                    if (!whole) {
+                                        x = 32 * c + 2 * j < vis ? x : 0.f;
+                                        y = 32 * c + 2 * j + 1 < vis ? y : 0.f;
+                                    }
+                                    sum[j & 1] += x;
+                                    sum[2 + (j & 1)] += y;
+                                    split_f16x2(x, y, pv[j], pv[16 + j]);
+                                }
+                                tc_st32(ts + 32 * c, pv);
+                            }
+                            stat[(((i >> 1) & 1) * 2 + slot) * kPtRows + r] = make_float2(m, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                            mbar_arrive(&st_full[slot]);
+                            tc_wait_st();
+                            tc_fence_before();
+                            mbar_arrive(&p_full[slot]);
+                        }
     } else {
+        // ---- softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        // ---- softmax: thread = row of the slot's query tile = tensor-memory lane
-        const int slot = (warp - 4) >> 2, qq = warp & 3;
-        const int r = 32 * qq + lane;
-        const uint32_t lanes = static_cast<uint32_t>(32 * qq) << 16;
-        const uint32_t ts = col_s(slot) + lanes, to = col_o(slot) + lanes;
-        const int tok = t0 + (NT == 2 ? slot * BQ : 0) + r / G;
-        const bool live = r < BQ * G && tok < p.nq;
-        const int last = live ? tok + shift : -1;  // last key the row sees
-        float m = -INFINITY, l = 0.f;
-        bool ok = true;
-#pragma unroll 1
-        for (int i = slot; i < steps; i += 2) {
-            const int k0 = (NT == 2 ? i >> 1 : i) * kPtKeys;
-            ok = __all_sync(0xffffffffu, wait(&s_full[slot], (i >> 1) & 1));
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t sv[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tc_ld32_nowait(ts + 32 * c, sv[c]);
-            tc_wait_ld();
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tc_reg_fence(sv[c]);
-            const int vis = last + 1 - k0;  // keys of the tile the row sees
-            if (!__all_sync(0xffffffffu, vis >= kPtKeys)) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (32 * c + j >= vis) sv[c][j] = 0xFF800000u;
-            }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int j = 0; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(sv[c][j]));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl2;
-            float alpha = 1.f;
-            bool grow = false;
-            if (m == -INFINITY) {
-                m = top;  // nothing summed so far: O and l are zero, or not yet written
-            } else if (top > m + kPtRescale) {
-                alpha = exp2_approx(m - top);
-                m = top;
-                grow = true;
-            }
-            if (__any_sync(0xffffffffu, grow)) {
-                // every earlier product of this slot completed before its scores did
-                l *= alpha;
-#pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[32];
-                    tc_ld32_nowait(to + 32 * c, o);
-                    tc_wait_ld();
-                    tc_reg_fence(o);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-                    tc_st32(to + 32 * c, o);
-                }
-            }
-            const float ms = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t pv[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float x = exp2_approx(fmaf(__uint_as_float(sv[2 * c + (j >> 4)][2 * (j & 15)]), a.sl2, -ms));
-                    const float y = exp2_approx(fmaf(__uint_as_float(sv[2 * c + (j >> 4)][2 * (j & 15) + 1]), a.sl2, -ms));
-                    sum[j & 1] += x;
-                    sum[2 + (j & 1)] += y;
-                    pv[j] = pack_pair<T>(x, y);
-                }
-                tc_st32(ts + 32 * c, pv);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&p_full[slot]);
-        }
-        const bool mine = steps > slot;  // the slot had a step
-        if (ok && mine) ok = __all_sync(0xffffffffu, wait(&o_final[slot], 0));
-        tc_fence_after();
-        // the row's output: O / l, plus what the cleared V rows would have added
-        float m_row = m, l_row = l, f_own = 1.f, f_other = 0.f;
-        constexpr int NC = NT == 2 ? D / 32 : D / 64;  // 32-column pieces this thread writes
-        const int c0 = NT == 2 ? 0 : slot * NC;
-        if constexpr (NT == 1) {
-            // the slots' halves of the key tiles, joined: each warpgroup hands the other half of
-            // its columns over through the ring (no copy or product uses it any more)
-            float2 *stat = reinterpret_cast<float2 *>(base);  // over Q: every product with it is complete
-            float *xch = reinterpret_cast<float *>(base + Ge::kOffRing) + slot * (D / 2) * kPtRows;
-            asm volatile("bar.sync 1, 256;" ::: "memory");  // both slots' products are complete
-            stat[slot * kPtRows + r] = make_float2(m, mine ? l : 0.f);
-            if (ok && mine) {
-#pragma unroll 1
-                for (int c = 0; c < NC; ++c) {
-                    uint32_t o[32];
-                    tc_ld32_nowait(to + 32 * ((slot ^ 1) * NC + c), o);
-                    tc_wait_ld();
-                    tc_reg_fence(o);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) xch[(32 * c + j) * kPtRows + r] = __uint_as_float(o[j]);
-                }
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            const float2 other = stat[(slot ^ 1) * kPtRows + r];
-            m_row = fmaxf(m, other.x);
-            const float mm = m_row == -INFINITY ? 0.f : m_row;
-            f_own = mine ? exp2_approx(m - mm) : 0.f;
-            f_other = exp2_approx(other.x - mm);
-            l_row = (mine ? l * f_own : 0.f) + other.y * f_other;
-        }
-        const float inv = l_row != 0.f ? 1.0f / l_row : 0.f;  // a row that sees no key: zeros
-        if (ok) {
-            T *dst = static_cast<T *>(a.out) + (p.q0 + tok) * a.o_tok + (kvh * G + r % G) * a.o_head;
-            const bool any_bad = bad[4 * kMaskedTiles] != 0;
-            const float *got = reinterpret_cast<const float *>(base + Ge::kOffRing) + (slot ^ 1) * (D / 2) * kPtRows;
-            const bool other_has = NT == 1 && steps > (slot ^ 1);
-#pragma unroll 1
-            for (int c = 0; c < NC; ++c) {
-                uint32_t o[32];
-                if (mine) {
-                    tc_ld32_nowait(to + 32 * (c0 + c), o);
-                    tc_wait_ld();
-                    tc_reg_fence(o);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = 0;
-                }
-                float x[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    x[j] = __uint_as_float(o[j]);
-                    if (NT == 1) x[j] = x[j] * f_own + (other_has ? got[(32 * c + j) * kPtRows + r] * f_other : 0.f);
-                }
-                if (any_bad && live) {
-                    const T *q = static_cast<const T *>(a.q) + (p.q0 + tok) * a.q_tok + (kvh * G + r % G) * a.q_head;
-                    for (int w = 0; w < 4 * kMaskedTiles; ++w) {
-                        for (uint32_t mask = bad[w]; mask; mask &= mask - 1) {
-                            const int key = first_masked * kPtKeys + 32 * w + __ffs(static_cast<int>(mask)) - 1;
-                            if (key > last) continue;
-                            const T *kr = static_cast<const T *>(a.k) + (p.k0 + key) * a.k_tok + kvh * a.k_head;
-                            const T *vr = static_cast<const T *>(a.v) + (p.k0 + key) * a.v_tok + kvh * a.v_head;
-                            float s = 0.f;
-                            for (int d = 0; d < D; ++d) s = fmaf(to_f32<T>(q[d]), to_f32<T>(kr[d]), s);
-                            const float pr = exp2_approx(fmaf(s, a.sl2, -m_row));
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) x[j] = fmaf(pr, to_f32<T>(vr[32 * (c0 + c) + j]), x[j]);
+                    const uint32_t ts = col_s(slot) + lanes, to = col_o(slot) + lanes;
+                    float m = -INFINITY, l = 0.f;
+                    bool ok = true;
+        #pragma unroll 1
+                    for (int i = slot; i < steps; i += 2) {
+                        const int k0 = (NT == 2 ? i >> 1 : i) * kPtKeys;
+                        ok = __all_sync(0xffffffffu, wait(&s_full[slot], (i >> 1) & 1));
+                        if (!ok) break;
+                        tc_fence_after();
+                        uint32_t sv[4][32];
+        #pragma unroll
+                        for (int c = 0; c < 4; ++c) tc_ld32_nowait(ts + 32 * c, sv[c]);
+                        tc_wait_ld();
+        #pragma unroll
+                        for (int c = 0; c < 4; ++c) tc_reg_fence(sv[c]);
+                        const int vis = last + 1 - k0;  // keys of the tile the row sees
+                        if (!__all_sync(0xffffffffu, vis >= kPtKeys)) {
+        #pragma unroll
+                            for (int c = 0; c < 4; ++c)
+        #pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (32 * c + j >= vis) sv[c][j] = 0xFF800000u;
+                        }
+                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        #pragma unroll
+                        for (int c = 0; c < 4; ++c)
+        #pragma unroll
+                            for (int j = 0; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(sv[c][j]));
+                        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl2;
+                        float alpha = 1.f;
+                        bool grow = false;
+                        if (m == -INFINITY) {
+                            m = top;  // nothing summed so far: O and l are zero, or not yet written
+                        } else if (top > m + kPtRescale) {
+                            alpha = exp2_approx(m - top);
+                            m = top;
+                            grow = true;
+                        }
+                        if (__any_sync(0xffffffffu, grow)) {
+                            // every earlier product of this slot completed before its scores did
+                            l *= alpha;
+        #pragma unroll 1
+                            for (int c = 0; c < D / 32; ++c) {
+                                uint32_t o[32];
+                                tc_ld32_nowait(to + 32 * c, o);
+                                tc_wait_ld();
+                                tc_reg_fence(o);
+        #pragma unroll
+                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                                tc_st32(to + 32 * c, o);
+                            }
+                        }
+                        const float ms = m == -INFINITY ? 0.f : m;
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        #pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t pv[32];
+        #pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                const float x = exp2_approx(fmaf(__uint_as_float(sv[2 * c + (j >> 4)][2 * (j & 15)]), a.sl2, -ms));
+                                const float y = exp2_approx(fmaf(__uint_as_float(sv[2 * c + (j >> 4)][2 * (j & 15) + 1]), a.sl2, -ms));
+                                sum[j & 1] += x;
+                                sum[2 + (j & 1)] += y;
+                                pv[j] = pack_pair<T>(x, y);
+                            }
+                            tc_st32(ts + 32 * c, pv);
+                        }
+                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        tc_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(&p_full[slot]);
+                    }
+                    const bool mine = steps > slot;  // the slot had a step
+                    if (ok && mine) ok = __all_sync(0xffffffffu, wait(&o_final[slot], 0));
+                    tc_fence_after();
+                    // the row's output: O / l, plus what the cleared V rows would have added
+                    float m_row = m, l_row = l, f_own = 1.f, f_other = 0.f;
+                    constexpr int NC = NT == 2 ? D / 32 : D / 64;  // 32-column pieces this thread writes
+                    const int c0 = NT == 2 ? 0 : slot * NC;
+                    if constexpr (NT == 1) {
+                        // the slots' halves of the key tiles, joined: each warpgroup hands the other half of
+                        // its columns over through the ring (no copy or product uses it any more)
+                        float2 *stat = reinterpret_cast<float2 *>(base);  // over Q: every product with it is complete
+                        float *xch = reinterpret_cast<float *>(base + Ge::kOffRing) + slot * (D / 2) * kPtRows;
+                        asm volatile("bar.sync 1, 256;" ::: "memory");  // both slots' products are complete
+                        stat[slot * kPtRows + r] = make_float2(m, mine ? l : 0.f);
+                        if (ok && mine) {
+        #pragma unroll 1
+                            for (int c = 0; c < NC; ++c) {
+                                uint32_t o[32];
+                                tc_ld32_nowait(to + 32 * ((slot ^ 1) * NC + c), o);
+                                tc_wait_ld();
+                                tc_reg_fence(o);
+        #pragma unroll
+                                for (int j = 0; j < 32; ++j) xch[(32 * c + j) * kPtRows + r] = __uint_as_float(o[j]);
+                            }
+                        }
+                        asm volatile("bar.sync 1, 256;" ::: "memory");
+                        const float2 other = stat[(slot ^ 1) * kPtRows + r];
+                        m_row = fmaxf(m, other.x);
+                        const float mm = m_row == -INFINITY ? 0.f : m_row;
+                        f_own = mine ? exp2_approx(m - mm) : 0.f;
+                        f_other = exp2_approx(other.x - mm);
+                        l_row = (mine ? l * f_own : 0.f) + other.y * f_other;
+                    }
+                    const float inv = l_row != 0.f ? 1.0f / l_row : 0.f;  // a row that sees no key: zeros
+                    if (ok) {
+                        const bool any_bad = bad[4 * kMaskedTiles] != 0;
+                        const float *got = reinterpret_cast<const float *>(base + Ge::kOffRing) + (slot ^ 1) * (D / 2) * kPtRows;
+                        const bool other_has = NT == 1 && steps > (slot ^ 1);
+        #pragma unroll 1
+                        for (int c = 0; c < NC; ++c) {
+                            uint32_t o[32];
+                            if (mine) {
+                                tc_ld32_nowait(to + 32 * (c0 + c), o);
+                                tc_wait_ld();
+                                tc_reg_fence(o);
+                            } else {
+        #pragma unroll
+                                for (int j = 0; j < 32; ++j) o[j] = 0;
+                            }
+                            float x[32];
+        #pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                x[j] = __uint_as_float(o[j]);
+                                if (NT == 1) x[j] = x[j] * f_own + (other_has ? got[(32 * c + j) * kPtRows + r] * f_other : 0.f);
+                                x[j] *= inv;
+                            }
+                            if (any_bad && live) add_cleared(x, 32 * (c0 + c), m_row, inv);
+                            if (live) {
+        #pragma unroll
+                                for (int j = 0; j < 32; j += 8)
+                                    *reinterpret_cast<uint4 *>(dst + 32 * (c0 + c) + j) =
+                                        make_uint4(pack_pair<T>(x[j], x[j + 1]), pack_pair<T>(x[j + 2], x[j + 3]),
+                                                   pack_pair<T>(x[j + 4], x[j + 5]), pack_pair<T>(x[j + 6], x[j + 7]));
+                            }
                         }
                     }
-                }
-                if (live) {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-                        *reinterpret_cast<uint4 *>(dst + 32 * (c0 + c) + j) =
-                            make_uint4(pack_pair<T>(x[j] * inv, x[j + 1] * inv), pack_pair<T>(x[j + 2] * inv, x[j + 3] * inv),
-                                       pack_pair<T>(x[j + 4] * inv, x[j + 5] * inv), pack_pair<T>(x[j + 6] * inv, x[j + 7] * inv));
-                }
-            }
-        }
     }
     tc_fence_before();
     __syncthreads();
@@ -430,30 +731,50 @@ bool row_map(CUtensorMap *m, bool bf16, const void *base, int64_t D, int64_t hea
 
 template <typename T, int D, int NT>
 cudaError_t pt_launch(const PackedArgs &a, cudaStream_t st) {
-    constexpr bool bf16 = !__is_same(T, __half);
+    constexpr bool bf16 = __is_same(T, __nv_bfloat16), split = __is_same(T, float);
+    using Ge = PtGeometry<D, NT, split ? 2 : 1>;
     auto kern = packed_tc_kernel<T, D, NT>;
     cudaError_t e = once_per_device(reinterpret_cast<const void *>(kern), ATTR_SMEM, [&] {
-        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(PtGeometry<D, NT>::kSmem));
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ge::kSmem));
     });
     if (e != cudaSuccess) return e;
     const int BQ = kPtRows / a.G;
-    CUtensorMap mq, mk, mv;
-    if (!row_map(&mq, bf16, a.q, D, a.Hq, a.total_q, a.q_head, a.q_tok, a.G, BQ) ||
-        !row_map(&mk, bf16, a.k, D, a.Hkv, a.total_k, a.k_head, a.k_tok, 1, kPtKeys) ||
-        !row_map(&mv, bf16, a.v, D, a.Hkv, a.total_k, a.v_head, a.v_tok, 1, kPtKeys))
-        return cudaErrorNotSupported;
     const int64_t ctas = most_packed_tiles(a.n_seqs, a.total_q, 1, NT * BQ) * a.Hkv;
     if (ctas > INT32_MAX) return cudaErrorNotSupported;
-    return b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPtThreads), PtGeometry<D, NT>::kSmem, st, false, mq,
-                       mk, mv, a);
+    CUtensorMap mq = {}, mk, mv;
+    SplitView sp;
+    if constexpr (split) {
+        const int64_t plane = a.total_k * a.Hkv * D;
+        __half *planes = static_cast<__half *>(a.ws);
+        int32_t *exps = reinterpret_cast<int32_t *>(planes + 4 * plane);
+        sp.exps = exps;
+        sp.total_k = a.total_k;
+        const int64_t tiles = most_packed_tiles(a.n_seqs, a.total_k, 1, kPtKeys) * a.Hkv * 2;
+        if (tiles > INT32_MAX || 2 * a.total_k > INT32_MAX ||
+            !row_map(&mk, false, planes, D, a.Hkv, 2 * a.total_k, D, a.Hkv * D, 1, kPtKeys) ||
+            !row_map(&mv, false, planes + 2 * plane, D, a.Hkv, 2 * a.total_k, D, a.Hkv * D, 1, kPtKeys))
+            return cudaErrorNotSupported;
+        e = b200_launch(packed_split_kernel<D>, dim3(static_cast<unsigned>(tiles)), dim3(kSplitThreads), 0, st, false, a,
+                        planes, exps);
+        if (e != cudaSuccess) return e;
+    } else {
+        if (!row_map(&mq, bf16, a.q, D, a.Hq, a.total_q, a.q_head, a.q_tok, a.G, BQ) ||
+            !row_map(&mk, bf16, a.k, D, a.Hkv, a.total_k, a.k_head, a.k_tok, 1, kPtKeys) ||
+            !row_map(&mv, bf16, a.v, D, a.Hkv, a.total_k, a.v_head, a.v_tok, 1, kPtKeys))
+            return cudaErrorNotSupported;
+    }
+    return b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPtThreads<T>), Ge::kSmem, st, split, mq, mk, mv, a, sp);
 }
 
 template <typename T, int D>
 cudaError_t pt_by_tiles(const PackedArgs &a, cudaStream_t st) {
-    // two query tiles a CTA once such CTAs fill the SMs
-    const int64_t pairs = a.total_q * a.G / (2 * kPtRows) * a.Hkv;
-    return pairs >= device_sm_count() ? pt_launch<T, D, 2>(a, st) : pt_launch<T, D, 1>(a, st);
+    if constexpr (__is_same(T, float)) {
+        return pt_launch<T, D, 1>(a, st);
+    } else {
+        // two query tiles a CTA once such CTAs fill the SMs
+        const int64_t pairs = a.total_q * a.G / (2 * kPtRows) * a.Hkv;
+        return pairs >= device_sm_count() ? pt_launch<T, D, 2>(a, st) : pt_launch<T, D, 1>(a, st);
+    }
 }
 
 template <typename T>
@@ -463,13 +784,19 @@ cudaError_t pt_by_dim(const PackedArgs &a, cudaStream_t st) {
 
 }  // namespace
 
+size_t packed_tc_workspace(int64_t n_seqs, int64_t total_k, int64_t D, int64_t Hkv, int32_t dtype) {
+    if (dtype != B200_DTYPE_F32) return 0;
+    // hi and lo planes of K and V, and the tiles' exponents
+    return static_cast<size_t>(total_k * Hkv * D * 8 + (total_k / kPtKeys + n_seqs + 1) * Hkv * 8);
+}
+
 cudaError_t packed_tc_launch(const PackedArgs &a, cudaStream_t st) {
     if (a.total_k == 0 || a.G > kPtRows) return cudaErrorNotSupported;
     switch (a.dtype) {
         case B200_DTYPE_F16: return pt_by_dim<__half>(a, st);
         case B200_DTYPE_BF16: return pt_by_dim<__nv_bfloat16>(a, st);
     }
-    return cudaErrorNotSupported;
+    return pt_by_dim<float>(a, st);
 }
 
 }  // namespace b200
