@@ -67,6 +67,69 @@ B200_DEVICE int plane_k(int t) { return NT == 2 ? 2 * t : (t == 0 ? 0 : 2 * t - 
 template <int NT>
 B200_DEVICE int plane_v(int t, int n) { return NT == 2 ? 2 * t + 1 : t + min(t + 2, n); }
 
+// Matrix descriptors of 128-byte-swizzled tiles differ only in their low word (address and
+// leading byte offset): 64-byte rows of 8-row atoms 1024 bytes apart, version 1. Forming
+// the words for an instruction by 64-bit arithmetic costs the issuing thread ~130 cycles,
+// twice the product's own 64; a 32-bit add of a constant does not.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+B200_DEVICE uint32_t desc_low(uint32_t saddr, uint32_t lbo) { return ((saddr & 0x3FFFFu) >> 4) | ((lbo >> 4) << 16); }
+// The whole warp runs these, one elected lane issues: with the operands the same in every
+// lane, addresses stay in uniform registers (from one lane's branch each instruction moves
+// its own there first).
+B200_DEVICE uint32_t elect_lane() {
+    uint32_t e;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+    return e;
+}
+B200_DEVICE void mma_ss(uint32_t e, uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n .reg .pred p, e;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %6, 0;\n mov.b64 da, {%1, %5};\n"
+        " mov.b64 db, {%2, %5};\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}" ::"r"(d),
+        "r"(a_low), "r"(b_low), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(kDescHigh), "r"(e)
+        : "memory");
+}
+B200_DEVICE void mma_ts(uint32_t e, uint32_t d, uint32_t a, uint32_t b_low, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n .reg .pred p, e;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %6, 0;\n mov.b64 db, {%2, %5};\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}" ::"r"(d),
+        "r"(a), "r"(b_low), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(kDescHigh), "r"(e)
+        : "memory");
+}
+B200_DEVICE void commit_if(uint32_t e, uint64_t *bar) {
+    asm volatile(
+        "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
+        " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_addr(bar)),
+        "r"(e)
+        : "memory");
+}
+
+// Two F32 operations in one instruction.
+B200_DEVICE uint64_t pair_of(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+B200_DEVICE float2 of_pair(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+B200_DEVICE uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+B200_DEVICE uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+B200_DEVICE float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 template <typename T>
 B200_DEVICE uint32_t pack_pair(float x, float y) {
     if constexpr (__is_same(T, __half)) {
@@ -182,7 +245,8 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     uint64_t *empty = bars + S;       // [S] plane read by its last product
     uint64_t *q_full = bars + 2 * S;
     uint64_t *s_full = q_full + 1;    // [2] scores of the slot's step complete (and all earlier products)
-    uint64_t *p_full = s_full + 2;    // [2] P written, O rescaled
+    uint64_t *p_part = s_full + 2;    // [2] O rescaled and the first 96 keys' P written (F32: all of P)
+    uint64_t *p_full = p_part + 2;    // [2] all of P written
     uint64_t *o_final = p_full + 2;   // [2] the slot's last product complete (F32: each step's)
     uint64_t *v_ok = o_final + 2;     // [kMaskedTiles] the masked tile's V checked
     uint64_t *v_ask = v_ok + kMaskedTiles;  // [kMaskedTiles] its V landed: to be checked
@@ -192,7 +256,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(idle + 1);
     uint32_t *bad = reinterpret_cast<uint32_t *>(base + Ge::kOffBad);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int G = a.G, BQ = kPtRows / G, MT = NT * BQ;  // tokens of a query tile, of the CTA
     const int kvh = blockIdx.x % a.Hkv;
     const PackedTile p =
@@ -213,6 +277,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         mbar_init(q_full, SPLIT ? 256 : 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&s_full[s], 1);
+            mbar_init(&p_part[s], 128);
             mbar_init(&p_full[s], 128);
             mbar_init(&o_final[s], 1);
             mbar_init(&o_empty[s], 128);
@@ -234,7 +299,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     if (SPLIT) grid_wait();  // the split planes
     const auto col_s = [&](int slot) { return tmem + static_cast<uint32_t>(slot * kPtKeys); };
     const auto col_o = [&](int slot) { return tmem + 256u + static_cast<uint32_t>(slot * 128); };
@@ -307,27 +372,31 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             // copies still landing in this CTA's shared memory
             if (!SPLIT) wait_poll(q_full, 0, nullptr);
             for (int i = max(0, issued - S); i < issued; ++i) wait_poll(&full[i % S], (i / S) & 1, nullptr);
-        } else if (warp == 1 && lane == 0 && nt > 0) {
+        } else if (warp == 1 && nt > 0) {
             // ---- tensor cores
+            const uint32_t e = elect_lane();
+            const auto all = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
             const auto at = [&](int pl) { return sbase + Ge::kOffRing + (pl % S) * Ge::kTile; };
-            const auto landed = [&](int pl) { return wait(&full[pl % S], (pl / S) & 1); };
+            const auto landed = [&](int pl) { return all(&full[pl % S], (pl / S) & 1); };
             // S (+)= a plane of Q . a plane of K
             const auto scores = [&](int slot, uint32_t q, int pl, bool add) {
+                const uint32_t d = col_s(slot), qa = desc_low(q, 16), ka = desc_low(at(pl), 16);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk)
-                    tc_mma_f16(col_s(slot), desc_k_sw128(q + (kk >> 2) * Ge::kBox) + 2 * (kk & 3),
-                               desc_k_sw128(at(pl) + (kk >> 2) * Ge::kBox) + 2 * (kk & 3), kIdS, add || kk > 0 ? 1u : 0u);
+                for (int kk = 0; kk < D / 16; ++kk) {  // 16 columns: 32 bytes inside a 128-byte row
+                    const uint32_t off = ((kk >> 2) * Ge::kBox + 32 * (kk & 3)) >> 4;
+                    mma_ss(e, d, qa + off, ka + off, kIdS, add || kk > 0);
+                }
             };
             // O (+)= P . a plane of V. P lies over the scores: 16 keys in 8 columns; F32: each 32
             // columns hold hi, then lo of their 32 keys
-            const auto values = [&](int slot, bool lo, int pl, bool add) {
+            const auto values = [&](int slot, bool lo, int pl, int from, int to, bool add) {
+                const uint32_t d = col_o(slot), pa = col_s(slot) + (lo ? 16 : 0), va = desc_low(at(pl), Ge::kBox);
 #pragma unroll
-                for (int kk = 0; kk < kPtKeys / 16; ++kk) {
-                    const uint32_t c = SPLIT ? 32 * (kk >> 1) + 8 * (kk & 1) + (lo ? 16 : 0) : 8 * kk;
-                    tc_mma_f16_ts(col_o(slot), col_s(slot) + c, desc_mn_sw128(at(pl) + kk * 2048, Ge::kBox), kIdO,
-                                  add || kk > 0 ? 1u : 0u);
-                }
+                for (int kk = from; kk < to; ++kk)  // 16 keys: two 1024-byte atoms
+                    mma_ts(e, d, pa + (SPLIT ? 32 * (kk >> 1) + 8 * (kk & 1) : 8 * kk), va + kk * (2048 >> 4), kIdO,
+                           add || kk > 0);
             };
+            constexpr int KK = kPtKeys / 16, KH = 3 * KK / 4;  // products of a V tile; of P's first part
             const auto issue_s = [&](int i) {
                 const int slot = i & 1, pl = PL * plane_k<NT>(NT == 2 ? i >> 1 : i);
                 const uint32_t q = sbase + (NT == 2 ? slot : 0) * Ge::kTile;
@@ -335,43 +404,49 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                 tc_fence_after();
                 scores(slot, q, pl, false);
                 if (SPLIT) {  // the small products first: the sum loses least
-                    tc_commit(smem_addr(&empty[pl % S]));
+                    commit_if(e, &empty[pl % S]);
                     if (!landed(pl + 1)) return false;
                     tc_fence_after();
                     scores(slot, q + Ge::kTile, pl + 1, true);
                     scores(slot, q, pl + 1, true);
                 }
-                tc_commit(smem_addr(&s_full[slot]));
-                if (NT == 1 || slot == 1) tc_commit(smem_addr(&empty[(pl + PL - 1) % S]));
+                commit_if(e, &s_full[slot]);
+                if (NT == 1 || slot == 1) commit_if(e, &empty[(pl + PL - 1) % S]);
                 return true;
             };
-            bool ok = wait(q_full, 0);
+            bool ok = all(q_full, 0);
             for (int i = 0; i < min(2, steps) && ok; ++i) ok = issue_s(i);
             for (int i = 0; i < steps && ok; ++i) {
                 const int slot = i & 1, t = NT == 2 ? i >> 1 : i, pl = PL * plane_v<NT>(t, nt);
                 const bool check = t >= first_masked && (NT == 1 || slot == 0);
                 ok = landed(pl) && (!SPLIT || !check || landed(pl + 1));
                 if (!ok) break;
-                if (check) mbar_arrive(&v_ask[t - first_masked]);  // done while the softmax runs
-                ok = wait(&p_full[slot], (i >> 1) & 1) && (!check || wait(&v_ok[t - first_masked], 0)) &&
-                     (!SPLIT || i < 2 || wait(&o_empty[slot], ((i >> 1) - 1) & 1));
+                if (check && lane == 0) mbar_arrive(&v_ask[t - first_masked]);  // done while the softmax runs
+                ok = all(&p_part[slot], (i >> 1) & 1) && (!check || all(&v_ok[t - first_masked], 0)) &&
+                     (!SPLIT || i < 2 || all(&o_empty[slot], ((i >> 1) - 1) & 1));
                 if (!ok) break;
                 tc_fence_after();
-                values(slot, false, pl, !SPLIT && i >= 2);
                 if (SPLIT) {
-                    tc_commit(smem_addr(&empty[pl % S]));
+                    values(slot, false, pl, 0, KK, false);
+                    commit_if(e, &empty[pl % S]);
                     ok = landed(pl + 1);
                     if (!ok) break;
                     tc_fence_after();
-                    values(slot, true, pl + 1, true);
-                    values(slot, false, pl + 1, true);
+                    values(slot, true, pl + 1, 0, KK, true);
+                    values(slot, false, pl + 1, 0, KK, true);
+                } else {
+                    values(slot, false, pl, 0, KH, i >= 2);
+                    ok = all(&p_full[slot], (i >> 1) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    values(slot, false, pl, KH, KK, true);
                 }
-                if (NT == 1 || slot == 1) tc_commit(smem_addr(&empty[(pl + PL - 1) % S]));
-                if (SPLIT || i + 2 >= steps) tc_commit(smem_addr(&o_final[slot]));
+                if (NT == 1 || slot == 1) commit_if(e, &empty[(pl + PL - 1) % S]);
+                if (SPLIT || i + 2 >= steps) commit_if(e, &o_final[slot]);
                 if (i + 2 < steps) ok = issue_s(i + 2);
             }
             // no product may still use tensor memory or the ring when the CTA exits
-            tc_commit(smem_addr(idle));
+            commit_if(e, idle);
             wait_poll(idle, 0, nullptr);
         } else if (warp >= 2) {
             // ---- V check: rows of the masked tiles that hold Inf or NaN, cleared and noted
@@ -567,7 +642,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                             mbar_arrive(&st_full[slot]);
                             tc_wait_st();
                             tc_fence_before();
-                            mbar_arrive(&p_full[slot]);
+                            mbar_arrive(&p_part[slot]);
                         }
     } else {
         // ---- softmax
@@ -596,12 +671,13 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                                     if (32 * c + j >= vis) sv[c][j] = 0xFF800000u;
                         }
                         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        #pragma unroll
-                        for (int c = 0; c < 4; ++c)
-        #pragma unroll
-                            for (int j = 0; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(sv[c][j]));
-                        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl2;
-                        float alpha = 1.f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int j = 0; j < 32; j += 2)
+                    mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], __uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1]));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl2;
+            float alpha = 1.f;
                         bool grow = false;
                         if (m == -INFINITY) {
                             m = top;  // nothing summed so far: O and l are zero, or not yet written
@@ -625,26 +701,33 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                             }
                         }
                         const float ms = m == -INFINITY ? 0.f : m;
-                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t pv[32];
-        #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const float x = exp2_approx(fmaf(__uint_as_float(sv[2 * c + (j >> 4)][2 * (j & 15)]), a.sl2, -ms));
-                                const float y = exp2_approx(fmaf(__uint_as_float(sv[2 * c + (j >> 4)][2 * (j & 15) + 1]), a.sl2, -ms));
-                                sum[j & 1] += x;
-                                sum[2 + (j & 1)] += y;
-                                pv[j] = pack_pair<T>(x, y);
-                            }
-                            tc_st32(ts + 32 * c, pv);
-                        }
-                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                        tc_wait_st();
-                        tc_fence_before();
-                        mbar_arrive(&p_full[slot]);
-                    }
-                    const bool mine = steps > slot;  // the slot had a step
+            const uint64_t scale2 = pair_of(a.sl2, a.sl2), minus2 = pair_of(-ms, -ms);
+            uint64_t sum[2] = {pair_of(l, 0.f), pair_of(0.f, 0.f)};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t pv[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const uint64_t s2 = pair_of(__uint_as_float(sv[c][2 * j]), __uint_as_float(sv[c][2 * j + 1]));
+                    const float2 x = of_pair(fma_pair(s2, scale2, minus2));
+                    const float px = exp2_approx(x.x), py = exp2_approx(x.y);
+                    sum[j & 1] = add_pair(sum[j & 1], pair_of(px, py));
+                    pv[j] = pack_pair<T>(px, py);
+                }
+                tc_st16(ts + 16 * c, pv);
+                if (c == 2) {  // the tensor cores may start on the first 96 keys
+                    tc_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&p_part[slot]);
+                }
+            }
+            const float2 two = of_pair(add_pair(sum[0], sum[1]));
+            l = two.x + two.y;
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_full[slot]);
+        }
+        const bool mine = steps > slot;  // the slot had a step
                     if (ok && mine) ok = __all_sync(0xffffffffu, wait(&o_final[slot], 0));
                     tc_fence_after();
                     // the row's output: O / l, plus what the cleared V rows would have added
