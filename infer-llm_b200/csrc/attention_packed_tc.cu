@@ -38,6 +38,8 @@
 #include "tcgen05.cuh"
 #include "tma.cuh"
 
+#include <type_traits>
+
 namespace b200 {
 namespace {
 
@@ -46,6 +48,7 @@ template <typename T>
 constexpr int kPtThreads = __is_same(T, float) ? 512 : 384;
 constexpr int kMaskedTiles = 4;  // key tiles in which some row of a CTA hides keys (at most 256 tokens)
 constexpr float kPtRescale = 8.0f;
+constexpr int kPolyStep = 4;  // 8192 BF16 keys: none 522 us, every 4th pair 504 to 513, every 2nd slower than none
 
 // PL: planes of an operand tile (2: hi and lo of F32)
 template <int D, int NT, int PL>
@@ -123,6 +126,32 @@ B200_DEVICE uint64_t add_pair(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+// 2^x of two values in FP32 arithmetic, for x <= 8: 2^round(x) by the exponent field times a
+// least-maximum polynomial of the rest in [-1/2, 1/2]. x below -125 gives 2^-125, so tiles
+// that hide keys (x = -inf) do not use it. Degree 3 is within 7.5e-5 (BF16 rounds P to
+// 2^-9), degree 4 within 2.6e-6 (F16 to 2^-12).
+template <bool BF16>
+B200_DEVICE float2 exp2_poly_pair(float2 x) {
+    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to whole numbers
+    const auto both = [](float v) { return pair_of(v, v); };
+    const uint64_t c = pair_of(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
+    const uint64_t t = add_pair(c, both(kMagic));
+    const uint64_t f = fma_pair(add_pair(t, both(-kMagic)), both(-1.0f), c);
+    uint64_t p;
+    if constexpr (BF16) {
+        p = fma_pair(f, both(0.0551716648f), both(0.242611125f));
+        p = fma_pair(p, f, both(0.693260968f));
+        p = fma_pair(p, f, both(0.999928057f));
+    } else {
+        p = fma_pair(f, both(0.00957010128f), both(0.0559178591f));
+        p = fma_pair(p, f, both(0.240247443f));
+        p = fma_pair(p, f, both(0.693121791f));
+        p = fma_pair(p, f, both(0.999999285f));
+    }
+    const float2 tf = of_pair(t), pf = of_pair(p);
+    return make_float2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(tf.x) << 23)),
+                       __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(tf.y) << 23)));
 }
 B200_DEVICE float max3(float a, float b, float c) {
     float r;
@@ -663,20 +692,23 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         #pragma unroll
                         for (int c = 0; c < 4; ++c) tc_reg_fence(sv[c]);
                         const int vis = last + 1 - k0;  // keys of the tile the row sees
-                        if (!__all_sync(0xffffffffu, vis >= kPtKeys)) {
+                        const bool whole = __all_sync(0xffffffffu, vis >= kPtKeys);
+            if (!whole) {
         #pragma unroll
                             for (int c = 0; c < 4; ++c)
         #pragma unroll
                                 for (int j = 0; j < 32; ++j)
                                     if (32 * c + j >= vis) sv[c][j] = 0xFF800000u;
                         }
-                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        float mx[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mx[j] = fmaxf(__uint_as_float(sv[0][2 * j]), __uint_as_float(sv[0][2 * j + 1]));
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
-                for (int j = 0; j < 32; j += 2)
-                    mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], __uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1]));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl2;
+                for (int j = c == 0 ? 16 : 0; j < 32; j += 2)
+                    mx[(j >> 1) & 7] = max3(mx[(j >> 1) & 7], __uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1]));
+            const float top = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * a.sl2;
             float alpha = 1.f;
                         bool grow = false;
                         if (m == -INFINITY) {
@@ -702,26 +734,34 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                         }
                         const float ms = m == -INFINITY ? 0.f : m;
             const uint64_t scale2 = pair_of(a.sl2, a.sl2), minus2 = pair_of(-ms, -ms);
-            uint64_t sum[2] = {pair_of(l, 0.f), pair_of(0.f, 0.f)};
+            uint64_t sum[4] = {pair_of(l, 0.f), 0, 0, 0};
+            // every kPolyStep-th pair by polynomial: the special-function unit takes 8 cycles a warp
+            // instruction and does not overlap much with the rest of one warp's work
+            const auto weigh = [&](auto poly) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t pv[16];
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t pv[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const uint64_t s2 = pair_of(__uint_as_float(sv[c][2 * j]), __uint_as_float(sv[c][2 * j + 1]));
-                    const float2 x = of_pair(fma_pair(s2, scale2, minus2));
-                    const float px = exp2_approx(x.x), py = exp2_approx(x.y);
-                    sum[j & 1] = add_pair(sum[j & 1], pair_of(px, py));
-                    pv[j] = pack_pair<T>(px, py);
+                    for (int j = 0; j < 16; ++j) {
+                        const uint64_t s2 = pair_of(__uint_as_float(sv[c][2 * j]), __uint_as_float(sv[c][2 * j + 1]));
+                        const float2 x = of_pair(fma_pair(s2, scale2, minus2));
+                        const float2 y = decltype(poly)::value && j % kPolyStep == kPolyStep - 1
+                                             ? exp2_poly_pair<kBf16>(x)
+                                             : make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                        sum[j & 3] = add_pair(sum[j & 3], pair_of(y.x, y.y));
+                        pv[j] = pack_pair<T>(y.x, y.y);
+                    }
+                    tc_st16(ts + 16 * c, pv);
+                    if (c == 2) {  // the tensor cores may start on the first 96 keys
+                        tc_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(&p_part[slot]);
+                    }
                 }
-                tc_st16(ts + 16 * c, pv);
-                if (c == 2) {  // the tensor cores may start on the first 96 keys
-                    tc_wait_st();
-                    tc_fence_before();
-                    mbar_arrive(&p_part[slot]);
-                }
-            }
-            const float2 two = of_pair(add_pair(sum[0], sum[1]));
+            };
+            if (whole) weigh(std::true_type{});
+            else weigh(std::false_type{});
+            const float2 two = of_pair(add_pair(add_pair(sum[0], sum[1]), add_pair(sum[2], sum[3])));
             l = two.x + two.y;
             tc_wait_st();
             tc_fence_before();
