@@ -10,14 +10,18 @@
 //  * A row belongs to one cluster of C CTAs, each with a contiguous chunk of the vocabulary
 //    kept in its shared memory, so the logits are read from HBM once. The CTAs exchange
 //    maxima, histograms and sums through distributed shared memory; no workspace.
-//  * Threshold: one histogram (count and weight) of the chunk over bins of equal width in
-//    (x - max) / T, merged over the cluster, gives the bin in which the k-th token, or the
-//    token that completes the nucleus, lies. Tokens below e^-28 of the likeliest have weight
-//    0 and are left out everywhere. The bin's tokens (at most kList, else the bin is split
-//    again over its ordered bit patterns) are gathered and ranked by comparison.
-//  * Draw: every warp sums the kept weights of its contiguous piece; a scan over the pieces
-//    names the one in which the drawn sum lies, and its warp walks it.
-// Bound: one read of the logits for a large batch; for a few rows the chain of about six
+//  * A histogram over bins of equal width in (x - max) / T, merged over the cluster, gives the bin
+//    in which the k-th token, or the token that completes the nucleus, lies. A weight is added as
+//    three words of 14 bits: 32-bit shared-memory additions run at full rate, 64-bit ones
+//    are compare-and-swap loops (16 us a row). Tokens below e^-28 of the likeliest have
+//    weight 0 and are left out everywhere.
+//  * If the bins up to it hold at most kList tokens, as for a head of a few hundred, the first
+//    CTA gathers them, ranks them by comparison and draws among them.
+//  * Otherwise the threshold is looked for in its bin alone: its tokens are ranked, or the bin is
+//    split again over its ordered bit patterns. Then the kept weight of each warp's
+//    contiguous piece is summed, and the CTA in whose chunk the drawn sum lies searches
+//    that piece.
+// Bound: one read of the logits for a large batch; for a few rows the chain of about four
 // cluster exchanges.
 #include "batch.cuh"
 #include "gemv.cuh"
@@ -46,25 +50,24 @@ struct SampleArgs {
 // Shared memory read by the other CTAs of the cluster, and this CTA's own.
 struct SampleShared {
     // exchanged
-    uint32_t cnt[kBins];
-    unsigned long long wgt[kBins];
-    uint32_t list[kList];
-    unsigned long long piece_w[kSmWarps];  // kept weight above K, a warp's piece
-    uint32_t piece_eq[kSmWarps];           // tokens equal to K
+    uint32_t cnt[kBins], wgt[3][kBins];  // tokens; their weights in words of 14 bits
+    uint32_t list[kList], list_at[kList];
+    unsigned long long part;     // kept weight above K
+    uint32_t equal;              // tokens equal to K
     float top;
     uint32_t listed, bad;
     // own
-    uint32_t mcnt[kBins], lcnt[kBins];     // merged: first histogram, later ones
-    unsigned long long mwgt[kBins], lwgt[kBins];
-    uint32_t akey[kList];
-    unsigned long long awgt[kList];
-    uint32_t warp_c[kSmWarps];
-    unsigned long long warp_w[kSmWarps];
+    uint32_t mcnt[kBins];             // the first histogram, merged
+    unsigned long long mwgt[kBins];
+    unsigned long long sorted[kList], awgt[kList];
+    uint32_t aat[kList];
+    uint32_t warp_c[kSmWarps], piece_eq[kSmWarps];
+    unsigned long long warp_w[kSmWarps], piece_w[kSmWarps];
     float warp_f[kSmWarps];
     uint32_t warp_b[kSmWarps];
     int32_t bin;
     uint32_t bin_c, key, ties;
-    unsigned long long above_c, above_w, sum;
+    unsigned long long above_c, above_w, upto_c, sum;
 };
 
 B200_DEVICE uint32_t ld_dsmem_u32(uint32_t addr) {
@@ -95,11 +98,18 @@ B200_DEVICE float key_value(uint32_t k) {
 struct Scale {
     float top, inv_t;
     B200_DEVICE float z(float x) const { return (x - top) * inv_t; }
+    // floor(2^40 e^z) from the bits of the exponential, which is at most 1 (a conversion to 64
+    // bits runs at a fraction of the rate of the shifts)
     B200_DEVICE unsigned long long weight(float x) const {
         const float y = z(x);
-        return y > kFloor ? __float2ull_rz(expf(y) * 1099511627776.0f) : 0ull;
+        if (!(y > kFloor)) return 0ull;
+        const uint32_t e = __float_as_uint(expf(y));
+        return (static_cast<unsigned long long>((e & 0x7FFFFFu) | 0x800000u) << 17) >> (127u - (e >> 23));
     }
-    B200_DEVICE int bin(float zz) const { return min(static_cast<int>(zz * (-kBins / -kFloor)), kBins - 1); }
+    // the bin nearest to kBins z / kFloor (adding 2^23 leaves the whole number in the low bits)
+    B200_DEVICE static int bin(float zz) {
+        return min(static_cast<int>(__float_as_uint(fmaf(zz, kBins / kFloor, 8388608.0f)) & 0x3FFu), kBins - 1);
+    }
 };
 
 template <typename T, bool HELD>
@@ -109,6 +119,24 @@ struct Chunk {
     B200_DEVICE float operator[](int i) const {
         if constexpr (HELD) return to_f32<T>(held[i]) + 0.0f;
         else return to_f32<T>(__ldg(held + i)) + 0.0f;
+    }
+    // fn(value, index) for the tokens [from + 4 lane, ...) below `to` of `lanes` lanes that take
+    // four consecutive ones at a time; `from` is a multiple of four
+    template <typename F>
+    B200_DEVICE void each(int from, int to, int lane, int lanes, F fn) const {
+        if constexpr (HELD) {
+            const int whole = from + ((to - from) & ~3);
+            for (int i = from + 4 * lane; i < whole; i += 4 * lanes) {
+                alignas(16) T v[4];
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(held + i);
+                else *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(held + i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) fn(to_f32<T>(v[j]) + 0.0f, i + j);
+            }
+            if (whole + lane < to) fn((*this)[whole + lane], whole + lane);
+        } else {
+            for (int i = from + lane; i < to; i += lanes) fn((*this)[i], i);
+        }
     }
 };
 
@@ -121,25 +149,67 @@ struct Sampler {
     int tid, warp, lane;
     uint32_t rank, nc;
 
-    // Merges the cluster's histograms into mc / mw (bin `tid` by each thread). The caller
-    // has passed a cluster barrier since they were filled.
-    B200_DEVICE void merge(uint32_t *mc, unsigned long long *mw) {
-        uint32_t c = 0;
-        unsigned long long w = 0;
-        for (uint32_t r = 0; r < nc; ++r) {
-            c += ld_dsmem_u32(dsmem_addr(&s.cnt[tid], r));
-            w += ld_dsmem_u64(dsmem_addr(&s.wgt[tid], r));
+    // Sum of v over the CTA, in every thread. Ends with a barrier.
+    B200_DEVICE unsigned long long cta_sum(unsigned long long v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0) s.warp_w[warp] = v;
+        __syncthreads();
+        unsigned long long t = 0;
+#pragma unroll
+        for (int w = 0; w < kSmWarps; ++w) t += s.warp_w[w];
+        __syncthreads();
+        return t;
+    }
+    // Sum of v over the threads before this one.
+    B200_DEVICE unsigned long long cta_before(unsigned long long v) {
+        unsigned long long incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
         }
-        mc[tid] = c;
-        mw[tid] = w;
+        if (lane == 31) s.warp_w[warp] = incl;
+        __syncthreads();
+        unsigned long long t = incl - v;
+        for (int w = 0; w < warp; ++w) t += s.warp_w[w];
+        __syncthreads();
+        return t;
+    }
+    // Bin `tid` of the cluster's histograms. The caller has passed a cluster barrier since they
+    // were filled.
+    B200_DEVICE uint32_t merged_count() const {
+        uint32_t c = 0;
+        for (uint32_t r = 0; r < nc; ++r) c += ld_dsmem_u32(dsmem_addr(&s.cnt[tid], r));
+        return c;
+    }
+    B200_DEVICE unsigned long long merged_weight() const {
+        unsigned long long w = 0;
+        for (uint32_t r = 0; r < nc; ++r)
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                w += static_cast<unsigned long long>(ld_dsmem_u32(dsmem_addr(&s.wgt[i][tid], r))) << (14 * i);
+        return w;
+    }
+    B200_DEVICE void clear_histogram() {
+        s.cnt[tid] = 0;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) s.wgt[i][tid] = 0;
+        __syncthreads();
+    }
+    B200_DEVICE void count(int b) { atomicAdd(&s.cnt[b], 1u); }
+    B200_DEVICE void add_weight(int b, unsigned long long w) {
+        // a chunk has at most 2^18 tokens: no word overflows
+        if (w & 0x3FFFu) atomicAdd(&s.wgt[0][b], static_cast<uint32_t>(w) & 0x3FFFu);
+        atomicAdd(&s.wgt[1][b], static_cast<uint32_t>(w >> 14) & 0x3FFFu);
+        if (w >> 28) atomicAdd(&s.wgt[2][b], static_cast<uint32_t>(w >> 28));
     }
 
-    // The bin in which the running measure (count or weight) reaches `target`, given what
-    // lies above the bins; s.bin = -1 if it does not. Leaves s.above_*, s.bin_c.
-    B200_DEVICE void find(const uint32_t *mc, const unsigned long long *mw, unsigned long long above_c,
-                          unsigned long long above_w, unsigned long long target, bool by_weight) {
-        const uint32_t c = mc[tid];
-        const unsigned long long w = mw[tid];
+    // The bin at which the running count or weight of the bins (bin `tid` holds c tokens of
+    // weight w), on top of what is ahead of them, reaches `target`: s.bin (-1 if it does not),
+    // s.bin_c, s.above_c and s.above_w (ahead of the bin), s.upto_c (tokens up to it).
+    B200_DEVICE void find(uint32_t c, unsigned long long w, unsigned long long ahead_c, unsigned long long ahead_w,
+                          unsigned long long target, bool by_weight) {
         uint32_t ic = c;
         unsigned long long iw = w;
 #pragma unroll
@@ -151,58 +221,113 @@ struct Sampler {
         if (lane == 31) s.warp_c[warp] = ic, s.warp_w[warp] = iw;
         if (tid == 0) s.bin = -1;
         __syncthreads();
-        unsigned long long pc = above_c, pw = above_w;
+        unsigned long long pc = ahead_c + (ic - c), pw = ahead_w + (iw - w);
         for (int i = 0; i < warp; ++i) pc += s.warp_c[i], pw += s.warp_w[i];
-        pc += ic - c;
-        pw += iw - w;
         const unsigned long long lo = by_weight ? pw : pc, hi = by_weight ? pw + w : pc + c;
         if (lo < target && target <= hi) {
             s.bin = tid;
             s.bin_c = c;
             s.above_c = pc;
             s.above_w = pw;
+            s.upto_c = pc + c;
         }
         __syncthreads();
     }
 
-    B200_DEVICE void clear_histogram() {
-        s.cnt[tid] = 0;
-        s.wgt[tid] = 0;
+    // Appends the tokens that `member(value, key)` names to this CTA's list.
+    template <typename F>
+    B200_DEVICE void collect(F member) {
+        if (tid == 0) s.listed = 0;
         __syncthreads();
+        x.each(0, x.n, tid, kSmThreads, [&](float v, int i) {
+            const uint32_t key = order_key(v);
+            if (member(v, key)) {
+                const uint32_t at = atomicAdd(&s.listed, 1u);
+                s.list[at] = key;
+                s.list_at[at] = static_cast<uint32_t>(i);
+            }
+        });
+    }
+    // Token `tid` of the cluster's lists, the CTAs' lists in order: its key and index in the
+    // vocabulary; returns the lists' length. The caller has passed a cluster barrier since they
+    // were filled.
+    B200_DEVICE uint32_t fetch_listed(uint32_t &key, uint32_t &at) {
+        uint32_t m[kMaxCluster], n = 0, from = 0, r = 0, base = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kMaxCluster; ++i) m[i] = i < nc ? ld_dsmem_u32(dsmem_addr(&s.listed, i)) : 0u;
+#pragma unroll
+        for (uint32_t i = 0; i < kMaxCluster; ++i) {
+            if (static_cast<uint32_t>(tid) >= n && static_cast<uint32_t>(tid) < n + m[i]) r = i, from = tid - n, base = i * a.chunk;
+            n += m[i];
+        }
+        key = at = 0;
+        if (static_cast<uint32_t>(tid) < n) {
+            key = ld_dsmem_u32(dsmem_addr(&s.list[from], r));
+            at = ld_dsmem_u32(dsmem_addr(&s.list_at[from], r)) + base;
+        }
+        return n;
     }
 
-    // Finds K and r for `target` (a count of tokens, or a sum of weights) from the merged
-    // first histogram: s.key, s.ties, and s.sum, the weight of the head they describe.
-    // Every CTA of the cluster takes the same path. False: the whole row is kept.
-    B200_DEVICE bool select(unsigned long long target, bool by_weight) {
-        find(s.mcnt, s.mwgt, 0, 0, target, by_weight);
+    // Sorts the first n threads' values, descending; the others' are 0 (bitonic; exchanges
+    // within a warp by shuffles, across warps through s.sorted).
+    B200_DEVICE unsigned long long sort_descending(unsigned long long v, uint32_t n) {
+        const int size = n <= 32 ? 32 : 1 << (32 - __clz(static_cast<int>(n - 1)));
+#pragma unroll 1
+        for (int k = 2; k <= size; k <<= 1) {
+#pragma unroll 1
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                unsigned long long o = 0;
+                if (j >= 32) {
+                    __syncthreads();
+                    s.sorted[tid] = v;
+                    __syncthreads();
+                    o = s.sorted[tid ^ j];
+                } else if (tid < size) {
+                    o = __shfl_xor_sync(0xffffffffu, v, j);
+                }
+                const bool larger = ((tid & j) == 0) == ((tid & k) == 0);  // this thread keeps the larger one
+                if (tid < size) v = (v > o) == larger ? v : o;
+            }
+        }
+        return v;
+    }
+
+    // Finds K and r (s.key, s.ties) for the head of `target` tokens, or of weight `target`,
+    // and s.sum, the head's weight, from the merged first histogram (`weights`: which has the
+    // weights too). False: the whole row is kept. Every CTA takes the same path.
+    B200_DEVICE bool select(unsigned long long target, bool by_weight, bool weights) {
+        find(s.mcnt[tid], s.mwgt[tid], 0, 0, target, by_weight);
         const int bin0 = s.bin;
         if (bin0 < 0) return false;
-        uint32_t lo = 0, hi = order_key(sc.top);
-        uint32_t n = s.bin_c;
+        uint32_t lo = 0, hi = order_key(sc.top), n = s.bin_c;
         unsigned long long ac = s.above_c, aw = s.above_w;
         const auto member = [&](float v, uint32_t key) {
             const float z = sc.z(v);
             return z > kFloor && sc.bin(z) == bin0 && key >= lo && key <= hi;
         };
+        if (n > kList) {
+            // the bin's values lie in an interval a little wider than its edges
+            const float width = -kFloor / kBins / sc.inv_t;
+            const float slack = 0.25f * width + 1e-5f * (fabsf(sc.top) + width * kBins);
+            const float x_hi = sc.top - width * (bin0 - 0.5f) + slack, x_lo = sc.top - width * (bin0 + 0.5f) - slack;
+            if (x_hi < sc.top) hi = order_key(x_hi);
+            if (x_lo > -INFINITY && x_lo < sc.top && bin0 < kBins - 1) lo = order_key(x_lo);
+        }
         while (n > kList && lo < hi) {  // split the bin over its bit patterns, descending
             const int shift = max(0, 32 - __clz(static_cast<int>(hi - lo)) - 9);
             cluster_sync();  // nobody reads the histogram any more
             clear_histogram();
-            for (int i = tid; i < x.n; i += kSmThreads) {
-                const float v = x[i];
+            x.each(0, x.n, tid, kSmThreads, [&](float v, int) {
                 const uint32_t key = order_key(v);
                 if (member(v, key)) {
-                    atomicAdd(&s.cnt[(hi - key) >> shift], 1u);
-                    atomicAdd(&s.wgt[(hi - key) >> shift], sc.weight(v));
+                    const int b = static_cast<int>((hi - key) >> shift);
+                    count(b);
+                    if (weights) add_weight(b, sc.weight(v));
                 }
-            }
+            });
             cluster_sync();
-            merge(s.lcnt, s.lwgt);
-            __syncthreads();
-            find(s.lcnt, s.lwgt, ac, aw, target, by_weight);
-            const uint32_t off = static_cast<uint32_t>(s.bin) << shift;
-            hi -= off;
+            find(merged_count(), weights ? merged_weight() : 0ull, ac, aw, target, by_weight);
+            hi -= static_cast<uint32_t>(s.bin) << shift;
             const uint32_t width = (1u << shift) - 1u;
             lo = hi - lo > width ? hi - width : lo;
             n = s.bin_c;
@@ -210,51 +335,77 @@ struct Sampler {
             aw = s.above_w;
             __syncthreads();
         }
+        uint32_t key = lo, at;
+        unsigned long long each = sc.weight(key_value(lo));
         if (n > kList) {  // one bit pattern is left
-            if (tid == 0) settle(lo, ac, aw, target, by_weight);
+            const unsigned long long r = by_weight ? (target - aw + each - 1) / each : target - ac;
+            if (tid == 0) s.key = lo, s.ties = static_cast<uint32_t>(r), s.sum = aw + r * each;
             __syncthreads();
             return true;
         }
-        if (tid == 0) s.listed = 0;
-        __syncthreads();
-        for (int i = tid; i < x.n; i += kSmThreads) {
-            const float v = x[i];
-            const uint32_t key = order_key(v);
-            if (member(v, key)) s.list[atomicAdd(&s.listed, 1u)] = key;
-        }
+        collect(member);
         cluster_sync();
-        uint32_t base = 0;
-        for (uint32_t r = 0; r < nc; ++r) {
-            const uint32_t m = ld_dsmem_u32(dsmem_addr(&s.listed, r));
-            if (tid < static_cast<int>(m)) s.akey[base + tid] = ld_dsmem_u32(dsmem_addr(&s.list[tid], r));
-            base += m;
-        }
+        fetch_listed(key, at);
         cluster_sync();  // the lists may be written again
-        if (tid < static_cast<int>(n)) s.awgt[tid] = sc.weight(key_value(s.akey[tid]));
+        // in order, the token at which the measure reaches the target
+        const bool have = tid < static_cast<int>(n);
+        const unsigned long long v =
+            sort_descending(have ? static_cast<unsigned long long>(key) << 32 | (0xFFFFFFFFu - at) : 0ull, n);
+        key = static_cast<uint32_t>(v >> 32);
+        each = have ? sc.weight(key_value(key)) : 0ull;
+        const unsigned long long before = aw + cta_before(each);
+        s.sorted[tid] = v;
         __syncthreads();
-        if (tid < static_cast<int>(n)) {
-            const uint32_t mine = s.akey[tid];
-            unsigned long long c = ac, w = aw, eq = 0;
-            for (uint32_t j = 0; j < n; ++j) {
-                const uint32_t k = s.akey[j];
-                if (k > mine) c += 1, w += s.awgt[j];
-                eq += k == mine;
-            }
-            const unsigned long long below = by_weight ? w : c;
-            if (below < target && target <= below + (by_weight ? eq * s.awgt[tid] : eq))
-                settle(mine, c, w, target, by_weight);  // equal tokens write the same values
+        if (have && (by_weight ? before < target && target <= before + each : ac + tid + 1 == target)) {
+            int first = tid;  // of the run of equal tokens
+            while (first > 0 && static_cast<uint32_t>(s.sorted[first - 1] >> 32) == key) --first;
+            s.key = key;
+            s.ties = static_cast<uint32_t>(tid - first) + 1;
+            s.sum = before + each;
         }
         __syncthreads();
         return true;
     }
 
-    B200_DEVICE void settle(uint32_t key, unsigned long long c, unsigned long long w, unsigned long long target,
-                            bool by_weight) {
-        const unsigned long long each = sc.weight(key_value(key));
-        const unsigned long long r = by_weight ? (target - w + each - 1) / each : target - c;
-        s.key = key;
-        s.ties = static_cast<uint32_t>(r);
-        s.sum = w + r * each;
+    B200_DEVICE unsigned long long share_of(float p, unsigned long long sum) const {
+        const double want = static_cast<double>(p) * static_cast<double>(sum);
+        return want >= 1.0 ? static_cast<unsigned long long>(want) : 1ull;
+    }
+    B200_DEVICE static unsigned long long drawn(float u, unsigned long long total) {
+        const double want = static_cast<double>(u) * static_cast<double>(total);
+        unsigned long long at = want > 0.0 ? static_cast<unsigned long long>(want) : 0ull;
+        return want >= static_cast<double>(total) || at >= total ? total - 1 : at;
+    }
+
+    // The whole draw among the listed tokens, which hold the kept head (first CTA).
+    B200_DEVICE void draw_listed(int32_t top_k, float top_p, unsigned long long row_sum, unsigned long long least, float u,
+                                 int32_t *out) {
+        uint32_t key, at;
+        const uint32_t n = fetch_listed(key, at);
+        const unsigned long long v = sort_descending(
+            static_cast<uint32_t>(tid) < n ? static_cast<unsigned long long>(key) << 32 | (0xFFFFFFFFu - at) : 0ull, n);
+        const uint32_t head = top_k > 0 ? min(n, static_cast<uint32_t>(top_k)) : n;
+        bool keep = static_cast<uint32_t>(tid) < head;
+        at = 0xFFFFFFFFu - static_cast<uint32_t>(v);
+        const unsigned long long w = keep ? sc.weight(key_value(static_cast<uint32_t>(v >> 32))) : 0ull;
+        if (top_p < 1.0f) {
+            const unsigned long long sum = top_k > 0 ? cta_sum(w) : row_sum;
+            const unsigned long long before = cta_before(w);
+            keep = keep && (tid == 0 || before < share_of(top_p, sum));
+        }
+        keep = keep && w >= least;
+        // the kept tokens by index: each sums the kept weight at smaller indices
+        s.aat[tid] = keep ? at : 0xFFFFFFFFu;
+        s.awgt[tid] = keep ? w : 0ull;
+        const unsigned long long total = cta_sum(keep ? w : 0ull);
+        const unsigned long long goal = drawn(u, total);
+        if (__any_sync(0xffffffffu, keep)) {
+            unsigned long long ahead = 0;
+#pragma unroll 4
+            for (uint32_t j = 0; j < head; ++j)
+                if (s.aat[j] < at) ahead += s.awgt[j];
+            if (keep && ahead <= goal && goal < ahead + w) *out = static_cast<int32_t>(at);
+        }
     }
 };
 
@@ -271,6 +422,11 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
     const T *src = static_cast<const T *>(a.logits) + row * a.row_stride + begin;
 
     // the chunk, its maximum, and whether it has a NaN or +inf
+    const float temp = __ldg(a.temperature + row);
+    const float u = __ldg(a.u + row);
+    const int32_t top_k = a.top_k ? __ldg(a.top_k + row) : 0;
+    const float top_p = a.top_p ? __ldg(a.top_p + row) : 1.0f;
+    const float min_p = a.min_p ? __ldg(a.min_p + row) : 0.0f;
     float mx = -INFINITY;
     bool bad = false;
     const auto take = [&](T v) {
@@ -300,17 +456,13 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
         if constexpr (HELD) held[i] = v;
         take(v);
     }
-    const float temp = __ldg(a.temperature + row);
-    const float u = __ldg(a.u + row);
-    const int32_t top_k = a.top_k ? __ldg(a.top_k + row) : 0;
-    const float top_p = a.top_p ? __ldg(a.top_p + row) : 1.0f;
-    const float min_p = a.min_p ? __ldg(a.min_p + row) : 0.0f;
     bad |= temp != temp || u != u || top_p != top_p || min_p != min_p;
     mx = warp_max(mx);
     bad = __any_sync(0xffffffffu, bad);
     if (lane == 0) s.warp_f[warp] = mx, s.warp_b[warp] = bad;
     s.cnt[tid] = 0;
-    s.wgt[tid] = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) s.wgt[i][tid] = 0;
     __syncthreads();
     if (warp == 0) {
         mx = warp_max(lane < kSmWarps ? s.warp_f[lane] : -INFINITY);
@@ -335,138 +487,155 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
     const float inv = 1.0f / temp;
     const bool cold = !(temp > 0.f) || inv == INFINITY;
     Sampler<T, HELD> f{a, s, {HELD ? held : src, n}, {mx + 0.0f, cold ? 1.0f : inv}, tid, warp, lane, rank, nc};
+    const bool by_k = !cold && top_k > 0 && top_k < a.vocab, by_p = !cold && top_p < 1.0f;
+    const double floor_p = static_cast<double>(fminf(fmaxf(min_p, 0.0f), 1.0f)) * 1099511627776.0;
+    const unsigned long long least = static_cast<unsigned long long>(floor_p);
 
     // the kept head: keys above `key`, and the first `ties` equal to it
     uint32_t key = 0, ties = 0;
     if (cold) {
         key = order_key(mx + 0.0f);
         ties = 1;
-    } else if (top_k > 0 && top_k < a.vocab || top_p < 1.0f) {
-        for (int i = tid; i < n; i += kSmThreads) {
-            const float v = f.x[i], z = f.sc.z(v);
-            if (z > kFloor) {
-                const int b = f.sc.bin(z);
-                atomicAdd(&s.cnt[b], 1u);
-                atomicAdd(&s.wgt[b], f.sc.weight(v));
-            }
+    } else if (by_k || by_p) {
+        // a short top-k is drawn from its list, without the bins' weights
+        bool weights = by_p && !(by_k && top_k <= kList / 2);
+        const auto fill = [&] {
+            f.x.each(0, n, tid, kSmThreads, [&](float v, int) {
+                const float z = f.sc.z(v);
+                if (z > kFloor) {
+                    const int b = f.sc.bin(z);
+                    f.count(b);
+                    if (weights) f.add_weight(b, f.sc.weight(v));
+                }
+            });
+            cluster_sync();
+            s.mcnt[tid] = f.merged_count();
+            s.mwgt[tid] = weights ? f.merged_weight() : 0ull;
+        };
+        fill();
+        unsigned long long sum = weights && !by_k ? f.cta_sum(s.mwgt[tid]) : 0ull;  // of the row
+        // the last bin that the head reaches into
+        if (by_k) f.find(s.mcnt[tid], s.mwgt[tid], 0, 0, static_cast<unsigned long long>(top_k), false);
+        else f.find(s.mcnt[tid], s.mwgt[tid], 0, 0, f.share_of(top_p, sum), true);
+        const int last = s.bin;
+        if (last >= 0 && s.upto_c <= kList) {
+            f.collect([&](float v, uint32_t) {
+                const float z = f.sc.z(v);
+                return z > kFloor && f.sc.bin(z) <= last;
+            });
+            cluster_sync();
+            if (rank == 0) f.draw_listed(by_k ? top_k : 0, top_p, sum, least, u, a.out + row);
+            cluster_sync();  // no CTA's shared memory goes away while it is read
+            return;
         }
-        cluster_sync();
-        f.merge(s.mcnt, s.mwgt);
+        if (by_p && !weights) {  // a short top-k among many equal tokens
+            weights = true;
+            cluster_sync();  // nobody reads the histogram any more
+            f.clear_histogram();
+            fill();
+        }
         __syncthreads();
-        unsigned long long sum = 0;
         bool cut = false;
-        if (top_k > 0) cut = f.select(static_cast<unsigned long long>(top_k), false);
-        if (cut) {
-            key = s.key, ties = s.ties, sum = s.sum;
-        } else {
-            for (int i = lane; i < kBins; i += 32) sum += s.mwgt[i];
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        }
+        if (by_k) cut = f.select(static_cast<unsigned long long>(top_k), false, weights);
+        if (cut) key = s.key, ties = s.ties, sum = s.sum;
         __syncthreads();
-        if (top_p < 1.0f) {
-            const double want = static_cast<double>(top_p) * static_cast<double>(sum);
-            const unsigned long long target = want >= 1.0 ? static_cast<unsigned long long>(want) : 1ull;
-            if (f.select(target, true)) key = s.key, ties = s.ties;
+        if (by_p) {
+            if (by_k && !cut) sum = f.cta_sum(s.mwgt[tid]);
+            if (f.select(f.share_of(top_p, sum), true, true)) key = s.key, ties = s.ties;
         }
     }
-    const double floor_p = static_cast<double>(fminf(fmaxf(min_p, 0.0f), 1.0f)) * 1099511627776.0;
-    const unsigned long long least = static_cast<unsigned long long>(floor_p);
 
     // kept weight of each warp's contiguous piece
-    const int piece = (a.chunk / kSmWarps + 31) / 32 * 32;
-    const int p0 = warp * piece, p1 = min(n, p0 + piece);
-    unsigned long long pw = 0;
-    uint32_t pe = 0;
-    for (int i = p0 + lane; i < p1; i += 32) {
-        const float v = f.x[i];
-        const uint32_t k = order_key(v);
-        if (k > key) {
-            const unsigned long long w = f.sc.weight(v);
-            if (w >= least) pw += w;
-        } else if (k == key) {
-            ++pe;
+    const int piece = (a.chunk / kSmWarps + 127) / 128 * 128;
+    {
+        const int p0 = min(n, warp * piece), p1 = min(n, p0 + piece);
+        unsigned long long pw = 0;
+        uint32_t pe = 0;
+        f.x.each(p0, p1, lane, 32, [&](float v, int) {
+            const uint32_t k = order_key(v);
+            if (k > key) {
+                const unsigned long long w = f.sc.weight(v);
+                if (w >= least) pw += w;
+            } else if (k == key) {
+                ++pe;
+            }
+        });
+        pe = __reduce_add_sync(0xffffffffu, pe);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) pw += __shfl_xor_sync(0xffffffffu, pw, o);
+        if (lane == 0) s.piece_w[warp] = pw, s.piece_eq[warp] = pe;
+        __syncthreads();
+        if (tid == 0) {
+            unsigned long long cw = 0;
+            uint32_t ce = 0;
+            for (int i = 0; i < kSmWarps; ++i) cw += s.piece_w[i], ce += s.piece_eq[i];
+            s.part = cw;
+            s.equal = ce;
         }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        pw += __shfl_xor_sync(0xffffffffu, pw, o);
-        pe += __shfl_xor_sync(0xffffffffu, pe, o);
-    }
-    if (lane == 0) s.piece_w[warp] = pw, s.piece_eq[warp] = pe;
     cluster_sync();
-    // every warp scans all pieces of the cluster (lane: pieces lane, lane + 32, ... in order)
     unsigned long long each = ties ? f.sc.weight(key_value(key)) : 0ull;
     if (each < least) each = 0;
-    const int pieces = static_cast<int>(nc) * kSmWarps;
-    unsigned long long total = 0, before = 0;  // before: kept weight ahead of this warp's piece
-    uint32_t eq_total = 0, eq_before = 0;
-    const int mine = static_cast<int>(rank) * kSmWarps + warp;
-    for (int i0 = 0; i0 < pieces; i0 += 32) {
-        const int i = i0 + lane;
-        unsigned long long w = 0;
-        uint32_t e = 0;
-        if (i < pieces) {
-            w = ld_dsmem_u64(dsmem_addr(&s.piece_w[i % kSmWarps], i / kSmWarps));
-            e = ld_dsmem_u32(dsmem_addr(&s.piece_eq[i % kSmWarps], i / kSmWarps));
-        }
-        uint32_t ie = e;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, ie, o);
-            if (lane >= o) ie += y;
-        }
-        const uint32_t eb = eq_total + ie - e;  // equal tokens ahead of piece i
-        const uint32_t kept = eb < ties ? min(e, ties - eb) : 0u;
-        unsigned long long iw = w + kept * each;
-        const unsigned long long own = iw;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long y = __shfl_up_sync(0xffffffffu, iw, o);
-            if (lane >= o) iw += y;
-        }
-        if (mine >= i0 && mine < i0 + 32) {
-            before = total + __shfl_sync(0xffffffffu, iw - own, mine - i0);
-            eq_before = __shfl_sync(0xffffffffu, eb, mine - i0);
-        }
-        total += __shfl_sync(0xffffffffu, iw, 31);
-        eq_total += __shfl_sync(0xffffffffu, ie, 31);
+    unsigned long long total = 0, before = 0;  // kept weight of the row; ahead of this chunk
+    uint32_t eq = 0, eq_before = 0;
+    for (uint32_t r = 0; r < nc; ++r) {
+        const uint32_t e = ld_dsmem_u32(dsmem_addr(&s.equal, r));
+        if (r == rank) before = total, eq_before = eq;
+        total += ld_dsmem_u64(dsmem_addr(&s.part, r)) + (eq < ties ? min(e, ties - eq) : 0u) * each;
+        eq += e;
     }
-    const double want = static_cast<double>(u) * static_cast<double>(total);
-    unsigned long long at = want > 0.0 ? static_cast<unsigned long long>(want) : 0ull;
-    if (want >= static_cast<double>(total) || at >= total) at = total - 1;
-    // the warp whose piece holds the drawn sum walks it
-    const uint32_t my_kept = eq_before < ties ? min(pe, ties - eq_before) : 0u;
-    if (at >= before && at < before + pw + my_kept * each) {
-        unsigned long long run = before;
-        uint32_t eq = eq_before;
-        for (int i0 = p0; i0 < p1; i0 += 32) {
-            const int i = i0 + lane;
-            unsigned long long w = 0;
-            bool same = false;
-            if (i < p1) {
-                const float v = f.x[i];
-                const uint32_t k = order_key(v);
-                same = k == key;
-                if (k > key) {
-                    w = f.sc.weight(v);
-                    if (w < least) w = 0;
-                }
-            }
-            const uint32_t sm = __ballot_sync(0xffffffffu, same);
-            if (same && eq + __popc(sm & ((1u << lane) - 1u)) < ties) w = each;
-            eq += __popc(sm);
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long y = __shfl_up_sync(0xffffffffu, w, o);
-                if (lane >= o) w += y;
-            }
-            const unsigned hit = __ballot_sync(0xffffffffu, run + w > at);
-            if (hit) {
-                if (lane == 0) a.out[row] = static_cast<int32_t>(begin + i0 + __ffs(hit) - 1);
+    const unsigned long long goal = f.drawn(u, total);
+    // the CTA in whose chunk the drawn sum lies: the piece, then the token
+    if (goal >= before) {
+        int p = -1;
+        unsigned long long at = before;
+        uint32_t ep = eq_before;
+        for (int i = 0; i < kSmWarps; ++i) {
+            const unsigned long long w = s.piece_w[i] + (ep < ties ? min(s.piece_eq[i], ties - ep) : 0u) * each;
+            if (goal < at + w) {
+                p = i;
                 break;
             }
-            run += __shfl_sync(0xffffffffu, w, 31);
+            at += w;
+            ep += s.piece_eq[i];
+        }
+        if (p >= 0) {  // the whole CTA: `per` consecutive tokens a thread
+            const int per = (piece + kSmThreads - 1) / kSmThreads;
+            const int i0 = min(n, min((p + 1) * piece, p * piece + tid * per));
+            const int i1 = min(n, min((p + 1) * piece, i0 + per));
+            unsigned long long w = 0, e = 0;
+            for (int i = i0; i < i1; ++i) {
+                const float v = f.x[i];
+                const uint32_t k = order_key(v);
+                if (k > key) {
+                    const unsigned long long x = f.sc.weight(v);
+                    if (x >= least) w += x;
+                }
+                e += k == key;
+            }
+            const unsigned long long eb = ep + f.cta_before(e);  // equal tokens ahead of this thread
+            unsigned long long kept = eb < ties ? (ties - eb < e ? ties - eb : e) : 0ull;
+            w += kept * each;
+            unsigned long long run = at + f.cta_before(w);
+            if (run <= goal && goal < run + w) {
+                for (int i = i0; i < i1; ++i) {
+                    const float v = f.x[i];
+                    const uint32_t k = order_key(v);
+                    unsigned long long x = 0;
+                    if (k > key) {
+                        x = f.sc.weight(v);
+                        if (x < least) x = 0;
+                    } else if (k == key && kept > 0) {
+                        x = each;
+                        --kept;
+                    }
+                    if (goal < run + x) {
+                        a.out[row] = static_cast<int32_t>(begin + i);
+                        break;
+                    }
+                    run += x;
+                }
+            }
         }
     }
     cluster_sync();  // no CTA's shared memory goes away while it is read
