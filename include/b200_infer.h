@@ -281,14 +281,15 @@ int b200_paged_kv_append(const void *k, int64_t k_tok_stride, int64_t k_head_str
  * spread evenly over the SMs; the parts of a split sequence are joined in a fixed
  * order, so results do not depend on timing. Keys in a block whose index is out of
  * range are left out. D 64 or 128. `workspace` as above
- * (b200_flash_attn_paged_batch_workspace_bytes). */
+ * (b200_flash_attn_paged_batch_workspace_bytes with max_keys = max_blocks * block_tokens;
+ * 0 for few sequences with short tables). */
 int b200_flash_attn_paged_batch(const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
                                 int64_t out_seq_stride, int64_t out_head_stride, const b200_kv_pool *pool,
                                 const int32_t *block_table, int64_t table_stride, int64_t max_blocks,
                                 const int32_t *seq_lens, int64_t n_seqs, int64_t Hq, float scale,
                                 void *workspace, size_t workspace_bytes, int32_t *dev_status, void *stream);
-size_t b200_flash_attn_paged_batch_workspace_bytes(int64_t n_seqs, int64_t D, int64_t Hq, int64_t Hkv,
-                                                   int32_t dtype);
+size_t b200_flash_attn_paged_batch_workspace_bytes(int64_t n_seqs, int64_t max_keys, int64_t D, int64_t Hq,
+                                                   int64_t Hkv, int32_t dtype);
 
 /* Samples one token per row of logits [n_rows][n_vocab] (row stride `row_stride`
  * elements, any alignment) from given uniform numbers u[n_rows] in [0, 1). Per row,

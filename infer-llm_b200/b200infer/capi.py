@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import subprocess
 
 PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))  # infer-llm_b200/
@@ -97,7 +98,7 @@ _SIGS = {
                              C.c_int),
     "b200_flash_attn_paged_batch": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _f32,
                                      _vp, _sz, _vp, _vp], C.c_int),
-    "b200_flash_attn_paged_batch_workspace_bytes": ([_i64] * 4 + [_i32], _sz),
+    "b200_flash_attn_paged_batch_workspace_bytes": ([_i64] * 5 + [_i32], _sz),
     "b200_sample": ([_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp], C.c_int),
     "b200_engine_inject_withhold": ([_vp, C.c_int32, C.c_int32], C.c_int),
     "b200_engine_set_decode_launch_counter": ([_vp, C.c_uint64], C.c_int),
@@ -316,9 +317,13 @@ class PagedKV:
 # go to the current torch stream of that device.
 
 class _KVPool(C.Structure):
+    """b200_kv_pool."""
     _fields_ = [("k", _vp), ("v", _vp), ("n_blocks", _i64), ("block_tokens", _i64), ("block_stride", _i64),
                 ("tok_stride", _i64), ("head_stride", _i64), ("n_head_kv", _i64), ("head_dim", _i64),
                 ("dtype", C.c_int32)]
+
+
+_POOL = struct.Struct("@PPqqqqqqqi4x")  # the same, packed (a call of its own per decode step and layer)
 
 
 class _Host:
@@ -328,6 +333,7 @@ class _Host:
     def __init__(self):
         import torch
         self.torch = torch
+        self.empty_like = torch.empty_like
         self.empty, self.i32, self.f32, self.u8 = torch.empty, torch.int32, torch.float32, torch.uint8
         self.dtypes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
         self.current = torch._C._cuda_getDevice
@@ -396,7 +402,7 @@ def _scratch(workspace, nbytes, like, dev):
 
 def _out_rows(out, q, dev):
     if out is None:
-        return _host.empty(q.shape, device=q.device, dtype=q.dtype)
+        return _host.empty_like(q)
     if out.shape != q.shape:
         raise ValueError("out: expected q's shape")
     _rows(out, "out", q.dtype, dev)
@@ -436,7 +442,7 @@ def _pool(k_pool, v_pool):
             k_pool.get_device() != v_pool.get_device() or s[3] != 1:
         raise ValueError("k_pool, v_pool: expected two (blocks, block_tokens, Hkv, D) tensors alike, last axis contiguous")
     n, bt, Hkv, D = k_pool.shape
-    return _KVPool(k_pool.data_ptr(), v_pool.data_ptr(), n, bt, s[0], s[1], s[2], Hkv, D, _dtype(k_pool)), Hkv, D
+    return _POOL.pack(k_pool.data_ptr(), v_pool.data_ptr(), n, bt, s[0], s[1], s[2], Hkv, D, _dtype(k_pool)), bt, Hkv, D
 
 
 def _table(t, n, dev):
@@ -457,7 +463,7 @@ def paged_kv_append(k, v, cu_new, seq_lens, k_pool, v_pool, block_table, status=
     kind = k.dtype
     if k_pool.get_device() != dev or k_pool.dtype != kind:
         raise ValueError(f"k_pool: expected {kind} on cuda:{dev}")
-    pool, Hkv, D = _pool(k_pool, v_pool)
+    pool, _, Hkv, D = _pool(k_pool, v_pool)
     ks, vs = _rows(k, "k", kind, dev), _rows(v, "v", kind, dev)
     T = k.shape[0]
     if k.shape != v.shape or k.shape[1] != Hkv or k.shape[2] != D:
@@ -466,7 +472,7 @@ def paged_kv_append(k, v, cu_new, seq_lens, k_pool, v_pool, block_table, status=
     table, stride, blocks = _table(block_table, n, dev)
     _chk("b200_paged_kv_append", h.append(
         k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _vector(cu_new, "cu_new", n + 1, h.i32, dev),
-        _vector(seq_lens, "seq_lens", n, h.i32, dev), n, T, C.byref(pool), table, stride, blocks, _status_word(status, dev),
+        _vector(seq_lens, "seq_lens", n, h.i32, dev), n, T, pool, table, stride, blocks, _status_word(status, dev),
         h.stream(dev)))
 
 
@@ -480,7 +486,7 @@ def flash_attn_paged_batch(q, k_pool, v_pool, block_table, seq_lens, scale=0.0, 
     kind, dt = q.dtype, _dtype(q)
     if k_pool.get_device() != dev or k_pool.dtype != kind:
         raise ValueError(f"k_pool: expected {kind} on cuda:{dev}")
-    pool, Hkv, Dk = _pool(k_pool, v_pool)
+    pool, bt, Hkv, Dk = _pool(k_pool, v_pool)
     qs = _rows(q, "q", kind, dev)
     n, Hq, D = q.shape
     if D != Dk or Hkv <= 0 or Hq % Hkv:
@@ -488,10 +494,10 @@ def flash_attn_paged_batch(q, k_pool, v_pool, block_table, seq_lens, scale=0.0, 
     table, stride, blocks = _table(block_table, n, dev)
     out = _out_rows(out, q, dev)
     os = out.stride()
-    nbytes = h.batch_bytes(n, D, Hq, Hkv, dt)
+    nbytes = h.batch_bytes(n, blocks * bt, D, Hq, Hkv, dt)
     ws = _scratch(workspace, nbytes, q, dev)
     _chk("b200_flash_attn_paged_batch", h.batch(
-        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], C.byref(pool), table, stride, blocks,
+        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], pool, table, stride, blocks,
         _vector(seq_lens, "seq_lens", n, h.i32, dev), n, Hq, scale, None if ws is None else ws.data_ptr(), nbytes,
         _status_word(status, dev), h.stream(dev)))
     return out

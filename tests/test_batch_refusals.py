@@ -83,8 +83,9 @@ def test_append(kw, code):
 
 
 @pytest.mark.parametrize("kw,code", [(dict(q=None), INVALID), (dict(Hq=3), INVALID), (dict(Hq=0), INVALID),
-                                     (dict(lens=None), INVALID), (dict(stride=1), INVALID), (dict(ws=None), INVALID),
-                                     (dict(wsb=16), INVALID), (dict(ws=P + 4), INVALID), (dict(q=P + 4), UNSUPPORTED),
+                                     (dict(lens=None), INVALID), (dict(stride=1), INVALID), (dict(n=200, ws=None), INVALID),
+                                     (dict(n=200, wsb=16), INVALID), (dict(n=200, ws=P + 4), INVALID),
+                                     (dict(q=P + 4), UNSUPPORTED),
                                      (dict(oh=65), UNSUPPORTED), (dict(n=0), OK)])
 def test_decode(kw, code):
     assert decode(**kw) == code

@@ -390,7 +390,7 @@ def test_calls_on_another_stream_and_in_a_graph(cuda):
     B.paged_kv_append(k, k, cumulative(lens), c.lens, c.k, c.v, c.table)
     q = torch.randn((2, Hq, D), device=cuda).bfloat16()
     out = torch.zeros_like(q)
-    ws = torch.empty(B.lib().b200_flash_attn_paged_batch_workspace_bytes(2, D, Hq, Hkv, 2), dtype=torch.uint8, device=cuda)
+    ws = torch.empty(B.lib().b200_flash_attn_paged_batch_workspace_bytes(2, c.table.shape[1] * bt, D, Hq, Hkv, 2), dtype=torch.uint8, device=cuda)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
