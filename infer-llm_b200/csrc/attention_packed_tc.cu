@@ -338,31 +338,31 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         return false;
     };
 
-            // softmax and output threads: a row of the slot's query tile, a lane of tensor memory
+    // softmax and output threads: a row of the slot's query tile, a lane of tensor memory
     const int slot = (warp - 4) >> 2, qq = warp & 3;
-            const int r = 32 * qq + lane;
-            const uint32_t lanes = static_cast<uint32_t>(32 * qq) << 16;
-            const int tok = t0 + (NT == 2 ? slot * BQ : 0) + r / G;
-            const bool live = r < BQ * G && tok < p.nq;
-            const int last = live ? tok + shift : -1;  // last key the row sees
-            const T *q_row = static_cast<const T *>(a.q) + (p.q0 + tok) * a.q_tok + (kvh * G + r % G) * a.q_head;
-            T *dst = static_cast<T *>(a.out) + (p.q0 + tok) * a.o_tok + (kvh * G + r % G) * a.o_head;
-            // x (columns [c, c + 32) of the row's output) plus the terms of the cleared V rows it sees
-            const auto add_cleared = [&](float (&x)[32], int c, float m_row, float inv) {
-                for (int w = 0; w < 4 * kMaskedTiles; ++w) {
-                    for (uint32_t mask = bad[w]; mask; mask &= mask - 1) {
-                        const int key = first_masked * kPtKeys + 32 * w + __ffs(static_cast<int>(mask)) - 1;
-                        if (key > last) continue;
-                        const T *kr = static_cast<const T *>(a.k) + (p.k0 + key) * a.k_tok + kvh * a.k_head;
-                        const T *vr = static_cast<const T *>(a.v) + (p.k0 + key) * a.v_tok + kvh * a.v_head;
-                        float s = 0.f;
-                        for (int d = 0; d < D; ++d) s = fmaf(to_f32<T>(q_row[d]), to_f32<T>(kr[d]), s);
-                        const float pr = exp2_approx(fmaf(s, a.sl2, -m_row)) * inv;
-    #pragma unroll
-                        for (int j = 0; j < 32; ++j) x[j] = fmaf(pr, to_f32<T>(vr[c + j]), x[j]);
-                    }
-                }
-            };
+    const int r = 32 * qq + lane;
+    const uint32_t lanes = static_cast<uint32_t>(32 * qq) << 16;
+    const int tok = t0 + (NT == 2 ? slot * BQ : 0) + r / G;
+    const bool live = r < BQ * G && tok < p.nq;
+    const int last = live ? tok + shift : -1;  // last key the row sees
+    const T *q_row = static_cast<const T *>(a.q) + (p.q0 + tok) * a.q_tok + (kvh * G + r % G) * a.q_head;
+    T *dst = static_cast<T *>(a.out) + (p.q0 + tok) * a.o_tok + (kvh * G + r % G) * a.o_head;
+    // x (columns [c, c + 32) of the row's output) plus the terms of the cleared V rows it sees
+    const auto add_cleared = [&](float (&x)[32], int c, float m_row, float inv) {
+        for (int w = 0; w < 4 * kMaskedTiles; ++w) {
+            for (uint32_t mask = bad[w]; mask; mask &= mask - 1) {
+                const int key = first_masked * kPtKeys + 32 * w + __ffs(static_cast<int>(mask)) - 1;
+                if (key > last) continue;
+                const T *kr = static_cast<const T *>(a.k) + (p.k0 + key) * a.k_tok + kvh * a.k_head;
+                const T *vr = static_cast<const T *>(a.v) + (p.k0 + key) * a.v_tok + kvh * a.v_head;
+                float s = 0.f;
+                for (int d = 0; d < D; ++d) s = fmaf(to_f32<T>(q_row[d]), to_f32<T>(kr[d]), s);
+                const float pr = exp2_approx(fmaf(s, a.sl2, -m_row)) * inv;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = fmaf(pr, to_f32<T>(vr[c + j]), x[j]);
+            }
+        }
+    };
 
     if (warp < 4) {
         if constexpr (SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
@@ -504,12 +504,11 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                     }
                     const uint32_t mask = __ballot_sync(0xffffffffu, odd);
                     if (mask) {
-                        if (odd)
-                            for (int c = 0; c < D / 8; ++c) {
-                                const uint32_t off = (c >> 3) * Ge::kBox + row * 128 + (c & 7) * 16;
-                                *reinterpret_cast<uint4 *>(v + off) = make_uint4(0, 0, 0, 0);
-                                *reinterpret_cast<uint4 *>(v2 + off) = make_uint4(0, 0, 0, 0);
-                            }
+                        for (int c = 0; odd && c < D / 8; ++c) {
+                            const uint32_t off = (c >> 3) * Ge::kBox + row * 128 + (c & 7) * 16;
+                            *reinterpret_cast<uint4 *>(v + off) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4 *>(v2 + off) = make_uint4(0, 0, 0, 0);
+                        }
                         if (lane == 0) {
                             bad[(t - first_masked) * 4 + row / 32] = mask;
                             bad[4 * kMaskedTiles] = 1;
@@ -527,64 +526,64 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             float2 *stat = reinterpret_cast<float2 *>(base + Ge::kOffStat);  // [step / 2 % 2][slot][row]
             const int32_t *exps = sp.exps + (split_index(p.k0, p.seq, 0) * a.Hkv + kvh) * 2;
             const int64_t ex_step = static_cast<int64_t>(a.Hkv) * 2;
-                            // the steps' O added up. Step i holds sum p v = O 2^(m + ev); l counts in 2^m
-                            float acc[D], L = 0.f, M = -INFINITY, R = -INFINITY;
-            #pragma unroll
-                            for (int d = 0; d < D; ++d) acc[d] = 0.f;
-                            int ev = steps > 0 ? __ldg(exps + 1) : 0;
-                            bool ok = true;
-            #pragma unroll 1
-                            for (int i = 0; i < steps; ++i) {
-                                const int sl = i & 1;
-                                ok = __all_sync(0xffffffffu, wait(&st_full[sl], (i >> 1) & 1) && wait(&o_final[sl], (i >> 1) & 1));
-                                if (!ok) break;
-                                tc_fence_after();
-                                const float2 st = stat[(((i >> 1) & 1) * 2 + sl) * kPtRows + r];
-                                const float e = st.x + static_cast<float>(ev);
-                                if (i + 1 < steps) ev = __ldg(exps + (i + 1) * ex_step + 1);
-                                if (st.x > M) {
-                                    L *= exp2_approx(M - st.x);
-                                    M = st.x;
-                                }
-                                const float f_l = st.x == -INFINITY ? 0.f : exp2_approx(st.x - M);
-                                L = fmaf(f_l, st.y, L);
-                                const float Rn = fmaxf(R, e);
-                                const float f_old = R == -INFINITY ? 0.f : exp2_approx(R - Rn);
-                                const float f_new = e == -INFINITY ? 0.f : exp2_approx(e - Rn);
-                                if (__any_sync(0xffffffffu, Rn > R)) {
-            #pragma unroll
-                                    for (int d = 0; d < D; ++d) acc[d] *= f_old;
-                                }
-                                R = Rn;
-            #pragma unroll
-                                for (int c = 0; c < D / 32; ++c) {
-                                    uint32_t o[32];
-                                    tc_ld32_nowait(col_o(sl) + lanes + 32 * c, o);
-                                    tc_wait_ld();
-                                    tc_reg_fence(o);
-            #pragma unroll
-                                    for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(o[j]), f_new, acc[32 * c + j]);
-                                }
-                                tc_fence_before();
-                                mbar_arrive(&o_empty[sl]);
-                            }
-                            const float inv = L != 0.f ? 1.0f / L : 0.f;  // a row that sees no key: zeros
-                            // P and l both carry 2^kTop; two factors, neither of which overflows
-                            const float half = R == -INFINITY ? 0.f : 0.5f * (R - M);
-                            const float undo = exp2_approx(half);
-                            if (ok && live) {
-                                const bool any_bad = bad[4 * kMaskedTiles] != 0;
-            #pragma unroll
-                                for (int c = 0; c < D / 32; ++c) {
-                                    float x[32];
-            #pragma unroll
-                                    for (int j = 0; j < 32; ++j) x[j] = acc[32 * c + j] * inv * undo * undo;
-                                    if (any_bad) add_cleared(x, 32 * c, M, inv * pow2(kTop));
-            #pragma unroll
-                                    for (int j = 0; j < 32; j += 4)
-                                        *reinterpret_cast<float4 *>(dst + 32 * c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-                                }
-                            }
+            // the steps' O added up. Step i holds sum p v = O 2^(m + ev); l counts in 2^m
+            float acc[D], L = 0.f, M = -INFINITY, R = -INFINITY;
+#pragma unroll
+            for (int d = 0; d < D; ++d) acc[d] = 0.f;
+            int ev = steps > 0 ? __ldg(exps + 1) : 0;
+            bool ok = true;
+#pragma unroll 1
+            for (int i = 0; i < steps; ++i) {
+                const int sl = i & 1;
+                ok = __all_sync(0xffffffffu, wait(&st_full[sl], (i >> 1) & 1) && wait(&o_final[sl], (i >> 1) & 1));
+                if (!ok) break;
+                tc_fence_after();
+                const float2 st = stat[(((i >> 1) & 1) * 2 + sl) * kPtRows + r];
+                const float e = st.x + static_cast<float>(ev);
+                if (i + 1 < steps) ev = __ldg(exps + (i + 1) * ex_step + 1);
+                if (st.x > M) {
+                    L *= exp2_approx(M - st.x);
+                    M = st.x;
+                }
+                const float f_l = st.x == -INFINITY ? 0.f : exp2_approx(st.x - M);
+                L = fmaf(f_l, st.y, L);
+                const float Rn = fmaxf(R, e);
+                const float f_old = R == -INFINITY ? 0.f : exp2_approx(R - Rn);
+                const float f_new = e == -INFINITY ? 0.f : exp2_approx(e - Rn);
+                if (__any_sync(0xffffffffu, Rn > R)) {
+#pragma unroll
+                    for (int d = 0; d < D; ++d) acc[d] *= f_old;
+                }
+                R = Rn;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tc_ld32_nowait(col_o(sl) + lanes + 32 * c, o);
+                    tc_wait_ld();
+                    tc_reg_fence(o);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(o[j]), f_new, acc[32 * c + j]);
+                }
+                tc_fence_before();
+                mbar_arrive(&o_empty[sl]);
+            }
+            const float inv = L != 0.f ? 1.0f / L : 0.f;  // a row that sees no key: zeros
+            // P and l both carry 2^kTop; two factors, neither of which overflows
+            const float half = R == -INFINITY ? 0.f : 0.5f * (R - M);
+            const float undo = exp2_approx(half);
+            if (ok && live) {
+                const bool any_bad = bad[4 * kMaskedTiles] != 0;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    float x[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) x[j] = acc[32 * c + j] * inv * undo * undo;
+                    if (any_bad) add_cleared(x, 32 * c, M, inv * pow2(kTop));
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<float4 *>(dst + 32 * c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                }
+            }
         }
     } else if constexpr (SPLIT) {
         // ---- F32 softmax
@@ -592,115 +591,115 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         float2 *stat = reinterpret_cast<float2 *>(base + Ge::kOffStat);  // [step / 2 % 2][slot][row]
         const int32_t *exps = sp.exps + (split_index(p.k0, p.seq, 0) * a.Hkv + kvh) * 2;
         const int64_t ex_step = static_cast<int64_t>(a.Hkv) * 2;
-                        // the row of Q as hi and lo planes: this warpgroup writes half of its columns
-                        const float4 *q4 = reinterpret_cast<const float4 *>(q_row);
-                        uint32_t top = 0;
+        // the row of Q as hi and lo planes: this warpgroup writes half of its columns
+        const float4 *q4 = reinterpret_cast<const float4 *>(q_row);
+        uint32_t top = 0;
 #pragma unroll 8
-                        for (int c = 0; c < D / 4; ++c) {
-                            const float4 x = live ? __ldg(q4 + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            top = max(max(top, max(finite_magnitude(x.x), finite_magnitude(x.y))),
-                                      max(finite_magnitude(x.z), finite_magnitude(x.w)));
-                        }
-                        const int eq = top_exponent(top) - kTop;
-                        const float s = pow2(-eq);
+        for (int c = 0; c < D / 4; ++c) {
+            const float4 x = live ? __ldg(q4 + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            top = max(max(top, max(finite_magnitude(x.x), finite_magnitude(x.y))),
+                      max(finite_magnitude(x.z), finite_magnitude(x.w)));
+        }
+        const int eq = top_exponent(top) - kTop;
+        const float s = pow2(-eq);
 #pragma unroll 2
-                        for (int c = 0; c < D / 16; ++c) {  // 16-byte chunks of eight halves
-                            const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-                            const float4 x = live ? __ldg(q4 + slot * (D / 8) + 2 * c) : zero;
-                            const float4 y = live ? __ldg(q4 + slot * (D / 8) + 2 * c + 1) : zero;
-                            const float e[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-                            __align__(16) __half h[8], lo[8];
+        for (int c = 0; c < D / 16; ++c) {  // 16-byte chunks of eight halves
+            const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 x = live ? __ldg(q4 + slot * (D / 8) + 2 * c) : zero;
+            const float4 y = live ? __ldg(q4 + slot * (D / 8) + 2 * c + 1) : zero;
+            const float e[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            __align__(16) __half h[8], lo[8];
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) split_f16(e[j] * s, h[j], lo[j]);
-                            const int chunk = slot * (D / 16) + c;
-                            unsigned char *at = base + (chunk >> 3) * Ge::kBox + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
-                            *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(h);
-                            *reinterpret_cast<uint4 *>(at + Ge::kTile) = *reinterpret_cast<const uint4 *>(lo);
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        mbar_arrive(q_full);
-                        const uint32_t ts = col_s(slot) + lanes;
-                        int ek = slot < steps ? __ldg(exps + slot * ex_step) : 0;
-        #pragma unroll 1
-                        for (int i = slot; i < steps; i += 2) {
-                            const float sl2 = a.sl2 * pow2(ek + eq);
-                            if (i + 2 < steps) ek = __ldg(exps + (i + 2) * ex_step);
-                            if (!__all_sync(0xffffffffu, wait(&s_full[slot], (i >> 1) & 1))) break;
-                            tc_fence_after();
-                            const int vis = last + 1 - i * kPtKeys;  // keys of the tile the row sees
-                            const bool whole = __all_sync(0xffffffffu, vis >= kPtKeys);
-                            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        #pragma unroll
-                            for (int c = 0; c < 4; c += 2) {
-                                uint32_t sv[2][32];
-                                tc_ld32_nowait(ts + 32 * c, sv[0]);
-                                tc_ld32_nowait(ts + 32 * c + 32, sv[1]);
-                                tc_wait_ld();
-        #pragma unroll
-                                for (int h = 0; h < 2; ++h) {
-                                    tc_reg_fence(sv[h]);
-        #pragma unroll
-                                    for (int j = 0; j < 32; ++j)
-                                        if (whole || 32 * (c + h) + j < vis) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(sv[h][j]));
-                                }
-                            }
-                            const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-                            const float shift_p = static_cast<float>(kTop) - (m == -INFINITY ? 0.f : m);
-                            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        #pragma unroll 1
-                            for (int c = 0; c < 4; ++c) {
-                                uint32_t sv[32], pv[32];
-                                tc_ld32_nowait(ts + 32 * c, sv);
-                                tc_wait_ld();
-                                tc_reg_fence(sv);
-        #pragma unroll
-                                for (int j = 0; j < 16; ++j) {
-                                    float x = exp2_approx(fmaf(__uint_as_float(sv[2 * j]), sl2, shift_p));
-                                    float y = exp2_approx(fmaf(__uint_as_float(sv[2 * j + 1]), sl2, shift_p));
-                                    if (!whole) {
-                                        x = 32 * c + 2 * j < vis ? x : 0.f;
-                                        y = 32 * c + 2 * j + 1 < vis ? y : 0.f;
-                                    }
-                                    sum[j & 1] += x;
-                                    sum[2 + (j & 1)] += y;
-                                    split_f16x2(x, y, pv[j], pv[16 + j]);
-                                }
-                                tc_st32(ts + 32 * c, pv);
-                            }
-                            stat[(((i >> 1) & 1) * 2 + slot) * kPtRows + r] = make_float2(m, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-                            mbar_arrive(&st_full[slot]);
-                            tc_wait_st();
-                            tc_fence_before();
-                            mbar_arrive(&p_part[slot]);
-                        }
+            for (int j = 0; j < 8; ++j) split_f16(e[j] * s, h[j], lo[j]);
+            const int chunk = slot * (D / 16) + c;
+            unsigned char *at = base + (chunk >> 3) * Ge::kBox + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+            *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(h);
+            *reinterpret_cast<uint4 *>(at + Ge::kTile) = *reinterpret_cast<const uint4 *>(lo);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(q_full);
+        const uint32_t ts = col_s(slot) + lanes;
+        int ek = slot < steps ? __ldg(exps + slot * ex_step) : 0;
+#pragma unroll 1
+        for (int i = slot; i < steps; i += 2) {
+            const float sl2 = a.sl2 * pow2(ek + eq);
+            if (i + 2 < steps) ek = __ldg(exps + (i + 2) * ex_step);
+            if (!__all_sync(0xffffffffu, wait(&s_full[slot], (i >> 1) & 1))) break;
+            tc_fence_after();
+            const int vis = last + 1 - i * kPtKeys;  // keys of the tile the row sees
+            const bool whole = __all_sync(0xffffffffu, vis >= kPtKeys);
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+                uint32_t sv[2][32];
+                tc_ld32_nowait(ts + 32 * c, sv[0]);
+                tc_ld32_nowait(ts + 32 * c + 32, sv[1]);
+                tc_wait_ld();
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    tc_reg_fence(sv[h]);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (whole || 32 * (c + h) + j < vis) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(sv[h][j]));
+                }
+            }
+            const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+            const float shift_p = static_cast<float>(kTop) - (m == -INFINITY ? 0.f : m);
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                uint32_t sv[32], pv[32];
+                tc_ld32_nowait(ts + 32 * c, sv);
+                tc_wait_ld();
+                tc_reg_fence(sv);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    float x = exp2_approx(fmaf(__uint_as_float(sv[2 * j]), sl2, shift_p));
+                    float y = exp2_approx(fmaf(__uint_as_float(sv[2 * j + 1]), sl2, shift_p));
+                    if (!whole) {
+                        x = 32 * c + 2 * j < vis ? x : 0.f;
+                        y = 32 * c + 2 * j + 1 < vis ? y : 0.f;
+                    }
+                    sum[j & 1] += x;
+                    sum[2 + (j & 1)] += y;
+                    split_f16x2(x, y, pv[j], pv[16 + j]);
+                }
+                tc_st32(ts + 32 * c, pv);
+            }
+            stat[(((i >> 1) & 1) * 2 + slot) * kPtRows + r] = make_float2(m, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+            mbar_arrive(&st_full[slot]);
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_part[slot]);
+        }
     } else {
         // ---- softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-                    const uint32_t ts = col_s(slot) + lanes, to = col_o(slot) + lanes;
-                    float m = -INFINITY, l = 0.f;
-                    bool ok = true;
-        #pragma unroll 1
-                    for (int i = slot; i < steps; i += 2) {
-                        const int k0 = (NT == 2 ? i >> 1 : i) * kPtKeys;
-                        ok = __all_sync(0xffffffffu, wait(&s_full[slot], (i >> 1) & 1));
-                        if (!ok) break;
-                        tc_fence_after();
-                        uint32_t sv[4][32];
-        #pragma unroll
-                        for (int c = 0; c < 4; ++c) tc_ld32_nowait(ts + 32 * c, sv[c]);
-                        tc_wait_ld();
-        #pragma unroll
-                        for (int c = 0; c < 4; ++c) tc_reg_fence(sv[c]);
-                        const int vis = last + 1 - k0;  // keys of the tile the row sees
-                        const bool whole = __all_sync(0xffffffffu, vis >= kPtKeys);
+        const uint32_t ts = col_s(slot) + lanes, to = col_o(slot) + lanes;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+#pragma unroll 1
+        for (int i = slot; i < steps; i += 2) {
+            const int k0 = (NT == 2 ? i >> 1 : i) * kPtKeys;
+            ok = __all_sync(0xffffffffu, wait(&s_full[slot], (i >> 1) & 1));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t sv[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tc_ld32_nowait(ts + 32 * c, sv[c]);
+            tc_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tc_reg_fence(sv[c]);
+            const int vis = last + 1 - k0;  // keys of the tile the row sees
+            const bool whole = __all_sync(0xffffffffu, vis >= kPtKeys);
             if (!whole) {
-        #pragma unroll
-                            for (int c = 0; c < 4; ++c)
-        #pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (32 * c + j >= vis) sv[c][j] = 0xFF800000u;
-                        }
-                        float mx[8];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (32 * c + j >= vis) sv[c][j] = 0xFF800000u;
+            }
+            float mx[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) mx[j] = fmaxf(__uint_as_float(sv[0][2 * j]), __uint_as_float(sv[0][2 * j + 1]));
 #pragma unroll
@@ -710,29 +709,29 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                     mx[(j >> 1) & 7] = max3(mx[(j >> 1) & 7], __uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1]));
             const float top = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * a.sl2;
             float alpha = 1.f;
-                        bool grow = false;
-                        if (m == -INFINITY) {
-                            m = top;  // nothing summed so far: O and l are zero, or not yet written
-                        } else if (top > m + kPtRescale) {
-                            alpha = exp2_approx(m - top);
-                            m = top;
-                            grow = true;
-                        }
-                        if (__any_sync(0xffffffffu, grow)) {
-                            // every earlier product of this slot completed before its scores did
-                            l *= alpha;
-        #pragma unroll 1
-                            for (int c = 0; c < D / 32; ++c) {
-                                uint32_t o[32];
-                                tc_ld32_nowait(to + 32 * c, o);
-                                tc_wait_ld();
-                                tc_reg_fence(o);
-        #pragma unroll
-                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-                                tc_st32(to + 32 * c, o);
-                            }
-                        }
-                        const float ms = m == -INFINITY ? 0.f : m;
+            bool grow = false;
+            if (m == -INFINITY) {
+                m = top;  // nothing summed so far: O and l are zero, or not yet written
+            } else if (top > m + kPtRescale) {
+                alpha = exp2_approx(m - top);
+                m = top;
+                grow = true;
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+                // every earlier product of this slot completed before its scores did
+                l *= alpha;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tc_ld32_nowait(to + 32 * c, o);
+                    tc_wait_ld();
+                    tc_reg_fence(o);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                    tc_st32(to + 32 * c, o);
+                }
+            }
+            const float ms = m == -INFINITY ? 0.f : m;
             const uint64_t scale2 = pair_of(a.sl2, a.sl2), minus2 = pair_of(-ms, -ms);
             uint64_t sum[4] = {pair_of(l, 0.f), 0, 0, 0};
             // every kPolyStep-th pair by polynomial: the special-function unit takes 8 cycles a warp
@@ -768,71 +767,71 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             mbar_arrive(&p_full[slot]);
         }
         const bool mine = steps > slot;  // the slot had a step
-                    if (ok && mine) ok = __all_sync(0xffffffffu, wait(&o_final[slot], 0));
-                    tc_fence_after();
-                    // the row's output: O / l, plus what the cleared V rows would have added
-                    float m_row = m, l_row = l, f_own = 1.f, f_other = 0.f;
-                    constexpr int NC = NT == 2 ? D / 32 : D / 64;  // 32-column pieces this thread writes
-                    const int c0 = NT == 2 ? 0 : slot * NC;
-                    if constexpr (NT == 1) {
-                        // the slots' halves of the key tiles, joined: each warpgroup hands the other half of
-                        // its columns over through the ring (no copy or product uses it any more)
-                        float2 *stat = reinterpret_cast<float2 *>(base);  // over Q: every product with it is complete
-                        float *xch = reinterpret_cast<float *>(base + Ge::kOffRing) + slot * (D / 2) * kPtRows;
-                        asm volatile("bar.sync 1, 256;" ::: "memory");  // both slots' products are complete
-                        stat[slot * kPtRows + r] = make_float2(m, mine ? l : 0.f);
-                        if (ok && mine) {
-        #pragma unroll 1
-                            for (int c = 0; c < NC; ++c) {
-                                uint32_t o[32];
-                                tc_ld32_nowait(to + 32 * ((slot ^ 1) * NC + c), o);
-                                tc_wait_ld();
-                                tc_reg_fence(o);
-        #pragma unroll
-                                for (int j = 0; j < 32; ++j) xch[(32 * c + j) * kPtRows + r] = __uint_as_float(o[j]);
-                            }
-                        }
-                        asm volatile("bar.sync 1, 256;" ::: "memory");
-                        const float2 other = stat[(slot ^ 1) * kPtRows + r];
-                        m_row = fmaxf(m, other.x);
-                        const float mm = m_row == -INFINITY ? 0.f : m_row;
-                        f_own = mine ? exp2_approx(m - mm) : 0.f;
-                        f_other = exp2_approx(other.x - mm);
-                        l_row = (mine ? l * f_own : 0.f) + other.y * f_other;
-                    }
-                    const float inv = l_row != 0.f ? 1.0f / l_row : 0.f;  // a row that sees no key: zeros
-                    if (ok) {
-                        const bool any_bad = bad[4 * kMaskedTiles] != 0;
-                        const float *got = reinterpret_cast<const float *>(base + Ge::kOffRing) + (slot ^ 1) * (D / 2) * kPtRows;
-                        const bool other_has = NT == 1 && steps > (slot ^ 1);
-        #pragma unroll 1
-                        for (int c = 0; c < NC; ++c) {
-                            uint32_t o[32];
-                            if (mine) {
-                                tc_ld32_nowait(to + 32 * (c0 + c), o);
-                                tc_wait_ld();
-                                tc_reg_fence(o);
-                            } else {
-        #pragma unroll
-                                for (int j = 0; j < 32; ++j) o[j] = 0;
-                            }
-                            float x[32];
-        #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                x[j] = __uint_as_float(o[j]);
-                                if (NT == 1) x[j] = x[j] * f_own + (other_has ? got[(32 * c + j) * kPtRows + r] * f_other : 0.f);
-                                x[j] *= inv;
-                            }
-                            if (any_bad && live) add_cleared(x, 32 * (c0 + c), m_row, inv);
-                            if (live) {
-        #pragma unroll
-                                for (int j = 0; j < 32; j += 8)
-                                    *reinterpret_cast<uint4 *>(dst + 32 * (c0 + c) + j) =
-                                        make_uint4(pack_pair<T>(x[j], x[j + 1]), pack_pair<T>(x[j + 2], x[j + 3]),
-                                                   pack_pair<T>(x[j + 4], x[j + 5]), pack_pair<T>(x[j + 6], x[j + 7]));
-                            }
-                        }
-                    }
+        if (ok && mine) ok = __all_sync(0xffffffffu, wait(&o_final[slot], 0));
+        tc_fence_after();
+        // the row's output: O / l, plus what the cleared V rows would have added
+        float m_row = m, l_row = l, f_own = 1.f, f_other = 0.f;
+        constexpr int NC = NT == 2 ? D / 32 : D / 64;  // 32-column pieces this thread writes
+        const int c0 = NT == 2 ? 0 : slot * NC;
+        if constexpr (NT == 1) {
+            // the slots' halves of the key tiles, joined: each warpgroup hands the other half of
+            // its columns over through the ring (no copy or product uses it any more)
+            float2 *stat = reinterpret_cast<float2 *>(base);  // over Q: every product with it is complete
+            float *xch = reinterpret_cast<float *>(base + Ge::kOffRing) + slot * (D / 2) * kPtRows;
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // both slots' products are complete
+            stat[slot * kPtRows + r] = make_float2(m, mine ? l : 0.f);
+            if (ok && mine) {
+#pragma unroll 1
+                for (int c = 0; c < NC; ++c) {
+                    uint32_t o[32];
+                    tc_ld32_nowait(to + 32 * ((slot ^ 1) * NC + c), o);
+                    tc_wait_ld();
+                    tc_reg_fence(o);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) xch[(32 * c + j) * kPtRows + r] = __uint_as_float(o[j]);
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float2 other = stat[(slot ^ 1) * kPtRows + r];
+            m_row = fmaxf(m, other.x);
+            const float mm = m_row == -INFINITY ? 0.f : m_row;
+            f_own = mine ? exp2_approx(m - mm) : 0.f;
+            f_other = exp2_approx(other.x - mm);
+            l_row = (mine ? l * f_own : 0.f) + other.y * f_other;
+        }
+        const float inv = l_row != 0.f ? 1.0f / l_row : 0.f;  // a row that sees no key: zeros
+        if (ok) {
+            const bool any_bad = bad[4 * kMaskedTiles] != 0;
+            const float *got = reinterpret_cast<const float *>(base + Ge::kOffRing) + (slot ^ 1) * (D / 2) * kPtRows;
+            const bool other_has = NT == 1 && steps > (slot ^ 1);
+#pragma unroll 1
+            for (int c = 0; c < NC; ++c) {
+                uint32_t o[32];
+                if (mine) {
+                    tc_ld32_nowait(to + 32 * (c0 + c), o);
+                    tc_wait_ld();
+                    tc_reg_fence(o);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = 0;
+                }
+                float x[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    x[j] = __uint_as_float(o[j]);
+                    if (NT == 1) x[j] = x[j] * f_own + (other_has ? got[(32 * c + j) * kPtRows + r] * f_other : 0.f);
+                    x[j] *= inv;
+                }
+                if (any_bad && live) add_cleared(x, 32 * (c0 + c), m_row, inv);
+                if (live) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                        *reinterpret_cast<uint4 *>(dst + 32 * (c0 + c) + j) =
+                            make_uint4(pack_pair<T>(x[j], x[j + 1]), pack_pair<T>(x[j + 2], x[j + 3]),
+                                       pack_pair<T>(x[j + 4], x[j + 5]), pack_pair<T>(x[j + 6], x[j + 7]));
+                }
+            }
+        }
     }
     tc_fence_before();
     __syncthreads();
