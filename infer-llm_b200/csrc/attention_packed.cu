@@ -165,8 +165,8 @@ extern "C" {
 
 size_t b200_flash_attn_packed_workspace_bytes(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t D, int64_t Hq,
                                               int64_t Hkv, int32_t dtype) {
-    if (n_seqs <= 0 || total_q <= 0 || total_k <= 0 || D <= 0 || Hkv <= 0 || Hq <= 0) return 0;
-    return packed_tc_workspace(n_seqs, total_k, D, Hkv, dtype);
+    if (n_seqs <= 0 || total_q <= 0 || total_k <= 0 || D <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv) return 0;
+    return packed_tc_workspace(n_seqs, total_q, total_k, D, Hq, Hkv, dtype);
 }
 
 int b200_flash_attn_packed(const void *q, int64_t q_tok_stride, int64_t q_head_stride, const void *k,

@@ -19,7 +19,8 @@ struct PackedArgs {
 };
 
 // The tensor-core kernel; cudaErrorNotSupported (nothing launched) where it does not apply.
-size_t packed_tc_workspace(int64_t n_seqs, int64_t total_k, int64_t D, int64_t Hkv, int32_t dtype);
+size_t packed_tc_workspace(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t D, int64_t Hq, int64_t Hkv,
+                           int32_t dtype);
 cudaError_t packed_tc_launch(const PackedArgs &a, cudaStream_t stream);
 
 }  // namespace b200

@@ -10,6 +10,8 @@
 //   NT = 2: two query tiles over the same key tiles (K and V are read once for both);
 //   NT = 1: one query tile, even key tiles in slot 0 and odd ones in slot 1, joined at the
 //           end (half as long a chain for calls with few query tiles).
+// With fewer query tiles than SMs and long contexts the key tiles are also cut into `parts`, a CTA
+// each (NT = 1); packed_join_kernel weighs the parts' rows by their sums.
 // A query tile's rows are tokens times the G heads of a KV head (row = token * G + head), as
 // many whole tokens as fit 128 rows, so the heads that share keys share every tile.
 // Warp roles: warp 0 TMA, warp 1 tensor cores, warps 2-3 V check, warps 4-11 softmax, and for
@@ -171,10 +173,13 @@ B200_DEVICE uint32_t pack_pair(float x, float y) {
 }
 
 // F32 operands split for the tensor cores: planes of F16 rows [2][total_k][Hkv][D], and per
-// (key tile, KV head) the exponents of K and of V.
+// (key tile, KV head) the exponents of K and of V. And the parts of a query tile's keys.
 struct SplitView {
     const int32_t *exps = nullptr;
     int64_t total_k = 0;
+    int parts = 1;            // of each query tile's keys
+    float *part_o = nullptr;  // [CTA][128][D], with parts > 1
+    float2 *part_ml = nullptr;
 };
 constexpr int kTop = 14;  // largest magnitudes in [2^14, 2^15); P <= 1 times 2^14
 
@@ -195,10 +200,12 @@ B200_DEVICE void split_f16(float x, __half &hi, __half &lo) {
     hi = __float2half_rn(x);
     lo = finite_magnitude(x) || x == 0.f ? __float2half_rn(x - __half2float(hi)) : __half(0.f);
 }
-B200_DEVICE void split_f16x2(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(x, y);
+B200_DEVICE void split_f16x2(uint64_t v, uint32_t &hi, uint32_t &lo) {
+    const float2 x = of_pair(v);
+    const __half2 h = __floats2half2_rn(x.x, x.y);
     const float2 f = __half22float2(h);
-    const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
+    const float2 d = of_pair(add_pair(v, pair_of(-f.x, -f.y)));
+    const __half2 r = __floats2half2_rn(d.x, d.y);
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&r);
 }
@@ -286,18 +293,6 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     uint32_t *bad = reinterpret_cast<uint32_t *>(base + Ge::kOffBad);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int G = a.G, BQ = kPtRows / G, MT = NT * BQ;  // tokens of a query tile, of the CTA
-    const int kvh = blockIdx.x % a.Hkv;
-    const PackedTile p =
-        find_packed_tile(a.cu_q, a.cu_k, a.n_seqs, a.total_q, a.total_k, 1, MT, blockIdx.x / a.Hkv, a.status);
-    if (p.seq < 0) return;
-    const int t0 = p.tile * MT;                        // first token
-    const int shift = p.nk - p.nq;                     // token t sees keys 0 .. t + shift
-    const int seen = min(p.nq, t0 + MT) + shift;       // keys the last token sees (may be <= 0)
-    const int nt = seen > 0 ? (seen + kPtKeys - 1) / kPtKeys : 0;  // key tiles
-    const int steps = NT * nt;
-    const int first_masked = max(0, (t0 + shift + 1) / kPtKeys);  // tiles from here on hide keys from some row
-
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 1);
@@ -318,6 +313,8 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         }
         mbar_init(idle, 1);
         fence_barrier_init();
+        for (const CUtensorMap *m : {&tq, &tk, &tv})
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
     }
     if (threadIdx.x < 4 * kMaskedTiles + 1) bad[threadIdx.x] = 0;
     if (warp == 2) {
@@ -325,6 +322,22 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+
+    const int G = a.G, BQ = kPtRows / G, MT = NT * BQ;  // tokens of a query tile, of the CTA
+    const int kvh = blockIdx.x / sp.parts % a.Hkv, part = blockIdx.x % sp.parts;
+    const PackedTile p = find_packed_tile(a.cu_q, a.cu_k, a.n_seqs, a.total_q, a.total_k, 1, MT,
+                                          blockIdx.x / (sp.parts * a.Hkv), a.status);
+    const bool some = p.seq >= 0;                      // not past the last tile
+    const int t0 = p.tile * MT;                        // first token
+    const int shift = p.nk - p.nq;                     // token t sees keys 0 .. t + shift
+    const int seen = min(p.nq, t0 + MT) + shift;       // keys the last token sees (may be <= 0)
+    const int tiles = some && seen > 0 ? (seen + kPtKeys - 1) / kPtKeys : 0;  // key tiles, of which this CTA's:
+    const int ta = tiles * part / sp.parts, nt = tiles * (part + 1) / sp.parts - ta;
+    const int steps = NT * nt;
+    // the CTA's tiles from this one on hide keys from some row
+    const int first_masked = max(0, (t0 + shift + 1) / kPtKeys - ta);
+    const int64_t k0 = p.k0 + static_cast<int64_t>(ta) * kPtKeys;  // its first key
+
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -343,18 +356,40 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     const int r = 32 * qq + lane;
     const uint32_t lanes = static_cast<uint32_t>(32 * qq) << 16;
     const int tok = t0 + (NT == 2 ? slot * BQ : 0) + r / G;
-    const bool live = r < BQ * G && tok < p.nq;
-    const int last = live ? tok + shift : -1;  // last key the row sees
+    const bool live = some && r < BQ * G && tok < p.nq;
+    const int last = live ? tok + shift - ta * kPtKeys : -1;  // last of the CTA's keys that the row sees
     const T *q_row = static_cast<const T *>(a.q) + (p.q0 + tok) * a.q_tok + (kvh * G + r % G) * a.q_head;
-    T *dst = static_cast<T *>(a.out) + (p.q0 + tok) * a.o_tok + (kvh * G + r % G) * a.o_head;
+    // Rows of a query tile (first token t) from shared memory to the output: a thread writes its
+    // row's 16-byte chunk c to row r, chunk c ^ (r % 8) of `stage`, and the group's threads
+    // then copy whole rows (a row written by its own thread reaches 32 lines an instruction).
+    constexpr int kRowChunks = D * static_cast<int>(sizeof(T)) / 16;
+    const auto store_rows = [&](const unsigned char *stage, int t, int id, int threads) {
+        const int step = threads / kRowChunks, dt = step / G, dg = step % G, c = id % kRowChunks;
+        int row = id / kRowChunks, g = row % G;
+        t += row / G;
+#pragma unroll 4
+        for (; row < BQ * G && t < p.nq; row += step) {
+            T *to_row = static_cast<T *>(a.out) + (p.q0 + t) * a.o_tok + (kvh * G + g) * a.o_head;
+            reinterpret_cast<uint4 *>(to_row)[c] =
+                *reinterpret_cast<const uint4 *>(stage + (row * kRowChunks + (c ^ (row & 7))) * 16);
+            t += dt;
+            g += dg;
+            if (g >= G) g -= G, ++t;
+        }
+    };
+    const auto staged = [&](unsigned char *stage, int c) {
+        return reinterpret_cast<uint4 *>(stage + (r * kRowChunks + (c ^ (r & 7))) * 16);
+    };
+    // this CTA's part of the row: its normalised output, and (m, l) to weigh it by
+    const int64_t part_row = static_cast<int64_t>(blockIdx.x) * kPtRows + r;
     // x (columns [c, c + 32) of the row's output) plus the terms of the cleared V rows it sees
     const auto add_cleared = [&](float (&x)[32], int c, float m_row, float inv) {
         for (int w = 0; w < 4 * kMaskedTiles; ++w) {
             for (uint32_t mask = bad[w]; mask; mask &= mask - 1) {
                 const int key = first_masked * kPtKeys + 32 * w + __ffs(static_cast<int>(mask)) - 1;
                 if (key > last) continue;
-                const T *kr = static_cast<const T *>(a.k) + (p.k0 + key) * a.k_tok + kvh * a.k_head;
-                const T *vr = static_cast<const T *>(a.v) + (p.k0 + key) * a.v_tok + kvh * a.v_head;
+                const T *kr = static_cast<const T *>(a.k) + (k0 + key) * a.k_tok + kvh * a.k_head;
+                const T *vr = static_cast<const T *>(a.v) + (k0 + key) * a.v_tok + kvh * a.v_head;
                 float s = 0.f;
                 for (int d = 0; d < D; ++d) s = fmaf(to_f32<T>(q_row[d]), to_f32<T>(kr[d]), s);
                 const float pr = exp2_approx(fmaf(s, a.sl2, -m_row)) * inv;
@@ -386,7 +421,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
 #pragma unroll
                     for (int b = 0; b < D / 64; ++b)
                         tma_load_3d(sbase + Ge::kOffRing + st * Ge::kTile + b * Ge::kBox, map, 64 * b, kvh,
-                                    static_cast<int32_t>(p.k0 + h * sp.total_k) + t * kPtKeys, smem_addr(&full[st]), pol);
+                                    static_cast<int32_t>(k0 + h * sp.total_k) + t * kPtKeys, smem_addr(&full[st]), pol);
                     ++issued;
                 }
                 return true;
@@ -522,9 +557,9 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     } else if (SPLIT && warp >= 12) {
         // ---- F32: the output's sum
         if constexpr (SPLIT) {
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
             float2 *stat = reinterpret_cast<float2 *>(base + Ge::kOffStat);  // [step / 2 % 2][slot][row]
-            const int32_t *exps = sp.exps + (split_index(p.k0, p.seq, 0) * a.Hkv + kvh) * 2;
+            const int32_t *exps = sp.exps + (split_index(p.k0, p.seq, ta) * a.Hkv + kvh) * 2;
             const int64_t ex_step = static_cast<int64_t>(a.Hkv) * 2;
             // the steps' O added up. Step i holds sum p v = O 2^(m + ev); l counts in 2^m
             float acc[D], L = 0.f, M = -INFINITY, R = -INFINITY;
@@ -556,13 +591,11 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                 }
                 R = Rn;
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[32];
-                    tc_ld32_nowait(col_o(sl) + lanes + 32 * c, o);
-                    tc_wait_ld();
-                    tc_reg_fence(o);
+                for (int c = 0; c < D / 16; ++c) {
+                    float o[16];
+                    tc_ld16(col_o(sl) + lanes + 16 * c, o);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) acc[32 * c + j] = fmaf(__uint_as_float(o[j]), f_new, acc[32 * c + j]);
+                    for (int j = 0; j < 16; ++j) acc[16 * c + j] = fmaf(o[j], f_new, acc[16 * c + j]);
                 }
                 tc_fence_before();
                 mbar_arrive(&o_empty[sl]);
@@ -571,43 +604,57 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             // P and l both carry 2^kTop; two factors, neither of which overflows
             const float half = R == -INFINITY ? 0.f : 0.5f * (R - M);
             const float undo = exp2_approx(half);
-            if (ok && live) {
+            if (sp.parts > 1 && live) sp.part_ml[part_row] = make_float2(M, L);
+            if (steps == 0) ok = __all_sync(0xffffffffu, wait(q_full, 0));  // Q's planes are written by now
+            if (ok) {
                 const bool any_bad = bad[4 * kMaskedTiles] != 0;
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
                     float x[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) x[j] = acc[32 * c + j] * inv * undo * undo;
-                    if (any_bad) add_cleared(x, 32 * c, M, inv * pow2(kTop));
+                    if (any_bad && live) add_cleared(x, 32 * c, M, inv * pow2(kTop));
+                    if (sp.parts == 1) {  // over Q: every product with it is complete
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4 *>(dst + 32 * c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<float4 *>(staged(base, 8 * c + j)) =
+                                make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+                    } else if (live) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            *reinterpret_cast<float4 *>(sp.part_o + part_row * D + 32 * c + j) =
+                                make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                    }
                 }
             }
+            named_sync(2, 128);
+            if (sp.parts == 1 && ok && some) store_rows(base, t0, r, 128);
         }
     } else if constexpr (SPLIT) {
         // ---- F32 softmax
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
         float2 *stat = reinterpret_cast<float2 *>(base + Ge::kOffStat);  // [step / 2 % 2][slot][row]
-        const int32_t *exps = sp.exps + (split_index(p.k0, p.seq, 0) * a.Hkv + kvh) * 2;
+        const int32_t *exps = sp.exps + (split_index(p.k0, p.seq, ta) * a.Hkv + kvh) * 2;
         const int64_t ex_step = static_cast<int64_t>(a.Hkv) * 2;
         // the row of Q as hi and lo planes: this warpgroup writes half of its columns
-        const float4 *q4 = reinterpret_cast<const float4 *>(q_row);
+        const float4 *q4 = reinterpret_cast<const float4 *>(q_row) + slot * (D / 8);
+        float4 x[D / 8];
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) x[c] = live ? __ldg(q4 + c) : make_float4(0.f, 0.f, 0.f, 0.f);
         uint32_t top = 0;
-#pragma unroll 8
-        for (int c = 0; c < D / 4; ++c) {
-            const float4 x = live ? __ldg(q4 + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-            top = max(max(top, max(finite_magnitude(x.x), finite_magnitude(x.y))),
-                      max(finite_magnitude(x.z), finite_magnitude(x.w)));
-        }
-        const int eq = top_exponent(top) - kTop;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+            top = max(max(top, max(finite_magnitude(x[c].x), finite_magnitude(x[c].y))),
+                      max(finite_magnitude(x[c].z), finite_magnitude(x[c].w)));
+        uint32_t *tops = reinterpret_cast<uint32_t *>(stat);  // free until the first scores
+        tops[slot * kPtRows + r] = top;
+        named_sync(3, 256);
+        const int eq = top_exponent(max(top, tops[(slot ^ 1) * kPtRows + r])) - kTop;
         const float s = pow2(-eq);
-#pragma unroll 2
+#pragma unroll
         for (int c = 0; c < D / 16; ++c) {  // 16-byte chunks of eight halves
-            const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-            const float4 x = live ? __ldg(q4 + slot * (D / 8) + 2 * c) : zero;
-            const float4 y = live ? __ldg(q4 + slot * (D / 8) + 2 * c + 1) : zero;
-            const float e[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            const float e[8] = {x[2 * c].x,     x[2 * c].y,     x[2 * c].z,     x[2 * c].w,
+                                x[2 * c + 1].x, x[2 * c + 1].y, x[2 * c + 1].z, x[2 * c + 1].w};
             __align__(16) __half h[8], lo[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) split_f16(e[j] * s, h[j], lo[j]);
@@ -628,25 +675,40 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             tc_fence_after();
             const int vis = last + 1 - i * kPtKeys;  // keys of the tile the row sees
             const bool whole = __all_sync(0xffffffffu, vis >= kPtKeys);
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            // hidden keys: scores of -inf, written back so that the second reading sees them too
+            float mx[8];
 #pragma unroll
             for (int c = 0; c < 4; c += 2) {
                 uint32_t sv[2][32];
                 tc_ld32_nowait(ts + 32 * c, sv[0]);
                 tc_ld32_nowait(ts + 32 * c + 32, sv[1]);
                 tc_wait_ld();
+                tc_reg_fence(sv[0]);
+                tc_reg_fence(sv[1]);
+                if (!whole) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    tc_reg_fence(sv[h]);
+                    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (whole || 32 * (c + h) + j < vis) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(sv[h][j]));
+                        for (int j = 0; j < 32; ++j)
+                            if (32 * (c + h) + j >= vis) sv[h][j] = 0xFF800000u;
+                        tc_st32(ts + 32 * (c + h), sv[h]);
+                    }
+                    tc_wait_st();
                 }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float u = __uint_as_float(sv[h][j]), v = __uint_as_float(sv[h][j + 1]);
+                        float &best = mx[(j >> 1) & 7];
+                        best = c == 0 && h == 0 && j < 16 ? fmaxf(u, v) : max3(best, u, v);
+                    }
             }
-            const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+            const float m = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * sl2;
             const float shift_p = static_cast<float>(kTop) - (m == -INFINITY ? 0.f : m);
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
+            const uint64_t scale2 = pair_of(sl2, sl2), shift2 = pair_of(shift_p, shift_p);
+            uint64_t sum2[4] = {};
+#pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t sv[32], pv[32];
                 tc_ld32_nowait(ts + 32 * c, sv);
@@ -654,19 +716,16 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                 tc_reg_fence(sv);
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    float x = exp2_approx(fmaf(__uint_as_float(sv[2 * j]), sl2, shift_p));
-                    float y = exp2_approx(fmaf(__uint_as_float(sv[2 * j + 1]), sl2, shift_p));
-                    if (!whole) {
-                        x = 32 * c + 2 * j < vis ? x : 0.f;
-                        y = 32 * c + 2 * j + 1 < vis ? y : 0.f;
-                    }
-                    sum[j & 1] += x;
-                    sum[2 + (j & 1)] += y;
-                    split_f16x2(x, y, pv[j], pv[16 + j]);
+                    const float2 y =
+                        of_pair(fma_pair(pair_of(__uint_as_float(sv[2 * j]), __uint_as_float(sv[2 * j + 1])), scale2, shift2));
+                    const uint64_t e2 = pair_of(exp2_approx(y.x), exp2_approx(y.y));
+                    sum2[j & 3] = add_pair(sum2[j & 3], e2);
+                    split_f16x2(e2, pv[j], pv[16 + j]);
                 }
                 tc_st32(ts + 32 * c, pv);
             }
-            stat[(((i >> 1) & 1) * 2 + slot) * kPtRows + r] = make_float2(m, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+            const float2 sum = of_pair(add_pair(add_pair(sum2[0], sum2[1]), add_pair(sum2[2], sum2[3])));
+            stat[(((i >> 1) & 1) * 2 + slot) * kPtRows + r] = make_float2(m, sum.x + sum.y);
             mbar_arrive(&st_full[slot]);
             tc_wait_st();
             tc_fence_before();
@@ -680,7 +739,6 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         bool ok = true;
 #pragma unroll 1
         for (int i = slot; i < steps; i += 2) {
-            const int k0 = (NT == 2 ? i >> 1 : i) * kPtKeys;
             ok = __all_sync(0xffffffffu, wait(&s_full[slot], (i >> 1) & 1));
             if (!ok) break;
             tc_fence_after();
@@ -690,7 +748,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             tc_wait_ld();
 #pragma unroll
             for (int c = 0; c < 4; ++c) tc_reg_fence(sv[c]);
-            const int vis = last + 1 - k0;  // keys of the tile the row sees
+            const int vis = last + 1 - (NT == 2 ? i >> 1 : i) * kPtKeys;  // keys of the tile the row sees
             const bool whole = __all_sync(0xffffffffu, vis >= kPtKeys);
             if (!whole) {
 #pragma unroll
@@ -778,7 +836,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             // its columns over through the ring (no copy or product uses it any more)
             float2 *stat = reinterpret_cast<float2 *>(base);  // over Q: every product with it is complete
             float *xch = reinterpret_cast<float *>(base + Ge::kOffRing) + slot * (D / 2) * kPtRows;
-            asm volatile("bar.sync 1, 256;" ::: "memory");  // both slots' products are complete
+            named_sync(1, 256);  // both slots' products are complete
             stat[slot * kPtRows + r] = make_float2(m, mine ? l : 0.f);
             if (ok && mine) {
 #pragma unroll 1
@@ -791,7 +849,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                     for (int j = 0; j < 32; ++j) xch[(32 * c + j) * kPtRows + r] = __uint_as_float(o[j]);
                 }
             }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            named_sync(1, 256);
             const float2 other = stat[(slot ^ 1) * kPtRows + r];
             m_row = fmaxf(m, other.x);
             const float mm = m_row == -INFINITY ? 0.f : m_row;
@@ -800,6 +858,8 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             l_row = (mine ? l * f_own : 0.f) + other.y * f_other;
         }
         const float inv = l_row != 0.f ? 1.0f / l_row : 0.f;  // a row that sees no key: zeros
+        // NT = 2: over the slot's query tile; NT = 1: in the ring behind what the slots exchanged
+        unsigned char *stage = base + (NT == 2 ? slot * Ge::kTile : Ge::kOffRing + D * kPtRows * 4);
         if (ok) {
             const bool any_bad = bad[4 * kMaskedTiles] != 0;
             const float *got = reinterpret_cast<const float *>(base + Ge::kOffRing) + (slot ^ 1) * (D / 2) * kPtRows;
@@ -823,14 +883,28 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                     x[j] *= inv;
                 }
                 if (any_bad && live) add_cleared(x, 32 * (c0 + c), m_row, inv);
-                if (live) {
+                if (sp.parts == 1) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-                        *reinterpret_cast<uint4 *>(dst + 32 * (c0 + c) + j) =
-                            make_uint4(pack_pair<T>(x[j], x[j + 1]), pack_pair<T>(x[j + 2], x[j + 3]),
-                                       pack_pair<T>(x[j + 4], x[j + 5]), pack_pair<T>(x[j + 6], x[j + 7]));
+                    for (int j = 0; j < 4; ++j)
+                        *staged(stage, 4 * (c0 + c) + j) =
+                            make_uint4(pack_pair<T>(x[8 * j], x[8 * j + 1]), pack_pair<T>(x[8 * j + 2], x[8 * j + 3]),
+                                       pack_pair<T>(x[8 * j + 4], x[8 * j + 5]), pack_pair<T>(x[8 * j + 6], x[8 * j + 7]));
+                } else if (live) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<float4 *>(sp.part_o + part_row * D + 32 * (c0 + c) + j) =
+                            make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
                 }
             }
+        }
+        if (sp.parts > 1) {
+            if (live && slot == 0) sp.part_ml[part_row] = make_float2(m_row, l_row);
+        } else if constexpr (NT == 2) {
+            named_sync(2 + slot, 128);
+            if (ok && some) store_rows(stage, t0 + slot * BQ, r, 128);
+        } else {
+            named_sync(1, 256);
+            if (ok && some) store_rows(stage, t0, 128 * slot + r, 256);
         }
     }
     tc_fence_before();
@@ -851,8 +925,68 @@ bool row_map(CUtensorMap *m, bool bf16, const void *base, int64_t D, int64_t hea
                       box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// The parts of each row joined: kPtJoinCtas CTAs per (query tile, KV head), a warp per row.
+constexpr int kPtJoinThreads = 256, kPtJoinCtas = 8;
+template <typename T, int D>
+__global__ void __launch_bounds__(kPtJoinThreads) packed_join_kernel(const PackedArgs a, const SplitView sp) {
+    constexpr int E = D / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, BQ = kPtRows / a.G;
+    const PackedTile p =
+        find_packed_tile(a.cu_q, a.cu_k, a.n_seqs, a.total_q, a.total_k, 1, BQ, blockIdx.x / (a.Hkv * kPtJoinCtas), nullptr);
+    const int at = blockIdx.x / kPtJoinCtas, kvh = at % a.Hkv;
+    grid_wait();
+    if (p.seq < 0) return;
+    const int rows = min(BQ, p.nq - p.tile * BQ) * a.G;
+    const int64_t first = static_cast<int64_t>(at) * sp.parts * kPtRows;
+    for (int r = blockIdx.x % kPtJoinCtas + kPtJoinCtas * warp; r < rows; r += kPtJoinCtas * kPtJoinThreads / 32) {
+        const float2 ml = lane < sp.parts ? __ldcg(sp.part_ml + first + lane * kPtRows + r) : make_float2(-INFINITY, 0.f);
+        const float M = warp_max(ml.x);
+        const float w = ml.y == 0.f ? 0.f : ml.y * exp2_approx(ml.x - (M == -INFINITY ? 0.f : M));
+        const float sum = warp_sum(w);
+        float o[E] = {};
+        for (int i = 0; i < sp.parts; ++i) {
+            const float f = __shfl_sync(0xffffffffu, w, i);
+            if (f == 0.f) continue;  // a part without keys for this row holds nothing
+            const float *src = sp.part_o + (first + i * kPtRows + r) * D + E * lane;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = fmaf(f, __ldcg(src + e), o[e]);
+        }
+        const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+        T *dst = static_cast<T *>(a.out) + (p.q0 + p.tile * BQ + r / a.G) * a.o_tok + (kvh * a.G + r % a.G) * a.o_head;
+#pragma unroll
+        for (int e = 0; e < E; ++e) dst[E * lane + e] = from_f32<T>(o[e] * inv);
+    }
+}
+
+// How a call is cut: query tiles a CTA, parts of the keys, CTAs at most.
+struct PtPlan {
+    int nt, parts;
+    int64_t ctas;
+};
+PtPlan pt_plan(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t G, int64_t Hkv, int32_t dtype) {
+    const int64_t sms = device_sm_count(), BQ = kPtRows / G;
+    PtPlan p = {1, 1, 0};
+    // two query tiles a CTA once such CTAs fill the SMs
+    if (dtype != B200_DTYPE_F32 && total_q / (2 * BQ) * Hkv >= sms) p.nt = 2;
+    const int64_t tiles = most_packed_tiles(n_seqs, total_q, 1, p.nt * BQ) * Hkv;
+    if (p.nt == 1 && tiles > 0) {
+        // as many parts as the SMs allow, each of at least four key tiles of a mean sequence
+        const int64_t keys = total_k / max64(1, n_seqs) / (4 * kPtKeys);
+        p.parts = static_cast<int>(max64(1, min64(8, min64(sms / tiles, keys))));
+    }
+    p.ctas = tiles * p.parts;
+    return p;
+}
+
+size_t split_bytes(int64_t n_seqs, int64_t total_k, int64_t D, int64_t Hkv, int32_t dtype) {
+    if (dtype != B200_DTYPE_F32) return 0;
+    // hi and lo planes of K and V, and the tiles' exponents
+    const size_t n = static_cast<size_t>(total_k * Hkv * D * 8 + (total_k / kPtKeys + n_seqs + 1) * Hkv * 8);
+    return (n + 255) / 256 * 256;
+}
+
 template <typename T, int D, int NT>
-cudaError_t pt_launch(const PackedArgs &a, cudaStream_t st) {
+cudaError_t pt_launch(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) {
     constexpr bool bf16 = __is_same(T, __nv_bfloat16), split = __is_same(T, float);
     using Ge = PtGeometry<D, NT, split ? 2 : 1>;
     auto kern = packed_tc_kernel<T, D, NT>;
@@ -861,10 +995,15 @@ cudaError_t pt_launch(const PackedArgs &a, cudaStream_t st) {
     });
     if (e != cudaSuccess) return e;
     const int BQ = kPtRows / a.G;
-    const int64_t ctas = most_packed_tiles(a.n_seqs, a.total_q, 1, NT * BQ) * a.Hkv;
-    if (ctas > INT32_MAX) return cudaErrorNotSupported;
+    if (plan.ctas > INT32_MAX / kPtJoinCtas) return cudaErrorNotSupported;
     CUtensorMap mq = {}, mk, mv;
     SplitView sp;
+    sp.parts = plan.parts;
+    if (plan.parts > 1) {
+        char *parts = static_cast<char *>(a.ws) + split_bytes(a.n_seqs, a.total_k, D, a.Hkv, a.dtype);
+        sp.part_ml = reinterpret_cast<float2 *>(parts);
+        sp.part_o = reinterpret_cast<float *>(sp.part_ml + plan.ctas * kPtRows);
+    }
     if constexpr (split) {
         const int64_t plane = a.total_k * a.Hkv * D;
         __half *planes = static_cast<__half *>(a.ws);
@@ -876,6 +1015,7 @@ cudaError_t pt_launch(const PackedArgs &a, cudaStream_t st) {
             !row_map(&mk, false, planes, D, a.Hkv, 2 * a.total_k, D, a.Hkv * D, 1, kPtKeys) ||
             !row_map(&mv, false, planes + 2 * plane, D, a.Hkv, 2 * a.total_k, D, a.Hkv * D, 1, kPtKeys))
             return cudaErrorNotSupported;
+        mq = mk;  // not used
         e = b200_launch(packed_split_kernel<D>, dim3(static_cast<unsigned>(tiles)), dim3(kSplitThreads), 0, st, false, a,
                         planes, exps);
         if (e != cudaSuccess) return e;
@@ -885,40 +1025,43 @@ cudaError_t pt_launch(const PackedArgs &a, cudaStream_t st) {
             !row_map(&mv, bf16, a.v, D, a.Hkv, a.total_k, a.v_head, a.v_tok, 1, kPtKeys))
             return cudaErrorNotSupported;
     }
-    return b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPtThreads<T>), Ge::kSmem, st, split, mq, mk, mv, a, sp);
+    e = b200_launch(kern, dim3(static_cast<unsigned>(plan.ctas)), dim3(kPtThreads<T>), Ge::kSmem, st, split, mq, mk, mv, a,
+                    sp);
+    if (e != cudaSuccess || plan.parts == 1) return e;
+    return b200_launch(packed_join_kernel<T, D>, dim3(static_cast<unsigned>(plan.ctas / plan.parts * kPtJoinCtas)),
+                       dim3(kPtJoinThreads), 0, st, true, a, sp);
 }
 
 template <typename T, int D>
-cudaError_t pt_by_tiles(const PackedArgs &a, cudaStream_t st) {
-    if constexpr (__is_same(T, float)) {
-        return pt_launch<T, D, 1>(a, st);
-    } else {
-        // two query tiles a CTA once such CTAs fill the SMs
-        const int64_t pairs = a.total_q * a.G / (2 * kPtRows) * a.Hkv;
-        return pairs >= device_sm_count() ? pt_launch<T, D, 2>(a, st) : pt_launch<T, D, 1>(a, st);
-    }
+cudaError_t pt_by_tiles(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) {
+    if constexpr (!__is_same(T, float))
+        if (plan.nt == 2) return pt_launch<T, D, 2>(a, plan, st);
+    return pt_launch<T, D, 1>(a, plan, st);
 }
 
 template <typename T>
-cudaError_t pt_by_dim(const PackedArgs &a, cudaStream_t st) {
-    return a.D == 128 ? pt_by_tiles<T, 128>(a, st) : pt_by_tiles<T, 64>(a, st);
+cudaError_t pt_by_dim(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) {
+    return a.D == 128 ? pt_by_tiles<T, 128>(a, plan, st) : pt_by_tiles<T, 64>(a, plan, st);
 }
 
 }  // namespace
 
-size_t packed_tc_workspace(int64_t n_seqs, int64_t total_k, int64_t D, int64_t Hkv, int32_t dtype) {
-    if (dtype != B200_DTYPE_F32) return 0;
-    // hi and lo planes of K and V, and the tiles' exponents
-    return static_cast<size_t>(total_k * Hkv * D * 8 + (total_k / kPtKeys + n_seqs + 1) * Hkv * 8);
+size_t packed_tc_workspace(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t D, int64_t Hq, int64_t Hkv,
+                           int32_t dtype) {
+    if (Hq / Hkv > kPtRows) return 0;
+    const PtPlan plan = pt_plan(n_seqs, total_q, total_k, Hq / Hkv, Hkv, dtype);
+    return split_bytes(n_seqs, total_k, D, Hkv, dtype) +
+           (plan.parts > 1 ? static_cast<size_t>(plan.ctas) * kPtRows * (D * 4 + 8) : 0);
 }
 
 cudaError_t packed_tc_launch(const PackedArgs &a, cudaStream_t st) {
     if (a.total_k == 0 || a.G > kPtRows) return cudaErrorNotSupported;
+    const PtPlan plan = pt_plan(a.n_seqs, a.total_q, a.total_k, a.G, a.Hkv, a.dtype);
     switch (a.dtype) {
-        case B200_DTYPE_F16: return pt_by_dim<__half>(a, st);
-        case B200_DTYPE_BF16: return pt_by_dim<__nv_bfloat16>(a, st);
+        case B200_DTYPE_F16: return pt_by_dim<__half>(a, plan, st);
+        case B200_DTYPE_BF16: return pt_by_dim<__nv_bfloat16>(a, plan, st);
     }
-    return pt_by_dim<float>(a, st);
+    return pt_by_dim<float>(a, plan, st);
 }
 
 }  // namespace b200
