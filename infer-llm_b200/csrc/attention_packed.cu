@@ -4,7 +4,8 @@
 // sequence. packed_ffma_kernel computes it with F32 FFMA for every type: 64 rows (tokens
 // times the heads that share a KV head) against 64-key tiles, running maximum and sum,
 // scores and output in registers as 4 x 4 and 4 x D/16 blocks a thread. The FFMA rate
-// bounds it.
+// bounds it. It serves what the tensor-core kernel does not: F32 calls with few keys, more than 128
+// query heads a KV head, strides that a tensor map cannot hold.
 #include "attention_packed.cuh"
 #include "gemv.cuh"
 
@@ -13,6 +14,18 @@ namespace {
 
 constexpr int kPkRows = 64, kPkKeys = 64, kPkThreads = 256;
 constexpr int kPkPad = kPkRows + 4;
+
+B200_DEVICE void load4(const float *p, float (&x)[4]) {
+    const float4 v = __ldg(reinterpret_cast<const float4 *>(p));
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+}
+template <typename T>
+B200_DEVICE void load4(const T *p, float (&x)[4]) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
+    const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(e[i]);
+}
 
 template <int D>
 constexpr size_t packed_smem() {
@@ -33,14 +46,17 @@ __global__ void __launch_bounds__(kPkThreads, 2) packed_ffma_kernel(const Packed
     const int rows = min(kPkRows, p.nq * a.G - p.tile * kPkRows);
     const int r0 = p.tile * kPkRows;
     const T *q = static_cast<const T *>(a.q), *k = static_cast<const T *>(a.k), *v = static_cast<const T *>(a.v);
-    for (int i = tid; i < kPkRows * D; i += kPkThreads) {
-        const int r = i / D, d = i - r * D;
-        float x = 0.f;
+    // four elements a load; lanes take neighbouring rows, so the transposed stores do not collide
+#pragma unroll
+    for (int i0 = 0; i0 < kPkRows * D / 4; i0 += kPkThreads) {
+        const int i = i0 + tid, r = i % kPkRows, d = i / kPkRows * 4;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
         if (r < rows) {
             const int tok = (r0 + r) / a.G, h = kvh * a.G + (r0 + r) % a.G;
-            x = to_f32<T>(q[(p.q0 + tok) * a.q_tok + h * a.q_head + d]);
+            load4(q + (p.q0 + tok) * a.q_tok + h * a.q_head + d, x);
         }
-        qt[d * kPkPad + r] = x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qt[(d + e) * kPkPad + r] = x[e];
     }
     int last[4];  // last key each row sees (relative to the sequence)
 #pragma unroll
@@ -56,12 +72,18 @@ __global__ void __launch_bounds__(kPkThreads, 2) packed_ffma_kernel(const Packed
     const int end = p.nk - p.nq + (r0 + rows - 1) / a.G + 1;  // keys the tile's last row sees
     for (int k0 = 0; k0 < end; k0 += kPkKeys) {
         __syncthreads();
-        for (int i = tid; i < kPkKeys * D; i += kPkThreads) {
-            const int j = i / D, d = i - j * D;
-            const bool ok = k0 + j < end;
+#pragma unroll
+        for (int i0 = 0; i0 < kPkKeys * D / 4; i0 += kPkThreads) {
+            const int i = i0 + tid, j = i % kPkKeys, d = i / kPkKeys * 4;
             const int64_t t = p.k0 + k0 + j;
-            kt[d * kPkPad + j] = ok ? to_f32<T>(k[t * a.k_tok + kvh * a.k_head + d]) : 0.f;
-            vs[i] = ok ? to_f32<T>(v[t * a.v_tok + kvh * a.v_head + d]) : 0.f;
+            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+            if (k0 + j < end) {
+                load4(k + t * a.k_tok + kvh * a.k_head + d, x);
+                load4(v + t * a.v_tok + kvh * a.v_head + d, y);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) kt[(d + e) * kPkPad + j] = x[e];
+            *reinterpret_cast<float4 *>(vs + j * D + d) = make_float4(y[0], y[1], y[2], y[3]);
         }
         __syncthreads();
         float s[4][4] = {};
@@ -138,6 +160,10 @@ __global__ void __launch_bounds__(kPkThreads, 2) packed_ffma_kernel(const Packed
     }
 }
 
+// F32 calls with so few keys in all take the FFMA kernel: one launch of two key tiles at most
+// against the tensor cores' two launches (37 tokens: 12.7 us a call against 17.5).
+bool packed_short(int32_t dtype, int64_t total_k) { return dtype == B200_DTYPE_F32 && total_k <= 2 * kPkKeys; }
+
 template <typename T, int D>
 cudaError_t packed_ffma_launch(const PackedArgs &a, cudaStream_t st) {
     auto kern = packed_ffma_kernel<T, D>;
@@ -165,7 +191,9 @@ extern "C" {
 
 size_t b200_flash_attn_packed_workspace_bytes(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t D, int64_t Hq,
                                               int64_t Hkv, int32_t dtype) {
-    if (n_seqs <= 0 || total_q <= 0 || total_k <= 0 || D <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv) return 0;
+    if (n_seqs <= 0 || total_q <= 0 || total_k <= 0 || D <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv ||
+        packed_short(dtype, total_k))
+        return 0;
     return packed_tc_workspace(n_seqs, total_q, total_k, D, Hq, Hkv, dtype);
 }
 
@@ -215,8 +243,10 @@ int b200_flash_attn_packed(const void *q, int64_t q_tok_stride, int64_t q_head_s
     a.ws = workspace;
     a.status = dev_status;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t tc = packed_tc_launch(a, st);
-    if (tc != cudaErrorNotSupported) return status_of(tc);
+    if (!packed_short(dtype, total_k)) {
+        const cudaError_t tc = packed_tc_launch(a, st);
+        if (tc != cudaErrorNotSupported) return status_of(tc);
+    }
     switch (dtype) {
         case B200_DTYPE_F16: return status_of(packed_by_dim<__half>(a, st));
         case B200_DTYPE_BF16: return status_of(packed_by_dim<__nv_bfloat16>(a, st));

@@ -58,12 +58,13 @@ struct PtGeometry {
     static_assert(PL == 1 || NT == 1, "F32 tiles leave room for one query tile");
     static constexpr uint32_t kBox = kPtKeys * 128;           // 64 elements of 128 rows
     static constexpr uint32_t kTile = (D / 64) * kBox;        // a plane of a 128-row tile of Q, K or V
-    static constexpr int kStages = D == 128 ? (PL == 2 ? 4 : NT == 2 ? 5 : 6) : 8;
+    static constexpr int kStages = D == 128 ? (NT * PL == 2 ? 5 : 6) : 8;
     static constexpr uint32_t kOffRing = NT * PL * kTile;
     static constexpr uint32_t kOffBar = kOffRing + kStages * kTile;
-    static constexpr uint32_t kOffStat = kOffBar + 384;       // F32: (m, l) of a slot's last two steps
-    static constexpr uint32_t kOffBad = kOffStat + (PL == 2 ? 4 * kPtRows * 8 : 0);        // [kMaskedTiles][4] words, then "any"
-    static constexpr size_t kSmem = 1024 + kOffBad + 128;
+    static constexpr uint32_t kOffStat = kOffBar + 384;       // F32: (m, l) of each slot's step
+    static constexpr uint32_t kOffBad = kOffStat + (PL == 2 ? 2 * kPtRows * 8 : 0);  // [kMaskedTiles][4] words, "any"
+    static constexpr size_t kSmem = kOffBad + 128;
+    static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
 };
 
 // K and V tiles of a key-tile sequence, numbered in the order of their first use.
@@ -272,10 +273,9 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     constexpr uint32_t kIdS = idesc_f16(kPtRows, kPtKeys, kBf16, false, false);
     constexpr uint32_t kIdO = idesc_f16(kPtRows, D, kBf16, false, true);
     constexpr int S = Ge::kStages;
-    extern __shared__ unsigned char pt_raw[];
-    const uint32_t raw = smem_addr(pt_raw);
-    const uint32_t sbase = (raw + 1023u) & ~1023u;
-    unsigned char *base = pt_raw + (sbase - raw);
+    extern __shared__ __align__(1024) unsigned char pt_smem[];  // as the swizzled tiles want
+    unsigned char *base = pt_smem;
+    const uint32_t sbase = smem_addr(base);
     uint64_t *bars = reinterpret_cast<uint64_t *>(base + Ge::kOffBar);
     uint64_t *full = bars;            // [S] a plane of a K or V tile landed
     uint64_t *empty = bars + S;       // [S] plane read by its last product
@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         // ---- F32: the output's sum
         if constexpr (SPLIT) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-            float2 *stat = reinterpret_cast<float2 *>(base + Ge::kOffStat);  // [step / 2 % 2][slot][row]
+            float2 *stat = reinterpret_cast<float2 *>(base + Ge::kOffStat);  // [slot][row]
             const int32_t *exps = sp.exps + (split_index(p.k0, p.seq, ta) * a.Hkv + kvh) * 2;
             const int64_t ex_step = static_cast<int64_t>(a.Hkv) * 2;
             // the steps' O added up. Step i holds sum p v = O 2^(m + ev); l counts in 2^m
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                 ok = __all_sync(0xffffffffu, wait(&st_full[sl], (i >> 1) & 1) && wait(&o_final[sl], (i >> 1) & 1));
                 if (!ok) break;
                 tc_fence_after();
-                const float2 st = stat[(((i >> 1) & 1) * 2 + sl) * kPtRows + r];
+                const float2 st = stat[sl * kPtRows + r];
                 const float e = st.x + static_cast<float>(ev);
                 if (i + 1 < steps) ev = __ldg(exps + (i + 1) * ex_step + 1);
                 if (st.x > M) {
@@ -633,7 +633,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     } else if constexpr (SPLIT) {
         // ---- F32 softmax
         asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
-        float2 *stat = reinterpret_cast<float2 *>(base + Ge::kOffStat);  // [step / 2 % 2][slot][row]
+        float2 *stat = reinterpret_cast<float2 *>(base + Ge::kOffStat);  // [slot][row]
         const int32_t *exps = sp.exps + (split_index(p.k0, p.seq, ta) * a.Hkv + kvh) * 2;
         const int64_t ex_step = static_cast<int64_t>(a.Hkv) * 2;
         // the row of Q as hi and lo planes: this warpgroup writes half of its columns
@@ -725,7 +725,9 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                 tc_st32(ts + 32 * c, pv);
             }
             const float2 sum = of_pair(add_pair(add_pair(sum2[0], sum2[1]), add_pair(sum2[2], sum2[3])));
-            stat[(((i >> 1) & 1) * 2 + slot) * kPtRows + r] = make_float2(m, sum.x + sum.y);
+            // the slot's last step has been added up (long since, as a rule), so its (m, l) too
+            if (i >= 2 && !__all_sync(0xffffffffu, wait(&o_empty[slot], ((i >> 1) - 1) & 1))) break;
+            stat[slot * kPtRows + r] = make_float2(m, sum.x + sum.y);
             mbar_arrive(&st_full[slot]);
             tc_wait_st();
             tc_fence_before();
