@@ -24,8 +24,8 @@
 //    KV head as the 16 rows. Tensor throughput is no limit here (128 instructions per
 //    32 KB of cache), which is why this is not a tcgen05 kernel: its M of 128 has no
 //    rows to fill. P enters the second product as two terms, P = hi + lo (each rounded to the
-//    element type), so P is not rounded to 8 or 11 bits: the extra instructions are
-//    hidden under the loads.
+//    element type), so P is not rounded to 8 or 11 bits; up to eight query heads the second
+//    term takes the unused rows 8 .. 15 of the same product.
 //  * F32 caches: FFMA. For the scores a lane takes a quarter of head_dim of one of 8 keys;
 //    for the output it takes head_dim / 32 columns of all 8.
 // Rows past a sequence's end are not read; they and keys of invalid blocks get weight 0.
@@ -222,7 +222,7 @@ struct WarpState {
     static constexpr bool FULL = HB > 8;
     static constexpr int R = FULL ? 2 : 1;  // head rows a lane holds
     uint32_t q[D / 16][2 * R];
-    float o[D / 8][2 * R];
+    float o[D / 8][4];  // head rows g and g + 8; without FULL, row g's shares of P's two terms
     float m[R], l[R];
 
     B200_DEVICE void begin(const PbArgs &a, const Place &p, int h0, int heads, float *, int lane) {
@@ -242,18 +242,18 @@ struct WarpState {
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
 #pragma unroll
-            for (int u = 0; u < 2 * R; ++u) o[i][u] = 0.f;
+            for (int u = 0; u < 4; ++u) o[i][u] = 0.f;
     }
 
     // 16 keys at sk / sv (rows of D elements, 16-byte chunk c of row r at c ^ (r & 7));
     // bit j of `live`: key j takes part.
     B200_DEVICE void keys(uint32_t sk, uint32_t sv, uint32_t live, float sl2, float *, int lane) {
         constexpr int RB = D * 2;
-        float s[2][2 * R];
+        float s[2][2 * R], odd[2][2 * R];  // two sums each: half as long a chain of dependent products
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int u = 0; u < 2 * R; ++u) s[j][u] = 0.f;
+            for (int u = 0; u < 2 * R; ++u) s[j][u] = odd[j][u] = 0.f;
         const int mat = lane >> 3, rr = lane & 7;
         {
             const uint32_t row = sk + ((mat >> 1) * 8 + rr) * RB;
@@ -261,9 +261,13 @@ struct WarpState {
             for (int ks = 0; ks < D / 16; ++ks) {
                 uint32_t kf[4];
                 ldsm4(kf, row + (((2 * ks + (mat & 1)) ^ rr) << 4));
-                mma16<T, FULL>(s[0], q[ks], kf[0], kf[1]);
-                mma16<T, FULL>(s[1], q[ks], kf[2], kf[3]);
+                mma16<T, FULL>(ks & 1 ? odd[0] : s[0], q[ks], kf[0], kf[1]);
+                mma16<T, FULL>(ks & 1 ? odd[1] : s[1], q[ks], kf[2], kf[3]);
             }
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int u = 0; u < 2 * R; ++u) s[j][u] += odd[j][u];
         }
         const int t2 = 2 * (lane & 3);
         uint32_t hi[2 * R], lo[2 * R];  // A fragments of P: [key half][row]
@@ -286,10 +290,9 @@ struct WarpState {
             if (__any_sync(0xffffffffu, mn > m[r])) {
                 l[r] *= al;
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    o[i][2 * r] *= al;
-                    o[i][2 * r + 1] *= al;
-                }
+                for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+                    for (int u = FULL ? 2 * r : 0; u < (FULL ? 2 * r + 2 : 4); ++u) o[i][u] *= al;
             }
             m[r] = mn;
 #pragma unroll
@@ -306,10 +309,16 @@ struct WarpState {
         for (int np = 0; np < D / 16; ++np) {
             uint32_t vf[4];
             ldsm4_t(vf, row + (((2 * np + (mat >> 1)) ^ rr) << 4));
-            mma16<T, FULL>(o[2 * np], hi, vf[0], vf[1]);
-            mma16<T, FULL>(o[2 * np], lo, vf[0], vf[1]);
-            mma16<T, FULL>(o[2 * np + 1], hi, vf[2], vf[3]);
-            mma16<T, FULL>(o[2 * np + 1], lo, vf[2], vf[3]);
+            if constexpr (FULL) {
+                mma16<T, true>(o[2 * np], hi, vf[0], vf[1]);
+                mma16<T, true>(o[2 * np], lo, vf[0], vf[1]);
+                mma16<T, true>(o[2 * np + 1], hi, vf[2], vf[3]);
+                mma16<T, true>(o[2 * np + 1], lo, vf[2], vf[3]);
+            } else {  // the unused rows 8 .. 15 take P's second term
+                const uint32_t both[4] = {hi[0], lo[0], hi[1], lo[1]};
+                mma16<T, true>(o[2 * np], both, vf[0], vf[1]);
+                mma16<T, true>(o[2 * np + 1], both, vf[2], vf[3]);
+            }
         }
     }
 
@@ -323,7 +332,8 @@ struct WarpState {
             const int h = g + 8 * r;
 #pragma unroll
             for (int i = 0; i < D / 8; ++i)
-                *reinterpret_cast<float2 *>(rec + h * D + 8 * i + 2 * t) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+                *reinterpret_cast<float2 *>(rec + h * D + 8 * i + 2 * t) =
+                    FULL ? make_float2(o[i][2 * r], o[i][2 * r + 1]) : make_float2(o[i][0] + o[i][2], o[i][1] + o[i][3]);
             if (t == 0) {
                 rec[HB * D + h] = m[r];
                 rec[HB * D + HB + h] = l[r];
