@@ -106,6 +106,13 @@ struct Scale {
         const uint32_t e = __float_as_uint(expf(y));
         return (static_cast<unsigned long long>((e & 0x7FFFFFu) | 0x800000u) << 17) >> (127u - (e >> 23));
     }
+    // A value below every token whose bin is at most b (b = kBins - 1: of any bin), and one above
+    // those of bin b on: wide enough for the rounding of z and of the bins' edges. One
+    // comparison then rules most tokens out; the exact test takes the rest.
+    B200_DEVICE float below(int b) const { return edge(b + 0.75f) - slack(); }
+    B200_DEVICE float above(int b) const { return edge(b - 0.75f) + slack(); }
+    B200_DEVICE float edge(float b) const { return top + kFloor / kBins / inv_t * b; }
+    B200_DEVICE float slack() const { return 1e-5f * (fabsf(top) - kFloor / inv_t); }
     // the bin nearest to kBins z / kFloor (adding 2^23 leaves the whole number in the low bits)
     B200_DEVICE static int bin(float zz) {
         return min(static_cast<int>(__float_as_uint(fmaf(zz, kBins / kFloor, 8388608.0f)) & 0x3FFu), kBins - 1);
@@ -234,16 +241,15 @@ struct Sampler {
         __syncthreads();
     }
 
-    // Appends the tokens that `member(value, key)` names to this CTA's list.
+    // Appends the tokens that `member(value)` names to this CTA's list.
     template <typename F>
     B200_DEVICE void collect(F member) {
         if (tid == 0) s.listed = 0;
         __syncthreads();
         x.each(0, x.n, tid, kSmThreads, [&](float v, int i) {
-            const uint32_t key = order_key(v);
-            if (member(v, key)) {
+            if (member(v)) {
                 const uint32_t at = atomicAdd(&s.listed, 1u);
-                s.list[at] = key;
+                s.list[at] = order_key(v);
                 s.list_at[at] = static_cast<uint32_t>(i);
             }
         });
@@ -301,26 +307,23 @@ struct Sampler {
         if (bin0 < 0) return false;
         uint32_t lo = 0, hi = order_key(sc.top), n = s.bin_c;
         unsigned long long ac = s.above_c, aw = s.above_w;
-        const auto member = [&](float v, uint32_t key) {
+        // the bin's values lie in an interval a little wider than its edges
+        const float x_lo = sc.below(bin0), x_hi = sc.above(bin0);
+        const auto member = [&](float v) {
+            if (v < x_lo || v > x_hi) return false;
             const float z = sc.z(v);
+            const uint32_t key = order_key(v);
             return z > kFloor && sc.bin(z) == bin0 && key >= lo && key <= hi;
         };
-        if (n > kList) {
-            // the bin's values lie in an interval a little wider than its edges
-            const float width = -kFloor / kBins / sc.inv_t;
-            const float slack = 0.25f * width + 1e-5f * (fabsf(sc.top) + width * kBins);
-            const float x_hi = sc.top - width * (bin0 - 0.5f) + slack, x_lo = sc.top - width * (bin0 + 0.5f) - slack;
-            if (x_hi < sc.top) hi = order_key(x_hi);
-            if (x_lo > -INFINITY && x_lo < sc.top && bin0 < kBins - 1) lo = order_key(x_lo);
-        }
+        if (x_hi < sc.top) hi = order_key(x_hi);
+        if (x_lo > -INFINITY && x_lo < sc.top) lo = order_key(x_lo);
         while (n > kList && lo < hi) {  // split the bin over its bit patterns, descending
             const int shift = max(0, 32 - __clz(static_cast<int>(hi - lo)) - 9);
             cluster_sync();  // nobody reads the histogram any more
             clear_histogram();
             x.each(0, x.n, tid, kSmThreads, [&](float v, int) {
-                const uint32_t key = order_key(v);
-                if (member(v, key)) {
-                    const int b = static_cast<int>((hi - key) >> shift);
+                if (member(v)) {
+                    const int b = static_cast<int>((hi - order_key(v)) >> shift);
                     count(b);
                     if (weights) add_weight(b, sc.weight(v));
                 }
@@ -500,7 +503,9 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
         // a short top-k is drawn from its list, without the bins' weights
         bool weights = by_p && !(by_k && top_k <= kList / 2);
         const auto fill = [&] {
+            const float low = f.sc.below(kBins - 1);
             f.x.each(0, n, tid, kSmThreads, [&](float v, int) {
+                if (v < low) return;
                 const float z = f.sc.z(v);
                 if (z > kFloor) {
                     const int b = f.sc.bin(z);
@@ -519,7 +524,9 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
         else f.find(s.mcnt[tid], s.mwgt[tid], 0, 0, f.share_of(top_p, sum), true);
         const int last = s.bin;
         if (last >= 0 && s.upto_c <= kList) {
-            f.collect([&](float v, uint32_t) {
+            const float low = f.sc.below(last);
+            f.collect([&](float v) {
+                if (v < low) return false;
                 const float z = f.sc.z(v);
                 return z > kFloor && f.sc.bin(z) <= last;
             });
@@ -551,12 +558,14 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
         const int p0 = min(n, warp * piece), p1 = min(n, p0 + piece);
         unsigned long long pw = 0;
         uint32_t pe = 0;
+        // (key 0 keeps the whole row)
+        const float k_value = key ? key_value(key) : -INFINITY, low = f.sc.below(kBins - 1);
         f.x.each(p0, p1, lane, 32, [&](float v, int) {
-            const uint32_t k = order_key(v);
-            if (k > key) {
+            if (v < k_value || v < low) return;
+            if (v > k_value) {
                 const unsigned long long w = f.sc.weight(v);
                 if (w >= least) pw += w;
-            } else if (k == key) {
+            } else {
                 ++pe;
             }
         });
