@@ -1022,7 +1022,7 @@ cudaError_t pt_launch(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) 
         sp.exps = exps;
         sp.total_k = a.total_k;
         const int64_t tiles = most_packed_tiles(a.n_seqs, a.total_k, 1, kPtKeys) * a.Hkv * 2;
-        if (tiles > INT32_MAX || 2 * a.total_k > INT32_MAX ||
+        if (tiles > INT32_MAX || 2 * a.total_k > INT32_MAX - 1024 ||
             !row_map(&mk, false, planes, D, a.Hkv, 2 * a.total_k, D, a.Hkv * D, 1, kPtKeys) ||
             !row_map(&mv, false, planes + 2 * plane, D, a.Hkv, 2 * a.total_k, D, a.Hkv * D, 1, kPtKeys))
             return cudaErrorNotSupported;

@@ -123,6 +123,36 @@ def test_packed_strides_scale_and_growing_scores(cuda, kind):
 
 
 @pytest.mark.parametrize("kind", list(DT))
+def test_packed_other_layouts(cuda, kind):
+    """Head-major K and V, one KV row shared by all heads (stride 0), token-strided Q."""
+    Hq, Hkv, D, ql = 8, 4, 64, [260, 31]
+    T = sum(ql)
+    g = gen(10)
+    q = torch.randn((T, 2, Hq, D), device=cuda, generator=g).to(DT[kind])[:, 1]
+    kv = torch.randn((2, Hkv, T, D), device=cuda, generator=g).to(DT[kind])
+    k, v = kv[0].transpose(0, 1), kv[1].transpose(0, 1)
+    one = torch.randn((T, 1, D), device=cuda, generator=g).to(DT[kind]).expand(T, Hkv, D)
+    for kk, vv in ((k, v), (one, v), (one, one)):
+        got = B.flash_attn_packed(q, kk, vv, cumulative(ql))
+        want, w = packed_exact(q, kk, vv, ql, ql)
+        check(got, want, w, kind, True)
+
+
+@pytest.mark.parametrize("kind", list(DT))
+def test_packed_many_short_sequences(cuda, kind):
+    """More sequences than a warp looks at in one round, many of them empty."""
+    Hq, Hkv, D = 4, 2, 64
+    ql = [(i * 5) % 7 if i % 3 else 0 for i in range(150)] + [200]
+    kl = [n + (i * 11) % 40 if n else 0 for i, n in enumerate(ql)]
+    g = gen(12)
+    q = torch.randn((sum(ql), Hq, D), device=cuda, generator=g).to(DT[kind])
+    k = torch.randn((sum(kl), Hkv, D), device=cuda, generator=g).to(DT[kind])
+    v = torch.randn((sum(kl), Hkv, D), device=cuda, generator=g).to(DT[kind])
+    want, w = packed_exact(q, k, v, ql, kl)
+    check(B.flash_attn_packed(q, k, v, cumulative(ql), cumulative(kl)), want, w, kind, True)
+
+
+@pytest.mark.parametrize("kind", list(DT))
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_packed_hidden_keys_of_any_value(cuda, kind, bad):
     """Non-finite K and V rows that a query does not see leave its row as it is: later keys of
