@@ -156,6 +156,11 @@ B200_DEVICE float2 exp2_poly_pair(float2 x) {
     return make_float2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(tf.x) << 23)),
                        __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(tf.y) << 23)));
 }
+B200_DEVICE uint64_t mul_pair(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 B200_DEVICE float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -342,7 +347,6 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    if (SPLIT) grid_wait();  // the split planes
     const auto col_s = [&](int slot) { return tmem + static_cast<uint32_t>(slot * kPtKeys); };
     const auto col_o = [&](int slot) { return tmem + 256u + static_cast<uint32_t>(slot * 128); };
     const auto wait = [&](uint64_t *bar, uint32_t parity) {
@@ -412,6 +416,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                         tma_load_3d(sbase + x * Ge::kTile + b * Ge::kBox, &tq, 64 * b, kvh * G,
                                     static_cast<int32_t>(p.q0) + t0 + x * BQ, smem_addr(q_full), pol);
             }
+            if (SPLIT) grid_wait();  // the split planes (Q is split here meanwhile)
             int issued = 0;
             const auto tile = [&](const CUtensorMap *map, int t) {
                 for (int h = PL - 1; h >= 0; --h) {  // lo, then hi
@@ -574,6 +579,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             float acc[D], L = 0.f, M = -INFINITY, R = -INFINITY;
 #pragma unroll
             for (int d = 0; d < D; ++d) acc[d] = 0.f;
+            grid_wait();  // the exponents
             int ev = steps > 0 ? __ldg(exps + 1) : 0;
             bool ok = true;
 #pragma unroll 1
@@ -662,18 +668,20 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         const float s = pow2(-eq);
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {  // 16-byte chunks of eight halves
-            const float e[8] = {x[2 * c].x,     x[2 * c].y,     x[2 * c].z,     x[2 * c].w,
-                                x[2 * c + 1].x, x[2 * c + 1].y, x[2 * c + 1].z, x[2 * c + 1].w};
-            __align__(16) __half h[8], lo[8];
+            const uint64_t s2 = pair_of(s, s), e[4] = {pair_of(x[2 * c].x, x[2 * c].y), pair_of(x[2 * c].z, x[2 * c].w),
+                                                       pair_of(x[2 * c + 1].x, x[2 * c + 1].y),
+                                                       pair_of(x[2 * c + 1].z, x[2 * c + 1].w)};
+            uint32_t h[4], lo[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) split_f16(e[j] * s, h[j], lo[j]);
+            for (int j = 0; j < 4; ++j) split_f16x2(mul_pair(e[j], s2), h[j], lo[j]);
             const int chunk = slot * (D / 16) + c;
             unsigned char *at = base + (chunk >> 3) * Ge::kBox + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
-            *reinterpret_cast<uint4 *>(at) = *reinterpret_cast<const uint4 *>(h);
-            *reinterpret_cast<uint4 *>(at + Ge::kTile) = *reinterpret_cast<const uint4 *>(lo);
+            *reinterpret_cast<uint4 *>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4 *>(at + Ge::kTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(q_full);
+        grid_wait();  // the exponents
         const uint32_t ts = col_s(slot) + lanes;
         int ek = slot < steps ? __ldg(exps + slot * ex_step) : 0;
 #pragma unroll 1
