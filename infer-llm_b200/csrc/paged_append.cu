@@ -14,51 +14,54 @@ struct AppendArgs {
     int64_t src_tok[2], src_head[2];  // bytes
     int64_t block_stride, tok_stride, head_stride;  // bytes
     const int32_t *cu, *lens, *table;
-    int64_t table_stride, max_blocks, n_blocks, block_tokens, n_tokens;
-    int32_t n_seqs, chunks, head_chunks, pieces;  // 16-byte chunks of a row / of a head, warps a row
+    int64_t table_stride, max_blocks, n_blocks, n_tokens;
+    uint32_t block_tokens;
+    int32_t n_seqs, chunks, head_chunks;  // 16-byte chunks of a row / of a head
+    int32_t step_heads, step_chunks;      // 32 chunks as whole heads and the rest
     int32_t *status;
+    B200_DEVICE void next(int &h, int &r) const {
+        h += step_heads, r += step_chunks;
+        if (r >= head_chunks) ++h, r -= head_chunks;
+    }
 };
 
 constexpr int kAppendThreads = 128;
 constexpr int kLaneChunks = 4;
 
 __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendArgs a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t w = static_cast<int64_t>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
-    const int64_t t = w / (2 * a.pieces);
+    const int lane = threadIdx.x & 31, kv = blockIdx.z;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
     if (t >= a.n_tokens) return;
-    const int rest = static_cast<int>(w - t * (2 * a.pieces));
-    const int kv = rest & 1, c0 = (rest >> 1) * 32 * kLaneChunks + lane;
+    // Head h and chunk r of it, for chunk c of the row; 32 chunks on is one addition with a carry.
+    const int c0 = blockIdx.y * 32 * kLaneChunks + lane;
+    const int h0 = static_cast<int>(static_cast<unsigned>(c0) / static_cast<unsigned>(a.head_chunks));
+    const int r0 = c0 - h0 * a.head_chunks;
     const char *src = a.src[kv] + t * a.src_tok[kv];
     uint4 x[kLaneChunks];
+    int h = h0, r = r0;
 #pragma unroll
     for (int i = 0; i < kLaneChunks; ++i) {
-        const int c = c0 + 32 * i;
-        if (c < a.chunks) {
-            const int h = c / a.head_chunks;
-            x[i] = __ldg(reinterpret_cast<const uint4 *>(src + h * a.src_head[kv] + (c - h * a.head_chunks) * 16));
-        }
+        if (c0 + 32 * i < a.chunks) x[i] = __ldg(reinterpret_cast<const uint4 *>(src + h * a.src_head[kv] + r * 16));
+        a.next(h, r);
     }
     const int s = warp_find_row(a.cu, a.n_seqs, t);
     if (s < 0) {
         if (lane == 0) set_status(a.status, B200_DEV_BAD_POSITION);
         return;
     }
-    const int64_t pos = static_cast<int64_t>(__ldg(a.lens + s)) - __ldg(a.cu + s + 1) + t;
-    const int64_t slot = pos < 0 ? -1 : pos / a.block_tokens;
+    const int64_t pos = static_cast<int64_t>(__ldg(a.lens + s)) - __ldg(a.cu + s + 1) + t;  // < 2^31: t is a row of s
+    const int64_t slot = pos < 0 ? -1 : static_cast<unsigned>(pos) / a.block_tokens;
     const int64_t blk = slot >= 0 && slot < a.max_blocks ? __ldg(a.table + s * a.table_stride + slot) : -1;
     if (blk < 0 || blk >= a.n_blocks) {
         if (lane == 0) set_status(a.status, B200_DEV_BAD_POSITION);
         return;
     }
     char *dst = a.dst[kv] + blk * a.block_stride + (pos - slot * a.block_tokens) * a.tok_stride;
+    h = h0, r = r0;
 #pragma unroll
     for (int i = 0; i < kLaneChunks; ++i) {
-        const int c = c0 + 32 * i;
-        if (c < a.chunks) {
-            const int h = c / a.head_chunks;
-            *reinterpret_cast<uint4 *>(dst + h * a.head_stride + (c - h * a.head_chunks) * 16) = x[i];
-        }
+        if (c0 + 32 * i < a.chunks) *reinterpret_cast<uint4 *>(dst + h * a.head_stride + r * 16) = x[i];
+        a.next(h, r);
     }
 }
 
@@ -100,16 +103,17 @@ extern "C" int b200_paged_kv_append(const void *k, int64_t k_tok_stride, int64_t
     a.table_stride = table_stride;
     a.max_blocks = max_blocks;
     a.n_blocks = pool->n_blocks;
-    a.block_tokens = pool->block_tokens;
+    a.block_tokens = static_cast<uint32_t>(pool->block_tokens);
     a.n_tokens = n_tokens;
     a.n_seqs = static_cast<int32_t>(n_seqs);
     a.head_chunks = static_cast<int32_t>(pool->head_dim * e / 16);
     a.chunks = static_cast<int32_t>(pool->n_head_kv) * a.head_chunks;
-    a.pieces = (a.chunks + 32 * kLaneChunks - 1) / (32 * kLaneChunks);
+    a.step_heads = 32 / a.head_chunks;
+    a.step_chunks = 32 % a.head_chunks;
     a.status = dev_status;
-    const int64_t warps = n_tokens * 2 * a.pieces;
-    const int64_t ctas = (warps + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
-    if (ctas > INT32_MAX) return B200_ERR_NOT_SUPPORTED;
-    paged_append_kernel<<<static_cast<unsigned>(ctas), kAppendThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    constexpr int kWarps = kAppendThreads / 32, kWarpChunks = 32 * kLaneChunks;
+    const dim3 grid(static_cast<unsigned>((n_tokens + kWarps - 1) / kWarps),
+                    static_cast<unsigned>((a.chunks + kWarpChunks - 1) / kWarpChunks), 2);  // y <= 2^15
+    paged_append_kernel<<<grid, kAppendThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
     return status_of(cudaGetLastError());
 }
