@@ -579,8 +579,10 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             float acc[D], L = 0.f, M = -INFINITY, R = -INFINITY;
 #pragma unroll
             for (int d = 0; d < D; ++d) acc[d] = 0.f;
-            grid_wait();  // the exponents
-            int ev = steps > 0 ? __ldg(exps + 1) : 0;
+            // The exponents. (They are read by plain loads: a load through the read-only path may be moved
+            // ahead of the wait, to where the split kernel is still at work.)
+            grid_wait();
+            int ev = steps > 0 ? __ldcg(exps + 1) : 0;
             bool ok = true;
 #pragma unroll 1
             for (int i = 0; i < steps; ++i) {
@@ -590,7 +592,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                 tc_fence_after();
                 const float2 st = stat[sl * kPtRows + r];
                 const float e = st.x + static_cast<float>(ev);
-                if (i + 1 < steps) ev = __ldg(exps + (i + 1) * ex_step + 1);
+                if (i + 1 < steps) ev = __ldcg(exps + (i + 1) * ex_step + 1);
                 if (st.x > M) {
                     L *= exp2_approx(M - st.x);
                     M = st.x;
@@ -683,11 +685,11 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         mbar_arrive(q_full);
         grid_wait();  // the exponents
         const uint32_t ts = col_s(slot) + lanes;
-        int ek = slot < steps ? __ldg(exps + slot * ex_step) : 0;
+        int ek = slot < steps ? __ldcg(exps + slot * ex_step) : 0;
 #pragma unroll 1
         for (int i = slot; i < steps; i += 2) {
             const float sl2 = a.sl2 * pow2(ek + eq);
-            if (i + 2 < steps) ek = __ldg(exps + (i + 2) * ex_step);
+            if (i + 2 < steps) ek = __ldcg(exps + (i + 2) * ex_step);
             if (!__all_sync(0xffffffffu, wait(&s_full[slot], (i >> 1) & 1))) break;
             tc_fence_after();
             const int vis = last + 1 - i * kPtKeys;  // keys of the tile the row sees

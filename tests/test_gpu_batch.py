@@ -105,6 +105,32 @@ def test_packed_long(cuda, kind, layout):
 
 
 @pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout", ["g2", "g2d64", "g16"])
+@pytest.mark.parametrize("lens", [([1], [5000]), ([3, 40, 1, 0], [6100, 45, 1, 7]), ([200, 9], [1700, 4003])],
+                         ids=["one", "short_beside_long", "chunks"])
+def test_packed_few_rows_long_contexts(cuda, kind, layout, lens):
+    """Few query tiles and many keys, so the keys of a tile are shared out among CTAs, some of
+    which get none; hidden keys that are no numbers."""
+    Hq, Hkv, D = LAYOUTS[layout]
+    ql, kl = lens
+    g = gen(17)
+    q = torch.randn((sum(ql), Hq, D), device=cuda, generator=g).to(DT[kind])
+    k = torch.randn((sum(kl), Hkv, D), device=cuda, generator=g).to(DT[kind])
+    v = (torch.randn((sum(kl), Hkv, D), device=cuda, generator=g) + 0.5).to(DT[kind])
+    want, w = packed_exact(q, k, v, ql, kl)
+    for fill in (0, 0x7C, 0xFF):  # what a workspace held before is never read
+        n = B.lib().b200_flash_attn_packed_workspace_bytes(len(ql), sum(ql), sum(kl), D, Hq, Hkv, list(DT).index(kind))
+        ws = torch.full((n,), fill, dtype=torch.uint8, device=cuda)
+        check(B.flash_attn_packed(q, k, v, cumulative(ql), cumulative(kl), workspace=ws), want, w, kind, True)
+    k[kl[0] - 1], v[kl[0] - 1] = math.nan, math.inf  # seen by the first sequence's last row alone
+    got = B.flash_attn_packed(q, k, v, cumulative(ql), cumulative(kl))
+    rows = [i for i in range(sum(ql)) if i != ql[0] - 1]
+    if rows:
+        check(got[rows], want[rows], w[rows], kind, True)
+    assert not torch.isfinite(got[ql[0] - 1].double()).any()
+
+
+@pytest.mark.parametrize("kind", list(DT))
 def test_packed_strides_scale_and_growing_scores(cuda, kind):
     """Q, K and V as views of one projection output, an output inside a wider tensor, a
     given scale, and scores that grow along the keys (the running maximum moves)."""
