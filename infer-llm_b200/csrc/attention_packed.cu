@@ -161,9 +161,10 @@ __global__ void __launch_bounds__(kPkThreads, 2) packed_ffma_kernel(const Packed
     }
 }
 
-// F32 calls with so few keys in all take the FFMA kernel: one launch of two key tiles at most
-// against the tensor cores' two launches (37 tokens: 12.7 us a call against 17.5).
-bool packed_short(int32_t dtype, int64_t total_k) { return dtype == B200_DTYPE_F32 && total_k <= 2 * kPkKeys; }
+// F32 calls with so few keys in all take the FFMA kernel: one launch of one key tile against the
+// tensor cores' two launches (16 / 8 heads of 128: 64 tokens 24.6 us against 25.6, 100 tokens 36.9
+// against 27.6; the second launch also costs the caller ~3 us).
+bool packed_short(int32_t dtype, int64_t total_k) { return dtype == B200_DTYPE_F32 && total_k <= kPkKeys; }
 
 template <typename T, int D>
 cudaError_t packed_ffma_launch(const PackedArgs &a, cudaStream_t st) {

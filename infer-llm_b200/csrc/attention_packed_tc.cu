@@ -987,12 +987,17 @@ struct PtPlan {
 PtPlan pt_plan(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t G, int64_t Hkv, int32_t dtype) {
     const int64_t sms = device_sm_count(), BQ = kPtRows / G;
     PtPlan p = {1, 1, 0};
-    // two query tiles a CTA once such CTAs fill the SMs
+    // Two query tiles a CTA once such CTAs fill the SMs: below that, one is faster (BF16, 16 / 8 heads of
+    // 128: 2048 tokens 35 us against 41, 4096 tokens 88 against 72; 32 / 8 heads, 2048 tokens: 64 against 47).
     if (dtype != B200_DTYPE_F32 && total_q / (2 * BQ) * Hkv >= sms) p.nt = 2;
     const int64_t tiles = most_packed_tiles(n_seqs, total_q, 1, p.nt * BQ) * Hkv;
     if (p.nt == 1 && tiles > 0) {
-        // as many parts as the SMs allow, each of at least four key tiles of a mean sequence
-        const int64_t keys = total_k / max64(1, n_seqs) / (4 * kPtKeys);
+        // As many parts as the SMs allow, each of so many key tiles of a mean sequence at least that the
+        // shorter chain pays for the join, a launch of ~4 us. A 16-bit tile takes ~1 us, an F32 one ~3 (one
+        // part against the parts taken here: one BF16 token, 1601 keys, 8 / 4 heads 24.6 us against 21.5,
+        // 8001 keys 71 against 26; but 200 tokens, 1500 keys 23.5 against 25.6 in two, so they stay whole.
+        // F32, 16 / 8 heads: 128 tokens, 1128 keys 52 against 50; 512 tokens 36, in two 40).
+        const int64_t keys = total_k / max64(1, n_seqs) / ((dtype == B200_DTYPE_F32 ? 4 : 6) * kPtKeys);
         p.parts = static_cast<int>(max64(1, min64(8, min64(sms / tiles, keys))));
     }
     p.ctas = tiles * p.parts;

@@ -40,7 +40,7 @@ constexpr int kPbThreads = 32 * kPbWarps;
 constexpr int kPbMostCtas = 320;
 constexpr int kJoinThreads = 256;
 constexpr int kCluster = 8;
-constexpr int kClusterKeys = 2048;
+constexpr int kClusterKeys = 4096;
 
 struct PbArgs {
     const void *q = nullptr;
@@ -153,7 +153,6 @@ struct Geometry {
     static constexpr size_t kMerge = static_cast<size_t>(kPbWarps) * kRec * 4;
     static constexpr size_t kQ = sizeof(T) == 4 ? static_cast<size_t>(kPbWarps) * HB * (4 * kQPad + 8) * 4 : 0;
     static constexpr size_t kSmem = kRing + kMerge + kQ + kPbWarps * kStages * 4;
-    static constexpr size_t kSmemCluster = kSmem + kRec * 4;  // and the CTA's record
 };
 
 B200_DEVICE void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -456,7 +455,8 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const PbArgs
     uint32_t *live = reinterpret_cast<uint32_t *>(pb_smem + Ge::kRing + Ge::kMerge + Ge::kQ) + warp * Ge::kStages;
     const uint32_t ring = smem_addr(pb_smem) + warp * Ge::kStages * 2 * Ge::kHalf;
 
-    float *own = reinterpret_cast<float *>(pb_smem + Ge::kSmem);  // CL: this CTA's record
+    // CL: this CTA's record. It takes the ring's place once every warp has read its last sub-tile.
+    float *own = reinterpret_cast<float *>(pb_smem);
     int64_t u0 = 0, u1 = 0;
     Place at = {};  // what is computed
     if constexpr (CL) {
@@ -684,8 +684,11 @@ __global__ void __launch_bounds__(kJoinThreads) paged_batch_join_kernel(const Pb
 
 int pb_max_ctas() { return device_sm_count() * 2 < kPbMostCtas ? device_sm_count() * 2 : kPbMostCtas; }
 
-// few pairs with short tables: a cluster each, no workspace
-bool pb_one_launch(int64_t pairs, int64_t max_keys) { return pairs * kCluster <= pb_max_ctas() && max_keys <= kClusterKeys; }
+// Few pairs with short tables: a cluster each, no workspace.
+bool pb_one_launch(int64_t pairs, int64_t max_keys) {
+    // at most the clusters that run at once: 32 on 148 SMs, as a GPC's last SMs hold no whole cluster
+    return pairs * (kCluster + 1) <= pb_max_ctas() && max_keys <= kClusterKeys;
+}
 
 // heads a block handles: the next instantiated size
 int pb_heads(int64_t G, bool f32) {
@@ -707,12 +710,12 @@ cudaError_t pb_launch(PbArgs a, int64_t Hkv, cudaStream_t st) {
     };
     if (pb_one_launch(pairs, a.max_keys)) {
         auto kern = paged_batch_kernel<T, D, HB, true>;
-        const cudaError_t e = allow(reinterpret_cast<const void *>(kern), Ge::kSmemCluster);
+        const cudaError_t e = allow(reinterpret_cast<const void *>(kern), Ge::kSmem);
         if (e != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(pairs * kCluster));
         cfg.blockDim = dim3(kPbThreads);
-        cfg.dynamicSmemBytes = Ge::kSmemCluster;
+        cfg.dynamicSmemBytes = Ge::kSmem;
         cfg.stream = st;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
