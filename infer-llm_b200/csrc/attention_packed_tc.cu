@@ -33,6 +33,12 @@
 //     step's O starts from zero (lo products first), and a fourth warpgroup adds the steps
 //     up in F32 registers, each with its own row maximum and V exponent. An FFMA kernel has no
 //     such rounding but a 20th of the rate; TF32 products would keep 11 bits.
+// Bound: at long contexts the chain scores -> softmax -> P -> product of a slot, against which the other
+// slot's runs: 8192 BF16 tokens, 32 / 8 heads of 128, 510 us, 1.08 PFLOP/s (66 % of a large library
+// matrix product's rate); the tensor cores are busy 55 to 60 % of the time. 2048 F32 tokens, 16 / 8 heads of
+// 128, 80 us (214 TFLOP/s of the call's, 640 of the three products), the split kernel 7 us of it. Short
+// calls: ~10 us of launch, tensor maps, first copies and epilogue. Two tiles a CTA and P over S take
+// all 512 columns of tensor memory and most of shared memory, hence one CTA an SM.
 // Every mbarrier wait is bounded; one that runs out records B200_DEV_TIMEOUT, and the CTA
 // waits (bounded) for its copies and products and frees its tensor memory.
 #include "attention_packed.cuh"
@@ -219,7 +225,8 @@ B200_DEVICE void split_f16x2(uint64_t v, uint32_t &hi, uint32_t &lo) {
 constexpr int kSplitThreads = 256;
 
 // One CTA: the K or V rows of one key tile and KV head, as hi and lo planes with the tile's
-// exponent. A pass over the bytes: HBM bounds it.
+// exponent. A pass over the bytes: HBM bounds it (2048 keys, 8 heads of 128: 17 MB in, 17 MB out, 7 us
+// with its launch; the attention kernel's start overlaps it).
 template <int D>
 __global__ void __launch_bounds__(kSplitThreads) packed_split_kernel(const PackedArgs a, __half *planes, int32_t *exps) {
     constexpr int V4 = D / 4, PER = kPtKeys * V4 / kSplitThreads;  // float4 a row, a thread
@@ -946,7 +953,8 @@ bool row_map(CUtensorMap *m, bool bf16, const void *base, int64_t D, int64_t hea
                       box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// The parts of each row joined: kPtJoinCtas CTAs per (query tile, KV head), a warp per row.
+// The parts of each row joined, o = sum l_i 2^(m_i - M) o_i / sum l_i 2^(m_i - M): kPtJoinCtas CTAs per
+// (query tile, KV head), a warp per row. A launch and one dependent read bound it (~4 us).
 constexpr int kPtJoinThreads = 256, kPtJoinCtas = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(kPtJoinThreads) packed_join_kernel(const PackedArgs a, const SplitView sp) {

@@ -2,7 +2,10 @@
 // of their sequences. A copy: bytes bound it (each row read once and written once), and
 // for one decode step's few rows the latency of one dependent chain, row -> sequence ->
 // block -> store. A warp takes up to 2 KB of one row of K or V: its loads (four of 16
-// bytes a lane) are issued before the lookups, so the chain and the loads overlap.
+// bytes a lane) are issued before the lookups, so the chain and the loads overlap. Index
+// arithmetic is 32-bit and one division a warp: in 64 bits it took two thirds of the issue
+// slots (4096 F32 rows of 8 heads of 128, 67 MB: 16.2 us, now 14.6, 4.6 TB/s). 64 BF16 rows: 5 us
+// on the device.
 #include "batch.cuh"
 
 namespace b200 {

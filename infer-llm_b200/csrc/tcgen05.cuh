@@ -39,19 +39,6 @@ B200_DEVICE uint64_t desc_mn_sw128_b32(uint32_t saddr, uint32_t lbo) {
     return d;
 }
 
-// Descriptor for an MN-major tile of 16-bit elements with the 128-byte swizzle: each
-// 128-byte row holds 64 consecutive M/N elements of one k; rows k .. k+7 form a 1024-byte
-// atom (stride byte offset 1024); the next 64 M/N elements start `lbo` bytes further
-// (leading byte offset). Stepping K by 16 advances the start address by 2048 bytes.
-B200_DEVICE uint64_t desc_mn_sw128(uint32_t saddr, uint32_t lbo) {
-    uint64_t d = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
-    d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
-    d |= static_cast<uint64_t>(1024 >> 4) << 32;
-    d |= static_cast<uint64_t>(1) << 46;
-    d |= static_cast<uint64_t>(2) << 61;
-    return d;
-}
-
 // Instruction descriptor of kind::f16: as idesc_tf32 below, with A and B both F16 (0)
 // or both BF16 (1).
 constexpr uint32_t idesc_f16(int M, int N, bool bf16, bool a_mn, bool b_mn) {
@@ -86,23 +73,6 @@ B200_DEVICE void tc_mma_tf32_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, u
     asm volatile(
         "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
         " tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
-        : "memory");
-}
-
-// The same products of 16-bit elements (K 16 an instruction); A in tensor memory holds two
-// elements of a row per 32-bit column.
-B200_DEVICE void tc_mma_f16(uint32_t tmem, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(tmem),
-        "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
-        : "memory");
-}
-B200_DEVICE void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(tmem_d),
         "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
         : "memory");
 }
