@@ -8,8 +8,9 @@
 // is sorted: K is found by counting.
 //
 //  * A row belongs to one cluster of C CTAs, each with a contiguous chunk of the vocabulary
-//    kept in its shared memory, so the logits are read from HBM once. The CTAs exchange
-//    maxima, histograms and sums through distributed shared memory; no workspace.
+//    kept in its shared memory, so the logits are read from HBM once; where many rows would queue for
+//    that room, or one has none, the passes read the chunk from L2. The CTAs exchange maxima,
+//    histograms and sums through distributed shared memory; no workspace.
 //  * A histogram over bins of equal width in (x - max) / T, merged over the cluster, gives the bin
 //    in which the k-th token, or the token that completes the nucleus, lies. A weight is added as
 //    three words of 14 bits: 32-bit shared-memory additions run at full rate, 64-bit ones
@@ -21,10 +22,10 @@
 //    split again over its ordered bit patterns. Then the kept weight of each warp's
 //    contiguous piece is summed, and the CTA in whose chunk the drawn sum lies searches
 //    that piece.
-// Bound: for a few rows the chain of about four cluster exchanges (151936 F32 logits: 16 us with one row, 29
-// with 32); for a large batch the instructions of the passes over the held chunks, each token's weight
-// (an exponential and a 64-bit shift) taking ~44 issue slots a warp, beside those chains: 256 rows 213 us,
-// 0.73 TB/s. About 30 rows are in work at once.
+// Bound: for a few rows the chain of about four cluster exchanges (151936 F32 logits: 18 us with one row); for
+// a large batch the instructions of the passes, each token's weight (an exponential and a 64-bit
+// shift) taking ~44 issue slots a warp, beside those chains: 256 rows of mixed filters 160 us, 0.97 TB/s;
+// greedy rows alone 55 us, 2.8 TB/s.
 #include "batch.cuh"
 #include "gemv.cuh"
 
@@ -144,7 +145,24 @@ struct Chunk {
             }
             if (whole + lane < to) fn((*this)[whole + lane], whole + lane);
         } else {
-            for (int i = from + lane; i < to; i += lanes) fn((*this)[i], i);
+            // from L2, as a rule: four loads of 16 bytes a thread in flight
+            constexpr int V = 16 / sizeof(T);
+            const int whole = (reinterpret_cast<uintptr_t>(held) & 15) == 0 ? from + (to - from) / V * V : from;
+            for (int i = from + V * lane; i < whole; i += 4 * V * lanes) {
+                uint4 r[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i + j * V * lanes < whole) r[j] = __ldg(reinterpret_cast<const uint4 *>(held + i + j * V * lanes));
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i + j * V * lanes < whole) {
+                        const T *e = reinterpret_cast<const T *>(&r[j]);
+#pragma unroll
+                        for (int q = 0; q < V; ++q) fn(to_f32<T>(e[q]) + 0.0f, i + j * V * lanes + q);
+                    }
+            }
+#pragma unroll 4
+            for (int i = whole + lane; i < to; i += lanes) fn((*this)[i], i);
         }
     }
 };
@@ -477,8 +495,10 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
     cluster_sync();
     mx = -INFINITY;
     bad = false;
+    uint32_t first = 0;  // the first chunk with the maximum
     for (uint32_t r = 0; r < nc; ++r) {
-        mx = fmaxf(mx, ld_dsmem(dsmem_addr(&s.top, r)));
+        const float top = ld_dsmem(dsmem_addr(&s.top, r));
+        if (top > mx) mx = top, first = r;
         bad |= ld_dsmem_u32(dsmem_addr(&s.bad, r)) != 0;
     }
     if (bad || mx == -INFINITY) {
@@ -490,18 +510,32 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
         return;
     }
     const float inv = 1.0f / temp;
-    const bool cold = !(temp > 0.f) || inv == INFINITY;
-    Sampler<T, HELD> f{a, s, {HELD ? held : src, n}, {mx + 0.0f, cold ? 1.0f : inv}, tid, warp, lane, rank, nc};
-    const bool by_k = !cold && top_k > 0 && top_k < a.vocab, by_p = !cold && top_p < 1.0f;
+    Sampler<T, HELD> f{a, s, {HELD ? held : src, n}, {mx + 0.0f, inv}, tid, warp, lane, rank, nc};
+    if (!(temp > 0.f) || inv == INFINITY) {
+        // the first token with the maximum, without sums (256 held rows of 151936 F32: 74 us, by sums 107)
+        if (rank == first) {
+            int best = INT_MAX;
+            f.x.each(0, n, tid, kSmThreads, [&](float v, int i) {
+                if (v == mx) best = min(best, i);
+            });
+            best = __reduce_min_sync(0xffffffffu, best);
+            if (lane == 0) s.warp_c[warp] = static_cast<uint32_t>(best);
+            __syncthreads();
+            if (warp == 0) {
+                const uint32_t at = __reduce_min_sync(0xffffffffu, s.warp_c[lane % kSmWarps]);
+                if (lane == 0) a.out[row] = static_cast<int32_t>(begin + at);
+            }
+        }
+        cluster_sync();  // no CTA's shared memory goes away while it is read
+        return;
+    }
+    const bool by_k = top_k > 0 && top_k < a.vocab, by_p = top_p < 1.0f;
     const double floor_p = static_cast<double>(fminf(fmaxf(min_p, 0.0f), 1.0f)) * 1099511627776.0;
     const unsigned long long least = static_cast<unsigned long long>(floor_p);
 
     // the kept head: keys above `key`, and the first `ties` equal to it
     uint32_t key = 0, ties = 0;
-    if (cold) {
-        key = order_key(mx + 0.0f);
-        ties = 1;
-    } else if (by_k || by_p) {
+    if (by_k || by_p) {
         // a short top-k is drawn from its list, without the bins' weights
         bool weights = by_p && !(by_k && top_k <= kList / 2);
         const auto fill = [&] {
@@ -688,10 +722,19 @@ cudaError_t sample_launch(SampleArgs a, int64_t rows, cudaStream_t st) {
     int c = 1;
     while (c < kMaxCluster && a.vocab > 2048 * c && rows * c < sms) c *= 2;
     while (c < kMaxCluster && kOwnBytes + (a.vocab + c - 1) / c * sizeof(T) > kHalfShared) c *= 2;
+    const auto bytes = [&] { return kOwnBytes + (a.vocab + c - 1) / c * sizeof(T) + 64 * sizeof(T); };
+    bool held = bytes() <= kMostShared;
+    // Rows of which an SM holds an eighth or two are few at a time, and each waits on its own exchanges. With
+    // more than three rounds of them the passes read the rows again from L2 instead, by fewer CTAs a
+    // row. F32, held in clusters of 8 against 2 or 4 from L2: 64 rows of 151936 74 us against 77 (held), 128
+    // rows 115 against 99, 256 rows 205 against 164 (4), 600 rows 441 against 290 (2) and 307 (4).
+    if (held && c == kMaxCluster && rows * c > 3 * sms * (bytes() <= kHalfShared ? 2 : 1)) {
+        held = false;
+        c = rows * 2 >= 5 * sms ? 2 : 4;
+    }
     a.cluster = c;
     a.chunk = static_cast<int32_t>(((a.vocab + c - 1) / c + 63) / 64 * 64);
-    if (kOwnBytes + static_cast<size_t>(a.chunk) * sizeof(T) <= kMostShared) return sample_launch_as<T, true>(a, rows, st);
-    return sample_launch_as<T, false>(a, rows, st);
+    return held ? sample_launch_as<T, true>(a, rows, st) : sample_launch_as<T, false>(a, rows, st);
 }
 
 }  // namespace

@@ -179,6 +179,28 @@ def test_packed_many_short_sequences(cuda, kind):
 
 
 @pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout", [(32, 8, 64), (16, 8, 128), (24, 8, 64)], ids=["g4d64", "g2d128", "g3d64"])
+def test_packed_many_tiles_with_hidden_keys(cuda, kind, layout):
+    """So many query tiles that a CTA takes two at a time; each sequence's last key is no number and
+    its last row alone sees it."""
+    Hq, Hkv, D = layout
+    ql, kl = [1500, 3, 1100], [1500, 130, 1171]
+    g = gen(19)
+    q = torch.randn((sum(ql), Hq, D), device=cuda, generator=g).to(DT[kind])
+    k = torch.randn((sum(kl), Hkv, D), device=cuda, generator=g).to(DT[kind])
+    v = torch.randn((sum(kl), Hkv, D), device=cuda, generator=g).to(DT[kind])
+    want, w = packed_exact(q, k, v, ql, kl)
+    check(B.flash_attn_packed(q, k, v, cumulative(ql), cumulative(kl)), want, w, kind, True)
+    ends = [i - 1 for i in cumulative(kl)[1:].tolist()]
+    k[ends], v[ends] = math.inf, math.nan
+    got = B.flash_attn_packed(q, k, v, cumulative(ql), cumulative(kl))
+    last = [i - 1 for i in cumulative(ql)[1:].tolist()]
+    rows = [i for i in range(sum(ql)) if i not in last]
+    check(got[rows], want[rows], w[rows], kind, True)
+    assert not torch.isfinite(got[last].double()).any()
+
+
+@pytest.mark.parametrize("kind", list(DT))
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_packed_hidden_keys_of_any_value(cuda, kind, bad):
     """Non-finite K and V rows that a query does not see leave its row as it is: later keys of

@@ -91,6 +91,33 @@ def test_filters(cuda, kind, vocab):
         check(x, *args, u, draw(x, *args, u))
 
 
+@pytest.mark.parametrize("kind,vocab", [(torch.float32, 600001), (torch.bfloat16, 1000003), (torch.float16, 2 ** 21)])
+def test_vocabularies_past_shared_memory(cuda, kind, vocab):
+    """Rows too long to be held on chip, which start at any element."""
+    n = 4
+    x = logits(n, vocab + 1, kind, vocab)[:, 1:]
+    u = np.array([0.02, 0.4, 0.77, 0.995], np.float32)
+    for args in ((1.0, 0, 1.0, 0.0), (0.0, 0, 1.0, 0.0), (0.8, 40, 0.9, 0.01), (1.3, 0, 0.9, 0.0), (0.9, 5000, 0.95, 0.02)):
+        check(x, *args, u, draw(x, *args, u))
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [1, 3, 700, 20011, 151936, 600001])
+def test_greedy_rows(cuda, kind, vocab):
+    """Temperature 0: the first of the largest, wherever it is, among equal ones and zeros of both signs."""
+    x = logits(6, vocab, kind, vocab)
+    x[1, vocab - 1] = x[1].max()
+    x[2] = -1.0
+    x[2, vocab // 2], x[2, vocab - 1] = -0.0, 0.0
+    x[3] = -math.inf
+    x[3, vocab - 1] = -5.0
+    x[4] = 7.0
+    x[5, vocab // 3] = 50.0
+    u = np.full(6, 0.5, np.float32)
+    got = draw(x, 0.0, None, None, None, u)
+    assert list(got) == [int(np.argmax(r)) for r in x.float().cpu().numpy()]
+
+
 @pytest.mark.parametrize("rows", [1, 3, 20, 40, 80, 160, 700])
 def test_row_counts(cuda, rows):
     """Every cluster size gives the same token."""
