@@ -17,15 +17,16 @@
 //    are compare-and-swap loops (16 us a row). Tokens below e^-28 of the likeliest have
 //    weight 0 and are left out everywhere.
 //  * If the bins up to it hold at most kList tokens, as for a head of a few hundred, the first
-//    CTA gathers them, ranks them by comparison and draws among them.
+//    CTA gathers them, sorts them and draws among them. For a short top-k the bins of the threads' own
+//    largest tokens tell where to stop, and nothing else is counted.
 //  * Otherwise the threshold is looked for in its bin alone: its tokens are ranked, or the bin is
 //    split again over its ordered bit patterns. Then the kept weight of each warp's
 //    contiguous piece is summed, and the CTA in whose chunk the drawn sum lies searches
 //    that piece.
-// Bound: for a few rows the chain of about four cluster exchanges (151936 F32 logits: 18 us with one row); for
+// Bound: for a few rows the chain of about four cluster exchanges (151936 F32 logits: 16 us with one row); for
 // a large batch the instructions of the passes, each token's weight (an exponential and a 64-bit
-// shift) taking ~44 issue slots a warp, beside those chains: 256 rows of mixed filters 160 us, 0.97 TB/s;
-// greedy rows alone 55 us, 2.8 TB/s.
+// shift) taking ~44 issue slots a warp, beside those chains. 256 rows of 151936 F32: greedy 55 us (2.8
+// TB/s), top-k 50 88, no filter 124, top-p 0.95 168 to 343 as the row is steep or flat, mixed filters 154.
 #include "batch.cuh"
 #include "gemv.cuh"
 
@@ -261,7 +262,8 @@ struct Sampler {
         __syncthreads();
     }
 
-    // Appends the tokens that `member(value)` names to this CTA's list.
+    // Appends the tokens that `member(value)` names to this CTA's list; s.listed counts those past
+    // its end too.
     template <typename F>
     B200_DEVICE void collect(F member) {
         if (tid == 0) s.listed = 0;
@@ -269,8 +271,10 @@ struct Sampler {
         x.each(0, x.n, tid, kSmThreads, [&](float v, int i) {
             if (member(v)) {
                 const uint32_t at = atomicAdd(&s.listed, 1u);
-                s.list[at] = order_key(v);
-                s.list_at[at] = static_cast<uint32_t>(i);
+                if (at < kList) {
+                    s.list[at] = order_key(v);
+                    s.list_at[at] = static_cast<uint32_t>(i);
+                }
             }
         });
     }
@@ -291,6 +295,20 @@ struct Sampler {
             key = ld_dsmem_u32(dsmem_addr(&s.list[from], r));
             at = ld_dsmem_u32(dsmem_addr(&s.list_at[from], r)) + base;
         }
+        return n;
+    }
+
+    // Appends the tokens of bins 0 to `last`, and returns the lists' length. Ends with a cluster barrier.
+    B200_DEVICE uint32_t collect_bins(int last) {
+        const float low = sc.below(last);
+        collect([&](float v) {
+            if (v < low) return false;
+            const float z = sc.z(v);
+            return z > kFloor && Scale::bin(z) <= last;
+        });
+        cluster_sync();
+        uint32_t n = 0;
+        for (uint32_t r = 0; r < nc; ++r) n += ld_dsmem_u32(dsmem_addr(&s.listed, r));
         return n;
     }
 
@@ -480,6 +498,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
         take(v);
     }
     bad |= temp != temp || u != u || top_p != top_p || min_p != min_p;
+    const float own = mx;
     mx = warp_max(mx);
     bad = __any_sync(0xffffffffu, bad);
     if (lane == 0) s.warp_f[warp] = mx, s.warp_b[warp] = bad;
@@ -536,50 +555,49 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
     // the kept head: keys above `key`, and the first `ties` equal to it
     uint32_t key = 0, ties = 0;
     if (by_k || by_p) {
-        // a short top-k is drawn from its list, without the bins' weights
-        bool weights = by_p && !(by_k && top_k <= kList / 2);
-        const auto fill = [&] {
-            const float low = f.sc.below(kBins - 1);
-            f.x.each(0, n, tid, kSmThreads, [&](float v, int) {
-                if (v < low) return;
-                const float z = f.sc.z(v);
-                if (z > kFloor) {
-                    const int b = f.sc.bin(z);
-                    f.count(b);
-                    if (weights) f.add_weight(b, f.sc.weight(v));
-                }
-            });
+        if (by_k && top_k <= kList / 2) {
+            // Of the threads' largest tokens, top_k lie in bins 0 to s.bin, so the head does. Those bins hold few
+            // more, as a rule, and no pass has to count all tokens.
+            const float z = f.sc.z(own);
+            if (z > kFloor) f.count(f.sc.bin(z));
             cluster_sync();
-            s.mcnt[tid] = f.merged_count();
-            s.mwgt[tid] = weights ? f.merged_weight() : 0ull;
-        };
-        fill();
-        unsigned long long sum = weights && !by_k ? f.cta_sum(s.mwgt[tid]) : 0ull;  // of the row
+            f.find(f.merged_count(), 0, 0, 0, static_cast<unsigned long long>(top_k), false);
+            const int last = s.bin;
+            if (last >= 0 && f.collect_bins(last) <= kList) {
+                if (rank == 0) f.draw_listed(top_k, top_p, 0, least, u, a.out + row);
+                cluster_sync();  // no CTA's shared memory goes away while it is read
+                return;
+            }
+            cluster_sync();  // nobody reads the histogram any more
+            f.clear_histogram();
+        }
+        const float low = f.sc.below(kBins - 1);
+        f.x.each(0, n, tid, kSmThreads, [&](float v, int) {
+            if (v < low) return;
+            const float z = f.sc.z(v);
+            if (z > kFloor) {
+                const int b = f.sc.bin(z);
+                f.count(b);
+                if (by_p) f.add_weight(b, f.sc.weight(v));
+            }
+        });
+        cluster_sync();
+        s.mcnt[tid] = f.merged_count();
+        s.mwgt[tid] = by_p ? f.merged_weight() : 0ull;
+        unsigned long long sum = by_p && !by_k ? f.cta_sum(s.mwgt[tid]) : 0ull;  // of the row
         // the last bin that the head reaches into
         if (by_k) f.find(s.mcnt[tid], s.mwgt[tid], 0, 0, static_cast<unsigned long long>(top_k), false);
         else f.find(s.mcnt[tid], s.mwgt[tid], 0, 0, f.share_of(top_p, sum), true);
         const int last = s.bin;
         if (last >= 0 && s.upto_c <= kList) {
-            const float low = f.sc.below(last);
-            f.collect([&](float v) {
-                if (v < low) return false;
-                const float z = f.sc.z(v);
-                return z > kFloor && f.sc.bin(z) <= last;
-            });
-            cluster_sync();
+            f.collect_bins(last);
             if (rank == 0) f.draw_listed(by_k ? top_k : 0, top_p, sum, least, u, a.out + row);
             cluster_sync();  // no CTA's shared memory goes away while it is read
             return;
         }
-        if (by_p && !weights) {  // a short top-k among many equal tokens
-            weights = true;
-            cluster_sync();  // nobody reads the histogram any more
-            f.clear_histogram();
-            fill();
-        }
         __syncthreads();
         bool cut = false;
-        if (by_k) cut = f.select(static_cast<unsigned long long>(top_k), false, weights);
+        if (by_k) cut = f.select(static_cast<unsigned long long>(top_k), false, by_p);
         if (cut) key = s.key, ties = s.ties, sum = s.sum;
         __syncthreads();
         if (by_p) {
@@ -594,8 +612,10 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
         const int p0 = min(n, warp * piece), p1 = min(n, p0 + piece);
         unsigned long long pw = 0;
         uint32_t pe = 0;
-        // (key 0 keeps the whole row)
-        const float k_value = key ? key_value(key) : -INFINITY, low = f.sc.below(kBins - 1);
+        // (key 0 keeps the whole row; min-p leaves out what lies below its own bin)
+        const float k_value = key ? key_value(key) : -INFINITY;
+        const float low = f.sc.below(least > 0 ? min(kBins - 1, static_cast<int>(logf(fminf(min_p, 1.0f)) * (kBins / kFloor)) + 2)
+                                               : kBins - 1);
         f.x.each(p0, p1, lane, 32, [&](float v, int) {
             if (v < k_value || v < low) return;
             if (v > k_value) {

@@ -146,6 +146,29 @@ def test_ties_and_flat_rows(cuda, vocab):
         check(close, *args, u, draw(close, *args, u))
 
 
+@pytest.mark.parametrize("vocab", [700, 40000, 600001])
+def test_short_top_k_in_odd_orders(cuda, vocab):
+    """A short top-k whose tokens share their logits with many others, or lie side by side, descending or
+    ascending along the row."""
+    u = np.array([0.0, 0.3, 0.6, 0.999], np.float32)
+    i = torch.arange(vocab, device="cuda").float()
+    rows = (torch.zeros(vocab, device="cuda"), (i * 7919 % 5), -(i / 16).floor() * 0.03, (i / 400).floor() * 0.02,
+            torch.where(i < 900, 9.0 + i * 2.0 ** -12, torch.sin(i)))
+    for row in rows:
+        x = row[None].expand(4, -1).contiguous()
+        for args in ((0.9, 7, 1.0, 0.0), (1.0, 200, 0.8, 0.0), (1.3, 256, 1.0, 0.05), (0.7, 100, 0.95, 0.3)):
+            check(x, *args, u, draw(x, *args, u))
+
+
+@pytest.mark.parametrize("min_p", [1e-9, 1e-4, 0.02, 0.5, 1.0, 3.0])
+def test_min_p_alone(cuda, min_p):
+    x = logits(4, 50021, torch.float32, 31)
+    x[1, :100] = x[1].max()
+    u = np.array([0.001, 0.3, 0.6, 0.999], np.float32)
+    for temp in (0.3, 1.0, 2.5):
+        check(x, temp, 0, 1.0, min_p, u, draw(x, temp, None, None, min_p, u))
+
+
 def test_masked_tokens_and_bad_rows(cuda):
     x = logits(8, 5000, torch.float32, 5)
     x[0, 100:] = -math.inf
