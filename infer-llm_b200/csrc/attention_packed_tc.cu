@@ -1,15 +1,17 @@
 // Packed causal attention on the 5th-generation tensor cores, for F16, BF16 and F32.
 //
-// A CTA owns two slots, each a 128-row accumulator: scores S (128 x 128 keys) and output O
-// (128 x D) in tensor memory, and one softmax warpgroup with a thread per row. A step i
-// belongs to slot i % 2:
+// A slot is a 128-row accumulator: scores S (128 x 128 keys) and output O (128 x D) in tensor
+// memory, and one softmax warpgroup with a thread per row. Two slots run on an SM, two of one CTA or
+// one of each of two CTAs. A step i belongs to slot i % SL:
 //   S = Q . K^T           (M 128, N 128 keys, K D; both operands in shared memory)
 //   P = 2^(S sl2 - m)     (softmax warps; 16-bit P written over S in tensor memory)
 //   O += P . V            (M 128, N D, K 128 keys; A = P from tensor memory)
 // While one slot's softmax runs, the tensor cores work for the other. The slots are
-//   NT = 2: two query tiles over the same key tiles (K and V are read once for both);
-//   NT = 1: one query tile, even key tiles in slot 0 and odd ones in slot 1, joined at the
-//           end (half as long a chain for calls with few query tiles).
+//   NT = 2, SL = 2: two query tiles over the same key tiles (K and V are read once for both);
+//   NT = 1, SL = 2: one query tile, even key tiles in slot 0 and odd ones in slot 1, joined at the
+//           end (half as long a chain for calls with few query tiles);
+//   NT = 1, SL = 1: one query tile in one slot, two CTAs an SM (short contexts: one CTA's start and
+//           end run beside the other's steps).
 // With fewer query tiles than SMs and long contexts the key tiles are also cut into `parts`, a CTA
 // each (NT = 1); packed_join_kernel weighs the parts' rows by their sums.
 // A query tile's rows are tokens times the G heads of a KV head (row = token * G + head), as
@@ -37,8 +39,9 @@
 // slot's runs: 8192 BF16 tokens, 32 / 8 heads of 128, 510 us, 1.08 PFLOP/s (66 % of a large library
 // matrix product's rate); the tensor cores are busy 55 to 60 % of the time. 2048 F32 tokens, 16 / 8 heads of
 // 128, 80 us (214 TFLOP/s of the call's, 640 of the three products), the split kernel 7 us of it. Short
-// calls: ~10 us of launch, tensor maps, first copies and epilogue. Two tiles a CTA and P over S take
-// all 512 columns of tensor memory and most of shared memory, hence one CTA an SM.
+// calls: a CTA's start and end, ~6 us (look-up 1, first copies 1.4, last product 0.8 to 1.7, output 2), beside ~0.9
+// us a step: 10 prompts of 1 to 1333 BF16 tokens, 16 / 8 heads of 128, 38 us. Two slots take all 512
+// columns of tensor memory and most of an SM's registers.
 // Every mbarrier wait is bounded; one that runs out records B200_DEV_TIMEOUT, and the CTA
 // waits (bounded) for its copies and products and frees its tensor memory.
 #include "attention_packed.cuh"
@@ -52,32 +55,87 @@ namespace b200 {
 namespace {
 
 constexpr int kPtRows = 128, kPtKeys = 128;
-template <typename T>
-constexpr int kPtThreads = __is_same(T, float) ? 512 : 384;
+template <typename T, int SL>
+constexpr int kPtThreads = 128 + 128 * SL + (__is_same(T, float) ? 128 : 0);
 constexpr int kMaskedTiles = 4;  // key tiles in which some row of a CTA hides keys (at most 256 tokens)
 constexpr float kPtRescale = 8.0f;
 constexpr int kPolyStep = 4;  // 8192 BF16 keys: none 522 us, every 4th pair 504 to 513, every 2nd slower than none
 
-// PL: planes of an operand tile (2: hi and lo of F32)
-template <int D, int NT, int PL>
+// NT: query tiles a CTA; SL: slots; PL: planes of an operand tile (2: hi and lo of F32)
+template <int D, int NT, int SL, int PL>
 struct PtGeometry {
     static_assert(PL == 1 || NT == 1, "F32 tiles leave room for one query tile");
     static constexpr uint32_t kBox = kPtKeys * 128;           // 64 elements of 128 rows
     static constexpr uint32_t kTile = (D / 64) * kBox;        // a plane of a 128-row tile of Q, K or V
-    static constexpr int kStages = D == 128 ? (NT * PL == 2 ? 5 : 6) : 8;
+    // one slot: two CTAs an SM
+    static constexpr int kStages = SL == 1 ? 256 / D : (D == 128 ? (NT * PL == 2 ? 5 : 6) : 8);
     static constexpr uint32_t kOffRing = NT * PL * kTile;
-    static constexpr uint32_t kOffBar = kOffRing + kStages * kTile;
+    static constexpr uint32_t kOffBar = kOffRing + kStages * kTile;  // 44 words, then the CTA's PackedTile
     static constexpr uint32_t kOffStat = kOffBar + 384;       // F32: (m, l) of each slot's step
     static constexpr uint32_t kOffBad = kOffStat + (PL == 2 ? 2 * kPtRows * 8 : 0);  // [kMaskedTiles][4] words, "any"
     static constexpr size_t kSmem = kOffBad + 128;
-    static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
+    static_assert(kSmem <= (SL == 1 ? 113 : 227) * 1024, "shared memory of an SM");
 };
 
 // K and V tiles of a key-tile sequence, numbered in the order of their first use.
-template <int NT>
-B200_DEVICE int plane_k(int t) { return NT == 2 ? 2 * t : (t == 0 ? 0 : 2 * t - 1); }
-template <int NT>
-B200_DEVICE int plane_v(int t, int n) { return NT == 2 ? 2 * t + 1 : t + min(t + 2, n); }
+// PAIRS: K and V of a tile follow one another; else K runs a tile ahead.
+template <bool PAIRS>
+B200_DEVICE int plane_k(int t) { return PAIRS ? 2 * t : (t == 0 ? 0 : 2 * t - 1); }
+template <bool PAIRS>
+B200_DEVICE int plane_v(int t, int n) { return PAIRS ? 2 * t + 1 : t + min(t + 2, n); }
+
+// Tile `at` of the query tiles of all sequences (M tokens each) in the order of their key tiles, most
+// first, so that the last CTAs to start are the shortest (10 prompts of 1 to 1333 BF16 tokens: 39 us against 46 in
+// the sequences' order). A whole warp: a lane a sequence (at most 32), and bisection over the number of key
+// tiles, which takes ~1 us more than find_packed_tile.
+B200_DEVICE PackedTile find_heaviest_tile(const PackedArgs &a, int M, int64_t at, int32_t *status) {
+    const int lane = threadIdx.x & 31;
+    int64_t q0 = 0, k0 = 0;
+    int nq = 0, nk = 0;
+    bool ok = true;
+    if (lane < a.n_seqs) {
+        const bool ok_q = packed_range(a.cu_q, lane, a.total_q, q0, nq), ok_k = packed_range(a.cu_k, lane, a.total_k, k0, nk);
+        ok = ok_q && (ok_k || nq == 0);
+        if (!ok) set_status(status, B200_DEV_BAD_POSITION);
+    }
+    // x / M for x < 2^31 by a product that is at most one too large
+    const unsigned scale = 0xFFFFFFFFu / static_cast<unsigned>(M) + 1u;
+    const auto over_m = [&](unsigned x) {
+        const unsigned y = M == 1 ? x : __umulhi(x, scale);
+        return static_cast<int>(y - (y * M > x ? 1u : 0u));
+    };
+    const int tiles = over_m(static_cast<unsigned>(nq) + static_cast<unsigned>(M) - 1u);
+    // the lane's tiles with at least c key tiles (the last token of tile i sees min(nq, (i + 1) M) + nk - nq keys)
+    const auto with = [&](int c) {
+        const int64_t x = static_cast<int64_t>(c - 1) * kPtKeys - (nk - nq);  // tokens that see fewer
+        if (c <= 0) return tiles;
+        return nq == 0 || nq <= x ? 0 : tiles - min(tiles - 1, over_m(static_cast<unsigned>(max64(0, x))));
+    };
+    PackedTile p;
+    int lo = 0, hi = __reduce_max_sync(0xffffffffu, (nk + kPtKeys - 1) / kPtKeys) + 1;  // key tiles of tile `at`: in [lo, hi)
+    if (static_cast<int64_t>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(tiles))) <= at) return p;
+    while (hi - lo > 1) {
+        const int c = (lo + hi) >> 1;
+        if (static_cast<int64_t>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(with(c)))) > at) lo = c;
+        else hi = c;
+    }
+    const int more = with(hi), same = with(lo) - more;
+    int incl = same;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    const int rank = static_cast<int>(at) - static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(more)));
+    const int l = __ffs(static_cast<int>(__ballot_sync(0xffffffffu, incl > rank))) - 1;
+    p.seq = __shfl_sync(0xffffffffu, ok ? lane : -1, l);
+    p.tile = __shfl_sync(0xffffffffu, tiles - more - same + (rank - (incl - same)), l);
+    p.nq = __shfl_sync(0xffffffffu, nq, l);
+    p.nk = __shfl_sync(0xffffffffu, nk, l);
+    p.q0 = __shfl_sync(0xffffffffu, q0, l);
+    p.k0 = __shfl_sync(0xffffffffu, k0, l);
+    return p;
+}
 
 // Matrix descriptors of 128-byte-swizzled tiles differ only in their low word (address and
 // leading byte offset): 64-byte rows of 8-row atoms 1024 bytes apart, version 1. Forming
@@ -192,6 +250,7 @@ struct SplitView {
     int parts = 1;            // of each query tile's keys
     float *part_o = nullptr;  // [CTA][128][D], with parts > 1
     float2 *part_ml = nullptr;
+    bool by_weight = false;   // query tiles in the order of their key tiles
 };
 constexpr int kTop = 14;  // largest magnitudes in [2^14, 2^15); P <= 1 times 2^14
 
@@ -274,13 +333,16 @@ __global__ void __launch_bounds__(kSplitThreads) packed_split_kernel(const Packe
     }
 }
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kPtThreads<T>, 1)
+template <typename T, int D, int NT, int SL>
+__global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     packed_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                      const __grid_constant__ CUtensorMap tv, const PackedArgs a, const SplitView sp) {
     constexpr bool SPLIT = __is_same(T, float);
     constexpr int PL = SPLIT ? 2 : 1;
-    using Ge = PtGeometry<D, NT, PL>;
+    using Ge = PtGeometry<D, NT, SL, PL>;
+    static_assert(SL == 2 || (NT == 1 && !SPLIT), "one slot holds one query tile");
+    constexpr bool kPairs = NT == 2 || SL == 1, kJoin = NT == 1 && SL == 2;  // kJoin: the slots halve the key tiles
+    constexpr int kColumns = 256 * SL;  // of tensor memory
     constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
     constexpr uint32_t kIdS = idesc_f16(kPtRows, kPtKeys, kBf16, false, false);
     constexpr uint32_t kIdO = idesc_f16(kPtRows, D, kBf16, false, true);
@@ -330,15 +392,32 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     }
     if (threadIdx.x < 4 * kMaskedTiles + 1) bad[threadIdx.x] = 0;
     if (warp == 2) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kColumns)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
 
     const int G = a.G, BQ = kPtRows / G, MT = NT * BQ;  // tokens of a query tile, of the CTA
     const int kvh = blockIdx.x / sp.parts % a.Hkv, part = blockIdx.x % sp.parts;
-    const PackedTile p = find_packed_tile(a.cu_q, a.cu_k, a.n_seqs, a.total_q, a.total_k, 1, MT,
-                                          blockIdx.x / (sp.parts * a.Hkv), a.status);
+    // (one warp looks, while others prepare barriers and tensor memory)
+    PackedTile *found = reinterpret_cast<PackedTile *>(bars + 44);
+    if (warp == 3) {
+        const int64_t at = blockIdx.x / (sp.parts * a.Hkv);
+        const PackedTile f = sp.by_weight ? find_heaviest_tile(a, MT, at, a.status)
+                                          : find_packed_tile(a.cu_q, a.cu_k, a.n_seqs, a.total_q, a.total_k, 1, MT, at, a.status);
+        if (lane == 0) *found = f;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    PackedTile p;
+    p.seq = __shfl_sync(0xffffffffu, found->seq, 0);
+    p.tile = __shfl_sync(0xffffffffu, found->tile, 0);
+    p.nq = __shfl_sync(0xffffffffu, found->nq, 0);
+    p.nk = __shfl_sync(0xffffffffu, found->nk, 0);
+    p.q0 = __shfl_sync(0xffffffffu, found->q0, 0);
+    p.k0 = __shfl_sync(0xffffffffu, found->k0, 0);
     const bool some = p.seq >= 0;                      // not past the last tile
     const int t0 = p.tile * MT;                        // first token
     const int shift = p.nk - p.nq;                     // token t sees keys 0 .. t + shift
@@ -350,12 +429,8 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     const int first_masked = max(0, (t0 + shift + 1) / kPtKeys - ta);
     const int64_t k0 = p.k0 + static_cast<int64_t>(ta) * kPtKeys;  // its first key
 
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const auto col_s = [&](int slot) { return tmem + static_cast<uint32_t>(slot * kPtKeys); };
-    const auto col_o = [&](int slot) { return tmem + 256u + static_cast<uint32_t>(slot * 128); };
+    const auto col_o = [&](int slot) { return tmem + 128u * SL + static_cast<uint32_t>(slot * 128); };
     const auto wait = [&](uint64_t *bar, uint32_t parity) {
         if (wait_poll(bar, parity, nullptr)) return true;
         set_status(a.status, B200_DEV_TIMEOUT);
@@ -412,6 +487,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
 
     if (warp < 4) {
         if constexpr (SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        else if constexpr (SL == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == 0 && lane == 0 && nt > 0) {
             // ---- TMA
@@ -439,7 +515,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                 return true;
             };
             bool ok = true;
-            if (NT == 1) {
+            if (!kPairs) {
                 ok = tile(&tk, 0) && (nt < 2 || tile(&tk, 1));
                 for (int t = 0; t < nt && ok; ++t) ok = tile(&tv, t) && (t + 2 >= nt || tile(&tk, t + 2));
             } else {
@@ -480,7 +556,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             };
             constexpr int KK = kPtKeys / 16, KH = 3 * KK / 4;  // products of a V tile; of P's first part
             const auto issue_s = [&](int i) {
-                const int slot = i & 1, pl = PL * plane_k<NT>(NT == 2 ? i >> 1 : i);
+                const int slot = i % SL, pl = PL * plane_k<kPairs>(NT == 2 ? i >> 1 : i);
                 const uint32_t q = sbase + (NT == 2 ? slot : 0) * Ge::kTile;
                 if (!landed(pl)) return false;
                 tc_fence_after();
@@ -497,9 +573,9 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                 return true;
             };
             bool ok = all(q_full, 0);
-            for (int i = 0; i < min(2, steps) && ok; ++i) ok = issue_s(i);
+            for (int i = 0; i < min(SL, steps) && ok; ++i) ok = issue_s(i);
             for (int i = 0; i < steps && ok; ++i) {
-                const int slot = i & 1, t = NT == 2 ? i >> 1 : i, pl = PL * plane_v<NT>(t, nt);
+                const int slot = i % SL, t = NT == 2 ? i >> 1 : i, pl = PL * plane_v<kPairs>(t, nt);
                 const bool check = t >= first_masked && (NT == 1 || slot == 0);
                 ok = landed(pl) && (!SPLIT || !check || landed(pl + 1));
                 if (!ok) break;
@@ -507,7 +583,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                     if (e) mbar_arrive(&v_ask[t - first_masked]);
                     __syncwarp();
                 }
-                ok = all(&p_part[slot], (i >> 1) & 1) && (!check || all(&v_ok[t - first_masked], 0)) &&
+                ok = all(&p_part[slot], (i / SL) & 1) && (!check || all(&v_ok[t - first_masked], 0)) &&
                      (!SPLIT || i < 2 || all(&o_empty[slot], ((i >> 1) - 1) & 1));
                 if (!ok) break;
                 tc_fence_after();
@@ -520,15 +596,15 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
                     values(slot, true, pl + 1, 0, KK, true);
                     values(slot, false, pl + 1, 0, KK, true);
                 } else {
-                    values(slot, false, pl, 0, KH, i >= 2);
-                    ok = all(&p_full[slot], (i >> 1) & 1);
+                    values(slot, false, pl, 0, KH, i >= SL);
+                    ok = all(&p_full[slot], (i / SL) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     values(slot, false, pl, KH, KK, true);
                 }
                 if (NT == 1 || slot == 1) commit_if(e, &empty[(pl + PL - 1) % S]);
-                if (SPLIT || i + 2 >= steps) commit_if(e, &o_final[slot]);
-                if (i + 2 < steps) ok = issue_s(i + 2);
+                if (SPLIT || i + SL >= steps) commit_if(e, &o_final[slot]);
+                if (i + SL < steps) ok = issue_s(i + SL);
             }
             // no product may still use tensor memory or the ring when the CTA exits
             commit_if(e, idle);
@@ -537,7 +613,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             // ---- V check: rows of the masked tiles that hold Inf or NaN, cleared and noted
             constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
             for (int t = first_masked; t < nt; ++t) {
-                const int pl = PL * plane_v<NT>(t, nt);
+                const int pl = PL * plane_v<kPairs>(t, nt);
                 // the tensor-core warp has seen this phase of `full` and holds it until the
                 // check is done, so its parity is not ambiguous here
                 if (!__all_sync(0xffffffffu, wait(&v_ask[t - first_masked], 0) && wait(&full[pl % S], (pl / S) & 1) &&
@@ -761,13 +837,14 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         }
     } else {
         // ---- softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        if constexpr (SL == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const uint32_t ts = col_s(slot) + lanes, to = col_o(slot) + lanes;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
 #pragma unroll 1
-        for (int i = slot; i < steps; i += 2) {
-            ok = __all_sync(0xffffffffu, wait(&s_full[slot], (i >> 1) & 1));
+        for (int i = slot; i < steps; i += SL) {
+            ok = __all_sync(0xffffffffu, wait(&s_full[slot], (i / SL) & 1));
             if (!ok) break;
             tc_fence_after();
             uint32_t sv[4][32];
@@ -857,9 +934,9 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         tc_fence_after();
         // the row's output: O / l, plus what the cleared V rows would have added
         float m_row = m, l_row = l, f_own = 1.f, f_other = 0.f;
-        constexpr int NC = NT == 2 ? D / 32 : D / 64;  // 32-column pieces this thread writes
-        const int c0 = NT == 2 ? 0 : slot * NC;
-        if constexpr (NT == 1) {
+        constexpr int NC = kJoin ? D / 64 : D / 32;  // 32-column pieces this thread writes
+        const int c0 = kJoin ? slot * NC : 0;
+        if constexpr (kJoin) {
             // the slots' halves of the key tiles, joined: each warpgroup hands the other half of
             // its columns over through the ring (no copy or product uses it any more)
             float2 *stat = reinterpret_cast<float2 *>(base);  // over Q: every product with it is complete
@@ -886,12 +963,12 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
             l_row = (mine ? l * f_own : 0.f) + other.y * f_other;
         }
         const float inv = l_row != 0.f ? 1.0f / l_row : 0.f;  // a row that sees no key: zeros
-        // NT = 2: over the slot's query tile; NT = 1: in the ring behind what the slots exchanged
-        unsigned char *stage = base + (NT == 2 ? slot * Ge::kTile : Ge::kOffRing + D * kPtRows * 4);
+        // over the slot's query tile; kJoin: in the ring behind what the slots exchanged
+        unsigned char *stage = base + (kJoin ? Ge::kOffRing + D * kPtRows * 4 : slot * Ge::kTile);
         if (ok) {
             const bool any_bad = bad[4 * kMaskedTiles] != 0;
             const float *got = reinterpret_cast<const float *>(base + Ge::kOffRing) + (slot ^ 1) * (D / 2) * kPtRows;
-            const bool other_has = NT == 1 && steps > (slot ^ 1);
+            const bool other_has = kJoin && steps > (slot ^ 1);
 #pragma unroll 1
             for (int c = 0; c < NC; ++c) {
                 uint32_t o[32];
@@ -907,7 +984,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
                     x[j] = __uint_as_float(o[j]);
-                    if (NT == 1) x[j] = x[j] * f_own + (other_has ? got[(32 * c + j) * kPtRows + r] * f_other : 0.f);
+                    if (kJoin) x[j] = x[j] * f_own + (other_has ? got[(32 * c + j) * kPtRows + r] * f_other : 0.f);
                     x[j] *= inv;
                 }
                 if (any_bad && live) add_cleared(x, 32 * (c0 + c), m_row, inv);
@@ -927,7 +1004,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
         }
         if (sp.parts > 1) {
             if (live && slot == 0) sp.part_ml[part_row] = make_float2(m_row, l_row);
-        } else if constexpr (NT == 2) {
+        } else if constexpr (!kJoin) {
             named_sync(2 + slot, 128);
             if (ok && some) store_rows(stage, t0 + slot * BQ, r, 128);
         } else {
@@ -939,7 +1016,7 @@ __global__ void __launch_bounds__(kPtThreads<T>, 1)
     __syncthreads();
     if (warp == 2) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
     }
 }
 
@@ -989,15 +1066,22 @@ __global__ void __launch_bounds__(kPtJoinThreads) packed_join_kernel(const Packe
 
 // How a call is cut: query tiles a CTA, parts of the keys, CTAs at most.
 struct PtPlan {
-    int nt, parts;
+    int nt, slots, parts;
     int64_t ctas;
 };
 PtPlan pt_plan(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t G, int64_t Hkv, int32_t dtype) {
     const int64_t sms = device_sm_count(), BQ = kPtRows / G;
-    PtPlan p = {1, 1, 0};
-    // Two query tiles a CTA once such CTAs fill the SMs: below that, one is faster (BF16, 16 / 8 heads of
-    // 128: 2048 tokens 35 us against 41, 4096 tokens 88 against 72; 32 / 8 heads, 2048 tokens: 64 against 47).
-    if (dtype != B200_DTYPE_F32 && total_q / (2 * BQ) * Hkv >= sms) p.nt = 2;
+    PtPlan p = {1, 2, 1, 0};
+    // 16-bit types, us for one tile in two slots / one tile in one slot / two tiles:
+    //  * long contexts: two tiles once such CTAs fill the SMs, else one in two slots (16 / 8 heads of
+    //    128: 2048 tokens 36 / 40 / 41, 4096 tokens 91 / 82 / 73, 8192 tokens 259 / 257 / 228);
+    //  * shorter ones: one slot and two CTAs an SM once the tiles outnumber the SMs: a CTA's start and end, ~6
+    //    us, then run beside another's work (10 prompts of 1 to 1333 tokens 53 / 39 / 45, 32 of 64 27 / 18 / 27,
+    //    16 of 300 53 / 37 / 41, 4 of 1024 53 / 39 / 39; but one of 2048 among short ones 35 / 39 / 41).
+    if (dtype != B200_DTYPE_F32) {
+        if (total_k / max64(1, n_seqs) >= 8 * kPtKeys) p.nt = total_q / (2 * BQ) * Hkv >= sms ? 2 : 1;
+        else if (most_packed_tiles(n_seqs, total_q, 1, BQ) * Hkv > sms) p.slots = 1;
+    }
     const int64_t tiles = most_packed_tiles(n_seqs, total_q, 1, p.nt * BQ) * Hkv;
     if (p.nt == 1 && tiles > 0) {
         // As many parts as the SMs allow, each of so many key tiles of a mean sequence at least that the
@@ -1019,11 +1103,11 @@ size_t split_bytes(int64_t n_seqs, int64_t total_k, int64_t D, int64_t Hkv, int3
     return (n + 255) / 256 * 256;
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int SL>
 cudaError_t pt_launch(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) {
     constexpr bool bf16 = __is_same(T, __nv_bfloat16), split = __is_same(T, float);
-    using Ge = PtGeometry<D, NT, split ? 2 : 1>;
-    auto kern = packed_tc_kernel<T, D, NT>;
+    using Ge = PtGeometry<D, NT, SL, split ? 2 : 1>;
+    auto kern = packed_tc_kernel<T, D, NT, SL>;
     cudaError_t e = once_per_device(reinterpret_cast<const void *>(kern), ATTR_SMEM, [&] {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ge::kSmem));
     });
@@ -1033,6 +1117,8 @@ cudaError_t pt_launch(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) 
     CUtensorMap mq = {}, mk, mv;
     SplitView sp;
     sp.parts = plan.parts;
+    // an order matters to CTAs that wait for others; parts (and the join's order) come with fewer CTAs
+    sp.by_weight = a.n_seqs > 1 && a.n_seqs <= 32 && plan.parts == 1 && plan.ctas > device_sm_count();
     if (plan.parts > 1) {
         char *parts = static_cast<char *>(a.ws) + split_bytes(a.n_seqs, a.total_k, D, a.Hkv, a.dtype);
         sp.part_ml = reinterpret_cast<float2 *>(parts);
@@ -1059,7 +1145,7 @@ cudaError_t pt_launch(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) 
             !row_map(&mv, bf16, a.v, D, a.Hkv, a.total_k, a.v_head, a.v_tok, 1, kPtKeys))
             return cudaErrorNotSupported;
     }
-    e = b200_launch(kern, dim3(static_cast<unsigned>(plan.ctas)), dim3(kPtThreads<T>), Ge::kSmem, st, split, mq, mk, mv, a,
+    e = b200_launch(kern, dim3(static_cast<unsigned>(plan.ctas)), dim3(kPtThreads<T, SL>), Ge::kSmem, st, split, mq, mk, mv, a,
                     sp);
     if (e != cudaSuccess || plan.parts == 1) return e;
     return b200_launch(packed_join_kernel<T, D>, dim3(static_cast<unsigned>(plan.ctas / plan.parts * kPtJoinCtas)),
@@ -1069,8 +1155,10 @@ cudaError_t pt_launch(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) 
 template <typename T, int D>
 cudaError_t pt_by_tiles(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) {
     if constexpr (!__is_same(T, float))
-        if (plan.nt == 2) return pt_launch<T, D, 2>(a, plan, st);
-    return pt_launch<T, D, 1>(a, plan, st);
+        if (plan.nt == 2) return pt_launch<T, D, 2, 2>(a, plan, st);
+    if constexpr (!__is_same(T, float))
+        if (plan.slots == 1) return pt_launch<T, D, 1, 1>(a, plan, st);
+    return pt_launch<T, D, 1, 2>(a, plan, st);
 }
 
 template <typename T>

@@ -88,8 +88,8 @@ B200_DEVICE PackedTile find_packed_tile(const int32_t *cu_q, const int32_t *cu_k
         int64_t q0 = 0;
         int nq = 0;
         if (s < n_seqs && !packed_range(cu_q, s, total_q, q0, nq)) set_status(status, B200_DEV_BAD_POSITION);
-        const int64_t n = (static_cast<int64_t>(nq) * G + M - 1) / M;
-        int64_t incl = n;
+        // (rows fit 31 bits, with room for a tile)
+        int64_t incl = (static_cast<unsigned>(nq) * static_cast<unsigned>(G) + static_cast<unsigned>(M) - 1u) / M;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);

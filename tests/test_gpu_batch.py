@@ -201,6 +201,28 @@ def test_packed_many_tiles_with_hidden_keys(cuda, kind, layout):
 
 
 @pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout", [(32, 8, 64), (16, 8, 128), (24, 8, 64)], ids=["g4d64", "g2d128", "g3d64"])
+@pytest.mark.parametrize("lens", [([2300, 1211], [2300, 1900]), ([1500, 0, 3, 900, 130] * 7, [1501, 9, 3, 900, 100] * 7),
+                                  ([90] * 40, [140] * 40)], ids=["two_tiles", "many", "more_than_lanes"])
+def test_packed_many_tiles_of_any_lengths(cuda, kind, layout, lens):
+    """Long contexts in pairs of tiles, and more sequences than a warp has lanes, some of them with
+    rows that see no key; the first sequence's last key is no number."""
+    Hq, Hkv, D = layout
+    ql, kl = lens
+    g = gen(23)
+    q = torch.randn((sum(ql), Hq, D), device=cuda, generator=g).to(DT[kind])
+    k = torch.randn((sum(kl), Hkv, D), device=cuda, generator=g).to(DT[kind])
+    v = torch.randn((sum(kl), Hkv, D), device=cuda, generator=g).to(DT[kind])
+    want, w = packed_exact(q, k, v, ql, kl)
+    check(B.flash_attn_packed(q, k, v, cumulative(ql), cumulative(kl)), want, w, kind, True)
+    k[kl[0] - 1], v[kl[0] - 1] = math.inf, math.nan
+    got = B.flash_attn_packed(q, k, v, cumulative(ql), cumulative(kl))
+    rows = [i for i in range(sum(ql)) if i != ql[0] - 1]
+    check(got[rows], want[rows], w[rows], kind, True)
+    assert not torch.isfinite(got[ql[0] - 1].double()).any()
+
+
+@pytest.mark.parametrize("kind", list(DT))
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_packed_hidden_keys_of_any_value(cuda, kind, bad):
     """Non-finite K and V rows that a query does not see leave its row as it is: later keys of
