@@ -85,9 +85,14 @@ B200_DEVICE PackedTile find_packed_tile(const int32_t *cu_q, const int32_t *cu_k
     int64_t before = 0;
     for (int base = 0; base < n_seqs; base += 32) {
         const int s = base + lane;
-        int64_t q0 = 0;
-        int nq = 0;
-        if (s < n_seqs && !packed_range(cu_q, s, total_q, q0, nq)) set_status(status, B200_DEV_BAD_POSITION);
+        int64_t q0 = 0, k0 = 0;
+        int nq = 0, nk = 0;
+        bool ok_k = true;  // (both ranges are read at once: one latency)
+        if (s < n_seqs) {
+            const bool ok_q = packed_range(cu_q, s, total_q, q0, nq);
+            ok_k = packed_range(cu_k, s, total_k, k0, nk);
+            if (!ok_q) set_status(status, B200_DEV_BAD_POSITION);
+        }
         // (rows fit 31 bits, with room for a tile)
         int64_t incl = (static_cast<unsigned>(nq) * static_cast<unsigned>(G) + static_cast<unsigned>(M) - 1u) / M;
 #pragma unroll
@@ -103,7 +108,9 @@ B200_DEVICE PackedTile find_packed_tile(const int32_t *cu_q, const int32_t *cu_k
             p.tile = static_cast<int>(end - 1 - at);
             p.q0 = __shfl_sync(0xffffffffu, q0, l);
             p.nq = __shfl_sync(0xffffffffu, nq, l);
-            if (!packed_range(cu_k, p.seq, total_k, p.k0, p.nk)) {
+            p.k0 = __shfl_sync(0xffffffffu, k0, l);
+            p.nk = __shfl_sync(0xffffffffu, nk, l);
+            if (!__shfl_sync(0xffffffffu, static_cast<int>(ok_k), l)) {
                 set_status(status, B200_DEV_BAD_POSITION);
                 p.seq = -1;
             }
