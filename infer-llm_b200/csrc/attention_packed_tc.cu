@@ -36,11 +36,11 @@
 //     up in F32 registers, each with its own row maximum and V exponent. An FFMA kernel has no
 //     such rounding but a 20th of the rate; TF32 products would keep 11 bits.
 // Bound: at long contexts the chain scores -> softmax -> P -> product of a slot, against which the other
-// slot's runs: 8192 BF16 tokens, 32 / 8 heads of 128, 510 us, 1.08 PFLOP/s (66 % of a large library
+// slot's runs: 8192 BF16 tokens, 32 / 8 heads of 128, 504 us, 1.09 PFLOP/s (66 % of a large library
 // matrix product's rate); the tensor cores are busy 55 to 60 % of the time. 2048 F32 tokens, 16 / 8 heads of
 // 128, 80 us (214 TFLOP/s of the call's, 640 of the three products), the split kernel 7 us of it. Short
 // calls: a CTA's start and end, ~6 us (look-up 1, first copies 1.4, last product 0.8 to 1.7, output 2), beside ~0.9
-// us a step: 10 prompts of 1 to 1333 BF16 tokens, 16 / 8 heads of 128, 38 us. Two slots take all 512
+// us a step: 10 prompts of 1 to 1333 BF16 tokens, 16 / 8 heads of 128, 35 us. Two slots take all 512
 // columns of tensor memory and most of an SM's registers.
 // Every mbarrier wait is bounded; one that runs out records B200_DEV_TIMEOUT, and the CTA
 // waits (bounded) for its copies and products and frees its tensor memory.

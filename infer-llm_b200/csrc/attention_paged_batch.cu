@@ -29,7 +29,7 @@
 //    term takes the unused rows 8 .. 15 of the same product.
 //  * F32 caches: FFMA. For the scores a lane takes a quarter of head_dim of one of 8 keys;
 //    for the output it takes head_dim / 32 columns of all 8.
-// Measured: 64 ragged BF16 sequences (132 k keys, 32 / 8 heads of 128, 541 MB) 102 us, 5.3 TB/s, 81 % of
+// Measured: 64 ragged BF16 sequences (132 k keys, 32 / 8 heads of 128, 541 MB) 98 to 102 us, 5.4 TB/s, 82 % of
 // a large copy's rate; 16 F32 sequences (587 MB) 98 us, 6.0 TB/s, 91 %. What is left is the join (~5 us)
 // and, for BF16, the latency of a warp's chain from copy to product. Eight warps an SM issue in 40 % of
 // the cycles.

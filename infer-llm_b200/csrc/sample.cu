@@ -26,7 +26,7 @@
 // Bound: for a few rows the chain of about four cluster exchanges (151936 F32 logits: 16 us with one row); for
 // a large batch the instructions of the passes, each token's weight (an exponential and a 64-bit
 // shift) taking ~44 issue slots a warp, beside those chains. 256 rows of 151936 F32: greedy 55 us (2.8
-// TB/s), top-k 50 88, no filter 124, top-p 0.95 168 to 343 as the row is steep or flat, mixed filters 154.
+// TB/s), top-k 50 88, no filter 124, top-p 0.95 168 to 343 as the row is steep or flat, mixed filters 153.
 #include "batch.cuh"
 #include "gemv.cuh"
 
