@@ -210,7 +210,8 @@ int b200_flash_attn_packed(const void *q, int64_t q_tok_stride, int64_t q_head_s
         return B200_ERR_INVALID_ARGUMENT;
     if (n_seqs == 0 || total_q == 0) return B200_OK;
     if (!q || !out || !cu_q || !cu_k || (total_k > 0 && (!k || !v))) return B200_ERR_INVALID_ARGUMENT;
-    if ((D != 64 && D != 128) || Hq > 65536 || n_seqs >= INT32_MAX || total_q * (Hq / Hkv) > kMostRows || total_k > kMostRows || !rows_aligned16(q, q_tok_stride, q_head_stride, e) ||
+    if ((D != 64 && D != 128) || Hq > 65536 || n_seqs >= INT32_MAX || total_q * (Hq / Hkv) > kMostRows ||
+        total_k > kMostRows || !rows_aligned16(q, q_tok_stride, q_head_stride, e) ||
         !rows_aligned16(k, k_tok_stride, k_head_stride, e) || !rows_aligned16(v, v_tok_stride, v_head_stride, e) ||
         !rows_aligned16(out, out_tok_stride, out_head_stride, e))
         return B200_ERR_NOT_SUPPORTED;

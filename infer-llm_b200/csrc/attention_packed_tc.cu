@@ -16,8 +16,9 @@
 // each (NT = 1); packed_join_kernel weighs the parts' rows by their sums.
 // A query tile's rows are tokens times the G heads of a KV head (row = token * G + head), as
 // many whole tokens as fit 128 rows, so the heads that share keys share every tile.
-// Warp roles: warp 0 TMA, warp 1 tensor cores, warps 2-3 V check, warps 4-11 softmax, and for
-// F32 warps 12-15 the output's sum.
+// Warp roles: warp 0 TMA, warp 1 tensor cores, warps 2-3 V check, then four softmax warps a slot, and
+// for F32 warps 12-15 the output's sum. They share out the CTA's registers (80 + 2 x 120 + 192 = 4 x 128
+// for F32, 88 + 2 x 208 = 3 x 168 with two slots, 56 + 200 = 2 x 128 with one).
 //   * The running maximum moves only when it grows by more than 2^8, so rescaling O is rare
 //     (the result is unchanged: every p is bounded by 2^8). Statistics are F32; P is
 //     rounded to the element type, the sum is taken before that.
