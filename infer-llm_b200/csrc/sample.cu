@@ -38,6 +38,7 @@ constexpr int kSmWarps = kSmThreads / 32;
 constexpr int kBins = 512;   // one a thread
 constexpr int kList = 512;   // tokens ranked directly, one a thread
 constexpr int kMaxCluster = 8;
+constexpr int kMostChunk = 1 << 18;  // tokens a CTA takes: so many words of 14 bits sum up within 32
 constexpr float kFloor = -28.0f;  // 2^40 e^-28 < 1
 static_assert(kBins == kSmThreads && kList == kSmThreads, "one bin and one listed token a thread");
 
@@ -227,7 +228,7 @@ struct Sampler {
     }
     B200_DEVICE void count(int b) { atomicAdd(&s.cnt[b], 1u); }
     B200_DEVICE void add_weight(int b, unsigned long long w) {
-        // a chunk has at most 2^18 tokens: no word overflows
+        // a chunk has at most kMostChunk tokens: no word overflows
         if (w & 0x3FFFu) atomicAdd(&s.wgt[0][b], static_cast<uint32_t>(w) & 0x3FFFu);
         atomicAdd(&s.wgt[1][b], static_cast<uint32_t>(w >> 14) & 0x3FFFu);
         if (w >> 28) atomicAdd(&s.wgt[2][b], static_cast<uint32_t>(w >> 28));
@@ -709,6 +710,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
 constexpr size_t kOwnBytes = (sizeof(SampleShared) + 15) / 16 * 16;
 constexpr size_t kMostShared = 227 * 1024;
 constexpr size_t kHalfShared = 113 * 1024;  // two CTAs an SM: 228 KB less 1 KB for each
+static_assert(kMostShared / 2 < kMostChunk / 2, "rows that fit eight CTAs' shared memory fit four chunks");
 
 template <typename T, bool HELD>
 cudaError_t sample_launch_as(const SampleArgs &a, int64_t rows, cudaStream_t st) {
@@ -750,7 +752,7 @@ cudaError_t sample_launch(SampleArgs a, int64_t rows, cudaStream_t st) {
     // rows 115 against 99, 256 rows 205 against 164 (4), 600 rows 441 against 290 (2) and 307 (4).
     if (held && c == kMaxCluster && rows * c > 3 * sms * (bytes() <= kHalfShared ? 2 : 1)) {
         held = false;
-        c = rows * 2 >= 5 * sms ? 2 : 4;
+        c = rows * 2 >= 5 * sms && a.vocab <= 2 * kMostChunk ? 2 : 4;
     }
     a.cluster = c;
     a.chunk = static_cast<int32_t>(((a.vocab + c - 1) / c + 63) / 64 * 64);
@@ -768,7 +770,7 @@ extern "C" int b200_sample(const void *logits, int64_t row_stride, int64_t n_row
     if (n_rows < 0 || n_vocab <= 0 || row_stride < 0 || !dtype_bytes(dtype)) return B200_ERR_INVALID_ARGUMENT;
     if (n_rows == 0) return B200_OK;
     if (!logits || !u || !temperature || !out_ids) return B200_ERR_INVALID_ARGUMENT;
-    if (n_vocab > (1 << 21) || n_rows > INT32_MAX / kMaxCluster) return B200_ERR_NOT_SUPPORTED;
+    if (n_vocab > kMaxCluster * kMostChunk || n_rows > INT32_MAX / kMaxCluster) return B200_ERR_NOT_SUPPORTED;
     SampleArgs a = {};
     a.logits = logits;
     a.row_stride = row_stride;
