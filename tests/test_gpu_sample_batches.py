@@ -13,6 +13,38 @@ from test_gpu_sample import check, draw, logits
 pytestmark = pytest.mark.gpu
 
 
+def settings(n, seed):
+    rng = np.random.default_rng(seed)
+    return (rng.choice([0.0, 0.6, 1.0, 1.7], n).astype(np.float32), rng.choice([0, 0, 5, 50, 700, 5000], n).astype(np.int32),
+            rng.choice([0.0, 0.5, 0.9, 0.99, 1.0], n).astype(np.float32),
+            rng.choice([0.0, 0.0, 0.02, 1.0], n).astype(np.float32)), rng.random(n).astype(np.float32)
+
+
+def alone(x, args, u, row):
+    return int(draw(x[row:row + 1], *[v[row] for v in args], u[row])[0])
+
+
+@pytest.mark.parametrize("kind,vocab", [(torch.float32, 151936), (torch.float32, 151935), (torch.bfloat16, 200001),
+                                        (torch.float16, 700000)])
+@pytest.mark.parametrize("rows", [120, 400])
+def test_large_batches(cuda, kind, vocab, rows):
+    """Mixed settings; random, flat and stepped rows; rows that start at any element."""
+    x = torch.empty((rows, vocab), device=cuda, dtype=kind)
+    for r in range(0, rows, 40):
+        x[r:r + 40] = logits(40, vocab, kind, rows + r)
+    i = torch.arange(vocab, device=cuda)
+    x[7] = 1.5
+    x[8] = (i * 7919 % 5).to(kind)
+    x[9] = (i * 7919 % 97).to(kind) * 0.25
+    args, u = settings(rows, vocab + rows)
+    got = draw(x, *args, u)
+    pick = sorted({7, 8, 9} | set(np.random.default_rng(1).integers(0, rows, 24).tolist()))
+    for r in pick:
+        assert int(got[r]) == alone(x, args, u, r), (r, [v[r] for v in args], u[r])
+    few = pick[:6] + [7, 8, 9]
+    check(x[few], *[v[few] for v in args], u[few], got[few])
+
+
 @pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("vocab", [524289, 800128])
 @pytest.mark.parametrize("rows", [60, 370, 500])
