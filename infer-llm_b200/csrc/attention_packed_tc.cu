@@ -196,8 +196,8 @@ B200_DEVICE uint64_t add_pair(uint64_t a, uint64_t b) {
     return r;
 }
 // 2^x of two values in FP32 arithmetic, for x <= 8: 2^round(x) by the exponent field times a
-// least-maximum polynomial of the rest in [-1/2, 1/2]. x below -125 gives 2^-125, so tiles
-// that hide keys (x = -inf) do not use it. Degree 3 is within 7.5e-5 (BF16 rounds P to
+// least-maximum polynomial of the rest in [-1/2, 1/2]. x below -125 gives 2^-125, and so does a NaN: it
+// serves tiles that hide no keys (x = -inf) and rows whose scores' maximum is finite. Degree 3 is within 7.5e-5 (BF16 rounds P to
 // 2^-9), degree 4 within 2.6e-6 (F16 to 2^-12).
 template <bool BF16>
 B200_DEVICE float2 exp2_poly_pair(float2 x) {
@@ -229,6 +229,17 @@ B200_DEVICE uint64_t mul_pair(uint64_t a, uint64_t b) {
 B200_DEVICE float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// NaN if one of them is
+B200_DEVICE float max2_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+B200_DEVICE float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -863,15 +874,15 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                     for (int j = 0; j < 32; ++j)
                         if (32 * c + j >= vis) sv[c][j] = 0xFF800000u;
             }
-            float mx[8];
+            float mx[8];  // (a NaN stays: such a row's weights must not go by the polynomial)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) mx[j] = fmaxf(__uint_as_float(sv[0][2 * j]), __uint_as_float(sv[0][2 * j + 1]));
+            for (int j = 0; j < 8; ++j) mx[j] = max2_nan(__uint_as_float(sv[0][2 * j]), __uint_as_float(sv[0][2 * j + 1]));
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
                 for (int j = c == 0 ? 16 : 0; j < 32; j += 2)
-                    mx[(j >> 1) & 7] = max3(mx[(j >> 1) & 7], __uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1]));
-            const float top = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * a.sl2;
+                    mx[(j >> 1) & 7] = max3_nan(mx[(j >> 1) & 7], __uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1]));
+            const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), max3_nan(mx[3], mx[4], mx[5]), max2_nan(mx[6], mx[7])) * a.sl2;
             float alpha = 1.f;
             bool grow = false;
             if (m == -INFINITY) {
@@ -881,7 +892,11 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                 m = top;
                 grow = true;
             }
-            if (__any_sync(0xffffffffu, grow)) {
+            // with a NaN or +inf among its scores a row has no weights, with -inf alone they are 0: not for the polynomial
+            const bool odd = whole && !(fabsf(top) < INFINITY);
+            bool by_poly = whole;
+            if (__any_sync(0xffffffffu, grow || odd)) {
+                by_poly = whole && !__any_sync(0xffffffffu, odd);
                 // every earlier product of this slot completed before its scores did
                 l *= alpha;
 #pragma unroll 1
@@ -922,7 +937,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                     }
                 }
             };
-            if (whole) weigh(std::true_type{});
+            if (by_poly) weigh(std::true_type{});
             else weigh(std::false_type{});
             const float2 two = of_pair(add_pair(add_pair(sum[0], sum[1]), add_pair(sum[2], sum[3])));
             l = two.x + two.y;
