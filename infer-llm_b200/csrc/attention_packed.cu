@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kPkThreads, 2) packed_ffma_kernel(const Packed
 #pragma unroll
         for (int w = 1; w < 16; w <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
         if (r >= rows) continue;
-        const float inv = last[i] >= 0 ? 1.0f / l[i] : 0.f;
+        const float inv = l[i] != 0.f ? 1.0f / l[i] : 0.f;  // no key, or scores of -inf alone: zeros
         T *dst = out + (p.q0 + (r0 + r) / a.G) * a.o_tok + (kvh * a.G + (r0 + r) % a.G) * a.o_head;
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)

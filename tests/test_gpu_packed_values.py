@@ -82,3 +82,7 @@ ROWS = {"short": ([6], [40]), "halves": ([6], [400]), "parts": ([3], [3100]), "o
 @pytest.mark.parametrize("lens", list(ROWS))
 def test_rows_with_scores_of_minus_inf_alone(cuda, kind, lens):
     rows_with_scores_of_minus_inf_alone(kind, *ROWS[lens])
+
+
+def test_f32_few_keys_with_scores_of_minus_inf_alone(cuda):
+    rows_with_scores_of_minus_inf_alone("f32", *ROWS["short"])
