@@ -24,14 +24,18 @@
 //     rounded to the element type, the sum is taken before that.
 //   * Hidden keys of a tile (past a row's last key, of the next sequence, or past the end)
 //     have P = 0, but 0 times a V that is no number is not 0. The V check looks for such
-//     rows in the tiles that hide keys, clears them in shared memory, and notes them; rows that do
-//     see one of them add its term in the epilogue.
+//     rows in the tiles that hide keys, clears them in shared memory, and notes them; 16-bit rows that
+//     do see one of them add its term in the epilogue.
 //   * F32 (NT = 1) runs as three F16 products. With a tile's values scaled by a power of two to a
 //     largest magnitude in [2^14, 2^15), x = hi + lo of two F16 numbers holds 22 bits
 //     of x (and an absolute 2^-39 of the tile's largest), and x y = hi hi + hi lo + lo hi
 //     up to 2^-22. packed_split_kernel writes K and V so, as hi and lo planes with one
 //     exponent per 128-key tile and KV head; Q rows are split by the softmax threads
-//     (an exponent per row), P by construction (p <= 1, times 2^14). The tensor cores
+//     (an exponent per row), P by construction (p <= 1, times 2^14). One exponent does only for rows and
+//     columns of like magnitude: a tile of K or V in which a row's or a column's largest is below 2^-10 of the
+//     tile's, or which holds Inf or NaN, is marked, and a CTA that met one does its rows over with F32
+//     FFMA (attention_packed_ffma.cuh; 2048 tokens, 16 / 8 heads of 128, with one such key 868 us, without 79). So
+//     neither hidden keys nor other columns cost a row its bits. The tensor cores
 //     round their sums toward zero: over a long row that bias reached 1e-5 at 8192 keys. So each
 //     step's O starts from zero (lo products first), and a fourth warpgroup adds the steps
 //     up in F32 registers, each with its own row maximum and V exponent. An FFMA kernel has no
@@ -45,7 +49,7 @@
 // columns of tensor memory and most of an SM's registers.
 // Every mbarrier wait is bounded; one that runs out records B200_DEV_TIMEOUT, and the CTA
 // waits (bounded) for its copies and products and frees its tensor memory.
-#include "attention_packed.cuh"
+#include "attention_packed_ffma.cuh"
 #include "gemv.cuh"
 #include "tcgen05.cuh"
 #include "tma.cuh"
@@ -73,9 +77,10 @@ struct PtGeometry {
     static constexpr uint32_t kOffRing = NT * PL * kTile;
     static constexpr uint32_t kOffBar = kOffRing + kStages * kTile;  // 44 words, then the CTA's PackedTile
     static constexpr uint32_t kOffStat = kOffBar + 384;       // F32: (m, l) of each slot's step
-    static constexpr uint32_t kOffBad = kOffStat + (PL == 2 ? 2 * kPtRows * 8 : 0);  // [kMaskedTiles][4] words, "any"
+    static constexpr uint32_t kOffBad = kOffStat + (PL == 2 ? 2 * kPtRows * 8 : 0);  // [kMaskedTiles][4] words, "any", "wide"
     static constexpr size_t kSmem = kOffBad + 128;
     static_assert(kSmem <= (SL == 1 ? 113 : 227) * 1024, "shared memory of an SM");
+    static_assert(PL == 1 || ffma_smem<D>() <= kOffBar, "rows done over by FFMA");
 };
 
 // K and V tiles of a key-tile sequence, numbered in the order of their first use.
@@ -265,6 +270,14 @@ struct SplitView {
     bool by_weight = false;   // query tiles in the order of their key tiles
 };
 constexpr int kTop = 14;  // largest magnitudes in [2^14, 2^15); P <= 1 times 2^14
+// Rows and columns within 2^10 of their tile's largest: their elements hold 22 bits, or an absolute 2^-29 of
+// the row's and the column's largest.
+constexpr int kSpread = 10;
+// A word of `exps`: the exponent, and whether the tile takes FFMA.
+B200_DEVICE int exps_word(int e, bool wide) { return 2 * e + static_cast<int>(wide); }
+B200_DEVICE int exps_exponent(int word) { return word >> 1; }
+B200_DEVICE bool exps_wide(int word) { return word & 1; }
+constexpr int kMostScale = 100;  // exponents of Q and K that add up past it: their product takes FFMA
 
 // A tile's place in `exps`: increasing along the packed keys for any lengths, since
 // floor(x) + ceil(y) <= floor(x + y) + 1.
@@ -296,14 +309,15 @@ B200_DEVICE void split_f16x2(uint64_t v, uint32_t &hi, uint32_t &lo) {
 constexpr int kSplitThreads = 256;
 
 // One CTA: the K or V rows of one key tile and KV head, as hi and lo planes with the tile's
-// exponent. A pass over the bytes: HBM bounds it (2048 keys, 8 heads of 128: 17 MB in, 17 MB out, 7 us
+// exponent, and whether its rows and columns spread too far for one. A pass over the bytes: HBM bounds it (2048 keys, 8 heads of 128: 17 MB in, 17 MB out, 7 us
 // with its launch; the attention kernel's start overlaps it).
 template <int D>
 __global__ void __launch_bounds__(kSplitThreads) packed_split_kernel(const PackedArgs a, __half *planes, int32_t *exps) {
     constexpr int V4 = D / 4, PER = kPtKeys * V4 / kSplitThreads;  // float4 a row, a thread
-    __shared__ uint32_t warp_top[kSplitThreads / 32];
+    constexpr int W = kSplitThreads / 32;
+    __shared__ uint32_t warp_top[W], warp_low[W], warp_any[W], col_top[W][D], col_low[D / 32];
     grid_launch_dependents();
-    const int kvh = (blockIdx.x >> 1) % a.Hkv, is_v = blockIdx.x & 1;
+    const int kvh = (blockIdx.x >> 1) % a.Hkv, is_v = blockIdx.x & 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const PackedTile p = find_packed_tile(a.cu_k, a.cu_k, a.n_seqs, a.total_k, a.total_k, 1, kPtKeys,
                                           (blockIdx.x >> 1) / a.Hkv, nullptr);
     if (p.seq < 0) return;
@@ -311,23 +325,63 @@ __global__ void __launch_bounds__(kSplitThreads) packed_split_kernel(const Packe
     const int64_t tok = is_v ? a.v_tok : a.k_tok;
     const int rows = min(kPtKeys, p.nk - p.tile * kPtKeys);
     const int64_t first = p.k0 + static_cast<int64_t>(p.tile) * kPtKeys;
+    // magnitudes: the largest finite one (`top`), of each row and column, the least of those that
+    // are not zero (`low`), and of any kind (`any`)
+    const auto nonzero = [](uint32_t m) { return m ? m : 0xFFFFFFFFu; };
     float4 x[PER];
-    uint32_t top = 0;
+    uint32_t low = 0xFFFFFFFFu, any = 0, top = 0, col[4] = {};
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int e = threadIdx.x + i * kSplitThreads, r = e / V4, c = e % V4;
         x[i] = r < rows ? __ldg(reinterpret_cast<const float4 *>(src + (first + r) * tok) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        top = max(max(top, max(finite_magnitude(x[i].x), finite_magnitude(x[i].y))),
-                  max(finite_magnitude(x[i].z), finite_magnitude(x[i].w)));
+        const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t row = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t m = finite_magnitude(v[j]);
+            any = max(any, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+            row = max(row, m);
+            col[j] = max(col[j], m);
+        }
+        if constexpr (V4 == 32) {
+            row = __reduce_max_sync(0xffffffffu, row);
+        } else {  // two rows a warp
+#pragma unroll
+            for (int o = V4 / 2; o > 0; o >>= 1) row = max(row, __shfl_xor_sync(0xffffffffu, row, o));
+        }
+        low = min(low, nonzero(row));
+        top = max(top, row);
     }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (V4 == 16) col[j] = max(col[j], __shfl_xor_sync(0xffffffffu, col[j], 16));
+        if (lane < V4) col_top[warp][4 * lane + j] = col[j];
+    }
+    if constexpr (V4 == 16) {
+        low = min(low, __shfl_xor_sync(0xffffffffu, low, 16));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    }
+    any = __reduce_max_sync(0xffffffffu, any);
+    if (lane == 0) warp_top[warp] = top, warp_low[warp] = low, warp_any[warp] = any;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kSplitThreads / 32; ++w) top = max(top, warp_top[w]);
-    const int e = top_exponent(top);
+    for (int w = 0; w < W; ++w) top = max(top, warp_top[w]);
+    const int e = top ? top_exponent(top) : kTop;  // (a tile of zeros: any)
     const float s = pow2(kTop - e);
-    if (threadIdx.x == 0) exps[(split_index(p.k0, p.seq, p.tile) * a.Hkv + kvh) * 2 + is_v] = e - kTop;
+    if (threadIdx.x < D) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) c = max(c, col_top[w][threadIdx.x]);
+        c = __reduce_min_sync(0xffffffffu, nonzero(c));
+        if (lane == 0) col_low[warp] = c;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 0; w < W; ++w) low = min(low, warp_low[w]), any = max(any, warp_any[w]);
+        for (int w = 0; w < D / 32; ++w) low = min(low, col_low[w]);
+        const bool wide = any >= 0x7F800000u || static_cast<int>(min(low, 0x7F800000u) >> 23) - 127 < e - kSpread;
+        exps[(split_index(p.k0, p.seq, p.tile) * a.Hkv + kvh) * 2 + is_v] = exps_word(e - kTop, wide);
+    }
     const int64_t plane = a.total_k * a.Hkv * D;
     __half *dst = planes + (is_v ? 2 * plane : 0) + kvh * D;
 #pragma unroll
@@ -402,7 +456,8 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
         for (const CUtensorMap *m : {&tq, &tk, &tv})
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
     }
-    if (threadIdx.x < 4 * kMaskedTiles + 1) bad[threadIdx.x] = 0;
+    if (threadIdx.x < 4 * kMaskedTiles + 2) bad[threadIdx.x] = 0;
+    uint32_t &any_wide = bad[4 * kMaskedTiles + 1];  // F32: a key tile was not held by two F16 numbers
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kColumns)
                      : "memory");
@@ -677,8 +732,8 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             // The exponents. (They are read by plain loads: a load through the read-only path may be moved
             // ahead of the wait, to where the split kernel is still at work.)
             grid_wait();
-            int ev = steps > 0 ? __ldcg(exps + 1) : 0;
-            bool ok = true;
+            int word = steps > 0 ? __ldcg(exps + 1) : 0;
+            bool ok = true, wide = false;
 #pragma unroll 1
             for (int i = 0; i < steps; ++i) {
                 const int sl = i & 1;
@@ -686,8 +741,9 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                 if (!ok) break;
                 tc_fence_after();
                 const float2 st = stat[sl * kPtRows + r];
-                const float e = st.x + static_cast<float>(ev);
-                if (i + 1 < steps) ev = __ldcg(exps + (i + 1) * ex_step + 1);
+                const float e = st.x + static_cast<float>(exps_exponent(word));
+                wide |= exps_wide(word);
+                if (i + 1 < steps) word = __ldcg(exps + (i + 1) * ex_step + 1);
                 if (st.x > M) {
                     L *= exp2_approx(M - st.x);
                     M = st.x;
@@ -716,16 +772,17 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             // P and l both carry 2^kTop; two factors, neither of which overflows
             const float half = R == -INFINITY ? 0.f : 0.5f * (R - M);
             const float undo = exp2_approx(half);
-            if (sp.parts > 1 && live) sp.part_ml[part_row] = make_float2(M, L);
             if (steps == 0) ok = __all_sync(0xffffffffu, wait(q_full, 0));  // Q's planes are written by now
+            if (wide) any_wide = 1;
+            named_sync(4, 384);
+            ok = ok && !any_wide;  // else the softmax threads do the rows over
+            if (ok && sp.parts > 1 && live) sp.part_ml[part_row] = make_float2(M, L);
             if (ok) {
-                const bool any_bad = bad[4 * kMaskedTiles] != 0;
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
                     float x[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) x[j] = acc[32 * c + j] * inv * undo * undo;
-                    if (any_bad && live) add_cleared(x, 32 * c, M, inv * pow2(kTop));
                     if (sp.parts == 1) {  // over Q: every product with it is complete
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
@@ -761,7 +818,8 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
         uint32_t *tops = reinterpret_cast<uint32_t *>(stat);  // free until the first scores
         tops[slot * kPtRows + r] = top;
         named_sync(3, 256);
-        const int eq = top_exponent(max(top, tops[(slot ^ 1) * kPtRows + r])) - kTop;
+        top = max(top, tops[(slot ^ 1) * kPtRows + r]);
+        const int eq = top ? top_exponent(top) - kTop : 0;
         const float s = pow2(-eq);
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {  // 16-byte chunks of eight halves
@@ -780,11 +838,14 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
         mbar_arrive(q_full);
         grid_wait();  // the exponents
         const uint32_t ts = col_s(slot) + lanes;
-        int ek = slot < steps ? __ldcg(exps + slot * ex_step) : 0;
+        int word = slot < steps ? __ldcg(exps + slot * ex_step) : 0;
+        bool wide = false;
 #pragma unroll 1
         for (int i = slot; i < steps; i += 2) {
-            const float sl2 = a.sl2 * pow2(ek + eq);
-            if (i + 2 < steps) ek = __ldcg(exps + (i + 2) * ex_step);
+            const int ex = exps_exponent(word) + eq;
+            wide |= exps_wide(word) || ex > kMostScale;
+            const float sl2 = a.sl2 * pow2(ex >> 1) * pow2(ex - (ex >> 1));  // (one factor ends at 2^-126)
+            if (i + 2 < steps) word = __ldcg(exps + (i + 2) * ex_step);
             if (!__all_sync(0xffffffffu, wait(&s_full[slot], (i >> 1) & 1))) break;
             tc_fence_after();
             const int vis = last + 1 - i * kPtKeys;  // keys of the tile the row sees
@@ -846,6 +907,28 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             tc_wait_st();
             tc_fence_before();
             mbar_arrive(&p_part[slot]);
+        }
+        if (wide) any_wide = 1;
+        named_sync(4, 384);  // every product is complete
+        if (any_wide) {
+            const int rows = min(BQ, p.nq - t0) * G, from = ta * kPtKeys, to = (ta + nt) * kPtKeys;
+            for (int r0 = 0; r0 < rows; r0 += kPkRows) {
+                named_sync(5, kPkThreads);  // the last rows' shared memory is free
+                ffma_rows<float, D>(
+                    a, p, kvh, t0 * G + r0, min(kPkRows, rows - r0), from, to, reinterpret_cast<float *>(base), threadIdx.x - 128,
+                    [] { named_sync(5, kPkThreads); },
+                    [&](int row, int c, const float (&x)[4], float m, float l) {
+                        row += r0;
+                        if (sp.parts == 1) {
+                            float *to_row = static_cast<float *>(a.out) + (p.q0 + t0 + row / G) * a.o_tok + (kvh * G + row % G) * a.o_head;
+                            *reinterpret_cast<float4 *>(to_row + c) = make_float4(x[0], x[1], x[2], x[3]);
+                        } else {
+                            const int64_t at = static_cast<int64_t>(blockIdx.x) * kPtRows + row;
+                            *reinterpret_cast<float4 *>(sp.part_o + at * D + c) = make_float4(x[0], x[1], x[2], x[3]);
+                            if (c == 0) sp.part_ml[at] = make_float2(m, l * pow2(kTop));  // as the other parts' sums
+                        }
+                    });
+            }
         }
     } else {
         // ---- softmax
