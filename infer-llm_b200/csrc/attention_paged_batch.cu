@@ -26,7 +26,8 @@
 //    32 KB of cache), which is why this is not a tcgen05 kernel: its M of 128 has no
 //    rows to fill. P enters the second product as two terms, P = hi + lo (each rounded to the
 //    element type), so P is not rounded to 8 or 11 bits; up to eight query heads the second
-//    term takes the unused rows 8 .. 15 of the same product.
+//    term takes the unused rows 8 .. 15 of the same product. Outputs that are no numbers are formed
+//    again with P as one F32 number (output_again), so that an infinite V counts as the formula says.
 //  * F32 caches: FFMA. For the scores a lane takes a quarter of head_dim of one of 8 keys;
 //    for the output it takes head_dim / 32 columns of all 8.
 // Measured: 64 ragged BF16 sequences (132 k keys, 32 / 8 heads of 128, 541 MB) 98 to 102 us, 5.4 TB/s, 82 % of
@@ -448,9 +449,55 @@ struct WarpState<float, D, HB> {
     }
 };
 
+// Columns [c0, c1) of one query head's output once more, by WARPS warps (a key each in turn) with P as
+// one F32 number. As two terms it is no factor for an infinite V: the second is often 0 or
+// negative, and inf - inf or 0 inf is not P inf. Only for 16-bit outputs that are no numbers.
+// smem: WARPS * (D + 2) floats.
+template <typename T, int D, int WARPS>
+__device__ __noinline__ void output_again(const PbArgs &a, int b, int head, int c0, int c1, float *smem) {
+    constexpr int E = D / 32;  // columns lane * E ... of a lane
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, len = seq_len(a, b);
+    const T *q = static_cast<const T *>(a.q) + b * a.q_seq + head * a.q_head + lane * E;
+    float qx[E], o[E] = {}, m = -INFINITY, l = 0.f;
+    for (int e = 0; e < E; ++e) qx[e] = to_f32<T>(q[e]);
+    for (int64_t key = warp; key < len; key += WARPS) {
+        const uint32_t k32 = static_cast<uint32_t>(key), slot = k32 / a.bt;
+        const int32_t blk = __ldg(a.table + b * a.table_stride + slot);
+        if (blk < 0 || blk >= a.n_blocks) continue;
+        const int64_t off = blk * a.block_stride + static_cast<int64_t>(k32 - slot * a.bt) * a.tok_stride + (head / a.G) * a.head_stride;
+        const T *k = reinterpret_cast<const T *>(a.k + off) + lane * E, *v = reinterpret_cast<const T *>(a.v + off) + lane * E;
+        float s = 0.f;
+        for (int e = 0; e < E; ++e) s = fmaf(qx[e], to_f32<T>(k[e]), s);
+        s = warp_sum(s) * a.sl2;
+        if (s > m) {
+            const float al = exp2_approx(m - s);
+            l *= al;
+            for (int e = 0; e < E; ++e) o[e] *= al;
+            m = s;
+        }
+        const float p = exp2_approx(s - (m == -INFINITY ? 0.f : m));
+        l += p;
+        for (int e = 0; e < E; ++e) o[e] = fmaf(p, to_f32<T>(v[e]), o[e]);
+    }
+    for (int e = 0; e < E; ++e) smem[warp * (D + 2) + lane * E + e] = o[e];
+    if (lane == 0) smem[warp * (D + 2) + D] = m, smem[warp * (D + 2) + D + 1] = l;
+    __syncthreads();
+    for (int c = c0 + static_cast<int>(threadIdx.x); c < c1; c += 32 * WARPS) {
+        float M = -INFINITY, ls = 0.f, os = 0.f;
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, smem[w * (D + 2) + D]);
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = exp2_approx(smem[w * (D + 2) + D] - (M == -INFINITY ? 0.f : M));
+            ls = fmaf(f, smem[w * (D + 2) + D + 1], ls);
+            os = fmaf(f, smem[w * (D + 2) + c], os);
+        }
+        static_cast<T *>(a.out)[b * a.o_seq + head * a.o_head + c] = from_f32<T>(ls != 0.f ? os / ls : 0.f);
+    }
+    __syncthreads();  // smem is free again
+}
+
 // CL: a cluster of kCluster CTAs takes one pair, and writes its output.
 template <typename T, int D, int HB, bool CL>
-__global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const PbArgs a) {
+__global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid_constant__ PbArgs a) {
     using Ge = Geometry<T, D, HB>;
     extern __shared__ __align__(128) unsigned char pb_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -599,8 +646,9 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const PbArgs
         cluster_sync();  // every CTA's record is written
         const int rank = blockIdx.x % kCluster;
         const int h0 = (start.vh / a.HG) * a.G + (start.vh % a.HG) * HB, heads = min(HB, a.G - (start.vh % a.HG) * HB);
-        const int n = heads * D;
-        for (int i = n * rank / kCluster + threadIdx.x; i < n * (rank + 1) / kCluster; i += kPbThreads) {
+        const int n = heads * D, i0 = n * rank / kCluster, i1 = n * (rank + 1) / kCluster;
+        bool odd = false;
+        for (int i = i0 + threadIdx.x; i < i1; i += kPbThreads) {
             const int g = i / D;
             float m[kCluster], l[kCluster], o[kCluster], M = -INFINITY;
 #pragma unroll
@@ -619,17 +667,23 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const PbArgs
                 ls = fmaf(f, l[c], ls);
                 os = fmaf(f, o[c], os);
             }
-            static_cast<T *>(a.out)[start.b * a.o_seq + (h0 + g) * a.o_head + (i - g * D)] =
-                from_f32<T>(ls != 0.f ? os / ls : 0.f);
+            const float x = ls != 0.f ? os / ls : 0.f;
+            odd |= !(fabsf(x) < INFINITY);
+            static_cast<T *>(a.out)[start.b * a.o_seq + (h0 + g) * a.o_head + (i - g * D)] = from_f32<T>(x);
+        }
+        if constexpr (sizeof(T) == 2) {
+            if (__syncthreads_or(odd))
+                for (int g = i0 / D; g * D < i1; ++g)
+                    output_again<T, D, kPbWarps>(a, start.b, h0 + g, max(0, i0 - g * D), min(D, i1 - g * D), merge);
         }
         cluster_sync();  // no CTA's shared memory goes away while it is read
     }
 }
 
-// Joins the parts of each pair that more than one CTA took, and clears the rows of empty
-// sequences. One CTA a pair.
+// Joins the parts of each pair that more than one CTA took, clears the rows of empty
+// sequences, and looks for 16-bit outputs that are no numbers. One CTA a pair.
 template <typename T, int D, int HB>
-__global__ void __launch_bounds__(kJoinThreads) paged_batch_join_kernel(const PbArgs a, const int64_t grid) {
+__global__ void __launch_bounds__(kJoinThreads) paged_batch_join_kernel(const __grid_constant__ PbArgs a, const int64_t grid) {
     using Ge = Geometry<T, D, HB>;
     __shared__ float factor[HB * kPbMostCtas], scale[HB];
     const int b = static_cast<int>(blockIdx.x / a.VH), vh = static_cast<int>(blockIdx.x % a.VH);
@@ -651,7 +705,22 @@ __global__ void __launch_bounds__(kJoinThreads) paged_batch_join_kernel(const Pb
         slot0 = share_begin(total, c0, ctas) >= ua ? 0 : 1;
     }
     grid_wait();
-    if (parts == 1) return;  // whole: written by its CTA
+    const auto again = [&](bool odd) {
+        if constexpr (sizeof(T) == 2) {
+            if (__syncthreads_or(odd))
+                for (int g = 0; g < heads; ++g) output_again<T, D, kJoinThreads / 32>(a, b, h0 + g, 0, D, factor);
+        }
+    };
+    if (parts == 1) {  // whole: written by its CTA
+        bool odd = false;
+        if constexpr (sizeof(T) == 2)
+            for (int i = tid; i < heads * D / 2; i += kJoinThreads) {
+                const float2 x = unpack2<T>(__ldcg(reinterpret_cast<const uint32_t *>(out + (2 * i / D) * a.o_head + 2 * i % D)));
+                odd |= !(fabsf(x.x) < INFINITY && fabsf(x.y) < INFINITY);
+            }
+        again(odd);
+        return;
+    }
     if (parts == 0) {
         for (int i = tid; i < heads * D; i += kJoinThreads) out[(i / D) * a.o_head + i % D] = from_f32<T>(0.f);
         return;
@@ -678,13 +747,16 @@ __global__ void __launch_bounds__(kJoinThreads) paged_batch_join_kernel(const Pb
         if (lane == 0) scale[g] = sum != 0.f ? 1.0f / sum : 0.f;
     }
     __syncthreads();
+    bool odd = false;
     for (int j = tid; j < heads * D; j += kJoinThreads) {
         const int g = j / D;
         float acc = 0.f;
 #pragma unroll 8
         for (int i = 0; i < parts; ++i) acc = fmaf(factor[g * kPbMostCtas + i], __ldcg(part(i) + j), acc);
+        odd |= !(fabsf(acc * scale[g]) < INFINITY);
         out[g * a.o_head + (j - g * D)] = from_f32<T>(acc * scale[g]);
     }
+    again(odd);
 }
 
 int pb_max_ctas() { return device_sm_count() * 2 < kPbMostCtas ? device_sm_count() * 2 : kPbMostCtas; }
