@@ -252,7 +252,8 @@ typedef struct b200_kv_pool {
  * row i of a sequence with nq queries and nk keys sees its keys 0 .. nk - nq + i (the
  * last query sees the last key); a row that sees none (nk < nq), or whose scores are all
  * -inf, is zero. Rows outside
- * every sequence are left untouched. scale <= 0 selects 1/sqrt(D). D 64 or 128, any
+ * every sequence are left untouched; but if a sequence's offsets are out of range, the rows that
+ * no other sequence covers are cleared. scale <= 0 selects 1/sqrt(D). D 64 or 128, any
  * Hq that is a multiple of Hkv. `workspace` (16-byte aligned, contents ignored) of
  * b200_flash_attn_packed_workspace_bytes(...) bytes; may be NULL where that is 0. */
 int b200_flash_attn_packed(const void *q, int64_t q_tok_stride, int64_t q_head_stride, const void *k,

@@ -412,7 +412,8 @@ def _out_rows(out, q, dev):
 def flash_attn_packed(q, k, v, cu_q, cu_k=None, scale=0.0, out=None, workspace=None, status=None):
     """Causal attention of packed sequences: q (Tq, Hq, D); k, v (Tk, Hkv, D); cu_q, cu_k int32
     (n + 1,) offsets of the n sequences (cu_k None: as cu_q). Row i of a sequence with nq
-    queries and nk keys sees its keys 0 .. nk - nq + i. Returns (Tq, Hq, D)."""
+    queries and nk keys sees its keys 0 .. nk - nq + i. Returns (Tq, Hq, D). Rows outside every
+    sequence are not written; offsets out of range leave zeros, and set `status`."""
     h, dev = _start(q)
     if h.current() != dev:
         return _elsewhere(flash_attn_packed, dev, q, k, v, cu_q, cu_k, scale, out, workspace, status)

@@ -18,6 +18,7 @@ __global__ void __launch_bounds__(kPkThreads, 2) packed_ffma_kernel(const Packed
     const int kvh = blockIdx.x % a.Hkv;
     const PackedTile p = find_packed_tile(a.cu_q, a.cu_k, a.n_seqs, a.total_q, a.total_k, a.G, kPkRows,
                                           blockIdx.x / a.Hkv, a.status);
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x < 32) clear_uncovered(a);
     if (p.seq < 0) return;
     const int r0 = p.tile * kPkRows, rows = min(kPkRows, p.nq * a.G - r0);
     T *out = static_cast<T *>(a.out);

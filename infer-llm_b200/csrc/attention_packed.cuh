@@ -18,6 +18,33 @@ struct PackedArgs {
     int32_t *status = nullptr;
 };
 
+// Where a sequence's offsets are out of range: reports it, and clears the query rows that no other
+// sequence covers, so that an output made for the call holds nothing else. Run by one warp of the
+// grid's last CTA, which found its own tile (or none) in the same offsets.
+B200_DEVICE void clear_uncovered(const PackedArgs &a) {
+    const int lane = threadIdx.x & 31;
+    int64_t q0, k0;
+    int nq, nk;
+    const auto runs = [&](int s) {  // (an empty sequence's keys do not matter)
+        const bool ok_q = packed_range(a.cu_q, s, a.total_q, q0, nq), ok_k = packed_range(a.cu_k, s, a.total_k, k0, nk);
+        return ok_q && (ok_k || nq == 0);
+    };
+    bool bad = false;
+    for (int s = lane; s < a.n_seqs; s += 32) bad |= !runs(s);
+    if (!__any_sync(0xffffffffu, bad)) return;
+    if (lane == 0) set_status(a.status, B200_DEV_BAD_POSITION);
+    const int64_t e = a.dtype == B200_DTYPE_F32 ? 4 : 2;
+    const int chunks = a.D * static_cast<int>(e) / 16;  // of a head
+    for (int64_t t = 0; t < a.total_q; ++t) {
+        bool in = false;
+        for (int s = lane; s < a.n_seqs; s += 32) in |= runs(s) && t >= q0 && t < q0 + nq;
+        if (__any_sync(0xffffffffu, in)) continue;
+        char *row = static_cast<char *>(a.out) + t * a.o_tok * e;
+        for (int c = lane; c < a.Hq * chunks; c += 32)
+            *reinterpret_cast<uint4 *>(row + (c / chunks) * a.o_head * e + c % chunks * 16) = make_uint4(0, 0, 0, 0);
+    }
+}
+
 // The tensor-core kernel; cudaErrorNotSupported (nothing launched) where it does not apply.
 size_t packed_tc_workspace(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t D, int64_t Hq, int64_t Hkv,
                            int32_t dtype);

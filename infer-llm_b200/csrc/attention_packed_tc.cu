@@ -462,6 +462,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kColumns)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (blockIdx.x == gridDim.x - 1) clear_uncovered(a);
     }
 
     const int G = a.G, BQ = kPtRows / G, MT = NT * BQ;  // tokens of a query tile, of the CTA

@@ -220,3 +220,31 @@ def test_f32_visible_infinite_values(cuda, layout, at):
     assert ((got.double() - exact).abs() <= bound)[..., rest].all()
     if see.start:
         assert ((got.double() - exact).abs() <= bound)[:see.start].all()
+
+
+# ---------------------------------------------------------------------------
+# offsets out of range
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [50, 170])
+@pytest.mark.parametrize("cu_q,cu_k,good", [
+    ([0, 20, 60, 50], None, [(0, 20)]), ([0, 20, 500, 700], None, [(0, 20)]), ([-5, 20, 30, 50], None, [(20, 30), (30, 50)]),
+    ([0, 20, 30, 50], [0, 20, 900, 50], [(0, 20)]), ([0, 20, 20, 50], [0, 20, -7, 50], [(0, 20)]),
+    ([30, 20, 10, 0], None, [])], ids=["past", "far", "negative", "keys", "keys_of_an_empty_one", "descending"])
+def test_bad_offsets_leave_zeros(cuda, kind, T, cu_q, cu_k, good):
+    """Rows that no sequence with offsets in range covers are zeros; the others are as ever."""
+    heads = (4, 2, 64)
+    q, k, v = inputs(39, heads, [T], [T], kind)
+    scale = lambda cu: None if cu is None else torch.tensor(  # noqa: E731
+        [c * T // 50 for c in cu], dtype=torch.int32, device=cuda)
+    out = torch.full_like(q, math.nan)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    B.flash_attn_packed(q, k, v, scale(cu_q), scale(cu_k), out=out, status=status)
+    assert int(status) == 2  # B200_DEV_BAD_POSITION
+    left = torch.ones(T, dtype=torch.bool, device=cuda)
+    for a, b in good:
+        a, b = a * T // 50, b * T // 50
+        want, w = packed_exact(q[a:b], k[a:b], v[a:b], [b - a], [b - a])
+        check(out[a:b], want, w, kind, True)
+        left[a:b] = False
+    assert (out[left] == 0).all()
