@@ -251,9 +251,9 @@ typedef struct b200_kv_pool {
  * k, v [total_k][Hkv][D]; cu_* are device int32 [n_seqs + 1], ascending from 0. Query
  * row i of a sequence with nq queries and nk keys sees its keys 0 .. nk - nq + i (the
  * last query sees the last key); a row that sees none (nk < nq), or whose scores are all
- * -inf, is zero. Rows outside
- * every sequence are left untouched; but if a sequence's offsets are out of range, the rows that
- * no other sequence covers are cleared. scale <= 0 selects 1/sqrt(D). D 64 or 128, any
+ * -inf, is zero. Rows outside every sequence are left untouched; but if a sequence's offsets
+ * are out of range, the rows that no other sequence covers are cleared. scale <= 0 selects
+ * 1/sqrt(D). D 64 or 128, any
  * Hq that is a multiple of Hkv. `workspace` (16-byte aligned, contents ignored) of
  * b200_flash_attn_packed_workspace_bytes(...) bytes; may be NULL where that is 0. */
 int b200_flash_attn_packed(const void *q, int64_t q_tok_stride, int64_t q_head_stride, const void *k,
@@ -279,11 +279,10 @@ int b200_paged_kv_append(const void *k, int64_t k_tok_stride, int64_t k_head_str
 /* GQA attention of one new token per sequence: q, out [n_seqs][Hq][D]; sequence s
  * attends to positions [0, seq_lens[s]) of the pool through its row of block_table (as
  * above; its own K / V already appended). A sequence of length 0 gives zeros, and so do
- * scores of -inf alone; one
- * longer than max_blocks * block_tokens is cut there. The keys of all sequences are
- * spread evenly over the SMs; the parts of a split sequence are joined in a fixed
- * order, so results do not depend on timing. Keys in a block whose index is out of
- * range are left out. D 64 or 128. `workspace` as above
+ * scores of -inf alone; one longer than max_blocks * block_tokens, or than 2^31 - 257, is cut
+ * there. The keys of all sequences are spread evenly over the SMs; the parts of a split
+ * sequence are joined in a fixed order, so results do not depend on timing. Keys in a block
+ * whose index is out of range are left out. D 64 or 128. `workspace` as above
  * (b200_flash_attn_paged_batch_workspace_bytes with max_keys = max_blocks * block_tokens;
  * 0 for few sequences with short tables). */
 int b200_flash_attn_paged_batch(const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,

@@ -47,6 +47,7 @@ constexpr int kPbMostCtas = 320;
 constexpr int kJoinThreads = 256;
 constexpr int kCluster = 8;
 constexpr int kClusterKeys = 4096;
+constexpr int64_t kMostKeys = INT32_MAX - 256;
 
 struct PbArgs {
     const void *q = nullptr;
@@ -868,9 +869,9 @@ int b200_flash_attn_paged_batch(const void *q, int64_t q_seq_stride, int64_t q_h
     if ((D != 64 && D != 128) || n_seqs >= INT32_MAX || Hq > 65536 || !rows_aligned16(q, q_seq_stride, q_head_stride, e) ||
         !rows_aligned16(out, out_seq_stride, out_head_stride, e))
         return B200_ERR_NOT_SUPPORTED;
-    // positions are 31-bit: a longer table's tail cannot be named by an int32 length
+    // a length and a tile past it fit 31 bits: the tail of a table of more positions is not used
     const int64_t max_keys =
-        max_blocks > INT32_MAX / pool->block_tokens ? INT32_MAX - 256 : max_blocks * pool->block_tokens;
+        max_blocks > kMostKeys / pool->block_tokens ? kMostKeys : max_blocks * pool->block_tokens;
     const size_t need = b200_flash_attn_paged_batch_workspace_bytes(n_seqs, max_keys, D, Hq, Hkv, pool->dtype);
     if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need))
         return B200_ERR_INVALID_ARGUMENT;

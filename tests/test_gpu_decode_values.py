@@ -1,4 +1,4 @@
-"""b200_flash_attn_paged_batch on values that are no numbers. Bounds: those of
+"""b200_flash_attn_paged_batch on values that are no numbers, and at the end of 31 bits. Bounds: those of
 test_gpu_batch.py, on the elements that are numbers."""
 import math
 
@@ -63,3 +63,21 @@ def test_nan_keys_and_scores_of_minus_inf(cuda, kind, layout):
     got = B.flash_attn_paged_batch(q, c.k, c.v, c.table, c.lens)
     assert torch.isnan(got[0].double()).all() and (got[1] == 0).all()
     check(got[2:], want[2:], w[2:], kind, False)
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+def test_lengths_up_to_31_bits(cuda, kind):
+    """One page of 2^31 - 1 positions that all share one row, and a length that reaches their end:
+    cut at 2^31 - 257 and reported. The sums of equal rows of 1/2 are exact up to the join, whose
+    rounding is far below half a unit of F16."""
+    Hq, D = 2, 64
+    row = torch.full((1, 1, 1, D), 0.5, device=cuda, dtype=DT[kind])
+    pool = row.expand(1, 2 ** 31 - 1, 1, D)
+    q = torch.randn((2, Hq, D), device=cuda).to(DT[kind])
+    table = torch.zeros((2, 1), dtype=torch.int32, device=cuda)
+    for length, code in ((2 ** 31 - 1, 2), (2 ** 31 - 257, 0), (2 ** 31 - 256, 2)):
+        status = torch.zeros(1, dtype=torch.int32, device=cuda)
+        lens = torch.tensor([length, 5], dtype=torch.int32, device=cuda)
+        got = B.flash_attn_paged_batch(q, pool, pool, table, lens, status=status)
+        assert int(status) == code
+        assert (got.half() == 0.5).all()
