@@ -615,8 +615,9 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const SampleArgs 
         uint32_t pe = 0;
         // (key 0 keeps the whole row; min-p leaves out what lies below its own bin)
         const float k_value = key ? key_value(key) : -INFINITY;
-        const float low = f.sc.below(least > 0 ? min(kBins - 1, static_cast<int>(logf(fminf(min_p, 1.0f)) * (kBins / kFloor)) + 2)
-                                               : kBins - 1);
+        // `least` whole units, not min_p: the two differ by up to a factor of two where min_p is a few units
+        const float low = f.sc.below(
+            least > 0 ? min(kBins - 1, static_cast<int>(logf(static_cast<float>(least) * 0x1p-40f) * (kBins / kFloor)) + 2) : kBins - 1);
         f.x.each(p0, p1, lane, 32, [&](float v, int) {
             if (v < k_value || v < low) return;
             if (v > k_value) {

@@ -60,3 +60,17 @@ def test_long_16_bit_rows_of_equal_logits(cuda, kind, vocab, rows):
         got = draw(x, *args, u)
         check(x[pick], *args, u[pick], got[pick])
         assert int(got[pick[2]]) == int(draw(x[:1], *args, u[pick[2]])[0])
+
+
+@pytest.mark.parametrize("vocab", [151936, 2 ** 20])
+def test_min_p_of_a_few_units(cuda, vocab):
+    """min_p of less than two units of 2^-40 keeps the tokens whose weight is one unit: they hold
+    the last vocab - 1 units of the sum."""
+    x = torch.full((1, vocab), -27.6, device=cuda)  # floor(2^40 e^-27.6) = 1
+    x[0, 0] = 0.0
+    u = np.float32(1) - np.float32(2.0 ** -24)  # 2^16 units before the end
+    want = int(np.floor(np.float64(u) * (2.0 ** 40 + vocab - 1)) - 2.0 ** 40) + 1
+    assert want > 0
+    for min_p in (0.0, 0.95e-12, 1.2e-12, 1.7e-12, 1.8e-12):
+        got = draw(x, 1.0, None, None, min_p, u)
+        assert int(got[0]) == want, (min_p, int(got[0]), want)
