@@ -10,8 +10,6 @@
 namespace b200 {
 namespace {
 
-constexpr int64_t kMostRows = INT32_MAX - 1024;  // row numbers of a tile past the last one fit 31 bits
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kPkThreads, 2) packed_ffma_kernel(const PackedArgs a) {
     extern __shared__ __align__(16) float pk_smem[];
@@ -79,7 +77,7 @@ int b200_flash_attn_packed(const void *q, int64_t q_tok_stride, int64_t q_head_s
         return B200_ERR_INVALID_ARGUMENT;
     if (n_seqs == 0 || total_q == 0) return B200_OK;
     if (!q || !out || !cu_q || !cu_k || (total_k > 0 && (!k || !v))) return B200_ERR_INVALID_ARGUMENT;
-    if ((D != 64 && D != 128) || Hq > 65536 || n_seqs >= INT32_MAX || total_q * (Hq / Hkv) > kMostRows ||
+    if ((D != 64 && D != 128) || Hq > 65536 || n_seqs > kMostRows || total_q > kMostRows / (Hq / Hkv) ||
         total_k > kMostRows || !rows_aligned16(q, q_tok_stride, q_head_stride, e) ||
         !rows_aligned16(k, k_tok_stride, k_head_stride, e) || !rows_aligned16(v, v_tok_stride, v_head_stride, e) ||
         !rows_aligned16(out, out_tok_stride, out_head_stride, e))

@@ -866,7 +866,7 @@ int b200_flash_attn_paged_batch(const void *q, int64_t q_seq_stride, int64_t q_h
     if (!q || !out || !block_table || !seq_lens || max_blocks <= 0 || table_stride < max_blocks)
         return B200_ERR_INVALID_ARGUMENT;
     const int e = dtype_bytes(pool->dtype);
-    if ((D != 64 && D != 128) || n_seqs >= INT32_MAX || Hq > 65536 || !rows_aligned16(q, q_seq_stride, q_head_stride, e) ||
+    if ((D != 64 && D != 128) || n_seqs > kMostRows || Hq > 65536 || !rows_aligned16(q, q_seq_stride, q_head_stride, e) ||
         !rows_aligned16(out, out_seq_stride, out_head_stride, e))
         return B200_ERR_NOT_SUPPORTED;
     // a length and a tile past it fit 31 bits: the tail of a table of more positions is not used

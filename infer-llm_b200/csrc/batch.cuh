@@ -36,6 +36,9 @@ B200_DEVICE float exp2_approx(float x) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Rows, keys and sequences of a call: numbers of a tile, or of 32 sequences, past the last one fit 31 bits.
+constexpr int64_t kMostRows = INT32_MAX - 1024;
+
 // The sequence s of [0, n) with cu[s] <= t < cu[s + 1], or -1. All lanes of a warp take
 // part and get the answer: each round 32 probes narrow the range 32-fold, so the chain
 // of dependent loads is log32(n) long. Offsets that are not ascending give some s or

@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
         return;
     }
     const int64_t pos = static_cast<int64_t>(__ldg(a.lens + s)) - __ldg(a.cu + s + 1) + t;  // < 2^31: t is a row of s
-    const int64_t slot = pos < 0 ? -1 : static_cast<unsigned>(pos) / a.block_tokens;
+    const int64_t slot = pos < 0 ? -1 : static_cast<int64_t>(static_cast<unsigned>(pos) / a.block_tokens);
     const int64_t blk = slot >= 0 && slot < a.max_blocks ? __ldg(a.table + s * a.table_stride + slot) : -1;
     if (blk < 0 || blk >= a.n_blocks) {
         if (lane == 0) set_status(a.status, B200_DEV_BAD_POSITION);
@@ -86,7 +86,7 @@ extern "C" int b200_paged_kv_append(const void *k, int64_t k_tok_stride, int64_t
         return B200_ERR_INVALID_ARGUMENT;
     const int e = dtype_bytes(pool->dtype);
     if (!rows_aligned16(k, k_tok_stride, k_head_stride, e) || !rows_aligned16(v, v_tok_stride, v_head_stride, e) ||
-        n_seqs >= INT32_MAX || n_tokens >= INT32_MAX || pool->n_head_kv * pool->head_dim > (1 << 24))
+        n_seqs > kMostRows || n_tokens > kMostRows || pool->n_head_kv > (1 << 24) / pool->head_dim)
         return B200_ERR_NOT_SUPPORTED;
     AppendArgs a = {};
     a.src[0] = static_cast<const char *>(k);
