@@ -228,7 +228,8 @@ int b200_argmax_noalloc(const float *logits, int64_t n, int32_t *out_id, int32_t
  * Batched serving: many sequences in one call. Lengths are device arrays, so the
  * calls take no host copy of them and can be captured into a CUDA graph once per
  * shape bound. Tensors are F32, F16 or BF16 (`dtype`, one for all tensors of a call;
- * sums, softmax statistics and accumulators are F32). Strides count elements; the
+ * sums, softmax statistics and accumulators are F32; what has fewer bits stands at the
+ * call). Strides count elements; the
  * head_dim axis is contiguous; every row must start on a 16-byte boundary
  * (B200_ERR_NOT_SUPPORTED otherwise). A device-side length, offset or block index out
  * of range is never followed: what it names is skipped and B200_DEV_BAD_POSITION is
@@ -253,8 +254,14 @@ typedef struct b200_kv_pool {
  * last query sees the last key); a row that sees none (nk < nq), or whose scores are all
  * -inf, is zero. Rows outside every sequence are left untouched; but if a sequence's offsets
  * are out of range, the rows that no other sequence covers are cleared. scale <= 0 selects
- * 1/sqrt(D). D 64 or 128, any
- * Hq that is a multiple of Hkv. `workspace` (16-byte aligned, contents ignored) of
+ * 1/sqrt(D). D 64 or 128, any Hq that is a multiple of Hkv.
+ * Bits: with 16-bit types a weight enters the second product as one number of the type,
+ * and a quarter of the exponentials are within 7.5e-5 (BF16) or 2.6e-6 (F16). F32 with more
+ * than 64 keys: Q, K, V and weights as two F16 numbers, 22 bits or an absolute 2^-29 of the
+ * largest element of the row (K, V: in each 128 keys, of the row and of the column); F32
+ * arithmetic where magnitudes spread too far for that, or are no numbers. An infinite V
+ * element a row sees makes its column infinite, or NaN where a 16-bit weight rounds to 0.
+ * A wait that runs out records B200_DEV_TIMEOUT and leaves that tile's rows unwritten. `workspace` (16-byte aligned, contents ignored) of
  * b200_flash_attn_packed_workspace_bytes(...) bytes; may be NULL where that is 0. */
 int b200_flash_attn_packed(const void *q, int64_t q_tok_stride, int64_t q_head_stride, const void *k,
                            int64_t k_tok_stride, int64_t k_head_stride, const void *v, int64_t v_tok_stride,

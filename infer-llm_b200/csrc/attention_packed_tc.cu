@@ -20,8 +20,10 @@
 // for F32 warps 12-15 the output's sum. They share out the CTA's registers (80 + 2 x 120 + 192 = 4 x 128
 // for F32, 88 + 2 x 208 = 3 x 168 with two slots, 56 + 200 = 2 x 128 with one).
 //   * The running maximum moves only when it grows by more than 2^8, so rescaling O is rare
-//     (the result is unchanged: every p is bounded by 2^8). Statistics are F32; P is
-//     rounded to the element type, the sum is taken before that.
+//     (the result is unchanged: every p is bounded by 2^8). Statistics are F32. 16-bit types: P is
+//     one number of the element type, the sum is taken before that rounding. It is what the second
+//     product takes at one product's cost; two terms of P would add half to the tensor work. The errors against
+//     64 bits grow by it from 1.5e-3 to 2.0e-3 of the output (8192 BF16 tokens) and from 2.1e-4 to 2.6e-4 (F16).
 //   * Hidden keys of a tile (past a row's last key, of the next sequence, or past the end)
 //     have P = 0, but 0 times a V that is no number is not 0. The V check looks for such
 //     rows in the tiles that hide keys, clears them in shared memory, and notes them; 16-bit rows that
@@ -41,9 +43,9 @@
 //     up in F32 registers, each with its own row maximum and V exponent. An FFMA kernel has no
 //     such rounding but a 20th of the rate; TF32 products would keep 11 bits.
 // Bound: at long contexts the chain scores -> softmax -> P -> product of a slot, against which the other
-// slot's runs: 8192 BF16 tokens, 32 / 8 heads of 128, 504 us, 1.09 PFLOP/s (66 % of a large library
-// matrix product's rate); the tensor cores are busy 55 to 60 % of the time. 2048 F32 tokens, 16 / 8 heads of
-// 128, 80 us (214 TFLOP/s of the call's, 640 of the three products), the split kernel 7 us of it. Short
+// slot's runs: 8192 BF16 tokens, 32 / 8 heads of 128, 505 to 522 us by GPU, 1.05 to 1.09 PFLOP/s (64 to 66 % of a
+// large library matrix product's rate); the tensor cores are busy 54 to 60 % of the time. 2048 F32 tokens, 16 / 8
+// heads of 128, 80 us (214 TFLOP/s of the call's, 640 of the three products), the split kernel 7 us of it. Short
 // calls: a CTA's start and end, ~6 us (look-up 1, first copies 1.4, last product 0.8 to 1.7, output 2), beside ~0.9
 // us a step: 10 prompts of 1 to 1333 BF16 tokens, 16 / 8 heads of 128, 35 us. Two slots take all 512
 // columns of tensor memory and most of an SM's registers.

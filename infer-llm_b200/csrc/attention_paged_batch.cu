@@ -2,9 +2,9 @@
 // K/V cache in F32, F16 or BF16.
 //
 // out_b = sum_j softmax_j(scale q_b . k_j) v_j over the keys j < seq_lens[b]. Every cached
-// row is read once and meets the G query heads that share it, so HBM bounds the operator
-// (2 G flops a byte at two bytes an element): what has to be had is many bytes in flight
-// on every SM however ragged the lengths are.
+// row is read once (once per 16 query heads of its KV head, of F32 per 8) and meets the query heads that share it, so
+// HBM bounds the operator (2 G flops a byte at two bytes an element): what has to be had is
+// many bytes in flight on every SM however ragged the lengths are.
 //
 //  * Work split: keys go in tiles of 4 sub-tiles (one a warp); all tiles of all
 //    (sequence, KV head) pairs form one line, of which each CTA takes an equal share
@@ -30,8 +30,8 @@
 //    again with P as one F32 number (output_again), so that an infinite V counts as the formula says.
 //  * F32 caches: FFMA. For the scores a lane takes a quarter of head_dim of one of 8 keys;
 //    for the output it takes head_dim / 32 columns of all 8.
-// Measured: 64 ragged BF16 sequences (132 k keys, 32 / 8 heads of 128, 541 MB) 98 to 102 us, 5.4 TB/s, 82 % of
-// a large copy's rate; 16 F32 sequences (587 MB) 98 us, 6.0 TB/s, 91 %. What is left is the join (~5 us)
+// Measured: 64 ragged BF16 sequences (132 k keys, 32 / 8 heads of 128, 541 MB) 98 to 104 us by GPU, 5.2 to 5.5 TB/s,
+// 79 to 84 % of a large copy's rate; 16 F32 sequences (587 MB) 99 us, 5.9 TB/s, 90 %. What is left is the join (~5 us)
 // and, for BF16, the latency of a warp's chain from copy to product. Eight warps an SM issue in 40 % of
 // the cycles.
 // Rows past a sequence's end are not read; they and keys of invalid blocks get weight 0.
