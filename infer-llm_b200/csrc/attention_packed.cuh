@@ -35,13 +35,21 @@ B200_DEVICE void clear_uncovered(const PackedArgs &a) {
     if (lane == 0) set_status(a.status, B200_DEV_BAD_POSITION);
     const int64_t e = a.dtype == B200_DTYPE_F32 ? 4 : 2;
     const int chunks = a.D * static_cast<int>(e) / 16;  // of a head
-    for (int64_t t = 0; t < a.total_q; ++t) {
-        bool in = false;
-        for (int s = lane; s < a.n_seqs; s += 32) in |= runs(s) && t >= q0 && t < q0 + nq;
-        if (__any_sync(0xffffffffu, in)) continue;
-        char *row = static_cast<char *>(a.out) + t * a.o_tok * e;
-        for (int c = lane; c < a.Hq * chunks; c += 32)
-            *reinterpret_cast<uint4 *>(row + (c / chunks) * a.o_head * e + c % chunks * 16) = make_uint4(0, 0, 0, 0);
+    for (int t = 0; t < a.total_q;) {  // from one covered run of rows to the next
+        int end = 0, next = static_cast<int>(a.total_q);
+        for (int s = lane; s < a.n_seqs; s += 32) {
+            if (!runs(s) || nq == 0) continue;
+            if (t < q0) next = min(next, static_cast<int>(q0));
+            else if (t < q0 + nq) end = max(end, static_cast<int>(q0 + nq));
+        }
+        end = __reduce_max_sync(0xffffffffu, end);
+        next = __reduce_min_sync(0xffffffffu, next);
+        for (; t < next && end == 0; ++t) {
+            char *row = static_cast<char *>(a.out) + t * a.o_tok * e;
+            for (int c = lane; c < a.Hq * chunks; c += 32)
+                *reinterpret_cast<uint4 *>(row + (c / chunks) * a.o_head * e + c % chunks * 16) = make_uint4(0, 0, 0, 0);
+        }
+        t = max(t, end);
     }
 }
 
