@@ -257,9 +257,9 @@ typedef struct b200_kv_pool {
  * 1/sqrt(D). D 64 or 128, any Hq that is a multiple of Hkv.
  * Bits: with 16-bit types a weight enters the second product as one number of the type,
  * and a quarter of the exponentials are within 7.5e-5 (BF16) or 2.6e-6 (F16). F32 with more
- * than 64 keys: Q, K, V and weights as two F16 numbers, 22 bits or an absolute 2^-29 of the
- * largest element of the row (K, V: in each 128 keys, of the row and of the column); F32
- * arithmetic where magnitudes spread too far for that, or are no numbers. An infinite V
+ * than 64 keys: Q, K, V and weights as two F16 numbers, 22 bits or an absolute 2^-39 (Q,
+ * weights) of the row's largest, 2^-23 (K) or 2^-33 (V) of the largest of the row and of the
+ * column in 128 keys; F32 arithmetic where magnitudes spread past 2^16, or are no numbers. An infinite V
  * element a row sees makes its column infinite, or NaN where a 16-bit weight rounds to 0.
  * A wait that runs out records B200_DEV_TIMEOUT and leaves that tile's rows unwritten. `workspace` (16-byte aligned, contents ignored) of
  * b200_flash_attn_packed_workspace_bytes(...) bytes; may be NULL where that is 0. */

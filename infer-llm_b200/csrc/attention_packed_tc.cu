@@ -33,10 +33,13 @@
 //     of x (and an absolute 2^-39 of the tile's largest), and x y = hi hi + hi lo + lo hi
 //     up to 2^-22. packed_split_kernel writes K and V so, as hi and lo planes with one
 //     exponent per 128-key tile and KV head; Q rows are split by the softmax threads
-//     (an exponent per row), P by construction (p <= 1, times 2^14). One exponent does only for rows and
-//     columns of like magnitude: a tile of K or V in which a row's or a column's largest is below 2^-10 of the
-//     tile's, or which holds Inf or NaN, is marked, and a CTA that met one does its rows over with F32
-//     FFMA (attention_packed_ffma.cuh; 2048 tokens, 16 / 8 heads of 128, with one such key 868 us, without 79). So
+//     (an exponent per row), P by construction (p <= 1, times 2^14). V, whose columns each make an output of their
+//     own, has its lo times 2^11: it is as large as hi then, not among F16's subnormals, and
+//     2^-50 of the tile's largest is held. P hi times it comes first, and the next product takes the sum times 2^-11
+//     (2048 tokens 82 us, with plain lo 81; K so too 85).
+//     One exponent does only for rows and columns of like magnitude: a tile of K or V in which a row's or a
+//     column's largest is below 2^-16 of the tile's, or which holds Inf or NaN, is marked, and a CTA that met one does
+//     its rows over with F32 FFMA (attention_packed_ffma.cuh; 2048 tokens with one such key 868 us). So
 //     neither hidden keys nor other columns cost a row its bits. The tensor cores
 //     round their sums toward zero: over a long row that bias reached 1e-5 at 8192 keys. So each
 //     step's O starts from zero (lo products first), and a fourth warpgroup adds the steps
@@ -45,7 +48,7 @@
 // Bound: at long contexts the chain scores -> softmax -> P -> product of a slot, against which the other
 // slot's runs: 8192 BF16 tokens, 32 / 8 heads of 128, 505 to 522 us by GPU, 1.05 to 1.09 PFLOP/s (64 to 66 % of a
 // large library matrix product's rate); the tensor cores are busy 54 to 60 % of the time. 2048 F32 tokens, 16 / 8
-// heads of 128, 80 us (214 TFLOP/s of the call's, 640 of the three products), the split kernel 7 us of it. Short
+// heads of 128, 82 us (209 TFLOP/s of the call's, 627 of the three products), the split kernel 7 us of it. Short
 // calls: a CTA's start and end, ~6 us (look-up 1, first copies 1.4, last product 0.8 to 1.7, output 2), beside ~0.9
 // us a step: 10 prompts of 1 to 1333 BF16 tokens, 16 / 8 heads of 128, 35 us. Two slots take all 512
 // columns of tensor memory and most of an SM's registers.
@@ -173,6 +176,15 @@ B200_DEVICE void mma_ts(uint32_t e, uint32_t d, uint32_t a, uint32_t b_low, uint
         "r"(a), "r"(b_low), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(kDescHigh), "r"(e)
         : "memory");
 }
+// The same onto D times 2^-kLoShift.
+constexpr int kLoShift = 11;
+B200_DEVICE void mma_ts_onto_lo(uint32_t e, uint32_t d, uint32_t a, uint32_t b_low, uint32_t idesc) {
+    asm volatile(
+        "{\n .reg .pred p, e;\n .reg .b64 db;\n setp.eq.b32 p, 0, 0;\n setp.ne.b32 e, %5, 0;\n mov.b64 db, {%2, %4};\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p, %6;\n}" ::"r"(d),
+        "r"(a), "r"(b_low), "r"(idesc), "r"(kDescHigh), "r"(e), "n"(kLoShift)
+        : "memory");
+}
 B200_DEVICE void commit_if(uint32_t e, uint64_t *bar) {
     asm volatile(
         "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
@@ -272,9 +284,9 @@ struct SplitView {
     bool by_weight = false;   // query tiles in the order of their key tiles
 };
 constexpr int kTop = 14;  // largest magnitudes in [2^14, 2^15); P <= 1 times 2^14
-// Rows and columns within 2^10 of their tile's largest: their elements hold 22 bits, or an absolute 2^-29 of
-// the row's and the column's largest.
-constexpr int kSpread = 10;
+// Rows and columns within 2^16 of their tile's largest: their elements hold 22 bits, or an absolute 2^-23 (K)
+// or 2^-33 (V) of the row's and the column's largest.
+constexpr int kSpread = 16;
 // A word of `exps`: the exponent, and whether the tile takes FFMA.
 B200_DEVICE int exps_word(int e, bool wide) { return 2 * e + static_cast<int>(wide); }
 B200_DEVICE int exps_exponent(int word) { return word >> 1; }
@@ -293,10 +305,11 @@ B200_DEVICE uint32_t finite_magnitude(float x) {
     const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
     return u < 0x7F800000u ? u : 0u;
 }
-// hi + lo = x (22 bits); a value that is no number stays one, in hi
-B200_DEVICE void split_f16(float x, __half &hi, __half &lo) {
+constexpr float kLoScale = static_cast<float>(1 << kLoShift);  // of V
+// hi + lo / lo_scale = x (22 bits); a value that is no number stays one, in hi
+B200_DEVICE void split_f16(float x, float lo_scale, __half &hi, __half &lo) {
     hi = __float2half_rn(x);
-    lo = finite_magnitude(x) || x == 0.f ? __float2half_rn(x - __half2float(hi)) : __half(0.f);
+    lo = finite_magnitude(x) || x == 0.f ? __float2half_rn((x - __half2float(hi)) * lo_scale) : __half(0.f);
 }
 B200_DEVICE void split_f16x2(uint64_t v, uint32_t &hi, uint32_t &lo) {
     const float2 x = of_pair(v);
@@ -369,7 +382,7 @@ __global__ void __launch_bounds__(kSplitThreads) packed_split_kernel(const Packe
 #pragma unroll
     for (int w = 0; w < W; ++w) top = max(top, warp_top[w]);
     const int e = top ? top_exponent(top) : kTop;  // (a tile of zeros: any)
-    const float s = pow2(kTop - e);
+    const float s = pow2(kTop - e), lo_scale = is_v ? kLoScale : 1.0f;
     if (threadIdx.x < D) {
         uint32_t c = 0;
 #pragma unroll
@@ -391,10 +404,10 @@ __global__ void __launch_bounds__(kSplitThreads) packed_split_kernel(const Packe
         const int el = threadIdx.x + i * kSplitThreads, r = el / V4, c = el % V4;
         if (r >= rows) continue;
         __half h[4], l[4];
-        split_f16(x[i].x * s, h[0], l[0]);
-        split_f16(x[i].y * s, h[1], l[1]);
-        split_f16(x[i].z * s, h[2], l[2]);
-        split_f16(x[i].w * s, h[3], l[3]);
+        split_f16(x[i].x * s, lo_scale, h[0], l[0]);
+        split_f16(x[i].y * s, lo_scale, h[1], l[1]);
+        split_f16(x[i].z * s, lo_scale, h[2], l[2]);
+        split_f16(x[i].w * s, lo_scale, h[3], l[3]);
         __half *d = dst + (first + r) * a.Hkv * D + 4 * c;
         *reinterpret_cast<uint2 *>(d) = *reinterpret_cast<const uint2 *>(h);
         *reinterpret_cast<uint2 *>(d + plane) = *reinterpret_cast<const uint2 *>(l);
@@ -617,12 +630,14 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             };
             // O (+)= P . a plane of V. P lies over the scores: 16 keys in 8 columns; F32: each 32
             // columns hold hi, then lo of their 32 keys
-            const auto values = [&](int slot, bool lo, int pl, int from, int to, bool add) {
+            const auto values = [&](int slot, bool lo, int pl, int from, int to, bool add, bool onto_lo) {
                 const uint32_t d = col_o(slot), pa = col_s(slot) + (lo ? 16 : 0), va = desc_low(at(pl), Ge::kBox);
 #pragma unroll
-                for (int kk = from; kk < to; ++kk)  // 16 keys: two 1024-byte atoms
-                    mma_ts(e, d, pa + (SPLIT ? 32 * (kk >> 1) + 8 * (kk & 1) : 8 * kk), va + kk * (2048 >> 4), kIdO,
-                           add || kk > 0);
+                for (int kk = from; kk < to; ++kk) {  // 16 keys: two 1024-byte atoms
+                    const uint32_t pk = pa + (SPLIT ? 32 * (kk >> 1) + 8 * (kk & 1) : 8 * kk), vk = va + kk * (2048 >> 4);
+                    if (onto_lo && kk == 0) mma_ts_onto_lo(e, d, pk, vk, kIdO);
+                    else mma_ts(e, d, pk, vk, kIdO, add || kk > 0);
+                }
             };
             constexpr int KK = kPtKeys / 16, KH = 3 * KK / 4;  // products of a V tile; of P's first part
             const auto issue_s = [&](int i) {
@@ -658,19 +673,19 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                 if (!ok) break;
                 tc_fence_after();
                 if (SPLIT) {
-                    values(slot, false, pl, 0, KK, false);
+                    values(slot, false, pl, 0, KK, false, false);
                     commit_if(e, &empty[pl % S]);
                     ok = landed(pl + 1);
                     if (!ok) break;
                     tc_fence_after();
-                    values(slot, true, pl + 1, 0, KK, true);
-                    values(slot, false, pl + 1, 0, KK, true);
+                    values(slot, true, pl + 1, 0, KK, true, true);
+                    values(slot, false, pl + 1, 0, KK, true, false);
                 } else {
-                    values(slot, false, pl, 0, KH, i >= SL);
+                    values(slot, false, pl, 0, KH, i >= SL, false);
                     ok = all(&p_full[slot], (i / SL) & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    values(slot, false, pl, KH, KK, true);
+                    values(slot, false, pl, KH, KK, true, false);
                 }
                 if (NT == 1 || slot == 1) commit_if(e, &empty[(pl + PL - 1) % S]);
                 if (SPLIT || i + SL >= steps) commit_if(e, &o_final[slot]);

@@ -149,10 +149,7 @@ def test_f32_hidden_keys_of_any_finite_value(cuda, layout, big, where):
     check_f32(got, q, k, v, 0, slice(0, 100))
 
 
-@pytest.mark.parametrize("layout", list(LAYOUTS))
-@pytest.mark.parametrize("power", [10, 20, 30])
-@pytest.mark.parametrize("case", ["v_columns", "k_columns", "v_rows", "k_rows"])
-def test_f32_magnitudes_within_a_tile(cuda, layout, power, case):
+def magnitudes_within_a_tile(layout, power, case):
     """Columns or rows of a tile that differ by 2^power: each output keeps its own digits."""
     T = 300
     q, k, v = inputs(34, LAYOUTS[layout], [T], [T], "f32")
@@ -168,6 +165,20 @@ def test_f32_magnitudes_within_a_tile(cuda, layout, power, case):
     else:
         k *= 2.0 ** (-power * (torch.arange(T, device="cuda") % 2))[:, None, None]
     check_f32(B.flash_attn_packed(q, k, v, cumulative([T])), q, k, v, 0)
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("power", [10, 20, 30])
+@pytest.mark.parametrize("case", ["v_columns", "k_columns", "v_rows", "k_rows"])
+def test_f32_magnitudes_within_a_tile(cuda, layout, power, case):
+    magnitudes_within_a_tile(layout, power, case)
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+@pytest.mark.parametrize("power", [12, 13, 15])
+@pytest.mark.parametrize("case", ["v_columns", "k_columns", "v_rows", "k_rows"])
+def test_f32_magnitudes_that_one_exponent_holds(cuda, layout, power, case):
+    magnitudes_within_a_tile(layout, power, case)
 
 
 @pytest.mark.parametrize("layout", list(LAYOUTS))
