@@ -48,7 +48,7 @@
 // Bound: at long contexts the chain scores -> softmax -> P -> product of a slot, against which the other
 // slot's runs: 8192 BF16 tokens, 32 / 8 heads of 128, 505 to 522 us by GPU, 1.05 to 1.09 PFLOP/s (64 to 66 % of a
 // large library matrix product's rate); the tensor cores are busy 54 to 60 % of the time. 2048 F32 tokens, 16 / 8
-// heads of 128, 82 us (209 TFLOP/s of the call's, 627 of the three products), the split kernel 7 us of it. Short
+// heads of 128, 81 to 82 us (209 to 212 TFLOP/s of the call's, 630 of the three products), the split kernel 7 us of it. Short
 // calls: a CTA's start and end, ~6 us (look-up 1, first copies 1.4, last product 0.8 to 1.7, output 2), beside ~0.9
 // us a step: 10 prompts of 1 to 1333 BF16 tokens, 16 / 8 heads of 128, 35 us. Two slots take all 512
 // columns of tensor memory and most of an SM's registers.

@@ -23,7 +23,7 @@
 //    split again over its ordered bit patterns. Then the kept weight of each warp's
 //    contiguous piece is summed, and the CTA in whose chunk the drawn sum lies searches
 //    that piece.
-// Bound: for a few rows the chain of about four cluster exchanges (151936 F32 logits: 14 to 17 us with one row); for
+// Bound: for a few rows the chain of about four cluster exchanges (151936 F32 logits: 14 to 18 us with one row); for
 // a large batch the instructions of the passes, each token's weight (an exponential and a 64-bit
 // shift) taking ~44 issue slots a warp, beside those chains. 256 rows of 151936 F32: greedy 55 us (2.8
 // TB/s), top-k 50 88, no filter 124, top-p 0.95 168 to 343 as the row is steep or flat, mixed filters 145 to 155.
@@ -740,7 +740,7 @@ cudaError_t sample_launch(SampleArgs a, int64_t rows, cudaStream_t st) {
     // CTAs a row: about 2,048 tokens each while a row's CTAs are fewer than the SMs; more
     // rows take fewer, as far as two chunks still fit an SM. F32, 1 / 2 / 4 / 8 CTAs a row: one row of
     // 32003 24.5 / 19.5 / 16.4 / 16.4 us; 64 rows 31 / 24 / 22 / 35, 256 rows 55 / 47 / 64 / 113; one row of
-    // 151936 104 / 59 / 25 / 22 (before top-k stopped at the threads' own largest tokens; 14 to 17 now).
+    // 151936 104 / 59 / 25 / 22 (before top-k stopped at the threads' own largest tokens; 14 to 18 now).
     const int64_t sms = device_sm_count();
     int c = 1;
     while (c < kMaxCluster && a.vocab > 2048 * c && rows * c < sms) c *= 2;
