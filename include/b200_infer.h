@@ -300,6 +300,90 @@ int b200_flash_attn_paged_batch(const void *q, int64_t q_seq_stride, int64_t q_h
 size_t b200_flash_attn_paged_batch_workspace_bytes(int64_t n_seqs, int64_t max_keys, int64_t D, int64_t Hq,
                                                    int64_t Hkv, int32_t dtype);
 
+/* A pool of cache blocks in 8 bits. A row (one token, one KV head: head_dim elements) is held
+ * as x = q 2^e: q in e4m3 (OCP FP8, no infinities) at
+ * k[b * block_stride + t * tok_stride + h * head_stride + d], and e in e8m0 (a byte, e + 127; 255 is NaN) at
+ * k_scale[b * scale_block_stride + t * scale_tok_stride + h * scale_head_stride]; V likewise. All strides
+ * count elements, here bytes. Rows of k and v must start on 16-byte boundaries; scales may be anywhere,
+ * and are read fastest where a head's lie next to each other (scale_tok_stride 1). head_dim 64 or 128. */
+typedef struct b200_kv_pool_q8 {
+    void *k, *v, *k_scale, *v_scale;
+    int64_t n_blocks, block_tokens;
+    int64_t block_stride, tok_stride, head_stride;
+    int64_t scale_block_stride, scale_tok_stride, scale_head_stride;
+    int64_t n_head_kv, head_dim;
+} b200_kv_pool_q8;
+
+/* b200_paged_kv_append into an 8-bit pool; k, v are F32, F16 or BF16 (`dtype`). Each row gets the least
+ * whole e >= -127 with max |x| <= 448 2^e, and its elements x 2^-e (exact) rounded to e4m3, ties to even: at
+ * most 2^-4 of the element off, or 2^(e - 10) where that is more. A row that holds an infinity or a NaN is
+ * held as zeros with the scale NaN, and reads as NaN. */
+int b200_paged_kv_append_q8(const void *k, int64_t k_tok_stride, int64_t k_head_stride, const void *v,
+                            int64_t v_tok_stride, int64_t v_head_stride, int32_t dtype, const int32_t *cu_new,
+                            const int32_t *seq_lens, int64_t n_seqs, int64_t n_tokens, const b200_kv_pool_q8 *pool,
+                            const int32_t *block_table, int64_t table_stride, int64_t max_blocks,
+                            int32_t *dev_status, void *stream);
+
+/* The inverse: rows of an 8-bit pool into packed rows k, v [n_rows][Hkv][D] of F32, F16 or BF16, as
+ * b200_flash_attn_packed takes them. Sequence s gets the rows [cu_rows[s], cu_rows[s + 1]), which are its last
+ * positions of the seq_lens[s] cached (all of them where the counts are equal). Values q 2^e are exact in F32
+ * and BF16 and rounded once to F16. Rows outside every sequence are left untouched; a row whose offsets, position or block
+ * are out of range is zero. */
+int b200_paged_kv_read_q8(const b200_kv_pool_q8 *pool, const int32_t *block_table, int64_t table_stride,
+                          int64_t max_blocks, const int32_t *cu_rows, const int32_t *seq_lens, int64_t n_seqs,
+                          int64_t n_rows, void *k, int64_t k_tok_stride, int64_t k_head_stride, void *v,
+                          int64_t v_tok_stride, int64_t v_head_stride, int32_t dtype, int32_t *dev_status, void *stream);
+
+/* b200_flash_attn_paged_batch over an 8-bit pool; q and out are F32, F16 or BF16 (`dtype`). The formula is that
+ * of the values q 2^e that the pool stands for; products are of F16 numbers (e4m3 is exact in F16) with F32 sums. Q rows
+ * and weights enter as two F16 numbers, 22 bits or an absolute 2^-39 of the row's largest. A scale of NaN makes the
+ * outputs that see the key NaN. */
+int b200_flash_attn_paged_batch_q8(const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
+                                   int64_t out_seq_stride, int64_t out_head_stride, int32_t dtype,
+                                   const b200_kv_pool_q8 *pool, const int32_t *block_table, int64_t table_stride,
+                                   int64_t max_blocks, const int32_t *seq_lens, int64_t n_seqs, int64_t Hq, float scale,
+                                   void *workspace, size_t workspace_bytes, int32_t *dev_status, void *stream);
+size_t b200_flash_attn_paged_batch_q8_workspace_bytes(int64_t n_seqs, int64_t max_keys, int64_t D, int64_t Hq,
+                                                      int64_t Hkv);
+
+/* b200_flash_attn_paged_batch for sequences that share prefixes (a common instruction, a document): group g is the
+ * sequences [cu_seqs[g], cu_seqs[g + 1]), which see the prefix_lens[g] positions of row g of prefix_table
+ * first, then the seq_lens[s] positions of their own rows of block_table (either may be 0; both tables name
+ * blocks of the one pool). Each prefix is read once for its group and its products run on the tensor
+ * cores with the group's rows together. Sequences outside every group see their own positions alone. A prefix with a
+ * block index out of range makes its group's rows zero; cu_seqs, prefix_lens and prefix_table are else treated as
+ * the other offsets, lengths and tables. */
+int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
+                                 int64_t out_seq_stride, int64_t out_head_stride, const b200_kv_pool *pool,
+                                 const int32_t *prefix_table, int64_t prefix_stride, int64_t prefix_blocks,
+                                 const int32_t *prefix_lens, const int32_t *cu_seqs, int64_t n_groups,
+                                 const int32_t *block_table, int64_t table_stride, int64_t max_blocks,
+                                 const int32_t *seq_lens, int64_t n_seqs, int64_t Hq, float scale, void *workspace,
+                                 size_t workspace_bytes, int32_t *dev_status, void *stream);
+size_t b200_flash_attn_paged_shared_workspace_bytes(int64_t n_seqs, int64_t max_keys, int64_t n_groups,
+                                                    int64_t max_prefix, int64_t D, int64_t Hq, int64_t Hkv, int32_t dtype);
+
+/* What a request says about its logits, before a token is drawn: per row of logits [n_rows][n_vocab], in
+ * this order,
+ *   repetition: a token of the row's history becomes x / r where x > 0, else x r;
+ *   frequency and presence: a token that the row has drawn `count` > 0 times (its history but the first
+ *   prompt_lens[row] tokens, the prompt; NULL: no prompt) becomes x - f count - p;
+ *   bias: x + bias_values[i] for token bias_ids[i] (of several for one token the last counts);
+ *   mask: a token whose bit (t % 32 of word t / 32 of the row's words) is 0 becomes -inf, whatever it was.
+ * Row s has the history tokens [cu_tokens[s], cu_tokens[s + 1]) and the biases [cu_bias[s], cu_bias[s + 1]). Sums are F32, in
+ * this order, rounded once to the type. out may be logits itself (with the same stride), and what does not
+ * change is then neither read nor written where a mask allows it; else the two may not overlap. Any of tokens (with cu_tokens),
+ * the three penalties (float32 [n_rows]; NULL: off), bias_ids (with bias_values and cu_bias) and mask may be NULL. Rows any
+ * alignment; strides count elements (of mask: words). A token id out of range or offsets that are not ascending within the
+ * given totals are left out and B200_DEV_BAD_TOKEN / B200_DEV_BAD_POSITION recorded; a repetition penalty
+ * that is not positive and finite, or another that is not finite, is off for its row and B200_DEV_BAD_LOGITS recorded. */
+int b200_adjust_logits(const void *logits, int64_t row_stride, void *out, int64_t out_row_stride, int64_t n_rows,
+                       int64_t n_vocab, int32_t dtype, const int32_t *tokens, int64_t n_tokens,
+                       const int32_t *cu_tokens, const int32_t *prompt_lens, const float *repetition,
+                       const float *frequency, const float *presence, const int32_t *bias_ids,
+                       const float *bias_values, int64_t n_biases, const int32_t *cu_bias, const uint32_t *mask,
+                       int64_t mask_stride, int32_t *dev_status, void *stream);
+
 /* Samples one token per row of logits [n_rows][n_vocab] (row stride `row_stride`
  * elements, any alignment) from given uniform numbers u[n_rows] in [0, 1). Per row,
  * with device arrays temperature (required) and top_k, top_p, min_p (each nullable:

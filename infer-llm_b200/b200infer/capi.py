@@ -99,6 +99,18 @@ _SIGS = {
     "b200_flash_attn_paged_batch": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _f32,
                                      _vp, _sz, _vp, _vp], C.c_int),
     "b200_flash_attn_paged_batch_workspace_bytes": ([_i64] * 5 + [_i32], _sz),
+    "b200_paged_kv_append_q8": ([_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp],
+                                C.c_int),
+    "b200_paged_kv_read_q8": ([_vp, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp],
+                              C.c_int),
+    "b200_flash_attn_paged_batch_q8": ([_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _f32,
+                                        _vp, _sz, _vp, _vp], C.c_int),
+    "b200_flash_attn_paged_batch_q8_workspace_bytes": ([_i64] * 5, _sz),
+    "b200_flash_attn_paged_shared": ([_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _i64,
+                                      _vp, _i64, _i64, _f32, _vp, _sz, _vp, _vp], C.c_int),
+    "b200_flash_attn_paged_shared_workspace_bytes": ([_i64] * 7 + [_i32], _sz),
+    "b200_adjust_logits": ([_vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp,
+                            _vp, _i64, _vp, _vp], C.c_int),
     "b200_sample": ([_vp, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp], C.c_int),
     "b200_engine_inject_withhold": ([_vp, C.c_int32, C.c_int32], C.c_int),
     "b200_engine_set_decode_launch_counter": ([_vp, C.c_uint64], C.c_int),
@@ -326,6 +338,16 @@ class _KVPool(C.Structure):
 _POOL = struct.Struct("@PPqqqqqqqi4x")  # the same, packed (a call of its own per decode step and layer)
 
 
+class _KVPoolQ8(C.Structure):
+    """b200_kv_pool_q8."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("n_blocks", _i64), ("block_tokens", _i64),
+                ("block_stride", _i64), ("tok_stride", _i64), ("head_stride", _i64), ("scale_block_stride", _i64),
+                ("scale_tok_stride", _i64), ("scale_head_stride", _i64), ("n_head_kv", _i64), ("head_dim", _i64)]
+
+
+_POOL_Q8 = struct.Struct("@PPPPqqqqqqqqqq")
+
+
 class _Host:
     """What the batched calls take from torch, looked up once: a decode step makes several of
     these calls per layer, and each is only microseconds on the device."""
@@ -342,6 +364,11 @@ class _Host:
         self.packed, self.packed_bytes = L.b200_flash_attn_packed, L.b200_flash_attn_packed_workspace_bytes
         self.batch, self.batch_bytes = L.b200_flash_attn_paged_batch, L.b200_flash_attn_paged_batch_workspace_bytes
         self.append, self.sample = L.b200_paged_kv_append, L.b200_sample
+        self.e4m3, self.e8m0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+        self.append_q8, self.read_q8 = L.b200_paged_kv_append_q8, L.b200_paged_kv_read_q8
+        self.batch_q8, self.batch_q8_bytes = L.b200_flash_attn_paged_batch_q8, L.b200_flash_attn_paged_batch_q8_workspace_bytes
+        self.shared, self.shared_bytes = L.b200_flash_attn_paged_shared, L.b200_flash_attn_paged_shared_workspace_bytes
+        self.adjust = L.b200_adjust_logits
 
 
 _host = None
@@ -500,6 +527,173 @@ def flash_attn_paged_batch(q, k_pool, v_pool, block_table, seq_lens, scale=0.0, 
     _chk("b200_flash_attn_paged_batch", h.batch(
         q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], pool, table, stride, blocks,
         _vector(seq_lens, "seq_lens", n, h.i32, dev), n, Hq, scale, None if ws is None else ws.data_ptr(), nbytes,
+        _status_word(status, dev), h.stream(dev)))
+    return out
+
+
+def _pool_q8(k_pool, v_pool, k_scale, v_scale, dev):
+    h = _host
+    s, e = k_pool.stride(), k_scale.stride()
+    if len(s) != 4 or k_pool.dtype != h.e4m3 or v_pool.dtype != h.e4m3 or k_pool.shape != v_pool.shape or \
+            s != v_pool.stride() or s[3] != 1 or k_pool.get_device() != dev or v_pool.get_device() != dev:
+        raise ValueError("k_pool, v_pool: expected two (blocks, block_tokens, Hkv, D) float8_e4m3fn tensors alike, last axis "
+                         f"contiguous, on cuda:{dev}")
+    n, bt, Hkv, D = k_pool.shape
+    if k_scale.dtype != h.e8m0 or v_scale.dtype != h.e8m0 or k_scale.shape != (n, Hkv, bt) or v_scale.shape != (n, Hkv, bt) or \
+            e != v_scale.stride() or k_scale.get_device() != dev or v_scale.get_device() != dev:
+        raise ValueError(f"k_scale, v_scale: expected two (blocks, Hkv, block_tokens) float8_e8m0fnu tensors alike on cuda:{dev}")
+    return _POOL_Q8.pack(k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, bt, s[0], s[1], s[2],
+                         e[0], e[2], e[1], Hkv, D), bt, Hkv, D
+
+
+def paged_kv_append_q8(k, v, cu_new, seq_lens, k_pool, v_pool, k_scale, v_scale, block_table, status=None):
+    """paged_kv_append into an 8-bit cache: k_pool, v_pool (blocks, block_tokens, Hkv, D) float8_e4m3fn and k_scale,
+    v_scale (blocks, Hkv, block_tokens) float8_e8m0fnu, one scale a row of D elements. Each row gets the least power of
+    two with which its largest element is at most 448; a row that holds an infinity or a NaN reads as NaN."""
+    h, dev = _start(k)
+    if h.current() != dev:
+        return _elsewhere(paged_kv_append_q8, dev, k, v, cu_new, seq_lens, k_pool, v_pool, k_scale, v_scale, block_table, status)
+    kind, dt = k.dtype, _dtype(k)
+    pool, _, Hkv, D = _pool_q8(k_pool, v_pool, k_scale, v_scale, dev)
+    ks, vs = _rows(k, "k", kind, dev), _rows(v, "v", kind, dev)
+    T = k.shape[0]
+    if k.shape != v.shape or k.shape[1] != Hkv or k.shape[2] != D:
+        raise ValueError("k, v: expected (T, Hkv, D)")
+    n = seq_lens.shape[0]
+    table, stride, blocks = _table(block_table, n, dev)
+    _chk("b200_paged_kv_append_q8", h.append_q8(
+        k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], dt, _vector(cu_new, "cu_new", n + 1, h.i32, dev),
+        _vector(seq_lens, "seq_lens", n, h.i32, dev), n, T, pool, table, stride, blocks, _status_word(status, dev),
+        h.stream(dev)))
+
+
+def paged_kv_read_q8(cu_rows, seq_lens, n_rows, k_pool, v_pool, k_scale, v_scale, block_table, dtype=None, k=None, v=None,
+                     status=None):
+    """Rows of an 8-bit cache as packed rows (n_rows, Hkv, D), k and v: sequence s gets the rows [cu_rows[s],
+    cu_rows[s + 1]), its last positions of the seq_lens[s] cached. `dtype` (None: bfloat16) is that of new tensors, else
+    they go to the given `k` and `v`, whose rows outside every sequence stay as they are (of new tensors: undefined).
+    For flash_attn_packed, where a prompt goes on behind a cached head."""
+    h, dev = _start(k_pool)
+    if h.current() != dev:
+        return _elsewhere(paged_kv_read_q8, dev, cu_rows, seq_lens, n_rows, k_pool, v_pool, k_scale, v_scale, block_table, dtype,
+                          k, v, status)
+    pool, _, Hkv, D = _pool_q8(k_pool, v_pool, k_scale, v_scale, dev)
+    if k is None and v is None:
+        kind = dtype or h.torch.bfloat16
+        k = h.empty((n_rows, Hkv, D), device=k_pool.device, dtype=kind)
+        v = h.empty_like(k)
+    elif k is None or v is None or k.shape != v.shape or k.shape != (n_rows, Hkv, D) or (dtype or k.dtype) != k.dtype:
+        raise ValueError("k, v: expected both (n_rows, Hkv, D), of `dtype`")
+    kind, dt = k.dtype, _dtype(k)
+    ks, vs = _rows(k, "k", kind, dev), _rows(v, "v", kind, dev)
+    n = seq_lens.shape[0]
+    table, stride, blocks = _table(block_table, n, dev)
+    _chk("b200_paged_kv_read_q8", h.read_q8(
+        pool, table, stride, blocks, _vector(cu_rows, "cu_rows", n + 1, h.i32, dev), _vector(seq_lens, "seq_lens", n, h.i32, dev),
+        n, n_rows, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], dt, _status_word(status, dev), h.stream(dev)))
+    return k, v
+
+
+def flash_attn_paged_batch_q8(q, k_pool, v_pool, k_scale, v_scale, block_table, seq_lens, scale=0.0, out=None, workspace=None,
+                              status=None):
+    """flash_attn_paged_batch over an 8-bit cache (arguments as for paged_kv_append_q8): q (n, Hq, D) of float32,
+    float16 or bfloat16 against the values that the cache stands for. Returns (n, Hq, D)."""
+    h, dev = _start(q)
+    if h.current() != dev:
+        return _elsewhere(flash_attn_paged_batch_q8, dev, q, k_pool, v_pool, k_scale, v_scale, block_table, seq_lens, scale, out,
+                          workspace, status)
+    kind, dt = q.dtype, _dtype(q)
+    pool, bt, Hkv, Dk = _pool_q8(k_pool, v_pool, k_scale, v_scale, dev)
+    qs = _rows(q, "q", kind, dev)
+    n, Hq, D = q.shape
+    if D != Dk or Hkv <= 0 or Hq % Hkv:
+        raise ValueError("q: shape does not go with the pools")
+    table, stride, blocks = _table(block_table, n, dev)
+    out = _out_rows(out, q, dev)
+    os = out.stride()
+    nbytes = h.batch_q8_bytes(n, blocks * bt, D, Hq, Hkv)
+    ws = _scratch(workspace, nbytes, q, dev)
+    _chk("b200_flash_attn_paged_batch_q8", h.batch_q8(
+        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], dt, pool, table, stride, blocks,
+        _vector(seq_lens, "seq_lens", n, h.i32, dev), n, Hq, scale, None if ws is None else ws.data_ptr(), nbytes,
+        _status_word(status, dev), h.stream(dev)))
+    return out
+
+
+def flash_attn_paged_shared(q, k_pool, v_pool, prefix_table, prefix_lens, cu_seqs, block_table, seq_lens, scale=0.0, out=None,
+                            workspace=None, status=None):
+    """flash_attn_paged_batch of sequences that share prefixes: group g, the sequences [cu_seqs[g], cu_seqs[g + 1]),
+    sees the prefix_lens[g] positions of row g of prefix_table first, then each its seq_lens[s] own positions
+    of block_table (int32; both name blocks of the pools). Returns (n, Hq, D)."""
+    h, dev = _start(q)
+    if h.current() != dev:
+        return _elsewhere(flash_attn_paged_shared, dev, q, k_pool, v_pool, prefix_table, prefix_lens, cu_seqs, block_table,
+                          seq_lens, scale, out, workspace, status)
+    kind, dt = q.dtype, _dtype(q)
+    if k_pool.get_device() != dev or k_pool.dtype != kind:
+        raise ValueError(f"k_pool: expected {kind} on cuda:{dev}")
+    pool, bt, Hkv, Dk = _pool(k_pool, v_pool)
+    qs = _rows(q, "q", kind, dev)
+    n, Hq, D = q.shape
+    if D != Dk or Hkv <= 0 or Hq % Hkv:
+        raise ValueError("q: shape does not go with the pools")
+    groups = prefix_lens.shape[0]
+    table, stride, blocks = _table(block_table, n, dev)
+    ptable, pstride, pblocks = _table(prefix_table, groups, dev)
+    out = _out_rows(out, q, dev)
+    os = out.stride()
+    nbytes = h.shared_bytes(n, blocks * bt, groups, pblocks * bt, D, Hq, Hkv, dt)
+    ws = _scratch(workspace, nbytes, q, dev)
+    _chk("b200_flash_attn_paged_shared", h.shared(
+        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], pool, ptable, pstride, pblocks,
+        _vector(prefix_lens, "prefix_lens", groups, h.i32, dev), _vector(cu_seqs, "cu_seqs", groups + 1, h.i32, dev), groups,
+        table, stride, blocks, _vector(seq_lens, "seq_lens", n, h.i32, dev), n, Hq, scale,
+        None if ws is None else ws.data_ptr(), nbytes, _status_word(status, dev), h.stream(dev)))
+    return out
+
+
+def adjust_logits(logits, tokens=None, cu_tokens=None, prompt_lens=None, repetition=None, frequency=None, presence=None,
+                  bias_ids=None, bias_values=None, cu_bias=None, mask=None, out=None, status=None):
+    """Logits (n, vocab) as their rows' requests want them before `sample`. Row s has the history `tokens`
+    [cu_tokens[s], cu_tokens[s + 1]) (int32), of which the first prompt_lens[s] are its prompt. In this order: a
+    token of the history is divided by (where positive, else multiplied by) repetition[s]; one drawn c > 0 times
+    after the prompt loses c frequency[s] + presence[s]; token bias_ids[i] gains bias_values[i], i in [cu_bias[s],
+    cu_bias[s + 1]) (the last of several for one token); tokens whose bit is 0 in mask (n, ceil(vocab / 32)) int32, bit t %
+    32 of word t / 32, become -inf. What is None is off. `out` (None: a new tensor) may be `logits`. Returns out."""
+    h, dev = _start(logits)
+    if h.current() != dev:
+        return _elsewhere(adjust_logits, dev, logits, tokens, cu_tokens, prompt_lens, repetition, frequency, presence, bias_ids,
+                          bias_values, cu_bias, mask, out, status)
+    st = logits.stride()
+    dt = _dtype(logits)
+    if len(st) != 2 or (st[1] != 1 and logits.shape[1] != 1):
+        raise ValueError("logits: expected (n, vocab), last axis contiguous")
+    n, vocab = logits.shape
+    if out is None:
+        out = h.empty((n, vocab), device=logits.device, dtype=logits.dtype)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.get_device() != dev or \
+            (out.stride(1) != 1 and vocab != 1):
+        raise ValueError("out: expected logits' shape and type, last axis contiguous")
+
+    def row(t, name, kind, m=n):
+        return None if t is None else _vector(t, name, m, kind, dev)
+
+    if (tokens is None) != (cu_tokens is None) or (bias_ids is None) != (bias_values is None) or \
+            (bias_ids is None) != (cu_bias is None):
+        raise ValueError("tokens and cu_tokens go together, and bias_ids, bias_values and cu_bias")
+    T, m = 0 if tokens is None else tokens.shape[0], 0 if bias_ids is None else bias_ids.shape[0]
+    words, word_stride = None, 0
+    if mask is not None:
+        ms = mask.stride()
+        if len(ms) != 2 or mask.shape[0] != n or mask.shape[1] * 32 < vocab or mask.dtype != h.i32 or \
+                mask.get_device() != dev or (ms[1] != 1 and mask.shape[1] != 1):
+            raise ValueError(f"mask: expected int32 (n, ceil(vocab / 32)) on cuda:{dev}, last axis contiguous")
+        words, word_stride = mask.data_ptr(), ms[0]
+    _chk("b200_adjust_logits", h.adjust(
+        logits.data_ptr(), st[0], out.data_ptr(), out.stride(0), n, vocab, dt, row(tokens, "tokens", h.i32, T), T,
+        row(cu_tokens, "cu_tokens", h.i32, n + 1), row(prompt_lens, "prompt_lens", h.i32), row(repetition, "repetition", h.f32),
+        row(frequency, "frequency", h.f32), row(presence, "presence", h.f32), row(bias_ids, "bias_ids", h.i32, m),
+        row(bias_values, "bias_values", h.f32, m), m, row(cu_bias, "cu_bias", h.i32, n + 1), words, word_stride,
         _status_word(status, dev), h.stream(dev)))
     return out
 
