@@ -1,14 +1,37 @@
 // b200_flash_attn_paged_batch_q8: one query token for each of many sequences against an 8-bit paged cache.
 //
-// out_b = sum_j softmax_j(scale 2^ek_j q_b . kq_j) 2^ev_j vq_j over the keys j < seq_lens[b].
-#include "attention_rows.cuh"
-#include "gemv.cuh"
+// out_b = sum_j softmax_j(t_j) 2^ev_j vq_j over the keys j < seq_lens[b], t_j = scale 2^ek_j q_b . kq_j, with kq, vq in e4m3. Every
+// cached row is read once (once per 16 query heads of its KV head), so HBM bounds the operator: 2 (D + 1) bytes and 4 D G flops a
+// key and KV head.
+//
+//  * Work split, copies and joins as for the 16-bit caches (attention_paged_batch.cu): all key tiles of all (sequence,
+//    KV head) pairs are one line cut into equal shares, each warp streams its own sub-tiles of 32 keys (8 KB of K and V at head_dim 128)
+//    through a private ring, and few short pairs take one launch of clusters.
+//  * Products are mma.sync m16n8k16 of F16 numbers for all query types: e4m3 is exact in F16. The order of the 16 dimensions of a
+//    product is free, so a lane takes four neighbouring bytes of a key (ldmatrix) as the two halves of its fragment. V comes
+//    transposed in pairs of dimensions; one byte permutation a word parts the even from the odd ones.
+//  * A row of Q is scaled by a power of two to a largest magnitude in [2^14, 2^15) and enters as one F16 number (F16, BF16: exact, or
+//    2^-39 of the row's largest) or as two (F32: 22 bits). Up to eight query heads the second takes the unused rows 8 .. 15
+//    of the same product.
+//  * The scales 2^ek multiply the scores. The scales 2^ev go into the weights: w_j = 2^(t_j log2 e + ev_j - N + 14), N the running maximum of
+//    the exponent, as two F16 numbers. N has a maximum of its own, so keys whose V is far larger than that of the heaviest key keep their
+//    bits; the sum of the weights goes by the scores' maximum M. At the end 2^(N - M - 14) takes both together.
+// Rows past a sequence's end are not read; they and keys of invalid blocks get weight 0.
+#include "paged_line.cuh"
 #include "paged_q8.cuh"
 
 namespace b200 {
 namespace {
 
-constexpr int64_t kMostKeys = INT32_MAX - 256;
+constexpr int kP8Warps = 4;
+constexpr int kP8Threads = 32 * kP8Warps;
+constexpr int kP8MostCtas = 320;
+constexpr int kP8JoinThreads = 256;
+constexpr int kP8Cluster = 8;
+constexpr int kP8ClusterKeys = 4096;
+constexpr int kP8Sub = 32;                  // keys of a warp's sub-tile
+constexpr int kP8Tile = kP8Sub * kP8Warps;  // keys of a tile
+constexpr int kP8Top = 14;                  // weights are at most 2^14, F16's largest power of two but one
 
 struct P8Args {
     const void *q = nullptr;
@@ -23,51 +46,525 @@ struct P8Args {
     int64_t table_stride = 0;
     int64_t max_keys = 0;  // positions a table row covers (fits 31 bits)
     uint32_t bt = 1;
-    int n_seqs = 0, G = 0, Hkv = 0;
-    float sl2 = 0.f;  // scale * log2 e
+    int n_seqs = 0, G = 0, VH = 0, HG = 0;  // query heads a KV head; (KV head, head group) pairs; groups a KV head
+    float sl2 = 0.f;                        // scale * log2 e
+    float *ws = nullptr;
     int32_t *status = nullptr;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(32 * kArWarps) paged_q8_rows_kernel(const __grid_constant__ P8Args a) {
-    constexpr int E = D / 32;
-    const int b = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.Hkv)), h = blockIdx.x % static_cast<unsigned>(a.Hkv);
-    const int64_t len = __ldg(a.lens + b), keys = min64(max64(len, 0), a.max_keys);
-    if (len != keys && threadIdx.x == 0 && h == 0) set_status(a.status, B200_DEV_BAD_POSITION);
-    const T *q = static_cast<const T *>(a.q) + b * a.q_seq + static_cast<int64_t>(h) * a.G * a.q_head;
-    T *out = static_cast<T *>(a.out) + b * a.o_seq + static_cast<int64_t>(h) * a.G * a.o_head;
-    attend_rows<D>(
-        a.G, keys, a.sl2,
-        [&](int64_t j, int lane, float (&k)[E], float (&v)[E]) {
-            const uint32_t slot = static_cast<uint32_t>(j) / a.bt;
-            const int64_t blk = __ldg(a.table + b * a.table_stride + slot), t = static_cast<uint32_t>(j) - slot * a.bt;
-            if (blk < 0 || blk >= a.n_blocks) {
-                set_status(a.status, B200_DEV_BAD_POSITION);
-                return false;
+template <int D, int HB>
+struct P8Geometry {
+    static constexpr int kStages = 3;
+    static constexpr int kChunks = D / 16;
+    static constexpr int kHalf = kP8Sub * D;     // K (or V) bytes of a sub-tile
+    static constexpr int kRec = HB * (D + 3);    // floats of a partial: o, then m, l, n
+    static constexpr size_t kRing = static_cast<size_t>(kP8Warps) * kStages * 2 * kHalf;
+    static constexpr size_t kStat = static_cast<size_t>(kP8Warps) * 3 * HB * 4;
+    static constexpr size_t kScale = static_cast<size_t>(kP8Warps) * kStages * kP8Sub * 8;
+    static constexpr size_t kSmem = kRing + kStat + kScale + kP8Warps * kStages * 4;
+    static constexpr size_t kSmemCluster = kSmem + kRec * 4;
+    static_assert(HB * D * 4 <= 2 * kHalf, "a warp's partial takes the place of its last sub-tile");
+    static_assert(2 * (kSmemCluster + 1024) <= 228 * 1024, "two CTAs an SM");
+};
+
+B200_DEVICE float p8_pow2(int e) { return __uint_as_float(static_cast<uint32_t>(max(-126, min(127, e)) + 127) << 23); }
+// 2^x of numbers that may leave its range by half
+B200_DEVICE float p8_unscale(float x, float e) {
+    const float f = exp2_approx(0.5f * e);
+    return x * f * f;
+}
+// m - M for running maxima of which both may be -inf
+B200_DEVICE float p8_less(float m, float M) { return m - (M == -INFINITY ? 0.f : M); }
+
+// One warp's running softmax: lane (g = lane / 4, t = lane % 4) holds head rows g (and g + 8 of 16), output columns
+// 16 c + 4 t .. + 3.
+template <typename T, int D, int HB>
+struct P8State {
+    static constexpr bool FULL = HB > 8, TWO = __is_same(T, float);
+    static constexpr int R = FULL ? 2 : 1;  // head rows a lane holds
+    uint32_t q[D / 16][2 * R], ql[TWO ? D / 16 : 1][2 * R];
+    float o[D / 16][2][4];  // even and odd columns: rows g and g + 8; without FULL, row g's shares of the weights' two terms
+    float m[R], l[R], n[R], qs[R];
+
+    B200_DEVICE void begin(const P8Args &a, int b, int h0, int heads, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            m[r] = n[r] = -INFINITY;
+            l[r] = 0.f;
+            const bool ok = g + 8 * r < heads;
+            const T *row = static_cast<const T *>(a.q) + b * a.q_seq + (h0 + g + 8 * r) * a.q_head + 4 * t;
+            float x[D / 16][4];
+            uint32_t top = 0;  // the largest finite magnitude
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s) {
+                if constexpr (TWO) {
+                    const float4 v = ok ? __ldg(reinterpret_cast<const float4 *>(row + 16 * s)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[s][0] = v.x, x[s][1] = v.y, x[s][2] = v.z, x[s][3] = v.w;
+                } else {
+                    const uint2 v = ok ? __ldg(reinterpret_cast<const uint2 *>(row + 16 * s)) : make_uint2(0, 0);
+                    const float2 lo = unpack2<T>(v.x), hi = unpack2<T>(v.y);
+                    x[s][0] = lo.x, x[s][1] = lo.y, x[s][2] = hi.x, x[s][3] = hi.y;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t u = __float_as_uint(x[s][i]) & 0x7FFFFFFFu;
+                    if (u < 0x7F800000u) top = max(top, u);
+                }
             }
-            const int64_t at = blk * a.block_stride + t * a.tok_stride + h * a.head_stride + lane * E;
-            const int64_t se = blk * a.scale_block + t * a.scale_tok + h * a.scale_head;
-            const float fk = e8m0_value(a.ke[se]), fv = e8m0_value(a.ve[se]);
-            for (int e = 0; e < E; e += 2) {
-                const uint32_t x = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t *>(a.k + at + e));
-                const uint32_t y = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t *>(a.v + at + e));
-                const float2 xf = __half22float2(*reinterpret_cast<const __half2 *>(&x));
-                const float2 yf = __half22float2(*reinterpret_cast<const __half2 *>(&y));
-                k[e] = xf.x * fk, k[e + 1] = xf.y * fk, v[e] = yf.x * fv, v[e + 1] = yf.y * fv;
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = top ? max(-100, static_cast<int>(top >> 23) - 127) - 14 : 0;
+            const float f = p8_pow2(-e);
+            qs[r] = a.sl2 * p8_pow2(e);
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const float y0 = x[s][2 * u] * f, y1 = x[s][2 * u + 1] * f;
+                    const uint32_t hi = pack2<__half>(y0, y1);
+                    q[s][u * R + r] = hi;
+                    if constexpr (TWO) {  // (the rest of an infinity or NaN would be NaN; it stays in the first)
+                        const float2 h = unpack2<__half>(hi);
+                        ql[s][u * R + r] = pack2<__half>(fabsf(y0) < INFINITY ? y0 - h.x : 0.f, fabsf(y1) < INFINITY ? y1 - h.y : 0.f);
+                    }
+                }
+        }
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[c][0][u] = o[c][1][u] = 0.f;
+    }
+
+    // 32 keys at sk / sv (rows of D bytes, chunks swizzled by `chunk_at`), their scales at `scales` (2^ek, ev); bit j of
+    // `live`: key j takes part.
+    B200_DEVICE void keys(uint32_t sk, uint32_t sv, uint32_t live, const float2 *scales, int lane) {
+        const int mat = lane >> 3, rr = lane & 7, t2 = 2 * (lane & 3);
+        float s[4][2 * (FULL || TWO ? 2 : 1)];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int u = 0; u < (FULL || TWO ? 4 : 2); ++u) s[j][u] = 0.f;
+        const uint32_t row = (8 * mat + rr) * D;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t kf[4];
+            ldsm4(kf, sk + row + chunk_at(ks, rr));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t b0 = e4m3x2_to_f16x2(kf[j]), b1 = e4m3x2_to_f16x2(kf[j] >> 16);
+                if constexpr (FULL) {
+                    mma16<__half, true>(s[j], q[ks], b0, b1);
+                    if constexpr (TWO) mma16<__half, true>(s[j], ql[ks], b0, b1);
+                } else if constexpr (TWO) {
+                    const uint32_t both[4] = {q[ks][0], ql[ks][0], q[ks][1], ql[ks][1]};
+                    mma16<__half, true>(s[j], both, b0, b1);
+                } else {
+                    mma16<__half, false>(s[j], q[ks], b0, b1);
+                }
             }
-            return true;
-        },
-        [&](int g, int d) { return to_f32<T>(q[g * a.q_head + d]); },
-        [&](int g, int d, float x) { out[g * a.o_head + d] = from_f32<T>(x); });
+        }
+        float ke[4][2], ve[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float4 x = *reinterpret_cast<const float4 *>(scales + 8 * j + t2);
+            ke[j][0] = x.x, ve[j][0] = x.y, ke[j][1] = x.z, ve[j][1] = x.w;
+        }
+        uint32_t hi[2][2 * R], lo[2][2 * R];  // A fragments of the weights: 16 keys each, [key half][row]
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float x[4][2], mx = -INFINITY, nx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float y = s[j][2 * r + u];
+                    if constexpr (TWO && !FULL) y += s[j][2 + u];
+                    x[j][u] = (live >> (8 * j + t2 + u)) & 1u ? y * qs[r] * ke[j][u] : -INFINITY;
+                    mx = fmaxf(mx, x[j][u]);
+                    nx = fmaxf(nx, x[j][u] + ve[j][u]);
+                }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            nx = fmaxf(nx, __shfl_xor_sync(0xffffffffu, nx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            nx = fmaxf(nx, __shfl_xor_sync(0xffffffffu, nx, 2));
+            const float mn = fmaxf(m[r], mx), nn = fmaxf(n[r], nx);
+            if (__any_sync(0xffffffffu, mn > m[r] || nn > n[r])) {
+                l[r] *= exp2_approx(p8_less(m[r], mn));
+                const float f = exp2_approx(p8_less(n[r], nn));
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+                    for (int u = FULL ? 2 * r : 0; u < (FULL ? 2 * r + 2 : 4); ++u) o[c][0][u] *= f, o[c][1][u] *= f;
+            }
+            m[r] = mn;
+            n[r] = nn;
+            const float ms = mn == -INFINITY ? 0.f : mn, ns = (nn == -INFINITY ? 0.f : nn) - static_cast<float>(kP8Top);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                l[r] += exp2_approx(x[j][0] - ms) + exp2_approx(x[j][1] - ms);
+                const float w0 = exp2_approx(x[j][0] + ve[j][0] - ns), w1 = exp2_approx(x[j][1] + ve[j][1] - ns);
+                const uint32_t h = pack2<__half>(w0, w1);
+                const float2 f = unpack2<__half>(h);
+                hi[j >> 1][(j & 1) * R + r] = h;
+                lo[j >> 1][(j & 1) * R + r] = pack2<__half>(w0 - f.x, w1 - f.y);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) {
+            uint32_t vf[4], x[4][2];
+            ldsm4_t(vf, sv + row + chunk_at(c, rr));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // (key, column) bytes 00 01 10 11 as even and odd columns
+                const uint32_t p = __byte_perm(vf[j], 0, 0x3120);
+                x[j][0] = e4m3x2_to_f16x2(p), x[j][1] = e4m3x2_to_f16x2(p >> 16);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if constexpr (FULL) {
+                        mma16<__half, true>(o[c][u], hi[h], x[2 * h][u], x[2 * h + 1][u]);
+                        mma16<__half, true>(o[c][u], lo[h], x[2 * h][u], x[2 * h + 1][u]);
+                    } else {  // the unused rows 8 .. 15 take the weights' second term
+                        const uint32_t both[4] = {hi[h][0], lo[h][0], hi[h][1], lo[h][1]};
+                        mma16<__half, true>(o[c][u], both, x[2 * h][u], x[2 * h + 1][u]);
+                    }
+                }
+        }
+    }
+    // chunk c of a row whose number is rr modulo 8, so that eight rows' chunks fall into eight different bank groups
+    static B200_DEVICE uint32_t chunk_at(int c, int rr) {
+        return static_cast<uint32_t>(D == 128 ? (c ^ rr) : (c ^ (rr >> 1))) << 4;
+    }
+
+    // this warp's partial: o [HB][D], and m, l, n [HB] each
+    B200_DEVICE void store(float *po, float *stat, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+            const int h = g + 8 * r;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                const float *e = o[c][0], *d = o[c][1];
+                *reinterpret_cast<float4 *>(po + h * D + 16 * c + 4 * t) =
+                    FULL ? make_float4(e[2 * r], d[2 * r], e[2 * r + 1], d[2 * r + 1])
+                         : make_float4(e[0] + e[2], d[0] + d[2], e[1] + e[3], d[1] + d[3]);
+            }
+            if (t == 0) stat[h] = m[r], stat[HB + h] = l[r], stat[2 * HB + h] = n[r];
+        }
+    }
+};
+
+// CL: a cluster of kP8Cluster CTAs takes one pair, and writes its output.
+template <typename T, int D, int HB, bool CL>
+__global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_constant__ P8Args a) {
+    using Ge = P8Geometry<D, HB>;
+    extern __shared__ __align__(128) unsigned char p8_smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float *stat = reinterpret_cast<float *>(p8_smem + Ge::kRing);  // [warp][m, l, n][HB]
+    float2 *scales = reinterpret_cast<float2 *>(p8_smem + Ge::kRing + Ge::kStat) + warp * Ge::kStages * kP8Sub;
+    uint32_t *live = reinterpret_cast<uint32_t *>(p8_smem + Ge::kRing + Ge::kStat + Ge::kScale) + warp * Ge::kStages;
+    float *own = reinterpret_cast<float *>(p8_smem + Ge::kSmem);  // CL: this CTA's record
+    const uint32_t ring_at = warp * Ge::kStages * 2 * Ge::kHalf, ring = smem_addr(p8_smem) + ring_at;
+
+    int64_t u0 = 0, u1 = 0;
+    Place at = {};  // what is computed
+    if constexpr (CL) {
+        const int pair = blockIdx.x / kP8Cluster, rank = blockIdx.x % kP8Cluster;
+        at.b = pair / a.VH;
+        at.vh = pair % a.VH;
+        at.len = seq_len(a, at.b);
+        at.tiles = (at.len + kP8Tile - 1) / kP8Tile;
+        at.t = at.tiles * rank / kP8Cluster;
+        at.left = at.tiles * (rank + 1) / kP8Cluster - at.t;
+        if (rank == 0 && at.vh == 0 && threadIdx.x == 0) report_length(a, at.b);
+        if (at.left == 0)  // no keys: nothing to add
+            for (int i = threadIdx.x; i < Ge::kRec; i += kP8Threads)
+                own[i] = i < HB * D || (i >= HB * (D + 1) && i < HB * (D + 2)) ? 0.f : -INFINITY;
+    } else {
+        grid_launch_dependents();  // the joining kernel waits for this grid's end
+        const int64_t total = tiles_before<kP8Tile>(a, a.n_seqs) * a.VH;
+        const int64_t ctas = min64(gridDim.x, total);
+        if (blockIdx.x >= ctas) return;
+        u0 = share_begin(total, blockIdx.x, ctas);
+        u1 = share_begin(total, blockIdx.x + 1, ctas);
+        at = place_at<kP8Tile>(a, u0, u1);
+    }
+    const Place start = at;
+    Place in = at;  // what is loaded: one block lookup ahead of `issue`
+    bool bad = false;
+
+    // each lane looks up its key of the sub-tile at `in`
+    uint32_t row_tok = 0;
+    int32_t row_blk = -1, row_head = 0;
+    bool row_in = false;
+    const auto lookup = [&] {
+        const int64_t key = static_cast<int64_t>(in.t) * kP8Tile + warp * kP8Sub + lane;
+        row_in = in.left > 0 && key < in.len;
+        if (row_in) {
+            const uint32_t k32 = static_cast<uint32_t>(key), slot = k32 / a.bt;
+            row_blk = __ldg(a.table + in.b * a.table_stride + slot);
+            row_tok = k32 - slot * a.bt;
+            row_head = in.vh / a.HG;
+        }
+    };
+    // Copies the looked-up sub-tile into `stage` and looks the next one up. Its scales are on their way to registers until the next
+    // call, or `put`, writes them to the stage.
+    uint32_t ke = 0, ve = 0;
+    int scale_stage = -1;
+    const auto put = [&] {
+        if (scale_stage >= 0)
+            scales[scale_stage * kP8Sub + lane] =
+                make_float2(e8m0_value(ke), ve == 255u ? __uint_as_float(0x7FC00000u) : static_cast<float>(static_cast<int>(ve) - 127));
+    };
+    const auto issue = [&](int stage) {
+        put();
+        const bool ok = row_in && row_blk >= 0 && row_blk < a.n_blocks;
+        bad |= row_in && !ok;
+        const int64_t off = ok ? row_blk * a.block_stride + row_tok * a.tok_stride + row_head * a.head_stride : -1;
+        const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+        if (lane == 0) live[stage] = mask;
+        ke = ve = 0;
+        scale_stage = stage;
+        if (ok) {
+            const int64_t se = row_blk * a.scale_block + row_tok * a.scale_tok + row_head * a.scale_head;
+            ke = __ldg(a.ke + se);
+            ve = __ldg(a.ve + se);
+        }
+        const uint32_t dst = ring + stage * 2 * Ge::kHalf;
+        constexpr int RPI = 32 / Ge::kChunks;  // rows an instruction covers
+        const int c = lane % Ge::kChunks, r0 = lane / Ge::kChunks;
+        if (mask) {
+#pragma unroll
+            for (int i = 0; i < kP8Sub / RPI; ++i) {
+                const int r = r0 + i * RPI;
+                const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                const uint32_t d = dst + r * D + P8State<T, D, HB>::chunk_at(c, r & 7);
+                const int n = o >= 0 ? 16 : 0;
+                const int64_t src = (o >= 0 ? o : 0) + c * 16;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(a.k + src), "r"(n) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + Ge::kHalf), "l"(a.v + src), "r"(n)
+                             : "memory");
+            }
+        }
+        cp_async_commit();
+        if (in.left > 0) place_next<kP8Tile>(a, in);
+        lookup();
+    };
+
+    lookup();
+#pragma unroll
+    for (int s = 0; s < Ge::kStages - 1; ++s) issue(s);
+    P8State<T, D, HB> st;
+    int stage = 0;
+    bool fresh = true;  // first tile of a part
+    int part_t0 = 0;
+#pragma unroll 1
+    while (at.left > 0) {
+        const int h0 = (at.vh / a.HG) * a.G + (at.vh % a.HG) * HB;  // first query head
+        const int heads = min(HB, a.G - (at.vh % a.HG) * HB);
+        if (fresh) {
+            st.begin(a, at.b, h0, heads, lane);
+            part_t0 = at.t;
+            fresh = false;
+        }
+        cp_async_wait<Ge::kStages - 2>();
+        __syncwarp();  // every lane's copies have landed, and the previous stage has been read
+        issue((stage + Ge::kStages - 1) % Ge::kStages);
+        __syncwarp();  // the scales are there
+        const uint32_t mask = live[stage];
+        const uint32_t sk = ring + stage * 2 * Ge::kHalf;
+        if (mask) st.keys(sk, sk + Ge::kHalf, mask, scales + stage * kP8Sub, lane);
+
+        const bool pair_end = at.t + 1 == at.tiles;
+        if (pair_end || at.left == 1) {
+            // the warps' partials, each in the place of its last sub-tile, joined in warp order
+            __syncwarp();
+            const uint32_t part_at = stage * 2 * Ge::kHalf;
+            st.store(reinterpret_cast<float *>(p8_smem + ring_at + part_at), stat + warp * 3 * HB, lane);
+            __syncthreads();
+            const bool whole = !CL && pair_end && part_t0 == 0;
+            // parts: slot 0 begins with the CTA's share, slot 1 with a pair
+            const int slot = part_t0 == 0 && at.left - 1 + (at.t + 1) != u1 - u0 ? 1 : 0;
+            float *rec = CL ? own : a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * Ge::kRec;
+            for (int i = threadIdx.x; i < heads * D; i += kP8Threads) {
+                const int g = i / D;
+                float M = -INFINITY, N = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kP8Warps; ++w) {
+                    M = fmaxf(M, stat[w * 3 * HB + g]);
+                    N = fmaxf(N, stat[w * 3 * HB + 2 * HB + g]);
+                }
+                float ls = 0.f, os = 0.f;
+#pragma unroll
+                for (int w = 0; w < kP8Warps; ++w) {
+                    const float *po = reinterpret_cast<const float *>(p8_smem + w * Ge::kStages * 2 * Ge::kHalf + part_at);
+                    ls = fmaf(exp2_approx(p8_less(stat[w * 3 * HB + g], M)), stat[w * 3 * HB + HB + g], ls);
+                    os = fmaf(exp2_approx(p8_less(stat[w * 3 * HB + 2 * HB + g], N)), po[i], os);
+                }
+                if (whole) {
+                    static_cast<T *>(a.out)[at.b * a.o_seq + (h0 + g) * a.o_head + (i - g * D)] =
+                        from_f32<T>(ls != 0.f ? p8_unscale(os / ls, p8_less(N, M) - static_cast<float>(kP8Top)) : 0.f);
+                } else {
+                    rec[i] = os;
+                    if (i == g * D) rec[HB * D + g] = M, rec[HB * (D + 1) + g] = ls, rec[HB * (D + 2) + g] = N;
+                }
+            }
+            __syncthreads();  // the partials have been read
+            fresh = true;
+        }
+        stage = (stage + 1) % Ge::kStages;
+        place_next<kP8Tile>(a, at);
+    }
+    cp_async_wait<0>();
+    if (bad) set_status(a.status, B200_DEV_BAD_POSITION);
+    if constexpr (CL) {
+        cluster_sync();  // every CTA's record is written
+        const int rank = blockIdx.x % kP8Cluster;
+        const int h0 = (start.vh / a.HG) * a.G + (start.vh % a.HG) * HB, heads = min(HB, a.G - (start.vh % a.HG) * HB);
+        const int n = heads * D, i0 = n * rank / kP8Cluster, i1 = n * (rank + 1) / kP8Cluster;
+        for (int i = i0 + threadIdx.x; i < i1; i += kP8Threads) {
+            const int g = i / D;
+            float m[kP8Cluster], l[kP8Cluster], s[kP8Cluster], o[kP8Cluster], M = -INFINITY, N = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < kP8Cluster; ++c) {
+                m[c] = ld_dsmem(dsmem_addr(own + HB * D + g, c));
+                l[c] = ld_dsmem(dsmem_addr(own + HB * (D + 1) + g, c));
+                s[c] = ld_dsmem(dsmem_addr(own + HB * (D + 2) + g, c));
+                o[c] = ld_dsmem(dsmem_addr(own + i, c));
+            }
+#pragma unroll
+            for (int c = 0; c < kP8Cluster; ++c) M = fmaxf(M, m[c]), N = fmaxf(N, s[c]);
+            float ls = 0.f, os = 0.f;
+#pragma unroll
+            for (int c = 0; c < kP8Cluster; ++c) {
+                ls = fmaf(exp2_approx(p8_less(m[c], M)), l[c], ls);
+                os = fmaf(exp2_approx(p8_less(s[c], N)), o[c], os);
+            }
+            static_cast<T *>(a.out)[start.b * a.o_seq + (h0 + g) * a.o_head + (i - g * D)] =
+                from_f32<T>(ls != 0.f ? p8_unscale(os / ls, p8_less(N, M) - static_cast<float>(kP8Top)) : 0.f);
+        }
+        cluster_sync();  // no CTA's shared memory goes away while it is read
+    }
+}
+
+// Joins the parts of each pair that more than one CTA took, and clears the rows of empty sequences. One CTA a pair.
+template <typename T, int D, int HB>
+__global__ void __launch_bounds__(kP8JoinThreads) paged_q8_join_kernel(const __grid_constant__ P8Args a, const int64_t grid) {
+    using Ge = P8Geometry<D, HB>;
+    __shared__ float factor[HB * kP8MostCtas], sum_of[HB], shift[HB];
+    const int b = static_cast<int>(blockIdx.x / a.VH), vh = static_cast<int>(blockIdx.x % a.VH);
+    const int64_t before = tiles_before<kP8Tile>(a, b);
+    const int64_t total = tiles_before<kP8Tile>(a, a.n_seqs) * a.VH;
+    const int64_t ctas = min64(grid, total);  // as in the main kernel
+    const int tiles = seq_tiles<kP8Tile>(a, b);
+    const int h0 = (vh / a.HG) * a.G + (vh % a.HG) * HB;
+    const int heads = min(HB, a.G - (vh % a.HG) * HB);
+    T *out = static_cast<T *>(a.out) + b * a.o_seq + h0 * a.o_head;
+    if (threadIdx.x == 0 && vh == 0) report_length(a, b);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int64_t c0 = 0;
+    int parts = 0, slot0 = 0;  // CTAs c0 .. c0 + parts - 1 hold parts; only the first's may be a second part
+    if (tiles > 0) {
+        const int64_t ua = before * a.VH + static_cast<int64_t>(vh) * tiles;
+        c0 = share_owner(total, ua, ctas);
+        parts = static_cast<int>(share_owner(total, ua + tiles - 1, ctas) - c0) + 1;
+        slot0 = share_begin(total, c0, ctas) >= ua ? 0 : 1;
+    }
+    grid_wait();
+    if (parts == 1) return;  // whole: written by its CTA
+    if (parts == 0) {
+        for (int i = tid; i < heads * D; i += kP8JoinThreads) out[(i / D) * a.o_head + i % D] = from_f32<T>(0.f);
+        return;
+    }
+    const float *first = a.ws + (c0 * 2 + slot0) * Ge::kRec, *rest = a.ws + c0 * 2 * Ge::kRec;
+    const auto part = [&](int i) { return i == 0 ? first : rest + static_cast<int64_t>(i) * 2 * Ge::kRec; };
+    // the parts' sums, and each part's factor 2^(n - N), a warp per head and a lane per part
+    for (int g = warp; g < heads; g += kP8JoinThreads / 32) {
+        float M = -INFINITY, N = -INFINITY;
+        for (int i = lane; i < parts; i += 32) {
+            M = fmaxf(M, __ldcg(part(i) + HB * D + g));
+            const float n = __ldcg(part(i) + HB * (D + 2) + g);
+            factor[g * kP8MostCtas + i] = n;
+            N = fmaxf(N, n);
+        }
+        M = warp_max(M);
+        N = warp_max(N);
+        float sum = 0.f;
+        for (int i = lane; i < parts; i += 32) {
+            sum = fmaf(exp2_approx(p8_less(__ldcg(part(i) + HB * D + g), M)), __ldcg(part(i) + HB * (D + 1) + g), sum);
+            factor[g * kP8MostCtas + i] = exp2_approx(p8_less(factor[g * kP8MostCtas + i], N));
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) sum_of[g] = sum, shift[g] = p8_less(N, M) - static_cast<float>(kP8Top);
+    }
+    __syncthreads();
+    for (int j = tid; j < heads * D; j += kP8JoinThreads) {
+        const int g = j / D;
+        float acc = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < parts; ++i) acc = fmaf(factor[g * kP8MostCtas + i], __ldcg(part(i) + j), acc);
+        out[g * a.o_head + (j - g * D)] = from_f32<T>(sum_of[g] != 0.f ? p8_unscale(acc / sum_of[g], shift[g]) : 0.f);
+    }
+}
+
+int p8_max_ctas() { return device_sm_count() * 2 < kP8MostCtas ? device_sm_count() * 2 : kP8MostCtas; }
+
+// Few pairs with short tables: a cluster each, no workspace.
+bool p8_one_launch(int64_t pairs, int64_t max_keys) {
+    return pairs * (kP8Cluster + 1) <= p8_max_ctas() && max_keys <= kP8ClusterKeys;
+}
+
+int p8_heads(int64_t G) { return G <= 8 ? 8 : 16; }  // heads a block handles
+
+template <typename T, int D, int HB>
+cudaError_t p8_launch(P8Args a, int64_t Hkv, cudaStream_t st) {
+    using Ge = P8Geometry<D, HB>;
+    a.HG = (a.G + HB - 1) / HB;
+    a.VH = static_cast<int>(Hkv) * a.HG;
+    const int64_t pairs = static_cast<int64_t>(a.n_seqs) * a.VH;
+    if (pairs > INT32_MAX) return cudaErrorNotSupported;
+    const auto allow = [](const void *kern, size_t bytes) {
+        return once_per_device(kern, ATTR_SMEM, [&] {
+            return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+        });
+    };
+    if (p8_one_launch(pairs, a.max_keys)) {
+        auto kern = paged_q8_kernel<T, D, HB, true>;
+        const cudaError_t e = allow(reinterpret_cast<const void *>(kern), Ge::kSmemCluster);
+        if (e != cudaSuccess) return e;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(pairs * kP8Cluster));
+        cfg.blockDim = dim3(kP8Threads);
+        cfg.dynamicSmemBytes = Ge::kSmemCluster;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = kP8Cluster;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, kern, a);
+    }
+    auto kern = paged_q8_kernel<T, D, HB, false>;
+    cudaError_t e = allow(reinterpret_cast<const void *>(kern), Ge::kSmem);
+    if (e != cudaSuccess) return e;
+    const int64_t most = (a.max_keys + kP8Tile - 1) / kP8Tile;  // tiles of the longest possible sequence
+    const int64_t ctas = min64(p8_max_ctas(), most > p8_max_ctas() ? p8_max_ctas() : pairs * most);
+    e = b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kP8Threads), Ge::kSmem, st, false, a);
+    if (e != cudaSuccess) return e;
+    return b200_launch(paged_q8_join_kernel<T, D, HB>, dim3(static_cast<unsigned>(pairs)), dim3(kP8JoinThreads), 0, st, true, a,
+                       ctas);
 }
 
 template <typename T>
-cudaError_t p8_by_dim(const P8Args &a, int64_t D, cudaStream_t st) {
-    const int64_t pairs = static_cast<int64_t>(a.n_seqs) * a.Hkv;
-    if (pairs > INT32_MAX) return cudaErrorNotSupported;
-    if (D == 128) paged_q8_rows_kernel<T, 128><<<static_cast<unsigned>(pairs), 32 * kArWarps, 0, st>>>(a);
-    else paged_q8_rows_kernel<T, 64><<<static_cast<unsigned>(pairs), 32 * kArWarps, 0, st>>>(a);
-    return cudaGetLastError();
+cudaError_t p8_by_dim(const P8Args &a, int64_t D, int64_t Hkv, cudaStream_t st) {
+    if (p8_heads(a.G) == 8) return D == 128 ? p8_launch<T, 128, 8>(a, Hkv, st) : p8_launch<T, 64, 8>(a, Hkv, st);
+    return D == 128 ? p8_launch<T, 128, 16>(a, Hkv, st) : p8_launch<T, 64, 16>(a, Hkv, st);
 }
 
 }  // namespace
@@ -78,7 +575,12 @@ using namespace b200;
 extern "C" {
 
 size_t b200_flash_attn_paged_batch_q8_workspace_bytes(int64_t n_seqs, int64_t max_keys, int64_t D, int64_t Hq, int64_t Hkv) {
-    return 0;
+    if (n_seqs <= 0 || max_keys <= 0 || D <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv) return 0;
+    const int64_t G = Hq / Hkv;
+    const int hb = p8_heads(G);
+    if (p8_one_launch(n_seqs * Hkv * ((G + hb - 1) / hb), max_keys)) return 0;
+    // two partial records a CTA (its share's first and last part)
+    return static_cast<size_t>(p8_max_ctas()) * 2 * hb * (D + 3) * 4;
 }
 
 int b200_flash_attn_paged_batch_q8(const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
@@ -129,15 +631,15 @@ int b200_flash_attn_paged_batch_q8(const void *q, int64_t q_seq_stride, int64_t 
     a.max_keys = max_keys;
     a.n_seqs = static_cast<int>(n_seqs);
     a.G = static_cast<int>(Hq / Hkv);
-    a.Hkv = static_cast<int>(Hkv);
     a.sl2 = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(D))) * kLog2e;
+    a.ws = static_cast<float *>(workspace);
     a.status = dev_status;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-        case B200_DTYPE_F16: return status_of(p8_by_dim<__half>(a, D, st));
-        case B200_DTYPE_BF16: return status_of(p8_by_dim<__nv_bfloat16>(a, D, st));
+        case B200_DTYPE_F16: return status_of(p8_by_dim<__half>(a, D, Hkv, st));
+        case B200_DTYPE_BF16: return status_of(p8_by_dim<__nv_bfloat16>(a, D, Hkv, st));
     }
-    return status_of(p8_by_dim<float>(a, D, st));
+    return status_of(p8_by_dim<float>(a, D, Hkv, st));
 }
 
 }  // extern "C"

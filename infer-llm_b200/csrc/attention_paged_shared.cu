@@ -2,12 +2,10 @@
 //
 // out_b = softmax over the keys of the prefix of b's group and b's own keys, of the one pool.
 #include "attention_rows.cuh"
-#include "gemv.cuh"
+#include "paged_line.cuh"
 
 namespace b200 {
 namespace {
-
-constexpr int64_t kMostKeys = INT32_MAX - 256;
 
 struct SharedArgs {
     const void *q = nullptr;
