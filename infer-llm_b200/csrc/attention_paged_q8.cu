@@ -25,12 +25,16 @@ namespace {
 
 constexpr int kP8Warps = 4;
 constexpr int kP8Threads = 32 * kP8Warps;
+constexpr int kP8Ctas = 2;  // an SM (three, of 168 registers, spill: 92 us against 80)
 constexpr int kP8MostCtas = 320;
 constexpr int kP8JoinThreads = 256;
 constexpr int kP8Cluster = 8;
 constexpr int kP8ClusterKeys = 4096;
 constexpr int kP8Sub = 32;                  // keys of a warp's sub-tile
 constexpr int kP8Tile = kP8Sub * kP8Warps;  // keys of a tile
+// Units of the line a tile and a pair's start and end take: 1.6 to 1.8 us against 2.4 (64 ragged sequences; shares of equal tiles ended
+// between 50 and 69 us).
+constexpr int kP8TileUnits = 2, kP8PairUnits = 3;
 constexpr int kP8Top = 14;                  // weights are at most 2^14, F16's largest power of two but one
 
 struct P8Args {
@@ -45,7 +49,7 @@ struct P8Args {
     const int32_t *table = nullptr, *lens = nullptr;
     int64_t table_stride = 0;
     int64_t max_keys = 0;  // positions a table row covers (fits 31 bits)
-    uint32_t bt = 1;
+    uint32_t bt = 1, bt_mul = 0, bt_shift = 0;  // x / bt = x bt_mul / 2^bt_shift for x < 2^31
     int n_seqs = 0, G = 0, VH = 0, HG = 0;  // query heads a KV head; (KV head, head group) pairs; groups a KV head
     float sl2 = 0.f;                        // scale * log2 e
     float *ws = nullptr;
@@ -54,7 +58,7 @@ struct P8Args {
 
 template <int D, int HB>
 struct P8Geometry {
-    static constexpr int kStages = 3;
+    static constexpr int kStages = 2;  // (three: 1 us more)
     static constexpr int kChunks = D / 16;
     static constexpr int kHalf = kP8Sub * D;     // K (or V) bytes of a sub-tile
     static constexpr int kRec = HB * (D + 3);    // floats of a partial: o, then m, l, n
@@ -64,7 +68,7 @@ struct P8Geometry {
     static constexpr size_t kSmem = kRing + kStat + kScale + kP8Warps * kStages * 4;
     static constexpr size_t kSmemCluster = kSmem + kRec * 4;
     static_assert(HB * D * 4 <= 2 * kHalf, "a warp's partial takes the place of its last sub-tile");
-    static_assert(2 * (kSmemCluster + 1024) <= 228 * 1024, "two CTAs an SM");
+    static_assert(kP8Ctas * (kSmemCluster + 1024) <= 228 * 1024, "CTAs of an SM");
 };
 
 B200_DEVICE float p8_pow2(int e) { return __uint_as_float(static_cast<uint32_t>(max(-126, min(127, e)) + 127) << 23); }
@@ -76,13 +80,28 @@ B200_DEVICE float p8_unscale(float x, float e) {
 // m - M for running maxima of which both may be -inf
 B200_DEVICE float p8_less(float m, float M) { return m - (M == -INFINITY ? 0.f : M); }
 
+// Four columns of a head's output: o 2^(N - M - 14) / l, `shift` being N - M; zeros where there is no weight.
+template <typename T>
+B200_DEVICE void p8_write(T *to, const float (&o)[4], float l, float shift) {
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+    T x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = from_f32<T>(l != 0.f ? p8_unscale(o[j] * inv, shift - static_cast<float>(kP8Top)) : 0.f);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(to) = *reinterpret_cast<const float4 *>(x);
+    else *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(x);
+}
+
 // One warp's running softmax: lane (g = lane / 4, t = lane % 4) holds head rows g (and g + 8 of 16), output columns
 // 16 c + 4 t .. + 3.
 template <typename T, int D, int HB>
 struct P8State {
     static constexpr bool FULL = HB > 8, TWO = __is_same(T, float);
     static constexpr int R = FULL ? 2 : 1;  // head rows a lane holds
-    uint32_t q[D / 16][2 * R], ql[TWO ? D / 16 : 1][2 * R];
+    // A fragments of Q. 16 heads: of 16 dimensions, and of their second terms. Up to 8 heads: rows 0 .. 7 and 8 .. 15 are the two terms
+    // (TWO), or 16 dimensions and the next 16, of which a product with a key's 16 dimensions uses one half. Every fragment is four registers
+    // in a row as the instruction wants them; zeros in half of them would have to be moved there each time.
+    static constexpr int NQ = FULL || TWO ? D / 16 : D / 32;
+    uint32_t q[NQ][4], ql[FULL && TWO ? NQ : 1][4];
     float o[D / 16][2][4];  // even and odd columns: rows g and g + 8; without FULL, row g's shares of the weights' two terms
     float m[R], l[R], n[R], qs[R];
 
@@ -123,10 +142,18 @@ struct P8State {
                 for (int u = 0; u < 2; ++u) {
                     const float y0 = x[s][2 * u] * f, y1 = x[s][2 * u + 1] * f;
                     const uint32_t hi = pack2<__half>(y0, y1);
-                    q[s][u * R + r] = hi;
+                    uint32_t lo = 0;
                     if constexpr (TWO) {  // (the rest of an infinity or NaN would be NaN; it stays in the first)
                         const float2 h = unpack2<__half>(hi);
-                        ql[s][u * R + r] = pack2<__half>(fabsf(y0) < INFINITY ? y0 - h.x : 0.f, fabsf(y1) < INFINITY ? y1 - h.y : 0.f);
+                        lo = pack2<__half>(fabsf(y0) < INFINITY ? y0 - h.x : 0.f, fabsf(y1) < INFINITY ? y1 - h.y : 0.f);
+                    }
+                    if constexpr (FULL) {
+                        q[s][2 * u + r] = hi;
+                        if constexpr (TWO) ql[s][2 * u + r] = lo;
+                    } else if constexpr (TWO) {
+                        q[s][2 * u] = hi, q[s][2 * u + 1] = lo;
+                    } else {
+                        q[s / 2][2 * u + s % 2] = hi;
                     }
                 }
         }
@@ -140,11 +167,14 @@ struct P8State {
     // `live`: key j takes part.
     B200_DEVICE void keys(uint32_t sk, uint32_t sv, uint32_t live, const float2 *scales, int lane) {
         const int mat = lane >> 3, rr = lane & 7, t2 = 2 * (lane & 3);
-        float s[4][2 * (FULL || TWO ? 2 : 1)];
+        constexpr int NS = FULL || TWO ? 1 : 2;  // sums: of even and odd 16 dimensions
+        float s[NS][4][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int i = 0; i < NS; ++i)
 #pragma unroll
-            for (int u = 0; u < (FULL || TWO ? 4 : 2); ++u) s[j][u] = 0.f;
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) s[i][j][u] = 0.f;
         const uint32_t row = (8 * mat + rr) * D;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
@@ -152,15 +182,13 @@ struct P8State {
             ldsm4(kf, sk + row + chunk_at(ks, rr));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t b0 = e4m3x2_to_f16x2(kf[j]), b1 = e4m3x2_to_f16x2(kf[j] >> 16);
+                uint32_t b0, b1;
+                e4m3x4_to_f16(kf[j], b0, b1);
                 if constexpr (FULL) {
-                    mma16<__half, true>(s[j], q[ks], b0, b1);
-                    if constexpr (TWO) mma16<__half, true>(s[j], ql[ks], b0, b1);
-                } else if constexpr (TWO) {
-                    const uint32_t both[4] = {q[ks][0], ql[ks][0], q[ks][1], ql[ks][1]};
-                    mma16<__half, true>(s[j], both, b0, b1);
+                    mma16<__half, true>(s[0][j], q[ks], b0, b1);
+                    if constexpr (TWO) mma16<__half, true>(s[0][j], ql[ks], b0, b1);
                 } else {
-                    mma16<__half, false>(s[j], q[ks], b0, b1);
+                    mma16<__half, true>(s[TWO ? 0 : ks % 2][j], q[TWO ? ks : ks / 2], b0, b1);
                 }
             }
         }
@@ -178,9 +206,9 @@ struct P8State {
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    float y = s[j][2 * r + u];
-                    if constexpr (TWO && !FULL) y += s[j][2 + u];
-                    x[j][u] = (live >> (8 * j + t2 + u)) & 1u ? y * qs[r] * ke[j][u] : -INFINITY;
+                    const float y = FULL ? s[0][j][2 * r + u] : s[0][j][u] + s[NS - 1][j][2 + u];
+                    x[j][u] = y * qs[r] * ke[j][u];
+                    if (live != ~0u && !((live >> (8 * j + t2 + u)) & 1u)) x[j][u] = -INFINITY;
                     mx = fmaxf(mx, x[j][u]);
                     nx = fmaxf(nx, x[j][u] + ve[j][u]);
                 }
@@ -216,8 +244,7 @@ struct P8State {
             ldsm4_t(vf, sv + row + chunk_at(c, rr));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {  // (key, column) bytes 00 01 10 11 as even and odd columns
-                const uint32_t p = __byte_perm(vf[j], 0, 0x3120);
-                x[j][0] = e4m3x2_to_f16x2(p), x[j][1] = e4m3x2_to_f16x2(p >> 16);
+                e4m3x4_to_f16(__byte_perm(vf[j], 0, 0x3120), x[j][0], x[j][1]);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -260,7 +287,7 @@ struct P8State {
 
 // CL: a cluster of kP8Cluster CTAs takes one pair, and writes its output.
 template <typename T, int D, int HB, bool CL>
-__global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_constant__ P8Args a) {
+__global__ void __launch_bounds__(kP8Threads, kP8Ctas) paged_q8_kernel(const __grid_constant__ P8Args a) {
     using Ge = P8Geometry<D, HB>;
     extern __shared__ __align__(128) unsigned char p8_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -270,7 +297,6 @@ __global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_co
     float *own = reinterpret_cast<float *>(p8_smem + Ge::kSmem);  // CL: this CTA's record
     const uint32_t ring_at = warp * Ge::kStages * 2 * Ge::kHalf, ring = smem_addr(p8_smem) + ring_at;
 
-    int64_t u0 = 0, u1 = 0;
     Place at = {};  // what is computed
     if constexpr (CL) {
         const int pair = blockIdx.x / kP8Cluster, rank = blockIdx.x % kP8Cluster;
@@ -279,19 +305,18 @@ __global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_co
         at.len = seq_len(a, at.b);
         at.tiles = (at.len + kP8Tile - 1) / kP8Tile;
         at.t = at.tiles * rank / kP8Cluster;
-        at.left = at.tiles * (rank + 1) / kP8Cluster - at.t;
+        at.left = (at.tiles * (rank + 1) / kP8Cluster - at.t) * kP8TileUnits;
         if (rank == 0 && at.vh == 0 && threadIdx.x == 0) report_length(a, at.b);
         if (at.left == 0)  // no keys: nothing to add
             for (int i = threadIdx.x; i < Ge::kRec; i += kP8Threads)
                 own[i] = i < HB * D || (i >= HB * (D + 1) && i < HB * (D + 2)) ? 0.f : -INFINITY;
     } else {
         grid_launch_dependents();  // the joining kernel waits for this grid's end
-        const int64_t total = tiles_before<kP8Tile>(a, a.n_seqs) * a.VH;
-        const int64_t ctas = min64(gridDim.x, total);
+        const int64_t total = tiles_before<kP8Tile, kP8TileUnits, kP8PairUnits>(a, a.n_seqs) * a.VH;
+        const int64_t ctas = min64(gridDim.x, total / kP8TileUnits);
         if (blockIdx.x >= ctas) return;
-        u0 = share_begin(total, blockIdx.x, ctas);
-        u1 = share_begin(total, blockIdx.x + 1, ctas);
-        at = place_at<kP8Tile>(a, u0, u1);
+        const int64_t u0 = share_begin(total, blockIdx.x, ctas), u1 = share_begin(total, blockIdx.x + 1, ctas);
+        at = place_at<kP8Tile, kP8TileUnits, kP8PairUnits>(a, u0, u1);
     }
     const Place start = at;
     Place in = at;  // what is loaded: one block lookup ahead of `issue`
@@ -305,10 +330,11 @@ __global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_co
         const int64_t key = static_cast<int64_t>(in.t) * kP8Tile + warp * kP8Sub + lane;
         row_in = in.left > 0 && key < in.len;
         if (row_in) {
-            const uint32_t k32 = static_cast<uint32_t>(key), slot = k32 / a.bt;
+            const uint32_t k32 = static_cast<uint32_t>(key);
+            const uint32_t slot = static_cast<uint32_t>(static_cast<uint64_t>(k32) * a.bt_mul >> a.bt_shift);
             row_blk = __ldg(a.table + in.b * a.table_stride + slot);
             row_tok = k32 - slot * a.bt;
-            row_head = in.vh / a.HG;
+            row_head = a.HG == 1 ? in.vh : in.vh / a.HG;
         }
     };
     // Copies the looked-up sub-tile into `stage` and looks the next one up. Its scales are on their way to registers until the next
@@ -324,7 +350,7 @@ __global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_co
         put();
         const bool ok = row_in && row_blk >= 0 && row_blk < a.n_blocks;
         bad |= row_in && !ok;
-        const int64_t off = ok ? row_blk * a.block_stride + row_tok * a.tok_stride + row_head * a.head_stride : -1;
+        const int64_t off = ok ? row_blk * a.block_stride + row_tok * a.tok_stride + row_head * a.head_stride : 0;
         const uint32_t mask = __ballot_sync(0xffffffffu, ok);
         if (lane == 0) live[stage] = mask;
         ke = ve = 0;
@@ -334,24 +360,30 @@ __global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_co
             ke = __ldg(a.ke + se);
             ve = __ldg(a.ve + se);
         }
-        const uint32_t dst = ring + stage * 2 * Ge::kHalf;
-        constexpr int RPI = 32 / Ge::kChunks;  // rows an instruction covers
+        constexpr int RPI = 32 / Ge::kChunks;  // rows an instruction covers: row r0 + i RPI, chunk c
         const int c = lane % Ge::kChunks, r0 = lane / Ge::kChunks;
-        if (mask) {
+        const uint32_t dst = ring + stage * 2 * Ge::kHalf + r0 * D;
+        const char *k = a.k + c * 16, *v = a.v + c * 16;
+        if (mask == ~0u) {
 #pragma unroll
             for (int i = 0; i < kP8Sub / RPI; ++i) {
-                const int r = r0 + i * RPI;
+                const int64_t o = __shfl_sync(0xffffffffu, off, r0 + i * RPI);
+                const uint32_t d = dst + i * RPI * D + P8State<T, D, HB>::chunk_at(c, (r0 + i * RPI) & 7);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(k + o) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + Ge::kHalf), "l"(v + o) : "memory");
+            }
+        } else if (mask) {  // rows that are not there are filled with zeros
+#pragma unroll 1
+            for (int i = 0; i < kP8Sub / RPI; ++i) {
+                const int r = r0 + i * RPI, n = (mask >> r) & 1u ? 16 : 0;
                 const int64_t o = __shfl_sync(0xffffffffu, off, r);
-                const uint32_t d = dst + r * D + P8State<T, D, HB>::chunk_at(c, r & 7);
-                const int n = o >= 0 ? 16 : 0;
-                const int64_t src = (o >= 0 ? o : 0) + c * 16;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(a.k + src), "r"(n) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + Ge::kHalf), "l"(a.v + src), "r"(n)
-                             : "memory");
+                const uint32_t d = dst + i * RPI * D + P8State<T, D, HB>::chunk_at(c, r & 7);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(k + o), "r"(n) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + Ge::kHalf), "l"(v + o), "r"(n) : "memory");
             }
         }
         cp_async_commit();
-        if (in.left > 0) place_next<kP8Tile>(a, in);
+        if (in.left > 0) place_next<kP8Tile, kP8TileUnits, kP8PairUnits>(a, in);
         lookup();
     };
 
@@ -361,12 +393,12 @@ __global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_co
     P8State<T, D, HB> st;
     int stage = 0;
     bool fresh = true;  // first tile of a part
-    int part_t0 = 0;
+    int part_t0 = 0, h0 = 0, heads = 0;  // of the part: its first tile and query head, its heads
 #pragma unroll 1
     while (at.left > 0) {
-        const int h0 = (at.vh / a.HG) * a.G + (at.vh % a.HG) * HB;  // first query head
-        const int heads = min(HB, a.G - (at.vh % a.HG) * HB);
         if (fresh) {
+            h0 = (at.vh / a.HG) * a.G + (at.vh % a.HG) * HB;
+            heads = min(HB, a.G - (at.vh % a.HG) * HB);
             st.begin(a, at.b, h0, heads, lane);
             part_t0 = at.t;
             fresh = false;
@@ -380,17 +412,16 @@ __global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_co
         if (mask) st.keys(sk, sk + Ge::kHalf, mask, scales + stage * kP8Sub, lane);
 
         const bool pair_end = at.t + 1 == at.tiles;
-        if (pair_end || at.left == 1) {
+        if (pair_end || at.left <= kP8TileUnits) {
             // the warps' partials, each in the place of its last sub-tile, joined in warp order
             __syncwarp();
             const uint32_t part_at = stage * 2 * Ge::kHalf;
             st.store(reinterpret_cast<float *>(p8_smem + ring_at + part_at), stat + warp * 3 * HB, lane);
             __syncthreads();
             const bool whole = !CL && pair_end && part_t0 == 0;
-            // parts: slot 0 begins with the CTA's share, slot 1 with a pair
-            const int slot = part_t0 == 0 && at.left - 1 + (at.t + 1) != u1 - u0 ? 1 : 0;
-            float *rec = CL ? own : a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * Ge::kRec;
-            for (int i = threadIdx.x; i < heads * D; i += kP8Threads) {
+            // a CTA has at most two parts: one that begins within a pair, and one that begins with a pair
+            float *rec = CL ? own : a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + (part_t0 == 0)) * Ge::kRec;
+            for (int i = 4 * threadIdx.x; i < heads * D; i += 4 * kP8Threads) {
                 const int g = i / D;
                 float M = -INFINITY, N = -INFINITY;
 #pragma unroll
@@ -398,18 +429,20 @@ __global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_co
                     M = fmaxf(M, stat[w * 3 * HB + g]);
                     N = fmaxf(N, stat[w * 3 * HB + 2 * HB + g]);
                 }
-                float ls = 0.f, os = 0.f;
+                float ls = 0.f, os[4] = {};
 #pragma unroll
                 for (int w = 0; w < kP8Warps; ++w) {
-                    const float *po = reinterpret_cast<const float *>(p8_smem + w * Ge::kStages * 2 * Ge::kHalf + part_at);
+                    const float4 x =
+                        *reinterpret_cast<const float4 *>(p8_smem + w * Ge::kStages * 2 * Ge::kHalf + part_at + i * 4);
                     ls = fmaf(exp2_approx(p8_less(stat[w * 3 * HB + g], M)), stat[w * 3 * HB + HB + g], ls);
-                    os = fmaf(exp2_approx(p8_less(stat[w * 3 * HB + 2 * HB + g], N)), po[i], os);
+                    const float f = exp2_approx(p8_less(stat[w * 3 * HB + 2 * HB + g], N));
+                    os[0] = fmaf(f, x.x, os[0]), os[1] = fmaf(f, x.y, os[1]);
+                    os[2] = fmaf(f, x.z, os[2]), os[3] = fmaf(f, x.w, os[3]);
                 }
                 if (whole) {
-                    static_cast<T *>(a.out)[at.b * a.o_seq + (h0 + g) * a.o_head + (i - g * D)] =
-                        from_f32<T>(ls != 0.f ? p8_unscale(os / ls, p8_less(N, M) - static_cast<float>(kP8Top)) : 0.f);
+                    p8_write<T>(static_cast<T *>(a.out) + at.b * a.o_seq + (h0 + g) * a.o_head + (i - g * D), os, ls, p8_less(N, M));
                 } else {
-                    rec[i] = os;
+                    *reinterpret_cast<float4 *>(rec + i) = make_float4(os[0], os[1], os[2], os[3]);
                     if (i == g * D) rec[HB * D + g] = M, rec[HB * (D + 1) + g] = ls, rec[HB * (D + 2) + g] = N;
                 }
             }
@@ -417,14 +450,15 @@ __global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_co
             fresh = true;
         }
         stage = (stage + 1) % Ge::kStages;
-        place_next<kP8Tile>(a, at);
+        place_next<kP8Tile, kP8TileUnits, kP8PairUnits>(a, at);
     }
     cp_async_wait<0>();
     if (bad) set_status(a.status, B200_DEV_BAD_POSITION);
     if constexpr (CL) {
         cluster_sync();  // every CTA's record is written
         const int rank = blockIdx.x % kP8Cluster;
-        const int h0 = (start.vh / a.HG) * a.G + (start.vh % a.HG) * HB, heads = min(HB, a.G - (start.vh % a.HG) * HB);
+        h0 = (start.vh / a.HG) * a.G + (start.vh % a.HG) * HB;
+        heads = min(HB, a.G - (start.vh % a.HG) * HB);
         const int n = heads * D, i0 = n * rank / kP8Cluster, i1 = n * (rank + 1) / kP8Cluster;
         for (int i = i0 + threadIdx.x; i < i1; i += kP8Threads) {
             const int g = i / D;
@@ -451,67 +485,66 @@ __global__ void __launch_bounds__(kP8Threads, 2) paged_q8_kernel(const __grid_co
     }
 }
 
-// Joins the parts of each pair that more than one CTA took, and clears the rows of empty sequences. One CTA a pair.
+// Joins the parts of each pair that more than one CTA took, and clears the rows of empty sequences. One CTA a pair, a thread four
+// columns at a time; it asks for all of a few parts' numbers at once, so that their latency is paid once.
 template <typename T, int D, int HB>
 __global__ void __launch_bounds__(kP8JoinThreads) paged_q8_join_kernel(const __grid_constant__ P8Args a, const int64_t grid) {
     using Ge = P8Geometry<D, HB>;
-    __shared__ float factor[HB * kP8MostCtas], sum_of[HB], shift[HB];
     const int b = static_cast<int>(blockIdx.x / a.VH), vh = static_cast<int>(blockIdx.x % a.VH);
-    const int64_t before = tiles_before<kP8Tile>(a, b);
-    const int64_t total = tiles_before<kP8Tile>(a, a.n_seqs) * a.VH;
-    const int64_t ctas = min64(grid, total);  // as in the main kernel
+    const int64_t before = tiles_before<kP8Tile, kP8TileUnits, kP8PairUnits>(a, b);
+    const int64_t total = tiles_before<kP8Tile, kP8TileUnits, kP8PairUnits>(a, a.n_seqs) * a.VH;
+    const int64_t ctas = min64(grid, total / kP8TileUnits);  // as in the main kernel
     const int tiles = seq_tiles<kP8Tile>(a, b);
     const int h0 = (vh / a.HG) * a.G + (vh % a.HG) * HB;
     const int heads = min(HB, a.G - (vh % a.HG) * HB);
     T *out = static_cast<T *>(a.out) + b * a.o_seq + h0 * a.o_head;
     if (threadIdx.x == 0 && vh == 0) report_length(a, b);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int64_t c0 = 0;
-    int parts = 0, slot0 = 0;  // CTAs c0 .. c0 + parts - 1 hold parts; only the first's may be a second part
+    int parts = 0;  // CTAs c0 .. c0 + parts - 1 hold parts
     if (tiles > 0) {
-        const int64_t ua = before * a.VH + static_cast<int64_t>(vh) * tiles;
+        const int64_t ua = before * a.VH + vh * units_of<kP8TileUnits, kP8PairUnits>(tiles);
         c0 = share_owner(total, ua, ctas);
-        parts = static_cast<int>(share_owner(total, ua + tiles - 1, ctas) - c0) + 1;
-        slot0 = share_begin(total, c0, ctas) >= ua ? 0 : 1;
+        parts = static_cast<int>(share_owner(total, ua + (tiles - 1) * kP8TileUnits, ctas) - c0) + 1;
     }
     grid_wait();
     if (parts == 1) return;  // whole: written by its CTA
-    if (parts == 0) {
-        for (int i = tid; i < heads * D; i += kP8JoinThreads) out[(i / D) * a.o_head + i % D] = from_f32<T>(0.f);
-        return;
-    }
-    const float *first = a.ws + (c0 * 2 + slot0) * Ge::kRec, *rest = a.ws + c0 * 2 * Ge::kRec;
-    const auto part = [&](int i) { return i == 0 ? first : rest + static_cast<int64_t>(i) * 2 * Ge::kRec; };
-    // the parts' sums, and each part's factor 2^(n - N), a warp per head and a lane per part
-    for (int g = warp; g < heads; g += kP8JoinThreads / 32) {
-        float M = -INFINITY, N = -INFINITY;
-        for (int i = lane; i < parts; i += 32) {
-            M = fmaxf(M, __ldcg(part(i) + HB * D + g));
-            const float n = __ldcg(part(i) + HB * (D + 2) + g);
-            factor[g * kP8MostCtas + i] = n;
-            N = fmaxf(N, n);
-        }
-        M = warp_max(M);
-        N = warp_max(N);
-        float sum = 0.f;
-        for (int i = lane; i < parts; i += 32) {
-            sum = fmaf(exp2_approx(p8_less(__ldcg(part(i) + HB * D + g), M)), __ldcg(part(i) + HB * (D + 1) + g), sum);
-            factor[g * kP8MostCtas + i] = exp2_approx(p8_less(factor[g * kP8MostCtas + i], N));
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) sum_of[g] = sum, shift[g] = p8_less(N, M) - static_cast<float>(kP8Top);
-    }
-    __syncthreads();
-    for (int j = tid; j < heads * D; j += kP8JoinThreads) {
+    const auto part = [&](int i) { return a.ws + ((c0 + i) * 2 + (i == 0)) * Ge::kRec; };
+    constexpr int kAtOnce = 4;
+    for (int j = 4 * threadIdx.x; j < heads * D; j += 4 * kP8JoinThreads) {
         const int g = j / D;
-        float acc = 0.f;
-#pragma unroll 8
-        for (int i = 0; i < parts; ++i) acc = fmaf(factor[g * kP8MostCtas + i], __ldcg(part(i) + j), acc);
-        out[g * a.o_head + (j - g * D)] = from_f32<T>(sum_of[g] != 0.f ? p8_unscale(acc / sum_of[g], shift[g]) : 0.f);
+        float M = -INFINITY, N = -INFINITY, l = 0.f, o[4] = {};
+        for (int i0 = 0; i0 < parts; i0 += kAtOnce) {
+            float m[kAtOnce], n[kAtOnce], ls[kAtOnce], Mn = M, Nn = N;
+            float4 x[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                const float *p = part(min(i0 + i, parts - 1));
+                x[i] = __ldcg(reinterpret_cast<const float4 *>(p + j));
+                m[i] = __ldcg(p + HB * D + g);
+                ls[i] = __ldcg(p + HB * (D + 1) + g);
+                n[i] = __ldcg(p + HB * (D + 2) + g);
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) Mn = fmaxf(Mn, m[i]), Nn = fmaxf(Nn, n[i]);
+            l *= exp2_approx(p8_less(M, Mn));
+            const float f = exp2_approx(p8_less(N, Nn));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] *= f;
+            M = Mn, N = Nn;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                if (i0 + i >= parts) break;
+                l = fmaf(exp2_approx(p8_less(m[i], M)), ls[i], l);
+                const float w = exp2_approx(p8_less(n[i], N));
+                o[0] = fmaf(w, x[i].x, o[0]), o[1] = fmaf(w, x[i].y, o[1]);
+                o[2] = fmaf(w, x[i].z, o[2]), o[3] = fmaf(w, x[i].w, o[3]);
+            }
+        }
+        p8_write<T>(out + g * a.o_head + (j - g * D), o, l, p8_less(N, M));
     }
 }
 
-int p8_max_ctas() { return device_sm_count() * 2 < kP8MostCtas ? device_sm_count() * 2 : kP8MostCtas; }
+int p8_max_ctas() { return device_sm_count() * kP8Ctas < kP8MostCtas ? device_sm_count() * kP8Ctas : kP8MostCtas; }
 
 // Few pairs with short tables: a cluster each, no workspace.
 bool p8_one_launch(int64_t pairs, int64_t max_keys) {
@@ -628,6 +661,9 @@ int b200_flash_attn_paged_batch_q8(const void *q, int64_t q_seq_stride, int64_t 
     a.lens = seq_lens;
     a.table_stride = table_stride;
     a.bt = static_cast<uint32_t>(pool->block_tokens);
+    // for the least l with bt <= 2^l: ceil(2^(31 + l) / bt) is below 2^32 and exceeds the quotient by less than 1
+    for (a.bt_shift = 31; (1ull << (a.bt_shift - 31)) < a.bt;) ++a.bt_shift;
+    a.bt_mul = static_cast<uint32_t>(((1ull << a.bt_shift) + a.bt - 1) / a.bt);
     a.max_keys = max_keys;
     a.n_seqs = static_cast<int>(n_seqs);
     a.G = static_cast<int>(Hq / Hkv);

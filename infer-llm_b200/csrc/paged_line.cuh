@@ -27,48 +27,61 @@ B200_DEVICE int seq_tiles(const A &a, int b) {
     return static_cast<int>((static_cast<int64_t>(seq_len(a, b)) + TILE - 1) / TILE);
 }
 
-// Tiles of the sequences before b (all sequences for b = n_seqs), by a whole warp.
-template <int TILE, typename A>
+// The line's units: TU a tile and PU more a (sequence, virtual head), for what its start and end cost. A tile belongs to the share that
+// has its first unit.
+template <int TU, int PU>
+B200_DEVICE int64_t units_of(int64_t tiles) { return tiles ? tiles * TU + PU : 0; }
+
+// Units of a virtual head of the sequences before b (all sequences for b = n_seqs), by a whole warp.
+template <int TILE, int TU = 1, int PU = 0, typename A>
 B200_DEVICE int64_t tiles_before(const A &a, int b) {
     int64_t n = 0;
-    for (int i = threadIdx.x & 31; i < b; i += 32) n += seq_tiles<TILE>(a, i);
+    for (int i = threadIdx.x & 31; i < b; i += 32) n += units_of<TU, PU>(seq_tiles<TILE>(a, i));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
 }
 
-// CTA c of n <= total takes the tiles [total c / n, total (c + 1) / n): at least one.
+// CTA c of n takes the units [total c / n, total (c + 1) / n): at least TU of them, so at least one tile of every pair that
+// it lies within, if n <= total / TU.
 B200_DEVICE int64_t share_begin(int64_t total, int64_t c, int64_t n) { return total * c / n; }
 B200_DEVICE int64_t share_owner(int64_t total, int64_t u, int64_t n) { return ((u + 1) * n - 1) / total; }
 
 // A place in the line of tiles: tile t of (sequence b, virtual head vh).
 struct Place {
     int b, vh, len, tiles, t;
-    int64_t left;  // tiles of this CTA's share from here on
+    int64_t left;  // units of this CTA's share from the tile's first on; none: past its end
 };
 
+// On to the first tile of the next virtual head, or sequence that has keys.
 template <int TILE, typename A>
-B200_DEVICE void place_next(const A &a, Place &p) {
-    --p.left;
-    if (++p.t < p.tiles || p.left == 0) return;
+B200_DEVICE void place_pair(const A &a, Place &p) {
     p.t = 0;
     if (++p.vh < a.VH) return;
     p.vh = 0;
-    do {  // the share has tiles left, so a sequence with some follows
+    do {  // the share has units left, so a sequence with some follows
         ++p.b;
         p.len = seq_len(a, p.b);
     } while (p.len == 0);
     p.tiles = (p.len + TILE - 1) / TILE;
 }
 
-template <int TILE, typename A>
+template <int TILE, int TU = 1, int PU = 0, typename A>
+B200_DEVICE void place_next(const A &a, Place &p) {
+    p.left -= TU;
+    if (++p.t < p.tiles || p.left <= 0) return;
+    p.left -= PU;
+    if (p.left > 0) place_pair<TILE>(a, p);
+}
+
+template <int TILE, int TU = 1, int PU = 0, typename A>
 B200_DEVICE Place place_at(const A &a, int64_t u0, int64_t u1) {
     const int lane = threadIdx.x & 31;
-    int64_t before = 0;  // tiles of the sequences before `base`
+    int64_t before = 0;  // units of the sequences before `base`
     Place p = {};
     for (int base = 0; base < a.n_seqs; base += 32) {
         const int b = base + lane;
-        const int64_t n = b < a.n_seqs ? seq_tiles<TILE>(a, b) : 0;
+        const int64_t n = b < a.n_seqs ? units_of<TU, PU>(seq_tiles<TILE>(a, b)) : 0;
         int64_t incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -82,10 +95,15 @@ B200_DEVICE Place place_at(const A &a, int64_t u0, int64_t u1) {
             p.b = base + l;
             p.len = seq_len(a, p.b);
             p.tiles = (p.len + TILE - 1) / TILE;
-            const int64_t in = u0 - excl * a.VH;
-            p.vh = static_cast<int>(in / p.tiles);
-            p.t = static_cast<int>(in - static_cast<int64_t>(p.vh) * p.tiles);
-            p.left = u1 - u0;
+            const int64_t in = u0 - excl * a.VH, pair = units_of<TU, PU>(p.tiles);
+            p.vh = static_cast<int>(in / pair);
+            const int64_t off = in - static_cast<int64_t>(p.vh) * pair;
+            p.t = static_cast<int>((off + TU - 1) / TU);
+            p.left = u1 - u0 - (static_cast<int64_t>(p.t) * TU - off);
+            if (PU && p.t >= p.tiles) {  // behind the last tile's first unit: the next pair's
+                p.left = u1 - u0 - (pair - off);
+                if (p.left > 0) place_pair<TILE>(a, p);
+            }
             break;
         }
         before += __shfl_sync(0xffffffffu, incl, 31);

@@ -126,11 +126,15 @@ __global__ void __launch_bounds__(kQ8Threads) paged_read_q8_kernel(const Q8Args 
         const float f = e8m0_value(b[i]);
         T x[E];
 #pragma unroll
-        for (int j = 0; j < E; j += 2) {
-            const uint32_t h2 = e4m3x2_to_f16x2(q[i][j / 4] >> (8 * (j & 2)));
-            const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h2));
-            x[j] = from_f32<T>(v.x * f);
-            x[j + 1] = from_f32<T>(v.y * f);
+        for (int j = 0; j < E; j += 4) {
+            uint32_t h[2];
+            e4m3x4_to_f16(q[i][j / 4], h[0], h[1]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&h[u]));
+                x[j + 2 * u] = from_f32<T>(v.x * f);
+                x[j + 2 * u + 1] = from_f32<T>(v.y * f);
+            }
         }
         *reinterpret_cast<uint4 *>(dst + (h0 + i * (32 / L)) * a.row_head[kv]) = *reinterpret_cast<const uint4 *>(x);
     }

@@ -20,11 +20,11 @@ B200_DEVICE uint32_t e8m0_of(uint32_t top_bits) {
 // 2^-e
 B200_DEVICE float e8m0_inverse(uint32_t b) { return __uint_as_float((254u - b) << 23); }  // b <= 247
 
-// Two e4m3 numbers as F16 (exact; the low byte in the low half).
-B200_DEVICE uint32_t e4m3x2_to_f16x2(uint32_t two) {
-    uint32_t r;
-    asm("{\n .reg .b16 x;\n cvt.u16.u32 x, %1;\n cvt.rn.f16x2.e4m3x2 %0, x;\n}" : "=r"(r) : "r"(two));
-    return r;
+// The four e4m3 numbers of a word as F16 (exact): bytes 0 and 1, and 2 and 3.
+B200_DEVICE void e4m3x4_to_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
 }
 
 inline int check_pool_q8(const b200_kv_pool_q8 *p) {
