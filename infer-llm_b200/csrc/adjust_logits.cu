@@ -2,11 +2,11 @@
 //
 //   x <- x / r or x r (known), x - f count - p (drawn), x + bias, -inf (masked)
 //
-// A pass over the logits, which HBM bounds; what has to be known of a token (how often it was drawn, whether the row knows it, its bias)
-// is gathered before, in shared memory, for the chunk of the vocabulary that a CTA takes: it
-// walks its row's history and counts what falls into its chunk. Counts are whole numbers, so their order does not matter.
-// A row's history is walked once per chunk, from L2: a chunk of 8192 tokens (19 of a vocabulary of 151936) keeps that
-// below the logits' own bytes up to 8192 F32 tokens of history; smaller chunks where there are few rows.
+// A pass over the logits, which HBM bounds, by CTAs that take a chunk of a row's vocabulary each. What a row's history and biases say
+// concerns few tokens: a CTA walks them for those of its chunk, sets a bit a token, counts the bits before each word, and so has a slot of its
+// own for each such token, in which it counts; the pass then writes the chunk with the masked tokens replaced, and last come the tokens
+// with slots, a thread each. Eight warps pass and four walk at the same time, since the walk's chain (offsets, tokens, counters) is as long
+// as the pass; each pass warp asks for its next vectors before it writes the last. Counts are whole numbers, so their order does not matter.
 #include "batch.cuh"
 #include "gemv.cuh"
 
@@ -17,7 +17,7 @@ struct AdjustArgs {
     const void *in = nullptr;
     void *out = nullptr;
     int64_t in_row = 0, out_row = 0, n_rows = 0, n_tokens = 0, n_biases = 0, mask_row = 0;  // rows: elements (mask: words)
-    int32_t vocab = 0, chunk = 0, chunks = 0;
+    int32_t vocab = 0;
     const int32_t *tokens = nullptr, *cu_tokens = nullptr, *prompt_lens = nullptr;
     const float *repetition = nullptr, *frequency = nullptr, *presence = nullptr;
     const int32_t *bias_ids = nullptr, *cu_bias = nullptr;
@@ -26,14 +26,16 @@ struct AdjustArgs {
     int32_t *status = nullptr;
 };
 
-constexpr int kAdThreads = 256;
-constexpr uint32_t kKnown = 1u << 31;  // a token of the history; the bits below count how often it was drawn
+constexpr int kAdPass = 256, kAdWalk = 128, kAdThreads = kAdPass + kAdWalk;  // threads that pass, and that walk
+constexpr int kAdUnroll = 2;                                     // vectors a thread of the pass takes at once
+constexpr int kAdChunk = 16384, kAdSlots = 2048, kAdAtOnce = 8;  // tokens and slots of a CTA at most; list entries a thread asks for at once
+constexpr uint32_t kKnown = 1u << 31;  // in a slot: a token of the history; the bits below count how often it was drawn
 
 // The row's range of a packed list, empty (and reported) where the offsets are out of order or range.
 B200_DEVICE void list_range(const int32_t *cu, int64_t row, int64_t total, int32_t *status, int64_t &from, int64_t &to) {
     from = __ldg(cu + row), to = __ldg(cu + row + 1);
     if (from >= 0 && from <= to && to <= total) return;
-    if (threadIdx.x == 0) set_status(status, B200_DEV_BAD_POSITION);
+    set_status(status, B200_DEV_BAD_POSITION);
     from = to = 0;
 }
 
@@ -42,128 +44,206 @@ B200_DEVICE float penalty(const float *p, int64_t row, float off, bool positive,
     if (!p) return off;
     const float x = __ldg(p + row);
     if (fabsf(x) < INFINITY && (!positive || x > 0.f)) return x;
-    if (threadIdx.x == 0) set_status(status, B200_DEV_BAD_LOGITS);
+    set_status(status, B200_DEV_BAD_LOGITS);
     return off;
 }
 
+// visit(i, load(i)) for i = tid, tid + kAdWalk, ... below n, kAdAtOnce loads at once.
+template <typename Load, typename Visit>
+B200_DEVICE void batches(int n, int tid, Load load, Visit visit) {
+    for (int i0 = tid; i0 < n; i0 += kAdAtOnce * kAdWalk) {
+        decltype(load(0)) x[kAdAtOnce] = {};
+#pragma unroll
+        for (int j = 0; j < kAdAtOnce; ++j)
+            if (i0 + j * kAdWalk < n) x[j] = load(i0 + j * kAdWalk);
+#pragma unroll
+        for (int j = 0; j < kAdAtOnce; ++j)
+            if (i0 + j * kAdWalk < n) visit(i0 + j * kAdWalk, x[j]);
+    }
+}
+
+// kAdUnroll vectors of a row from token t on, kAdPass vectors apart.
 template <typename T>
-__global__ void __launch_bounds__(kAdThreads) adjust_logits_kernel(const __grid_constant__ AdjustArgs a) {
-    constexpr int V = 16 / sizeof(T);
-    extern __shared__ __align__(16) uint32_t ad_smem[];
-    const int64_t row = blockIdx.x / static_cast<unsigned>(a.chunks);
-    const int first = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.chunks)) * a.chunk;
+struct Vectors {
+    static constexpr int V = 16 / sizeof(T);
+    static constexpr uint32_t kAll = (1u << V) - 1u;
+    uint4 x[kAdUnroll];
+    uint32_t allowed[kAdUnroll];  // bit j: token t + j may be drawn
+
+    B200_DEVICE void fetch(const T *in, const uint32_t *mask, int t, int vocab, bool in_place) {
+#pragma unroll
+        for (int i = 0; i < kAdUnroll; ++i, t += V * kAdPass) {
+            if (!in_place && t >= 0 && t + V <= vocab) x[i] = __ldg(reinterpret_cast<const uint4 *>(in + t));
+            allowed[i] = kAll;
+            if (mask && t < vocab) {
+                const int at = max(t, 0), w = at >> 5;
+                const uint32_t lo = __ldg(mask + w);
+                const uint32_t hi = (at & 31) > 32 - V && w < (vocab - 1) >> 5 ? __ldg(mask + w + 1) : 0u;
+                allowed[i] = __funnelshift_r(lo, hi, at & 31) << (at - t) & kAll;
+            }
+        }
+    }
+    // wide: out's rows are aligned as in's
+    B200_DEVICE void write(const T *in, T *out, int t, int vocab, bool in_place, bool wide) {
+#pragma unroll
+        for (int i = 0; i < kAdUnroll; ++i, t += V * kAdPass) {
+            if (t >= vocab) break;
+            if (in_place && allowed[i] == kAll) continue;
+            if (t >= 0 && t + V <= vocab) {
+                if (in_place && allowed[i]) x[i] = *reinterpret_cast<const uint4 *>(in + t);
+                T *e = reinterpret_cast<T *>(&x[i]);
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (!(allowed[i] >> j & 1u)) e[j] = from_f32<T>(-INFINITY);
+                if (wide) {
+                    *reinterpret_cast<uint4 *>(out + t) = x[i];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) out[t + j] = e[j];
+                }
+            } else {  // the row's first and last tokens
+                for (int j = max(0, -t); j < V && t + j < vocab; ++j)
+                    out[t + j] = allowed[i] >> j & 1u ? in[t + j] : from_f32<T>(-INFINITY);
+            }
+        }
+    }
+};
+
+// steps: the chunk is steps * kAdUnroll vectors a thread of the pass.
+template <typename T>
+__global__ void __launch_bounds__(kAdThreads, 4) adjust_logits_kernel(const __grid_constant__ AdjustArgs a, const int steps) {
+    constexpr int V = 16 / sizeof(T), kStep = kAdUnroll * V * kAdPass, kWords = kAdChunk / 32, kPer = kWords / kAdWalk;
+    static_assert(kPer == 4 && kAdChunk % kStep == 0, "four words a thread that walks, whole steps");
+    __shared__ __align__(16) uint32_t named[kWords];  // bit t % 32 of word t / 32: token begin + t is named
+    __shared__ __align__(8) uint16_t before[kWords];  // named tokens before the word
+    __shared__ uint32_t known[kAdSlots], bias[kAdSlots];
+    __shared__ uint16_t token[kAdSlots];
+    __shared__ int warp_sums[kAdWalk / 32], total;
+    const int64_t row = blockIdx.x;
     const T *in = static_cast<const T *>(a.in) + row * a.in_row;
     T *out = static_cast<T *>(a.out) + row * a.out_row;
-    // The chunk begins where its vectors are aligned in `in`: up to V - 1 elements before `first`
+    // The chunk begins where its vectors are aligned in `in`, up to V - 1 elements before a multiple of its size. (The last
+    // chunk's end is the row's: chunks * steps * kStep >= vocab + V - 1.)
     const int skew = static_cast<int>(reinterpret_cast<uintptr_t>(in) / sizeof(T) % V);
-    const int begin = first - skew, end = min(begin + a.chunk, a.vocab);  // this CTA's tokens
-    // (the last chunk's end is the row's: chunks * chunk >= vocab + V)
-    const bool in_place = a.in == a.out;
-    const bool wide = reinterpret_cast<uintptr_t>(out) / sizeof(T) % V == static_cast<unsigned>(skew);
-    uint32_t *known = ad_smem, *bias = ad_smem + (a.tokens ? a.chunk : 0);
-    const int words = (a.tokens ? a.chunk : 0) + (a.bias_ids ? a.chunk : 0);
-    bool any = false;  // a token of this chunk is known or biased
-    float rep = 1.f, freq = 0.f, pres = 0.f;
-    if (words) {
-        for (int i = threadIdx.x; i < words / 4; i += kAdThreads) reinterpret_cast<uint4 *>(ad_smem)[i] = make_uint4(0, 0, 0, 0);
-        __syncthreads();
-        if (a.tokens) {
-            rep = penalty(a.repetition, row, 1.f, true, a.status);
-            freq = penalty(a.frequency, row, 0.f, false, a.status);
-            pres = penalty(a.presence, row, 0.f, false, a.status);
-            int64_t from, to;
-            list_range(a.cu_tokens, row, a.n_tokens, a.status, from, to);
-            const int64_t drawn = from + (a.prompt_lens ? max(0, __ldg(a.prompt_lens + row)) : 0);
-            for (int64_t i = from + threadIdx.x; i < to; i += kAdThreads) {
-                const int t = __ldg(a.tokens + i);
-                if (t < 0 || t >= a.vocab) set_status(a.status, B200_DEV_BAD_TOKEN);
-                else if (t >= begin && t < end) {
-                    any = true;
-                    if (i >= drawn) atomicAdd(known + (t - begin), 1u);
-                    atomicOr(known + (t - begin), kKnown);
-                }
-            }
-        }
-        if (a.bias_ids) {
-            int64_t from, to;
-            list_range(a.cu_bias, row, a.n_biases, a.status, from, to);
-            for (int64_t i = from + threadIdx.x; i < to; i += kAdThreads) {
-                const int t = __ldg(a.bias_ids + i);
-                if (t < 0 || t >= a.vocab) set_status(a.status, B200_DEV_BAD_TOKEN);
-                else if (t >= begin && t < end) {
-                    any = true;
-                    atomicMax(bias + (t - begin), static_cast<uint32_t>(i + 1));  // of several the last
-                }
-            }
-        }
-        any = __syncthreads_or(any);
-    }
-    const auto adjusted = [&](T x, int t) {
-        float y = to_f32<T>(x);
-        if (a.tokens) {
-            const uint32_t u = known[t - begin];
-            if (u) {
-                y = y > 0.f ? y / rep : y * rep;
-                const uint32_t count = u & ~kKnown;
-                if (count) y = y - freq * static_cast<float>(count) - pres;
-            }
-        }
-        if (a.bias_ids) {
-            const uint32_t i = bias[t - begin];
-            if (i) y += __ldg(a.bias_values + (i - 1));
-        }
-        return from_f32<T>(y);
-    };
+    const int begin = static_cast<int>(blockIdx.y) * steps * kStep - skew;
     const uint32_t *mask = a.mask ? a.mask + row * a.mask_row : nullptr;
-    const int last_word = (a.vocab - 1) >> 5;
-    for (int t = begin + V * static_cast<int>(threadIdx.x); t < end; t += V * kAdThreads) {
-        uint32_t allowed = ~0u;  // bit j: token t + j may be drawn
-        if (mask) {
-            const int at = max(t, 0), w = at >> 5;
-            const uint32_t lo = __ldg(mask + w), hi = w < last_word ? __ldg(mask + w + 1) : 0u;
-            allowed = __funnelshift_r(lo, hi, at & 31) << (at - t);
+    const bool walks = threadIdx.x >= kAdPass;
+    const int tid = walks ? threadIdx.x - kAdPass : threadIdx.x, lane = tid & 31;
+
+    // The lists, and a slot a token that they name: the first kAdSlots, the others later. Threads that walk only.
+    int64_t bias_from = 0;
+    const int32_t *tokens = nullptr, *biases = nullptr;
+    int n = 0, m = 0, prompt = 0;
+    const uint32_t least = static_cast<uint32_t>(max(begin, 0)), span = static_cast<uint32_t>(min(begin + steps * kStep, a.vocab)) - least;
+    const auto in_chunk = [&](int t) { return static_cast<uint32_t>(t) - least < span; };
+    const auto count = [&](int first) {
+        for (int i = tid; i < min(total - first, kAdSlots); i += kAdWalk) known[i] = bias[i] = 0;
+        named_sync(1, kAdWalk);
+        const auto slot_of = [&](int t) {  // kAdSlots and more: none
+            if (!in_chunk(t)) return ~0u;
+            const uint32_t at = static_cast<uint32_t>(t - begin), w = at >> 5;
+            const uint32_t slot = before[w] + __popc(named[w] & ((1u << (at & 31)) - 1u)) - static_cast<uint32_t>(first);
+            if (slot < kAdSlots) token[slot] = static_cast<uint16_t>(at);
+            return slot;
+        };
+        batches(n, tid, [&](int i) { return __ldg(tokens + i); }, [&](int i, int t) {
+            const uint32_t slot = slot_of(t);
+            if (slot >= kAdSlots) return;
+            atomicOr(known + slot, kKnown);
+            if (i >= prompt) atomicAdd(known + slot, 1u);
+        });
+        batches(m, tid, [&](int i) { return __ldg(biases + i); }, [&](int i, int t) {
+            const uint32_t slot = slot_of(t);
+            if (slot < kAdSlots) atomicMax(bias + slot, static_cast<uint32_t>(i + 1));  // of several the last
+        });
+    };
+    if (!walks) {
+        const bool in_place = a.in == a.out, wide = static_cast<int>(reinterpret_cast<uintptr_t>(out) / sizeof(T) % V) == skew;
+        Vectors<T> now, next;
+        int t = begin + V * tid;
+        now.fetch(in, mask, t, a.vocab, in_place);
+        for (int step = 1; step < steps; ++step, t += kStep) {
+            next.fetch(in, mask, t + kStep, a.vocab, in_place);
+            now.write(in, out, t, a.vocab, in_place, wide);
+            now = next;
         }
-        const bool whole = t >= 0 && t + V <= a.vocab;
-        constexpr uint32_t kAll = (1u << V) - 1u;
-        if (in_place && !any && (allowed & kAll) == kAll) continue;
-        if (whole) {
-            uint4 u = *reinterpret_cast<const uint4 *>(in + t);
-            T *e = reinterpret_cast<T *>(&u);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if (any) e[j] = adjusted(e[j], t + j);
-                if (!(allowed >> j & 1u)) e[j] = from_f32<T>(-INFINITY);
-            }
-            if (wide) {
-                *reinterpret_cast<uint4 *>(out + t) = u;
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) out[t + j] = e[j];
-            }
-        } else {
-            for (int j = max(0, -t); j < V && t + j < a.vocab; ++j) {
-                const T x = any ? adjusted(in[t + j], t + j) : in[t + j];
-                out[t + j] = allowed >> j & 1u ? x : from_f32<T>(-INFINITY);
-            }
+        now.write(in, out, t, a.vocab, in_place, wide);
+    } else {
+        int64_t from = 0, to = 0, bias_to = 0;
+        if (a.tokens) {
+            list_range(a.cu_tokens, row, a.n_tokens, a.status, from, to);
+            if (a.prompt_lens) prompt = max(0, __ldg(a.prompt_lens + row));
         }
+        if (a.bias_ids) list_range(a.cu_bias, row, a.n_biases, a.status, bias_from, bias_to);
+        tokens = a.tokens + from, biases = a.bias_ids + bias_from;
+        n = static_cast<int>(to - from), m = static_cast<int>(bias_to - bias_from);
+        *reinterpret_cast<uint4 *>(named + kPer * tid) = make_uint4(0, 0, 0, 0);
+        named_sync(1, kAdWalk);
+        bool odd = false;  // an id that names no token (the first chunk's CTA reports it)
+        const auto mark = [&](int, int t) {
+            const uint32_t at = static_cast<uint32_t>(t - begin);
+            if (in_chunk(t)) atomicOr(named + (at >> 5), 1u << (at & 31));
+            odd |= static_cast<uint32_t>(t) >= static_cast<uint32_t>(a.vocab);
+        };
+        batches(n, tid, [&](int i) { return __ldg(tokens + i); }, mark);
+        batches(m, tid, [&](int i) { return __ldg(biases + i); }, mark);
+        if (odd && blockIdx.y == 0) set_status(a.status, B200_DEV_BAD_TOKEN);
+        named_sync(1, kAdWalk);
+        const uint4 w4 = *reinterpret_cast<const uint4 *>(named + kPer * tid);
+        const int c0 = __popc(w4.x), c1 = c0 + __popc(w4.y), c2 = c1 + __popc(w4.z), own = c2 + __popc(w4.w);
+        int up_to = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, up_to, o);
+            if (lane >= o) up_to += y;
+        }
+        if (lane == 31) warp_sums[tid >> 5] = up_to;
+        named_sync(1, kAdWalk);
+        int base = up_to - own, sum = 0;
+#pragma unroll
+        for (int w = 0; w < kAdWalk / 32; ++w) {
+            if (w < tid >> 5) base += warp_sums[w];
+            sum += warp_sums[w];
+        }
+        *reinterpret_cast<ushort4 *>(before + kPer * tid) = make_ushort4(base, base + c0, base + c1, base + c2);
+        if (tid == 0) total = sum;
+        named_sync(1, kAdWalk);
+        if (sum > 0) count(0);
+    }
+    __syncthreads();  // the slots are counted, and the pass has written their tokens
+    if (total == 0) return;
+    const float rep = penalty(a.tokens ? a.repetition : nullptr, row, 1.f, true, a.status);
+    const float freq = penalty(a.tokens ? a.frequency : nullptr, row, 0.f, false, a.status);
+    const float pres = penalty(a.tokens ? a.presence : nullptr, row, 0.f, false, a.status);
+    const float *bias_values = a.bias_ids ? a.bias_values + __ldg(a.cu_bias + row) : nullptr;
+    for (int first = 0;;) {
+        for (int i = threadIdx.x; i < min(total - first, kAdSlots); i += kAdThreads) {
+            const int t = begin + token[i];
+            const uint32_t u = known[i], drawn = u & ~kKnown, b = bias[i];
+            if (mask && !(__ldg(mask + (t >> 5)) >> (t & 31) & 1u)) continue;
+            float y = to_f32<T>(in[t]);  // in place: still what it was
+            if (u) y = y > 0.f ? y / rep : y * rep;
+            if (drawn) y = y - freq * static_cast<float>(drawn) - pres;
+            if (b) y += __ldg(bias_values + (b - 1));
+            out[t] = from_f32<T>(y);
+        }
+        first += kAdSlots;
+        if (first >= total) return;
+        __syncthreads();  // the slots are free again
+        if (walks) count(first);
+        __syncthreads();
     }
 }
 
 template <typename T>
-cudaError_t adjust_launch(AdjustArgs a, cudaStream_t st) {
-    constexpr int V = 16 / sizeof(T);
-    a.chunk = 8192;
-    while (a.chunk > 1024 && a.n_rows * ((a.vocab + a.chunk - 1) / a.chunk) < 4 * device_sm_count()) a.chunk /= 2;
-    a.chunks = (a.vocab + V - 1 + a.chunk - 1) / a.chunk;
-    if (a.n_rows > INT32_MAX / a.chunks) return cudaErrorNotSupported;
-    const size_t smem = static_cast<size_t>(a.chunk) * 4 * ((a.tokens ? 1 : 0) + (a.bias_ids ? 1 : 0));
-    auto kern = adjust_logits_kernel<T>;
-    const cudaError_t e = once_per_device(reinterpret_cast<const void *>(kern), ATTR_SMEM, [&] {
-        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
-    });
-    if (e != cudaSuccess) return e;
-    kern<<<static_cast<unsigned>(a.n_rows * a.chunks), kAdThreads, smem, st>>>(a);
-    return cudaGetLastError();
+cudaError_t adjust_launch(const AdjustArgs &a, cudaStream_t st) {
+    constexpr int V = 16 / sizeof(T), kStep = kAdUnroll * V * kAdPass;
+    int steps = kAdChunk / kStep;
+    const auto chunks = [&] { return (a.vocab + V - 1 + steps * kStep - 1) / (steps * kStep); };
+    while (steps > 1 && a.n_rows * chunks() < 4 * device_sm_count()) steps /= 2;  // fewer CTAs than run at once
+    if (a.n_rows > INT32_MAX) return cudaErrorNotSupported;
+    const dim3 grid(static_cast<unsigned>(a.n_rows), static_cast<unsigned>(chunks()));  // y <= 2^10 + 1
+    return b200_launch(adjust_logits_kernel<T>, grid, dim3(kAdThreads), 0, st, false, a, steps);
 }
 
 }  // namespace
