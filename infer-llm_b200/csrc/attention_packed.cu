@@ -20,7 +20,7 @@ __global__ void __launch_bounds__(kPkThreads, 2) packed_ffma_kernel(const Packed
     if (p.seq < 0) return;
     const int r0 = p.tile * kPkRows, rows = min(kPkRows, p.nq * a.G - r0);
     T *out = static_cast<T *>(a.out);
-    ffma_rows<T, D>(a, p, kvh, r0, rows, 0, p.nk, pk_smem, threadIdx.x, [] { __syncthreads(); },
+    ffma_rows<T, D, true>(a, p, kvh, r0, rows, 0, p.nk, PackedKeys<T>(a, p, kvh), pk_smem, threadIdx.x, [] { __syncthreads(); },
                     [&](int r, int c, const float (&x)[4], float, float) {
                         T *dst = out + (p.q0 + (r0 + r) / a.G) * a.o_tok + (kvh * a.G + (r0 + r) % a.G) * a.o_head + c;
 #pragma unroll

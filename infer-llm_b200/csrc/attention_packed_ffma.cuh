@@ -31,17 +31,17 @@ constexpr size_t ffma_smem() {
 }
 
 // Rows [r0, r0 + rows) (row = token * G + head of the KV head's group; at most kPkRows) of sequence p against its
-// keys [first, end), by kPkThreads threads, of which this is `tid`; sync() is their barrier and
+// keys [first, end) (CAUSAL: those that each sees; key(j, k, v) points at key j's rows, false: it takes no part), by kPkThreads threads, of which this is `tid`; sync() is their barrier and
 // smem (16-byte aligned, ffma_smem<D>() bytes) theirs. store(row, column, x, m, l) gets each row's
 // output four columns at a time, already over l, its maximum (in powers of two) and its sum.
-template <typename T, int D, typename Sync, typename Store>
-B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, int r0, int rows, int first, int end,
+template <typename T, int D, bool CAUSAL, typename Key, typename Sync, typename Store>
+B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, int r0, int rows, int first, int end, Key key,
                            float *smem, int tid, Sync sync, Store store) {
     float *qt = smem;                  // [D][row]
     float *kt = qt + D * kPkPad;       // [D][key]; then P [key][row]
     float *vs = kt + D * kPkPad;       // [key][D]
     const int ty = tid >> 4, tx = tid & 15;
-    const T *q = static_cast<const T *>(a.q), *k = static_cast<const T *>(a.k), *v = static_cast<const T *>(a.v);
+    const T *q = static_cast<const T *>(a.q);
     // four elements a load; lanes take neighbouring rows, so the transposed stores do not collide
 #pragma unroll
     for (int i0 = 0; i0 < kPkRows * D / 4; i0 += kPkThreads) {
@@ -54,10 +54,11 @@ B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, in
 #pragma unroll
         for (int e = 0; e < 4; ++e) qt[(d + e) * kPkPad + r] = x[e];
     }
-    end = min(end, p.nk - p.nq + (r0 + rows - 1) / a.G + 1);  // the keys the last row sees
+    if (CAUSAL) end = min(end, p.nk - p.nq + (r0 + rows - 1) / a.G + 1);  // the keys the last row sees
     int last[4];  // last key each row sees (relative to the sequence)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) last[i] = 4 * ty + i < rows ? min(end - 1, p.nk - p.nq + (r0 + 4 * ty + i) / a.G) : -1;
+    for (int i = 0; i < 4; ++i)
+        last[i] = 4 * ty + i < rows ? (CAUSAL ? min(end - 1, p.nk - p.nq + (r0 + 4 * ty + i) / a.G) : end - 1) : -1;
     float m[4], l[4], o[4][D / 16];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -71,11 +72,11 @@ B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, in
 #pragma unroll
         for (int i0 = 0; i0 < kPkKeys * D / 4; i0 += kPkThreads) {
             const int i = i0 + tid, j = i % kPkKeys, d = i / kPkKeys * 4;
-            const int64_t t = p.k0 + k0 + j;
             float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-            if (k0 + j < end) {
-                load4(k + t * a.k_tok + kvh * a.k_head + d, x);
-                load4(v + t * a.v_tok + kvh * a.v_head + d, y);
+            const T *k, *v;
+            if (k0 + j < end && key(k0 + j, k, v)) {
+                load4(k + d, x);
+                load4(v + d, y);
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) kt[(d + e) * kPkPad + j] = x[e];
@@ -122,7 +123,7 @@ B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, in
         sync();
         // a key that a row does not see has P = 0, and 0 times a V that is no number would
         // not be 0: such products are left out where the tile has hidden keys
-        const bool all = k0 + kPkKeys - 1 <= min(end - 1, p.nk - p.nq + r0 / a.G);
+        const bool all = k0 + kPkKeys - 1 <= (CAUSAL ? min(end - 1, p.nk - p.nq + r0 / a.G) : end - 1);
 #pragma unroll 4
         for (int j = 0; j < kPkKeys; ++j) {
             const float4 x = *reinterpret_cast<const float4 *>(kt + j * kPkPad + 4 * ty);
@@ -154,5 +155,19 @@ B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, in
         }
     }
 }
+
+// ffma_rows' keys of a packed sequence.
+template <typename T>
+struct PackedKeys {
+    const T *k, *v;
+    int64_t k_tok, v_tok;
+    B200_DEVICE PackedKeys(const PackedArgs &a, const PackedTile &p, int kvh)
+        : k(static_cast<const T *>(a.k) + p.k0 * a.k_tok + kvh * a.k_head),
+          v(static_cast<const T *>(a.v) + p.k0 * a.v_tok + kvh * a.v_head), k_tok(a.k_tok), v_tok(a.v_tok) {}
+    B200_DEVICE bool operator()(int j, const T *&kr, const T *&vr) const {
+        kr = k + j * k_tok, vr = v + j * v_tok;
+        return true;
+    }
+};
 
 }  // namespace b200

@@ -56,6 +56,7 @@
 // waits (bounded) for its copies and products and frees its tensor memory.
 #include "attention_packed_ffma.cuh"
 #include "gemv.cuh"
+#include "shared_prefix.cuh"
 #include "tcgen05.cuh"
 #include "tma.cuh"
 
@@ -414,14 +415,18 @@ __global__ void __launch_bounds__(kSplitThreads) packed_split_kernel(const Packe
     }
 }
 
-template <typename T, int D, int NT, int SL>
+// PX: a row is a sequence of a group that shares a prefix, times a head; every row sees every key. K and V come from the pool's blocks, in
+// boxes of px_rows positions (the largest power of two that the blocks are made of), a lane of the copying warp a box.
+template <typename T, int D, int NT, int SL, bool PX>
 __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     packed_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                     const __grid_constant__ CUtensorMap tv, const PackedArgs a, const SplitView sp) {
+                     const __grid_constant__ CUtensorMap tv, const PackedArgs a, const SplitView sp, const PrefixArgs px,
+                     const int px_rows) {
     constexpr bool SPLIT = __is_same(T, float);
     constexpr int PL = SPLIT ? 2 : 1;
     using Ge = PtGeometry<D, NT, SL, PL>;
     static_assert(SL == 2 || (NT == 1 && !SPLIT), "one slot holds one query tile");
+    static_assert(!PX || (NT == 1 && SL == 2 && !SPLIT), "prefixes: one tile in two slots, 16-bit types");
     constexpr bool kPairs = NT == 2 || SL == 1, kJoin = NT == 1 && SL == 2;  // kJoin: the slots halve the key tiles
     constexpr int kColumns = 256 * SL;  // of tensor memory
     constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
@@ -448,6 +453,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     uint32_t *bad = reinterpret_cast<uint32_t *>(base + Ge::kOffBad);
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    if constexpr (PX) grid_launch_dependents();  // the kernel of the sequences' own keys waits for this grid's end
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 1);
@@ -471,13 +477,15 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
         for (const CUtensorMap *m : {&tq, &tk, &tv})
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
     }
-    if (threadIdx.x < 4 * kMaskedTiles + 2) bad[threadIdx.x] = 0;
+    if (threadIdx.x < 4 * kMaskedTiles + 3) bad[threadIdx.x] = 0;
+    uint32_t &bad_block = bad[4 * kMaskedTiles + 2];  // PX: a block of this CTA's keys is out of range
     uint32_t &any_wide = bad[4 * kMaskedTiles + 1];  // F32: a key tile was not held by two F16 numbers
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(kColumns)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        if (blockIdx.x == gridDim.x - 1) clear_uncovered(a);
+        if constexpr (!PX)
+            if (blockIdx.x == gridDim.x - 1) clear_uncovered(a);
     }
 
     const int G = a.G, BQ = kPtRows / G, MT = NT * BQ;  // tokens of a query tile, of the CTA
@@ -486,9 +494,14 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     PackedTile *found = reinterpret_cast<PackedTile *>(bars + 44);
     if (warp == 3) {
         const int64_t at = blockIdx.x / (sp.parts * a.Hkv);
-        const PackedTile f = sp.by_weight ? find_heaviest_tile(a, MT, at, a.status)
-                                          : find_packed_tile(a.cu_q, a.cu_k, a.n_seqs, a.total_q, a.total_k, 1, MT, at, a.status);
-        if (lane == 0) *found = f;
+        if constexpr (PX) {
+            const PackedTile f = find_prefix_tile(px, 1, MT, at);
+            if (lane == 0) *found = f;
+        } else {
+            const PackedTile f = sp.by_weight ? find_heaviest_tile(a, MT, at, a.status)
+                                              : find_packed_tile(a.cu_q, a.cu_k, a.n_seqs, a.total_q, a.total_k, 1, MT, at, a.status);
+            if (lane == 0) *found = f;
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -504,12 +517,12 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     const bool some = p.seq >= 0;                      // not past the last tile
     const int t0 = p.tile * MT;                        // first token
     const int shift = p.nk - p.nq;                     // token t sees keys 0 .. t + shift
-    const int seen = min(p.nq, t0 + MT) + shift;       // keys the last token sees (may be <= 0)
+    const int seen = PX ? p.nk : min(p.nq, t0 + MT) + shift;  // keys the last token sees (may be <= 0)
     const int tiles = some && seen > 0 ? (seen + kPtKeys - 1) / kPtKeys : 0;  // key tiles, of which this CTA's:
     const int ta = tiles * part / sp.parts, nt = tiles * (part + 1) / sp.parts - ta;
     const int steps = NT * nt;
     // the CTA's tiles from this one on hide keys from some row
-    const int first_masked = max(0, (t0 + shift + 1) / kPtKeys - ta);
+    const int first_masked = max(0, (PX ? p.nk : t0 + shift + 1) / kPtKeys - ta);
     const int64_t k0 = p.k0 + static_cast<int64_t>(ta) * kPtKeys;  // its first key
 
     const auto col_s = [&](int slot) { return tmem + static_cast<uint32_t>(slot * kPtKeys); };
@@ -526,7 +539,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     const uint32_t lanes = static_cast<uint32_t>(32 * qq) << 16;
     const int tok = t0 + (NT == 2 ? slot * BQ : 0) + r / G;
     const bool live = some && r < BQ * G && tok < p.nq;
-    const int last = live ? tok + shift - ta * kPtKeys : -1;  // last of the CTA's keys that the row sees
+    const int last = live ? (PX ? p.nk - 1 : tok + shift) - ta * kPtKeys : -1;  // last of the CTA's keys that the row sees
     const T *q_row = static_cast<const T *>(a.q) + (p.q0 + tok) * a.q_tok + (kvh * G + r % G) * a.q_head;
     // Rows of a query tile (first token t) from shared memory to the output: a thread writes its
     // row's 16-byte chunk c to row r, chunk c ^ (r % 8) of `stage`, and the group's threads
@@ -550,15 +563,20 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
         return reinterpret_cast<uint4 *>(stage + (r * kRowChunks + (c ^ (r & 7))) * 16);
     };
     // this CTA's part of the row: its normalised output, and (m, l) to weigh it by
-    const int64_t part_row = static_cast<int64_t>(blockIdx.x) * kPtRows + r;
+    const int64_t part_row = PX ? prefix_row(px, part, p.q0 + tok, kvh * G + r % G) : static_cast<int64_t>(blockIdx.x) * kPtRows + r;
+    float *part_o = PX ? px.o : sp.part_o;
+    float2 *part_ml = PX ? px.ml : sp.part_ml;
+    const bool whole_out = !PX && sp.parts == 1;  // the row's output is written, not a part of it
     // x (columns [c, c + 32) of the row's output) plus the terms of the cleared V rows it sees
     const auto add_cleared = [&](float (&x)[32], int c, float m_row, float inv) {
         for (int w = 0; w < 4 * kMaskedTiles; ++w) {
             for (uint32_t mask = bad[w]; mask; mask &= mask - 1) {
                 const int key = first_masked * kPtKeys + 32 * w + __ffs(static_cast<int>(mask)) - 1;
                 if (key > last) continue;
-                const T *kr = static_cast<const T *>(a.k) + (k0 + key) * a.k_tok + kvh * a.k_head;
-                const T *vr = static_cast<const T *>(a.v) + (k0 + key) * a.v_tok + kvh * a.v_head;
+                const int64_t at = PX ? prefix_key(px, p.seq, kvh, ta * kPtKeys + key) : 0;
+                if (PX && at < 0) continue;
+                const T *kr = static_cast<const T *>(a.k) + (PX ? at : (k0 + key) * a.k_tok + kvh * a.k_head);
+                const T *vr = static_cast<const T *>(a.v) + (PX ? at : (k0 + key) * a.v_tok + kvh * a.v_head);
                 float s = 0.f;
                 for (int d = 0; d < D; ++d) s = fmaf(to_f32<T>(q_row[d]), to_f32<T>(kr[d]), s);
                 const float pr = exp2_approx(fmaf(s, a.sl2, -m_row)) * inv;
@@ -572,7 +590,50 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
         if constexpr (SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         else if constexpr (SL == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (warp == 0 && lane == 0 && nt > 0) {
+        if (PX && warp == 0 && nt > 0) {
+            // ---- TMA, a lane a box of K or V
+            const uint64_t pol = policy_evict_last();
+            if (lane == 0) {
+                mbar_arrive_expect_tx(q_full, (D / 64) * static_cast<uint32_t>(BQ * G) * 128u);
+                for (int b = 0; b < D / 64; ++b)
+                    tma_load_3d(sbase + b * Ge::kBox, &tq, 64 * b, kvh * G, static_cast<int32_t>(p.q0) + t0, smem_addr(q_full), pol);
+            }
+            const int boxes = kPtKeys / px_rows;
+            const int64_t no_block = px.n_blocks;  // reads as zeros
+            const auto block_of = [&](int t, int box) {
+                const int pos = (ta + t) * kPtKeys + box * px_rows;
+                if (t >= nt || box >= boxes || pos >= p.nk) return static_cast<int32_t>(no_block);
+                const int32_t blk = __ldg(px.table + p.seq * px.table_stride + static_cast<uint32_t>(pos) / px.bt);
+                return blk < 0 || blk >= no_block ? static_cast<int32_t>(no_block) : blk;
+            };
+            int issued = 0;
+            const auto tile = [&](const CUtensorMap *map, int t, int32_t block) {
+                const int st = issued % S;
+                if (issued >= S && !__all_sync(0xffffffffu, wait(&empty[st], ((issued / S) - 1) & 1))) return false;
+                if (lane == 0) mbar_arrive_expect_tx(&full[st], Ge::kTile);
+                __syncwarp();
+                for (int box = lane; box < boxes; box += 32) {
+                    const int32_t blk = box == lane ? block : block_of(t, box);
+                    const int32_t in = static_cast<int32_t>(static_cast<uint32_t>((ta + t) * kPtKeys + box * px_rows) % px.bt);
+#pragma unroll
+                    for (int b = 0; b < D / 64; ++b)
+                        tma_load_4d(sbase + Ge::kOffRing + st * Ge::kTile + b * Ge::kBox + box * px_rows * 128, map, 64 * b, kvh, in, blk,
+                                    smem_addr(&full[st]), pol);
+                }
+                ++issued;
+                return true;
+            };
+            int32_t b0 = block_of(0, lane), b1 = block_of(1, lane), b2 = block_of(2, lane);  // of tiles t, t + 1, t + 2
+            bool ok = tile(&tk, 0, b0) && (nt < 2 || tile(&tk, 1, b1));
+            for (int t = 0; t < nt && ok; ++t) {
+                const int32_t b3 = block_of(t + 3, lane);
+                ok = tile(&tv, t, b0) && (t + 2 >= nt || tile(&tk, t + 2, b2));
+                b0 = b1, b1 = b2, b2 = b3;
+            }
+            // copies still landing in this CTA's shared memory
+            wait_poll(q_full, 0, nullptr);
+            for (int i = max(0, issued - S); i < issued; ++i) wait_poll(&full[i % S], (i / S) & 1, nullptr);
+        } else if (!PX && warp == 0 && lane == 0 && nt > 0) {
             // ---- TMA
             const uint64_t pol = policy_evict_last();  // K / V are read again by the other query tiles
             if (!SPLIT) {
@@ -695,6 +756,8 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             commit_if(e, idle);
             wait_poll(idle, 0, nullptr);
         } else if (warp >= 2) {
+            if constexpr (PX)
+                if (prefix_bad(px, p.seq, ta * kPtKeys, min(p.nk, (ta + nt) * kPtKeys), threadIdx.x - 64, 64)) bad_block = 1;
             // ---- V check: rows of the masked tiles that hold Inf or NaN, cleared and noted
             constexpr uint32_t kExp = kBf16 ? 0x7F80u : 0x7C00u;
             for (int t = first_masked; t < nt; ++t) {
@@ -794,14 +857,14 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             if (wide) any_wide = 1;
             named_sync(4, 384);
             ok = ok && !any_wide;  // else the softmax threads do the rows over
-            if (ok && sp.parts > 1 && live) sp.part_ml[part_row] = make_float2(M, L);
+            if (ok && !whole_out && live) part_ml[part_row] = make_float2(M, L);
             if (ok) {
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
                     float x[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) x[j] = acc[32 * c + j] * inv * undo * undo;
-                    if (sp.parts == 1) {  // over Q: every product with it is complete
+                    if (whole_out) {  // over Q: every product with it is complete
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
                             *reinterpret_cast<float4 *>(staged(base, 8 * c + j)) =
@@ -809,13 +872,13 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                     } else if (live) {
 #pragma unroll
                         for (int j = 0; j < 32; j += 4)
-                            *reinterpret_cast<float4 *>(sp.part_o + part_row * D + 32 * c + j) =
+                            *reinterpret_cast<float4 *>(part_o + part_row * D + 32 * c + j) =
                                 make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
                     }
                 }
             }
             named_sync(2, 128);
-            if (sp.parts == 1 && ok && some) store_rows(base, t0, r, 128);
+            if (whole_out && ok && some) store_rows(base, t0, r, 128);
         }
     } else if constexpr (SPLIT) {
         // ---- F32 softmax
@@ -932,8 +995,9 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             const int rows = min(BQ, p.nq - t0) * G, from = ta * kPtKeys, to = (ta + nt) * kPtKeys;
             for (int r0 = 0; r0 < rows; r0 += kPkRows) {
                 named_sync(5, kPkThreads);  // the last rows' shared memory is free
-                ffma_rows<float, D>(
-                    a, p, kvh, t0 * G + r0, min(kPkRows, rows - r0), from, to, reinterpret_cast<float *>(base), threadIdx.x - 128,
+                ffma_rows<float, D, true>(
+                    a, p, kvh, t0 * G + r0, min(kPkRows, rows - r0), from, to, PackedKeys<float>(a, p, kvh),
+                    reinterpret_cast<float *>(base), threadIdx.x - 128,
                     [] { named_sync(5, kPkThreads); },
                     [&](int row, int c, const float (&x)[4], float m, float l) {
                         row += r0;
@@ -1105,7 +1169,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                     x[j] *= inv;
                 }
                 if (any_bad && live) add_cleared(x, 32 * (c0 + c), m_row, inv);
-                if (sp.parts == 1) {
+                if (whole_out) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         *staged(stage, 4 * (c0 + c) + j) =
@@ -1114,13 +1178,13 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                 } else if (live) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4 *>(sp.part_o + part_row * D + 32 * (c0 + c) + j) =
+                        *reinterpret_cast<float4 *>(part_o + part_row * D + 32 * (c0 + c) + j) =
                             make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
                 }
             }
         }
-        if (sp.parts > 1) {
-            if (live && slot == 0) sp.part_ml[part_row] = make_float2(m_row, l_row);
+        if (!whole_out) {
+            if (live && slot == 0) part_ml[part_row] = make_float2(m_row, PX && !ok ? -1.f : l_row);  // (-1: not to be used)
         } else if constexpr (!kJoin) {
             named_sync(2 + slot, 128);
             if (ok && some) store_rows(stage, t0 + slot * BQ, r, 128);
@@ -1131,6 +1195,12 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (PX) {
+        if (bad_block) {  // the joining kernel clears the group's rows
+            if (warp >= 4 && slot == 0 && live) part_ml[part_row] = make_float2(0.f, -1.f);
+            if (threadIdx.x == 0) set_status(a.status, B200_DEV_BAD_POSITION);
+        }
+    }
     if (warp == 2) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kColumns) : "memory");
@@ -1224,7 +1294,7 @@ template <typename T, int D, int NT, int SL>
 cudaError_t pt_launch(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) {
     constexpr bool bf16 = __is_same(T, __nv_bfloat16), split = __is_same(T, float);
     using Ge = PtGeometry<D, NT, SL, split ? 2 : 1>;
-    auto kern = packed_tc_kernel<T, D, NT, SL>;
+    auto kern = packed_tc_kernel<T, D, NT, SL, false>;
     cudaError_t e = once_per_device(reinterpret_cast<const void *>(kern), ATTR_SMEM, [&] {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ge::kSmem));
     });
@@ -1263,7 +1333,7 @@ cudaError_t pt_launch(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) 
             return cudaErrorNotSupported;
     }
     e = b200_launch(kern, dim3(static_cast<unsigned>(plan.ctas)), dim3(kPtThreads<T, SL>), Ge::kSmem, st, split, mq, mk, mv, a,
-                    sp);
+                    sp, PrefixArgs(), 0);
     if (e != cudaSuccess || plan.parts == 1) return e;
     return b200_launch(packed_join_kernel<T, D>, dim3(static_cast<unsigned>(plan.ctas / plan.parts * kPtJoinCtas)),
                        dim3(kPtJoinThreads), 0, st, true, a, sp);
@@ -1283,7 +1353,45 @@ cudaError_t pt_by_dim(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) 
     return a.D == 128 ? pt_by_tiles<T, 128>(a, plan, st) : pt_by_tiles<T, 64>(a, plan, st);
 }
 
+template <typename T, int D>
+cudaError_t px_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st) {
+    constexpr bool bf16 = __is_same(T, __nv_bfloat16);
+    using Ge = PtGeometry<D, 1, 2, 1>;
+    auto kern = packed_tc_kernel<T, D, 1, 2, true>;
+    const cudaError_t e = once_per_device(reinterpret_cast<const void *>(kern), ATTR_SMEM, [&] {
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ge::kSmem));
+    });
+    if (e != cudaSuccess) return e;
+    const int BQ = kPtRows / a.G;
+    int rows = 1;  // positions of a box: within a block and a tile
+    while (rows < kPtKeys && p.bt % (2 * rows) == 0) rows *= 2;
+    // a block's positions, heads and elements, and the blocks
+    const auto pool_map = [&](CUtensorMap *m, const void *base) {
+        const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.Hkv), p.bt, static_cast<uint64_t>(p.n_blocks)};
+        const uint64_t strides[3] = {static_cast<uint64_t>(p.head_stride) * 2, static_cast<uint64_t>(p.tok_stride) * 2,
+                                     static_cast<uint64_t>(p.block_stride) * 2};
+        const uint32_t box[4] = {64, 1, static_cast<uint32_t>(rows), 1};
+        return tma_encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, base, 4, dims, strides, box,
+                          CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    CUtensorMap mq, mk, mv;
+    const int64_t ctas = most_packed_tiles(p.n_groups, a.total_q, 1, BQ) * a.Hkv * p.parts;
+    if (ctas > INT32_MAX || !row_map(&mq, bf16, a.q, D, a.Hq, a.total_q, a.q_head, a.q_tok, a.G, BQ) || !pool_map(&mk, a.k) ||
+        !pool_map(&mv, a.v))
+        return cudaErrorNotSupported;
+    SplitView sp;
+    sp.parts = p.parts;
+    return b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPtThreads<T, 2>), Ge::kSmem, st, false, mq, mk, mv, a, sp, p,
+                       rows);
+}
+
 }  // namespace
+
+cudaError_t prefix_tc_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st) {
+    if (a.G > kPtRows || a.dtype == B200_DTYPE_F32) return cudaErrorNotSupported;
+    if (a.dtype == B200_DTYPE_F16) return a.D == 128 ? px_launch<__half, 128>(a, p, st) : px_launch<__half, 64>(a, p, st);
+    return a.D == 128 ? px_launch<__nv_bfloat16, 128>(a, p, st) : px_launch<__nv_bfloat16, 64>(a, p, st);
+}
 
 size_t packed_tc_workspace(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t D, int64_t Hq, int64_t Hkv,
                            int32_t dtype) {

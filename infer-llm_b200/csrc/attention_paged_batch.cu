@@ -35,7 +35,7 @@
 // and, for BF16, the latency of a warp's chain from copy to product. Eight warps an SM issue in 40 % of
 // the cycles.
 // Rows past a sequence's end are not read; they and keys of invalid blocks get weight 0.
-#include "paged_line.cuh"
+#include "paged_batch.cuh"
 
 namespace b200 {
 namespace {
@@ -47,23 +47,6 @@ constexpr int kJoinThreads = 256;
 constexpr int kCluster = 8;
 constexpr int kClusterKeys = 4096;
 
-struct PbArgs {
-    const void *q = nullptr;
-    void *out = nullptr;
-    int64_t q_seq = 0, q_head = 0, o_seq = 0, o_head = 0;  // elements
-    const char *k = nullptr, *v = nullptr;
-    int64_t block_stride = 0, tok_stride = 0, head_stride = 0;  // bytes
-    int64_t n_blocks = 0;
-    const int32_t *table = nullptr, *lens = nullptr;
-    int64_t table_stride = 0;
-    int64_t max_keys = 0;  // positions a table row covers (fits 31 bits)
-    uint32_t bt = 1;
-    int n_seqs = 0, G = 0, VH = 0, HG = 0;  // query heads a KV head; (KV head, head group) pairs; groups a KV head
-    float sl2 = 0.f;                        // scale * log2 e
-    float *ws = nullptr;
-    int32_t *status = nullptr;
-};
-
 template <typename T, int D, int HB>
 struct Geometry {
     static constexpr int kSub = sizeof(T) == 4 ? 8 : 16;      // keys of a warp's sub-tile
@@ -74,6 +57,7 @@ struct Geometry {
     // two CTAs an SM: the merge area of many heads leaves room for two stages
     static constexpr int kStages = HB > 8 || (sizeof(T) == 4 && HB > 2) ? 2 : 3;
     static constexpr int kRec = HB * (D + 2);                 // floats of a partial: o, m, l
+    static constexpr int kRecAt = (kRec + 3) / 4 * 4;         // with prefixes, whose join reads 16 bytes at once: from record to record
     static constexpr int kQPad = D / 4 + 4;                   // F32: a quarter of a query row, padded
     static constexpr size_t kRing = static_cast<size_t>(kPbWarps) * kStages * 2 * kHalf;
     static constexpr size_t kMerge = static_cast<size_t>(kPbWarps) * kRec * 4;
@@ -314,18 +298,14 @@ struct WarpState<float, D, HB> {
 // one F32 number. As two terms it is no factor for an infinite V: the second is often 0 or
 // negative, and inf - inf or 0 inf is not P inf. Only for 16-bit outputs that are no numbers.
 // smem: WARPS * (D + 2) floats.
-template <typename T, int D, int WARPS>
-__device__ __noinline__ void output_again(const PbArgs &a, int b, int head, int c0, int c1, float *smem) {
+template <typename T, int D, int WARPS, bool PX>
+__device__ __noinline__ void output_again(const PbArgs &a, const PrefixArgs &px, int b, int head, int c0, int c1, float *smem) {
     constexpr int E = D / 32;  // columns lane * E ... of a lane
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, len = seq_len(a, b);
     const T *q = static_cast<const T *>(a.q) + b * a.q_seq + head * a.q_head + lane * E;
     float qx[E], o[E] = {}, m = -INFINITY, l = 0.f;
     for (int e = 0; e < E; ++e) qx[e] = to_f32<T>(q[e]);
-    for (int64_t key = warp; key < len; key += WARPS) {
-        const uint32_t k32 = static_cast<uint32_t>(key), slot = k32 / a.bt;
-        const int32_t blk = __ldg(a.table + b * a.table_stride + slot);
-        if (blk < 0 || blk >= a.n_blocks) continue;
-        const int64_t off = blk * a.block_stride + static_cast<int64_t>(k32 - slot * a.bt) * a.tok_stride + (head / a.G) * a.head_stride;
+    const auto see = [&](int64_t off) {  // of the pool's bytes
         const T *k = reinterpret_cast<const T *>(a.k + off) + lane * E, *v = reinterpret_cast<const T *>(a.v + off) + lane * E;
         float s = 0.f;
         for (int e = 0; e < E; ++e) s = fmaf(qx[e], to_f32<T>(k[e]), s);
@@ -339,6 +319,19 @@ __device__ __noinline__ void output_again(const PbArgs &a, int b, int head, int 
         const float p = exp2_approx(s - (m == -INFINITY ? 0.f : m));
         l += p;
         for (int e = 0; e < E; ++e) o[e] = fmaf(p, to_f32<T>(v[e]), o[e]);
+    };
+    if constexpr (PX) {
+        const int group = prefix_group(px, b), n = group < 0 ? 0 : prefix_len(px, group);
+        for (int key = warp; key < n; key += WARPS) {
+            const int64_t off = prefix_key(px, group, head / a.G, key);
+            if (off >= 0) see(off * static_cast<int64_t>(sizeof(T)));
+        }
+    }
+    for (int64_t key = warp; key < len; key += WARPS) {
+        const uint32_t k32 = static_cast<uint32_t>(key), slot = k32 / a.bt;
+        const int32_t blk = __ldg(a.table + b * a.table_stride + slot);
+        if (blk < 0 || blk >= a.n_blocks) continue;
+        see(blk * a.block_stride + static_cast<int64_t>(k32 - slot * a.bt) * a.tok_stride + (head / a.G) * a.head_stride);
     }
     for (int e = 0; e < E; ++e) smem[warp * (D + 2) + lane * E + e] = o[e];
     if (lane == 0) smem[warp * (D + 2) + D] = m, smem[warp * (D + 2) + D + 1] = l;
@@ -356,9 +349,57 @@ __device__ __noinline__ void output_again(const PbArgs &a, int b, int head, int 
     __syncthreads();  // smem is free again
 }
 
-// CL: a cluster of kCluster CTAs takes one pair, and writes its output.
-template <typename T, int D, int HB, bool CL>
-__global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid_constant__ PbArgs a) {
+// Partial outputs of one query head joined, four columns of them.
+struct Joined {
+    float m = -INFINITY, l = 0.f, o[4] = {};
+    bool void_prefix = false;
+    // a part's maximum and sum, its columns, and what they are to be multiplied by (1, or the sum of normalised ones)
+    B200_DEVICE void add(float pm, float pl, const float4 &x, float by) {
+        const float M = fmaxf(m, pm), ms = M == -INFINITY ? 0.f : M;
+        const float f = exp2_approx(m - ms), g = exp2_approx(pm - ms);
+        m = M;
+        l = fmaf(l, f, g * pl);
+        const float w = by == 0.f ? 0.f : g * by;  // (a part without keys holds nothing)
+        o[0] = fmaf(o[0], f, w == 0.f ? 0.f : w * x.x), o[1] = fmaf(o[1], f, w == 0.f ? 0.f : w * x.y);
+        o[2] = fmaf(o[2], f, w == 0.f ? 0.f : w * x.z), o[3] = fmaf(o[3], f, w == 0.f ? 0.f : w * x.w);
+    }
+};
+
+// Adds the parts of the prefix of row b, query head h, columns c .. c + 3.
+template <int D>
+B200_DEVICE void join_prefix(const PrefixArgs &px, int b, int h, int c, Joined &j) {
+    constexpr int kAtOnce = 4;
+    for (int i0 = 0; i0 < px.parts; i0 += kAtOnce) {
+        float2 ml[kAtOnce];
+        float4 x[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int64_t row = prefix_row(px, min(i0 + i, px.parts - 1), b, h);
+            ml[i] = __ldcg(px.ml + row);
+            x[i] = __ldcg(reinterpret_cast<const float4 *>(px.o + row * D + c));
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (i0 + i >= px.parts) break;
+            j.void_prefix |= ml[i].y < 0.f;
+            j.add(ml[i].x, ml[i].y, x[i], ml[i].y);
+        }
+    }
+}
+
+// Reports offsets and lengths of the groups that are out of range. One CTA.
+B200_DEVICE void report_groups(const PrefixArgs &px, int32_t *status) {
+    for (int g = threadIdx.x; g < px.n_groups; g += blockDim.x) {
+        int64_t first;
+        int n;
+        const int64_t len = __ldg(px.lens + g);
+        if (!packed_range(px.cu, g, px.n_seqs, first, n) || len < 0 || len > px.max_keys) set_status(status, B200_DEV_BAD_POSITION);
+    }
+}
+
+// CL: a cluster of kCluster CTAs takes one pair, and writes its output. PX: there are prefixes to join.
+template <typename T, int D, int HB, bool CL, bool PX>
+__global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid_constant__ PbArgs a, const __grid_constant__ PrefixArgs px) {
     using Ge = Geometry<T, D, HB>;
     extern __shared__ __align__(128) unsigned char pb_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -388,7 +429,10 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
         grid_launch_dependents();  // the joining kernel waits for this grid's end
         const int64_t total = tiles_before<Ge::kTile>(a, a.n_seqs) * a.VH;
         const int64_t ctas = min64(gridDim.x, total);
-        if (blockIdx.x >= ctas) return;
+        if (blockIdx.x >= ctas) {
+            if (PX) grid_wait();
+            return;
+        }
         u0 = share_begin(total, blockIdx.x, ctas);
         u1 = share_begin(total, blockIdx.x + 1, ctas);
         at = place_at<Ge::kTile>(a, u0, u1);
@@ -472,7 +516,8 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
             const bool whole = !CL && pair_end && part_t0 == 0;
             // parts: slot 0 begins with the CTA's share, slot 1 with a pair
             const int slot = part_t0 == 0 && at.left - 1 + (at.t + 1) != u1 - u0 ? 1 : 0;
-            float *rec = CL ? own : a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * Ge::kRec;
+            float *rec = CL ? own : a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * (PX ? Ge::kRecAt : Ge::kRec);
+            if (PX && whole) rec = a.whole + (static_cast<int64_t>(at.b) * a.VH + at.vh) * Ge::kRecAt;
             for (int i = threadIdx.x; i < heads * D; i += kPbThreads) {
                 const int g = i / D;
                 float M = -INFINITY;
@@ -486,7 +531,7 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
                     ls = fmaf(f, merge[w * Ge::kRec + HB * D + HB + g], ls);
                     os = fmaf(f, merge[w * Ge::kRec + i], os);
                 }
-                if (whole) {
+                if (!PX && whole) {
                     static_cast<T *>(a.out)[at.b * a.o_seq + (h0 + g) * a.o_head + (i - g * D)] =
                         from_f32<T>(ls > 0.f || ls != ls ? os / ls : 0.f);
                 } else {
@@ -503,8 +548,14 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
     }
     cp_async_wait<0>();
     if (bad) set_status(a.status, B200_DEV_BAD_POSITION);
+    if constexpr (PX) grid_wait();  // the prefixes' parts are written (and this grid ends after theirs)
     if constexpr (CL) {
         cluster_sync();  // every CTA's record is written
+        int group = -1;
+        if constexpr (PX) {
+            group = prefix_group(px, start.b);
+            if (blockIdx.x == 0) report_groups(px, a.status);
+        }
         const int rank = blockIdx.x % kCluster;
         const int h0 = (start.vh / a.HG) * a.G + (start.vh % a.HG) * HB, heads = min(HB, a.G - (start.vh % a.HG) * HB);
         const int n = heads * D, i0 = n * rank / kCluster, i1 = n * (rank + 1) / kCluster;
@@ -528,14 +579,28 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
                 ls = fmaf(f, l[c], ls);
                 os = fmaf(f, o[c], os);
             }
-            const float x = ls != 0.f ? os / ls : 0.f;
+            bool empty = false;
+            if constexpr (PX) {
+                if (group >= 0) {
+                    Joined j;
+                    j.add(M, ls, make_float4(os, 0.f, 0.f, 0.f), 1.f);
+                    for (int p = 0; p < px.parts; ++p) {
+                        const int64_t row = prefix_row(px, p, start.b, h0 + g);
+                        const float2 ml = __ldcg(px.ml + row);
+                        empty |= ml.y < 0.f;
+                        j.add(ml.x, ml.y, make_float4(__ldcg(px.o + row * D + (i - g * D)), 0.f, 0.f, 0.f), ml.y);
+                    }
+                    ls = j.l, os = j.o[0];
+                }
+            }
+            const float x = ls != 0.f && !empty ? os / ls : 0.f;
             odd |= !(fabsf(x) < INFINITY);
             static_cast<T *>(a.out)[start.b * a.o_seq + (h0 + g) * a.o_head + (i - g * D)] = from_f32<T>(x);
         }
         if constexpr (sizeof(T) == 2) {
             if (__syncthreads_or(odd))
                 for (int g = i0 / D; g * D < i1; ++g)
-                    output_again<T, D, kPbWarps>(a, start.b, h0 + g, max(0, i0 - g * D), min(D, i1 - g * D), merge);
+                    output_again<T, D, kPbWarps, PX>(a, px, start.b, h0 + g, max(0, i0 - g * D), min(D, i1 - g * D), merge);
         }
         cluster_sync();  // no CTA's shared memory goes away while it is read
     }
@@ -569,7 +634,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_batch_join_kernel(const __
     const auto again = [&](bool odd) {
         if constexpr (sizeof(T) == 2) {
             if (__syncthreads_or(odd))
-                for (int g = 0; g < heads; ++g) output_again<T, D, kJoinThreads / 32>(a, b, h0 + g, 0, D, factor);
+                for (int g = 0; g < heads; ++g) output_again<T, D, kJoinThreads / 32, false>(a, PrefixArgs(), b, h0 + g, 0, D, factor);
         }
     };
     if (parts == 1) {  // whole: written by its CTA
@@ -620,6 +685,61 @@ __global__ void __launch_bounds__(kJoinThreads) paged_batch_join_kernel(const __
     again(odd);
 }
 
+// With prefixes: the parts of each pair's own keys, or its one record, and the parts of its prefix. One CTA a pair, a thread four columns
+// at a time.
+template <typename T, int D, int HB>
+__global__ void __launch_bounds__(kJoinThreads) paged_batch_prefix_join_kernel(const __grid_constant__ PbArgs a,
+                                                                               const __grid_constant__ PrefixArgs px, const int64_t grid) {
+    using Ge = Geometry<T, D, HB>;
+    __shared__ float again[(kJoinThreads / 32) * (D + 2)];
+    const int b = static_cast<int>(blockIdx.x / a.VH), vh = static_cast<int>(blockIdx.x % a.VH);
+    const int64_t before = tiles_before<Ge::kTile>(a, b);
+    const int64_t total = tiles_before<Ge::kTile>(a, a.n_seqs) * a.VH;
+    const int64_t ctas = min64(grid, total);  // as in the main kernel
+    const int tiles = seq_tiles<Ge::kTile>(a, b), group = prefix_group(px, b);
+    const int h0 = (vh / a.HG) * a.G + (vh % a.HG) * HB;
+    const int heads = min(HB, a.G - (vh % a.HG) * HB);
+    T *out = static_cast<T *>(a.out) + b * a.o_seq + h0 * a.o_head;
+    if (threadIdx.x == 0 && vh == 0) report_length(a, b);
+    if (blockIdx.x == 0) report_groups(px, a.status);
+    int64_t c0 = 0;
+    int parts = 0, slot0 = 0;  // CTAs c0 .. c0 + parts - 1 hold parts; only the first's may be a second part
+    if (tiles > 0) {
+        const int64_t ua = before * a.VH + static_cast<int64_t>(vh) * tiles;
+        c0 = share_owner(total, ua, ctas);
+        parts = static_cast<int>(share_owner(total, ua + tiles - 1, ctas) - c0) + 1;
+        slot0 = share_begin(total, c0, ctas) >= ua ? 0 : 1;
+    }
+    grid_wait();
+    const float *first = parts == 1 ? a.whole + static_cast<int64_t>(blockIdx.x) * Ge::kRecAt : a.ws + (c0 * 2 + slot0) * Ge::kRecAt;
+    const auto part = [&](int i) { return i == 0 ? first : a.ws + (c0 + i) * 2 * Ge::kRecAt; };
+    bool odd = false;
+    for (int i = 4 * threadIdx.x; i < heads * D; i += 4 * kJoinThreads) {
+        const int g = i / D;
+        Joined j;
+        for (int p = 0; p < parts; ++p) {
+            const float *rec = part(p);
+            j.add(__ldcg(rec + HB * D + g), __ldcg(rec + HB * D + HB + g), __ldcg(reinterpret_cast<const float4 *>(rec + i)), 1.f);
+        }
+        if (group >= 0) join_prefix<D>(px, b, h0 + g, i - g * D, j);
+        const float inv = j.l != 0.f && !j.void_prefix ? 1.0f / j.l : 0.f;
+        T x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float y = inv != 0.f ? j.o[e] * inv : 0.f;
+            odd |= !(fabsf(y) < INFINITY);
+            x[e] = from_f32<T>(y);
+        }
+        T *to = out + g * a.o_head + (i - g * D);
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(to) = *reinterpret_cast<const float4 *>(x);
+        else *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(x);
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (__syncthreads_or(odd))
+            for (int g = 0; g < heads; ++g) output_again<T, D, kJoinThreads / 32, true>(a, px, b, h0 + g, 0, D, again);
+    }
+}
+
 int pb_max_ctas() { return device_sm_count() * 2 < kPbMostCtas ? device_sm_count() * 2 : kPbMostCtas; }
 
 // Few pairs with short tables: a cluster each, no workspace.
@@ -634,8 +754,8 @@ int pb_heads(int64_t G, bool f32) {
     return G <= 1 ? 1 : (G <= 2 ? 2 : (G <= 4 ? 4 : 8));
 }
 
-template <typename T, int D, int HB>
-cudaError_t pb_launch(PbArgs a, int64_t Hkv, cudaStream_t st) {
+template <typename T, int D, int HB, bool PX>
+cudaError_t pb_launch(PbArgs a, const PrefixArgs &px, int64_t Hkv, cudaStream_t st) {
     using Ge = Geometry<T, D, HB>;
     a.HG = (a.G + HB - 1) / HB;
     a.VH = static_cast<int>(Hkv) * a.HG;
@@ -647,7 +767,7 @@ cudaError_t pb_launch(PbArgs a, int64_t Hkv, cudaStream_t st) {
         });
     };
     if (pb_one_launch(pairs, a.max_keys)) {
-        auto kern = paged_batch_kernel<T, D, HB, true>;
+        auto kern = paged_batch_kernel<T, D, HB, true, PX>;
         const cudaError_t e = allow(reinterpret_cast<const void *>(kern), Ge::kSmem);
         if (e != cudaSuccess) return e;
         cudaLaunchConfig_t cfg = {};
@@ -655,47 +775,90 @@ cudaError_t pb_launch(PbArgs a, int64_t Hkv, cudaStream_t st) {
         cfg.blockDim = dim3(kPbThreads);
         cfg.dynamicSmemBytes = Ge::kSmem;
         cfg.stream = st;
-        cudaLaunchAttribute attr[1];
+        cudaLaunchAttribute attr[2];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = kCluster;
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        return cudaLaunchKernelEx(&cfg, kern, a);
+        cfg.numAttrs = PX && px.parts > 0 ? 2 : 1;
+        return cudaLaunchKernelEx(&cfg, kern, a, px);
     }
-    auto kern = paged_batch_kernel<T, D, HB, false>;
+    auto kern = paged_batch_kernel<T, D, HB, false, PX>;
     cudaError_t e = allow(reinterpret_cast<const void *>(kern), Ge::kSmem);
     if (e != cudaSuccess) return e;
     const int64_t most = (a.max_keys + Ge::kTile - 1) / Ge::kTile;  // tiles of the longest possible sequence
     const int64_t ctas = min64(pb_max_ctas(), most > pb_max_ctas() ? pb_max_ctas() : pairs * most);
-    e = b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPbThreads), Ge::kSmem, st, false, a);
+    e = b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPbThreads), Ge::kSmem, st, PX && px.parts > 0, a, px);
     if (e != cudaSuccess) return e;
-    return b200_launch(paged_batch_join_kernel<T, D, HB>, dim3(static_cast<unsigned>(pairs)), dim3(kJoinThreads), 0, st, true,
-                       a, ctas);
+    if constexpr (PX)
+        return b200_launch(paged_batch_prefix_join_kernel<T, D, HB>, dim3(static_cast<unsigned>(pairs)), dim3(kJoinThreads), 0, st, true,
+                           a, px, ctas);
+    else
+        return b200_launch(paged_batch_join_kernel<T, D, HB>, dim3(static_cast<unsigned>(pairs)), dim3(kJoinThreads), 0, st, true,
+                           a, ctas);
 }
 
-template <typename T, int D>
-cudaError_t pb_by_heads(const PbArgs &a, int64_t Hkv, cudaStream_t st) {
+template <typename T, int D, bool PX>
+cudaError_t pb_by_heads(const PbArgs &a, const PrefixArgs &px, int64_t Hkv, cudaStream_t st) {
     const int hb = pb_heads(a.G, sizeof(T) == 4);
     if constexpr (sizeof(T) == 4) {
         switch (hb) {
-            case 1: return pb_launch<T, D, 1>(a, Hkv, st);
-            case 2: return pb_launch<T, D, 2>(a, Hkv, st);
-            case 4: return pb_launch<T, D, 4>(a, Hkv, st);
+            case 1: return pb_launch<T, D, 1, PX>(a, px, Hkv, st);
+            case 2: return pb_launch<T, D, 2, PX>(a, px, Hkv, st);
+            case 4: return pb_launch<T, D, 4, PX>(a, px, Hkv, st);
         }
-        return pb_launch<T, D, 8>(a, Hkv, st);
+        return pb_launch<T, D, 8, PX>(a, px, Hkv, st);
     } else {
-        return hb == 8 ? pb_launch<T, D, 8>(a, Hkv, st) : pb_launch<T, D, 16>(a, Hkv, st);
+        return hb == 8 ? pb_launch<T, D, 8, PX>(a, px, Hkv, st) : pb_launch<T, D, 16, PX>(a, px, Hkv, st);
     }
 }
 
-template <typename T>
-cudaError_t pb_by_dim(const PbArgs &a, int64_t Hkv, int64_t D, cudaStream_t st) {
-    return D == 128 ? pb_by_heads<T, 128>(a, Hkv, st) : pb_by_heads<T, 64>(a, Hkv, st);
+template <typename T, bool PX>
+cudaError_t pb_by_dim(const PbArgs &a, const PrefixArgs &px, int64_t Hkv, int64_t D, cudaStream_t st) {
+    return D == 128 ? pb_by_heads<T, 128, PX>(a, px, Hkv, st) : pb_by_heads<T, 64, PX>(a, px, Hkv, st);
+}
+
+template <bool PX>
+cudaError_t pb_by_type(const PbArgs &a, const PrefixArgs &px, int64_t Hkv, int64_t D, int32_t dtype, cudaStream_t st) {
+    switch (dtype) {
+        case B200_DTYPE_F16: return pb_by_dim<__half, PX>(a, px, Hkv, D, st);
+        case B200_DTYPE_BF16: return pb_by_dim<__nv_bfloat16, PX>(a, px, Hkv, D, st);
+    }
+    return pb_by_dim<float, PX>(a, px, Hkv, D, st);
+}
+
+// Bytes of the CTAs' records, and of the pairs' (with prefixes), 0 in one launch.
+struct PbBytes {
+    size_t ctas = 0, pairs = 0;
+};
+PbBytes pb_bytes(int64_t n_seqs, int64_t max_keys, int64_t D, int64_t G, int64_t Hkv, int32_t dtype) {
+    const int hb = pb_heads(G, dtype == B200_DTYPE_F32);
+    const int64_t pairs = n_seqs * Hkv * ((G + hb - 1) / hb);
+    PbBytes n;
+    if (pb_one_launch(pairs, max_keys)) return n;
+    const size_t rec = static_cast<size_t>(hb * (D + 2) + 3) / 4 * 16;
+    n.ctas = pb_max_ctas() * 2 * rec;  // two partial records a CTA (its share's first and last part)
+    n.pairs = pairs * rec;
+    return n;
 }
 
 }  // namespace
+
+size_t paged_batch_prefix_bytes(int64_t n_seqs, int64_t max_keys, int64_t D, int64_t G, int64_t Hkv, int32_t dtype) {
+    const PbBytes n = pb_bytes(n_seqs, max_keys, D, G, Hkv, dtype);
+    return n.ctas + n.pairs;
+}
+
+cudaError_t paged_batch_prefix_launch(PbArgs a, const PrefixArgs &px, int64_t Hkv, int64_t D, int32_t dtype, void *workspace, cudaStream_t st) {
+    const PbBytes n = pb_bytes(a.n_seqs, a.max_keys, D, a.G, Hkv, dtype);
+    a.ws = static_cast<float *>(workspace);
+    a.whole = reinterpret_cast<float *>(static_cast<char *>(workspace) + n.ctas);
+    return pb_by_type<true>(a, px, Hkv, D, dtype, st);
+}
+
 }  // namespace b200
 
 using namespace b200;
@@ -705,11 +868,7 @@ extern "C" {
 size_t b200_flash_attn_paged_batch_workspace_bytes(int64_t n_seqs, int64_t max_keys, int64_t D, int64_t Hq, int64_t Hkv,
                                                    int32_t dtype) {
     if (n_seqs <= 0 || max_keys <= 0 || D <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || !dtype_bytes(dtype)) return 0;
-    const int64_t G = Hq / Hkv;
-    const int hb = pb_heads(G, dtype == B200_DTYPE_F32);
-    if (pb_one_launch(n_seqs * Hkv * ((G + hb - 1) / hb), max_keys)) return 0;
-    // two partial records a CTA (its share's first and last part)
-    return static_cast<size_t>(pb_max_ctas()) * 2 * hb * (D + 2) * 4;
+    return pb_bytes(n_seqs, max_keys, D, Hq / Hkv, Hkv, dtype).ctas;
 }
 
 int b200_flash_attn_paged_batch(const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
@@ -758,12 +917,7 @@ int b200_flash_attn_paged_batch(const void *q, int64_t q_seq_stride, int64_t q_h
     a.sl2 = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(D))) * kLog2e;
     a.ws = static_cast<float *>(workspace);
     a.status = dev_status;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    switch (pool->dtype) {
-        case B200_DTYPE_F16: return status_of(pb_by_dim<__half>(a, Hkv, D, st));
-        case B200_DTYPE_BF16: return status_of(pb_by_dim<__nv_bfloat16>(a, Hkv, D, st));
-    }
-    return status_of(pb_by_dim<float>(a, Hkv, D, st));
+    return status_of(pb_by_type<false>(a, PrefixArgs(), Hkv, D, pool->dtype, static_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

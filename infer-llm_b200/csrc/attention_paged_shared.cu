@@ -1,82 +1,92 @@
 // b200_flash_attn_paged_shared: one query token for each of many sequences that share prefixes, against a paged K/V cache.
 //
-// out_b = softmax over the keys of the prefix of b's group and b's own keys, of the one pool.
-#include "attention_rows.cuh"
-#include "paged_line.cuh"
+// out_b = softmax over the keys of the prefix of b's group and b's own keys, of the one pool. Three kernels, each of which may start
+// while the one before ends:
+//  * the prefixes: the rows of a group (its sequences times the query heads of a KV head) against its prefix in tiles, so that each key
+//    is read once for up to 128 rows. 16-bit types: the packed attention's tensor-core kernel (attention_packed_tc.cu), whose K and V tiles
+//    are copied block by block. F32, more than 128 query heads a KV head, or strides that a tensor map cannot hold: F32 FFMA
+//    (prefix_ffma_kernel). A prefix is cut into as many parts as fill the SMs.
+//  * the sequences' own keys, as in the batched decode (attention_paged_batch.cu);
+//  * the join of all parts.
+#include "attention_packed_ffma.cuh"
+#include "paged_batch.cuh"
 
 namespace b200 {
 namespace {
 
-struct SharedArgs {
-    const void *q = nullptr;
-    void *out = nullptr;
-    int64_t q_seq = 0, q_head = 0, o_seq = 0, o_head = 0;  // elements
-    const char *k = nullptr, *v = nullptr;
-    int64_t block_stride = 0, tok_stride = 0, head_stride = 0;  // elements
-    int64_t n_blocks = 0;
-    const int32_t *table = nullptr, *lens = nullptr, *prefix_table = nullptr, *prefix_lens = nullptr, *cu = nullptr;
-    int64_t table_stride = 0, prefix_stride = 0;
-    int64_t max_keys = 0, max_prefix = 0;  // positions a table row covers (fits 31 bits)
-    uint32_t bt = 1;
-    int n_seqs = 0, n_groups = 0, G = 0, Hkv = 0;
-    float sl2 = 0.f;  // scale * log2 e
-    int32_t *status = nullptr;
-};
+// A CTA: 64 rows of a group and KV head against a part of the prefix's keys.
+template <typename T, int D>
+__global__ void __launch_bounds__(kPkThreads, 2) prefix_ffma_kernel(const PackedArgs a, const PrefixArgs px) {
+    extern __shared__ __align__(16) float pf_smem[];
+    grid_launch_dependents();
+    const int part = blockIdx.x % px.parts, kvh = blockIdx.x / px.parts % a.Hkv;
+    const PackedTile p = find_prefix_tile(px, a.G, kPkRows, blockIdx.x / (px.parts * a.Hkv));
+    if (p.seq < 0) return;
+    const int r0 = p.tile * kPkRows, rows = min(kPkRows, p.nq * a.G - r0);
+    const int64_t tiles = (static_cast<int64_t>(p.nk) + kPkKeys - 1) / kPkKeys;
+    const int first = static_cast<int>(tiles * part / px.parts) * kPkKeys;
+    const int end = static_cast<int>(min64(p.nk, tiles * (part + 1) / px.parts * kPkKeys));
+    const auto row_of = [&](int r) { return prefix_row(px, part, p.q0 + (r0 + r) / a.G, kvh * a.G + (r0 + r) % a.G); };
+    if (__syncthreads_or(prefix_bad(px, p.seq, first, end, threadIdx.x, kPkThreads))) {
+        if (threadIdx.x == 0) set_status(a.status, B200_DEV_BAD_POSITION);
+        if (threadIdx.x < rows) px.ml[row_of(threadIdx.x)] = make_float2(0.f, -1.f);  // the joining kernel clears the group's rows
+        return;
+    }
+    const T *k0 = static_cast<const T *>(a.k), *v0 = static_cast<const T *>(a.v);
+    ffma_rows<T, D, false>(
+        a, p, kvh, r0, rows, first, end,
+        [&](int j, const T *&k, const T *&v) {
+            const int64_t at = prefix_key(px, p.seq, kvh, j);
+            k = k0 + at, v = v0 + at;
+            return at >= 0;
+        },
+        pf_smem, threadIdx.x, [] { __syncthreads(); },
+        [&](int r, int c, const float (&x)[4], float m, float l) {
+            const int64_t row = row_of(r);
+            *reinterpret_cast<float4 *>(px.o + row * D + c) = make_float4(x[0], x[1], x[2], x[3]);
+            if (c == 0) px.ml[row] = make_float2(m, l);
+        });
+}
+
+int64_t prefix_tiles(int64_t n_seqs, int64_t n_groups, int64_t G, int64_t Hkv, bool tc) {
+    return (tc ? most_packed_tiles(n_groups, n_seqs, 1, kPrefixTcRows / G) : most_packed_tiles(n_groups, n_seqs, G, kPkRows)) * Hkv;
+}
+
+// Parts of each prefix's keys: as many as the CTAs that run at once allow, of two key tiles at least.
+int prefix_parts(int64_t n_seqs, int64_t n_groups, int64_t max_prefix, int64_t G, int64_t Hkv, int32_t dtype) {
+    if (n_groups <= 0 || max_prefix <= 0) return 0;
+    const bool tc = dtype != B200_DTYPE_F32 && G <= kPrefixTcRows;
+    const int64_t ctas = device_sm_count() * (tc ? 1 : 2), keys = 2 * (tc ? 128 : kPkKeys);
+    return static_cast<int>(max64(1, min64(min64(32, (max_prefix + keys - 1) / keys), ctas / max64(1, prefix_tiles(n_seqs, n_groups, G, Hkv, tc)))));
+}
+
+size_t prefix_bytes(int64_t n_seqs, int64_t parts, int64_t D, int64_t Hq) {
+    return (static_cast<size_t>(parts) * n_seqs * Hq * (D * 4 + 8) + 15) / 16 * 16;
+}
 
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kArWarps) shared_rows_kernel(const __grid_constant__ SharedArgs a) {
-    constexpr int E = D / 32;
-    const int b = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.Hkv)), h = blockIdx.x % static_cast<unsigned>(a.Hkv);
-    const int64_t len = __ldg(a.lens + b), keys = min64(max64(len, 0), a.max_keys);
-    const int group = a.n_groups ? warp_find_row(a.cu, a.n_groups, b) : -1;
-    const bool in = group >= 0 && __ldg(a.cu + group) >= 0 && __ldg(a.cu + group + 1) <= a.n_seqs;
-    const int64_t plen = in ? __ldg(a.prefix_lens + group) : 0, prefix = min64(max64(plen, 0), a.max_prefix);
-    if ((len != keys || plen != prefix) && threadIdx.x == 0 && h == 0) set_status(a.status, B200_DEV_BAD_POSITION);
-    if (blockIdx.x == 0)
-        for (int g = threadIdx.x; g < a.n_groups; g += blockDim.x) {
-            int64_t f;
-            int n;
-            if (!packed_range(a.cu, g, a.n_seqs, f, n)) set_status(a.status, B200_DEV_BAD_POSITION);
-        }
-    bool bad = false;
-    const auto block_of = [&](const int32_t *table, uint32_t slot) { return static_cast<int64_t>(__ldg(table + slot)); };
-    const int32_t *ptable = a.prefix_table + (in ? group : 0) * a.prefix_stride;
-    for (int64_t s = threadIdx.x; s * a.bt < prefix; s += blockDim.x) {
-        const int64_t blk = block_of(ptable, static_cast<uint32_t>(s));
-        bad |= blk < 0 || blk >= a.n_blocks;
-    }
-    bad = __syncthreads_or(bad);
-    if (bad && threadIdx.x == 0) set_status(a.status, B200_DEV_BAD_POSITION);
-    const T *q = static_cast<const T *>(a.q) + b * a.q_seq + static_cast<int64_t>(h) * a.G * a.q_head;
-    T *out = static_cast<T *>(a.out) + b * a.o_seq + static_cast<int64_t>(h) * a.G * a.o_head;
-    attend_rows<D>(
-        a.G, bad ? 0 : prefix + keys, a.sl2,
-        [&](int64_t j, int lane, float (&k)[E], float (&v)[E]) {
-            const bool own = j >= prefix;
-            const uint32_t pos = static_cast<uint32_t>(own ? j - prefix : j), slot = pos / a.bt;
-            const int64_t blk = block_of(own ? a.table + b * a.table_stride : ptable, slot);
-            if (blk < 0 || blk >= a.n_blocks) {
-                set_status(a.status, B200_DEV_BAD_POSITION);
-                return false;
-            }
-            const int64_t at = blk * a.block_stride + (pos - slot * a.bt) * a.tok_stride + h * a.head_stride + lane * E;
-            for (int e = 0; e < E; ++e) {
-                k[e] = to_f32<T>(reinterpret_cast<const T *>(a.k)[at + e]);
-                v[e] = to_f32<T>(reinterpret_cast<const T *>(a.v)[at + e]);
-            }
-            return true;
-        },
-        [&](int g, int d) { return to_f32<T>(q[g * a.q_head + d]); },
-        [&](int g, int d, float x) { out[g * a.o_head + d] = from_f32<T>(x); });
+cudaError_t prefix_ffma_launch(const PackedArgs &a, const PrefixArgs &px, cudaStream_t st) {
+    auto kern = prefix_ffma_kernel<T, D>;
+    const cudaError_t e = once_per_device(reinterpret_cast<const void *>(kern), ATTR_SMEM, [&] {
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ffma_smem<D>()));
+    });
+    if (e != cudaSuccess) return e;
+    const int64_t ctas = prefix_tiles(px.n_seqs, px.n_groups, a.G, a.Hkv, false) * px.parts;
+    if (ctas > INT32_MAX) return cudaErrorNotSupported;
+    return b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPkThreads), ffma_smem<D>(), st, false, a, px);
 }
 
 template <typename T>
-cudaError_t shared_by_dim(const SharedArgs &a, int64_t D, cudaStream_t st) {
-    const int64_t pairs = static_cast<int64_t>(a.n_seqs) * a.Hkv;
-    if (pairs > INT32_MAX) return cudaErrorNotSupported;
-    if (D == 128) shared_rows_kernel<T, 128><<<static_cast<unsigned>(pairs), 32 * kArWarps, 0, st>>>(a);
-    else shared_rows_kernel<T, 64><<<static_cast<unsigned>(pairs), 32 * kArWarps, 0, st>>>(a);
-    return cudaGetLastError();
+cudaError_t prefix_ffma_by_dim(const PackedArgs &a, const PrefixArgs &px, cudaStream_t st) {
+    return a.D == 128 ? prefix_ffma_launch<T, 128>(a, px, st) : prefix_ffma_launch<T, 64>(a, px, st);
+}
+
+cudaError_t prefix_ffma_by_type(const PackedArgs &a, const PrefixArgs &px, cudaStream_t st) {
+    switch (a.dtype) {
+        case B200_DTYPE_F16: return prefix_ffma_by_dim<__half>(a, px, st);
+        case B200_DTYPE_BF16: return prefix_ffma_by_dim<__nv_bfloat16>(a, px, st);
+    }
+    return prefix_ffma_by_dim<float>(a, px, st);
 }
 
 }  // namespace
@@ -88,7 +98,11 @@ extern "C" {
 
 size_t b200_flash_attn_paged_shared_workspace_bytes(int64_t n_seqs, int64_t max_keys, int64_t n_groups, int64_t max_prefix,
                                                     int64_t D, int64_t Hq, int64_t Hkv, int32_t dtype) {
-    return 0;
+    if (n_seqs <= 0 || max_keys <= 0 || n_groups < 0 || max_prefix < 0 || D <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv ||
+        !dtype_bytes(dtype))
+        return 0;
+    return prefix_bytes(n_seqs, prefix_parts(n_seqs, n_groups, max_prefix, Hq / Hkv, Hkv, dtype), D, Hq) +
+           paged_batch_prefix_bytes(n_seqs, max_keys, D, Hq / Hkv, Hkv, dtype);
 }
 
 int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
@@ -114,13 +128,51 @@ int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_
     const auto positions = [&](int64_t blocks) {
         return blocks > kMostKeys / pool->block_tokens ? kMostKeys : blocks * pool->block_tokens;
     };
-    SharedArgs a;
-    a.max_keys = positions(max_blocks);
-    a.max_prefix = n_groups ? positions(prefix_blocks) : 0;
+    const int64_t max_keys = positions(max_blocks), max_prefix = n_groups ? positions(prefix_blocks) : 0;
     const size_t need =
-        b200_flash_attn_paged_shared_workspace_bytes(n_seqs, a.max_keys, n_groups, a.max_prefix, D, Hq, Hkv, pool->dtype);
+        b200_flash_attn_paged_shared_workspace_bytes(n_seqs, max_keys, n_groups, max_prefix, D, Hq, Hkv, pool->dtype);
     if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < need))
         return B200_ERR_INVALID_ARGUMENT;
+    const float sl2 = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(D))) * kLog2e;
+    PrefixArgs px;
+    px.cu = cu_seqs;
+    px.lens = prefix_lens;
+    px.table = prefix_table;
+    px.table_stride = prefix_stride;
+    px.max_keys = max_prefix;
+    px.n_blocks = pool->n_blocks;
+    px.block_stride = pool->block_stride;
+    px.tok_stride = pool->tok_stride;
+    px.head_stride = pool->head_stride;
+    px.bt = static_cast<uint32_t>(pool->block_tokens);
+    px.n_groups = static_cast<int32_t>(n_groups);
+    px.n_seqs = static_cast<int32_t>(n_seqs);
+    px.Hq = static_cast<int32_t>(Hq);
+    px.parts = prefix_parts(n_seqs, n_groups, max_prefix, Hq / Hkv, Hkv, pool->dtype);
+    px.o = static_cast<float *>(workspace);
+    px.ml = reinterpret_cast<float2 *>(px.o + px.parts * n_seqs * Hq * D);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (px.parts > 0) {
+        PackedArgs p;
+        p.q = q;
+        p.k = pool->k;
+        p.v = pool->v;
+        p.q_tok = q_seq_stride;
+        p.q_head = q_head_stride;
+        p.total_q = n_seqs;
+        p.n_seqs = px.n_groups;
+        p.Hq = px.Hq;
+        p.Hkv = static_cast<int>(Hkv);
+        p.G = static_cast<int>(Hq / Hkv);
+        p.D = static_cast<int>(D);
+        p.sl2 = sl2;
+        p.dtype = pool->dtype;
+        p.status = dev_status;
+        cudaError_t rc2 = prefix_tc_launch(p, px, st);
+        if (rc2 == cudaErrorNotSupported) rc2 = prefix_ffma_by_type(p, px, st);
+        if (rc2 != cudaSuccess) return status_of(rc2);
+    }
+    PbArgs a;
     a.q = q;
     a.out = out;
     a.q_seq = q_seq_stride;
@@ -129,30 +181,21 @@ int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_
     a.o_head = out_head_stride;
     a.k = static_cast<const char *>(pool->k);
     a.v = static_cast<const char *>(pool->v);
-    a.block_stride = pool->block_stride;
-    a.tok_stride = pool->tok_stride;
-    a.head_stride = pool->head_stride;
+    a.block_stride = pool->block_stride * e;
+    a.tok_stride = pool->tok_stride * e;
+    a.head_stride = pool->head_stride * e;
     a.n_blocks = pool->n_blocks;
     a.table = block_table;
     a.lens = seq_lens;
-    a.prefix_table = prefix_table;
-    a.prefix_lens = prefix_lens;
-    a.cu = cu_seqs;
     a.table_stride = table_stride;
-    a.prefix_stride = prefix_stride;
     a.bt = static_cast<uint32_t>(pool->block_tokens);
+    a.max_keys = max_keys;
     a.n_seqs = static_cast<int>(n_seqs);
-    a.n_groups = static_cast<int>(n_groups);
     a.G = static_cast<int>(Hq / Hkv);
-    a.Hkv = static_cast<int>(Hkv);
-    a.sl2 = (scale > 0.f ? scale : 1.0f / sqrtf(static_cast<float>(D))) * kLog2e;
+    a.sl2 = sl2;
     a.status = dev_status;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    switch (pool->dtype) {
-        case B200_DTYPE_F16: return status_of(shared_by_dim<__half>(a, D, st));
-        case B200_DTYPE_BF16: return status_of(shared_by_dim<__nv_bfloat16>(a, D, st));
-    }
-    return status_of(shared_by_dim<float>(a, D, st));
+    return status_of(paged_batch_prefix_launch(a, px, Hkv, D, pool->dtype,
+                                               static_cast<char *>(workspace) + prefix_bytes(n_seqs, px.parts, D, Hq), st));
 }
 
 }  // extern "C"

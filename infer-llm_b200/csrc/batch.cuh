@@ -80,9 +80,10 @@ B200_DEVICE bool packed_range(const int32_t *cu, int s, int64_t total, int64_t &
 }
 
 // Tile `at` of the line of all tiles (a sequence's last tiles, which see the most keys,
-// first), found by a whole warp; each lane takes every 32nd sequence.
-B200_DEVICE PackedTile find_packed_tile(const int32_t *cu_q, const int32_t *cu_k, int n_seqs, int64_t total_q,
-                                        int64_t total_k, int G, int M, int64_t at, int32_t *status) {
+// first), found by a whole warp; each lane takes every 32nd sequence. keys(s, k0, nk) gives a sequence's keys, false: out of range.
+template <typename Keys>
+B200_DEVICE PackedTile find_tile(const int32_t *cu_q, int n_seqs, int64_t total_q, int G, int M, int64_t at, int32_t *status,
+                                 Keys keys) {
     const int lane = threadIdx.x & 31;
     PackedTile p;
     int64_t before = 0;
@@ -93,7 +94,7 @@ B200_DEVICE PackedTile find_packed_tile(const int32_t *cu_q, const int32_t *cu_k
         bool ok_k = true;  // (both ranges are read at once: one latency)
         if (s < n_seqs) {
             const bool ok_q = packed_range(cu_q, s, total_q, q0, nq);
-            ok_k = packed_range(cu_k, s, total_k, k0, nk);
+            ok_k = keys(s, k0, nk);
             if (!ok_q) set_status(status, B200_DEV_BAD_POSITION);
         }
         // (rows fit 31 bits, with room for a tile)
@@ -122,6 +123,11 @@ B200_DEVICE PackedTile find_packed_tile(const int32_t *cu_q, const int32_t *cu_k
         before += __shfl_sync(0xffffffffu, incl, 31);
     }
     return p;
+}
+B200_DEVICE PackedTile find_packed_tile(const int32_t *cu_q, const int32_t *cu_k, int n_seqs, int64_t total_q,
+                                        int64_t total_k, int G, int M, int64_t at, int32_t *status) {
+    return find_tile(cu_q, n_seqs, total_q, G, M, at, status,
+                     [&](int s, int64_t &k0, int &nk) { return packed_range(cu_k, s, total_k, k0, nk); });
 }
 
 // At most this many tiles, whatever the lengths are.

@@ -1,0 +1,64 @@
+// Prefixes that groups of sequences share (b200_flash_attn_paged_shared): their kernels leave, for each part of a prefix's keys and each
+// (sequence, query head) of its group, the normalised output of those keys with its maximum (in powers of two) and
+// sum; the kernel of the sequences' own keys joins them.
+#pragma once
+
+#include "attention_packed.cuh"
+
+namespace b200 {
+
+struct PrefixArgs {
+    const int32_t *cu = nullptr, *lens = nullptr, *table = nullptr;  // groups' sequences, lengths, blocks
+    int64_t table_stride = 0, max_keys = 0, n_blocks = 0;            // max_keys: positions a table row covers (fits 31 bits)
+    int64_t block_stride = 0, tok_stride = 0, head_stride = 0;       // of the pool, elements
+    uint32_t bt = 1;
+    int32_t n_groups = 0, n_seqs = 0, Hq = 0, parts = 0;
+    float *o = nullptr;    // [part][sequence][query head][D]
+    float2 *ml = nullptr;  // [part][sequence][query head]: maximum, sum (-1: the group's prefix names a block out of range)
+};
+
+B200_DEVICE int prefix_len(const PrefixArgs &a, int group) {
+    const int64_t n = __ldg(a.lens + group);
+    return static_cast<int>(n < 0 ? 0 : (n > a.max_keys ? a.max_keys : n));
+}
+// The group of sequence b, or -1; by a whole warp.
+B200_DEVICE int prefix_group(const PrefixArgs &a, int b) {
+    const int g = a.n_groups > 0 ? warp_find_row(a.cu, a.n_groups, b) : -1;
+    return g >= 0 && __ldg(a.cu + g) >= 0 && __ldg(a.cu + g + 1) <= a.n_seqs ? g : -1;
+}
+// Where part i's numbers for (sequence b, query head h) are.
+B200_DEVICE int64_t prefix_row(const PrefixArgs &a, int part, int64_t b, int h) {
+    return (static_cast<int64_t>(part) * a.n_seqs + b) * a.Hq + h;
+}
+// Elements from the pool's start to KV head h of a prefix's position; -1: the block is out of range.
+B200_DEVICE int64_t prefix_key(const PrefixArgs &a, int group, int h, int pos) {
+    const uint32_t slot = static_cast<uint32_t>(pos) / a.bt;
+    const int64_t blk = __ldg(a.table + group * a.table_stride + slot);
+    if (blk < 0 || blk >= a.n_blocks) return -1;
+    return blk * a.block_stride + static_cast<int64_t>(static_cast<uint32_t>(pos) - slot * a.bt) * a.tok_stride + h * a.head_stride;
+}
+// Whether one of the blocks of positions [from, to) is out of range, for lane `lane` of `lanes`.
+B200_DEVICE bool prefix_bad(const PrefixArgs &a, int group, int from, int to, int lane, int lanes) {
+    bool bad = false;
+    if (from >= to) return bad;
+    const int64_t last = static_cast<uint32_t>(to - 1) / a.bt;
+    for (int64_t s = static_cast<uint32_t>(from) / a.bt + lane; s <= last; s += lanes) {
+        const int32_t blk = __ldg(a.table + group * a.table_stride + s);
+        bad |= blk < 0 || blk >= a.n_blocks;
+    }
+    return bad;
+}
+// Tile `at` of M rows of the line of all groups' tiles, a row being a sequence with one of G heads; by a whole warp.
+B200_DEVICE PackedTile find_prefix_tile(const PrefixArgs &a, int G, int M, int64_t at) {
+    return find_tile(a.cu, a.n_groups, a.n_seqs, G, M, at, nullptr, [&](int s, int64_t &k0, int &nk) {
+        k0 = 0;
+        nk = prefix_len(a, s);
+        return true;
+    });
+}
+
+// Tensor-core kernel of the prefixes for F16 and BF16; cudaErrorNotSupported (nothing launched) where it does not apply.
+cudaError_t prefix_tc_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st);
+constexpr int kPrefixTcRows = 128;  // of a tile: whole sequences times the heads of a KV head
+
+}  // namespace b200

@@ -28,4 +28,13 @@ B200_DEVICE void tma_load_3d(uint32_t dst, const CUtensorMap *map, int32_t x, in
         : "memory");
 }
 
+B200_DEVICE void tma_load_4d(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z, int32_t w, uint32_t bar,
+                             uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar), "l"(policy)
+        : "memory");
+}
+
 }  // namespace b200
