@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     constexpr int PL = SPLIT ? 2 : 1;
     using Ge = PtGeometry<D, NT, SL, PL>;
     static_assert(SL == 2 || (NT == 1 && !SPLIT), "one slot holds one query tile");
-    static_assert(!PX || (NT == 1 && SL == 2 && !SPLIT), "prefixes: one tile in two slots, 16-bit types");
+    static_assert(!PX || (SL == 2 && !SPLIT), "prefixes: two slots, 16-bit types");
     constexpr bool kPairs = NT == 2 || SL == 1, kJoin = NT == 1 && SL == 2;  // kJoin: the slots halve the key tiles
     constexpr int kColumns = 256 * SL;  // of tensor memory
     constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
@@ -594,9 +594,11 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             // ---- TMA, a lane a box of K or V
             const uint64_t pol = policy_evict_last();
             if (lane == 0) {
-                mbar_arrive_expect_tx(q_full, (D / 64) * static_cast<uint32_t>(BQ * G) * 128u);
-                for (int b = 0; b < D / 64; ++b)
-                    tma_load_3d(sbase + b * Ge::kBox, &tq, 64 * b, kvh * G, static_cast<int32_t>(p.q0) + t0, smem_addr(q_full), pol);
+                mbar_arrive_expect_tx(q_full, NT * (D / 64) * static_cast<uint32_t>(BQ * G) * 128u);
+                for (int x = 0; x < NT; ++x)
+                    for (int b = 0; b < D / 64; ++b)
+                        tma_load_3d(sbase + x * Ge::kTile + b * Ge::kBox, &tq, 64 * b, kvh * G,
+                                    static_cast<int32_t>(p.q0) + t0 + x * BQ, smem_addr(q_full), pol);
             }
             const int boxes = kPtKeys / px_rows;
             const int64_t no_block = px.n_blocks;  // reads as zeros
@@ -624,10 +626,11 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                 return true;
             };
             int32_t b0 = block_of(0, lane), b1 = block_of(1, lane), b2 = block_of(2, lane);  // of tiles t, t + 1, t + 2
-            bool ok = tile(&tk, 0, b0) && (nt < 2 || tile(&tk, 1, b1));
+            bool ok = kPairs || (tile(&tk, 0, b0) && (nt < 2 || tile(&tk, 1, b1)));
             for (int t = 0; t < nt && ok; ++t) {
                 const int32_t b3 = block_of(t + 3, lane);
-                ok = tile(&tv, t, b0) && (t + 2 >= nt || tile(&tk, t + 2, b2));
+                if (kPairs) ok = tile(&tk, t, b0) && tile(&tv, t, b0);
+                else ok = tile(&tv, t, b0) && (t + 2 >= nt || tile(&tk, t + 2, b2));
                 b0 = b1, b1 = b2, b2 = b3;
             }
             // copies still landing in this CTA's shared memory
@@ -1175,6 +1178,22 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                         *staged(stage, 4 * (c0 + c) + j) =
                             make_uint4(pack_pair<T>(x[8 * j], x[8 * j + 1]), pack_pair<T>(x[8 * j + 2], x[8 * j + 3]),
                                        pack_pair<T>(x[8 * j + 4], x[8 * j + 5]), pack_pair<T>(x[8 * j + 6], x[8 * j + 7]));
+                } else if constexpr (PX) {
+                    // 32 columns of the warp's 32 rows through shared memory, so that whole lines are written
+                    float4 *mine32 = reinterpret_cast<float4 *>(stage + (kJoin ? 4 * slot + qq : qq) * 4096);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        mine32[8 * lane + (j ^ (lane & 7))] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+                    __syncwarp();
+                    const uint32_t rows = __ballot_sync(0xffffffffu, live);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int rr = 4 * i + (lane >> 3), j = lane & 7;
+                        const int64_t to_row = __shfl_sync(0xffffffffu, part_row, rr);
+                        if (rows >> rr & 1u)
+                            *reinterpret_cast<float4 *>(part_o + to_row * D + 32 * (c0 + c) + 4 * j) = mine32[8 * rr + (j ^ (rr & 7))];
+                    }
+                    __syncwarp();
                 } else if (live) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 4)
@@ -1184,7 +1203,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             }
         }
         if (!whole_out) {
-            if (live && slot == 0) part_ml[part_row] = make_float2(m_row, PX && !ok ? -1.f : l_row);  // (-1: not to be used)
+            if (live && (!kJoin || slot == 0)) part_ml[part_row] = make_float2(m_row, PX && !ok ? -1.f : l_row);  // (-1: not to be used)
         } else if constexpr (!kJoin) {
             named_sync(2 + slot, 128);
             if (ok && some) store_rows(stage, t0 + slot * BQ, r, 128);
@@ -1197,7 +1216,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     __syncthreads();
     if constexpr (PX) {
         if (bad_block) {  // the joining kernel clears the group's rows
-            if (warp >= 4 && slot == 0 && live) part_ml[part_row] = make_float2(0.f, -1.f);
+            if (warp >= 4 && (!kJoin || slot == 0) && live) part_ml[part_row] = make_float2(0.f, -1.f);
             if (threadIdx.x == 0) set_status(a.status, B200_DEV_BAD_POSITION);
         }
     }
@@ -1353,11 +1372,11 @@ cudaError_t pt_by_dim(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) 
     return a.D == 128 ? pt_by_tiles<T, 128>(a, plan, st) : pt_by_tiles<T, 64>(a, plan, st);
 }
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 cudaError_t px_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st) {
     constexpr bool bf16 = __is_same(T, __nv_bfloat16);
-    using Ge = PtGeometry<D, 1, 2, 1>;
-    auto kern = packed_tc_kernel<T, D, 1, 2, true>;
+    using Ge = PtGeometry<D, NT, 2, 1>;
+    auto kern = packed_tc_kernel<T, D, NT, 2, true>;
     const cudaError_t e = once_per_device(reinterpret_cast<const void *>(kern), ATTR_SMEM, [&] {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ge::kSmem));
     });
@@ -1375,7 +1394,7 @@ cudaError_t px_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st)
                           CU_TENSOR_MAP_SWIZZLE_128B);
     };
     CUtensorMap mq, mk, mv;
-    const int64_t ctas = most_packed_tiles(p.n_groups, a.total_q, 1, BQ) * a.Hkv * p.parts;
+    const int64_t ctas = most_packed_tiles(p.n_groups, a.total_q, 1, NT * BQ) * a.Hkv * p.parts;
     if (ctas > INT32_MAX || !row_map(&mq, bf16, a.q, D, a.Hq, a.total_q, a.q_head, a.q_tok, a.G, BQ) || !pool_map(&mk, a.k) ||
         !pool_map(&mv, a.v))
         return cudaErrorNotSupported;
@@ -1387,10 +1406,15 @@ cudaError_t px_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st)
 
 }  // namespace
 
+template <typename T, int D>
+cudaError_t px_by_tiles(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st) {
+    return p.tiles == 2 ? px_launch<T, D, 2>(a, p, st) : px_launch<T, D, 1>(a, p, st);
+}
+
 cudaError_t prefix_tc_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st) {
     if (a.G > kPtRows || a.dtype == B200_DTYPE_F32) return cudaErrorNotSupported;
-    if (a.dtype == B200_DTYPE_F16) return a.D == 128 ? px_launch<__half, 128>(a, p, st) : px_launch<__half, 64>(a, p, st);
-    return a.D == 128 ? px_launch<__nv_bfloat16, 128>(a, p, st) : px_launch<__nv_bfloat16, 64>(a, p, st);
+    if (a.dtype == B200_DTYPE_F16) return a.D == 128 ? px_by_tiles<__half, 128>(a, p, st) : px_by_tiles<__half, 64>(a, p, st);
+    return a.D == 128 ? px_by_tiles<__nv_bfloat16, 128>(a, p, st) : px_by_tiles<__nv_bfloat16, 64>(a, p, st);
 }
 
 size_t packed_tc_workspace(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t D, int64_t Hq, int64_t Hkv,

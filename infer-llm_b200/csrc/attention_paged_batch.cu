@@ -43,9 +43,15 @@ namespace {
 constexpr int kPbWarps = 4;
 constexpr int kPbThreads = 32 * kPbWarps;
 constexpr int kPbMostCtas = 320;
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kPxJoinThreads = 256;
 constexpr int kCluster = 8;
 constexpr int kClusterKeys = 4096;
+// Units of the line of tiles that a tile and a pair's start and end take. With prefixes the shares are weighed by them (64 ragged
+// BF16 sequences over their own 33 k keys TODO us, unweighed TODO); without, a tile is a unit.
+template <bool PX>
+constexpr int kTileUnits = PX ? 2 : 1;
+template <bool PX>
+constexpr int kPairUnits = PX ? 3 : 0;
 
 template <typename T, int D, int HB>
 struct Geometry {
@@ -365,28 +371,6 @@ struct Joined {
     }
 };
 
-// Adds the parts of the prefix of row b, query head h, columns c .. c + 3.
-template <int D>
-B200_DEVICE void join_prefix(const PrefixArgs &px, int b, int h, int c, Joined &j) {
-    constexpr int kAtOnce = 4;
-    for (int i0 = 0; i0 < px.parts; i0 += kAtOnce) {
-        float2 ml[kAtOnce];
-        float4 x[kAtOnce];
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            const int64_t row = prefix_row(px, min(i0 + i, px.parts - 1), b, h);
-            ml[i] = __ldcg(px.ml + row);
-            x[i] = __ldcg(reinterpret_cast<const float4 *>(px.o + row * D + c));
-        }
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            if (i0 + i >= px.parts) break;
-            j.void_prefix |= ml[i].y < 0.f;
-            j.add(ml[i].x, ml[i].y, x[i], ml[i].y);
-        }
-    }
-}
-
 // Reports offsets and lengths of the groups that are out of range. One CTA.
 B200_DEVICE void report_groups(const PrefixArgs &px, int32_t *status) {
     for (int g = threadIdx.x; g < px.n_groups; g += blockDim.x) {
@@ -420,27 +404,28 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
         at.len = seq_len(a, at.b);
         at.tiles = (at.len + Ge::kTile - 1) / Ge::kTile;
         at.t = at.tiles * rank / kCluster;
-        at.left = at.tiles * (rank + 1) / kCluster - at.t;
+        at.left = (at.tiles * (rank + 1) / kCluster - at.t) * kTileUnits<PX>;
         if (rank == 0 && at.vh == 0 && threadIdx.x == 0) report_length(a, at.b);
         if (at.left == 0)  // no keys: nothing to add
             for (int i = threadIdx.x; i < Ge::kRec; i += kPbThreads)
                 own[i] = i >= HB * D && i < HB * D + HB ? -INFINITY : 0.f;
     } else {
         grid_launch_dependents();  // the joining kernel waits for this grid's end
-        const int64_t total = tiles_before<Ge::kTile>(a, a.n_seqs) * a.VH;
-        const int64_t ctas = min64(gridDim.x, total);
+        const int64_t total = tiles_before<Ge::kTile, kTileUnits<PX>, kPairUnits<PX>>(a, a.n_seqs) * a.VH;
+        const int64_t ctas = min64(gridDim.x, total / kTileUnits<PX>);
         if (blockIdx.x >= ctas) {
-            if (PX) grid_wait();
+            if (PX && blockIdx.x == gridDim.x - 1) grid_wait();
             return;
         }
         u0 = share_begin(total, blockIdx.x, ctas);
         u1 = share_begin(total, blockIdx.x + 1, ctas);
-        at = place_at<Ge::kTile>(a, u0, u1);
+        at = place_at<Ge::kTile, kTileUnits<PX>, kPairUnits<PX>>(a, u0, u1);
     }
     const Place start = at;
     Place in = at;  // what is loaded: one block lookup ahead of `issue`
     bool bad = false;
 
+    const uint64_t once = PX ? policy_evict_first() : 0;
     // lane r < kSub looks up key row r of the sub-tile at `in`
     int64_t row_off = -1;  // byte offset in the pool; -1: no row
     int32_t row_blk = -1;
@@ -472,13 +457,22 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
                 const uint32_t d = dst + r * Ge::kRow + ((c ^ (r & 7)) << 4);
                 const int n = o >= 0 ? 16 : 0;
                 const int64_t src = (o >= 0 ? o : 0) + c * 16;
+                if constexpr (PX) {  // these keys are read once; the prefixes' parts are to stay in L2
+                    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(d), "l"(a.k + src), "r"(n),
+                                 "l"(once)
+                                 : "memory");
+                    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(d + Ge::kHalf),
+                                 "l"(a.v + src), "r"(n), "l"(once)
+                                 : "memory");
+                    continue;
+                }
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(a.k + src), "r"(n) : "memory");
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + Ge::kHalf), "l"(a.v + src), "r"(n)
                              : "memory");
             }
         }
         cp_async_commit();
-        if (in.left > 0) place_next<Ge::kTile>(a, in);
+        if (in.left > 0) place_next<Ge::kTile, kTileUnits<PX>, kPairUnits<PX>>(a, in);
         lookup();
     };
 
@@ -507,7 +501,7 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
         stage = (stage + 1) % Ge::kStages;
 
         const bool pair_end = at.t + 1 == at.tiles;
-        if (pair_end || at.left == 1) {
+        if (pair_end || at.left <= kTileUnits<PX>) {
             // the warps' partials, joined in warp order
             if (!first) __syncthreads();  // the previous part's partials have been read
             first = false;
@@ -515,7 +509,7 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
             __syncthreads();
             const bool whole = !CL && pair_end && part_t0 == 0;
             // parts: slot 0 begins with the CTA's share, slot 1 with a pair
-            const int slot = part_t0 == 0 && at.left - 1 + (at.t + 1) != u1 - u0 ? 1 : 0;
+            const int slot = part_t0 == 0 && (PX || at.left - 1 + (at.t + 1) != u1 - u0) ? 1 : 0;
             float *rec = CL ? own : a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * (PX ? Ge::kRecAt : Ge::kRec);
             if (PX && whole) rec = a.whole + (static_cast<int64_t>(at.b) * a.VH + at.vh) * Ge::kRecAt;
             for (int i = threadIdx.x; i < heads * D; i += kPbThreads) {
@@ -544,11 +538,13 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
             }
             fresh = true;
         }
-        place_next<Ge::kTile>(a, at);
+        place_next<Ge::kTile, kTileUnits<PX>, kPairUnits<PX>>(a, at);
     }
     cp_async_wait<0>();
     if (bad) set_status(a.status, B200_DEV_BAD_POSITION);
-    if constexpr (PX) grid_wait();  // the prefixes' parts are written (and this grid ends after theirs)
+    // The prefixes' parts are written. In two launches the join needs them, so one CTA's wait does: this grid ends after theirs.
+    // (The others would hold room that the grid's later CTAs want.)
+    if (PX && (CL || blockIdx.x == gridDim.x - 1)) grid_wait();
     if constexpr (CL) {
         cluster_sync();  // every CTA's record is written
         int group = -1;
@@ -685,17 +681,19 @@ __global__ void __launch_bounds__(kJoinThreads) paged_batch_join_kernel(const __
     again(odd);
 }
 
-// With prefixes: the parts of each pair's own keys, or its one record, and the parts of its prefix. One CTA a pair, a thread four columns
-// at a time.
+// With prefixes: the parts of each pair's own keys, or its one record, and the parts of its prefix. One CTA a pair, a thread four
+// columns at a time; where the pair has fewer columns than threads, several threads share out the parts.
 template <typename T, int D, int HB>
-__global__ void __launch_bounds__(kJoinThreads) paged_batch_prefix_join_kernel(const __grid_constant__ PbArgs a,
+__global__ void __launch_bounds__(kPxJoinThreads) paged_batch_prefix_join_kernel(const __grid_constant__ PbArgs a,
                                                                                const __grid_constant__ PrefixArgs px, const int64_t grid) {
     using Ge = Geometry<T, D, HB>;
-    __shared__ float again[(kJoinThreads / 32) * (D + 2)];
+    __shared__ __align__(16) float shared[kPxJoinThreads * 8];  // a Joined each
+    static_assert((kPxJoinThreads / 32) * (D + 2) <= kPxJoinThreads * 8, "output_again's part");
     const int b = static_cast<int>(blockIdx.x / a.VH), vh = static_cast<int>(blockIdx.x % a.VH);
-    const int64_t before = tiles_before<Ge::kTile>(a, b);
-    const int64_t total = tiles_before<Ge::kTile>(a, a.n_seqs) * a.VH;
-    const int64_t ctas = min64(grid, total);  // as in the main kernel
+    constexpr int TU = kTileUnits<true>, PU = kPairUnits<true>;
+    const int64_t before = tiles_before<Ge::kTile, TU, PU>(a, b);
+    const int64_t total = tiles_before<Ge::kTile, TU, PU>(a, a.n_seqs) * a.VH;
+    const int64_t ctas = min64(grid, total / TU);  // as in the main kernel
     const int tiles = seq_tiles<Ge::kTile>(a, b), group = prefix_group(px, b);
     const int h0 = (vh / a.HG) * a.G + (vh % a.HG) * HB;
     const int heads = min(HB, a.G - (vh % a.HG) * HB);
@@ -703,25 +701,61 @@ __global__ void __launch_bounds__(kJoinThreads) paged_batch_prefix_join_kernel(c
     if (threadIdx.x == 0 && vh == 0) report_length(a, b);
     if (blockIdx.x == 0) report_groups(px, a.status);
     int64_t c0 = 0;
-    int parts = 0, slot0 = 0;  // CTAs c0 .. c0 + parts - 1 hold parts; only the first's may be a second part
+    int parts = 0;  // CTAs c0 .. c0 + parts - 1 hold parts; the first's begins with the pair
     if (tiles > 0) {
-        const int64_t ua = before * a.VH + static_cast<int64_t>(vh) * tiles;
+        const int64_t ua = before * a.VH + vh * units_of<TU, PU>(tiles);
         c0 = share_owner(total, ua, ctas);
-        parts = static_cast<int>(share_owner(total, ua + tiles - 1, ctas) - c0) + 1;
-        slot0 = share_begin(total, c0, ctas) >= ua ? 0 : 1;
+        parts = static_cast<int>(share_owner(total, ua + (tiles - 1) * TU, ctas) - c0) + 1;
     }
     grid_wait();
-    const float *first = parts == 1 ? a.whole + static_cast<int64_t>(blockIdx.x) * Ge::kRecAt : a.ws + (c0 * 2 + slot0) * Ge::kRecAt;
+    const float *first = parts == 1 ? a.whole + static_cast<int64_t>(blockIdx.x) * Ge::kRecAt : a.ws + (c0 * 2 + 1) * Ge::kRecAt;
     const auto part = [&](int i) { return i == 0 ? first : a.ws + (c0 + i) * 2 * Ge::kRecAt; };
+    constexpr int kAtOnce = 6;
+    const int columns = heads * (D / 4);              // of four; at most kPxJoinThreads times two
+    const int share = max(1, kPxJoinThreads / columns);  // threads that share out a column's parts
     bool odd = false;
-    for (int i = 4 * threadIdx.x; i < heads * D; i += 4 * kJoinThreads) {
-        const int g = i / D;
+    for (int col0 = 0; col0 < columns; col0 += kPxJoinThreads) {
+        const int col = share == 1 ? col0 + static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x) % columns;
+        const int mine = share == 1 ? 0 : static_cast<int>(threadIdx.x) / columns;
+        const bool has = col < columns && mine < share;
+        const int g = col / (D / 4), c = col % (D / 4) * 4;
         Joined j;
-        for (int p = 0; p < parts; ++p) {
-            const float *rec = part(p);
-            j.add(__ldcg(rec + HB * D + g), __ldcg(rec + HB * D + HB + g), __ldcg(reinterpret_cast<const float4 *>(rec + i)), 1.f);
+        if (has) {
+            for (int p = mine; p < parts; p += share) {
+                const float *rec = part(p);
+                j.add(__ldcg(rec + HB * D + g), __ldcg(rec + HB * D + HB + g),
+                      __ldcg(reinterpret_cast<const float4 *>(rec + g * D + c)), 1.f);
+            }
+            for (int i0 = mine; group >= 0 && i0 < px.parts; i0 += kAtOnce * share) {
+                float2 ml[kAtOnce];
+                float4 x[kAtOnce];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const int64_t row = prefix_row(px, min(i0 + i * share, px.parts - 1), b, h0 + g);
+                    ml[i] = __ldcg(px.ml + row);
+                    x[i] = __ldcg(reinterpret_cast<const float4 *>(px.o + row * D + c));
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    if (i0 + i * share >= px.parts) break;
+                    j.void_prefix |= ml[i].y < 0.f;
+                    j.add(ml[i].x, ml[i].y, x[i], ml[i].y);
+                }
+            }
         }
-        if (group >= 0) join_prefix<D>(px, b, h0 + g, i - g * D, j);
+        if (share > 1) {
+            float *own = shared + threadIdx.x * 8;
+            *reinterpret_cast<float4 *>(own) = make_float4(j.o[0], j.o[1], j.o[2], j.o[3]);
+            own[4] = j.m, own[5] = j.l, own[6] = j.void_prefix ? 1.f : 0.f;
+            __syncthreads();
+            if (mine == 0)
+                for (int s = 1; s < share; ++s) {
+                    const float *other = own + s * columns * 8;
+                    j.add(other[4], other[5], *reinterpret_cast<const float4 *>(other), 1.f);
+                    j.void_prefix |= other[6] != 0.f;
+                }
+        }
+        if (!has || mine) continue;
         const float inv = j.l != 0.f && !j.void_prefix ? 1.0f / j.l : 0.f;
         T x[4];
 #pragma unroll
@@ -730,13 +764,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_batch_prefix_join_kernel(c
             odd |= !(fabsf(y) < INFINITY);
             x[e] = from_f32<T>(y);
         }
-        T *to = out + g * a.o_head + (i - g * D);
+        T *to = out + g * a.o_head + c;
         if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(to) = *reinterpret_cast<const float4 *>(x);
         else *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(x);
     }
     if constexpr (sizeof(T) == 2) {
         if (__syncthreads_or(odd))
-            for (int g = 0; g < heads; ++g) output_again<T, D, kJoinThreads / 32, true>(a, px, b, h0 + g, 0, D, again);
+            for (int g = 0; g < heads; ++g) output_again<T, D, kPxJoinThreads / 32, true>(a, px, b, h0 + g, 0, D, shared);
     }
 }
 
@@ -794,7 +828,7 @@ cudaError_t pb_launch(PbArgs a, const PrefixArgs &px, int64_t Hkv, cudaStream_t 
     e = b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPbThreads), Ge::kSmem, st, PX && px.parts > 0, a, px);
     if (e != cudaSuccess) return e;
     if constexpr (PX)
-        return b200_launch(paged_batch_prefix_join_kernel<T, D, HB>, dim3(static_cast<unsigned>(pairs)), dim3(kJoinThreads), 0, st, true,
+        return b200_launch(paged_batch_prefix_join_kernel<T, D, HB>, dim3(static_cast<unsigned>(pairs)), dim3(kPxJoinThreads), 0, st, true,
                            a, px, ctas);
     else
         return b200_launch(paged_batch_join_kernel<T, D, HB>, dim3(static_cast<unsigned>(pairs)), dim3(kJoinThreads), 0, st, true,

@@ -14,6 +14,8 @@
 namespace b200 {
 namespace {
 
+constexpr int64_t kPrefixParts = 32;  // at most: the join reads all of a row's
+
 // A CTA: 64 rows of a group and KV head against a part of the prefix's keys.
 template <typename T, int D>
 __global__ void __launch_bounds__(kPkThreads, 2) prefix_ffma_kernel(const PackedArgs a, const PrefixArgs px) {
@@ -48,16 +50,27 @@ __global__ void __launch_bounds__(kPkThreads, 2) prefix_ffma_kernel(const Packed
         });
 }
 
-int64_t prefix_tiles(int64_t n_seqs, int64_t n_groups, int64_t G, int64_t Hkv, bool tc) {
-    return (tc ? most_packed_tiles(n_groups, n_seqs, 1, kPrefixTcRows / G) : most_packed_tiles(n_groups, n_seqs, G, kPkRows)) * Hkv;
-}
-
-// Parts of each prefix's keys: as many as the CTAs that run at once allow, of two key tiles at least.
-int prefix_parts(int64_t n_seqs, int64_t n_groups, int64_t max_prefix, int64_t G, int64_t Hkv, int32_t dtype) {
-    if (n_groups <= 0 || max_prefix <= 0) return 0;
-    const bool tc = dtype != B200_DTYPE_F32 && G <= kPrefixTcRows;
-    const int64_t ctas = device_sm_count() * (tc ? 1 : 2), keys = 2 * (tc ? 128 : kPkKeys);
-    return static_cast<int>(max64(1, min64(min64(32, (max_prefix + keys - 1) / keys), ctas / max64(1, prefix_tiles(n_seqs, n_groups, G, Hkv, tc)))));
+// How the prefixes are cut: rows of a tile (sequences, or with FFMA sequences times heads), tiles a CTA, parts of the keys.
+struct PrefixPlan {
+    bool tc = false;
+    int tiles = 1, parts = 0;
+    int64_t rows = 0;  // of a CTA
+};
+PrefixPlan prefix_plan(int64_t n_seqs, int64_t n_groups, int64_t max_prefix, int64_t G, int64_t Hkv, int32_t dtype) {
+    PrefixPlan p;
+    if (n_groups <= 0 || n_seqs <= 0 || max_prefix <= 0) return p;
+    p.tc = dtype != B200_DTYPE_F32 && G <= kPrefixTcRows;
+    // As if groups were alike. A group of more than one tile takes two a CTA, over the same keys.
+    const int64_t groups = min64(n_groups, n_seqs), each = (n_seqs + groups - 1) / groups, rows = p.tc ? each : each * G;
+    p.rows = p.tc ? kPrefixTcRows / G : kPkRows;
+    if (p.tc && rows > p.rows) p.tiles = 2;
+    p.rows *= p.tiles;
+    const int64_t ctas = groups * ((rows + p.rows - 1) / p.rows) * Hkv;
+    // As many parts as the CTAs that run at once allow, of two key tiles at least (one, where two tiles of rows alternate).
+    const int64_t keys = p.tc ? 256 / p.tiles : 2 * kPkKeys;
+    const int64_t most = min64(kPrefixParts, (max_prefix + keys - 1) / keys);
+    p.parts = static_cast<int>(max64(1, min64(most, device_sm_count() * (p.tc ? 1 : 2) / ctas)));
+    return p;
 }
 
 size_t prefix_bytes(int64_t n_seqs, int64_t parts, int64_t D, int64_t Hq) {
@@ -71,7 +84,7 @@ cudaError_t prefix_ffma_launch(const PackedArgs &a, const PrefixArgs &px, cudaSt
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ffma_smem<D>()));
     });
     if (e != cudaSuccess) return e;
-    const int64_t ctas = prefix_tiles(px.n_seqs, px.n_groups, a.G, a.Hkv, false) * px.parts;
+    const int64_t ctas = most_packed_tiles(px.n_groups, px.n_seqs, a.G, kPkRows) * a.Hkv * px.parts;
     if (ctas > INT32_MAX) return cudaErrorNotSupported;
     return b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPkThreads), ffma_smem<D>(), st, false, a, px);
 }
@@ -101,7 +114,7 @@ size_t b200_flash_attn_paged_shared_workspace_bytes(int64_t n_seqs, int64_t max_
     if (n_seqs <= 0 || max_keys <= 0 || n_groups < 0 || max_prefix < 0 || D <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv ||
         !dtype_bytes(dtype))
         return 0;
-    return prefix_bytes(n_seqs, prefix_parts(n_seqs, n_groups, max_prefix, Hq / Hkv, Hkv, dtype), D, Hq) +
+    return prefix_bytes(n_seqs, prefix_plan(n_seqs, n_groups, max_prefix, Hq / Hkv, Hkv, dtype).parts, D, Hq) +
            paged_batch_prefix_bytes(n_seqs, max_keys, D, Hq / Hkv, Hkv, dtype);
 }
 
@@ -148,7 +161,9 @@ int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_
     px.n_groups = static_cast<int32_t>(n_groups);
     px.n_seqs = static_cast<int32_t>(n_seqs);
     px.Hq = static_cast<int32_t>(Hq);
-    px.parts = prefix_parts(n_seqs, n_groups, max_prefix, Hq / Hkv, Hkv, pool->dtype);
+    const PrefixPlan plan = prefix_plan(n_seqs, n_groups, max_prefix, Hq / Hkv, Hkv, pool->dtype);
+    px.parts = plan.parts;
+    px.tiles = plan.tiles;
     px.o = static_cast<float *>(workspace);
     px.ml = reinterpret_cast<float2 *>(px.o + px.parts * n_seqs * Hq * D);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -12,7 +12,7 @@ struct PrefixArgs {
     int64_t table_stride = 0, max_keys = 0, n_blocks = 0;            // max_keys: positions a table row covers (fits 31 bits)
     int64_t block_stride = 0, tok_stride = 0, head_stride = 0;       // of the pool, elements
     uint32_t bt = 1;
-    int32_t n_groups = 0, n_seqs = 0, Hq = 0, parts = 0;
+    int32_t n_groups = 0, n_seqs = 0, Hq = 0, parts = 0, tiles = 1;  // tiles: of rows, a CTA of the tensor-core kernel
     float *o = nullptr;    // [part][sequence][query head][D]
     float2 *ml = nullptr;  // [part][sequence][query head]: maximum, sum (-1: the group's prefix names a block out of range)
 };
