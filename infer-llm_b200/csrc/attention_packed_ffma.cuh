@@ -25,16 +25,28 @@ B200_DEVICE void load4(const T *p, float (&x)[4]) {
     for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(e[i]);
 }
 
+// RT neighbouring numbers of shared memory.
+template <int RT>
+B200_DEVICE void read_rows(const float *p, float (&x)[RT]) {
+    if constexpr (RT == 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(p);
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else {
+        static_assert(RT == 1, "four rows a thread, or one");
+        x[0] = *p;
+    }
+}
+
 template <int D>
 constexpr size_t ffma_smem() {
     return (2 * static_cast<size_t>(D) * kPkPad + static_cast<size_t>(kPkKeys) * D) * 4;
 }
 
 // Rows [r0, r0 + rows) (row = token * G + head of the KV head's group; at most kPkRows) of sequence p against its
-// keys [first, end) (CAUSAL: those that each sees; key(j, k, v) points at key j's rows, false: it takes no part), by kPkThreads threads, of which this is `tid`; sync() is their barrier and
+// keys [first, end), RT rows a thread (fewer than kPkRows: 16 RT at most) (CAUSAL: those that each sees; key(j, k, v) points at key j's rows, false: it takes no part), by kPkThreads threads, of which this is `tid`; sync() is their barrier and
 // smem (16-byte aligned, ffma_smem<D>() bytes) theirs. store(row, column, x, m, l) gets each row's
 // output four columns at a time, already over l, its maximum (in powers of two) and its sum.
-template <typename T, int D, bool CAUSAL, typename Key, typename Sync, typename Store>
+template <typename T, int D, bool CAUSAL, int RT = 4, typename Key, typename Sync, typename Store>
 B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, int r0, int rows, int first, int end, Key key,
                            float *smem, int tid, Sync sync, Store store) {
     float *qt = smem;                  // [D][row]
@@ -44,8 +56,8 @@ B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, in
     const T *q = static_cast<const T *>(a.q);
     // four elements a load; lanes take neighbouring rows, so the transposed stores do not collide
 #pragma unroll
-    for (int i0 = 0; i0 < kPkRows * D / 4; i0 += kPkThreads) {
-        const int i = i0 + tid, r = i % kPkRows, d = i / kPkRows * 4;
+    for (int i0 = 0; i0 < 16 * RT * D / 4; i0 += kPkThreads) {
+        const int i = i0 + tid, r = i % (16 * RT), d = i / (16 * RT) * 4;
         float x[4] = {0.f, 0.f, 0.f, 0.f};
         if (r < rows) {
             const int tok = (r0 + r) / a.G, h = kvh * a.G + (r0 + r) % a.G;
@@ -55,13 +67,13 @@ B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, in
         for (int e = 0; e < 4; ++e) qt[(d + e) * kPkPad + r] = x[e];
     }
     if (CAUSAL) end = min(end, p.nk - p.nq + (r0 + rows - 1) / a.G + 1);  // the keys the last row sees
-    int last[4];  // last key each row sees (relative to the sequence)
+    int last[RT];  // last key each row sees (relative to the sequence)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        last[i] = 4 * ty + i < rows ? (CAUSAL ? min(end - 1, p.nk - p.nq + (r0 + 4 * ty + i) / a.G) : end - 1) : -1;
-    float m[4], l[4], o[4][D / 16];
+    for (int i = 0; i < RT; ++i)
+        last[i] = RT * ty + i < rows ? (CAUSAL ? min(end - 1, p.nk - p.nq + (r0 + RT * ty + i) / a.G) : end - 1) : -1;
+    float m[RT], l[RT], o[RT][D / 16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RT; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
@@ -69,12 +81,15 @@ B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, in
     }
     for (int k0 = first; k0 < end; k0 += kPkKeys) {
         sync();
+        static_assert(kPkThreads % kPkKeys == 0, "a thread loads of one key");
+        const int j = tid % kPkKeys;
+        const T *k = nullptr, *v = nullptr;
+        const bool has = k0 + j < end && key(k0 + j, k, v);
 #pragma unroll
         for (int i0 = 0; i0 < kPkKeys * D / 4; i0 += kPkThreads) {
-            const int i = i0 + tid, j = i % kPkKeys, d = i / kPkKeys * 4;
+            const int d = (i0 + tid) / kPkKeys * 4;
             float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-            const T *k, *v;
-            if (k0 + j < end && key(k0 + j, k, v)) {
+            if (has) {
                 load4(k + d, x);
                 load4(v + d, y);
             }
@@ -83,19 +98,19 @@ B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, in
             *reinterpret_cast<float4 *>(vs + j * D + d) = make_float4(y[0], y[1], y[2], y[3]);
         }
         sync();
-        float s[4][4] = {};
+        float s[RT][4] = {};
 #pragma unroll 8
         for (int d = 0; d < D; ++d) {
-            const float4 x = *reinterpret_cast<const float4 *>(qt + d * kPkPad + 4 * ty);
-            const float4 y = *reinterpret_cast<const float4 *>(kt + d * kPkPad + 4 * tx);
-            const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+            float xs[RT], ys[4];
+            read_rows<RT>(qt + d * kPkPad + RT * ty, xs);
+            read_rows<4>(kt + d * kPkPad + 4 * tx, ys);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < RT; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[i][j] = fmaf(xs[i], ys[j], s[i][j]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < RT; ++i) {
             float mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -118,22 +133,25 @@ B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, in
         }
         sync();  // the keys have been read
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<float4 *>(kt + (4 * tx + j) * kPkPad + 4 * ty) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+        for (int j = 0; j < 4; ++j) {
+            float *to = kt + (4 * tx + j) * kPkPad + RT * ty;
+            if constexpr (RT == 4) *reinterpret_cast<float4 *>(to) = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+            else *to = s[0][j];
+        }
         sync();
         // a key that a row does not see has P = 0, and 0 times a V that is no number would
         // not be 0: such products are left out where the tile has hidden keys
         const bool all = k0 + kPkKeys - 1 <= (CAUSAL ? min(end - 1, p.nk - p.nq + r0 / a.G) : end - 1);
 #pragma unroll 4
         for (int j = 0; j < kPkKeys; ++j) {
-            const float4 x = *reinterpret_cast<const float4 *>(kt + j * kPkPad + 4 * ty);
-            const float xs[4] = {x.x, x.y, x.z, x.w};
+            float xs[RT];
+            read_rows<RT>(kt + j * kPkPad + RT * ty, xs);
 #pragma unroll
             for (int c = 0; c < D / 64; ++c) {
-                const float4 y = *reinterpret_cast<const float4 *>(vs + j * D + 64 * c + 4 * tx);
-                const float ys[4] = {y.x, y.y, y.z, y.w};
+                float ys[4];
+                read_rows<4>(vs + j * D + 64 * c + 4 * tx, ys);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < RT; ++i)
                     if (all || k0 + j <= last[i]) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[i][4 * c + e] = fmaf(xs[i], ys[e], o[i][4 * c + e]);
@@ -142,8 +160,8 @@ B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, in
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = 4 * ty + i;
+    for (int i = 0; i < RT; ++i) {
+        const int r = RT * ty + i;
 #pragma unroll
         for (int w = 1; w < 16; w <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
         if (r >= rows) continue;

@@ -327,18 +327,30 @@ constexpr int kSplitThreads = 256;
 // One CTA: the K or V rows of one key tile and KV head, as hi and lo planes with the tile's
 // exponent, and whether its rows and columns spread too far for one. A pass over the bytes: HBM bounds it (2048 keys, 8 heads of 128: 17 MB in, 17 MB out, 7 us
 // with its launch; the attention kernel's start overlaps it).
-template <int D>
-__global__ void __launch_bounds__(kSplitThreads) packed_split_kernel(const PackedArgs a, __half *planes, int32_t *exps) {
+// PX: of a prefix's blocks, tile after tile of a group's room.
+template <int D, bool PX>
+__global__ void __launch_bounds__(kSplitThreads)
+    packed_split_kernel(const PackedArgs a, const PrefixArgs px, __half *planes, int32_t *exps) {
     constexpr int V4 = D / 4, PER = kPtKeys * V4 / kSplitThreads;  // float4 a row, a thread
     constexpr int W = kSplitThreads / 32;
     __shared__ uint32_t warp_top[W], warp_low[W], warp_any[W], col_top[W][D], col_low[D / 32];
     grid_launch_dependents();
     const int kvh = (blockIdx.x >> 1) % a.Hkv, is_v = blockIdx.x & 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const PackedTile p = find_packed_tile(a.cu_k, a.cu_k, a.n_seqs, a.total_k, a.total_k, 1, kPtKeys,
-                                          (blockIdx.x >> 1) / a.Hkv, nullptr);
-    if (p.seq < 0) return;
+    PackedTile p;
+    if constexpr (PX) {
+        const int tiles = static_cast<int>(px.room / kPtKeys), at = static_cast<int>((blockIdx.x >> 1) / a.Hkv);
+        p.seq = at / tiles;
+        p.tile = at % tiles;
+        p.k0 = p.seq * px.room;
+        p.nk = prefix_len(px, p.seq);
+        if (static_cast<int64_t>(p.tile) * kPtKeys >= p.nk) return;
+    } else {
+        p = find_packed_tile(a.cu_k, a.cu_k, a.n_seqs, a.total_k, a.total_k, 1, kPtKeys, (blockIdx.x >> 1) / a.Hkv, nullptr);
+        if (p.seq < 0) return;
+    }
     const float *src = static_cast<const float *>(is_v ? a.v : a.k) + kvh * (is_v ? a.v_head : a.k_head);
     const int64_t tok = is_v ? a.v_tok : a.k_tok;
+    static_assert(PER * (32 / V4) <= 32, "a lane looks up one row");
     const int rows = min(kPtKeys, p.nk - p.tile * kPtKeys);
     const int64_t first = p.k0 + static_cast<int64_t>(p.tile) * kPtKeys;
     // magnitudes: the largest finite one (`top`), of each row and column, the least of those that
@@ -346,10 +358,23 @@ __global__ void __launch_bounds__(kSplitThreads) packed_split_kernel(const Packe
     const auto nonzero = [](uint32_t m) { return m ? m : 0xFFFFFFFFu; };
     float4 x[PER];
     uint32_t low = 0xFFFFFFFFu, any = 0, top = 0, col[4] = {};
+    // PX: lane (i, row of the warp) looks up where the warp's i-th rows are, so that all lookups are one latency
+    constexpr int RW = 32 / V4;
+    int64_t where = -1;
+    if constexpr (PX) {
+        const int r = warp * RW + lane % RW + lane / RW * (kSplitThreads / V4);
+        if (lane < PER * RW && r < rows) where = prefix_key(px, p.seq, kvh, p.tile * kPtKeys + r);
+    }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int e = threadIdx.x + i * kSplitThreads, r = e / V4, c = e % V4;
-        x[i] = r < rows ? __ldg(reinterpret_cast<const float4 *>(src + (first + r) * tok) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        if constexpr (PX) {
+            const int64_t at = __shfl_sync(0xffffffffu, where, i * RW + lane / V4);
+            x[i] = at >= 0 ? __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(is_v ? a.v : a.k) + at) + c)
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+            x[i] = r < rows ? __ldg(reinterpret_cast<const float4 *>(src + (first + r) * tok) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
         const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
         uint32_t row = 0;
 #pragma unroll
@@ -398,7 +423,7 @@ __global__ void __launch_bounds__(kSplitThreads) packed_split_kernel(const Packe
         const bool wide = any >= 0x7F800000u || static_cast<int>(min(low, 0x7F800000u) >> 23) - 127 < e - kSpread;
         exps[(split_index(p.k0, p.seq, p.tile) * a.Hkv + kvh) * 2 + is_v] = exps_word(e - kTop, wide);
     }
-    const int64_t plane = a.total_k * a.Hkv * D;
+    const int64_t plane = (PX ? px.n_groups * px.room : a.total_k) * a.Hkv * D;
     __half *dst = planes + (is_v ? 2 * plane : 0) + kvh * D;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -426,7 +451,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     constexpr int PL = SPLIT ? 2 : 1;
     using Ge = PtGeometry<D, NT, SL, PL>;
     static_assert(SL == 2 || (NT == 1 && !SPLIT), "one slot holds one query tile");
-    static_assert(!PX || (SL == 2 && !SPLIT), "prefixes: two slots, 16-bit types");
+    static_assert(!PX || SL == 2, "prefixes: two slots");
     constexpr bool kPairs = NT == 2 || SL == 1, kJoin = NT == 1 && SL == 2;  // kJoin: the slots halve the key tiles
     constexpr int kColumns = 256 * SL;  // of tensor memory
     constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
@@ -590,7 +615,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
         if constexpr (SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         else if constexpr (SL == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (PX && warp == 0 && nt > 0) {
+        if (PX && !SPLIT && warp == 0 && nt > 0) {
             // ---- TMA, a lane a box of K or V
             const uint64_t pol = policy_evict_last();
             if (lane == 0) {
@@ -636,7 +661,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             // copies still landing in this CTA's shared memory
             wait_poll(q_full, 0, nullptr);
             for (int i = max(0, issued - S); i < issued; ++i) wait_poll(&full[i % S], (i / S) & 1, nullptr);
-        } else if (!PX && warp == 0 && lane == 0 && nt > 0) {
+        } else if ((!PX || SPLIT) && warp == 0 && lane == 0 && nt > 0) {
             // ---- TMA
             const uint64_t pol = policy_evict_last();  // K / V are read again by the other query tiles
             if (!SPLIT) {
@@ -859,8 +884,9 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             if (steps == 0) ok = __all_sync(0xffffffffu, wait(q_full, 0));  // Q's planes are written by now
             if (wide) any_wide = 1;
             named_sync(4, 384);
+            if (PX && !ok && live) part_ml[part_row] = make_float2(0.f, -1.f);  // not to be used
             ok = ok && !any_wide;  // else the softmax threads do the rows over
-            if (ok && !whole_out && live) part_ml[part_row] = make_float2(M, L);
+            if (ok && !whole_out && live) part_ml[part_row] = make_float2(M, PX ? L * pow2(-kTop) : L);
             if (ok) {
 #pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
@@ -998,21 +1024,26 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
             const int rows = min(BQ, p.nq - t0) * G, from = ta * kPtKeys, to = (ta + nt) * kPtKeys;
             for (int r0 = 0; r0 < rows; r0 += kPkRows) {
                 named_sync(5, kPkThreads);  // the last rows' shared memory is free
-                ffma_rows<float, D, true>(
-                    a, p, kvh, t0 * G + r0, min(kPkRows, rows - r0), from, to, PackedKeys<float>(a, p, kvh),
-                    reinterpret_cast<float *>(base), threadIdx.x - 128,
-                    [] { named_sync(5, kPkThreads); },
-                    [&](int row, int c, const float (&x)[4], float m, float l) {
-                        row += r0;
-                        if (sp.parts == 1) {
-                            float *to_row = static_cast<float *>(a.out) + (p.q0 + t0 + row / G) * a.o_tok + (kvh * G + row % G) * a.o_head;
-                            *reinterpret_cast<float4 *>(to_row + c) = make_float4(x[0], x[1], x[2], x[3]);
-                        } else {
-                            const int64_t at = static_cast<int64_t>(blockIdx.x) * kPtRows + row;
-                            *reinterpret_cast<float4 *>(sp.part_o + at * D + c) = make_float4(x[0], x[1], x[2], x[3]);
-                            if (c == 0) sp.part_ml[at] = make_float2(m, l * pow2(kTop));  // as the other parts' sums
-                        }
-                    });
+                const auto sync = [] { named_sync(5, kPkThreads); };
+                const auto store = [&](int row, int c, const float (&x)[4], float m, float l) {
+                    row += r0;
+                    const int64_t q_at = p.q0 + t0 + row / G;
+                    if (whole_out) {
+                        float *to_row = static_cast<float *>(a.out) + q_at * a.o_tok + (kvh * G + row % G) * a.o_head;
+                        *reinterpret_cast<float4 *>(to_row + c) = make_float4(x[0], x[1], x[2], x[3]);
+                    } else {
+                        const int64_t at = PX ? prefix_row(px, part, q_at, kvh * G + row % G) : static_cast<int64_t>(blockIdx.x) * kPtRows + row;
+                        *reinterpret_cast<float4 *>(part_o + at * D + c) = make_float4(x[0], x[1], x[2], x[3]);
+                        if (c == 0) part_ml[at] = make_float2(m, PX ? l : l * pow2(kTop));  // as the other parts' sums
+                    }
+                };
+                if constexpr (PX)
+                    ffma_rows<float, D, false>(a, p, kvh, t0 * G + r0, min(kPkRows, rows - r0), from, min(to, p.nk),
+                                               PrefixKeys<float>(a, px, p.seq, kvh), reinterpret_cast<float *>(base),
+                                               threadIdx.x - 128, sync, store);
+                else
+                    ffma_rows<float, D, true>(a, p, kvh, t0 * G + r0, min(kPkRows, rows - r0), from, to, PackedKeys<float>(a, p, kvh),
+                                              reinterpret_cast<float *>(base), threadIdx.x - 128, sync, store);
             }
         }
     } else {
@@ -1216,7 +1247,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     __syncthreads();
     if constexpr (PX) {
         if (bad_block) {  // the joining kernel clears the group's rows
-            if (warp >= 4 && (!kJoin || slot == 0) && live) part_ml[part_row] = make_float2(0.f, -1.f);
+            if ((SPLIT ? warp >= 12 : warp >= 4 && (!kJoin || slot == 0)) && live) part_ml[part_row] = make_float2(0.f, -1.f);
             if (threadIdx.x == 0) set_status(a.status, B200_DEV_BAD_POSITION);
         }
     }
@@ -1342,8 +1373,8 @@ cudaError_t pt_launch(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) 
             !row_map(&mv, false, planes + 2 * plane, D, a.Hkv, 2 * a.total_k, D, a.Hkv * D, 1, kPtKeys))
             return cudaErrorNotSupported;
         mq = mk;  // not used
-        e = b200_launch(packed_split_kernel<D>, dim3(static_cast<unsigned>(tiles)), dim3(kSplitThreads), 0, st, false, a,
-                        planes, exps);
+        e = b200_launch(packed_split_kernel<D, false>, dim3(static_cast<unsigned>(tiles)), dim3(kSplitThreads), 0, st, false, a,
+                        PrefixArgs(), planes, exps);
         if (e != cudaSuccess) return e;
     } else {
         if (!row_map(&mq, bf16, a.q, D, a.Hq, a.total_q, a.q_head, a.q_tok, a.G, BQ) ||
@@ -1374,10 +1405,10 @@ cudaError_t pt_by_dim(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) 
 
 template <typename T, int D, int NT>
 cudaError_t px_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st) {
-    constexpr bool bf16 = __is_same(T, __nv_bfloat16);
-    using Ge = PtGeometry<D, NT, 2, 1>;
+    constexpr bool bf16 = __is_same(T, __nv_bfloat16), split = __is_same(T, float);
+    using Ge = PtGeometry<D, NT, 2, split ? 2 : 1>;
     auto kern = packed_tc_kernel<T, D, NT, 2, true>;
-    const cudaError_t e = once_per_device(reinterpret_cast<const void *>(kern), ATTR_SMEM, [&] {
+    cudaError_t e = once_per_device(reinterpret_cast<const void *>(kern), ATTR_SMEM, [&] {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Ge::kSmem));
     });
     if (e != cudaSuccess) return e;
@@ -1393,28 +1424,50 @@ cudaError_t px_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st)
         return tma_encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, base, 4, dims, strides, box,
                           CU_TENSOR_MAP_SWIZZLE_128B);
     };
-    CUtensorMap mq, mk, mv;
-    const int64_t ctas = most_packed_tiles(p.n_groups, a.total_q, 1, NT * BQ) * a.Hkv * p.parts;
-    if (ctas > INT32_MAX || !row_map(&mq, bf16, a.q, D, a.Hq, a.total_q, a.q_head, a.q_tok, a.G, BQ) || !pool_map(&mk, a.k) ||
-        !pool_map(&mv, a.v))
-        return cudaErrorNotSupported;
+    CUtensorMap mq = {}, mk, mv;
     SplitView sp;
     sp.parts = p.parts;
-    return b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPtThreads<T, 2>), Ge::kSmem, st, false, mq, mk, mv, a, sp, p,
-                       rows);
+    const int64_t ctas = most_packed_tiles(p.n_groups, a.total_q, 1, NT * BQ) * a.Hkv * p.parts;
+    if (ctas > INT32_MAX) return cudaErrorNotSupported;
+    if constexpr (split) {
+        const int64_t total = p.n_groups * p.room, plane = total * a.Hkv * D, tiles = total / kPtKeys * a.Hkv * 2;
+        __half *planes = static_cast<__half *>(p.planes);
+        int32_t *exps = reinterpret_cast<int32_t *>(planes + 4 * plane);
+        sp.exps = exps;
+        sp.total_k = total;
+        if (!planes || tiles > INT32_MAX || 2 * total > INT32_MAX - 1024 ||
+            !row_map(&mk, false, planes, D, a.Hkv, 2 * total, D, a.Hkv * D, 1, kPtKeys) ||
+            !row_map(&mv, false, planes + 2 * plane, D, a.Hkv, 2 * total, D, a.Hkv * D, 1, kPtKeys))
+            return cudaErrorNotSupported;
+        mq = mk;  // not used
+        e = b200_launch(packed_split_kernel<D, true>, dim3(static_cast<unsigned>(tiles)), dim3(kSplitThreads), 0, st, false, a, p, planes,
+                        exps);
+        if (e != cudaSuccess) return e;
+    } else if (!row_map(&mq, bf16, a.q, D, a.Hq, a.total_q, a.q_head, a.q_tok, a.G, BQ) || !pool_map(&mk, a.k) || !pool_map(&mv, a.v)) {
+        return cudaErrorNotSupported;
+    }
+    return b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPtThreads<T, 2>), Ge::kSmem, st, split, mq, mk, mv, a, sp, p, rows);
 }
-
-}  // namespace
 
 template <typename T, int D>
 cudaError_t px_by_tiles(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st) {
     return p.tiles == 2 ? px_launch<T, D, 2>(a, p, st) : px_launch<T, D, 1>(a, p, st);
 }
 
+}  // namespace
+
+size_t prefix_planes_bytes(int64_t n_groups, int64_t room, int64_t D, int64_t Hkv) {
+    return split_bytes(n_groups, n_groups * room, D, Hkv, B200_DTYPE_F32);
+}
+
 cudaError_t prefix_tc_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st) {
-    if (a.G > kPtRows || a.dtype == B200_DTYPE_F32) return cudaErrorNotSupported;
-    if (a.dtype == B200_DTYPE_F16) return a.D == 128 ? px_by_tiles<__half, 128>(a, p, st) : px_by_tiles<__half, 64>(a, p, st);
-    return a.D == 128 ? px_by_tiles<__nv_bfloat16, 128>(a, p, st) : px_by_tiles<__nv_bfloat16, 64>(a, p, st);
+    if (a.G > kPtRows) return cudaErrorNotSupported;
+    switch (a.dtype) {
+        case B200_DTYPE_F16: return a.D == 128 ? px_by_tiles<__half, 128>(a, p, st) : px_by_tiles<__half, 64>(a, p, st);
+        case B200_DTYPE_BF16: return a.D == 128 ? px_by_tiles<__nv_bfloat16, 128>(a, p, st) : px_by_tiles<__nv_bfloat16, 64>(a, p, st);
+    }
+    if (!p.planes) return cudaErrorNotSupported;
+    return a.D == 128 ? px_launch<float, 128, 1>(a, p, st) : px_launch<float, 64, 1>(a, p, st);
 }
 
 size_t packed_tc_workspace(int64_t n_seqs, int64_t total_q, int64_t total_k, int64_t D, int64_t Hq, int64_t Hkv,

@@ -4,8 +4,9 @@
 // while the one before ends:
 //  * the prefixes: the rows of a group (its sequences times the query heads of a KV head) against its prefix in tiles, so that each key
 //    is read once for up to 128 rows. 16-bit types: the packed attention's tensor-core kernel (attention_packed_tc.cu), whose K and V tiles
-//    are copied block by block. F32, more than 128 query heads a KV head, or strides that a tensor map cannot hold: F32 FFMA
-//    (prefix_ffma_kernel). A prefix is cut into as many parts as fill the SMs.
+//    are copied block by block; F32 as three F16 products of planes that a kernel before writes from the blocks. Few F32 rows with short
+//    prefixes, more than 128 query heads a KV head, or strides that a tensor map cannot hold: F32 FFMA (prefix_ffma_kernel). A prefix
+//    is cut into as many parts as fill the SMs.
 //  * the sequences' own keys, as in the batched decode (attention_paged_batch.cu);
 //  * the join of all parts.
 #include "attention_packed_ffma.cuh"
@@ -14,17 +15,18 @@
 namespace b200 {
 namespace {
 
+constexpr int64_t kPrefixShort = 2048;
 constexpr int64_t kPrefixParts = 32;  // at most: the join reads all of a row's
 
-// A CTA: 64 rows of a group and KV head against a part of the prefix's keys.
-template <typename T, int D>
+// A CTA: 64 rows (RT 4) or 16 (RT 1) of a group and KV head against a part of the prefix's keys.
+template <typename T, int D, int RT>
 __global__ void __launch_bounds__(kPkThreads, 2) prefix_ffma_kernel(const PackedArgs a, const PrefixArgs px) {
     extern __shared__ __align__(16) float pf_smem[];
     grid_launch_dependents();
     const int part = blockIdx.x % px.parts, kvh = blockIdx.x / px.parts % a.Hkv;
-    const PackedTile p = find_prefix_tile(px, a.G, kPkRows, blockIdx.x / (px.parts * a.Hkv));
+    const PackedTile p = find_prefix_tile(px, a.G, 16 * RT, blockIdx.x / (px.parts * a.Hkv));
     if (p.seq < 0) return;
-    const int r0 = p.tile * kPkRows, rows = min(kPkRows, p.nq * a.G - r0);
+    const int r0 = p.tile * 16 * RT, rows = min(16 * RT, p.nq * a.G - r0);
     const int64_t tiles = (static_cast<int64_t>(p.nk) + kPkKeys - 1) / kPkKeys;
     const int first = static_cast<int>(tiles * part / px.parts) * kPkKeys;
     const int end = static_cast<int>(min64(p.nk, tiles * (part + 1) / px.parts * kPkKeys));
@@ -34,15 +36,8 @@ __global__ void __launch_bounds__(kPkThreads, 2) prefix_ffma_kernel(const Packed
         if (threadIdx.x < rows) px.ml[row_of(threadIdx.x)] = make_float2(0.f, -1.f);  // the joining kernel clears the group's rows
         return;
     }
-    const T *k0 = static_cast<const T *>(a.k), *v0 = static_cast<const T *>(a.v);
-    ffma_rows<T, D, false>(
-        a, p, kvh, r0, rows, first, end,
-        [&](int j, const T *&k, const T *&v) {
-            const int64_t at = prefix_key(px, p.seq, kvh, j);
-            k = k0 + at, v = v0 + at;
-            return at >= 0;
-        },
-        pf_smem, threadIdx.x, [] { __syncthreads(); },
+    ffma_rows<T, D, false, RT>(
+        a, p, kvh, r0, rows, first, end, PrefixKeys<T>(a, px, p.seq, kvh), pf_smem, threadIdx.x, [] { __syncthreads(); },
         [&](int r, int c, const float (&x)[4], float m, float l) {
             const int64_t row = row_of(r);
             *reinterpret_cast<float4 *>(px.o + row * D + c) = make_float4(x[0], x[1], x[2], x[3]);
@@ -52,54 +47,71 @@ __global__ void __launch_bounds__(kPkThreads, 2) prefix_ffma_kernel(const Packed
 
 // How the prefixes are cut: rows of a tile (sequences, or with FFMA sequences times heads), tiles a CTA, parts of the keys.
 struct PrefixPlan {
-    bool tc = false;
+    bool tc = false, few = false;  // few: FFMA tiles of 16 rows
     int tiles = 1, parts = 0;
-    int64_t rows = 0;  // of a CTA
+    int64_t room = 0;  // F32 on the tensor cores: positions a group in the planes
 };
-PrefixPlan prefix_plan(int64_t n_seqs, int64_t n_groups, int64_t max_prefix, int64_t G, int64_t Hkv, int32_t dtype) {
+constexpr size_t kPrefixMostPlanes = size_t(1) << 30;
+PrefixPlan prefix_plan(int64_t n_seqs, int64_t n_groups, int64_t max_prefix, int64_t D, int64_t G, int64_t Hkv, int32_t dtype) {
     PrefixPlan p;
     if (n_groups <= 0 || n_seqs <= 0 || max_prefix <= 0) return p;
-    p.tc = dtype != B200_DTYPE_F32 && G <= kPrefixTcRows;
-    // As if groups were alike. A group of more than one tile takes two a CTA, over the same keys.
-    const int64_t groups = min64(n_groups, n_seqs), each = (n_seqs + groups - 1) / groups, rows = p.tc ? each : each * G;
-    p.rows = p.tc ? kPrefixTcRows / G : kPkRows;
-    if (p.tc && rows > p.rows) p.tiles = 2;
-    p.rows *= p.tiles;
-    const int64_t ctas = groups * ((rows + p.rows - 1) / p.rows) * Hkv;
-    // As many parts as the CTAs that run at once allow, of two key tiles at least (one, where two tiles of rows alternate).
-    const int64_t keys = p.tc ? 256 / p.tiles : 2 * kPkKeys;
+    // As if groups were alike.
+    const int64_t groups = min64(n_groups, n_seqs), each = (n_seqs + groups - 1) / groups;
+    p.few = each * G <= 16;
+    p.tc = G <= kPrefixTcRows;
+    if (dtype == B200_DTYPE_F32 && p.tc) {
+        // F32 takes the tensor cores unless few rows meet short prefixes (16 / 8 heads of 128, whole calls, FFMA against tensor
+        // cores: 16 rows of 2000 keys 30.8 us against 31.8, 8 of 8192 94 against 83; 32 rows of 1000 35 against 28.5, 40 of 300 35
+        // against 28.7, 128 of 8192 180 against 86), or the planes, which are as long as the table, grow past a GiB.
+        p.room = (max_prefix + 127) / 128 * 128;
+        p.tc = !(p.few && max_prefix <= kPrefixShort) && n_groups <= INT32_MAX / p.room &&
+               p.room * n_groups <= static_cast<int64_t>(kPrefixMostPlanes / 8) / (D * Hkv);
+        if (!p.tc) p.room = 0;
+    }
+    int64_t rows = p.tc ? kPrefixTcRows / G : (p.few ? 16 : kPkRows);
+    // 16-bit types: a group of more than one tile takes two a CTA, over the same keys.
+    if (p.tc && dtype != B200_DTYPE_F32 && each > rows) p.tiles = 2;
+    rows *= p.tiles;
+    const int64_t ctas = groups * (((p.tc ? each : each * G) + rows - 1) / rows) * Hkv;
+    // As many parts as the CTAs that run at once allow, of two key tiles at least (one, where two tiles of rows alternate or are few).
+    const int64_t keys = p.tc ? 256 / p.tiles : (p.few ? kPkKeys : 2 * kPkKeys);
     const int64_t most = min64(kPrefixParts, (max_prefix + keys - 1) / keys);
     p.parts = static_cast<int>(max64(1, min64(most, device_sm_count() * (p.tc ? 1 : 2) / ctas)));
     return p;
 }
 
-size_t prefix_bytes(int64_t n_seqs, int64_t parts, int64_t D, int64_t Hq) {
-    return (static_cast<size_t>(parts) * n_seqs * Hq * (D * 4 + 8) + 15) / 16 * 16;
+// Bytes of the parts, and of the planes behind them.
+size_t prefix_parts_bytes(int64_t n_seqs, const PrefixPlan &p, int64_t D, int64_t Hq) {
+    return (static_cast<size_t>(p.parts) * n_seqs * Hq * (D * 4 + 8) + 127) / 128 * 128;
+}
+size_t prefix_bytes(int64_t n_seqs, int64_t n_groups, const PrefixPlan &p, int64_t D, int64_t Hq, int64_t Hkv) {
+    return prefix_parts_bytes(n_seqs, p, D, Hq) + (p.room ? prefix_planes_bytes(n_groups, p.room, D, Hkv) : 0);
 }
 
-template <typename T, int D>
+template <typename T, int D, int RT>
 cudaError_t prefix_ffma_launch(const PackedArgs &a, const PrefixArgs &px, cudaStream_t st) {
-    auto kern = prefix_ffma_kernel<T, D>;
+    auto kern = prefix_ffma_kernel<T, D, RT>;
     const cudaError_t e = once_per_device(reinterpret_cast<const void *>(kern), ATTR_SMEM, [&] {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ffma_smem<D>()));
     });
     if (e != cudaSuccess) return e;
-    const int64_t ctas = most_packed_tiles(px.n_groups, px.n_seqs, a.G, kPkRows) * a.Hkv * px.parts;
+    const int64_t ctas = most_packed_tiles(px.n_groups, px.n_seqs, a.G, 16 * RT) * a.Hkv * px.parts;
     if (ctas > INT32_MAX) return cudaErrorNotSupported;
     return b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPkThreads), ffma_smem<D>(), st, false, a, px);
 }
 
 template <typename T>
-cudaError_t prefix_ffma_by_dim(const PackedArgs &a, const PrefixArgs &px, cudaStream_t st) {
-    return a.D == 128 ? prefix_ffma_launch<T, 128>(a, px, st) : prefix_ffma_launch<T, 64>(a, px, st);
+cudaError_t prefix_ffma_by_dim(const PackedArgs &a, const PrefixArgs &px, bool few, cudaStream_t st) {
+    if (few) return a.D == 128 ? prefix_ffma_launch<T, 128, 1>(a, px, st) : prefix_ffma_launch<T, 64, 1>(a, px, st);
+    return a.D == 128 ? prefix_ffma_launch<T, 128, 4>(a, px, st) : prefix_ffma_launch<T, 64, 4>(a, px, st);
 }
 
-cudaError_t prefix_ffma_by_type(const PackedArgs &a, const PrefixArgs &px, cudaStream_t st) {
+cudaError_t prefix_ffma_by_type(const PackedArgs &a, const PrefixArgs &px, bool few, cudaStream_t st) {
     switch (a.dtype) {
-        case B200_DTYPE_F16: return prefix_ffma_by_dim<__half>(a, px, st);
-        case B200_DTYPE_BF16: return prefix_ffma_by_dim<__nv_bfloat16>(a, px, st);
+        case B200_DTYPE_F16: return prefix_ffma_by_dim<__half>(a, px, few, st);
+        case B200_DTYPE_BF16: return prefix_ffma_by_dim<__nv_bfloat16>(a, px, few, st);
     }
-    return prefix_ffma_by_dim<float>(a, px, st);
+    return prefix_ffma_by_dim<float>(a, px, few, st);
 }
 
 }  // namespace
@@ -114,7 +126,7 @@ size_t b200_flash_attn_paged_shared_workspace_bytes(int64_t n_seqs, int64_t max_
     if (n_seqs <= 0 || max_keys <= 0 || n_groups < 0 || max_prefix < 0 || D <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv ||
         !dtype_bytes(dtype))
         return 0;
-    return prefix_bytes(n_seqs, prefix_plan(n_seqs, n_groups, max_prefix, Hq / Hkv, Hkv, dtype).parts, D, Hq) +
+    return prefix_bytes(n_seqs, n_groups, prefix_plan(n_seqs, n_groups, max_prefix, D, Hq / Hkv, Hkv, dtype), D, Hq, Hkv) +
            paged_batch_prefix_bytes(n_seqs, max_keys, D, Hq / Hkv, Hkv, dtype);
 }
 
@@ -161,11 +173,13 @@ int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_
     px.n_groups = static_cast<int32_t>(n_groups);
     px.n_seqs = static_cast<int32_t>(n_seqs);
     px.Hq = static_cast<int32_t>(Hq);
-    const PrefixPlan plan = prefix_plan(n_seqs, n_groups, max_prefix, Hq / Hkv, Hkv, pool->dtype);
+    const PrefixPlan plan = prefix_plan(n_seqs, n_groups, max_prefix, D, Hq / Hkv, Hkv, pool->dtype);
     px.parts = plan.parts;
     px.tiles = plan.tiles;
     px.o = static_cast<float *>(workspace);
     px.ml = reinterpret_cast<float2 *>(px.o + px.parts * n_seqs * Hq * D);
+    px.room = plan.room;
+    px.planes = plan.room ? static_cast<char *>(workspace) + prefix_parts_bytes(n_seqs, plan, D, Hq) : nullptr;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (px.parts > 0) {
         PackedArgs p;
@@ -183,8 +197,8 @@ int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_
         p.sl2 = sl2;
         p.dtype = pool->dtype;
         p.status = dev_status;
-        cudaError_t rc2 = prefix_tc_launch(p, px, st);
-        if (rc2 == cudaErrorNotSupported) rc2 = prefix_ffma_by_type(p, px, st);
+        cudaError_t rc2 = plan.tc ? prefix_tc_launch(p, px, st) : cudaErrorNotSupported;
+        if (rc2 == cudaErrorNotSupported) rc2 = prefix_ffma_by_type(p, px, plan.few, st);
         if (rc2 != cudaSuccess) return status_of(rc2);
     }
     PbArgs a;
@@ -210,7 +224,7 @@ int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_
     a.sl2 = sl2;
     a.status = dev_status;
     return status_of(paged_batch_prefix_launch(a, px, Hkv, D, pool->dtype,
-                                               static_cast<char *>(workspace) + prefix_bytes(n_seqs, px.parts, D, Hq), st));
+                                               static_cast<char *>(workspace) + prefix_bytes(n_seqs, n_groups, plan, D, Hq, Hkv), st));
 }
 
 }  // extern "C"

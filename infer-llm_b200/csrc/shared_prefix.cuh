@@ -13,6 +13,9 @@ struct PrefixArgs {
     int64_t block_stride = 0, tok_stride = 0, head_stride = 0;       // of the pool, elements
     uint32_t bt = 1;
     int32_t n_groups = 0, n_seqs = 0, Hq = 0, parts = 0, tiles = 1;  // tiles: of rows, a CTA of the tensor-core kernel
+    // F32 on the tensor cores: K and V as planes of F16 numbers with room for `room` positions a group (a multiple of 128), then exponents
+    void *planes = nullptr;
+    int64_t room = 0;
     float *o = nullptr;    // [part][sequence][query head][D]
     float2 *ml = nullptr;  // [part][sequence][query head]: maximum, sum (-1: the group's prefix names a block out of range)
 };
@@ -51,13 +54,29 @@ B200_DEVICE bool prefix_bad(const PrefixArgs &a, int group, int from, int to, in
 // Tile `at` of M rows of the line of all groups' tiles, a row being a sequence with one of G heads; by a whole warp.
 B200_DEVICE PackedTile find_prefix_tile(const PrefixArgs &a, int G, int M, int64_t at) {
     return find_tile(a.cu, a.n_groups, a.n_seqs, G, M, at, nullptr, [&](int s, int64_t &k0, int &nk) {
-        k0 = 0;
+        k0 = s * a.room;
         nk = prefix_len(a, s);
         return true;
     });
 }
 
-// Tensor-core kernel of the prefixes for F16 and BF16; cudaErrorNotSupported (nothing launched) where it does not apply.
+// ffma_rows' keys of a prefix.
+template <typename T>
+struct PrefixKeys {
+    const T *k, *v;
+    const PrefixArgs &px;
+    int group, kvh;
+    B200_DEVICE PrefixKeys(const PackedArgs &a, const PrefixArgs &p, int g, int h)
+        : k(static_cast<const T *>(a.k)), v(static_cast<const T *>(a.v)), px(p), group(g), kvh(h) {}
+    B200_DEVICE bool operator()(int j, const T *&kr, const T *&vr) const {
+        const int64_t at = prefix_key(px, group, kvh, j);
+        kr = k + at, vr = v + at;
+        return at >= 0;
+    }
+};
+
+// Tensor-core kernel of the prefixes, F32 with `planes` of so many bytes; cudaErrorNotSupported (nothing launched) where it does not apply.
+size_t prefix_planes_bytes(int64_t n_groups, int64_t room, int64_t D, int64_t Hkv);
 cudaError_t prefix_tc_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st);
 constexpr int kPrefixTcRows = 128;  // of a tile: whole sequences times the heads of a KV head
 
