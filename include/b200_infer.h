@@ -371,8 +371,8 @@ size_t b200_flash_attn_paged_shared_workspace_bytes(int64_t n_seqs, int64_t max_
  *   bias: x + bias_values[i] for token bias_ids[i] (of several for one token the last counts);
  *   mask: a token whose bit (t % 32 of word t / 32 of the row's words) is 0 becomes -inf, whatever it was.
  * Row s has the history tokens [cu_tokens[s], cu_tokens[s + 1]) and the biases [cu_bias[s], cu_bias[s + 1]). Sums are F32, in
- * this order, rounded once to the type. out may be logits itself (with the same stride), and what does not
- * change is then neither read nor written where a mask allows it; else the two may not overlap. Any of tokens (with cu_tokens),
+ * this order, rounded once to the type. out may be logits itself (with the same stride), and without a mask only
+ * the tokens that the lists name are then read and written; else the two may not overlap. Any of tokens (with cu_tokens),
  * the three penalties (float32 [n_rows]; NULL: off), bias_ids (with bias_values and cu_bias) and mask may be NULL. Rows any
  * alignment; strides count elements (of mask: words). A token id out of range or offsets that are not ascending within the
  * given totals are left out and B200_DEV_BAD_TOKEN / B200_DEV_BAD_POSITION recorded; a repetition penalty
