@@ -661,9 +661,7 @@ int b200_flash_attn_paged_batch_q8(const void *q, int64_t q_seq_stride, int64_t 
     a.lens = seq_lens;
     a.table_stride = table_stride;
     a.bt = static_cast<uint32_t>(pool->block_tokens);
-    // for the least l with bt <= 2^l: ceil(2^(31 + l) / bt) is below 2^32 and exceeds the quotient by less than 1
-    for (a.bt_shift = 31; (1ull << (a.bt_shift - 31)) < a.bt;) ++a.bt_shift;
-    a.bt_mul = static_cast<uint32_t>(((1ull << a.bt_shift) + a.bt - 1) / a.bt);
+    reciprocal31(a.bt, a.bt_mul, a.bt_shift);
     a.max_keys = max_keys;
     a.n_seqs = static_cast<int>(n_seqs);
     a.G = static_cast<int>(Hq / Hkv);

@@ -135,6 +135,13 @@ inline int64_t most_packed_tiles(int64_t n_seqs, int64_t total_q, int64_t G, int
     return total_q * G / M + min64(n_seqs, total_q);
 }
 
+// x / d = x mul / 2^shift for x < 2^31, d >= 1: for the least l with d <= 2^l, ceil(2^(31 + l) / d) is below 2^32 and
+// its product exceeds the quotient by less than 1.
+inline void reciprocal31(uint32_t d, uint32_t &mul, uint32_t &shift) {
+    for (shift = 31; (1ull << (shift - 31)) < d;) ++shift;
+    mul = static_cast<uint32_t>(((1ull << shift) + d - 1) / d);
+}
+
 inline bool rows_aligned16(const void *p, int64_t s0, int64_t s1, int elem_bytes) {
     return ((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(s0 * elem_bytes) |
              static_cast<uintptr_t>(s1 * elem_bytes)) & 15) == 0;
