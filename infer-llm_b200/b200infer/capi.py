@@ -377,11 +377,12 @@ _host = None
 def _start(t):
     """(host, device index) for a call whose first tensor is t."""
     global _host
-    if not t.is_cuda:
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError("expected CUDA tensors")
     if _host is None:
         _host = _Host()
-    return _host, t.get_device()
+    return _host, dev
 
 
 def _elsewhere(fn, dev, *args, **kw):
@@ -400,13 +401,13 @@ def _dtype(t):
 def _rows(t, name, dtype, dev):
     """Checks a (rows, heads, D) tensor with a contiguous last axis; its shape and strides."""
     st = t.stride()
-    if len(st) != 3 or t.dtype != dtype or t.get_device() != dev or (st[2] != 1 and t.shape[2] != 1):
+    if len(st) != 3 or t.dtype is not dtype or t.get_device() != dev or (st[2] != 1 and t.shape[2] != 1):
         raise ValueError(f"{name}: expected (rows, heads, D) of {dtype} on cuda:{dev}, last axis contiguous")
     return st
 
 
 def _vector(t, name, n, dtype, dev):
-    if t.dtype != dtype or t.get_device() != dev or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name}: expected {n} contiguous {dtype} on cuda:{dev}")
     return t.data_ptr()
 
@@ -473,12 +474,12 @@ def _pool(k_pool, v_pool):
     return _POOL.pack(k_pool.data_ptr(), v_pool.data_ptr(), n, bt, s[0], s[1], s[2], Hkv, D, _dtype(k_pool)), bt, Hkv, D
 
 
-def _table(t, n, dev):
-    if t.dim() != 2 or t.shape[0] != n or t.dtype != _host.i32 or t.get_device() != dev or \
-            (t.stride(1) != 1 and t.shape[1] != 1):
-        raise ValueError(f"block_table: expected int32 ({n}, blocks) on cuda:{dev}")
+def _table(t, n, dev, name="block_table"):
+    st, shape = t.stride(), t.shape
+    if len(st) != 2 or shape[0] != n or t.dtype is not _host.i32 or t.get_device() != dev or (st[1] != 1 and shape[1] != 1):
+        raise ValueError(f"{name}: expected int32 ({n}, blocks) on cuda:{dev}")
     # a table of one row may report any stride; the rows must not overlap
-    return t.data_ptr(), t.stride(0) if n > 1 else t.shape[1], t.shape[1]
+    return t.data_ptr(), st[0] if n > 1 else shape[1], shape[1]
 
 
 def paged_kv_append(k, v, cu_new, seq_lens, k_pool, v_pool, block_table, status=None):
@@ -532,15 +533,16 @@ def flash_attn_paged_batch(q, k_pool, v_pool, block_table, seq_lens, scale=0.0, 
 
 
 def _pool_q8(k_pool, v_pool, k_scale, v_scale, dev):
-    h = _host
-    s, e = k_pool.stride(), k_scale.stride()
-    if len(s) != 4 or k_pool.dtype != h.e4m3 or v_pool.dtype != h.e4m3 or k_pool.shape != v_pool.shape or \
-            s != v_pool.stride() or s[3] != 1 or k_pool.get_device() != dev or v_pool.get_device() != dev:
+    e4m3, e8m0 = _host.e4m3, _host.e8m0
+    s, e, shape = k_pool.stride(), k_scale.stride(), k_pool.shape
+    if len(s) != 4 or s[3] != 1 or k_pool.dtype is not e4m3 or v_pool.dtype is not e4m3 or v_pool.shape != shape or \
+            v_pool.stride() != s or k_pool.get_device() != dev or v_pool.get_device() != dev:
         raise ValueError("k_pool, v_pool: expected two (blocks, block_tokens, Hkv, D) float8_e4m3fn tensors alike, last axis "
                          f"contiguous, on cuda:{dev}")
-    n, bt, Hkv, D = k_pool.shape
-    if k_scale.dtype != h.e8m0 or v_scale.dtype != h.e8m0 or k_scale.shape != (n, Hkv, bt) or v_scale.shape != (n, Hkv, bt) or \
-            e != v_scale.stride() or k_scale.get_device() != dev or v_scale.get_device() != dev:
+    n, bt, Hkv, D = shape
+    shape = (n, Hkv, bt)
+    if k_scale.dtype is not e8m0 or v_scale.dtype is not e8m0 or k_scale.shape != shape or v_scale.shape != shape or \
+            v_scale.stride() != e or k_scale.get_device() != dev or v_scale.get_device() != dev:
         raise ValueError(f"k_scale, v_scale: expected two (blocks, Hkv, block_tokens) float8_e8m0fnu tensors alike on cuda:{dev}")
     return _POOL_Q8.pack(k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, bt, s[0], s[1], s[2],
                          e[0], e[2], e[1], Hkv, D), bt, Hkv, D
@@ -556,8 +558,8 @@ def paged_kv_append_q8(k, v, cu_new, seq_lens, k_pool, v_pool, k_scale, v_scale,
     kind, dt = k.dtype, _dtype(k)
     pool, _, Hkv, D = _pool_q8(k_pool, v_pool, k_scale, v_scale, dev)
     ks, vs = _rows(k, "k", kind, dev), _rows(v, "v", kind, dev)
-    T = k.shape[0]
-    if k.shape != v.shape or k.shape[1] != Hkv or k.shape[2] != D:
+    T, heads, dim = shape = k.shape
+    if v.shape != shape or heads != Hkv or dim != D:
         raise ValueError("k, v: expected (T, Hkv, D)")
     n = seq_lens.shape[0]
     table, stride, blocks = _table(block_table, n, dev)
@@ -579,13 +581,15 @@ def paged_kv_read_q8(cu_rows, seq_lens, n_rows, k_pool, v_pool, k_scale, v_scale
                           k, v, status)
     pool, _, Hkv, D = _pool_q8(k_pool, v_pool, k_scale, v_scale, dev)
     if k is None and v is None:
-        kind = dtype or h.torch.bfloat16
-        k = h.empty((n_rows, Hkv, D), device=k_pool.device, dtype=kind)
+        k = h.empty((n_rows, Hkv, D), device=k_pool.device, dtype=dtype or h.torch.bfloat16)
         v = h.empty_like(k)
+        dt = _dtype(k)
+        ks = vs = (Hkv * D, D)
     elif k is None or v is None or k.shape != v.shape or k.shape != (n_rows, Hkv, D) or (dtype or k.dtype) != k.dtype:
         raise ValueError("k, v: expected both (n_rows, Hkv, D), of `dtype`")
-    kind, dt = k.dtype, _dtype(k)
-    ks, vs = _rows(k, "k", kind, dev), _rows(v, "v", kind, dev)
+    else:
+        kind, dt = k.dtype, _dtype(k)
+        ks, vs = _rows(k, "k", kind, dev), _rows(v, "v", kind, dev)
     n = seq_lens.shape[0]
     table, stride, blocks = _table(block_table, n, dev)
     _chk("b200_paged_kv_read_q8", h.read_q8(
@@ -639,7 +643,7 @@ def flash_attn_paged_shared(q, k_pool, v_pool, prefix_table, prefix_lens, cu_seq
         raise ValueError("q: shape does not go with the pools")
     groups = prefix_lens.shape[0]
     table, stride, blocks = _table(block_table, n, dev)
-    ptable, pstride, pblocks = _table(prefix_table, groups, dev)
+    ptable, pstride, pblocks = _table(prefix_table, groups, dev, "prefix_table")
     out = _out_rows(out, q, dev)
     os = out.stride()
     nbytes = h.shared_bytes(n, blocks * bt, groups, pblocks * bt, D, Hq, Hkv, dt)
