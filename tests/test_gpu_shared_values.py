@@ -1,0 +1,167 @@
+"""Shared-prefix attention with groups that fill tiles of rows (the tensor-core kernels of every type): values that are no
+numbers, magnitudes that spread, hidden content, bad blocks, group sizes. Bounds as in test_gpu_shared.py."""
+import math
+
+import pytest
+import torch
+
+import b200infer as B
+from test_gpu_shared import BAD_POSITION, DT, Batch, check, ints
+
+pytestmark = pytest.mark.gpu
+
+MANY = dict(prefix=[700, 130], seqs=[40, 11], lens=[(i * 29) % 60 for i in range(51)])
+
+
+def many(layout, kind, seed, block=16):
+    return Batch(MANY["prefix"], MANY["seqs"], MANY["lens"], block, layout, kind, seed)
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout", ["g2", "g4", "g2d64", "g16"])
+def test_nan_keys(cuda, kind, layout):
+    """A NaN in a prefix's key reaches its group's rows of that KV head alone, at any place in a tile."""
+    b = many(layout, kind, 3)
+    want, w = b.want()
+    Hq, Hkv = b.q.shape[1], b.k.shape[2]
+    G, h = Hq // Hkv, Hkv - 1
+    for place in (0, 1, 130, 255, 698, 699):
+        keep = b.k.clone()
+        b.k[b.prefix_table[0, place // 16], place % 16, h, 7] = math.nan
+        got = B.flash_attn_paged_shared(*b.args())
+        odd = torch.zeros(got.shape[:2], dtype=torch.bool, device=cuda)
+        odd[:40, h * G:] = True
+        assert torch.isnan(got[odd]).all()
+        check(got[~odd], want[~odd], w[~odd], kind)
+        b.k = keep
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout", ["g2", "g2d64"])
+def test_infinite_values(cuda, kind, layout):
+    """An infinite element of V, of a prefix or of a sequence, makes that column of the rows that see it infinite."""
+    b = many(layout, kind, 5)
+    b.v[b.prefix_table[0, 2], 5, 1, 9] = math.inf
+    b.v[b.prefix_table[1, 8], 1, 0, 3] = -math.inf
+    b.v[b.table[7, 0], 0, 0, 60] = math.inf
+    want, w = b.want()
+    got = B.flash_attn_paged_shared(*b.args())
+    fine = torch.isfinite(want)
+    assert int((~fine).sum()) == (40 + 11 + 1) * b.q.shape[1] // b.k.shape[2]
+    assert torch.equal(got.double()[~fine], want[~fine])
+    w = torch.where(fine, w, 0.0)
+    check(torch.where(fine, got.double(), 0.0).to(DT[kind]), torch.where(fine, want, 0.0), w, kind)
+
+
+@pytest.mark.parametrize("kind", list(DT))
+def test_scores_of_minus_infinity(cuda, kind):
+    """Keys with scores of -inf count for nothing, and a row that has only such keys is zero."""
+    b = Batch([256, 100], [40, 3], [(i * 7) % 5 for i in range(43)], 16, "g2", kind, 7)
+    b.q.fill_(1.0)
+    b.k[b.prefix_table[0].long()] = -math.inf
+    got = B.flash_attn_paged_shared(*b.args())
+    b.prefix[0] = 0
+    want, w = b.want()
+    check(got, want, w, kind)
+    assert (got[0] == 0).all()
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout", ["g2", "g4", "g2d64"])
+@pytest.mark.parametrize("block", [16, 100, 7, 128, 1, 6])
+def test_hidden_content(cuda, kind, layout, block):
+    """What lies behind the ends, in last blocks and unused ones, does not count, whatever it is; blocks of any size."""
+    b = many(layout, kind, 9, block)
+    want = b.want()
+    used = torch.zeros(b.k.shape[:2], dtype=torch.bool, device=cuda)
+    for table, lens in ((b.prefix_table, b.prefix), (b.table, b.own)):
+        for i, n in enumerate(lens):
+            pos = torch.arange(n, device=cuda)
+            used[table[i].long()[pos // block], pos % block] = True
+    for bad in (math.nan, math.inf, -math.inf):
+        b.k[~used] = bad
+        b.v[~used] = bad
+        check(B.flash_attn_paged_shared(*b.args()), *want, kind)
+
+
+@pytest.mark.parametrize("layout", ["g2", "g2d64", "g16"])
+def test_spread_magnitudes(cuda, layout):
+    """F32 columns, keys and values whose magnitudes differ by far more than one exponent holds."""
+    b = many(layout, "f32", 11)
+    b.v[..., 3] *= 2.0 ** -40
+    b.k[b.prefix_table[0, 5]] *= 2.0 ** -30
+    b.v[b.prefix_table[0, 6]] *= 2.0 ** 30
+    want, _ = b.want()
+    got = B.flash_attn_paged_shared(*b.args())
+    for rows in (slice(0, 40), slice(40, 51)):  # each group and column by its own magnitude
+        for d in (3, 4):
+            x, y = got[rows, :, d].double(), want[rows, :, d]
+            assert ((x - y).abs() <= 1e-5 * (y.abs() + float(y.square().mean().sqrt()))).all()
+
+
+@pytest.mark.parametrize("kind", list(DT))
+def test_bad_blocks(cuda, kind):
+    """A block out of range anywhere in a prefix clears its group's rows, whichever part of the keys it falls into."""
+    b = many("g4", kind, 13)
+    want, w = b.want()
+    status = ints([0])
+    for at in (0, 20, 43):
+        keep = int(b.prefix_table[0, at])
+        for bad in (-1, b.k.shape[0], 2 ** 31 - 1):
+            b.prefix_table[0, at] = bad
+            status.zero_()
+            got = B.flash_attn_paged_shared(*b.args(), status=status)
+            assert int(status) == BAD_POSITION and (got[:40] == 0).all()
+            check(got[40:], want[40:], w[40:], kind)
+        b.prefix_table[0, at] = keep
+    status.zero_()
+    check(B.flash_attn_paged_shared(*b.args(), status=status), want, w, kind)
+    assert int(status) == 0
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout", ["g2", "g3", "g16"])
+@pytest.mark.parametrize("seqs", [[64, 1], [65], [7] * 20, [0, 33, 0, 0, 2], [129, 63, 64]])
+def test_group_sizes(cuda, kind, layout, seqs):
+    """Groups of a tile's rows, one more, many small ones, empty ones."""
+    n = sum(seqs)
+    b = Batch([(i * 97) % 300 for i in range(len(seqs))], seqs, [(i * 13) % 40 for i in range(n)], 16, layout, kind, 15)
+    check(B.flash_attn_paged_shared(*b.args()), *b.want(), kind)
+
+
+@pytest.mark.parametrize("kind", list(DT))
+def test_many_heads_share_keys(cuda, kind):
+    """More query heads a KV head than a tile has rows."""
+    g = torch.Generator(device="cuda").manual_seed(17)
+    b = Batch([150], [3], [20, 0, 5], 16, "g20", kind, 17)
+    b.q = torch.randn((3, 150, 64), device=cuda, generator=g).to(DT[kind])
+    check(B.flash_attn_paged_shared(*b.args()), *b.want(), kind)
+
+
+@pytest.mark.parametrize("kind", list(DT))
+def test_wide_tables(cuda, kind):
+    """Tables far wider than the prefixes in them (F32: too wide for planes, so F32 arithmetic)."""
+    b = many("g2", kind, 19)
+    wide = torch.full((2, 200000 if kind == "f32" else 3000), -1, dtype=torch.int32, device=cuda)
+    wide[:, :b.prefix_table.shape[1]] = b.prefix_table
+    b.prefix_table = wide
+    check(B.flash_attn_paged_shared(*b.args()), *b.want(), kind)
+
+
+@pytest.mark.parametrize("kind", list(DT))
+def test_in_a_graph(cuda, kind):
+    b = many("g2", kind, 21)
+    a = [t.clone() for t in b.args()]
+    B.flash_attn_paged_shared(*a)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = B.flash_attn_paged_shared(*a)
+    for lens in ([700, 130], [1, 0], [128, 129]):
+        b.prefix = lens
+        a[4].copy_(ints(lens))
+        a[0].copy_(a[0].flip(0))
+        b.q = a[0]
+        for _ in range(2):
+            graph.replay()
+        check(out, *b.want(), kind)
