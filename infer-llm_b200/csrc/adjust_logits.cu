@@ -104,7 +104,9 @@ __global__ void __launch_bounds__(kAdThreads, kAdCtas) adjust_logits_kernel(cons
     int64_t bias_from = 0;
     const int32_t *tokens = nullptr, *biases = nullptr;
     int n = 0, m = 0, prompt = 0;
-    const uint32_t least = static_cast<uint32_t>(max(begin, 0)), span = static_cast<uint32_t>(min(begin + steps * kStep, a.vocab)) - least;
+    // (a last chunk that only another alignment needs begins behind the row: its span is nothing)
+    const uint32_t least = static_cast<uint32_t>(max(begin, 0));
+    const uint32_t span = static_cast<uint32_t>(max(0, min(begin + steps * kStep, a.vocab) - max(begin, 0)));
     const auto in_chunk = [&](int t) { return static_cast<uint32_t>(t) - least < span; };
     const auto count = [&](int first) {
         for (int i = tid; i < min(total - first, kAdSlots); i += kAdWalk) known[i] = bias[i] = 0;

@@ -216,6 +216,23 @@ def test_out_of_range(cuda):
         assert int(status) == BAD_LOGITS
 
 
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("vocab", [4089, 4093, 4094, 4095, 4096, 8191, 16379, 16383])
+@pytest.mark.parametrize("n", [1, 600])
+def test_ids_behind_a_row_that_ends_with_a_chunk(cuda, kind, vocab, n):
+    """Ids past the vocabulary touch neither their row nor what lies behind it, where a chunk begins behind the row's end too."""
+    x = torch.randn((n + 8, vocab), device=cuda, generator=gen(23)).to(DT[kind])
+    out = torch.full_like(x, 7.0)
+    ids = [vocab, vocab + 1, vocab + 100, vocab + 5000, 2 ** 31 - 1, -1, -2 ** 31, 3]
+    t, cu = pack([ids] * n)
+    status = ints([0])
+    B.adjust_logits(x[:n], t, cu, presence=floats([1.0] * n), bias_ids=t, bias_values=floats([2.0] * len(t)), cu_bias=cu,
+                    out=out[:n], status=status)
+    assert int(status) == BAD_TOKEN
+    check(out[:n], *expected(x[:n], [[3]] * n, [0] * n, [1.0] * n, [0.0] * n, [1.0] * n, [[(3, 2.0)]] * n, None), x[:n])
+    assert (out[n:] == 7.0).all()
+
+
 def test_prompt_lengths_past_the_history(cuda):
     x = torch.randn((3, 50), device=cuda, generator=gen(20))
     h = [[1, 1, 2], [3], [4, 4]]
