@@ -207,7 +207,7 @@ struct P8State {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const float y = FULL ? s[0][j][2 * r + u] : s[0][j][u] + s[NS - 1][j][2 + u];
-                    x[j][u] = y * qs[r] * ke[j][u];
+                    x[j][u] = y * (qs[r] * ke[j][u]);  // (a large row of Q against small keys, or the inverse, stays in range)
                     if (live != ~0u && !((live >> (8 * j + t2 + u)) & 1u)) x[j][u] = -INFINITY;
                     mx = fmaxf(mx, x[j][u]);
                     nx = fmaxf(nx, x[j][u] + ve[j][u]);

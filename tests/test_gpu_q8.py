@@ -311,8 +311,9 @@ def decode_want(c, q, scale=None):
 
 @pytest.mark.parametrize("kind", list(DT))
 @pytest.mark.parametrize("layout", list(LAYOUTS))
-@pytest.mark.parametrize("block,lens", [(16, [1]), (16, [301]), (8, [5, 0, 1, 64, 33, 129, 1000]), (100, [77, 2500, 0, 100])],
-                         ids=["single", "one", "ragged", "pages_of_100"])
+@pytest.mark.parametrize("block,lens", [(16, [1]), (16, [301]), (8, [5, 0, 1, 64, 33, 129, 1000]), (100, [77, 2500, 0, 100]),
+                                        (1, [40, 3]), (5000, [4999, 2])],
+                         ids=["single", "one", "ragged", "pages_of_100", "pages_of_one", "one_page"])
 def test_decode(cuda, kind, layout, block, lens):
     Hq, Hkv, D = LAYOUTS[layout]
     c = filled(lens, block, Hkv, D, 21, kind)
@@ -364,6 +365,20 @@ def test_decode_growing_scores_and_spread_magnitudes(cuda, layout):
     got, want = B.flash_attn_paged_batch_q8(q, *c.args, c.table, c.seq_lens), decode_want(c, q)
     for s in range(3):
         check(got[s], want[s], "f32")
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("layout", ["g2", "g2d64", "g16"])
+@pytest.mark.parametrize("up", [105, -105])
+def test_decode_large_rows_of_q_with_small_keys(cuda, kind, layout, up):
+    """Rows of Q and keys at the two ends of the exponents' range, whose products lie in its middle."""
+    Hq, Hkv, D = LAYOUTS[layout]
+    g = gen(60)
+    c = Cache([300, 17], 16, Hkv, D, 61)
+    k, v = (torch.randn((317, Hkv, D), device=cuda, generator=g) for _ in range(2))
+    c.fill(k * 2.0 ** -up, v, cumulative(c.lens))
+    q = (torch.randn((2, Hq, D), device=cuda, generator=g) * 2.0 ** up).to(DT[kind])
+    check(B.flash_attn_paged_batch_q8(q, *c.args, c.table, c.seq_lens), decode_want(c, q), kind)
 
 
 def test_decode_light_keys_with_large_values(cuda):
