@@ -381,6 +381,39 @@ B200_DEVICE void report_groups(const PrefixArgs &px, int32_t *status) {
     }
 }
 
+// The CTAs' shares of the line of `total` units: with prefixes, the first `early` CTAs, which run beside the prefixes' kernel on SMs of their
+// own, take `gap` units more than those that start when it ends, or all where that is enough for them. CTA c takes
+// the units [begin(c), begin(c + 1)), TU of them at least.
+struct Shares {
+    int64_t total, ctas, early, gap;
+    B200_DEVICE int64_t line() const { return total + (ctas - early) * gap; }  // the late CTAs' gaps as units that hold nothing
+    B200_DEVICE int64_t begin(int64_t c) const {
+        return (line() * c - (c > early ? ctas * gap * (c - early) : 0)) / ctas;
+    }
+    B200_DEVICE int64_t owner(int64_t u) const {
+        const int64_t c = share_owner(line(), u, ctas);
+        return c < early ? c : ((u + 1) * ctas - ctas * gap * early - 1) / (line() - ctas * gap);
+    }
+};
+template <int TU>
+B200_DEVICE Shares prefix_shares(const PrefixArgs &px, int64_t total, int64_t grid) {  // by a whole warp
+    constexpr int kLate = 8;  // units that a late CTA takes at least, for its start
+    Shares s = {total, min64(grid, total / TU), 0, 0};
+    if (px.early <= 0 || px.early >= s.ctas) return s;
+    int longest = 0;
+    for (int g = threadIdx.x & 31; g < px.n_groups; g += 32) longest = max(longest, prefix_len(px, g));
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    const int64_t tiles = (static_cast<int64_t>(longest) + 127) / 128;
+    const int64_t gap = tiles ? px.gap_start + px.gap_tile * ((tiles + px.parts - 1) / px.parts) : 0;
+    if (total <= px.early * (gap + kLate)) {
+        s.ctas = min64(px.early, s.ctas);
+    } else if (total >= s.ctas * kLate) {
+        s.early = px.early;
+        s.gap = min64(gap, (total - s.ctas * kLate) / px.early);
+    }
+    return s;
+}
+
 // CL: a cluster of kCluster CTAs takes one pair, and writes its output. PX: there are prefixes to join.
 template <typename T, int D, int HB, bool CL, bool PX>
 __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid_constant__ PbArgs a, const __grid_constant__ PrefixArgs px) {
@@ -412,13 +445,14 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
     } else {
         grid_launch_dependents();  // the joining kernel waits for this grid's end
         const int64_t total = tiles_before<Ge::kTile, kTileUnits<PX>, kPairUnits<PX>>(a, a.n_seqs) * a.VH;
-        const int64_t ctas = min64(gridDim.x, total / kTileUnits<PX>);
-        if (blockIdx.x >= ctas) {
+        Shares shares = {total, min64(gridDim.x, total / kTileUnits<PX>), 0, 0};
+        if constexpr (PX) shares = prefix_shares<kTileUnits<PX>>(px, total, gridDim.x);
+        if (blockIdx.x >= shares.ctas) {
             if (PX && blockIdx.x == gridDim.x - 1) grid_wait();
             return;
         }
-        u0 = share_begin(total, blockIdx.x, ctas);
-        u1 = share_begin(total, blockIdx.x + 1, ctas);
+        u0 = PX ? shares.begin(blockIdx.x) : share_begin(total, blockIdx.x, shares.ctas);
+        u1 = PX ? shares.begin(blockIdx.x + 1) : share_begin(total, blockIdx.x + 1, shares.ctas);
         at = place_at<Ge::kTile, kTileUnits<PX>, kPairUnits<PX>>(a, u0, u1);
     }
     const Place start = at;
@@ -693,7 +727,7 @@ __global__ void __launch_bounds__(kPxJoinThreads) paged_batch_prefix_join_kernel
     constexpr int TU = kTileUnits<true>, PU = kPairUnits<true>;
     const int64_t before = tiles_before<Ge::kTile, TU, PU>(a, b);
     const int64_t total = tiles_before<Ge::kTile, TU, PU>(a, a.n_seqs) * a.VH;
-    const int64_t ctas = min64(grid, total / TU);  // as in the main kernel
+    const Shares shares = prefix_shares<TU>(px, total, grid);  // as in the main kernel
     const int tiles = seq_tiles<Ge::kTile>(a, b), group = prefix_group(px, b);
     const int h0 = (vh / a.HG) * a.G + (vh % a.HG) * HB;
     const int heads = min(HB, a.G - (vh % a.HG) * HB);
@@ -704,8 +738,8 @@ __global__ void __launch_bounds__(kPxJoinThreads) paged_batch_prefix_join_kernel
     int parts = 0;  // CTAs c0 .. c0 + parts - 1 hold parts; the first's begins with the pair
     if (tiles > 0) {
         const int64_t ua = before * a.VH + vh * units_of<TU, PU>(tiles);
-        c0 = share_owner(total, ua, ctas);
-        parts = static_cast<int>(share_owner(total, ua + (tiles - 1) * TU, ctas) - c0) + 1;
+        c0 = shares.owner(ua);
+        parts = static_cast<int>(shares.owner(ua + (tiles - 1) * TU) - c0) + 1;
     }
     grid_wait();
     const float *first = parts == 1 ? a.whole + static_cast<int64_t>(blockIdx.x) * Ge::kRecAt : a.ws + (c0 * 2 + 1) * Ge::kRecAt;

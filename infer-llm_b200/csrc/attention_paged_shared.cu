@@ -9,9 +9,9 @@
 //    is cut into as many parts as fill the SMs.
 //  * the sequences' own keys, as in the batched decode (attention_paged_batch.cu);
 //  * the join of all parts.
-// 64 BF16 sequences of 32 / 8 heads of 128 behind one prefix of 8192 keys, with 33 k keys of their own (165 MB): 57 us, of which the
-// prefixes ~22, own keys ~27 and the join ~8. A prefix CTA takes an SM's shared memory, so own keys wait for it (a small one beside them 61
-// against 63, but 56 against 47 behind 16384 keys). 8 F32 sequences behind 301 keys: 20 us, 14 of them the FFMA tiles' chain.
+// 64 BF16 sequences of 32 / 8 heads of 128 behind one prefix of 8192 keys, with 33 k keys of their own (165 MB): 46 us, of which the
+// join 5 to 6 after the own keys' end. A prefix CTA takes an SM's shared memory, so own keys run on the SMs that the plan leaves them (a small
+// CTA beside theirs took 61 against 63, but 56 against 47 behind 16384 keys). 8 F32 sequences behind 301 keys: 20 us, 14 of them the FFMA tiles' chain.
 #include "attention_packed_ffma.cuh"
 #include "paged_batch.cuh"
 
@@ -53,9 +53,16 @@ struct PrefixPlan {
     bool tc = false, few = false;  // few: FFMA tiles of 16 rows
     int tiles = 1, parts = 0;
     int64_t room = 0;  // F32 on the tensor cores: positions a group in the planes
+    int64_t early = 0;  // CTAs of the own keys that the prefixes' SMs leave room for
 };
+// Model of the tensor-core kernel and of the own keys' (us, kB a us): what a CTA's start and end and a tile of 128 keys take, and the rate of
+// own keys on all SMs.
+constexpr float kPxStart = 8.f, kPxStartF32 = 16.f, kPxTile = 2.2f, kPxOwnRate = 4500.f;
+// The same start and tile in units of the own keys' line (0.7 us).
+constexpr int kGapStart = 10, kGapStartF32 = 20, kGapTile = 3;
 constexpr size_t kPrefixMostPlanes = size_t(1) << 30;
-PrefixPlan prefix_plan(int64_t n_seqs, int64_t n_groups, int64_t max_prefix, int64_t D, int64_t G, int64_t Hkv, int32_t dtype) {
+PrefixPlan prefix_plan(int64_t n_seqs, int64_t max_keys, int64_t n_groups, int64_t max_prefix, int64_t D, int64_t G, int64_t Hkv,
+                       int32_t dtype) {
     PrefixPlan p;
     if (n_groups <= 0 || n_seqs <= 0 || max_prefix <= 0) return p;
     // As if groups were alike.
@@ -79,7 +86,22 @@ PrefixPlan prefix_plan(int64_t n_seqs, int64_t n_groups, int64_t max_prefix, int
     // As many parts as the CTAs that run at once allow, of two key tiles at least (one, where two tiles of rows alternate or are few).
     const int64_t keys = p.tc ? 256 / p.tiles : (p.few ? kPkKeys : 2 * kPkKeys);
     const int64_t most = min64(kPrefixParts, (max_prefix + keys - 1) / keys);
-    p.parts = static_cast<int>(max64(1, min64(most, device_sm_count() * (p.tc ? 1 : 2) / ctas)));
+    const int64_t sms = device_sm_count(), room = max64(1, min64(most, (p.tc ? sms * 3 / 4 : 2 * sms) / ctas));
+    p.parts = static_cast<int>(room);
+    if (!p.tc) return p;
+    // Own keys run beside the prefixes on the SMs that these leave. The fewest parts with which the prefixes end before their
+    // keys do, as if own lengths were half of what the table holds: fewer starts, and less to join. (Whole calls with all, 112, 80, 56, 40 and
+    // 24 SMs for the prefixes, the rule's last: 64 BF16 sequences behind 8192 keys with 33 k of their own 57, 53, 49.5, 49, 45, 61.5; 46.
+    // 16 behind 4096 with 16 k 37, 36, 33, 30, 29, 35; 29.6. 64 behind 16384 with one each 47, 41, 47, 57, 73, 107; 41.)
+    const float own = 0.5f * n_seqs * max_keys * Hkv * D * (dtype == B200_DTYPE_F32 ? 8 : 4) * 1e-3f / kPxOwnRate;
+    const int64_t key_tiles = (max_prefix + 127) / 128;
+    for (int64_t parts = 1; parts < room; ++parts) {
+        const float t = (dtype == B200_DTYPE_F32 ? kPxStartF32 : kPxStart) + kPxTile * ((key_tiles + parts - 1) / parts);
+        if (t > 0.9f * (own + t * ctas * parts / sms)) continue;
+        p.parts = static_cast<int>(parts);
+        break;
+    }
+    p.early = 2 * max64(0, sms - ctas * p.parts);
     return p;
 }
 
@@ -98,7 +120,7 @@ cudaError_t prefix_ffma_launch(const PackedArgs &a, const PrefixArgs &px, cudaSt
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ffma_smem<D>()));
     });
     if (e != cudaSuccess) return e;
-    const int64_t ctas = most_packed_tiles(px.n_groups, px.n_seqs, a.G, 16 * RT) * a.Hkv * px.parts;
+    const int64_t ctas = most_prefix_tiles(px.n_groups, px.n_seqs, a.G, 16 * RT) * a.Hkv * px.parts;
     if (ctas > INT32_MAX) return cudaErrorNotSupported;
     return b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPkThreads), ffma_smem<D>(), st, false, a, px);
 }
@@ -129,7 +151,7 @@ size_t b200_flash_attn_paged_shared_workspace_bytes(int64_t n_seqs, int64_t max_
     if (n_seqs <= 0 || max_keys <= 0 || n_groups < 0 || max_prefix < 0 || D <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv ||
         !dtype_bytes(dtype))
         return 0;
-    return prefix_bytes(n_seqs, n_groups, prefix_plan(n_seqs, n_groups, max_prefix, D, Hq / Hkv, Hkv, dtype), D, Hq, Hkv) +
+    return prefix_bytes(n_seqs, n_groups, prefix_plan(n_seqs, max_keys, n_groups, max_prefix, D, Hq / Hkv, Hkv, dtype), D, Hq, Hkv) +
            paged_batch_prefix_bytes(n_seqs, max_keys, D, Hq / Hkv, Hkv, dtype);
 }
 
@@ -176,9 +198,12 @@ int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_
     px.n_groups = static_cast<int32_t>(n_groups);
     px.n_seqs = static_cast<int32_t>(n_seqs);
     px.Hq = static_cast<int32_t>(Hq);
-    const PrefixPlan plan = prefix_plan(n_seqs, n_groups, max_prefix, D, Hq / Hkv, Hkv, pool->dtype);
+    const PrefixPlan plan = prefix_plan(n_seqs, max_keys, n_groups, max_prefix, D, Hq / Hkv, Hkv, pool->dtype);
     px.parts = plan.parts;
     px.tiles = plan.tiles;
+    px.early = static_cast<int32_t>(plan.early);
+    px.gap_start = pool->dtype == B200_DTYPE_F32 ? kGapStartF32 : kGapStart;
+    px.gap_tile = kGapTile;
     px.o = static_cast<float *>(workspace);
     px.ml = reinterpret_cast<float2 *>(px.o + px.parts * n_seqs * Hq * D);
     px.room = plan.room;
@@ -201,7 +226,10 @@ int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_
         p.dtype = pool->dtype;
         p.status = dev_status;
         cudaError_t rc2 = plan.tc ? prefix_tc_launch(p, px, st) : cudaErrorNotSupported;
-        if (rc2 == cudaErrorNotSupported) rc2 = prefix_ffma_by_type(p, px, plan.few, st);
+        if (rc2 == cudaErrorNotSupported) {
+            px.early = 0;
+            rc2 = prefix_ffma_by_type(p, px, plan.few, st);
+        }
         if (rc2 != cudaSuccess) return status_of(rc2);
     }
     PbArgs a;

@@ -16,6 +16,9 @@ struct PrefixArgs {
     // F32 on the tensor cores: K and V as planes of F16 numbers with room for `room` positions a group (a multiple of 128), then exponents
     void *planes = nullptr;
     int64_t room = 0;
+    // CTAs of the own keys that run beside the prefixes' kernel, and how much longer than the others: units of their line of tiles, of the
+    // prefix kernel's start and of each key tile of its longest part
+    int32_t early = 0, gap_start = 0, gap_tile = 0;
     float *o = nullptr;    // [part][sequence][query head][D]
     float2 *ml = nullptr;  // [part][sequence][query head]: maximum, sum (-1: the group's prefix names a block out of range)
 };
@@ -50,6 +53,11 @@ B200_DEVICE bool prefix_bad(const PrefixArgs &a, int group, int from, int to, in
         bad |= blk < 0 || blk >= a.n_blocks;
     }
     return bad;
+}
+// At most so many tiles of M rows in all groups, a sequence being G rows.
+inline int64_t most_prefix_tiles(int64_t n_groups, int64_t n_seqs, int64_t G, int64_t M) {
+    const int64_t groups = min64(n_groups, n_seqs);
+    return groups + (n_seqs * G - groups) / M;
 }
 // Tile `at` of M rows of the line of all groups' tiles, a row being a sequence with one of G heads; by a whole warp.
 B200_DEVICE PackedTile find_prefix_tile(const PrefixArgs &a, int G, int M, int64_t at) {

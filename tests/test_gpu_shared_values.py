@@ -165,3 +165,17 @@ def test_in_a_graph(cuda, kind):
         for _ in range(2):
             graph.replay()
         check(out, *b.want(), kind)
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout", ["g2", "g2d64", "g16"])
+def test_long_and_short_own_keys_beside_prefixes(cuda, kind, layout):
+    """Any split of the work between the prefixes' kernel and the own keys', whose shares depend on the lengths alone."""
+    full = [(i * 389) % 2500 for i in range(48)]
+    b = Batch([8000, 300], [37, 9], full, 16, layout, kind, 23)
+    a = list(b.args())
+    for prefix in ([8000, 300], [1000, 300], [1, 0], [0, 129]):
+        for own in (full, [0] * 48, [min(n, 1) for n in full], [min(n, 130) for n in full], [n if i % 16 == 5 else 0 for i, n in enumerate(full)]):
+            b.prefix, b.own = prefix, own
+            a[4], a[7] = ints(prefix), ints(own)
+            check(B.flash_attn_paged_shared(*a), *b.want(), kind)
