@@ -322,17 +322,19 @@ B200_DEVICE void split_f16x2(uint64_t v, uint32_t &hi, uint32_t &lo) {
     lo = *reinterpret_cast<const uint32_t *>(&r);
 }
 
-constexpr int kSplitThreads = 256;
+template <int D>
+constexpr int kSplitThreads = 4 * D;  // a thread holds eight float4 of the tile
 
 // One CTA: the K or V rows of one key tile and KV head, as hi and lo planes with the tile's
 // exponent, and whether its rows and columns spread too far for one. A pass over the bytes: HBM bounds it (2048 keys, 8 heads of 128: 17 MB in, 17 MB out, 7 us
-// with its launch; the attention kernel's start overlaps it).
-// PX: of a prefix's blocks, tile after tile of a group's room.
+// with its launch; the attention kernel's start overlaps it). All loads come before the first reduction, which would else wait for each.
+// PX: of a prefix's blocks, tile after tile of a group's room, read past L2's room for the planes (8192 keys, 8 heads of 128, 67 MB in and out:
+// 31 us; with half the threads 33, with loads and reductions in one loop 42, both 47; with twice the threads 45).
 template <int D, bool PX>
-__global__ void __launch_bounds__(kSplitThreads)
+__global__ void __launch_bounds__(kSplitThreads<D>, 256 / D)
     packed_split_kernel(const PackedArgs a, const PrefixArgs px, __half *planes, int32_t *exps) {
-    constexpr int V4 = D / 4, PER = kPtKeys * V4 / kSplitThreads;  // float4 a row, a thread
-    constexpr int W = kSplitThreads / 32;
+    constexpr int V4 = D / 4, PER = kPtKeys * V4 / kSplitThreads<D>;  // float4 a row, a thread
+    constexpr int W = kSplitThreads<D> / 32;
     __shared__ uint32_t warp_top[W], warp_low[W], warp_any[W], col_top[W][D], col_low[D / 32];
     grid_launch_dependents();
     const int kvh = (blockIdx.x >> 1) % a.Hkv, is_v = blockIdx.x & 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -362,19 +364,22 @@ __global__ void __launch_bounds__(kSplitThreads)
     constexpr int RW = 32 / V4;
     int64_t where = -1;
     if constexpr (PX) {
-        const int r = warp * RW + lane % RW + lane / RW * (kSplitThreads / V4);
+        const int r = warp * RW + lane % RW + lane / RW * (kSplitThreads<D> / V4);
         if (lane < PER * RW && r < rows) where = prefix_key(px, p.seq, kvh, p.tile * kPtKeys + r);
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int e = threadIdx.x + i * kSplitThreads, r = e / V4, c = e % V4;
+        const int e = threadIdx.x + i * kSplitThreads<D>, r = e / V4, c = e % V4;
         if constexpr (PX) {
             const int64_t at = __shfl_sync(0xffffffffu, where, i * RW + lane / V4);
-            x[i] = at >= 0 ? __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(is_v ? a.v : a.k) + at) + c)
+            x[i] = at >= 0 ? __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(is_v ? a.v : a.k) + at) + c)
                            : make_float4(0.f, 0.f, 0.f, 0.f);
         } else {
             x[i] = r < rows ? __ldg(reinterpret_cast<const float4 *>(src + (first + r) * tok) + c) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
         const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
         uint32_t row = 0;
 #pragma unroll
@@ -427,7 +432,7 @@ __global__ void __launch_bounds__(kSplitThreads)
     __half *dst = planes + (is_v ? 2 * plane : 0) + kvh * D;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int el = threadIdx.x + i * kSplitThreads, r = el / V4, c = el % V4;
+        const int el = threadIdx.x + i * kSplitThreads<D>, r = el / V4, c = el % V4;
         if (r >= rows) continue;
         __half h[4], l[4];
         split_f16(x[i].x * s, lo_scale, h[0], l[0]);
@@ -1373,7 +1378,7 @@ cudaError_t pt_launch(const PackedArgs &a, const PtPlan &plan, cudaStream_t st) 
             !row_map(&mv, false, planes + 2 * plane, D, a.Hkv, 2 * a.total_k, D, a.Hkv * D, 1, kPtKeys))
             return cudaErrorNotSupported;
         mq = mk;  // not used
-        e = b200_launch(packed_split_kernel<D, false>, dim3(static_cast<unsigned>(tiles)), dim3(kSplitThreads), 0, st, false, a,
+        e = b200_launch(packed_split_kernel<D, false>, dim3(static_cast<unsigned>(tiles)), dim3(kSplitThreads<D>), 0, st, false, a,
                         PrefixArgs(), planes, exps);
         if (e != cudaSuccess) return e;
     } else {
@@ -1440,7 +1445,7 @@ cudaError_t px_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st)
             !row_map(&mv, false, planes + 2 * plane, D, a.Hkv, 2 * total, D, a.Hkv * D, 1, kPtKeys))
             return cudaErrorNotSupported;
         mq = mk;  // not used
-        e = b200_launch(packed_split_kernel<D, true>, dim3(static_cast<unsigned>(tiles)), dim3(kSplitThreads), 0, st, false, a, p, planes,
+        e = b200_launch(packed_split_kernel<D, true>, dim3(static_cast<unsigned>(tiles)), dim3(kSplitThreads<D>), 0, st, false, a, p, planes,
                         exps);
         if (e != cudaSuccess) return e;
     } else if (!row_map(&mq, bf16, a.q, D, a.Hq, a.total_q, a.q_head, a.q_tok, a.G, BQ) || !pool_map(&mk, a.k) || !pool_map(&mv, a.v)) {
