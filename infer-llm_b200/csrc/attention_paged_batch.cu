@@ -414,7 +414,8 @@ B200_DEVICE Shares prefix_shares(const PrefixArgs &px, int64_t total, int64_t gr
     return s;
 }
 
-// CL: a cluster of kCluster CTAs takes one pair, and writes its output. PX: there are prefixes to join.
+// CL: a cluster of kCluster CTAs takes one pair, and writes its output. PX: there are prefixes to join, or (CL) to read as
+// a sequence's first keys; a block of one that is out of range clears the sequence's rows.
 template <typename T, int D, int HB, bool CL, bool PX>
 __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid_constant__ PbArgs a, const __grid_constant__ PrefixArgs px) {
     using Ge = Geometry<T, D, HB>;
@@ -430,11 +431,16 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
     float *own = reinterpret_cast<float *>(pb_smem);
     int64_t u0 = 0, u1 = 0;
     Place at = {};  // what is computed
+    int group = -1, before = 0;  // CL and PX: the pair's group, and keys of its prefix that come before its own
     if constexpr (CL) {
         const int pair = blockIdx.x / kCluster, rank = blockIdx.x % kCluster;
         at.b = pair / a.VH;
         at.vh = pair % a.VH;
-        at.len = seq_len(a, at.b);
+        if constexpr (PX) {
+            group = prefix_group(px, at.b);
+            if (px.within && group >= 0) before = prefix_len(px, group);
+        }
+        at.len = before + seq_len(a, at.b);
         at.tiles = (at.len + Ge::kTile - 1) / Ge::kTile;
         at.t = at.tiles * rank / kCluster;
         at.left = (at.tiles * (rank + 1) / kCluster - at.t) * kTileUnits<PX>;
@@ -457,19 +463,26 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
     }
     const Place start = at;
     Place in = at;  // what is loaded: one block lookup ahead of `issue`
-    bool bad = false;
+    bool bad = false, bad_prefix = false;
 
-    const uint64_t once = PX ? policy_evict_first() : 0;
+    const uint64_t once = PX && !CL ? policy_evict_first() : 0;
     // lane r < kSub looks up key row r of the sub-tile at `in`
     int64_t row_off = -1;  // byte offset in the pool; -1: no row
     int32_t row_blk = -1;
-    bool row_in = false;
+    bool row_in = false, row_prefix = false;
     auto lookup = [&] {
         const int64_t key = static_cast<int64_t>(in.t) * Ge::kTile + warp * Ge::kSub + (lane & (Ge::kSub - 1));
         row_in = in.left > 0 && key < in.len;
         if (row_in) {
-            const uint32_t k32 = static_cast<uint32_t>(key), slot = k32 / a.bt;
-            row_blk = __ldg(a.table + in.b * a.table_stride + slot);
+            uint32_t k32 = static_cast<uint32_t>(key);
+            const int32_t *table = a.table + in.b * a.table_stride;
+            if constexpr (CL && PX) {
+                row_prefix = k32 < static_cast<uint32_t>(before);
+                if (row_prefix) table = px.table + group * px.table_stride;
+                else k32 -= static_cast<uint32_t>(before);
+            }
+            const uint32_t slot = k32 / a.bt;
+            row_blk = __ldg(table + slot);
             row_off = static_cast<int64_t>(k32 - slot * a.bt) * a.tok_stride + (in.vh / a.HG) * a.head_stride;
         }
     };
@@ -477,6 +490,7 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
     auto issue = [&](int stage) {
         const bool ok = row_in && row_blk >= 0 && row_blk < a.n_blocks;
         bad |= row_in && !ok;
+        bad_prefix |= row_in && !ok && row_prefix;
         const int64_t off = ok ? row_off + row_blk * a.block_stride : -1;
         const uint32_t mask = __ballot_sync(0xffffffffu, ok) & ((1u << Ge::kSub) - 1u);
         if (lane == 0) live[stage] = mask;
@@ -491,7 +505,7 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
                 const uint32_t d = dst + r * Ge::kRow + ((c ^ (r & 7)) << 4);
                 const int n = o >= 0 ? 16 : 0;
                 const int64_t src = (o >= 0 ? o : 0) + c * 16;
-                if constexpr (PX) {  // these keys are read once; the prefixes' parts are to stay in L2
+                if constexpr (PX && !CL) {  // these keys are read once; the prefixes' parts are to stay in L2
                     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(d), "l"(a.k + src), "r"(n),
                                  "l"(once)
                                  : "memory");
@@ -580,12 +594,13 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
     // (The others would hold room that the grid's later CTAs want.)
     if (PX && (CL || blockIdx.x == gridDim.x - 1)) grid_wait();
     if constexpr (CL) {
-        cluster_sync();  // every CTA's record is written
-        int group = -1;
+        __shared__ float void_here;
         if constexpr (PX) {
-            group = prefix_group(px, start.b);
+            const int v = __syncthreads_or(bad_prefix);
+            if (threadIdx.x == 0) void_here = v ? 1.f : 0.f;
             if (blockIdx.x == 0) report_groups(px, a.status);
         }
+        cluster_sync();  // every CTA's record is written
         const int rank = blockIdx.x % kCluster;
         const int h0 = (start.vh / a.HG) * a.G + (start.vh % a.HG) * HB, heads = min(HB, a.G - (start.vh % a.HG) * HB);
         const int n = heads * D, i0 = n * rank / kCluster, i1 = n * (rank + 1) / kCluster;
@@ -611,7 +626,10 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
             }
             bool empty = false;
             if constexpr (PX) {
-                if (group >= 0) {
+                if (px.within) {
+#pragma unroll
+                    for (int c = 0; c < kCluster; ++c) empty |= ld_dsmem(dsmem_addr(&void_here, c)) != 0.f;
+                } else if (group >= 0) {
                     Joined j;
                     j.add(M, ls, make_float4(os, 0.f, 0.f, 0.f), 1.f);
                     for (int p = 0; p < px.parts; ++p) {
@@ -914,6 +932,11 @@ PbBytes pb_bytes(int64_t n_seqs, int64_t max_keys, int64_t D, int64_t G, int64_t
 }
 
 }  // namespace
+
+bool paged_batch_one_launch(int64_t n_seqs, int64_t max_keys, int64_t G, int64_t Hkv, int32_t dtype) {
+    const int hb = pb_heads(G, dtype == B200_DTYPE_F32);
+    return pb_one_launch(n_seqs * Hkv * ((G + hb - 1) / hb), max_keys);
+}
 
 size_t paged_batch_prefix_bytes(int64_t n_seqs, int64_t max_keys, int64_t D, int64_t G, int64_t Hkv, int32_t dtype) {
     const PbBytes n = pb_bytes(n_seqs, max_keys, D, G, Hkv, dtype);

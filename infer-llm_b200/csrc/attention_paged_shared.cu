@@ -9,9 +9,10 @@
 //    is cut into as many parts as fill the SMs.
 //  * the sequences' own keys, as in the batched decode (attention_paged_batch.cu);
 //  * the join of all parts.
+// Few short sequences take one launch of the batched decode instead, whose clusters read a prefix's keys as their sequence's first.
 // 64 BF16 sequences of 32 / 8 heads of 128 behind one prefix of 8192 keys, with 33 k keys of their own (165 MB): 46 us, of which the
 // join 5 to 6 after the own keys' end. A prefix CTA takes an SM's shared memory, so own keys run on the SMs that the plan leaves them (a small
-// CTA beside theirs took 61 against 63, but 56 against 47 behind 16384 keys). 8 F32 sequences behind 301 keys: 20 us, 14 of them the FFMA tiles' chain.
+// CTA beside theirs took 61 against 63, but 56 against 47 behind 16384 keys). 4 F32 sequences of 16 / 8 heads behind 301 keys: 12 us, one launch.
 #include "attention_packed_ffma.cuh"
 #include "paged_batch.cuh"
 
@@ -50,6 +51,7 @@ __global__ void __launch_bounds__(kPkThreads, 2) prefix_ffma_kernel(const Packed
 
 // How the prefixes are cut: rows of a tile (sequences, or with FFMA sequences times heads), tiles a CTA, parts of the keys.
 struct PrefixPlan {
+    bool within = false;           // no kernel of their own
     bool tc = false, few = false;  // few: FFMA tiles of 16 rows
     int tiles = 1, parts = 0;
     int64_t room = 0;  // F32 on the tensor cores: positions a group in the planes
@@ -65,6 +67,11 @@ PrefixPlan prefix_plan(int64_t n_seqs, int64_t max_keys, int64_t n_groups, int64
                        int32_t dtype) {
     PrefixPlan p;
     if (n_groups <= 0 || n_seqs <= 0 || max_prefix <= 0) return p;
+    // Few short pairs, prefixes included: one launch that reads a prefix once a sequence, from L2 after the first (4 sequences of 16 / 8 heads of
+    // 128 behind 300, 2000 and 3500 keys, one launch against a kernel of the prefixes' and the own keys': F32 12 us against 19, 18.5
+    // against 31, 24.6 against 45; BF16 12 against 17, 12.7 against 22.6, 16.6 against 24.5).
+    p.within = paged_batch_one_launch(n_seqs, max_keys + max_prefix, G, Hkv, dtype);
+    if (p.within) return p;
     // As if groups were alike.
     const int64_t groups = min64(n_groups, n_seqs), each = (n_seqs + groups - 1) / groups;
     p.few = each * G <= 16;
@@ -201,6 +208,7 @@ int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_
     const PrefixPlan plan = prefix_plan(n_seqs, max_keys, n_groups, max_prefix, D, Hq / Hkv, Hkv, pool->dtype);
     px.parts = plan.parts;
     px.tiles = plan.tiles;
+    px.within = plan.within;
     px.early = static_cast<int32_t>(plan.early);
     px.gap_start = pool->dtype == B200_DTYPE_F32 ? kGapStartF32 : kGapStart;
     px.gap_tile = kGapTile;

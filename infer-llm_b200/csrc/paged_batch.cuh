@@ -24,6 +24,8 @@ struct PbArgs {
     int32_t *status = nullptr;
 };
 
+// Whether sequences with so many keys, prefixes included, take one launch of clusters.
+bool paged_batch_one_launch(int64_t n_seqs, int64_t max_keys, int64_t G, int64_t Hkv, int32_t dtype);
 // The sequences' own keys, joined with what the prefixes' kernel left (launched before on the stream; it lets this grid start early).
 // `a.ws` and `a.whole` as the sizes of paged_batch_prefix_bytes.
 size_t paged_batch_prefix_bytes(int64_t n_seqs, int64_t max_keys, int64_t D, int64_t G, int64_t Hkv, int32_t dtype);

@@ -19,6 +19,7 @@ struct PrefixArgs {
     // CTAs of the own keys that run beside the prefixes' kernel, and how much longer than the others: units of their line of tiles, of the
     // prefix kernel's start and of each key tile of its longest part
     int32_t early = 0, gap_start = 0, gap_tile = 0;
+    bool within = false;  // the own keys' kernel takes each sequence's prefix as its first keys; no other runs
     float *o = nullptr;    // [part][sequence][query head][D]
     float2 *ml = nullptr;  // [part][sequence][query head]: maximum, sum (-1: the group's prefix names a block out of range)
 };

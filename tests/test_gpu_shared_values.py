@@ -179,3 +179,48 @@ def test_long_and_short_own_keys_beside_prefixes(cuda, kind, layout):
             b.prefix, b.own = prefix, own
             a[4], a[7] = ints(prefix), ints(own)
             check(B.flash_attn_paged_shared(*a), *b.want(), kind)
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout", ["g1", "g2", "g2d64", "g4", "g16"])
+@pytest.mark.parametrize("wide", [False, True])
+def test_few_sequences(cuda, kind, layout, wide):
+    """One launch, with the prefixes' keys as the sequences' first or (tables wider than 4096 positions) as parts."""
+    b = Batch([301, 0, 47], [2, 1, 0], [3, 0, 40, 17][:4 if layout in ("g2d64", "g16") else 3], 16, layout, kind, 25)
+    b.group.pop(3, None)
+    if wide:
+        table = torch.full((3, 400), -1, dtype=torch.int32, device=cuda)
+        table[:, :b.prefix_table.shape[1]] = b.prefix_table
+        b.prefix_table = table
+    status = ints([0])
+    want, w = b.want()
+    check(B.flash_attn_paged_shared(*b.args(), status=status), want, w, kind)
+    assert int(status) == 0
+    used = torch.zeros(b.k.shape[:2], dtype=torch.bool, device=cuda)  # hidden content does not count
+    for t, lens in ((b.prefix_table, b.prefix), (b.table, b.own)):
+        for i, n in enumerate(lens):
+            pos = torch.arange(n, device=cuda)
+            used[t[i].long()[pos // 16], pos % 16] = True
+    b.k[~used], b.v[~used] = math.nan, math.inf
+    check(B.flash_attn_paged_shared(*b.args()), want, w, kind)
+    for at in (0, 18):  # a bad block of a prefix clears its group
+        keep = int(b.prefix_table[0, at])
+        b.prefix_table[0, at] = b.k.shape[0]
+        status.zero_()
+        got = B.flash_attn_paged_shared(*b.args(), status=status)
+        assert int(status) == BAD_POSITION and (got[:2] == 0).all()
+        check(got[2:], want[2:], w[2:], kind)
+        b.prefix_table[0, at] = keep
+    for prefix, cu in (([301, -4, 47], None), ([301, 0, 47], [0, 2, 1, 3])):  # lengths and offsets out of range are reported
+        a = list(b.args())
+        a[4] = ints(prefix)
+        if cu:
+            a[5] = ints(cu)
+        status.zero_()
+        got = B.flash_attn_paged_shared(*a, status=status)
+        assert int(status) == BAD_POSITION and torch.isfinite(got.double()).all()
+        check(got[:1], want[:1], w[:1], kind)
+    b.v[b.prefix_table[0, 2], 5, 0, 9] = math.inf
+    rep = b.q.shape[1] // b.k.shape[2]
+    got = B.flash_attn_paged_shared(*b.args())
+    assert (got[:2, :rep, 9] == math.inf).all() and int((~torch.isfinite(got)).sum()) == 2 * rep
