@@ -224,3 +224,24 @@ def test_few_sequences(cuda, kind, layout, wide):
     rep = b.q.shape[1] // b.k.shape[2]
     got = B.flash_attn_paged_shared(*b.args())
     assert (got[:2, :rep, 9] == math.inf).all() and int((~torch.isfinite(got)).sum()) == 2 * rep
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout", ["g2", "g2d64", "g4"])
+@pytest.mark.parametrize("order", ["tokens", "heads", "apart"])
+@pytest.mark.parametrize("block", [8, 16, 24, 256])
+def test_pools_in_any_order(cuda, kind, layout, order, block):
+    """Pools that lie token by token, head by head, or with room between heads."""
+    b = many(layout, kind, 27, block)
+    want = b.want()
+    n, _, Hkv, D = b.k.shape
+    for name in ("k", "v"):
+        x = getattr(b, name)
+        if order == "heads":
+            x = x.transpose(1, 2).contiguous().transpose(1, 2)
+        elif order == "apart":
+            wide = torch.full((n, block, Hkv, 2 * D), math.nan, dtype=x.dtype, device=cuda)
+            wide[..., :D] = x
+            x = wide[..., :D]
+        setattr(b, name, x)
+    check(B.flash_attn_paged_shared(*b.args()), *want, kind)
