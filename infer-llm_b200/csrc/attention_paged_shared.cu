@@ -6,7 +6,7 @@
 //    is read once for up to 128 rows. 16-bit types: the packed attention's tensor-core kernel (attention_packed_tc.cu), whose K and V tiles
 //    are copied block by block; F32 as three F16 products of planes that a kernel before writes from the blocks. Few F32 rows with short
 //    prefixes, more than 128 query heads a KV head, or strides that a tensor map cannot hold: F32 FFMA (prefix_ffma_kernel). A prefix
-//    is cut into as many parts as fill the SMs.
+//    is cut into parts, a CTA each (prefix_plan).
 //  * the sequences' own keys, as in the batched decode (attention_paged_batch.cu);
 //  * the join of all parts.
 // Few short sequences take one launch of the batched decode instead, whose clusters read a prefix's keys as their sequence's first.
@@ -101,10 +101,13 @@ PrefixPlan prefix_plan(int64_t n_seqs, int64_t max_keys, int64_t n_groups, int64
     // 24 SMs for the prefixes, the rule's last: 64 BF16 sequences behind 8192 keys with 33 k of their own 57, 53, 49.5, 49, 45, 61.5; 46.
     // 16 behind 4096 with 16 k 37, 36, 33, 30, 29, 35; 29.6. 64 behind 16384 with one each 47, 41, 47, 57, 73, 107; 41.)
     const float own = 0.5f * n_seqs * max_keys * Hkv * D * (dtype == B200_DTYPE_F32 ? 8 : 4) * 1e-3f / kPxOwnRate;
-    const int64_t key_tiles = (max_prefix + 127) / 128;
+    const auto time = [&](int64_t parts) {
+        return (dtype == B200_DTYPE_F32 ? kPxStartF32 : kPxStart) + kPxTile * (((max_prefix + 127) / 128 + parts - 1) / parts);
+    };
     for (int64_t parts = 1; parts < room; ++parts) {
-        const float t = (dtype == B200_DTYPE_F32 ? kPxStartF32 : kPxStart) + kPxTile * ((key_tiles + parts - 1) / parts);
-        if (t > 0.9f * (own + t * ctas * parts / sms)) continue;
+        const float t = time(parts);
+        // (twice the shortest time at most: tables may be far wider than their sequences are long)
+        if (t > 0.9f * (own + t * ctas * parts / sms) || t > 2.f * time(room)) continue;
         p.parts = static_cast<int>(parts);
         break;
     }
