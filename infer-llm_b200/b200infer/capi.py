@@ -8,6 +8,7 @@ torch stream to the library. Shapes follow the reference's node semantics:
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 import struct
 import subprocess
@@ -362,12 +363,13 @@ class _Host:
         self.stream = torch._C._cuda_getCurrentRawStream
         L = lib()
         self.packed, self.packed_bytes = L.b200_flash_attn_packed, L.b200_flash_attn_packed_workspace_bytes
-        self.batch, self.batch_bytes = L.b200_flash_attn_paged_batch, L.b200_flash_attn_paged_batch_workspace_bytes
+        self.batch, self.batch_bytes = L.b200_flash_attn_paged_batch, _by_sizes(L.b200_flash_attn_paged_batch_workspace_bytes)
         self.append, self.sample = L.b200_paged_kv_append, L.b200_sample
         self.e4m3, self.e8m0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
         self.append_q8, self.read_q8 = L.b200_paged_kv_append_q8, L.b200_paged_kv_read_q8
-        self.batch_q8, self.batch_q8_bytes = L.b200_flash_attn_paged_batch_q8, L.b200_flash_attn_paged_batch_q8_workspace_bytes
-        self.shared, self.shared_bytes = L.b200_flash_attn_paged_shared, L.b200_flash_attn_paged_shared_workspace_bytes
+        self.batch_q8 = L.b200_flash_attn_paged_batch_q8
+        self.batch_q8_bytes = _by_sizes(L.b200_flash_attn_paged_batch_q8_workspace_bytes)
+        self.shared, self.shared_bytes = L.b200_flash_attn_paged_shared, _by_sizes(L.b200_flash_attn_paged_shared_workspace_bytes)
         self.adjust = L.b200_adjust_logits
 
 
@@ -420,9 +422,14 @@ def _status_word(status, dev):
     return status.data_ptr()
 
 
+def _by_sizes(fn):
+    """A function of a device and sizes that decode steps repeat: their workspaces' bytes, 1 us less once known."""
+    return functools.lru_cache(maxsize=1024)(lambda dev, *sizes: fn(*sizes))
+
+
 def _scratch(workspace, nbytes, like, dev):
     if workspace is None:
-        return _host.empty(nbytes, device=like.device, dtype=_host.u8) if nbytes else None
+        return like.new_empty(nbytes, dtype=_host.u8) if nbytes else None
     if not workspace.is_contiguous() or workspace.get_device() != dev or workspace.nbytes < nbytes:
         raise ValueError(f"workspace: expected {nbytes} bytes on cuda:{dev}")
     return workspace
@@ -523,7 +530,7 @@ def flash_attn_paged_batch(q, k_pool, v_pool, block_table, seq_lens, scale=0.0, 
     table, stride, blocks = _table(block_table, n, dev)
     out = _out_rows(out, q, dev)
     os = out.stride()
-    nbytes = h.batch_bytes(n, blocks * bt, D, Hq, Hkv, dt)
+    nbytes = h.batch_bytes(dev, n, blocks * bt, D, Hq, Hkv, dt)
     ws = _scratch(workspace, nbytes, q, dev)
     _chk("b200_flash_attn_paged_batch", h.batch(
         q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], pool, table, stride, blocks,
@@ -581,7 +588,7 @@ def paged_kv_read_q8(cu_rows, seq_lens, n_rows, k_pool, v_pool, k_scale, v_scale
                           k, v, status)
     pool, _, Hkv, D = _pool_q8(k_pool, v_pool, k_scale, v_scale, dev)
     if k is None and v is None:
-        k = h.empty((n_rows, Hkv, D), device=k_pool.device, dtype=dtype or h.torch.bfloat16)
+        k = k_pool.new_empty((n_rows, Hkv, D), dtype=dtype or h.torch.bfloat16)
         v = h.empty_like(k)
         dt = _dtype(k)
         ks = vs = (Hkv * D, D)
@@ -615,7 +622,7 @@ def flash_attn_paged_batch_q8(q, k_pool, v_pool, k_scale, v_scale, block_table, 
     table, stride, blocks = _table(block_table, n, dev)
     out = _out_rows(out, q, dev)
     os = out.stride()
-    nbytes = h.batch_q8_bytes(n, blocks * bt, D, Hq, Hkv)
+    nbytes = h.batch_q8_bytes(dev, n, blocks * bt, D, Hq, Hkv)
     ws = _scratch(workspace, nbytes, q, dev)
     _chk("b200_flash_attn_paged_batch_q8", h.batch_q8(
         q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], dt, pool, table, stride, blocks,
@@ -646,7 +653,7 @@ def flash_attn_paged_shared(q, k_pool, v_pool, prefix_table, prefix_lens, cu_seq
     ptable, pstride, pblocks = _table(prefix_table, groups, dev, "prefix_table")
     out = _out_rows(out, q, dev)
     os = out.stride()
-    nbytes = h.shared_bytes(n, blocks * bt, groups, pblocks * bt, D, Hq, Hkv, dt)
+    nbytes = h.shared_bytes(dev, n, blocks * bt, groups, pblocks * bt, D, Hq, Hkv, dt)
     ws = _scratch(workspace, nbytes, q, dev)
     _chk("b200_flash_attn_paged_shared", h.shared(
         q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], pool, ptable, pstride, pblocks,
@@ -674,7 +681,7 @@ def adjust_logits(logits, tokens=None, cu_tokens=None, prompt_lens=None, repetit
         raise ValueError("logits: expected (n, vocab), last axis contiguous")
     n, vocab = logits.shape
     if out is None:
-        out = h.empty((n, vocab), device=logits.device, dtype=logits.dtype)
+        out = h.empty_like(logits) if st[0] == vocab else logits.new_empty((n, vocab))
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.get_device() != dev or \
             (out.stride(1) != 1 and vocab != 1):
         raise ValueError("out: expected logits' shape and type, last axis contiguous")
