@@ -1432,7 +1432,7 @@ cudaError_t px_launch(const PackedArgs &a, const PrefixArgs &p, cudaStream_t st)
     CUtensorMap mq = {}, mk, mv;
     SplitView sp;
     sp.parts = p.parts;
-    const int64_t ctas = most_prefix_tiles(p.n_groups, a.total_q, 1, NT * BQ) * a.Hkv * p.parts;
+    const int64_t ctas = p.tiles_run * a.Hkv * p.parts;
     if (ctas > INT32_MAX) return cudaErrorNotSupported;
     if constexpr (split) {
         const int64_t total = p.n_groups * p.room, plane = total * a.Hkv * D, tiles = total / kPtKeys * a.Hkv * 2;

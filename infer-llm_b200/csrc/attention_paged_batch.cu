@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
     float *own = reinterpret_cast<float *>(pb_smem);
     int64_t u0 = 0, u1 = 0;
     Place at = {};  // what is computed
+    bool bad = false, bad_prefix = false;  // a block out of range; of the prefix, or its parts are not there
     int group = -1, before = 0;  // CL and PX: the pair's group, and keys of its prefix that come before its own
     if constexpr (CL) {
         const int pair = blockIdx.x / kCluster, rank = blockIdx.x % kCluster;
@@ -439,6 +440,7 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
         if constexpr (PX) {
             group = prefix_group(px, at.b);
             if (px.within && group >= 0) before = prefix_len(px, group);
+            bad_prefix = !px.within && group >= 0 && prefix_tiles_before(px, group + 1) > px.tiles_run;
         }
         at.len = before + seq_len(a, at.b);
         at.tiles = (at.len + Ge::kTile - 1) / Ge::kTile;
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
         Shares shares = {total, min64(gridDim.x, total / kTileUnits<PX>), 0, 0};
         if constexpr (PX) shares = prefix_shares<kTileUnits<PX>>(px, total, gridDim.x);
         if (blockIdx.x >= shares.ctas) {
-            if (PX && blockIdx.x == gridDim.x - 1) grid_wait();
+            if (PX && blockIdx.x == gridDim.x - 1) prefixes_done(px);
             return;
         }
         u0 = PX ? shares.begin(blockIdx.x) : share_begin(total, blockIdx.x, shares.ctas);
@@ -463,7 +465,6 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
     }
     const Place start = at;
     Place in = at;  // what is loaded: one block lookup ahead of `issue`
-    bool bad = false, bad_prefix = false;
 
     const uint64_t once = PX && !CL ? policy_evict_first() : 0;
     // lane r < kSub looks up key row r of the sub-tile at `in`
@@ -592,7 +593,10 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
     if (bad) set_status(a.status, B200_DEV_BAD_POSITION);
     // The prefixes' parts are written. In two launches the join needs them, so one CTA's wait does: this grid ends after theirs.
     // (The others would hold room that the grid's later CTAs want.)
-    if (PX && (CL || blockIdx.x == gridDim.x - 1)) grid_wait();
+    if constexpr (PX) {
+        if constexpr (CL) grid_wait();
+        else if (blockIdx.x == gridDim.x - 1) prefixes_done(px);
+    }
     if constexpr (CL) {
         __shared__ float void_here;
         if constexpr (PX) {
@@ -626,10 +630,9 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
             }
             bool empty = false;
             if constexpr (PX) {
-                if (px.within) {
 #pragma unroll
-                    for (int c = 0; c < kCluster; ++c) empty |= ld_dsmem(dsmem_addr(&void_here, c)) != 0.f;
-                } else if (group >= 0) {
+                for (int c = 0; c < kCluster; ++c) empty |= ld_dsmem(dsmem_addr(&void_here, c)) != 0.f;
+                if (!px.within && group >= 0 && !empty) {
                     Joined j;
                     j.add(M, ls, make_float4(os, 0.f, 0.f, 0.f), 1.f);
                     for (int p = 0; p < px.parts; ++p) {

@@ -130,7 +130,7 @@ cudaError_t prefix_ffma_launch(const PackedArgs &a, const PrefixArgs &px, cudaSt
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ffma_smem<D>()));
     });
     if (e != cudaSuccess) return e;
-    const int64_t ctas = most_prefix_tiles(px.n_groups, px.n_seqs, a.G, 16 * RT) * a.Hkv * px.parts;
+    const int64_t ctas = px.tiles_run * a.Hkv * px.parts;
     if (ctas > INT32_MAX) return cudaErrorNotSupported;
     return b200_launch(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPkThreads), ffma_smem<D>(), st, false, a, px);
 }
@@ -236,9 +236,14 @@ int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_
         p.sl2 = sl2;
         p.dtype = pool->dtype;
         p.status = dev_status;
+        px.tile_rows = static_cast<int32_t>(plan.tiles * (kPrefixTcRows / p.G));
+        px.tiles_run = plan.tc ? most_prefix_tiles(n_groups, n_seqs, 1, px.tile_rows) : 0;
         cudaError_t rc2 = plan.tc ? prefix_tc_launch(p, px, st) : cudaErrorNotSupported;
         if (rc2 == cudaErrorNotSupported) {
             px.early = 0;
+            px.tile_rows = plan.few ? 16 : kPkRows;
+            px.tile_heads = p.G;
+            px.tiles_run = most_prefix_tiles(n_groups, n_seqs, p.G, px.tile_rows);
             rc2 = prefix_ffma_by_type(p, px, plan.few, st);
         }
         if (rc2 != cudaSuccess) return status_of(rc2);

@@ -16,6 +16,9 @@ struct PrefixArgs {
     // F32 on the tensor cores: K and V as planes of F16 numbers with room for `room` positions a group (a multiple of 128), then exponents
     void *planes = nullptr;
     int64_t room = 0;
+    // The prefixes' tiles: rows, rows a sequence counts for, and tiles that the grid has room for.
+    int32_t tile_rows = 1, tile_heads = 1;
+    int64_t tiles_run = 0;
     // CTAs of the own keys that run beside the prefixes' kernel, and how much longer than the others: units of their line of tiles, of the
     // prefix kernel's start and of each key tile of its longest part
     int32_t early = 0, gap_start = 0, gap_tile = 0;
@@ -59,6 +62,33 @@ B200_DEVICE bool prefix_bad(const PrefixArgs &a, int group, int from, int to, in
 inline int64_t most_prefix_tiles(int64_t n_groups, int64_t n_seqs, int64_t G, int64_t M) {
     const int64_t groups = min64(n_groups, n_seqs);
     return groups + (n_seqs * G - groups) / M;
+}
+// Tiles of the groups before `end`, by a whole warp. More than tiles_run only where offsets out of order make groups overlap.
+B200_DEVICE int64_t prefix_tiles_before(const PrefixArgs &a, int end) {
+    int64_t tiles = 0;
+    for (int g = threadIdx.x & 31; g < end; g += 32) {
+        int64_t first = 0;
+        int n = 0;
+        if (packed_range(a.cu, g, a.n_seqs, first, n))
+            tiles += (static_cast<int64_t>(n) * a.tile_heads + a.tile_rows - 1) / a.tile_rows;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    return tiles;
+}
+// Waits for the prefixes' grid; then, by one CTA, what it had no room for is marked as not to be used.
+B200_DEVICE void prefixes_done(const PrefixArgs &a) {
+    const int64_t tiles = a.parts > 0 ? prefix_tiles_before(a, a.n_groups) : 0;
+    grid_wait();
+    if (tiles <= a.tiles_run) return;
+    for (int g = 0; g < a.n_groups; ++g) {
+        int64_t first = 0;
+        int n = 0;
+        if (prefix_tiles_before(a, g + 1) <= a.tiles_run || !packed_range(a.cu, g, a.n_seqs, first, n)) continue;
+        const int64_t rows = static_cast<int64_t>(n) * a.Hq;
+        for (int part = 0; part < a.parts; ++part)
+            for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) a.ml[prefix_row(a, part, first, 0) + i] = make_float2(0.f, -1.f);
+    }
 }
 // Tile `at` of M rows of the line of all groups' tiles, a row being a sequence with one of G heads; by a whole warp.
 B200_DEVICE PackedTile find_prefix_tile(const PrefixArgs &a, int G, int M, int64_t at) {

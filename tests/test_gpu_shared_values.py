@@ -245,3 +245,26 @@ def test_pools_in_any_order(cuda, kind, layout, order, block):
             x = wide[..., :D]
         setattr(b, name, x)
     check(B.flash_attn_paged_shared(*b.args()), *want, kind)
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout,n", [("g16", 48), ("g4", 200), ("g20", 30), ("g16", 30)])
+def test_groups_that_overlap(cuda, kind, layout, n):
+    """Offsets out of order that make groups overlap are reported; whatever such a row shows is no old content."""
+    b = Batch([500, 60, 300, 60, 700], [n], [(i * 7) % 40 for i in range(n)], 16, layout, kind, 29)
+    a = list(b.args())
+    end = n - 1
+    a[5] = ints([0, end, 0, end, 0, end])
+    groups = b.keys(0)[0].shape[0] - b.own[0]
+    assert groups == 500
+    status = ints([0])
+    seen = []
+    for fill in (0xFF, 0x00, 0x7F):
+        ws = torch.full((1 << 27,), fill, dtype=torch.uint8, device=cuda)
+        status.zero_()
+        seen.append(B.flash_attn_paged_shared(*a, workspace=ws, status=status))
+        assert int(status) == BAD_POSITION
+        assert torch.isfinite(seen[-1].double()).all()
+    alone = B.flash_attn_paged_batch(b.q[end:].contiguous(), b.k, b.v, b.table[end:].contiguous(), ints(b.own[end:]))
+    for got in seen:
+        assert torch.allclose(got[end:].double(), alone.double(), rtol=1e-2, atol=1e-2)
