@@ -351,9 +351,11 @@ size_t b200_flash_attn_paged_batch_q8_workspace_bytes(int64_t n_seqs, int64_t ma
  * first, then the seq_lens[s] positions of their own rows of block_table (either may be 0; both tables name
  * blocks of the one pool). Each prefix is read once for up to 128 rows (sequences times query heads) of its group. As in
  * b200_flash_attn_packed, its weights are rounded to the element type for 16-bit caches, and its F32 products are three of F16 numbers with
- * 22 bits, or F32 FFMA (short prefixes with few rows, more than 128 query heads a KV head, planes past a GiB of workspace). Sequences outside every group see their own positions alone. A prefix with a
- * block index out of range makes its group's rows zero; cu_seqs, prefix_lens and prefix_table are else treated as
- * the other offsets, lengths and tables. */
+ * 22 bits, or F32 FFMA (short prefixes with few rows, more than 128 query heads a KV head, planes past a GiB of workspace). Few
+ * short sequences (at most 4096 positions with their prefix) run as in b200_flash_attn_paged_batch. Sequences outside every
+ * group see their own positions alone. A prefix with a block index out of range makes its group's rows zero; cu_seqs,
+ * prefix_lens and prefix_table are else treated as the other offsets, lengths and tables. `workspace` as there, with max_prefix =
+ * prefix_blocks * block_tokens; one for n_seqs does for fewer, but F32 planes come and go with n_groups. */
 int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
                                  int64_t out_seq_stride, int64_t out_head_stride, const b200_kv_pool *pool,
                                  const int32_t *prefix_table, int64_t prefix_stride, int64_t prefix_blocks,

@@ -115,9 +115,12 @@ PrefixPlan prefix_plan(int64_t n_seqs, int64_t max_keys, int64_t n_groups, int64
     return p;
 }
 
-// Bytes of the parts, and of the planes behind them.
+// Bytes of the parts, and of the planes behind them. Several parts hold at most the rows of the CTAs that run at once, whatever the sizes
+// are, so that room for them does for calls of fewer sequences too.
 size_t prefix_parts_bytes(int64_t n_seqs, const PrefixPlan &p, int64_t D, int64_t Hq) {
-    return (static_cast<size_t>(p.parts) * n_seqs * Hq * (D * 4 + 8) + 127) / 128 * 128;
+    if (p.parts == 0) return 0;
+    const int64_t sms = device_sm_count(), at_once = max64(sms * 3 / 4 * 2 * kPrefixTcRows, 2 * sms * kPkRows);
+    return (static_cast<size_t>(max64(n_seqs * Hq, at_once)) * (D * 4 + 8) + 127) / 128 * 128;
 }
 size_t prefix_bytes(int64_t n_seqs, int64_t n_groups, const PrefixPlan &p, int64_t D, int64_t Hq, int64_t Hkv) {
     return prefix_parts_bytes(n_seqs, p, D, Hq) + (p.room ? prefix_planes_bytes(n_groups, p.room, D, Hkv) : 0);

@@ -124,3 +124,12 @@ def test_shared_pool_and_workspace():
                                      (dict(x=P + 1, out=P + 1, dtype=2), UNSUPPORTED), (dict(n=2 ** 40), UNSUPPORTED), (dict(n=0), OK)])
 def test_adjust(kw, code):
     assert adjust(**kw) == code
+
+
+@pytest.mark.parametrize("dtype", [1, 2])
+@pytest.mark.parametrize("heads", [(32, 8), (16, 8), (16, 1), (150, 1)])
+def test_workspace_for_many_sequences_does_for_fewer(dtype, heads):
+    size = L.lib().b200_flash_attn_paged_shared_workspace_bytes
+    for keys, groups, prefix in ((1024, 1, 8192), (4096, 4, 1000), (16, 1, 100000)):
+        sizes = [size(n, keys, groups, prefix, 128, *heads, dtype) for n in list(range(1, 200)) + [500, 5000]]
+        assert sizes == sorted(sizes)
