@@ -48,7 +48,7 @@
 // Bound: at long contexts the chain scores -> softmax -> P -> product of a slot, against which the other
 // slot's runs: 8192 BF16 tokens, 32 / 8 heads of 128, 505 to 522 us by GPU, 1.05 to 1.09 PFLOP/s (64 to 66 % of a
 // large library matrix product's rate); the tensor cores are busy 54 to 60 % of the time. 2048 F32 tokens, 16 / 8
-// heads of 128, 81 to 82 us (209 to 212 TFLOP/s of the call's, 630 of the three products), the split kernel 7 us of it. Short
+// heads of 128, 76 to 79 us (217 to 225 TFLOP/s of the call's, 660 of the three products), 3 of them less since the split kernel is faster. Short
 // calls: a CTA's start and end, ~6 us (look-up 1, first copies 1.4, last product 0.8 to 1.7, output 2), beside ~0.9
 // us a step: 10 prompts of 1 to 1333 BF16 tokens, 16 / 8 heads of 128, 35 us. Two slots take all 512
 // columns of tensor memory and most of an SM's registers.
@@ -326,8 +326,8 @@ template <int D>
 constexpr int kSplitThreads = 4 * D;  // a thread holds eight float4 of the tile
 
 // One CTA: the K or V rows of one key tile and KV head, as hi and lo planes with the tile's
-// exponent, and whether its rows and columns spread too far for one. A pass over the bytes: HBM bounds it (2048 keys, 8 heads of 128: 17 MB in, 17 MB out, 7 us
-// with its launch; the attention kernel's start overlaps it). All loads come before the first reduction, which would else wait for each.
+// exponent, and whether its rows and columns spread too far for one. A pass over the bytes: HBM bounds it (2048 keys, 8 heads of 128: 17 MB in, 17 MB out;
+// the attention kernel's start overlaps it). All loads come before the first reduction, which would else wait for each.
 // PX: of a prefix's blocks, tile after tile of a group's room, read past L2's room for the planes (8192 keys, 8 heads of 128, 67 MB in and out:
 // 31 us; with half the threads 33, with loads and reductions in one loop 42, both 47; with twice the threads 45).
 template <int D, bool PX>
