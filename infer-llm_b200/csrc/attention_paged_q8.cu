@@ -16,7 +16,7 @@
 //  * The scales 2^ek multiply the scores. The scales 2^ev go into the weights: w_j = 2^(t_j log2 e + ev_j - N + 14), N the running maximum of
 //    the exponent, as two F16 numbers. N has a maximum of its own, so keys whose V is far larger than that of the heaviest key keep their
 //    bits; the sum of the weights goes by the scores' maximum M. At the end 2^(N - M - 14) takes both together.
-// 64 BF16 sequences of 5 to 4069 keys, 32 / 8 heads of 128 (273 MB): 61 to 63 us with the join, 4.4 TB/s, 67 % of a large copy's rate; 16 F32
+// 64 BF16 sequences of 5 to 4069 keys, 32 / 8 heads of 128 (273 MB): 61 to 64 us with the join, 4.4 TB/s, 67 % of a large copy's rate; 16 F32
 // sequences of 1500 to 7548 keys, 16 / 8 heads (147 MB): 37 us, 3.9 TB/s. With half the bytes a key the instructions count as much as HBM
 // (issue active 41 %, two CTAs an SM), and the start (3.6 us of dependent look-ups), the pairs' ends and the join (4 to 5 us) weigh twice.
 // Rows past a sequence's end are not read; they and keys of invalid blocks get weight 0.
