@@ -349,9 +349,9 @@ size_t b200_flash_attn_paged_batch_q8_workspace_bytes(int64_t n_seqs, int64_t ma
 /* b200_flash_attn_paged_batch for sequences that share prefixes (a common instruction, a document): group g is the
  * sequences [cu_seqs[g], cu_seqs[g + 1]), which see the prefix_lens[g] positions of row g of prefix_table
  * first, then the seq_lens[s] positions of their own rows of block_table (either may be 0; both tables name
- * blocks of the one pool). Each prefix is read once for up to 128 rows (sequences times query heads) of its group. As in
- * b200_flash_attn_packed, its weights are rounded to the element type for 16-bit caches, and its F32 products are three of F16 numbers with
- * 22 bits, or F32 FFMA (short prefixes with few rows, more than 128 query heads a KV head, planes past a GiB of workspace). Few
+ * blocks of the one pool). Each prefix is read once for up to 128 rows (sequences times query heads) of its group. Weights
+ * are two numbers of the element type for 16-bit caches, as in b200_flash_attn_paged_batch; a prefix's F32 products are three of F16 numbers
+ * with 22 bits, or F32 FFMA (short prefixes with few rows, more than 128 query heads a KV head, planes past a GiB of workspace). Few
  * short sequences (at most 4096 positions with their prefix) run as in b200_flash_attn_paged_batch. Sequences outside every
  * group see their own positions alone. A prefix with a block index out of range makes its group's rows zero; cu_seqs,
  * prefix_lens and prefix_table are else treated as the other offsets, lengths and tables. `workspace` as there, with max_prefix =

@@ -24,6 +24,9 @@
 //     one number of the element type, the sum is taken before that rounding. It is what the second
 //     product takes at one product's cost; two terms of P would add half to the tensor work. The errors against
 //     64 bits grow by it from 1.5e-3 to 2.0e-3 of the output (8192 BF16 tokens) and from 2.1e-4 to 2.6e-4 (F16).
+//     A shared prefix's P has two terms and no polynomial, since its rows' own keys have them too: the
+//     products of V are twice as many, 2.5 us a step of two tiles of rows against 2.3, and an output is off by its
+//     own rounding alone (64 BF16 sequences behind 8192 keys: 1.7e-3, with one term 2.3e-3).
 //   * Hidden keys of a tile (past a row's last key, of the next sequence, or past the end)
 //     have P = 0, but 0 times a V that is no number is not 0. The V check looks for such
 //     rows in the tiles that hide keys, clears them in shared memory, and notes them; 16-bit rows that
@@ -273,6 +276,11 @@ B200_DEVICE uint32_t pack_pair(float x, float y) {
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 }
+template <typename T>
+B200_DEVICE float2 unpack_pair(uint32_t u) {
+    if constexpr (__is_same(T, __half)) return __half22float2(*reinterpret_cast<const __half2 *>(&u));
+    else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u));
+}
 
 // F32 operands split for the tensor cores: planes of F16 rows [2][total_k][Hkv][D], and per
 // (key tile, KV head) the exponents of K and of V. And the parts of a query tile's keys.
@@ -458,6 +466,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
     static_assert(SL == 2 || (NT == 1 && !SPLIT), "one slot holds one query tile");
     static_assert(!PX || SL == 2, "prefixes: two slots");
     constexpr bool kPairs = NT == 2 || SL == 1, kJoin = NT == 1 && SL == 2;  // kJoin: the slots halve the key tiles
+    constexpr bool kTwo = SPLIT || PX;  // P as two terms
     constexpr int kColumns = 256 * SL;  // of tensor memory
     constexpr bool kBf16 = __is_same(T, __nv_bfloat16);
     constexpr uint32_t kIdS = idesc_f16(kPtRows, kPtKeys, kBf16, false, false);
@@ -722,13 +731,13 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                     mma_ss(e, d, qa + off, ka + off, kIdS, add || kk > 0);
                 }
             };
-            // O (+)= P . a plane of V. P lies over the scores: 16 keys in 8 columns; F32: each 32
-            // columns hold hi, then lo of their 32 keys
+            // O (+)= P . a plane of V. P lies over the scores: 16 keys in 8 columns; as two terms: hi, then
+            // lo of 16 keys, of F32 of 32
             const auto values = [&](int slot, bool lo, int pl, int from, int to, bool add, bool onto_lo) {
-                const uint32_t d = col_o(slot), pa = col_s(slot) + (lo ? 16 : 0), va = desc_low(at(pl), Ge::kBox);
+                const uint32_t d = col_o(slot), pa = col_s(slot) + (lo ? (SPLIT ? 16 : 8) : 0), va = desc_low(at(pl), Ge::kBox);
 #pragma unroll
                 for (int kk = from; kk < to; ++kk) {  // 16 keys: two 1024-byte atoms
-                    const uint32_t pk = pa + (SPLIT ? 32 * (kk >> 1) + 8 * (kk & 1) : 8 * kk), vk = va + kk * (2048 >> 4);
+                    const uint32_t pk = pa + (SPLIT ? 32 * (kk >> 1) + 8 * (kk & 1) : (kTwo ? 16 : 8) * kk), vk = va + kk * (2048 >> 4);
                     if (onto_lo && kk == 0) mma_ts_onto_lo(e, d, pk, vk, kIdO);
                     else mma_ts(e, d, pk, vk, kIdO, add || kk > 0);
                 }
@@ -776,10 +785,12 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                     values(slot, false, pl + 1, 0, KK, true, false);
                 } else {
                     values(slot, false, pl, 0, KH, i >= SL, false);
+                    if (kTwo) values(slot, true, pl, 0, KH, true, false);
                     ok = all(&p_full[slot], (i / SL) & 1);
                     if (!ok) break;
                     tc_fence_after();
                     values(slot, false, pl, KH, KK, true, false);
+                    if (kTwo) values(slot, true, pl, KH, KK, true, false);
                 }
                 if (NT == 1 || slot == 1) commit_if(e, &empty[(pl + PL - 1) % S]);
                 if (SPLIT || i + SL >= steps) commit_if(e, &o_final[slot]);
@@ -1131,9 +1142,17 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                                              ? exp2_poly_pair<kBf16>(x)
                                              : make_float2(exp2_approx(x.x), exp2_approx(x.y));
                         sum[j & 3] = add_pair(sum[j & 3], pair_of(y.x, y.y));
-                        pv[j] = pack_pair<T>(y.x, y.y);
+                        if constexpr (kTwo) {  // 16 keys: hi, then lo
+                            const uint32_t hi = pack_pair<T>(y.x, y.y);
+                            const float2 h = unpack_pair<T>(hi), lo = of_pair(add_pair(pair_of(y.x, y.y), pair_of(-h.x, -h.y)));
+                            pv[j & 7] = hi;
+                            pv[8 + (j & 7)] = pack_pair<T>(lo.x, lo.y);
+                            if ((j & 7) == 7) tc_st16(ts + 32 * c + 2 * (j & 8), pv);
+                        } else {
+                            pv[j] = pack_pair<T>(y.x, y.y);
+                        }
                     }
-                    tc_st16(ts + 16 * c, pv);
+                    if constexpr (!kTwo) tc_st16(ts + 16 * c, pv);
                     if (c == 2) {  // the tensor cores may start on the first 96 keys
                         tc_wait_st();
                         tc_fence_before();
@@ -1141,7 +1160,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                     }
                 }
             };
-            if (by_poly) weigh(std::true_type{});
+            if (!kTwo && by_poly) weigh(std::bool_constant<!kTwo>{});
             else weigh(std::false_type{});
             const float2 two = of_pair(add_pair(add_pair(sum[0], sum[1]), add_pair(sum[2], sum[3])));
             l = two.x + two.y;

@@ -59,7 +59,7 @@ struct PrefixPlan {
 };
 // Model of the tensor-core kernel and of the own keys' (us, kB a us): what a CTA's start and end and a tile of 128 keys take, and the rate of
 // own keys on all SMs.
-constexpr float kPxStart = 8.f, kPxStartF32 = 16.f, kPxTile = 2.2f, kPxOwnRate = 4500.f;
+constexpr float kPxStart = 8.f, kPxStartF32 = 16.f, kPxTile = 2.5f, kPxTileF32 = 2.2f, kPxOwnRate = 4500.f;
 // The same start and tile in units of the own keys' line (0.7 us).
 constexpr int kGapStart = 10, kGapStartF32 = 20, kGapTile = 3;
 constexpr size_t kPrefixMostPlanes = size_t(1) << 30;
@@ -102,7 +102,8 @@ PrefixPlan prefix_plan(int64_t n_seqs, int64_t max_keys, int64_t n_groups, int64
     // 16 behind 4096 with 16 k 37, 36, 33, 30, 29, 35; 29.6. 64 behind 16384 with one each 47, 41, 47, 57, 73, 107; 41.)
     const float own = 0.5f * n_seqs * max_keys * Hkv * D * (dtype == B200_DTYPE_F32 ? 8 : 4) * 1e-3f / kPxOwnRate;
     const auto time = [&](int64_t parts) {
-        return (dtype == B200_DTYPE_F32 ? kPxStartF32 : kPxStart) + kPxTile * (((max_prefix + 127) / 128 + parts - 1) / parts);
+        const int64_t steps = ((max_prefix + 127) / 128 + parts - 1) / parts;
+        return dtype == B200_DTYPE_F32 ? kPxStartF32 + kPxTileF32 * steps : kPxStart + kPxTile * steps;
     };
     for (int64_t parts = 1; parts < room; ++parts) {
         const float t = time(parts);
