@@ -379,7 +379,8 @@ size_t b200_flash_attn_paged_shared_workspace_bytes(int64_t n_seqs, int64_t max_
  * the three penalties (float32 [n_rows]; NULL: off), bias_ids (with bias_values and cu_bias) and mask may be NULL. Rows any
  * alignment; strides count elements (of mask: words). A token id out of range or offsets that are not ascending within the
  * given totals are left out and B200_DEV_BAD_TOKEN / B200_DEV_BAD_POSITION recorded; a repetition penalty
- * that is not positive and finite, or another that is not finite, is off for its row and B200_DEV_BAD_LOGITS recorded. */
+ * that is not positive and finite, or another that is not finite, is off for its row and B200_DEV_BAD_LOGITS recorded. Offsets
+ * and penalties that are given are looked at for every row, whether its lists hold anything or not. */
 int b200_adjust_logits(const void *logits, int64_t row_stride, void *out, int64_t out_row_stride, int64_t n_rows,
                        int64_t n_vocab, int32_t dtype, const int32_t *tokens, int64_t n_tokens,
                        const int32_t *cu_tokens, const int32_t *prompt_lens, const float *repetition,

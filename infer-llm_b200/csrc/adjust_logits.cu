@@ -198,11 +198,10 @@ __global__ void __launch_bounds__(kAdThreads, kAdCtas) adjust_logits_kernel(cons
         if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     } else if (walks) {
         int64_t from = 0, to = 0, bias_to = 0;
-        if (a.tokens) {
-            list_range(a.cu_tokens, row, a.n_tokens, a.status, from, to);
-            if (a.prompt_lens) prompt = max(0, __ldg(a.prompt_lens + row));
-        }
-        if (a.bias_ids) list_range(a.cu_bias, row, a.n_biases, a.status, bias_from, bias_to);
+        // (offsets are looked at where the lists hold nothing too)
+        if (a.cu_tokens) list_range(a.cu_tokens, row, a.n_tokens, a.status, from, to);
+        if (a.tokens && a.prompt_lens) prompt = max(0, __ldg(a.prompt_lens + row));
+        if (a.cu_bias) list_range(a.cu_bias, row, a.n_biases, a.status, bias_from, bias_to);
         tokens = a.tokens + from, biases = a.bias_ids + bias_from;
         n = static_cast<int>(to - from), m = static_cast<int>(bias_to - bias_from);
         *reinterpret_cast<uint4 *>(named + kPer * tid) = make_uint4(0, 0, 0, 0);
@@ -239,10 +238,12 @@ __global__ void __launch_bounds__(kAdThreads, kAdCtas) adjust_logits_kernel(cons
         if (sum > 0) count(0);
     }
     __syncthreads();  // the slots are counted, and the pass has written their tokens
+    if (total == 0 && (blockIdx.y || threadIdx.x)) return;
+    // (the first chunk's CTA looks at the row's penalties where it has no token for them too)
+    const float rep = penalty(a.repetition, row, 1.f, true, a.status);
+    const float freq = penalty(a.frequency, row, 0.f, false, a.status);
+    const float pres = penalty(a.presence, row, 0.f, false, a.status);
     if (total == 0) return;
-    const float rep = penalty(a.tokens ? a.repetition : nullptr, row, 1.f, true, a.status);
-    const float freq = penalty(a.tokens ? a.frequency : nullptr, row, 0.f, false, a.status);
-    const float pres = penalty(a.tokens ? a.presence : nullptr, row, 0.f, false, a.status);
     const float *bias_values = a.bias_ids ? a.bias_values + __ldg(a.cu_bias + row) : nullptr;
     for (int first = 0;;) {
         for (int i = threadIdx.x; i < min(total - first, kAdSlots); i += kAdThreads) {
