@@ -317,7 +317,8 @@ typedef struct b200_kv_pool_q8 {
 /* b200_paged_kv_append into an 8-bit pool; k, v are F32, F16 or BF16 (`dtype`). Each row gets the least
  * whole e >= -127 with max |x| <= 448 2^e, and its elements x 2^-e (exact) rounded to e4m3, ties to even: at
  * most 2^-4 of the element off, or 2^(e - 10) where that is more. A row that holds an infinity or a NaN is
- * held as zeros with the scale NaN, and reads as NaN. */
+ * held as zeros with the scale NaN, and reads as NaN. Rows outside every sequence, and those whose offsets, position or
+ * block are out of range, are left out and B200_DEV_BAD_POSITION recorded. */
 int b200_paged_kv_append_q8(const void *k, int64_t k_tok_stride, int64_t k_head_stride, const void *v,
                             int64_t v_tok_stride, int64_t v_head_stride, int32_t dtype, const int32_t *cu_new,
                             const int32_t *seq_lens, int64_t n_seqs, int64_t n_tokens, const b200_kv_pool_q8 *pool,

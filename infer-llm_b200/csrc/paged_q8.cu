@@ -27,10 +27,11 @@ struct Q8Args {
 
 constexpr int kQ8Threads = 128, kQ8Chunks = 4;
 
-// Block and place in it of packed row t of sequence s, a sequence's rows being its last positions; false if out of range.
+// Block and place in it of packed row t of sequence s, a sequence's rows being its last positions; false if the sequence's
+// offsets, the position or the block are out of range.
 B200_DEVICE bool q8_place(const Q8Args &a, int s, int64_t t, int64_t &block, int64_t &place) {
-    const int64_t pos = static_cast<int64_t>(__ldg(a.lens + s)) - __ldg(a.cu + s + 1) + t;  // < 2^31: t is a row of s
-    if (pos < 0) return false;
+    const int64_t end = __ldg(a.cu + s + 1), pos = __ldg(a.lens + s) - end + t;  // < 2^31: t is a row of s
+    if (__ldg(a.cu + s) < 0 || end > a.n_tokens || pos < 0) return false;
     const int64_t slot = static_cast<int64_t>(static_cast<uint64_t>(pos) * a.bt_mul >> a.bt_shift);
     if (slot >= a.max_blocks) return false;
     block = __ldg(a.table + s * a.table_stride + slot);
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(kQ8Threads) paged_read_q8_kernel(const Q8Args 
     if (s < 0 && (t < __ldg(a.cu) || t >= __ldg(a.cu + a.n_seqs))) return;
     const int c0 = blockIdx.y * 32 * kQ8Chunks + lane, h0 = c0 / L, r = c0 % L;
     int64_t block = 0, place = 0;
-    const bool ok = s >= 0 && __ldg(a.cu + s) >= 0 && __ldg(a.cu + s + 1) <= a.n_tokens && q8_place(a, s, t, block, place);
+    const bool ok = s >= 0 && q8_place(a, s, t, block, place);
     if (!ok && lane == 0) set_status(a.status, B200_DEV_BAD_POSITION);
     const int64_t data_at = block * a.block_stride + place * a.tok_stride + h0 * a.head_stride + r * E;
     const int64_t scale_at = block * a.scale_block + place * a.scale_tok + h0 * a.scale_head;
