@@ -316,7 +316,8 @@ typedef struct b200_kv_pool_q8 {
 
 /* b200_paged_kv_append into an 8-bit pool; k, v are F32, F16 or BF16 (`dtype`). Each row gets the least
  * whole e >= -127 with max |x| <= 448 2^e, and its elements x 2^-e (exact) rounded to e4m3, ties to even: at
- * most 2^-4 of the element off, or 2^(e - 10) where that is more. A row that holds an infinity or a NaN is
+ * most 2^-4 of the element off, or 2^(e - 10) where that is more. (Elements of 248 2^120 or more become 2^128, which reads as
+ * infinite.) A row that holds an infinity or a NaN is
  * held as zeros with the scale NaN, and reads as NaN. Rows outside every sequence, and those whose offsets, position or
  * block are out of range, are left out and B200_DEV_BAD_POSITION recorded. */
 int b200_paged_kv_append_q8(const void *k, int64_t k_tok_stride, int64_t k_head_stride, const void *v,
@@ -328,7 +329,7 @@ int b200_paged_kv_append_q8(const void *k, int64_t k_tok_stride, int64_t k_head_
 /* The inverse: rows of an 8-bit pool into packed rows k, v [n_rows][Hkv][D] of F32, F16 or BF16, as
  * b200_flash_attn_packed takes them. Sequence s gets the rows [cu_rows[s], cu_rows[s + 1]), which are its last
  * positions of the seq_lens[s] cached (all of them where the counts are equal). Values q 2^e are exact in F32
- * and BF16 and rounded once to F16. Rows outside every sequence are left untouched; a row whose offsets, position or block
+ * (infinite past its largest) and in BF16 (which rounds to multiples of 2^-133), and rounded once to F16. Rows outside every sequence are left untouched; a row whose offsets, position or block
  * are out of range is zero. */
 int b200_paged_kv_read_q8(const b200_kv_pool_q8 *pool, const int32_t *block_table, int64_t table_stride,
                           int64_t max_blocks, const int32_t *cu_rows, const int32_t *seq_lens, int64_t n_seqs,
