@@ -355,8 +355,9 @@ size_t b200_flash_attn_paged_batch_q8_workspace_bytes(int64_t n_seqs, int64_t ma
  * are two numbers of the element type for 16-bit caches, as in b200_flash_attn_paged_batch; a prefix's F32 products are three of F16 numbers
  * with 22 bits, or F32 FFMA (short prefixes with few rows, more than 128 query heads a KV head, planes past a GiB of workspace). Few
  * short sequences (at most 4096 positions with their prefix) run as in b200_flash_attn_paged_batch. Sequences outside every
- * group see their own positions alone. A prefix with a block index out of range makes its group's rows zero; cu_seqs,
- * prefix_lens and prefix_table are else treated as the other offsets, lengths and tables. `workspace` as there, with max_prefix =
+ * group see their own positions alone. A prefix with a block index out of range makes its group's rows zero. Where cu_seqs
+ * is out of order, rows of sequences that several groups name are zero (others may be, where such groups have more tiles than groups in
+ * order). cu_seqs, prefix_lens and prefix_table are else treated as the other offsets, lengths and tables. `workspace` as there, with max_prefix =
  * prefix_blocks * block_tokens; one for n_seqs does for fewer, but F32 planes come and go with n_groups. */
 int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
                                  int64_t out_seq_stride, int64_t out_head_stride, const b200_kv_pool *pool,

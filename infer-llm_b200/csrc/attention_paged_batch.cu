@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
     float *own = reinterpret_cast<float *>(pb_smem);
     int64_t u0 = 0, u1 = 0;
     Place at = {};  // what is computed
-    bool bad = false, bad_prefix = false;  // a block out of range; of the prefix, or its parts are not there
+    bool bad = false, bad_prefix = false;  // a block out of range; of the prefix, or its parts are not there or several groups'
     int group = -1, before = 0;  // CL and PX: the pair's group, and keys of its prefix that come before its own
     if constexpr (CL) {
         const int pair = blockIdx.x / kCluster, rank = blockIdx.x % kCluster;
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kPbThreads, 2) paged_batch_kernel(const __grid
         if constexpr (PX) {
             group = prefix_group(px, at.b);
             if (px.within && group >= 0) before = prefix_len(px, group);
-            bad_prefix = !px.within && group >= 0 && prefix_tiles_before(px, group + 1) > px.tiles_run;
+            bad_prefix = group == kSeveralGroups || (!px.within && group >= 0 && prefix_tiles_before(px, group + 1) > px.tiles_run);
         }
         at.len = before + seq_len(a, at.b);
         at.tiles = (at.len + Ge::kTile - 1) / Ge::kTile;
@@ -775,6 +775,7 @@ __global__ void __launch_bounds__(kPxJoinThreads) paged_batch_prefix_join_kernel
         const bool has = col < columns && mine < share;
         const int g = col / (D / 4), c = col % (D / 4) * 4;
         Joined j;
+        j.void_prefix = group == kSeveralGroups;
         if (has) {
             for (int p = mine; p < parts; p += share) {
                 const float *rec = part(p);

@@ -31,10 +31,18 @@ B200_DEVICE int prefix_len(const PrefixArgs &a, int group) {
     const int64_t n = __ldg(a.lens + group);
     return static_cast<int>(n < 0 ? 0 : (n > a.max_keys ? a.max_keys : n));
 }
-// The group of sequence b, or -1; by a whole warp.
+// The group of sequence b, by a whole warp: -1 if none names it, kSeveralGroups if more than one does, which takes offsets out of
+// order. Their CTAs write the same places of the parts then, in any order, so such a row is cleared.
+constexpr int kSeveralGroups = -2;
 B200_DEVICE int prefix_group(const PrefixArgs &a, int b) {
-    const int g = a.n_groups > 0 ? warp_find_row(a.cu, a.n_groups, b) : -1;
-    return g >= 0 && __ldg(a.cu + g) >= 0 && __ldg(a.cu + g + 1) <= a.n_seqs ? g : -1;
+    int group = -1, n = 0;
+    for (int g = threadIdx.x & 31; g < a.n_groups; g += 32) {
+        const int from = __ldg(a.cu + g), to = __ldg(a.cu + g + 1);
+        if (from >= 0 && from <= b && b < to && to <= a.n_seqs) group = g, ++n;
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    group = __reduce_max_sync(0xffffffffu, group);
+    return n > 1 ? kSeveralGroups : group;
 }
 // Where part i's numbers for (sequence b, query head h) are.
 B200_DEVICE int64_t prefix_row(const PrefixArgs &a, int part, int64_t b, int h) {
