@@ -13,9 +13,10 @@
 //  * A row of Q is scaled by a power of two to a largest magnitude in [2^14, 2^15) and enters as one F16 number (F16, BF16: exact, or
 //    2^-39 of the row's largest) or as two (F32: 22 bits). Up to eight query heads the second takes the unused rows 8 .. 15
 //    of the same product.
-//  * The scales 2^ek multiply the scores. The scales 2^ev go into the weights: w_j = 2^(t_j log2 e + ev_j - N + 14), N the running maximum of
-//    the exponent, as two F16 numbers. N has a maximum of its own, so keys whose V is far larger than that of the heaviest key keep their
-//    bits; the sum of the weights goes by the scores' maximum M. At the end 2^(N - M - 14) takes both together.
+//  * The scales 2^ek multiply the scores. The scales 2^ev go into the weights: w_j = 2^(t_j log2 e - M + ev_j - N + 14), M the running maximum
+//    of the scores and N the least whole number that no t_j log2 e - M + ev_j passes, as two F16 numbers. N is a maximum of its own, so keys whose
+//    V is far larger than that of the heaviest key keep their bits; the sum of the weights goes by M. At the end 2^(N - 14) takes both together.
+//    N counts from M, so that scores however large leave ev_j its bits, and is whole, so that differences of N are exact.
 // 64 BF16 sequences of 5 to 4069 keys, 32 / 8 heads of 128 (273 MB): 61 to 64 us with the join, 4.4 TB/s, 67 % of a large copy's rate; 16 F32
 // sequences of 1500 to 7548 keys, 16 / 8 heads (147 MB): 37 us, 3.9 TB/s. With half the bytes a key the instructions count as much as HBM
 // (issue active 41 %, two CTAs an SM), and the start (3.6 us of dependent look-ups), the pairs' ends and the join (4 to 5 us) weigh twice.
@@ -38,7 +39,8 @@ constexpr int kP8Tile = kP8Sub * kP8Warps;  // keys of a tile
 // Units of the line a tile and a pair's start and end take: 1.6 to 1.8 us against 2.4 (64 ragged sequences; shares of equal tiles ended
 // between 50 and 69 us).
 constexpr int kP8TileUnits = 2, kP8PairUnits = 3;
-constexpr int kP8Top = 14;                  // weights are at most 2^14, F16's largest power of two but one
+constexpr int kP8Top = 14;                  // weights are at most 2^14 (2^14.2), F16's largest power of two but one
+constexpr float kP8Large = 1048576.f;       // scores from here on, in powers of two, hold 1/8 at best
 
 struct P8Args {
     const void *q = nullptr;
@@ -75,21 +77,27 @@ struct P8Geometry {
 };
 
 B200_DEVICE float p8_pow2(int e) { return __uint_as_float(static_cast<uint32_t>(max(-126, min(127, e)) + 127) << 23); }
-// 2^x of numbers that may leave its range by half
-B200_DEVICE float p8_unscale(float x, float e) {
-    const float f = exp2_approx(0.5f * e);
-    return x * f * f;
+// x 2^(n - 14) for a whole n; -inf: there was no weight, or only such as are no numbers
+B200_DEVICE float p8_unscale(float x, float n) {
+    const int e = static_cast<int>(fmaxf(n, -1000.f)) - kP8Top, half = e >> 1;  // 2^e may lie outside F32's range
+    return x * p8_pow2(half) * p8_pow2(e - half);
+}
+// the smaller of x >= 0 and F32's largest; NaN stays
+B200_DEVICE float p8_finite(float x) {
+    float y;
+    asm("min.NaN.f32 %0, %1, 0f7F7FFFFF;" : "=f"(y) : "f"(x));
+    return y;
 }
 // m - M for running maxima of which both may be -inf
 B200_DEVICE float p8_less(float m, float M) { return m - (M == -INFINITY ? 0.f : M); }
 
-// Four columns of a head's output: o 2^(N - M - 14) / l, `shift` being N - M; zeros where there is no weight.
+// Four columns of a head's output: o 2^(N - 14) / l; zeros where there is no weight.
 template <typename T>
-B200_DEVICE void p8_write(T *to, const float (&o)[4], float l, float shift) {
+B200_DEVICE void p8_write(T *to, const float (&o)[4], float l, float n) {
     const float inv = l != 0.f ? 1.0f / l : 0.f;
     T x[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = from_f32<T>(l != 0.f ? p8_unscale(o[j] * inv, shift - static_cast<float>(kP8Top)) : 0.f);
+    for (int j = 0; j < 4; ++j) x[j] = from_f32<T>(l != 0.f ? p8_unscale(o[j] * inv, n) : 0.f);
     if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(to) = *reinterpret_cast<const float4 *>(x);
     else *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(x);
 }
@@ -210,7 +218,8 @@ struct P8State {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const float y = FULL ? s[0][j][2 * r + u] : s[0][j][u] + s[NS - 1][j][2 + u];
-                    x[j][u] = y * (qs[r] * ke[j][u]);  // (a large row of Q against small keys, or the inverse, stays in range)
+                    // (a large row of Q against small keys, or the inverse, stays in range; a score of 0 is one for any scales)
+                    x[j][u] = y * p8_finite(qs[r] * ke[j][u]);
                     if (live != ~0u && !((live >> (8 * j + t2 + u)) & 1u)) x[j][u] = -INFINITY;
                     mx = fmaxf(mx, x[j][u]);
                     nx = fmaxf(nx, x[j][u] + ve[j][u]);
@@ -219,10 +228,26 @@ struct P8State {
             nx = fmaxf(nx, __shfl_xor_sync(0xffffffffu, nx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             nx = fmaxf(nx, __shfl_xor_sync(0xffffffffu, nx, 2));
-            const float mn = fmaxf(m[r], mx), nn = fmaxf(n[r], nx);
-            if (__any_sync(0xffffffffu, mn > m[r] || nn > n[r])) {
-                l[r] *= exp2_approx(p8_less(m[r], mn));
-                const float f = exp2_approx(p8_less(n[r], nn));
+            const float mn = fmaxf(m[r], mx), ms = mn == -INFINITY ? 0.f : mn, moved = m[r] - ms;
+            float nn = ceilf(fmaxf(n[r] + moved, nx - ms));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) x[j][u] -= ms;
+            const bool large = fabsf(ms) >= kP8Large;
+            if (__any_sync(0xffffffffu, mn > m[r] || nn > n[r] || large)) {
+                if (__any_sync(0xffffffffu, large)) {  // ev is lost in such scores, not in their differences
+                    nx = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) nx = fmaxf(nx, x[j][u] + ve[j][u]);
+                    nx = fmaxf(nx, __shfl_xor_sync(0xffffffffu, nx, 1));
+                    nx = fmaxf(nx, __shfl_xor_sync(0xffffffffu, nx, 2));
+                    nn = ceilf(fmaxf(n[r] + moved, nx));
+                }
+                l[r] *= exp2_approx(moved);
+                const float f = exp2_approx(p8_less(n[r], nn) + moved);
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c)
 #pragma unroll
@@ -230,11 +255,11 @@ struct P8State {
             }
             m[r] = mn;
             n[r] = nn;
-            const float ms = mn == -INFINITY ? 0.f : mn, ns = (nn == -INFINITY ? 0.f : nn) - static_cast<float>(kP8Top);
+            const float ns = (nn == -INFINITY ? 0.f : nn) - static_cast<float>(kP8Top);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                l[r] += exp2_approx(x[j][0] - ms) + exp2_approx(x[j][1] - ms);
-                const float w0 = exp2_approx(x[j][0] + ve[j][0] - ns), w1 = exp2_approx(x[j][1] + ve[j][1] - ns);
+                l[r] += exp2_approx(x[j][0]) + exp2_approx(x[j][1]);
+                const float w0 = exp2_approx(x[j][0] + (ve[j][0] - ns)), w1 = exp2_approx(x[j][1] + (ve[j][1] - ns));
                 const uint32_t h = pack2<__half>(w0, w1);
                 const float2 f = unpack2<__half>(h);
                 hi[j >> 1][(j & 1) * R + r] = h;
@@ -426,24 +451,24 @@ __global__ void __launch_bounds__(kP8Threads, kP8Ctas) paged_q8_kernel(const __g
             float *rec = CL ? own : a.ws + (static_cast<int64_t>(blockIdx.x) * 2 + (part_t0 == 0)) * Ge::kRec;
             for (int i = 4 * threadIdx.x; i < heads * D; i += 4 * kP8Threads) {
                 const int g = i / D;
-                float M = -INFINITY, N = -INFINITY;
+                float M = -INFINITY, N = -INFINITY, ls = 0.f, os[4] = {};
 #pragma unroll
-                for (int w = 0; w < kP8Warps; ++w) {
-                    M = fmaxf(M, stat[w * 3 * HB + g]);
-                    N = fmaxf(N, stat[w * 3 * HB + 2 * HB + g]);
-                }
-                float ls = 0.f, os[4] = {};
+                for (int w = 0; w < kP8Warps; ++w) M = fmaxf(M, stat[w * 3 * HB + g]);
+#pragma unroll
+                for (int w = 0; w < kP8Warps; ++w) N = fmaxf(N, stat[w * 3 * HB + 2 * HB + g] + p8_less(stat[w * 3 * HB + g], M));
+                N = ceilf(N);
 #pragma unroll
                 for (int w = 0; w < kP8Warps; ++w) {
                     const float4 x =
                         *reinterpret_cast<const float4 *>(p8_smem + w * Ge::kStages * 2 * Ge::kHalf + part_at + i * 4);
-                    ls = fmaf(exp2_approx(p8_less(stat[w * 3 * HB + g], M)), stat[w * 3 * HB + HB + g], ls);
-                    const float f = exp2_approx(p8_less(stat[w * 3 * HB + 2 * HB + g], N));
+                    const float moved = p8_less(stat[w * 3 * HB + g], M);
+                    ls = fmaf(exp2_approx(moved), stat[w * 3 * HB + HB + g], ls);
+                    const float f = exp2_approx(p8_less(stat[w * 3 * HB + 2 * HB + g], N) + moved);
                     os[0] = fmaf(f, x.x, os[0]), os[1] = fmaf(f, x.y, os[1]);
                     os[2] = fmaf(f, x.z, os[2]), os[3] = fmaf(f, x.w, os[3]);
                 }
                 if (whole) {
-                    p8_write<T>(static_cast<T *>(a.out) + at.b * a.o_seq + (h0 + g) * a.o_head + (i - g * D), os, ls, p8_less(N, M));
+                    p8_write<T>(static_cast<T *>(a.out) + at.b * a.o_seq + (h0 + g) * a.o_head + (i - g * D), os, ls, N);
                 } else {
                     *reinterpret_cast<float4 *>(rec + i) = make_float4(os[0], os[1], os[2], os[3]);
                     if (i == g * D) rec[HB * D + g] = M, rec[HB * (D + 1) + g] = ls, rec[HB * (D + 2) + g] = N;
@@ -474,24 +499,28 @@ __global__ void __launch_bounds__(kP8Threads, kP8Ctas) paged_q8_kernel(const __g
                 o[c] = ld_dsmem(dsmem_addr(own + i, c));
             }
 #pragma unroll
-            for (int c = 0; c < kP8Cluster; ++c) M = fmaxf(M, m[c]), N = fmaxf(N, s[c]);
+            for (int c = 0; c < kP8Cluster; ++c) M = fmaxf(M, m[c]);
+#pragma unroll
+            for (int c = 0; c < kP8Cluster; ++c) m[c] = p8_less(m[c], M), N = fmaxf(N, s[c] + m[c]);
+            N = ceilf(N);
             float ls = 0.f, os = 0.f;
 #pragma unroll
             for (int c = 0; c < kP8Cluster; ++c) {
-                ls = fmaf(exp2_approx(p8_less(m[c], M)), l[c], ls);
-                os = fmaf(exp2_approx(p8_less(s[c], N)), o[c], os);
+                ls = fmaf(exp2_approx(m[c]), l[c], ls);
+                os = fmaf(exp2_approx(p8_less(s[c], N) + m[c]), o[c], os);
             }
             static_cast<T *>(a.out)[start.b * a.o_seq + (h0 + g) * a.o_head + (i - g * D)] =
-                from_f32<T>(ls != 0.f ? p8_unscale(os / ls, p8_less(N, M) - static_cast<float>(kP8Top)) : 0.f);
+                from_f32<T>(ls != 0.f ? p8_unscale(os / ls, N) : 0.f);
         }
         cluster_sync();  // no CTA's shared memory goes away while it is read
     }
 }
 
 // Joins the parts of each pair that more than one CTA took, and clears the rows of empty sequences. One CTA a pair, a thread four
-// columns at a time; it asks for all of a few parts' numbers at once, so that their latency is paid once.
+// columns at a time; it asks for all of a few parts' numbers at once, so that their latency is paid once. (The registers of two CTAs an SM:
+// with the compiler's own choice, 48, some loads wait for others; 16 F32 sequences 38.9 us against 37.4.)
 template <typename T, int D, int HB>
-__global__ void __launch_bounds__(kP8JoinThreads) paged_q8_join_kernel(const __grid_constant__ P8Args a, const int64_t grid) {
+__global__ void __launch_bounds__(kP8JoinThreads, 2) paged_q8_join_kernel(const __grid_constant__ P8Args a, const int64_t grid) {
     using Ge = P8Geometry<D, HB>;
     const int b = static_cast<int>(blockIdx.x / a.VH), vh = static_cast<int>(blockIdx.x % a.VH);
     const int64_t before = tiles_before<kP8Tile, kP8TileUnits, kP8PairUnits>(a, b);
@@ -517,7 +546,7 @@ __global__ void __launch_bounds__(kP8JoinThreads) paged_q8_join_kernel(const __g
         const int g = j / D;
         float M = -INFINITY, N = -INFINITY, l = 0.f, o[4] = {};
         for (int i0 = 0; i0 < parts; i0 += kAtOnce) {
-            float m[kAtOnce], n[kAtOnce], ls[kAtOnce], Mn = M, Nn = N;
+            float m[kAtOnce], n[kAtOnce], ls[kAtOnce], Mn = M;
             float4 x[kAtOnce];
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i) {
@@ -528,22 +557,27 @@ __global__ void __launch_bounds__(kP8JoinThreads) paged_q8_join_kernel(const __g
                 n[i] = __ldcg(p + HB * (D + 2) + g);
             }
 #pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) Mn = fmaxf(Mn, m[i]), Nn = fmaxf(Nn, n[i]);
-            l *= exp2_approx(p8_less(M, Mn));
-            const float f = exp2_approx(p8_less(N, Nn));
+            for (int i = 0; i < kAtOnce; ++i) Mn = fmaxf(Mn, m[i]);
+            const float moved = p8_less(M, Mn);
+            float Nn = N + moved;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) m[i] = p8_less(m[i], Mn), Nn = fmaxf(Nn, n[i] + m[i]);
+            Nn = ceilf(Nn);
+            l *= exp2_approx(moved);
+            const float f = exp2_approx(p8_less(N, Nn) + moved);
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] *= f;
             M = Mn, N = Nn;
 #pragma unroll
             for (int i = 0; i < kAtOnce; ++i) {
                 if (i0 + i >= parts) break;
-                l = fmaf(exp2_approx(p8_less(m[i], M)), ls[i], l);
-                const float w = exp2_approx(p8_less(n[i], N));
+                l = fmaf(exp2_approx(m[i]), ls[i], l);
+                const float w = exp2_approx(p8_less(n[i], N) + m[i]);
                 o[0] = fmaf(w, x[i].x, o[0]), o[1] = fmaf(w, x[i].y, o[1]);
                 o[2] = fmaf(w, x[i].z, o[2]), o[3] = fmaf(w, x[i].w, o[3]);
             }
         }
-        p8_write<T>(out + g * a.o_head + (j - g * D), o, l, p8_less(N, M));
+        p8_write<T>(out + g * a.o_head + (j - g * D), o, l, N);
     }
 }
 
