@@ -301,6 +301,9 @@ B200_DEVICE int exps_word(int e, bool wide) { return 2 * e + static_cast<int>(wi
 B200_DEVICE int exps_exponent(int word) { return word >> 1; }
 B200_DEVICE bool exps_wide(int word) { return word & 1; }
 constexpr int kMostScale = 100;  // exponents of Q and K that add up past it: their product takes FFMA
+// Scores (in powers of two) from here on: s sl2 - m in one operation is off by up to 2^-23 of m from the rounded m that it should be 0
+// for, and weights leave F16's range. F32 tiles take FFMA then (its scores are rounded first), 16-bit prefixes are formed again by the join.
+constexpr float kLargeScoreF32 = 8388608.f, kLargeScore = 67108864.f;
 
 // A tile's place in `exps`: increasing along the packed keys for any lengths, since
 // floor(x) + ceil(y) <= floor(x + y) + 1.
@@ -1006,6 +1009,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                     }
             }
             const float m = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * sl2;
+            wide |= fabsf(m) >= kLargeScoreF32 && m != -INFINITY;
             const float shift_p = static_cast<float>(kTop) - (m == -INFINITY ? 0.f : m);
             const uint64_t scale2 = pair_of(sl2, sl2), shift2 = pair_of(shift_p, shift_p);
             uint64_t sum2[4] = {};
@@ -1257,6 +1261,7 @@ __global__ void __launch_bounds__(kPtThreads<T, SL>, SL == 1 ? 2 : 1)
                 }
             }
         }
+        if (PX && fabsf(m_row) >= kLargeScore && m_row != -INFINITY) l_row = __uint_as_float(0x7FC00000u);
         if (!whole_out) {
             if (live && (!kJoin || slot == 0)) part_ml[part_row] = make_float2(m_row, PX && !ok ? -1.f : l_row);  // (-1: not to be used)
         } else if constexpr (!kJoin) {

@@ -13,7 +13,7 @@ from test_gpu_q8 import DT, UNIT, Cache, cumulative, gen, ints
 
 pytestmark = pytest.mark.gpu
 
-TARGETS = [1e4, 1e6, 3e7, 1e8, 1e10, 1e15, 1e25]
+TARGETS = [1e4, 3e7, 1e8, 1e10, 1e25]
 
 
 def rows(n, target, Hq, Hkv, D, kind):
@@ -83,3 +83,37 @@ def test_8_bit_cache_scores_of_zero_between_large_rows(cuda, kind):
     want = c.values(0)[1].mean(0).repeat_interleave(2, 0)
     got = B.flash_attn_paged_batch_q8(q, *c.args, c.table, c.seq_lens)[0].double()
     assert ((got - want).abs() <= UNIT[kind] * want.abs() + 1e-5 * (want.abs() + float(want.square().mean().sqrt()))).all()
+
+
+def pool(x, block=16):
+    n = -(-x.shape[0] // block)
+    p = torch.zeros((n, block) + x.shape[1:], dtype=x.dtype, device=x.device)
+    p.view(-1, *x.shape[1:])[:x.shape[0]] = x
+    return p
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("layout", [(16, 8, 128), (8, 4, 64)])
+@pytest.mark.parametrize("n", [1, 300, 2500])
+@pytest.mark.parametrize("seqs", [9, 150])
+@pytest.mark.parametrize("target", TARGETS)
+def test_shared_prefix(cuda, kind, layout, n, seqs, target):
+    if not possible(kind, target):
+        return
+    q, k, v = rows(n, target, *layout, kind)
+    kp, vp = pool(k), pool(v)
+    table = torch.arange(kp.shape[0], dtype=torch.int32, device=cuda)[None]
+    own = torch.zeros((seqs, 1), dtype=torch.int32, device=cuda)  # the first key again, of some
+    lens = [s % 2 if n > 1 else 0 for s in range(seqs)]
+    got = B.flash_attn_paged_shared(q.expand(seqs, -1, -1).contiguous(), kp, vp, table, ints([n]), ints([0, seqs]), own, ints(lens))
+    close(got, v[min(3, n - 1)].repeat_interleave(layout[0] // layout[1], 0), kind)
+
+
+@pytest.mark.parametrize("layout", [(16, 8, 128), (8, 4, 64)])
+@pytest.mark.parametrize("n", [300, 2500])
+@pytest.mark.parametrize("target", TARGETS)
+def test_packed_f32(cuda, layout, n, target):
+    """Queries of a prompt's end, each behind the deciding key."""
+    q, k, v = rows(n, target, *layout, "f32")
+    got = B.flash_attn_packed(q.expand(200, -1, -1).contiguous(), k, v, ints([0, 200]), ints([0, n]))
+    close(got, v[3].repeat_interleave(2, 0), "f32")
