@@ -314,12 +314,12 @@ typedef struct b200_kv_pool_q8 {
     int64_t n_head_kv, head_dim;
 } b200_kv_pool_q8;
 
-/* b200_paged_kv_append into an 8-bit pool; k, v are F32, F16 or BF16 (`dtype`). Each row gets the least
- * whole e >= -127 with max |x| <= 448 2^e, and its elements x 2^-e (exact) rounded to e4m3, ties to even: at
- * most 2^-4 of the element off, or 2^(e - 10) where that is more. (Elements of 248 2^120 or more become 2^128, which reads as
- * infinite.) A row that holds an infinity or a NaN is
- * held as zeros with the scale NaN, and reads as NaN. Rows outside every sequence, and those whose offsets, position or
- * block are out of range, are left out and B200_DEV_BAD_POSITION recorded. */
+/* b200_paged_kv_append into an 8-bit pool; k, v are F32, F16 or BF16 (`dtype`). Each row gets the least whole e >=
+ * -127 with max |x| <= 448 2^e, and its elements x 2^-e (exact) rounded to e4m3, ties to even: at most 2^-4 of the
+ * element off, or 2^(e - 10) where that is more. (Elements of 248 2^120 or more become 2^128, which reads as
+ * infinite.) A row that holds an infinity or a NaN is held as zeros with the scale NaN, and reads as NaN. Rows
+ * outside every sequence, and those whose offsets, position or block are out of range, are left out and
+ * B200_DEV_BAD_POSITION recorded. */
 int b200_paged_kv_append_q8(const void *k, int64_t k_tok_stride, int64_t k_head_stride, const void *v,
                             int64_t v_tok_stride, int64_t v_head_stride, int32_t dtype, const int32_t *cu_new,
                             const int32_t *seq_lens, int64_t n_seqs, int64_t n_tokens, const b200_kv_pool_q8 *pool,
@@ -329,8 +329,8 @@ int b200_paged_kv_append_q8(const void *k, int64_t k_tok_stride, int64_t k_head_
 /* The inverse: rows of an 8-bit pool into packed rows k, v [n_rows][Hkv][D] of F32, F16 or BF16, as
  * b200_flash_attn_packed takes them. Sequence s gets the rows [cu_rows[s], cu_rows[s + 1]), which are its last
  * positions of the seq_lens[s] cached (all of them where the counts are equal). Values q 2^e are exact in F32
- * (infinite past its largest) and in BF16 (which rounds to multiples of 2^-133), and rounded once to F16. Rows outside every sequence are left untouched; a row whose offsets, position or block
- * are out of range is zero. */
+ * (infinite past its largest) and in BF16 (which rounds to multiples of 2^-133), and rounded once to F16. Rows
+ * outside every sequence are left untouched; a row whose offsets, position or block are out of range is zero. */
 int b200_paged_kv_read_q8(const b200_kv_pool_q8 *pool, const int32_t *block_table, int64_t table_stride,
                           int64_t max_blocks, const int32_t *cu_rows, const int32_t *seq_lens, int64_t n_seqs,
                           int64_t n_rows, void *k, int64_t k_tok_stride, int64_t k_head_stride, void *v,
@@ -349,16 +349,22 @@ size_t b200_flash_attn_paged_batch_q8_workspace_bytes(int64_t n_seqs, int64_t ma
                                                       int64_t Hkv);
 
 /* b200_flash_attn_paged_batch for sequences that share prefixes (a common instruction, a document): group g is the
- * sequences [cu_seqs[g], cu_seqs[g + 1]), which see the prefix_lens[g] positions of row g of prefix_table
- * first, then the seq_lens[s] positions of their own rows of block_table (either may be 0; both tables name
- * blocks of the one pool). Each prefix is read once for up to 128 rows (sequences times query heads) of its group. Weights
- * are two numbers of the element type for 16-bit caches, as in b200_flash_attn_paged_batch; a prefix's F32 products are three of F16 numbers
- * with 22 bits, or F32 FFMA (short prefixes with few rows, more than 128 query heads a KV head, planes past a GiB of workspace). Few
- * short sequences (at most 4096 positions with their prefix) run as in b200_flash_attn_paged_batch. Sequences outside every
- * group see their own positions alone. A prefix with a block index out of range makes its group's rows zero. Where cu_seqs
- * is out of order, rows of sequences that several groups name are zero (others may be, where such groups have more tiles than groups in
- * order). cu_seqs, prefix_lens and prefix_table are else treated as the other offsets, lengths and tables. `workspace` as there, with max_prefix =
- * prefix_blocks * block_tokens; one for n_seqs does for fewer, but F32 planes come and go with n_groups. */
+ * sequences [cu_seqs[g], cu_seqs[g + 1]), which see the prefix_lens[g] positions of row g of prefix_table first,
+ * then the seq_lens[s] positions of their own rows of block_table (either may be 0; both tables name blocks of the
+ * one pool). Each prefix is read once for up to 128 rows (sequences times query heads) of its group. Weights are two
+ * numbers of the element type for 16-bit caches, as in b200_flash_attn_paged_batch; a prefix's F32 products are
+ * three of F16 numbers with 22 bits, or F32 FFMA (short prefixes with few rows, more than 128 query heads a KV head,
+ * planes past a GiB of workspace). Few short sequences (at most 4096 positions with their prefix) run as in
+ * b200_flash_attn_paged_batch. Sequences outside every group see their own positions alone. Work is cut as if all
+ * n_groups groups were alike and tables full, so sequences without a prefix are best left outside, and tables no
+ * wider than they have to be (F32 planes are as large as prefix_table). A few sequences behind a long prefix can be
+ * faster by b200_flash_attn_paged_batch over tables that name the prefix's blocks first. Rows whose result is no
+ * finite number are formed again key by key for 16-bit caches, in milliseconds behind a long prefix, as there. A
+ * prefix with a block index out of range makes its group's rows zero. Where cu_seqs is out of order, rows of
+ * sequences that several groups name are zero (others may be, where such groups have more tiles than groups in
+ * order). cu_seqs, prefix_lens and prefix_table are else treated as the other offsets, lengths and tables.
+ * `workspace` as there, with max_prefix = prefix_blocks * block_tokens; one for n_seqs does for fewer, but F32
+ * planes come and go with n_groups. */
 int b200_flash_attn_paged_shared(const void *q, int64_t q_seq_stride, int64_t q_head_stride, void *out,
                                  int64_t out_seq_stride, int64_t out_head_stride, const b200_kv_pool *pool,
                                  const int32_t *prefix_table, int64_t prefix_stride, int64_t prefix_blocks,

@@ -3,14 +3,15 @@
 //   x <- x / r or x r (known), x - f count - p (drawn), x + bias, -inf (masked)
 //
 // A pass over the logits, which HBM bounds, by CTAs that take a chunk of a row's vocabulary each. What a row's history and biases say
-// concerns few tokens: a CTA walks them for those of its chunk, sets a bit a token, counts the bits before each word, and so has a slot of its
-// own for each such token, in which it counts; the pass then writes the chunk with the masked tokens replaced, and last come the tokens
-// with slots, a thread each. Half of the warps pass and half walk at the same time, since the walk's chain (offsets, tokens, counters) is as
-// long as the pass. The pass goes through a ring in shared memory that bulk copies fill and empty; a thread takes a mask word and its 32 tokens.
-// 256 rows of 151936 F32 with up to 4000 tokens of history, masks and biases: 70 us, 4.5 TB/s, 69 % of a large copy's rate; the pass alone 55
-// with masks, 53 without (a library copy of these bytes 51). What is left is the walk, and the named tokens' scattered reads and writes.
-// Otherwise: a mask word looked up for each vector of four 74 us for the pass; the pass through registers 82 in all, whole chunks in shared
-// memory 112, two kernels 80 to 123; three stages and three CTAs an SM 74, five CTAs with half the slots 71. Counts are whole numbers, so their order does not matter.
+// concerns few tokens: a CTA walks them for those of its chunk, sets a bit a token, counts the bits before each word, and so has a
+// slot of its own for each such token, in which it counts; the pass then writes the chunk with the masked tokens replaced, and
+// last come the tokens with slots, a thread each. Half of the warps pass and half walk at the same time, since the walk's chain
+// (offsets, tokens, counters) is as long as the pass. The pass goes through a ring in shared memory that bulk copies fill and
+// empty; a thread takes a mask word and its 32 tokens. 256 rows of 151936 F32 with up to 4000 tokens of history, masks and biases:
+// 70 us, 4.5 TB/s, 69 % of a large copy's rate; the pass alone 55 with masks, 53 without (a library copy of these bytes 51). What
+// is left is the walk, and the named tokens' scattered reads and writes. Otherwise: a mask word looked up for each vector of four
+// 74 us for the pass, 88 in all; the pass through registers 82 in all, whole chunks in shared memory 112, two kernels 80 to 123;
+// three stages and three CTAs an SM 74, five CTAs with half the slots 71. Counts are whole numbers, so their order does not matter.
 #include "batch.cuh"
 #include "gemv.cuh"
 #include "tcgen05.cuh"

@@ -42,10 +42,12 @@ constexpr size_t ffma_smem() {
     return (2 * static_cast<size_t>(D) * kPkPad + static_cast<size_t>(kPkKeys) * D) * 4;
 }
 
-// Rows [r0, r0 + rows) (row = token * G + head of the KV head's group; at most kPkRows) of sequence p against its
-// keys [first, end), RT rows a thread (fewer than kPkRows: 16 RT at most) (CAUSAL: those that each sees; key(j, k, v) points at key j's rows, false: it takes no part), by kPkThreads threads, of which this is `tid`; sync() is their barrier and
-// smem (16-byte aligned, ffma_smem<D>() bytes) theirs. store(row, column, x, m, l) gets each row's
-// output four columns at a time, already over l, its maximum (in powers of two) and its sum.
+// Rows [r0, r0 + rows) of sequence p (row = token * G + head of the KV head's group) against its keys [first, end), with CAUSAL
+// those that each row sees. kPkThreads threads take RT rows each, so rows is at most 16 RT (kPkRows with RT 4); this one is `tid`.
+//  * key(j, k, v) points at key j's rows; false: it takes no part.
+//  * sync() is the threads' barrier, smem (16-byte aligned, ffma_smem<D>() bytes) theirs.
+//  * store(row, column, x, m, l) gets each row's output four columns at a time, already over l, its maximum (in powers of
+//    two) and its sum.
 template <typename T, int D, bool CAUSAL, int RT = 4, typename Key, typename Sync, typename Store>
 B200_DEVICE void ffma_rows(const PackedArgs &a, const PackedTile &p, int kvh, int r0, int rows, int first, int end, Key key,
                            float *smem, int tid, Sync sync, Store store) {

@@ -51,7 +51,7 @@
 // Bound: at long contexts the chain scores -> softmax -> P -> product of a slot, against which the other
 // slot's runs: 8192 BF16 tokens, 32 / 8 heads of 128, 505 to 522 us by GPU, 1.05 to 1.09 PFLOP/s (64 to 66 % of a
 // large library matrix product's rate); the tensor cores are busy 54 to 60 % of the time. 2048 F32 tokens, 16 / 8
-// heads of 128, 76 to 79 us (217 to 225 TFLOP/s of the call's, 660 of the three products), 3 of them less since the split kernel is faster. Short
+// heads of 128, 76 to 79 us (217 to 225 TFLOP/s of the call's, 660 of the three products). Short
 // calls: a CTA's start and end, ~6 us (look-up 1, first copies 1.4, last product 0.8 to 1.7, output 2), beside ~0.9
 // us a step: 10 prompts of 1 to 1333 BF16 tokens, 16 / 8 heads of 128, 35 us. Two slots take all 512
 // columns of tensor memory and most of an SM's registers.
@@ -302,7 +302,8 @@ B200_DEVICE int exps_exponent(int word) { return word >> 1; }
 B200_DEVICE bool exps_wide(int word) { return word & 1; }
 constexpr int kMostScale = 100;  // exponents of Q and K that add up past it: their product takes FFMA
 // Scores (in powers of two) from here on: s sl2 - m in one operation is off by up to 2^-23 of m from the rounded m that it should be 0
-// for, and weights leave F16's range. F32 tiles take FFMA then (its scores are rounded first), 16-bit prefixes are formed again by the join.
+// for, and weights leave F16's range. F32 tiles take FFMA then (its scores are rounded first), 16-bit prefixes are formed again by
+// the join.
 constexpr float kLargeScoreF32 = 8388608.f, kLargeScore = 67108864.f;
 
 // A tile's place in `exps`: increasing along the packed keys for any lengths, since
@@ -337,10 +338,11 @@ template <int D>
 constexpr int kSplitThreads = 4 * D;  // a thread holds eight float4 of the tile
 
 // One CTA: the K or V rows of one key tile and KV head, as hi and lo planes with the tile's
-// exponent, and whether its rows and columns spread too far for one. A pass over the bytes: HBM bounds it (2048 keys, 8 heads of 128: 17 MB in, 17 MB out;
-// the attention kernel's start overlaps it). All loads come before the first reduction, which would else wait for each.
-// PX: of a prefix's blocks, tile after tile of a group's room, read past L2's room for the planes (8192 keys, 8 heads of 128, 67 MB in and out:
-// 31 us; with half the threads 33, with loads and reductions in one loop 42, both 47; with twice the threads 45).
+// exponent, and whether its rows and columns spread too far for one. The arithmetic of the split bounds it (math pipe; 2048 keys, 8
+// heads of 128: 17 MB in, 17 MB out; the attention kernel's start overlaps it). All loads come before the first reduction, which
+// would else wait for each.
+// PX: of a prefix's blocks, tile after tile of a group's room, read past L2's room for the planes (8192 keys, 8 heads of 128, 67 MB
+// in and out: 31 us; with half the threads 33, with loads and reductions in one loop 42, both 47; with twice the threads 45).
 template <int D, bool PX>
 __global__ void __launch_bounds__(kSplitThreads<D>, 256 / D)
     packed_split_kernel(const PackedArgs a, const PrefixArgs px, __half *planes, int32_t *exps) {

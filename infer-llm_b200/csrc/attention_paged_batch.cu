@@ -381,8 +381,8 @@ B200_DEVICE void report_groups(const PrefixArgs &px, int32_t *status) {
     }
 }
 
-// The CTAs' shares of the line of `total` units: with prefixes, the first `early` CTAs, which run beside the prefixes' kernel on SMs of their
-// own, take `gap` units more than those that start when it ends, or all where that is enough for them. CTA c takes
+// The CTAs' shares of the line of `total` units: with prefixes, the first `early` CTAs, which run beside the prefixes' kernel on
+// SMs of their own, take `gap` units more than those that start when it ends, or all where that is enough for them. CTA c takes
 // the units [begin(c), begin(c + 1)), TU of them at least.
 struct Shares {
     int64_t total, ctas, early, gap;

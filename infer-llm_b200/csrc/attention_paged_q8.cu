@@ -13,13 +13,15 @@
 //  * A row of Q is scaled by a power of two to a largest magnitude in [2^14, 2^15) and enters as one F16 number (F16, BF16: exact, or
 //    2^-39 of the row's largest) or as two (F32: 22 bits). Up to eight query heads the second takes the unused rows 8 .. 15
 //    of the same product.
-//  * The scales 2^ek multiply the scores. The scales 2^ev go into the weights: w_j = 2^(t_j log2 e - M + ev_j - N + 14), M the running maximum
-//    of the scores and N the least whole number that no t_j log2 e - M + ev_j passes, as two F16 numbers. N is a maximum of its own, so keys whose
-//    V is far larger than that of the heaviest key keep their bits; the sum of the weights goes by M. At the end 2^(N - 14) takes both together.
-//    N counts from M, so that scores however large leave ev_j its bits, and is whole, so that differences of N are exact.
-// 64 BF16 sequences of 5 to 4069 keys, 32 / 8 heads of 128 (273 MB): 61 to 64 us with the join, 4.4 TB/s, 67 % of a large copy's rate; 16 F32
-// sequences of 1500 to 7548 keys, 16 / 8 heads (147 MB): 37 us, 3.9 TB/s. With half the bytes a key the instructions count as much as HBM
-// (issue active 41 %, two CTAs an SM), and the start (3.6 us of dependent look-ups), the pairs' ends and the join (4 to 5 us) weigh twice.
+//  * The scales 2^ek multiply the scores. The scales 2^ev go into the weights: w_j = 2^(t_j log2 e - M + ev_j - N + 14), M the
+//    running maximum of the scores and N the least whole number that no t_j log2 e - M + ev_j passes, as two F16 numbers. N is a
+//    maximum of its own, so keys whose V is far larger than that of the heaviest key keep their bits; the sum of the weights goes
+//    by M. At the end 2^(N - 14) takes both together. N counts from M, so that scores however large leave ev_j its bits, and is
+//    whole, so that differences of N are exact.
+// 64 BF16 sequences of 5 to 4069 keys, 32 / 8 heads of 128 (273 MB): 62 to 64 us with the join, 4.3 TB/s, 66 % of a large copy's
+// rate; 16 F32 sequences of 1500 to 7548 keys, 16 / 8 heads (147 MB): 37.5 us, 3.9 TB/s. No unit is full (issue active 45 %,
+// tensor pipe 29 %): eight warps an SM wait for the fixed latencies of one chain, and the start (3.6 us of dependent look-ups),
+// the pairs' ends and the join (4 to 5 us) weigh twice at half the bytes a key.
 // Rows past a sequence's end are not read; they and keys of invalid blocks get weight 0.
 #include "paged_line.cuh"
 #include "paged_q8.cuh"
@@ -109,8 +111,8 @@ struct P8State {
     static constexpr bool FULL = HB > 8, TWO = __is_same(T, float);
     static constexpr int R = FULL ? 2 : 1;  // head rows a lane holds
     // A fragments of Q. 16 heads: of 16 dimensions, and of their second terms. Up to 8 heads: rows 0 .. 7 and 8 .. 15 are the two terms
-    // (TWO), or 16 dimensions and the next 16, of which a product with a key's 16 dimensions uses one half. Every fragment is four registers
-    // in a row as the instruction wants them; zeros in half of them would have to be moved there each time.
+    // (TWO), or 16 dimensions and the next 16, of which a product with a key's 16 dimensions uses one half. Every fragment is four
+    // registers in a row as the instruction wants them; zeros in half of them would have to be moved there each time.
     static constexpr int NQ = FULL || TWO ? D / 16 : D / 32;
     uint32_t q[NQ][4], ql[FULL && TWO ? NQ : 1][4];
     float o[D / 16][2][4];  // even and odd columns: rows g and g + 8; without FULL, row g's shares of the weights' two terms

@@ -10,9 +10,10 @@
 //  * the sequences' own keys, as in the batched decode (attention_paged_batch.cu);
 //  * the join of all parts.
 // Few short sequences take one launch of the batched decode instead, whose clusters read a prefix's keys as their sequence's first.
-// 64 BF16 sequences of 32 / 8 heads of 128 behind one prefix of 8192 keys, with 33 k keys of their own (165 MB): 46 us, of which the
-// join 5 to 6 after the own keys' end. A prefix CTA takes an SM's shared memory, so own keys run on the SMs that the plan leaves them (a small
-// CTA beside theirs took 61 against 63, but 56 against 47 behind 16384 keys). 4 F32 sequences of 16 / 8 heads behind 301 keys: 12 us, one launch.
+// 64 BF16 sequences of 32 / 8 heads of 128 behind one prefix of 8192 keys, with 33 k keys of their own (165 MB): 45 to 47 us, of which the
+// join 5 to 6 after the own keys' end. A prefix CTA takes an SM's shared memory, so own keys run on the SMs that the plan leaves
+// them (a small CTA beside theirs took 61 against 63, but 56 against 47 behind 16384 keys). 4 F32 sequences of 16 / 8 heads behind
+// 301 keys: 12 us, one launch.
 #include "attention_packed_ffma.cuh"
 #include "paged_batch.cuh"
 
@@ -57,8 +58,8 @@ struct PrefixPlan {
     int64_t room = 0;  // F32 on the tensor cores: positions a group in the planes
     int64_t early = 0;  // CTAs of the own keys that the prefixes' SMs leave room for
 };
-// Model of the tensor-core kernel and of the own keys' (us, kB a us): what a CTA's start and end and a tile of 128 keys take, and the rate of
-// own keys on all SMs.
+// Model of the tensor-core kernel and of the own keys' (us, kB a us): what a CTA's start and end and a tile of 128 keys take, and
+// the rate of own keys on all SMs.
 constexpr float kPxStart = 8.f, kPxStartF32 = 16.f, kPxTile = 2.5f, kPxTileF32 = 2.2f, kPxOwnRate = 4500.f;
 // The same start and tile in units of the own keys' line (0.7 us).
 constexpr int kGapStart = 10, kGapStartF32 = 20, kGapTile = 3;
@@ -67,12 +68,13 @@ PrefixPlan prefix_plan(int64_t n_seqs, int64_t max_keys, int64_t n_groups, int64
                        int32_t dtype) {
     PrefixPlan p;
     if (n_groups <= 0 || n_seqs <= 0 || max_prefix <= 0) return p;
-    // Few short pairs, prefixes included: one launch that reads a prefix once a sequence, from L2 after the first (4 sequences of 16 / 8 heads of
-    // 128 behind 300, 2000 and 3500 keys, one launch against a kernel of the prefixes' and the own keys': F32 12 us against 19, 18.5
-    // against 31, 24.6 against 45; BF16 12 against 17, 12.7 against 22.6, 16.6 against 24.5).
+    // Few short pairs, prefixes included: one launch that reads a prefix once a sequence, from L2 after the first (4 sequences of
+    // 16 / 8 heads of 128 behind 300, 2000 and 3500 keys, one launch against a kernel of the prefixes' and the own keys': F32 12
+    // us against 19, 18.5 against 31, 24.6 against 45; BF16 12 against 17, 12.7 against 22.6, 16.6 against 24.5).
     p.within = paged_batch_one_launch(n_seqs, max_keys + max_prefix, G, Hkv, dtype);
     if (p.within) return p;
-    // As if groups were alike.
+    // As if groups were alike, since the host knows neither lengths nor counts. (One of 32 sequences behind 8192 keys among 32 of
+    // one sequence each takes one part: 147 us, against 45 with those 32 outside every group.)
     const int64_t groups = min64(n_groups, n_seqs), each = (n_seqs + groups - 1) / groups;
     p.few = each * G <= 16;
     p.tc = G <= kPrefixTcRows;
@@ -97,9 +99,10 @@ PrefixPlan prefix_plan(int64_t n_seqs, int64_t max_keys, int64_t n_groups, int64
     p.parts = static_cast<int>(room);
     if (!p.tc) return p;
     // Own keys run beside the prefixes on the SMs that these leave. The fewest parts with which the prefixes end before their
-    // keys do, as if own lengths were half of what the table holds: fewer starts, and less to join. (Whole calls with all, 112, 80, 56, 40 and
-    // 24 SMs for the prefixes, the rule's last: 64 BF16 sequences behind 8192 keys with 33 k of their own 57, 53, 49.5, 49, 45, 61.5; 46.
-    // 16 behind 4096 with 16 k 37, 36, 33, 30, 29, 35; 29.6. 64 behind 16384 with one each 47, 41, 47, 57, 73, 107; 41.)
+    // keys do, as if own lengths were half of what the table holds: fewer starts, and less to join. (Whole calls with all, 112,
+    // 80, 56, 40 and 24 SMs for the prefixes, the rule's last: 64 BF16 sequences behind 8192 keys with 33 k of their own 57, 53,
+    // 49.5, 49, 45, 61.5; 46. 16 behind 4096 with 16 k 37, 36, 33, 30, 29, 35; 29.6. 64 behind 16384 with one each 47, 41, 47, 57,
+    // 73, 107; 41.)
     const float own = 0.5f * n_seqs * max_keys * Hkv * D * (dtype == B200_DTYPE_F32 ? 8 : 4) * 1e-3f / kPxOwnRate;
     const auto time = [&](int64_t parts) {
         const int64_t steps = ((max_prefix + 127) / 128 + parts - 1) / parts;

@@ -1,4 +1,5 @@
-// Arguments of the batched one-token attention over paged caches (b200_flash_attn_paged_batch), and its launch for sequences that share prefixes.
+// Arguments of the batched one-token attention over paged caches (b200_flash_attn_paged_batch), and its launch for sequences that
+// share prefixes.
 #pragma once
 
 #include "paged_line.cuh"

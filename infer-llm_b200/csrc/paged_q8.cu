@@ -3,9 +3,9 @@
 // A row x of D elements becomes q = e4m3(x 2^-e) and e, the least whole number with max |x| <= 448 2^e. A power of two as
 // scale leaves x 2^-e exact, so an element is rounded once and the answer does not depend on how a quotient is
 // rounded; within a factor of two of the range it costs e4m3, whose steps are relative, no accuracy.
-// Both are passes over bytes: 4096 F32 rows of 8 heads of 128 (42 MB) into the cache 14 us a call, 3.0 TB/s; 32 k BF16 rows (198 MB) out of it
-// 36 us, 5.5 TB/s, 84 % of a large copy's rate. For one decode step's few rows the dependent chain row -> sequence -> block -> store bounds them
-// (64 rows 3 us on the device).
+// Both are passes over bytes: 4096 F32 rows of 8 heads of 128 (42 MB) into the cache 14 us a call, 3.0 TB/s; 32 k BF16 rows (198
+// MB) out of it 36 us, 5.5 TB/s, 84 % of a large copy's rate. For one decode step's few rows the dependent chain row -> sequence
+// -> block -> store bounds them (64 rows 3 us on the device).
 #include "paged_q8.cuh"
 
 namespace b200 {
@@ -93,7 +93,8 @@ __global__ void __launch_bounds__(kQ8Threads) paged_append_q8_kernel(const Q8Arg
     }
 }
 
-// The same chunks the other way, K and V by one warp: its lookups serve both (198 MB 39 -> 36 us; append, whose loads come before them, 13.9 -> 14.4).
+// The same chunks the other way, K and V by one warp: its lookups serve both (198 MB 39 -> 36 us; append, whose loads come before
+// them, 13.9 -> 14.4).
 template <typename T, int D>
 __global__ void __launch_bounds__(kQ8Threads) paged_read_q8_kernel(const Q8Args a) {
     constexpr int E = 16 / sizeof(T), L = D / E;
