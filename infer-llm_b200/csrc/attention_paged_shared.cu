@@ -61,7 +61,7 @@ struct PrefixPlan {
 // Model of the tensor-core kernel and of the own keys' (us, kB a us): what a CTA's start and end and a tile of 128 keys take, and
 // the rate of own keys on all SMs.
 constexpr float kPxStart = 8.f, kPxStartF32 = 16.f, kPxTile = 2.5f, kPxTileF32 = 2.2f, kPxOwnRate = 4500.f;
-// The same start and tile in units of the own keys' line (0.7 us).
+// About the same start and tile, rounded down to whole units of the own keys' line (0.7 us).
 constexpr int kGapStart = 10, kGapStartF32 = 20, kGapTile = 3;
 constexpr size_t kPrefixMostPlanes = size_t(1) << 30;
 PrefixPlan prefix_plan(int64_t n_seqs, int64_t max_keys, int64_t n_groups, int64_t max_prefix, int64_t D, int64_t G, int64_t Hkv,
